@@ -399,6 +399,85 @@ int nsx_attn_decode_qkv(const float *qkv, const float *q_bias, const float *k_bi
 /* *pos += n on the stream (one thread). */
 int nsx_pos_advance(int32_t *pos, int32_t n, void *stream);
 
+/* ---- decoding with drafted tokens ----
+ * No reference counterpart (the reference decodes one token per forward,
+ * api.py:193-237). A pass over several drafted tokens: their attention over
+ * the cache and one another, their verification against the target model's
+ * logits, and the accepted ones' rows into the caches.
+ * Nodes: up to NSX_TREE_MAX_NODES drafted tokens. parents (device int32,
+ * n_nodes; NULL: a chain) holds each node's parent, an earlier node; anything
+ * else (-1) makes it a first node. Node i stands at position *pos + depth(i),
+ * *pos being the number of rows in the cache. */
+#define NSX_TREE_MAX_NODES 64
+/* Workspace bytes that serve every call of up to max_nodes nodes and any
+ * window over a cache of ctx_max rows; -1 for sizes the calls refuse. */
+int64_t nsx_tree_workspace_bytes(int n_head, int n_kv, int head_dim, int max_nodes, int64_t ctx_max);
+/* The attention of model/gpt_oss.py:73-85 for several query tokens at once:
+ * node i sees the cache's rows 0 .. *pos - 1, its ancestors and itself, of
+ * these the last `window` positions when window > 0. q: [n_nodes][n_head][64]
+ * fp32, rotated. Caches [n_kv][ctx_max][64] and the nodes' own rows
+ * [n_kv][max_nodes][64], all of kv_dtype (NSX_DT_*). sinks, scale, n_head and
+ * n_kv as nsx_attn_decode. out: [n_nodes][n_head][64] fp32. A key of weight
+ * zero takes no part, whatever its value row holds. Nothing is written unless
+ * 0 <= *pos <= ctx_max. The buffers are 16-byte aligned; the workspace need
+ * not be cleared and is free for other use once the call's work on the stream
+ * is done. */
+int nsx_tree_attn(const float *q, const void *k_cache, const void *v_cache, int kv_dtype,
+                  const void *node_k, const void *node_v, const int32_t *parents, int n_nodes,
+                  int max_nodes, const float *sinks, int n_head, int n_kv, int head_dim,
+                  const int32_t *pos, int64_t ctx_max, int window, float scale, void *workspace,
+                  int64_t workspace_bytes, float *out, void *stream);
+/* The same from the nodes' raw q | k | v projections, [n_nodes][n_head + 2
+ * n_kv][64] fp32, left unchanged: bias and rotary at each node's position (the
+ * bits of nsx_rope_kv_append at that position), the nodes' key and value rows
+ * rounded to kv_dtype into node_k and node_v, then nsx_tree_attn. */
+int nsx_tree_attn_qkv(const float *qkv, const float *q_bias, const float *k_bias, const float *v_bias,
+                      const float *inv_freq, float amplitude, const void *k_cache, const void *v_cache,
+                      int kv_dtype, void *node_k, void *node_v, const int32_t *parents, int n_nodes,
+                      int max_nodes, const float *sinks, int n_head, int n_kv, int head_dim,
+                      const int32_t *pos, int64_t ctx_max, int window, float scale, void *workspace,
+                      int64_t workspace_bytes, float *out, void *stream);
+/* Rows path[0 .. min(*count, n_nodes) - 1] of the nodes into the caches' rows
+ * *pos, *pos + 1, ..., for all layers ([n_layer][n_kv][ctx_max][64] caches,
+ * [n_layer][n_kv][max_nodes][64] nodes), then *pos += *count, at most to
+ * ctx_max. Rows past ctx_max and entries of path outside [0, max_nodes) are
+ * not copied; other rows stay as they are. */
+int nsx_tree_commit(void *k_caches, void *v_caches, const void *node_k, const void *node_v, int kv_dtype,
+                    int n_layer, int n_kv, int head_dim, int n_nodes, int max_nodes, const int32_t *path,
+                    const int32_t *count, int32_t *pos, int64_t ctx_max, void *stream);
+/* Which drafted tokens the target model accepts, and the token that follows
+ * them, for `batch` sequences of n_nodes nodes each. Node 0 is the sequence's
+ * last known token, every other one a draft under its parent; row i of a
+ * sequence's logits ([batch][n_nodes] rows of vocab elements, row_stride
+ * elements apart) is the target's distribution behind node i, p = softmax(
+ * logits / temperature). From node 0 on, the current node's children are tried
+ * in order, x a child's token and u its entry of uniforms ([batch][n_nodes], in
+ * [0, 1)):
+ *   draft_probs NULL: accepted when u * left < p(x), left being what the
+ *     refused children leave of p (a token refused before has nothing left);
+ *     the following token is drawn from p without the refused tokens;
+ *   draft_probs q ([batch][n_nodes - 1][vocab] fp32, row i the distribution
+ *     that node i + 1 was drawn from; chains only): accepted when u * q(x) <
+ *     p(x); after a refusal the following token is drawn from max(p - q, 0).
+ * A draw takes the first token, in index order, at which the running sum of
+ * the weights exceeds uniforms[0] times their total. temperature 0: p is one
+ * at the largest logit, the lowest index of equals (uniforms may be NULL).
+ * Probabilities, sums and comparisons are in 64 bits. A NaN logit counts as
+ * -infinity; a drafted token outside [0, vocab) is refused.
+ * tokens: [batch][n_nodes]; parents: NULL (chains), one tree of n_nodes for
+ * all sequences (parents_stride 0), or one each, parents_stride entries apart;
+ * lengths: NULL, or how many of its nodes each sequence has (0: none, a padded
+ * sequence). count: nodes accepted, node 0 among them; path: [batch][n_nodes],
+ * the accepted nodes in order, then -1; token: the one that follows, -1 where
+ * a sequence has no nodes or its last row no weight. batch * n_nodes < 65536,
+ * vocab up to 4194304, temperature 0 or 1e-30 to 1e30. */
+int64_t nsx_verify_workspace_bytes(int64_t batch, int n_nodes, int64_t vocab);
+int nsx_verify(const void *logits, int logits_dtype, int64_t row_stride, int64_t batch, int n_nodes,
+               int64_t vocab, const int32_t *tokens, const int32_t *parents, int64_t parents_stride,
+               const int32_t *lengths, const float *uniforms, const float *draft_probs, double temperature,
+               int32_t *count, int32_t *path, int32_t *token, void *workspace, int64_t workspace_bytes,
+               void *stream);
+
 /* ---- disk reader: GGUF bytes from a file into device (or host) memory ----
  * Replaces the reference's thread-pool reader and the disk side of its
  * streaming source (io/reader.py AsyncReader, io/stream.py StreamingSource):

@@ -95,6 +95,14 @@ _SIGS = {
     "nsx_attn_decode_qkv": (_i, [_p, _p, _p, _p, _p, C.c_float, _p, _i, _i, _i, _p, _p, _p, _i64, _i, C.c_float,
                                  _p, _p, _p]),
     "nsx_pos_advance": (_i, [_p, C.c_int32, _p]),
+    "nsx_tree_workspace_bytes": (_i64, [_i, _i, _i, _i, _i64]),
+    "nsx_tree_attn": (_i, [_p, _p, _p, _i, _p, _p, _p, _i, _i, _p, _i, _i, _i, _p, _i64, _i, C.c_float, _p, _i64, _p,
+                           _p]),
+    "nsx_tree_attn_qkv": (_i, [_p, _p, _p, _p, _p, C.c_float, _p, _p, _i, _p, _p, _p, _i, _i, _p, _i, _i, _i, _p, _i64,
+                               _i, C.c_float, _p, _i64, _p, _p]),
+    "nsx_tree_commit": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p, _p, _p, _i64, _p]),
+    "nsx_verify_workspace_bytes": (_i64, [_i64, _i, _i64]),
+    "nsx_verify": (_i, [_p, _i, _i64, _i64, _i, _i64, _p, _p, _i64, _p, _p, _p, C.c_double, _p, _p, _p, _p, _i64, _p]),
     "nsx_reader_open": (_i, [C.c_char_p, _i, _i, _i, _i64, _i, _p, C.POINTER(_p)]),
     "nsx_reader_submit": (_i, [_p, _i64, _i64, _p, _i, _p, C.POINTER(C.c_uint64)]),
     "nsx_reader_poll": (_i, [_p, C.c_uint64]),
@@ -105,6 +113,7 @@ _SIGS = {
 PHASE_ROUTER, PHASE_GATE_UP, PHASE_DOWN, PHASE_COMBINE = 0, 1, 2, 3
 CHAIN_GATE_UP, CHAIN_DOWN = 1, 2  # nsx_moe_chain_t1 phases
 STATIC_WORKSPACE_BYTES = 32 << 20  # NSX_STATIC_WORKSPACE_BYTES
+TREE_MAX_NODES = 64  # NSX_TREE_MAX_NODES
 
 
 class NativeError(RuntimeError):

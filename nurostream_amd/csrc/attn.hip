@@ -16,6 +16,7 @@
 // Both grids are sized for ctx_max, so their shape does not depend on the
 // position; each workgroup takes its share of the keys up to it.
 #include "nsx_common.h"
+#include "rope.h"
 
 #include <algorithm>
 #include <type_traits>
@@ -23,19 +24,14 @@
 
 namespace {
 
-constexpr int ATTN_D = 64;        // head_dim (GPT-OSS)
 constexpr int ATTN_TILE = 16;     // keys per wave and matrix-core step
 constexpr int ATTN_NW = 4;        // waves of a split's workgroup
 constexpr int ATTN_FINAL_NW = 8;  // waves of the only workgroup of a kv head: a tile each at 128 keys
 constexpr int ATTN_FINAL_KEYS = 128;  // up to this many keys one workgroup per kv head does everything
-constexpr int ATTN_MAX_REP = 16;  // query heads per kv head (columns of the matrix-core step)
 // Splits of a kv head's keys: enough workgroups for two on each of the 256 CUs, at most what the combine
 // kernel's lanes hold, and none shorter than a tile per wave.
 constexpr int ATTN_MAX_SPLIT = 128;
 constexpr int ATTN_GRID = 512;
-// A running maximum's start. Finite, not -infinity: keys that all score -infinity (overflowed scores) then get weight
-// e^-infinity = 0 beside it, where the difference of two infinities would make the head NaN.
-constexpr float ATTN_LOWEST = -3.4028235e38f;
 
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
@@ -46,33 +42,6 @@ __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
-}
-
-// Rotary of element d of a 64-element head row at position p: x = the
-// element, partner = element d ^ 32 (both with bias), rotate_half pairing
-// (gpt_oss.py:42-58, ops.py:95-104). Explicit fmaf so that every kernel that
-// applies it rounds the same way.
-__device__ __forceinline__ float rope_elem(float x, float partner, int d, int p, const float* __restrict__ inv_freq,
-                                           float amp) {
-  const float ang = (float)p * inv_freq[d & (ATTN_D / 2 - 1)];  // fp32, as positions.float() * inv
-  float s, c;
-  sincosf(ang, &s, &c);
-  c *= amp;
-  s *= amp;
-  const float ps = partner * s;
-  return d < ATTN_D / 2 ? fmaf(x, c, -ps) : fmaf(x, c, ps);
-}
-
-// The same for the pair (element d < 32, element d + 32): one sine and cosine serve both.
-__device__ __forceinline__ void rope_pair(float& x0, float& x1, int p, float inv_freq, float amp) {
-  const float ang = (float)p * inv_freq;
-  float s, c;
-  sincosf(ang, &s, &c);
-  c *= amp;
-  s *= amp;
-  const float y0 = fmaf(x0, c, -(x1 * s));
-  x1 = fmaf(x1, c, x0 * s);
-  x0 = y0;
 }
 
 // One wave per row of the q | k | v block: bias, then rotary for q and k

@@ -1,0 +1,580 @@
+// Attention of drafted tokens over a KV cache and over one another (gfx950).
+//
+// N drafted tokens (nodes) hang off the cache's last row as a tree: parents[i] < i is node i's parent, anything else
+// makes it a first node. Node i stands at position pos + depth(i). It sees the cache's rows 0 .. pos - 1 and, of the
+// nodes, its ancestors and itself -- the last `window` positions of those when window > 0 -- and the softmax has a
+// sink, as the one-token attention (attn.hip):
+//   out_i = sum_j e^(s_ij - m) v_j / (sum_j e^(s_ij - m) + e^(sink - m)),  s_ij = scale q_i . k_j,  m the largest.
+// The nodes' key and value rows live beside the cache ([n_kv][max_nodes][64], the cache's type), so that refused
+// drafts never touch it; tree_commit_kernel moves the accepted ones in.
+//
+// Cache and node rows: fp32, fp16 or bf16; queries, sums and outputs fp32.
+#include "nsx_common.h"
+#include "rope.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace {
+
+constexpr int TREE_KEYS = 32;       // keys per wave and step
+constexpr int TREE_NW = 4;          // waves of a workgroup
+constexpr int TREE_MAX_SPLIT = 128;  // splits of a kv head's keys: the combine kernel's lanes hold two each
+constexpr int TREE_GRID = 512;      // workgroups to fill the chip with: two on each of 256 CUs
+constexpr float LOG2E = 1.44269504088896340736f;
+
+struct TreeArgs {
+  const float* q;  // [nodes][n_head][64], rotated
+  const void *kc, *vc, *dk, *dv;
+  const int32_t *parents, *pos;
+  int64_t ctx_max;
+  int window, n_rep, n_kv, n_head, nodes, max_nodes, nsplit, ncb;
+  float scale2;  // scale * log2(e): the softmax is taken in powers of two
+  float* part;
+  const float* sinks;
+  float* out;
+};
+
+// Lane i's node: its ancestors and itself as bits, from the parent list, each round doubling the path's length.
+// Every lane of the wave takes part; lanes past `nodes` hold only their own bit.
+__device__ __forceinline__ uint64_t tree_lineage(const int32_t* __restrict__ parents, int nodes, int lane) {
+  int up = -1;
+  if (lane < nodes) {
+    up = parents ? parents[lane] : lane - 1;
+    if (up >= lane) up = -1;
+  }
+  up = up < 0 ? -1 : up;
+  uint64_t bits = 1ull << lane;
+#pragma unroll
+  for (int r = 0; r < 6; ++r) {
+    const int from = up < 0 ? lane : up;
+    const uint32_t lo = __shfl((uint32_t)bits, from, 64), hi = __shfl((uint32_t)(bits >> 32), from, 64);
+    const int next = __shfl(up, from, 64);
+    if (up >= 0) {
+      bits |= (uint64_t)hi << 32 | lo;
+      up = next;
+    }
+  }
+  return bits;
+}
+
+template <typename KT>
+__device__ __forceinline__ void store_kv(void* p, int64_t i, float v) {
+  if constexpr (std::is_same_v<KT, float>) ((float*)p)[i] = v;
+  else if constexpr (std::is_same_v<KT, _Float16>) ((_Float16*)p)[i] = (_Float16)v;
+  else ((uint16_t*)p)[i] = (uint16_t)nsx_f2bf(v);
+}
+struct Bf16 {
+  uint16_t bits;
+};
+
+// One wave per row of the nodes' q | k | v blocks: bias, rotary at the node's position for q and k; q rows into
+// q_out, k and v rows beside the cache.
+template <typename KT>
+__global__ __launch_bounds__(256) void tree_rope_kernel(const float* __restrict__ qkv, const float* __restrict__ bq,
+                                                        const float* __restrict__ bk, const float* __restrict__ bv,
+                                                        const float* __restrict__ inv_freq, float amp, int n_head,
+                                                        int n_kv, const int32_t* __restrict__ parents,
+                                                        const int32_t* __restrict__ pos_ptr, int64_t ctx_max,
+                                                        int nodes, int max_nodes, float* __restrict__ q_out,
+                                                        void* __restrict__ dk, void* __restrict__ dv) {
+  const int lane = threadIdx.x & 63, rows = n_head + 2 * n_kv;
+  const int w = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (w >= nodes * rows) return;
+  const int node = w / rows, r = w % rows;
+  const int p = *pos_ptr;
+  const uint64_t line = tree_lineage(parents, nodes, lane);
+  if (p < 0 || p > ctx_max) return;
+  const uint64_t mine = (uint64_t)__shfl((uint32_t)(line >> 32), node, 64) << 32 | __shfl((uint32_t)line, node, 64);
+  const int at = p + __popcll(mine) - 1;
+  float x = qkv[((int64_t)node * rows + r) * ATTN_D + lane];
+  const float* b = r < n_head ? bq : r < n_head + n_kv ? bk : bv;
+  const int rb = r < n_head ? r : r < n_head + n_kv ? r - n_head : r - n_head - n_kv;
+  if (b) x += b[rb * ATTN_D + lane];
+  if (r >= n_head + n_kv) {
+    store_kv<KT>(dv, ((int64_t)rb * max_nodes + node) * ATTN_D + lane, x);
+    return;
+  }
+  const float y = rope_elem(x, __shfl_xor(x, ATTN_D / 2, 64), lane, at, inv_freq, amp);
+  if (r < n_head) q_out[((int64_t)node * n_head + r) * ATTN_D + lane] = y;
+  else store_kv<KT>(dk, ((int64_t)rb * max_nodes + node) * ATTN_D + lane, y);
+}
+
+// A 16-byte run of 8 two-byte elements, or two runs of 4 floats 16 dimensions apart, as 8 floats.
+template <typename KT>
+struct Rows;
+template <>
+struct Rows<float> {
+  // The 8 dimensions that lane group g of the matrix-core step holds of dimensions 32 j ..: 4 g .. + 3 and the same
+  // 16 further on, so that a load instruction takes 64 contiguous bytes of each row.
+  static __device__ __forceinline__ int dim(int j, int g, int e) { return 32 * j + 16 * (e >> 2) + 4 * g + (e & 3); }
+  struct K8 {
+    v4f a, b;
+  };
+  using V4 = v4f;
+  static __device__ __forceinline__ K8 k8(const void* row, int j, int g) {
+    const float* p = (const float*)row + 32 * j + 4 * g;
+    return K8{*(const v4f*)p, *(const v4f*)(p + 16)};
+  }
+  static __device__ __forceinline__ V4 v4(const void* row, int i) { return *(const v4f*)((const float*)row + 4 * i); }
+  static __device__ __forceinline__ float k(const K8& x, int e) { return e < 4 ? x.a[e & 3] : x.b[e & 3]; }
+  static __device__ __forceinline__ float v(const V4& x, int d) { return x[d]; }
+};
+template <typename KT>
+struct Rows16 {  // dimensions 32 j + 8 g .. + 7
+  static __device__ __forceinline__ int dim(int j, int g, int e) { return 32 * j + 8 * g + e; }
+  using K8 = v4u;
+  using V4 = v2u;
+  static __device__ __forceinline__ K8 k8(const void* row, int j, int g) {
+    return *(const v4u*)((const uint16_t*)row + 32 * j + 8 * g);
+  }
+  static __device__ __forceinline__ V4 v4(const void* row, int i) { return *(const v2u*)((const uint16_t*)row + 4 * i); }
+  static __device__ __forceinline__ float one(uint32_t w, int hi) {
+    if constexpr (std::is_same_v<KT, Bf16>) return __builtin_bit_cast(float, hi ? w & 0xffff0000u : w << 16);
+    else return nsx_h2f(hi ? w >> 16 : w & 0xffffu);
+  }
+  static __device__ __forceinline__ float k(const K8& x, int e) { return one(x[e >> 1], e & 1); }
+  static __device__ __forceinline__ float v(const V4& x, int d) { return one(x[d >> 1], d & 1); }
+};
+template <>
+struct Rows<_Float16> : Rows16<_Float16> {};
+template <>
+struct Rows<Bf16> : Rows16<Bf16> {};
+
+__device__ __forceinline__ void lds_barrier() {  // LDS writes visible; global loads stay in flight
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028235e38f; }
+
+// Workgroup (kv head g, block cb of 16 NC query columns, split c of the keys). A column is a (node, query head of the
+// kv head) pair, node-major. The keys are the cache's rows from the first that any node sees, in tiles of 32, then the
+// nodes' own rows in tiles of their own; a split is a run of tiles and wave w takes every TREE_NW'th of them. Splits
+// past the present length return at once: the grid goes by ctx_max, so that it does not depend on the position.
+//
+// A tile: scores by v_mfma_f32_16x16x4_f32 (A = 16 keys x 4 dimensions, B = 4 dimensions x 16 columns), each lane
+// holding key l % 16 and 8 of every 32 dimensions; lane l's results are column l % 16 and keys 4 (l / 16) .. + 3 of each
+// 16. These are the B operand of the second product as they stand, when A's lane l holds of each value row the keys
+// of its group and dimensions 4 (l % 16) ..: D then has column l % 16, dimensions 16 (l / 16) + 4 r + dt. So every row
+// is read once by one wave, in 16-byte pieces, and nothing is exchanged but the running maximum (two shuffles).
+//
+// A key with weight zero takes no part whatever its value row holds (0 * NaN would be NaN): a wave whose sums are not
+// finite at the end goes through its tiles again, adding values one key at a time under their weights.
+template <typename KT, int NC>
+__global__ __launch_bounds__(64 * TREE_NW) void tree_attn_kernel(TreeArgs a) {
+  using R = Rows<KT>;
+  constexpr int NT = 64 * TREE_NW, COLS = 16 * NC, QS = ATTN_D + 4;
+  __shared__ __align__(16) float qs[COLS][QS];  // the columns' queries
+  __shared__ __align__(16) float sacc[TREE_NW][COLS][QS];
+  __shared__ float sm[TREE_NW][COLS], sl[TREE_NW][COLS];
+  __shared__ uint64_t svis[64];
+  __shared__ int sdep[64];
+  const int t = threadIdx.x, lane = t & 63, i16 = lane & 15, kq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int g = blockIdx.x % a.n_kv, cb = blockIdx.x / a.n_kv, c = blockIdx.y;
+  const int P = *a.pos;
+  if (P < 0 || P > a.ctx_max) return;
+  const int lo = a.window > 0 ? max(0, P + 1 - a.window) : 0;
+  const int pt = (P - lo + TREE_KEYS - 1) / TREE_KEYS, nt = pt + (a.nodes + TREE_KEYS - 1) / TREE_KEYS;
+  const int per = ((nt + a.nsplit - 1) / a.nsplit + TREE_NW - 1) / TREE_NW * TREE_NW;
+  const int t0 = c * per, t1 = min(nt, t0 + per);
+  if (t0 >= t1) return;
+  const int ncol = a.nodes * a.n_rep, col0 = cb * COLS;
+  if (wave == 0) {
+    uint64_t line = tree_lineage(a.parents, a.nodes, lane);
+    const int dep = __popcll(line) - 1;
+    if (a.window > 0 && a.window < a.nodes) {  // ancestors out of the window
+      for (int j = 0; j < a.nodes; ++j)
+        if (dep - __shfl(dep, j, 64) >= a.window) line &= ~(1ull << j);
+    }
+    svis[lane] = line;
+    sdep[lane] = dep;
+  }
+  for (int i = t; i < COLS * (ATTN_D / 4); i += NT) {
+    const int col = min(col0 + i / (ATTN_D / 4), ncol - 1), d = i % (ATTN_D / 4) * 4;
+    const int node = col / a.n_rep, h = g * a.n_rep + col % a.n_rep;
+    *(v4f*)&qs[i / (ATTN_D / 4)][d] = *(const v4f*)(a.q + ((int64_t)node * a.n_head + h) * ATTN_D + d);
+  }
+  lds_barrier();
+  uint64_t vis[NC];
+  int from[NC], deepest = 0;  // the column's first visible cache row
+#pragma unroll
+  for (int ct = 0; ct < NC; ++ct) {
+    const int node = min(col0 + 16 * ct + i16, ncol - 1) / a.n_rep;
+    vis[ct] = svis[node];
+    from[ct] = a.window > 0 ? P + sdep[node] + 1 - a.window : 0;
+    deepest = max(deepest, from[ct]);
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) deepest = max(deepest, __shfl_xor(deepest, o, 64));
+  deepest = __builtin_amdgcn_readfirstlane(deepest);
+
+  float m[NC], l[NC];
+  v4f acc[NC][4];
+  float* sp = &sacc[wave][0][0];  // the second way's weights, [key][column]
+  static_assert(TREE_KEYS * COLS <= COLS * QS, "weights of a tile in the wave's part of sacc");
+  auto pass = [&](auto slow_tag) {
+    constexpr bool SLOW = decltype(slow_tag)::value;
+#pragma unroll
+    for (int ct = 0; ct < NC; ++ct) {
+      m[ct] = ATTN_LOWEST;
+      l[ct] = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) acc[ct][dt] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int tile = t0 + wave; tile < t1; tile += TREE_NW) {
+      const bool own = tile >= pt;  // the nodes' rows
+      const int r0 = own ? (tile - pt) * TREE_KEYS : lo + tile * TREE_KEYS, last = (own ? a.nodes : P) - 1;
+      const int64_t base = ((int64_t)g * (own ? a.max_nodes : a.ctx_max)) * (ATTN_D * (int64_t)sizeof(KT));
+      const char* kb = (const char*)(own ? a.dk : a.kc) + base;
+      const char* vb = (const char*)(own ? a.dv : a.vc) + base;
+      auto row = [&](int k) { return (int64_t)min(r0 + k, last) * (ATTN_D * (int64_t)sizeof(KT)); };
+      typename R::K8 kr[2][2];
+      typename R::V4 vr[8];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) kr[kt][j] = R::k8(kb + row(16 * kt + i16), j, kq);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) vr[e] = R::v4(vb + row(16 * (e >> 2) + 4 * kq + (e & 3)), i16);
+      const bool masked = own || r0 + TREE_KEYS > P || r0 < deepest;
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct) {
+        v4f s[2] = {};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float qv[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) qv[e] = qs[16 * ct + i16][R::dim(j, kq, e)];
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              s[kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(R::k(kr[kt][j], e), qv[e], s[kt], 0, 0, 0);
+        }
+        float p[8], mx = ATTN_LOWEST;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = s[e >> 2][e & 3] * a.scale2;
+          if (masked) {
+            const int k = r0 + 16 * (e >> 2) + 4 * kq + (e & 3);
+            const bool on = own ? k < a.nodes && (vis[ct] >> k & 1) : k < P && k >= from[ct];
+            p[e] = on ? p[e] : -INFINITY;
+          }
+          mx = fmaxf(mx, p[e]);
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        const float mn = fmaxf(m[ct], fmaxf(mx, __shfl_xor(mx, 32, 64)));
+        const float corr = __builtin_amdgcn_exp2f(m[ct] - mn);  // (first tile: of nothing)
+        m[ct] = mn;
+        float ls = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(p[e] - mn);
+          ls += p[e];
+        }
+        l[ct] = fmaf(l[ct], corr, ls);  // this lane group's keys; the groups are added at the end
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) acc[ct][dt] *= corr;
+        if constexpr (!SLOW) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt)
+              acc[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(R::v(vr[e], dt), p[e], acc[ct][dt], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sp[(16 * (e >> 2) + 4 * kq + (e & 3)) * COLS + 16 * ct + i16] = p[e];
+        }
+      }
+      if constexpr (SLOW) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll 1
+        for (int k = 0; k < TREE_KEYS; ++k) {
+          const char* vrow = vb + row(k);
+          typename R::V4 v[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = R::v4(vrow, 4 * kq + r);
+#pragma unroll
+          for (int ct = 0; ct < NC; ++ct) {
+            const float w = sp[k * COLS + 16 * ct + i16];
+            if (w != 0.f) {
+#pragma unroll
+              for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[ct][dt][r] = fmaf(w, R::v(v[r], dt), acc[ct][dt][r]);
+            }
+          }
+        }
+      }
+    }
+  };
+  pass(std::false_type{});
+  bool ok = true;
+#pragma unroll
+  for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) ok = ok && finite(acc[ct][dt][r]);
+  if (!__all(ok)) pass(std::true_type{});
+
+#pragma unroll
+  for (int ct = 0; ct < NC; ++ct) {
+    l[ct] += __shfl_xor(l[ct], 16, 64);
+    l[ct] += __shfl_xor(l[ct], 32, 64);
+    if (kq == 0) {
+      sm[wave][16 * ct + i16] = m[ct];
+      sl[wave][16 * ct + i16] = l[ct];
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      *(v4f*)&sacc[wave][16 * ct + i16][16 * kq + 4 * r] = v4f{acc[ct][0][r], acc[ct][1][r], acc[ct][2][r], acc[ct][3][r]};
+  }
+  lds_barrier();
+  const bool whole = a.nsplit == 1;
+  for (int i = t; i < min(COLS, ncol - col0) * ATTN_D; i += NT) {
+    const int cc = i / ATTN_D, d = i % ATTN_D, col = col0 + cc;
+    const int h = g * a.n_rep + col % a.n_rep;
+    const int64_t row = (int64_t)(col / a.n_rep) * a.n_head + h;
+    const float sink = whole && a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
+    float M = sink;
+#pragma unroll
+    for (int w = 0; w < TREE_NW; ++w) M = fmaxf(M, sm[w][cc]);
+    float Z = whole && a.sinks ? __builtin_amdgcn_exp2f(sink - M) : 0.f, v = 0.f;
+#pragma unroll
+    for (int w = 0; w < TREE_NW; ++w) {  // (a wave without a tile has weight 0)
+      const float e = __builtin_amdgcn_exp2f(sm[w][cc] - M);
+      Z = fmaf(e, sl[w][cc], Z);
+      v = fmaf(e, sacc[w][cc][d], v);
+    }
+    if (whole) {
+      a.out[row * ATTN_D + d] = v / Z;
+    } else {
+      a.part[(row * a.nsplit + c) * ATTN_D + d] = v;
+      if (d == 0) {
+        float* ml = a.part + ((int64_t)a.nodes * a.n_head * ATTN_D + row * 2) * a.nsplit + 2 * c;
+        ml[0] = M;
+        ml[1] = Z;
+      }
+    }
+  }
+}
+
+// One workgroup per (node, query head): merge the live splits with the sink. Every wave forms all the splits' weights
+// (lane = split), then wave w sums the values of splits w, w + 4, ... (lane = dimension) and the four sums meet in LDS.
+__global__ __launch_bounds__(256) void tree_combine_kernel(TreeArgs a) {
+  constexpr int LPS = TREE_MAX_SPLIT / 64;  // splits per lane
+  __shared__ float ws[TREE_MAX_SPLIT];
+  __shared__ float red[4][ATTN_D];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t row = blockIdx.x;
+  const int P = *a.pos;
+  if (P < 0 || P > a.ctx_max) return;
+  const int lo = a.window > 0 ? max(0, P + 1 - a.window) : 0;
+  const int nt = (P - lo + TREE_KEYS - 1) / TREE_KEYS + (a.nodes + TREE_KEYS - 1) / TREE_KEYS;
+  const int per = ((nt + a.nsplit - 1) / a.nsplit + TREE_NW - 1) / TREE_NW * TREE_NW;
+  const int nc = (nt + per - 1) / per;  // 1 <= nc <= nsplit
+  const float* ml = a.part + ((int64_t)a.nodes * a.n_head * ATTN_D + row * 2) * a.nsplit;
+  const float sink = a.sinks ? a.sinks[row % a.n_head] * LOG2E : -INFINITY;
+  float mv[LPS], lv[LPS], M = sink;
+#pragma unroll
+  for (int i = 0; i < LPS; ++i) {
+    const int s = min(lane + 64 * i, nc - 1);
+    mv[i] = ml[2 * s];
+    lv[i] = ml[2 * s + 1];
+    M = fmaxf(M, mv[i]);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+  float z = 0.f;
+#pragma unroll
+  for (int i = 0; i < LPS; ++i) {
+    const bool on = lane + 64 * i < nc;
+    const float e = on ? __builtin_amdgcn_exp2f(mv[i] - M) : 0.f;
+    if (wave == 0) ws[lane + 64 * i] = e;
+    z = on ? fmaf(e, lv[i], z) : z;
+  }
+  const float Z = nsx_wave_sum(z) + (a.sinks ? __builtin_amdgcn_exp2f(sink - M) : 0.f);
+  __syncthreads();
+  const float* pv = a.part + row * a.nsplit * ATTN_D + lane;
+  float v = 0.f;
+  for (int c0 = wave; c0 < nc; c0 += 4) v = fmaf(ws[c0], pv[(int64_t)c0 * ATTN_D], v);
+  red[wave][lane] = v;
+  __syncthreads();
+  if (wave == 0) a.out[row * ATTN_D + lane] = ((red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane])) / Z;
+}
+
+// Accepted nodes' rows into the caches: path[j] to row pos + j for j < count. One 16-byte piece of one row per thread
+// over (layer, kv head, j, piece), keys and values.
+__global__ __launch_bounds__(256) void tree_commit_kernel(char* __restrict__ kc, char* __restrict__ vc,
+                                                          const char* __restrict__ dk, const char* __restrict__ dv,
+                                                          int row_bytes, int heads, int nodes, int max_nodes,
+                                                          const int32_t* __restrict__ path,
+                                                          const int32_t* __restrict__ count,
+                                                          const int32_t* __restrict__ pos, int64_t ctx_max) {
+  const int pieces = row_bytes / 16;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int p = *pos, n = min(*count, nodes);
+  const int c = (int)(i % pieces), j = (int)(i / pieces % nodes);
+  const int64_t h = i / pieces / nodes;
+  if (h >= heads || j >= n || p < 0 || (int64_t)p + j >= ctx_max) return;
+  const int src = path[j];
+  if (src < 0 || src >= max_nodes) return;
+  const int64_t from = (h * max_nodes + src) * row_bytes + 16 * c, to = (h * ctx_max + p + j) * row_bytes + 16 * c;
+  const v4u k = *(const v4u*)(dk + from), v = *(const v4u*)(dv + from);
+  *(v4u*)(kc + to) = k;
+  *(v4u*)(vc + to) = v;
+}
+
+__global__ void tree_advance_kernel(int32_t* pos, const int32_t* count, int nodes, int64_t ctx_max) {
+  if (threadIdx.x == 0 && *pos >= 0 && *pos <= ctx_max)
+    *pos = (int32_t)min((int64_t)*pos + max(0, min(*count, nodes)), ctx_max);
+}
+
+// ---------------------------------------------------------------------------
+
+// Column tiles of 16 per workgroup.
+int tree_nc(int64_t cols) { return cols <= 16 ? 1 : cols <= 32 ? 2 : 4; }
+
+// Splits per kv head and column block for a cache of ctx_max rows.
+int tree_splits(int n_kv, int n_rep, int nodes, int64_t ctx_max, int window) {
+  const int64_t cols = (int64_t)nodes * n_rep, ncb = nsx_cdiv(cols, 16 * tree_nc(cols));
+  const int64_t keys = window > 0 ? std::min<int64_t>(ctx_max, window) : ctx_max;
+  const int64_t tiles = nsx_cdiv(keys, TREE_KEYS) + nsx_cdiv(nodes, TREE_KEYS);
+  if (tiles <= 2 * TREE_NW) return 1;
+  return (int)std::min<int64_t>({nsx_cdiv(tiles, TREE_NW), nsx_cdiv(TREE_GRID, n_kv * ncb), TREE_MAX_SPLIT});
+}
+
+int64_t tree_bytes(int n_head, int n_kv, int nodes, int64_t ctx_max, int window) {
+  const int64_t rows = (int64_t)nodes * n_head;
+  // the rotated queries, then a split's values and (maximum, sum) per row
+  return rows * ATTN_D * 4 + rows * tree_splits(n_kv, n_head / n_kv, nodes, ctx_max, window) * (ATTN_D + 2) * 4;
+}
+
+int tree_shapes(int n_head, int n_kv, int head_dim, int nodes, int max_nodes, int64_t ctx_max, int window) {
+  NSX_REQUIRE(head_dim == ATTN_D, NSX_ENOTIMPL, "head_dim %d (the kernels are written for 64)", head_dim);
+  NSX_REQUIRE(n_head > 0 && n_kv > 0 && n_head % n_kv == 0 && n_head / n_kv <= ATTN_MAX_REP, NSX_EINVAL,
+              "n_head=%d, n_kv=%d: n_head must be a multiple of n_kv, at most %d per kv head", n_head, n_kv,
+              ATTN_MAX_REP);
+  NSX_REQUIRE(n_kv <= 65536, NSX_EINVAL, "n_kv=%d", n_kv);
+  NSX_REQUIRE(nodes > 0 && nodes <= max_nodes && max_nodes <= NSX_TREE_MAX_NODES, NSX_EINVAL,
+              "%d nodes of at most %d (limit %d)", nodes, max_nodes, NSX_TREE_MAX_NODES);
+  NSX_REQUIRE(ctx_max > 0 && ctx_max < (1ll << 31) - 64 && window >= 0, NSX_EINVAL, "ctx_max=%lld window=%d",
+              (long long)ctx_max, window);
+  return NSX_OK;
+}
+
+template <typename KT>
+int tree_attn_typed(TreeArgs& a, hipStream_t st) {
+  const int nc = tree_nc((int64_t)a.nodes * a.n_rep);
+  a.ncb = (int)nsx_cdiv((int64_t)a.nodes * a.n_rep, 16 * nc);
+  const dim3 grid(a.n_kv * a.ncb, a.nsplit), block(64 * TREE_NW);
+  if (nc == 1) hipLaunchKernelGGL((tree_attn_kernel<KT, 1>), grid, block, 0, st, a);
+  else if (nc == 2) hipLaunchKernelGGL((tree_attn_kernel<KT, 2>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((tree_attn_kernel<KT, 4>), grid, block, 0, st, a);
+  NSX_LAUNCHED();
+  if (a.nsplit > 1) {
+    hipLaunchKernelGGL(tree_combine_kernel, dim3(a.nodes * a.n_head), dim3(256), 0, st, a);
+    NSX_LAUNCHED();
+  }
+  return NSX_OK;
+}
+
+int tree_attn_launch(TreeArgs& a, int kv_dtype, hipStream_t st) {
+  if (kv_dtype == NSX_DT_F32) return tree_attn_typed<float>(a, st);
+  if (kv_dtype == NSX_DT_F16) return tree_attn_typed<_Float16>(a, st);
+  return tree_attn_typed<Bf16>(a, st);
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+int64_t kv_elem(int dt) { return dt == NSX_DT_F32 ? 4 : 2; }
+
+}  // namespace
+
+extern "C" int64_t nsx_tree_workspace_bytes(int n_head, int n_kv, int head_dim, int max_nodes, int64_t ctx_max) {
+  if (tree_shapes(n_head, n_kv, head_dim, max_nodes, max_nodes, ctx_max, 0) != NSX_OK) return -1;
+  int64_t most = 0;  // fewer nodes or a window may take more splits, never more than the cache's rows do
+  for (int n = 1; n <= max_nodes; ++n) most = std::max(most, tree_bytes(n_head, n_kv, n, ctx_max, 0));
+  return most;
+}
+
+static int tree_checks(const void* kc, const void* vc, int kv_dtype, const void* dk, const void* dv, const int32_t* pos,
+                       const void* workspace, int64_t workspace_bytes, const float* out, int n_head, int n_kv,
+                       int nodes, int64_t ctx_max, int window) {
+  NSX_REQUIRE(kv_dtype == NSX_DT_F32 || kv_dtype == NSX_DT_F16 || kv_dtype == NSX_DT_BF16, NSX_ETYPE,
+              "cache element type %d", kv_dtype);
+  NSX_REQUIRE(kc && vc && dk && dv && pos && workspace && out, NSX_EINVAL, "null buffer");
+  NSX_REQUIRE(aligned16(kc) && aligned16(vc) && aligned16(dk) && aligned16(dv) && aligned16(workspace) && aligned16(out),
+              NSX_EINVAL, "the caches, the nodes' rows, the workspace and out must be 16-byte aligned");
+  const int64_t need = tree_bytes(n_head, n_kv, nodes, ctx_max, window);
+  NSX_REQUIRE(workspace_bytes >= need, NSX_EINVAL, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+              (long long)need);
+  return NSX_OK;
+}
+
+extern "C" int nsx_tree_attn(const float* q, const void* k_cache, const void* v_cache, int kv_dtype,
+                             const void* node_k, const void* node_v, const int32_t* parents, int n_nodes,
+                             int max_nodes, const float* sinks, int n_head, int n_kv, int head_dim,
+                             const int32_t* pos, int64_t ctx_max, int window, float scale, void* workspace,
+                             int64_t workspace_bytes, float* out, void* stream) {
+  if (const int rc = tree_shapes(n_head, n_kv, head_dim, n_nodes, max_nodes, ctx_max, window)) return rc;
+  NSX_REQUIRE(q && aligned16(q), NSX_EINVAL, "q must be a 16-byte aligned buffer");
+  if (const int rc = tree_checks(k_cache, v_cache, kv_dtype, node_k, node_v, pos, workspace, workspace_bytes, out,
+                                 n_head, n_kv, n_nodes, ctx_max, window))
+    return rc;
+  const int nsplit = tree_splits(n_kv, n_head / n_kv, n_nodes, ctx_max, window);
+  TreeArgs a{q, k_cache, v_cache, node_k, node_v, parents, pos, ctx_max, window, n_head / n_kv, n_kv, n_head, n_nodes,
+             max_nodes, nsplit, 0, scale * LOG2E, (float*)workspace + (int64_t)n_nodes * n_head * ATTN_D, sinks, out};
+  return tree_attn_launch(a, kv_dtype, (hipStream_t)stream);
+}
+
+extern "C" int nsx_tree_attn_qkv(const float* qkv, const float* q_bias, const float* k_bias, const float* v_bias,
+                                 const float* inv_freq, float amplitude, const void* k_cache, const void* v_cache,
+                                 int kv_dtype, void* node_k, void* node_v, const int32_t* parents, int n_nodes,
+                                 int max_nodes, const float* sinks, int n_head, int n_kv, int head_dim,
+                                 const int32_t* pos, int64_t ctx_max, int window, float scale, void* workspace,
+                                 int64_t workspace_bytes, float* out, void* stream) {
+  if (const int rc = tree_shapes(n_head, n_kv, head_dim, n_nodes, max_nodes, ctx_max, window)) return rc;
+  NSX_REQUIRE(qkv && inv_freq, NSX_EINVAL, "null buffer");
+  if (const int rc = tree_checks(k_cache, v_cache, kv_dtype, node_k, node_v, pos, workspace, workspace_bytes, out,
+                                 n_head, n_kv, n_nodes, ctx_max, window))
+    return rc;
+  hipStream_t st = (hipStream_t)stream;
+  float* q = (float*)workspace;
+  const dim3 grid((unsigned)nsx_cdiv((int64_t)n_nodes * (n_head + 2 * n_kv), 4)), block(256);
+  auto rope = [&](auto tag) {
+    hipLaunchKernelGGL((tree_rope_kernel<decltype(tag)>), grid, block, 0, st, qkv, q_bias, k_bias, v_bias, inv_freq,
+                       amplitude, n_head, n_kv, parents, pos, ctx_max, n_nodes, max_nodes, q, node_k, node_v);
+  };
+  if (kv_dtype == NSX_DT_F32) rope(float{});
+  else if (kv_dtype == NSX_DT_F16) rope(_Float16{});
+  else rope(Bf16{});
+  NSX_LAUNCHED();
+  const int nsplit = tree_splits(n_kv, n_head / n_kv, n_nodes, ctx_max, window);
+  TreeArgs a{q, k_cache, v_cache, node_k, node_v, parents, pos, ctx_max, window, n_head / n_kv, n_kv, n_head, n_nodes,
+             max_nodes, nsplit, 0, scale * LOG2E, q + (int64_t)n_nodes * n_head * ATTN_D, sinks, out};
+  return tree_attn_launch(a, kv_dtype, st);
+}
+
+extern "C" int nsx_tree_commit(void* k_caches, void* v_caches, const void* node_k, const void* node_v, int kv_dtype,
+                               int n_layer, int n_kv, int head_dim, int n_nodes, int max_nodes, const int32_t* path,
+                               const int32_t* count, int32_t* pos, int64_t ctx_max, void* stream) {
+  if (const int rc = tree_shapes(n_kv, n_kv, head_dim, n_nodes, max_nodes, ctx_max, 0)) return rc;
+  NSX_REQUIRE(n_layer > 0 && (int64_t)n_layer * n_kv < (1 << 24), NSX_EINVAL, "n_layer=%d", n_layer);
+  NSX_REQUIRE(kv_dtype == NSX_DT_F32 || kv_dtype == NSX_DT_F16 || kv_dtype == NSX_DT_BF16, NSX_ETYPE,
+              "cache element type %d", kv_dtype);
+  NSX_REQUIRE(k_caches && v_caches && node_k && node_v && path && count && pos, NSX_EINVAL, "null buffer");
+  NSX_REQUIRE(aligned16(k_caches) && aligned16(v_caches) && aligned16(node_k) && aligned16(node_v), NSX_EINVAL,
+              "the caches and the nodes' rows must be 16-byte aligned");
+  hipStream_t st = (hipStream_t)stream;
+  const int row = (int)(ATTN_D * kv_elem(kv_dtype)), heads = n_layer * n_kv;
+  const int64_t work = (int64_t)heads * n_nodes * (row / 16);
+  hipLaunchKernelGGL(tree_commit_kernel, dim3((unsigned)nsx_cdiv(work, 256)), dim3(256), 0, st, (char*)k_caches,
+                     (char*)v_caches, (const char*)node_k, (const char*)node_v, row, heads, n_nodes, max_nodes, path,
+                     count, pos, ctx_max);
+  NSX_LAUNCHED();
+  hipLaunchKernelGGL(tree_advance_kernel, dim3(1), dim3(64), 0, st, pos, count, n_nodes, ctx_max);
+  NSX_LAUNCHED();
+  return NSX_OK;
+}

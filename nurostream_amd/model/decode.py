@@ -76,18 +76,24 @@ def yarn_inv_freq(cfg: AttnConfig, device) -> tuple[torch.Tensor, float]:
 
 
 class DeviceKV:
-    """Per-layer K/V history in HBM, [n_kv][ctx_max][head_dim] fp32 each, and
-    the next token's position as a device int32 (`pos`) with a host mirror
-    (`length`)."""
+    """Per-layer K/V history in HBM, [n_kv][ctx_max][head_dim] each, and the
+    next token's position as a device int32 (`pos`) with a host mirror
+    (`length`). The layers' caches `k` and `v` are views of one tensor each
+    (`k_stack`, `v_stack`). dtype: fp32; or float16 / bfloat16, half the bytes,
+    for model.draft's attention (one token being a tree of one node) -- the
+    one-token calls below take fp32 caches."""
 
-    def __init__(self, n_layer: int, cfg: AttnConfig, ctx_max: int, device) -> None:
+    def __init__(self, n_layer: int, cfg: AttnConfig, ctx_max: int, device, dtype: torch.dtype = torch.float32) -> None:
         if ctx_max < 1:
             raise ValueError("ctx_max must be positive")
+        N.act_dtype_code(dtype)
         self.device = torch.device(device)
         self.ctx_max = int(ctx_max)
-        shape = (cfg.n_head_kv, self.ctx_max, cfg.head_dim)
-        self.k = [torch.zeros(shape, dtype=torch.float32, device=self.device) for _ in range(n_layer)]
-        self.v = [torch.zeros(shape, dtype=torch.float32, device=self.device) for _ in range(n_layer)]
+        self.dtype = dtype
+        shape = (n_layer, cfg.n_head_kv, self.ctx_max, cfg.head_dim)
+        self.k_stack = torch.zeros(shape, dtype=dtype, device=self.device)
+        self.v_stack = torch.zeros(shape, dtype=dtype, device=self.device)
+        self.k, self.v = list(self.k_stack.unbind(0)), list(self.v_stack.unbind(0))
         self.pos = torch.zeros(1, dtype=torch.int32, device=self.device)
         nb = N.load().nsx_attn_workspace_bytes(cfg.n_head, cfg.head_dim, self.ctx_max)
         if nb < 0:
@@ -103,9 +109,15 @@ class DeviceKV:
         self.length = 0
 
 
+def _fp32_cache(kv: DeviceKV, what: str) -> None:
+    if kv.dtype != torch.float32:
+        raise TypeError(f"{what} takes an fp32 cache (this one is {kv.dtype}: model.draft.tree_attn_qkv reads it)")
+
+
 def rope_kv_append(qkv: torch.Tensor, bq, bk, bv, cfg: AttnConfig, inv_freq: torch.Tensor, amp: float,
                    kv: DeviceKV, layer: int) -> None:
     """Bias, rotary on the q and k rows (q in place), k and v into the cache at kv.pos."""
+    _fp32_cache(kv, "rope_kv_append")
     ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     N.check(N.load().nsx_rope_kv_append(qkv.data_ptr(), ptr(bq), ptr(bk), ptr(bv), cfg.n_head, cfg.n_head_kv,
                                         cfg.head_dim, inv_freq.data_ptr(), float(amp), kv.pos.data_ptr(),
@@ -116,6 +128,7 @@ def rope_kv_append(qkv: torch.Tensor, bq, bk, bv, cfg: AttnConfig, inv_freq: tor
 def attn_decode(q: torch.Tensor, kv: DeviceKV, layer: int, sinks: torch.Tensor | None, window: int,
                 cfg: AttnConfig, out: torch.Tensor | None = None) -> torch.Tensor:
     """Sink attention of the token at kv.pos over the layer's cache -> (n_head, head_dim)."""
+    _fp32_cache(kv, "attn_decode")
     y = torch.empty((cfg.n_head, cfg.head_dim), dtype=torch.float32, device=q.device) if out is None else out
     N.check(N.load().nsx_attn_decode(q.data_ptr(), kv.k[layer].data_ptr(), kv.v[layer].data_ptr(),
                                      None if sinks is None else sinks.data_ptr(), cfg.n_head, cfg.n_head_kv,
@@ -130,6 +143,7 @@ def attn_decode_qkv(qkv: torch.Tensor, bq, bk, bv, cfg: AttnConfig, inv_freq: to
                     out: torch.Tensor | None = None) -> torch.Tensor:
     """rope_kv_append + attn_decode as one launch (two with the chunk combine); qkv (the raw
     projection, no bias) is left unchanged. Bit-identical to the two calls."""
+    _fp32_cache(kv, "attn_decode_qkv")
     y = torch.empty((cfg.n_head, cfg.head_dim), dtype=torch.float32, device=qkv.device) if out is None else out
     ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     N.check(N.load().nsx_attn_decode_qkv(qkv.data_ptr(), ptr(bq), ptr(bk), ptr(bv), inv_freq.data_ptr(), float(amp),

@@ -1,0 +1,191 @@
+"""Decoding with drafted tokens: several tokens per pass, checked against the target model's own distribution.
+
+A pass takes a tree of up to 64 nodes (`MAX_NODES`): node 0 the sequence's last known token, the others drafts of what
+may follow, each under its parent. `parents` (device int32) holds every node's parent, an earlier node; None is a
+chain, which is also how a piece of a prompt goes through.
+- `DraftKV`: the nodes' key and value rows, beside a `DeviceKV` (refused drafts never touch the cache);
+- `tree_attn_qkv` / `tree_attn`: a layer's attention of the nodes over the cache and their ancestors, from the raw
+  projections or from rotated queries and finished rows;
+- `verify`: which nodes the target accepts, and the token that follows them;
+- `commit`: the accepted nodes' rows into the caches, the position moved on.
+The reference decodes one token per forward (api.py:193-237); these have no counterpart in it. Calls that share a
+DraftKV (its rows and its workspace) must not overlap.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from .. import _native as N
+from .decode import AttnConfig, DeviceKV
+
+MAX_NODES = N.TREE_MAX_NODES
+
+
+class DraftKV:
+    """Key and value rows of up to max_nodes drafted tokens, [n_layer][n_kv][max_nodes][head_dim] in the cache's type
+    (`k`, `v`: a view per layer), and the attention's workspace."""
+
+    def __init__(self, kv: DeviceKV, cfg: AttnConfig, max_nodes: int = 16) -> None:
+        if not 1 <= max_nodes <= MAX_NODES:
+            raise ValueError(f"max_nodes {max_nodes}: 1 to {MAX_NODES}")
+        n_layer, n_kv, _, head_dim = kv.k_stack.shape
+        if (n_kv, head_dim) != (cfg.n_head_kv, cfg.head_dim):
+            raise ValueError(f"a cache of {n_kv} heads of {head_dim} for a model with {cfg.n_head_kv} of {cfg.head_dim}")
+        nb = N.load().nsx_tree_workspace_bytes(cfg.n_head, n_kv, head_dim, int(max_nodes), kv.ctx_max)
+        if nb < 0:
+            raise NotImplementedError(N.load().nsx_last_error().decode(errors="replace"))
+        self.kv, self.max_nodes, self.n_head = kv, int(max_nodes), cfg.n_head
+        shape = (n_layer, n_kv, self.max_nodes, head_dim)
+        self.k_stack = torch.zeros(shape, dtype=kv.dtype, device=kv.device)
+        self.v_stack = torch.zeros(shape, dtype=kv.dtype, device=kv.device)
+        self.k, self.v = list(self.k_stack.unbind(0)), list(self.v_stack.unbind(0))
+        self.workspace = torch.empty(nb, dtype=torch.uint8, device=kv.device)
+        self._dt = N.act_dtype_code(kv.dtype)
+
+
+def _check(name: str, t, dtype, device, numel: int | None = None) -> None:
+    if t is None:
+        return
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not {device}")
+    if not t.is_contiguous() or (numel is not None and t.numel() != numel):
+        raise ValueError(f"{name} must be contiguous{'' if numel is None else f' with {numel} elements'}, "
+                         f"got {tuple(t.shape)}")
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _tree(x: torch.Tensor, row: int, name: str, draft: DraftKV, layer: int, cfg: AttnConfig, sinks, parents, out):
+    """Checks shared by both attention calls -> (nodes, out)."""
+    kv = draft.kv
+    N.require_device(x)
+    n = x.numel() // row if x.dim() > 1 else 1
+    _check(name, x, torch.float32, kv.k_stack.device, n * row)
+    if not 1 <= n <= draft.max_nodes:
+        raise ValueError(f"{n} nodes: this DraftKV holds 1 to {draft.max_nodes}")
+    if cfg.n_head != draft.n_head:
+        raise ValueError(f"{cfg.n_head} query heads; the DraftKV was made for {draft.n_head}")
+    if not 0 <= layer < len(draft.k):
+        raise IndexError(f"layer {layer} of {len(draft.k)}")
+    _check("parents", parents, torch.int32, x.device, n)
+    _check("sinks", sinks, torch.float32, x.device, cfg.n_head)
+    _check("out", out, torch.float32, x.device, n * cfg.n_head * cfg.head_dim)
+    if out is None:
+        out = torch.empty((n, cfg.n_head, cfg.head_dim), dtype=torch.float32, device=x.device)
+    return n, out
+
+
+def tree_attn(q: torch.Tensor, cfg: AttnConfig, draft: DraftKV, layer: int, sinks: torch.Tensor | None, window: int,
+              parents: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Sink attention of the nodes' rotated queries (n, n_head * head_dim) over the layer's cache (kv.pos rows) and the
+    rows that draft.k / draft.v hold of their ancestors and themselves, the last `window` positions of those when
+    window > 0 -> (n, n_head, head_dim) fp32."""
+    n, y = _tree(q, cfg.n_head * cfg.head_dim, "q", draft, layer, cfg, sinks, parents, out)
+    kv = draft.kv
+    with torch.cuda.device(q.device):
+        N.check(N.load().nsx_tree_attn(q.data_ptr(), kv.k[layer].data_ptr(), kv.v[layer].data_ptr(), draft._dt,
+                                       draft.k[layer].data_ptr(), draft.v[layer].data_ptr(), _ptr(parents), n,
+                                       draft.max_nodes, _ptr(sinks), cfg.n_head, cfg.n_head_kv, cfg.head_dim,
+                                       kv.pos.data_ptr(), kv.ctx_max, int(window), 1.0 / math.sqrt(cfg.head_dim),
+                                       draft.workspace.data_ptr(), draft.workspace.numel(), y.data_ptr(),
+                                       N.stream_ptr(q.device)), "tree_attn")
+    return y
+
+
+def tree_attn_qkv(qkv: torch.Tensor, bq, bk, bv, cfg: AttnConfig, inv_freq: torch.Tensor, amp: float, draft: DraftKV,
+                  layer: int, sinks: torch.Tensor | None, window: int, parents: torch.Tensor | None = None,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """tree_attn from the nodes' raw q | k | v projections (n, (n_head + 2 n_kv) * head_dim), left unchanged: bias and
+    rotary at each node's position, its key and value rows (in the cache's type) into draft.k / draft.v."""
+    d, dev = cfg.head_dim, qkv.device
+    n, y = _tree(qkv, (cfg.n_head + 2 * cfg.n_head_kv) * d, "qkv", draft, layer, cfg, sinks, parents, out)
+    for name, t, m in (("bq", bq, cfg.n_head * d), ("bk", bk, cfg.n_head_kv * d), ("bv", bv, cfg.n_head_kv * d),
+                       ("inv_freq", inv_freq, d // 2)):
+        _check(name, t, torch.float32, dev, m)
+    kv = draft.kv
+    with torch.cuda.device(dev):
+        N.check(N.load().nsx_tree_attn_qkv(qkv.data_ptr(), _ptr(bq), _ptr(bk), _ptr(bv), inv_freq.data_ptr(),
+                                           float(amp), kv.k[layer].data_ptr(), kv.v[layer].data_ptr(), draft._dt,
+                                           draft.k[layer].data_ptr(), draft.v[layer].data_ptr(), _ptr(parents), n,
+                                           draft.max_nodes, _ptr(sinks), cfg.n_head, cfg.n_head_kv, d,
+                                           kv.pos.data_ptr(), kv.ctx_max, int(window), 1.0 / math.sqrt(d),
+                                           draft.workspace.data_ptr(), draft.workspace.numel(), y.data_ptr(),
+                                           N.stream_ptr(dev)), "tree_attn_qkv")
+    return y
+
+
+def commit(draft: DraftKV, path: torch.Tensor, count: torch.Tensor) -> None:
+    """Rows path[0 .. count - 1] of every layer's nodes into the caches' rows kv.pos, kv.pos + 1, ..., then kv.pos +=
+    count on the device (path, count: device int32, as `verify` returns them for one sequence). The host's kv.length
+    is the caller's to move on, by the count once it is known there."""
+    kv = draft.kv
+    N.require_device(path, count)
+    _check("path", path, torch.int32, kv.k_stack.device)
+    _check("count", count, torch.int32, path.device, 1)
+    n_layer, n_kv, m, d = draft.k_stack.shape
+    if not 1 <= path.numel() <= m:
+        raise ValueError(f"a path of {path.numel()} nodes: 1 to {m}")
+    with torch.cuda.device(path.device):
+        N.check(N.load().nsx_tree_commit(kv.k_stack.data_ptr(), kv.v_stack.data_ptr(), draft.k_stack.data_ptr(),
+                                         draft.v_stack.data_ptr(), draft._dt, n_layer, n_kv, d, path.numel(), m,
+                                         path.data_ptr(), count.data_ptr(), kv.pos.data_ptr(), kv.ctx_max,
+                                         N.stream_ptr(path.device)), "commit")
+
+
+def verify(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tensor | None = None, *,
+           parents: torch.Tensor | None = None, draft_probs: torch.Tensor | None = None, temperature: float = 0.0,
+           lengths: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Which drafted tokens the target model accepts -> (count (B,), path (B, n), token (B,)), int32 on the device.
+
+    logits (n, vocab) or (B, n, vocab) fp32 / fp16 / bf16: row i the target's distribution behind node i. tokens (B, n)
+    int32, node 0 the last known token; uniforms (B, n) fp32 in [0, 1) (not needed at temperature 0). From node 0 on, a
+    drafted child is accepted with the probability that leaves the tokens distributed as softmax(logits / temperature)
+    would draw them: drafts taken as they are, or, with draft_probs (B, n - 1, vocab) fp32, drawn from those (chains).
+    Temperature 0 accepts the largest logit's token, the lowest index of equals. parents: (n,) for all sequences or
+    (B, n); lengths (B,) int32: how many of its nodes each sequence has. count: nodes accepted, node 0 among them;
+    path: their indices, then -1; token: what follows them (drawn with uniforms[:, 0]), -1 where there is none."""
+    if logits.dim() not in (2, 3):
+        raise ValueError(f"logits of shape {tuple(logits.shape)}: (n, vocab) or (B, n, vocab)")
+    N.require_device(logits)
+    dt = N.act_dtype_code(logits.dtype)
+    x = logits if logits.dim() == 3 else logits[None]
+    B, n, V = x.shape
+    dev = x.device
+    # rows may lie apart (a padded vocabulary), all by the same stride
+    ld = x.stride(1) if n > 1 else x.stride(0) if B > 1 else V
+    if V and (x.stride(2) != 1 or ld < V or (n > 1 and B > 1 and x.stride(0) != n * ld)):
+        x = x.contiguous()
+        ld = V
+    _check("tokens", tokens, torch.int32, dev, B * n)
+    _check("uniforms", uniforms, torch.float32, dev, B * n)
+    _check("draft_probs", draft_probs, torch.float32, dev, B * (n - 1) * V)
+    _check("lengths", lengths, torch.int32, dev, B)
+    stride = 0
+    if parents is not None:
+        _check("parents", parents, torch.int32, dev, n if parents.dim() == 1 else B * n)
+        stride = 0 if parents.dim() == 1 else n
+        if draft_probs is not None:
+            raise ValueError("draft probabilities go with chains (no parents)")
+    temperature = float(temperature)
+    if temperature != 0.0 and uniforms is None:
+        raise ValueError("a temperature above 0 needs uniforms")
+    count = torch.empty(B, dtype=torch.int32, device=dev)
+    path = torch.empty((B, n), dtype=torch.int32, device=dev)
+    token = torch.empty(B, dtype=torch.int32, device=dev)
+    lib = N.load()
+    nb = max(0, lib.nsx_verify_workspace_bytes(B, n, V))
+    ws = torch.empty(max(nb, 16), dtype=torch.uint8, device=dev)  # stream-ordered scratch, as the outputs
+    with torch.cuda.device(dev):
+        N.check(lib.nsx_verify(x.data_ptr(), dt, ld, B, n, V, tokens.data_ptr(), _ptr(parents), stride, _ptr(lengths),
+                               _ptr(uniforms), _ptr(draft_probs), temperature, count.data_ptr(), path.data_ptr(),
+                               token.data_ptr(), ws.data_ptr(), ws.numel(), N.stream_ptr(dev)), "verify")
+    return count, path, token
+
+
+__all__ = ["MAX_NODES", "DraftKV", "tree_attn", "tree_attn_qkv", "commit", "verify"]
