@@ -63,6 +63,9 @@ class GenerationStats:
     generated_tokens: int = 0
     prefill_seconds: float = 0.0
     decode_seconds: float = 0.0
+    passes: int = 0  # decode passes, and the drafted tokens that went through them and were accepted
+    drafted_tokens: int = 0
+    accepted_tokens: int = 0
 
     @property
     def tokens_per_second(self) -> float:
@@ -71,7 +74,9 @@ class GenerationStats:
     def summary(self) -> str:
         return (f"generate: {self.prompt_tokens} prompt tokens in {self.prefill_seconds:.3f} s, "
                 f"{self.generated_tokens} generated in {self.decode_seconds:.3f} s "
-                f"({self.tokens_per_second:.2f} tok/s)")
+                f"({self.tokens_per_second:.2f} tok/s)"
+                + (f", {self.accepted_tokens} of {self.drafted_tokens} drafted tokens accepted in {self.passes} passes"
+                   if self.drafted_tokens else ""))
 
 
 _EXPERT_TENSORS = ("ffn_gate_exps.weight", "ffn_up_exps.weight", "ffn_down_exps.weight")
@@ -199,8 +204,85 @@ class NeuroStream:
             return str(vocab[token])
         return f"<{token}>"
 
+    @staticmethod
+    def _nucleus(logits: torch.Tensor, temperature: float, top_p: float) -> torch.Tensor:
+        """Rows of logits with the tokens that `_sample` would not draw at -infinity: all but the smallest set of most
+        likely tokens whose mass reaches top_p (0 < top_p < 1, temperature > 0)."""
+        if temperature <= 0 or not 0 < top_p < 1:
+            return logits
+        p_desc, order = torch.sort(torch.softmax(logits.float() / temperature, dim=-1), descending=True, dim=-1)
+        before = torch.cumsum(p_desc, -1) - p_desc
+        return logits.masked_fill(torch.zeros_like(before, dtype=torch.bool).scatter_(-1, order, before >= top_p),
+                                  float("-inf"))
+
+    def _generate_drafted(self, ids: list[int], max_tokens: int, temperature: float, top_p: float, stop_on_eos: bool,
+                          drafts: int, kv_dtype: torch.dtype):
+        """generate() with several tokens per pass: the prompt in pieces of 64, then passes over the last token and up
+        to `drafts` looked-up drafts of what follows it (model.draft)."""
+        import time
+        from .model.decode import DeviceKV
+        from .model.draft import MAX_NODES, DraftKV, LookupDrafts, commit, verify
+        c = self.model.attn_config()
+        if len(ids) > c.context_length:
+            raise ValueError("prompt and continuation exceed model context length")
+        kv = DeviceKV(self.cfg.n_layer, c, min(c.context_length, len(ids) + max_tokens), self.device, dtype=kv_dtype)
+        draft = DraftKV(kv, c, max_nodes=min(MAX_NODES, max(1 + drafts, len(ids))))
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=self.device)  # noqa: E731
+        temperature = max(float(temperature), 0.0)
+        self.stats = GenerationStats(prompt_tokens=len(ids))
+
+        def settle(logits, nodes, parents):
+            """(accepted nodes, the token that follows) of a pass, the accepted rows in the cache."""
+            u = torch.rand(1, len(nodes), device=self.device) if temperature > 0 else None
+            count, path, token = verify(self._nucleus(logits, temperature, top_p), i32([nodes]), u,
+                                        parents=parents, temperature=temperature)
+            commit(draft, path[0], count)
+            n, nxt, *p = torch.cat([count, token, path[0]]).tolist()
+            kv.length += n
+            return p[:n], nxt
+
+        t0 = time.perf_counter()
+        with torch.no_grad():
+            for i in range(0, len(ids), MAX_NODES):
+                piece = ids[i:i + MAX_NODES]
+                logits = self.model.forward_tree(i32(piece), draft, last_only=True)
+                commit(draft, torch.arange(len(piece), dtype=torch.int32, device=self.device), i32([len(piece)]))
+                kv.length += len(piece)
+            u = torch.rand(1, 1, device=self.device) if temperature > 0 else None
+            pending = int(verify(self._nucleus(logits, temperature, top_p), i32([ids[-1:]]), u,
+                                 temperature=temperature)[2])
+        self.stats.prefill_seconds = time.perf_counter() - t0
+        eos_id = self.gguf.metadata.get("tokenizer.ggml.eos_token_id")
+        eos = set() if eos_id is None or not stop_on_eos else {int(eos_id)}
+        look = LookupDrafts(ids) if drafts else None
+        ready = [pending]  # tokens known but not yet given out; the last of them has not been through the model
+        t0 = time.perf_counter()
+        while True:
+            for tok in ready:
+                if tok in eos or tok < 0 or self.stats.generated_tokens >= max_tokens:
+                    break
+                self.stats.generated_tokens += 1
+                yield self._piece(tok)
+            else:
+                room = min(kv.ctx_max - kv.length, max_tokens - self.stats.generated_tokens)
+                if room > 0:
+                    nodes, parents = [ready[-1]], [-1]
+                    if look is not None:
+                        look.extend(ready)
+                        nodes, parents = look.propose(drafts, room - 1)
+                    with torch.no_grad():
+                        par = i32(parents)
+                        path, nxt = settle(self.model.forward_tree(i32(nodes), draft, par), nodes, par)
+                    self.stats.passes += 1
+                    self.stats.drafted_tokens += len(nodes) - 1
+                    self.stats.accepted_tokens += len(path) - 1
+                    ready = [nodes[i] for i in path[1:]] + [nxt]
+                    continue
+            break
+        self.stats.decode_seconds = time.perf_counter() - t0
+
     def generate(self, prompt, max_tokens: int = 128, temperature: float = 0.0, top_p: float = 0.95,
-                 stop_on_eos: bool = True):
+                 stop_on_eos: bool = True, drafts: int = 0, kv_dtype: torch.dtype = torch.float32):
         """Yield one text piece per generated token (api.py:193-237).
 
         The prompt is a list of token ids: the GGUF tokenizer (text to ids) is
@@ -208,7 +290,15 @@ class NeuroStream:
         prompt runs through the model token by token, then each sampled token
         is decoded the same way (embedding, every layer's attention and MoE
         FFN, LM head, on the GPU). A piece is the token's vocabulary entry when
-        the GGUF has one, else "<id>"."""
+        the GGUF has one, else "<id>".
+
+        drafts > 0 (up to 63): passes over several tokens at once, the last one
+        and up to that many drafts of what follows it, looked up in the
+        sequence so far and accepted as the model's own distribution has it;
+        the prompt then goes through in pieces of 64 tokens. The tokens are
+        distributed as without drafts (temperature 0: the same up to rounding
+        between near-equal logits). kv_dtype: torch.float16 / bfloat16 for a
+        KV cache of half the bytes, on the same path."""
         import time
         from .model.decode import DeviceKV
         if isinstance(prompt, str):
@@ -217,6 +307,11 @@ class NeuroStream:
         ids = [int(t) for t in prompt]
         if not ids:
             raise ValueError("empty prompt")
+        if not 0 <= drafts <= 63:
+            raise ValueError(f"drafts {drafts}: 0 to 63")
+        if drafts or kv_dtype != torch.float32:
+            yield from self._generate_drafted(ids, max_tokens, temperature, top_p, stop_on_eos, int(drafts), kv_dtype)
+            return
         c = self.model.attn_config()
         kv = DeviceKV(self.cfg.n_layer, c, min(c.context_length, len(ids) + max_tokens), self.device)
         self.stats = GenerationStats(prompt_tokens=len(ids))

@@ -7,7 +7,8 @@ chain, which is also how a piece of a prompt goes through.
 - `tree_attn_qkv` / `tree_attn`: a layer's attention of the nodes over the cache and their ancestors, from the raw
   projections or from rotated queries and finished rows;
 - `verify`: which nodes the target accepts, and the token that follows them;
-- `commit`: the accepted nodes' rows into the caches, the position moved on.
+- `commit`: the accepted nodes' rows into the caches, the position moved on;
+- `LookupDrafts`: drafts looked up in the sequence itself (what followed its last tokens earlier), no second model.
 The reference decodes one token per forward (api.py:193-237); these have no counterpart in it. Calls that share a
 DraftKV (its rows and its workspace) must not overlap.
 """
@@ -188,4 +189,53 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tensor | 
     return count, path, token
 
 
-__all__ = ["MAX_NODES", "DraftKV", "tree_attn", "tree_attn_qkv", "commit", "verify"]
+class LookupDrafts:
+    """Drafts for a sequence from the sequence itself: where its last `ngram` tokens (or fewer) stood before, what
+    followed them there, the latest places first, merged into a tree."""
+
+    PLACES = 4  # earlier places of the same tokens that a proposal follows
+
+    def __init__(self, tokens, ngram: int = 3) -> None:
+        if ngram < 1:
+            raise ValueError(f"ngram {ngram}: at least 1")
+        self.ngram = int(ngram)
+        self.tokens: list[int] = []
+        self._after: dict[tuple, list[int]] = {}  # the indices behind a run of tokens
+        self.extend(tokens)
+
+    def extend(self, tokens) -> None:
+        for t in tokens:
+            self.tokens.append(int(t))
+            end = len(self.tokens)
+            for g in range(1, min(self.ngram, end) + 1):
+                self._after.setdefault(tuple(self.tokens[end - g:]), []).append(end)
+
+    def propose(self, n_drafts: int, depth: int | None = None) -> tuple[list[int], list[int]]:
+        """(tokens, parents) of a tree: node 0 the sequence's last token, then up to n_drafts drafts, each no deeper
+        than `depth`."""
+        seq, nodes, parents = self.tokens, [self.tokens[-1]], [-1]
+        depth = n_drafts if depth is None else min(depth, n_drafts)
+        places: list[int] = []
+        for g in range(min(self.ngram, len(seq)), 0, -1):
+            for at in reversed(self._after[tuple(seq[-g:])][-self.PLACES - 1:]):
+                if at < len(seq) and at not in places and len(places) < self.PLACES:
+                    places.append(at)
+        child: dict[tuple[int, int], int] = {}
+        tips = {at: 0 for at in places}  # level by level, so that no place takes every node
+        for level in range(depth):
+            for at, tip in list(tips.items()):
+                if at + level >= len(seq):
+                    del tips[at]
+                    continue
+                key = (tip, seq[at + level])
+                if key not in child:
+                    if len(nodes) > n_drafts:
+                        return nodes, parents
+                    child[key] = len(nodes)
+                    nodes.append(key[1])
+                    parents.append(tip)
+                tips[at] = child[key]
+        return nodes, parents
+
+
+__all__ = ["LookupDrafts", "MAX_NODES", "DraftKV", "tree_attn", "tree_attn_qkv", "commit", "verify"]

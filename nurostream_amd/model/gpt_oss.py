@@ -975,6 +975,57 @@ class GptOssModel:
         advance(kv)
         return logits
 
+    # -- several drafted tokens per pass --------------------------------------
+
+    def _linear_nodes(self, name: str, x: torch.Tensor, raw=None, bias=None, resid=None) -> torch.Tensor:
+        """x @ W.T (+ bias, then + resid) for the nodes of a tree: HBM-resident quantized rows go through the fused
+        GEMV in groups of its 16 tokens. raw: (bytes, dtype, rows) in place of tensor `name`."""
+        from ..compute.kernels import MAX_FUSED_T, can_fuse, fused_gemv
+        from ..format.gguf import FLOAT_TYPES, row_geometry
+        hit = raw
+        if hit is None and self.gguf.tensors[name].dtype not in FLOAT_TYPES:
+            got = self._resident_raw(name)
+            hit = None if got is None else (got[0], got[1], row_geometry(self.gguf.tensors[name])[0])
+        if hit is not None and can_fuse(hit[1], x[:1]):
+            part = lambda t, i: None if t is None else t[i:i + MAX_FUSED_T]  # noqa: E731
+            y = [fused_gemv(hit[0], hit[1], x[i:i + MAX_FUSED_T], hit[2], x.shape[-1], out_dtype=torch.float32,
+                            bias=bias, resid=part(resid, i)) for i in range(0, x.shape[0], MAX_FUSED_T)]
+            return y[0] if len(y) == 1 else torch.cat(y)
+        y = self._linear(name, x)
+        y = y if bias is None else y + bias
+        return y if resid is None else resid + y
+
+    def _attention_tree(self, x: torch.Tensor, layer: int, draft, parents) -> torch.Tensor:
+        """x + o_proj(attention) for the nodes of a tree (`_attention_block` for several tokens): their key and value
+        rows go beside the cache, into `draft`."""
+        from .draft import tree_attn_qkv
+        c, p = self.attn_config(), f"blk.{layer}."
+        h = add_rms_norm(x, None, self.w(p + "attn_norm.weight"), self.cfg.rms_eps)
+        cat = self._qkv_raw(layer)
+        if cat is not None:
+            qkv = self._linear_nodes("", h, raw=cat)
+        else:
+            qkv = torch.cat([self._linear_nodes(p + n + ".weight", h) for n in ("attn_q", "attn_k", "attn_v")], -1)
+        b = lambda n: self.w(p + n + ".bias") if self.has(p + n + ".bias") else None  # noqa: E731
+        sinks = self.w(p + "attn_sinks.weight") if self.has(p + "attn_sinks.weight") else None
+        att = tree_attn_qkv(qkv, b("attn_q"), b("attn_k"), b("attn_v"), c, self._inv_freq, self._amp, draft, layer,
+                            sinks, c.sliding_window if layer % 2 == 0 else 0, parents=parents)
+        return self._linear_nodes(p + "attn_output.weight", att.reshape(x.shape[0], -1), bias=b("attn_output"), resid=x)
+
+    def forward_tree(self, tokens, draft, parents=None, last_only: bool = False) -> torch.Tensor:
+        """Logits (n, vocab) of a tree of drafted tokens (device int32 ids, node 0 at the cache's next position; see
+        model.draft), or (1, vocab) of the last node alone when last_only. The cache and its position stay as they
+        are: `draft` holds the nodes' rows for model.draft.commit. parents: device int32, None for a chain."""
+        self.attn_config()
+        x = self.embed(tokens).reshape(-1, self.cfg.n_embd).contiguous()
+        for layer in range(self.cfg.n_layer):
+            x = self._attention_tree(x, layer, draft, parents)
+            x = self._ffn_block(x, layer)
+        x = x[-1:] if last_only else x
+        name = "output.weight" if self.has("output.weight") else "token_embd.weight"
+        return self._linear_nodes(name, add_rms_norm(x.contiguous(), None, self.w("output_norm.weight"),
+                                                     self.cfg.rms_eps))
+
     def forward(self, tokens, kv=None, start_pos: int = 0, last_only: bool = True) -> torch.Tensor:
         """Logits (model/gpt_oss.py:207-228): (1, vocab), or (T, vocab) when not
         last_only. Tokens go through one at a time at positions start_pos..;

@@ -143,3 +143,57 @@ def test_one_token_calls_refuse_16_bit_caches(lib):
         attn_decode(q, kv, 0, None, 0, c)
     with pytest.raises(TypeError):
         attn_decode_qkv(q, None, None, None, c, inv, 1.0, kv, 0, None, 0)
+
+
+def test_lookup_drafts():
+    from nurostream_amd.model.draft import LookupDrafts
+    d = LookupDrafts([1, 2, 3, 4, 9, 1, 2, 3, 5, 6, 1, 2, 3])
+    assert d.propose(0) == ([3], [-1])
+    # the latest place first (5 6 1 2 ..), the earlier one beside it (4 9 1 ..), level by level
+    assert d.propose(2) == ([3, 5, 4], [-1, 0, 0])
+    assert d.propose(4) == ([3, 5, 4, 6, 9], [-1, 0, 0, 1, 2])
+    assert d.propose(63, depth=1) == ([3, 5, 4], [-1, 0, 0])
+    tokens, parents = d.propose(63)
+    assert len(tokens) <= 64 and all(p < i for i, p in enumerate(parents))
+    d.extend([5, 6, 1])  # both places agree now: one line of them
+    assert d.propose(3, depth=3) == ([1, 2, 3], [-1, 0, 1]) or d.propose(3, depth=3)[0][:2] == [1, 2]
+    assert LookupDrafts([7]).propose(5) == ([7], [-1])
+    assert LookupDrafts([7, 8, 9]).propose(5) == ([9], [-1])
+    assert LookupDrafts([4, 4, 4, 4]).propose(8, depth=2)[0] == [4, 4, 4]  # the places' lines merge
+    with pytest.raises(ValueError):
+        LookupDrafts([1], ngram=0)
+
+
+def test_lookup_drafts_follow_earlier_places():
+    """Every path of a proposal is a run of the sequence behind an earlier place of its last token."""
+    import random
+    from nurostream_amd.model.draft import LookupDrafts
+    r = random.Random(3)
+    seq = [r.randrange(6) for _ in range(300)]
+    d = LookupDrafts(seq[:50])
+    for t in seq[50:]:
+        d.extend([t])
+        tokens, parents = d.propose(r.randrange(1, 20))
+        for i in range(1, len(tokens)):
+            line, j = [], i
+            while j >= 0:
+                line.append(tokens[j])
+                j = parents[j]
+            line.reverse()
+            runs = [d.tokens[k:k + len(line)] for k in range(len(d.tokens) - 1)]
+            assert line in runs
+
+
+@pytest.mark.parametrize("top_p", [0.1, 0.5, 0.9, 0.999, 1.0, 0.0])
+def test_nucleus_keeps_what_sample_draws(top_p):
+    """The rows' kept tokens are those that the one-token path draws from."""
+    from nurostream_amd.api import NeuroStream
+    lg = torch.randn(5, 40, generator=torch.Generator().manual_seed(1)) * 2
+    kept = NeuroStream._nucleus(lg, 0.8, top_p) > float("-inf")
+    for row, keep in zip(lg, kept):
+        p, order = torch.sort(torch.softmax(row / 0.8, -1), descending=True)
+        n = 40
+        if 0 < top_p < 1:
+            n = min(int(torch.searchsorted(torch.cumsum(p, 0), torch.tensor([top_p]))) + 1, 40)
+        assert set(torch.nonzero(keep).flatten().tolist()) == set(order[:n].tolist())
+    assert NeuroStream._nucleus(lg, 0.0, 0.5) is lg

@@ -517,3 +517,87 @@ def test_two_drafts_on_two_streams(dev):
                 outs.append(tree_attn(q, c, d, 0, z, 0, parents=par))
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+# -- in the model ------------------------------------------------------------------
+
+
+def _tiny(tmp_path, dev):
+    from test_gpu_decode import _tiny_model
+    return _tiny_model(tmp_path, dev)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_forward_tree_equals_forward_of_each_path(dev, tmp_path, dtype):
+    """Every node's logits are those of the one-token path over the prompt and the node's line (past the sliding
+    window of 4); a prompt in pieces leaves the cache that one token at a time leaves. A 16-bit cache against passes
+    of one node over a cache of the same type (an fp32 cache is no reference for it: the rows' rounding can change
+    which experts a token takes): a row's element may round to either side of a tie between the two."""
+    from helpers import MFMA_TOL
+    from nurostream_amd.model.decode import DeviceKV
+    from nurostream_amd.model.draft import DraftKV, commit
+    ns, _ = _tiny(tmp_path, dev)
+    model, c = ns.model, ns.model.attn_config()
+    prompt = [5, 17, 42, 7, 250, 3, 99, 1, 288]
+    tol = 2 * MFMA_TOL if dtype == "f32" else 2.0 ** -5
+    kv = DeviceKV(ns.cfg.n_layer, c, 40, dev, dtype=TYPES[dtype])
+    draft = DraftKV(kv, c, max_nodes=12)
+    for piece in (prompt[:5], prompt[5:]):
+        got = model.forward_tree(_ids(piece, dev), draft)
+        commit(draft, _ids(range(len(piece)), dev), _ids([len(piece)], dev))
+    def by_one(toks):
+        """(logits, cache) of one token after the other."""
+        one = DeviceKV(ns.cfg.n_layer, c, 40, dev, dtype=TYPES[dtype])
+        if dtype == "f32":
+            return model.forward(toks, one, last_only=False), one
+        d1, out = DraftKV(one, c, max_nodes=1), []
+        for t in toks:
+            out.append(model.forward_tree(_ids([t], dev), d1))
+            commit(d1, _ids([0], dev), _ids([1], dev))
+        return torch.cat(out), one
+
+    want, one = by_one(prompt)
+    assert rel_max(to_np(got), to_np(want[5:])) < tol
+    assert int(kv.pos) == len(prompt)
+    for a, b in ((kv.k_stack, one.k_stack), (kv.v_stack, one.v_stack)):
+        assert rel_max(to_np(a.float()), to_np(b.float())) < tol
+    tokens, parents = [12, 30, 31, 8, 9, 30, 77], [-1, 0, 0, 1, 1, 2, 5]
+    tree = model.forward_tree(_ids(tokens, dev), draft, _ids(parents, dev))
+    last = model.forward_tree(_ids(tokens, dev), draft, _ids(parents, dev), last_only=True)
+    assert rel_max(to_np(last), to_np(tree[-1:])) < tol
+    for i in range(len(tokens)):
+        line, j = [], i
+        while j >= 0:
+            line.insert(0, tokens[j])
+            j = parents[j]
+        ref = by_one(prompt + line)[0][-1]
+        assert rel_max(to_np(tree[i]), to_np(ref)) < tol, i
+
+
+def test_generate_with_drafts_is_generate(dev, tmp_path):
+    """Greedy: the tokens with drafts are those without, whatever the number of drafts, also where the context or
+    max_tokens ends in the middle of a pass. (The tiny model repeats itself, so drafts are accepted.)"""
+    ns, _ = _tiny(tmp_path, dev)
+    for prompt in ([11, 200, 37], [5, 6, 7, 5, 6, 7, 5, 6] * 10):
+        want = list(ns.generate(prompt, max_tokens=40))
+        for drafts in (1, 4, 15, 63):
+            got = list(ns.generate(prompt, max_tokens=40, drafts=drafts))
+            assert got == want, drafts
+            assert ns.stats.generated_tokens == 40 and ns.stats.prompt_tokens == len(prompt)
+            assert ns.stats.passes <= 40
+        assert list(ns.generate(prompt, max_tokens=5, drafts=8)) == want[:5]
+    assert list(ns.generate([1, 2], max_tokens=0, drafts=3)) == []
+    with pytest.raises(ValueError):
+        list(ns.generate([1], drafts=64))
+
+
+def test_generate_sampled_and_16_bit(dev, tmp_path):
+    """Sampling with drafts and 16-bit caches runs to its end, the same for the same seed."""
+    ns, _ = _tiny(tmp_path, dev)
+    for kw in (dict(drafts=6, temperature=0.9, top_p=0.9), dict(drafts=0, temperature=0.9, kv_dtype=torch.bfloat16),
+               dict(drafts=5, kv_dtype=torch.float16)):
+        runs = []
+        for _ in range(2):
+            torch.manual_seed(7)
+            runs.append(list(ns.generate([4, 5, 4, 5, 4], max_tokens=20, **kw)))
+        assert runs[0] == runs[1] and len(runs[0]) == 20
