@@ -100,35 +100,70 @@ __global__ __launch_bounds__(256) void tree_rope_kernel(const float* __restrict_
   else store_kv<KT>(dk, ((int64_t)rb * max_nodes + node) * ATTN_D + lane, y);
 }
 
-// A 16-byte run of 8 two-byte elements, or two runs of 4 floats 16 dimensions apart, as 8 floats.
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ b8 as_b8(v4u x) { return __builtin_bit_cast(b8, x); }
+
+// Two bf16 from the upper halves of two fp32.
+__device__ __forceinline__ uint32_t top2(float lo, float hi) {
+  return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo), 0x07060302u);
+}
+__device__ __forceinline__ float below(float x) {  // what the upper half leaves of x
+  return x - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & 0xffff0000u);
+}
+// The first NT bf16 terms of 8 fp32: each takes 8 bits toward zero, so three hold all 24, and a product of two values
+// overflows, if at all, with one sign in all of its terms.
+template <int NT>
+__device__ __forceinline__ void split8(const float (&x)[8], v4u (&t)[NT]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+    for (int k = 0; k < NT; ++k) {
+      t[k][i] = top2(a, b);
+      if (k + 1 < NT) a = below(a), b = below(b);
+    }
+  }
+}
+
+// How a wave holds 32 rows of a type: K8, 8 dimensions of a key row; V4, 4 dimensions of a value row; NT, the bf16
+// terms that an element takes exactly.
 template <typename KT>
 struct Rows;
 template <>
 struct Rows<float> {
-  // The 8 dimensions that lane group g of the matrix-core step holds of dimensions 32 j ..: 4 g .. + 3 and the same
-  // 16 further on, so that a load instruction takes 64 contiguous bytes of each row.
+  static constexpr int NT = 3, BYTES = 4 * ATTN_D;
+  // The 8 dimensions that lane group g of a product holds of dimensions 32 j ..: 4 g .. + 3 and the same 16 further on, so
+  // that a load instruction takes 64 contiguous bytes of each row.
   static __device__ __forceinline__ int dim(int j, int g, int e) { return 32 * j + 16 * (e >> 2) + 4 * g + (e & 3); }
   struct K8 {
-    v4f a, b;
+    v4u a, b;
   };
-  using V4 = v4f;
-  static __device__ __forceinline__ K8 k8(const void* row, int j, int g) {
-    const float* p = (const float*)row + 32 * j + 4 * g;
-    return K8{*(const v4f*)p, *(const v4f*)(p + 16)};
+  using V4 = v4u;
+  static __device__ __forceinline__ K8 k8(__amdgpu_buffer_rsrc_t r, int row, int j, int g) {
+    const int o = row * BYTES + 128 * j + 16 * g;
+    return K8{__builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(r, o, 0, 0)),
+              __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(r, o + 64, 0, 0))};
   }
-  static __device__ __forceinline__ V4 v4(const void* row, int i) { return *(const v4f*)((const float*)row + 4 * i); }
-  static __device__ __forceinline__ float k(const K8& x, int e) { return e < 4 ? x.a[e & 3] : x.b[e & 3]; }
-  static __device__ __forceinline__ float v(const V4& x, int d) { return x[d]; }
+  static __device__ __forceinline__ V4 v4(__amdgpu_buffer_rsrc_t r, int row, int i) {
+    return __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(r, row * BYTES + 16 * i, 0, 0));
+  }
+  static __device__ __forceinline__ float k(const K8& x, int e) {
+    return __builtin_bit_cast(float, e < 4 ? x.a[e & 3] : x.b[e & 3]);
+  }
+  static __device__ __forceinline__ float v(const V4& x, int d) { return __builtin_bit_cast(float, (uint32_t)x[d]); }
 };
 template <typename KT>
 struct Rows16 {  // dimensions 32 j + 8 g .. + 7
+  static constexpr int NT = std::is_same_v<KT, Bf16> ? 1 : 2, BYTES = 2 * ATTN_D;
   static __device__ __forceinline__ int dim(int j, int g, int e) { return 32 * j + 8 * g + e; }
   using K8 = v4u;
   using V4 = v2u;
-  static __device__ __forceinline__ K8 k8(const void* row, int j, int g) {
-    return *(const v4u*)((const uint16_t*)row + 32 * j + 8 * g);
+  static __device__ __forceinline__ K8 k8(__amdgpu_buffer_rsrc_t r, int row, int j, int g) {
+    return __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(r, row * BYTES + 64 * j + 16 * g, 0, 0));
   }
-  static __device__ __forceinline__ V4 v4(const void* row, int i) { return *(const v2u*)((const uint16_t*)row + 4 * i); }
+  static __device__ __forceinline__ V4 v4(__amdgpu_buffer_rsrc_t r, int row, int i) {
+    return __builtin_bit_cast(v2u, __builtin_amdgcn_raw_buffer_load_b64(r, row * BYTES + 8 * i, 0, 0));
+  }
   static __device__ __forceinline__ float one(uint32_t w, int hi) {
     if constexpr (std::is_same_v<KT, Bf16>) return __builtin_bit_cast(float, hi ? w & 0xffff0000u : w << 16);
     else return nsx_h2f(hi ? w >> 16 : w & 0xffffu);
@@ -141,6 +176,32 @@ struct Rows<_Float16> : Rows16<_Float16> {};
 template <>
 struct Rows<Bf16> : Rows16<Bf16> {};
 
+template <typename KT>
+__device__ __forceinline__ void key_terms(const typename Rows<KT>::K8& x, v4u (&t)[Rows<KT>::NT]) {
+  if constexpr (Rows<KT>::NT == 1) {
+    t[0] = x;
+  } else {
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = Rows<KT>::k(x, e);
+    split8(f, t);
+  }
+}
+// Dimension d of a lane's 8 value rows.
+template <typename KT>
+__device__ __forceinline__ void value_terms(const typename Rows<KT>::V4 (&x)[8], int d, v4u (&t)[Rows<KT>::NT]) {
+  if constexpr (Rows<KT>::NT == 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      t[0][i] = __builtin_amdgcn_perm(x[2 * i + 1][d >> 1], x[2 * i][d >> 1], d & 1 ? 0x07060302u : 0x05040100u);
+  } else {
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = Rows<KT>::v(x[e], d);
+    split8(f, t);
+  }
+}
+
 __device__ __forceinline__ void lds_barrier() {  // LDS writes visible; global loads stay in flight
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
@@ -152,20 +213,29 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028235e3
 // nodes' own rows in tiles of their own; a split is a run of tiles and wave w takes every TREE_NW'th of them. Splits
 // past the present length return at once: the grid goes by ctx_max, so that it does not depend on the position.
 //
-// A tile: scores by v_mfma_f32_16x16x4_f32 (A = 16 keys x 4 dimensions, B = 4 dimensions x 16 columns), each lane
-// holding key l % 16 and 8 of every 32 dimensions; lane l's results are column l % 16 and keys 4 (l / 16) .. + 3 of each
-// 16. These are the B operand of the second product as they stand, when A's lane l holds of each value row the keys
-// of its group and dimensions 4 (l % 16) ..: D then has column l % 16, dimensions 16 (l / 16) + 4 r + dt. So every row
-// is read once by one wave, in 16-byte pieces, and nothing is exchanged but the running maximum (two shuffles).
+// A tile: scores by v_mfma_f32_16x16x32_bf16, A = 16 keys x 32 dimensions, B = 32 dimensions x 16 columns, an element
+// being the sum of its bf16 terms (three of an fp32 value, two of an fp16 one, exactly; of their products those of
+// 2^-22 and less are left out). Lane l's results are column l % 16 and keys 4 (l / 16) .. + 3 of each 16: the B operand
+// of the second product as they stand, when A's lane l holds of each value row the keys of its group and dimensions
+// 4 (l % 16) ..; D then has column l % 16, dimensions 16 (l / 16) + 4 r + dt. So every row is read once by one wave, in
+// pieces of 8 or 16 bytes, and turned into terms once for the wave's 16 NC columns, whose own terms lie in LDS.
+//
+// The softmax's reference m only moves (and the sums are only rescaled) when a tile has a score beyond 2^8 times it:
+// weights stay below 2^8, a sum of 2^31 of them below 2^39. So a tile mostly needs no exchange between lanes.
 //
 // A key with weight zero takes no part whatever its value row holds (0 * NaN would be NaN): a wave whose sums are not
-// finite at the end goes through its tiles again, adding values one key at a time under their weights.
+// finite at the end goes through its tiles again, with products in fp32 and values added one key at a time under their
+// weights. (That is also what infinite keys and values take: of their terms the second is NaN.)
 template <typename KT, int NC>
-__global__ __launch_bounds__(64 * TREE_NW) void tree_attn_kernel(TreeArgs a) {
+__global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) {
   using R = Rows<KT>;
-  constexpr int NT = 64 * TREE_NW, COLS = 16 * NC, QS = ATTN_D + 4;
-  __shared__ __align__(16) float qs[COLS][QS];  // the columns' queries
-  __shared__ __align__(16) float sacc[TREE_NW][COLS][QS];
+  constexpr int NT = 64 * TREE_NW, COLS = 16 * NC, KTN = R::NT;
+  constexpr int QROW = 2 * ATTN_D + 16, OROW = ATTN_D + 4;  // bytes of a column's term, floats of a column's sums
+  constexpr int QBYTES = 3 * COLS * QROW, PBYTES = TREE_KEYS * COLS * 4;
+  constexpr int LDS = std::max(QBYTES + TREE_NW * PBYTES, TREE_NW * COLS * OROW * 4);
+  // first the columns' query terms [term][column] and behind them each wave's weights of a tile (the second way); in the
+  // end each wave's sums
+  __shared__ __align__(16) uint8_t lds[LDS];
   __shared__ float sm[TREE_NW][COLS], sl[TREE_NW][COLS];
   __shared__ uint64_t svis[64];
   __shared__ int sdep[64];
@@ -180,6 +250,32 @@ __global__ __launch_bounds__(64 * TREE_NW) void tree_attn_kernel(TreeArgs a) {
   const int t0 = c * per, t1 = min(nt, t0 + per);
   if (t0 >= t1) return;
   const int ncol = a.nodes * a.n_rep, col0 = cb * COLS;
+
+  typename R::K8 kr[2][2];
+  typename R::V4 vr[8];
+  auto rsrc = [&](int tile, bool values) {  // rows past the last read as zero
+    const bool own = tile >= pt;
+    const int r0 = own ? (tile - pt) * TREE_KEYS : lo + tile * TREE_KEYS, rows = (own ? a.nodes : P) - r0;
+    const char* base = (const char*)(own ? (values ? a.dv : a.dk) : (values ? a.vc : a.kc));
+    return nsx_rsrc(base + ((int64_t)g * (own ? a.max_nodes : a.ctx_max) + r0) * R::BYTES,
+                    (uint32_t)min(rows, TREE_KEYS) * R::BYTES);
+  };
+  auto load_k = [&](int tile) {
+    const auto r = rsrc(tile, false);
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) kr[kt][j] = R::k8(r, 16 * kt + i16, j, kq);
+  };
+  auto load_v = [&](int tile) {
+    const auto r = rsrc(tile, true);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) vr[e] = R::v4(r, 16 * (e >> 2) + 4 * kq + (e & 3), i16);
+  };
+  const int first = t0 + wave, last = t1 - 1;
+  load_k(min(first, last));
+  load_v(min(first, last));
+
   if (wave == 0) {
     uint64_t line = tree_lineage(a.parents, a.nodes, lane);
     const int dep = __popcll(line) - 1;
@@ -190,31 +286,37 @@ __global__ __launch_bounds__(64 * TREE_NW) void tree_attn_kernel(TreeArgs a) {
     svis[lane] = line;
     sdep[lane] = dep;
   }
-  for (int i = t; i < COLS * (ATTN_D / 4); i += NT) {
-    const int col = min(col0 + i / (ATTN_D / 4), ncol - 1), d = i % (ATTN_D / 4) * 4;
+  for (int i = t; i < COLS * (ATTN_D / 8); i += NT) {
+    const int cc = i / (ATTN_D / 8), col = min(col0 + cc, ncol - 1), j = i / 4 % 2, gg = i % 4;
     const int node = col / a.n_rep, h = g * a.n_rep + col % a.n_rep;
-    *(v4f*)&qs[i / (ATTN_D / 4)][d] = *(const v4f*)(a.q + ((int64_t)node * a.n_head + h) * ATTN_D + d);
+    const float* qp = a.q + ((int64_t)node * a.n_head + h) * ATTN_D;
+    const v4f x0 = *(const v4f*)(qp + R::dim(j, gg, 0)), x1 = *(const v4f*)(qp + R::dim(j, gg, 4));
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = (e < 4 ? x0[e & 3] : x1[e & 3]) * a.scale2;
+    v4u tm[3];
+    split8(x, tm);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) *(v4u*)&lds[(k * COLS + cc) * QROW + (4 * j + gg) * 16] = tm[k];
   }
   lds_barrier();
-  uint64_t vis[NC];
-  int from[NC], deepest = 0;  // the column's first visible cache row
+  int q0 = i16 * QROW + kq * 16;
+  auto query = [&](int k, int ct, int j) { return *(const v4u*)&lds[q0 + (k * COLS + 16 * ct) * QROW + 64 * j]; };
+  // a column's node: what it sees of the nodes, its first visible row of the cache
+  auto node_of = [&](int ct) { return min(col0 + 16 * ct + i16, ncol - 1) / a.n_rep; };
+  int deepest = 0;  // the last of the columns' first rows
+  if (a.window > 0) {
 #pragma unroll
-  for (int ct = 0; ct < NC; ++ct) {
-    const int node = min(col0 + 16 * ct + i16, ncol - 1) / a.n_rep;
-    vis[ct] = svis[node];
-    from[ct] = a.window > 0 ? P + sdep[node] + 1 - a.window : 0;
-    deepest = max(deepest, from[ct]);
+    for (int ct = 0; ct < NC; ++ct) deepest = max(deepest, P + sdep[node_of(ct)] + 1 - a.window);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) deepest = max(deepest, __shfl_xor(deepest, o, 64));
+    deepest = __builtin_amdgcn_readfirstlane(deepest);
   }
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) deepest = max(deepest, __shfl_xor(deepest, o, 64));
-  deepest = __builtin_amdgcn_readfirstlane(deepest);
 
   float m[NC], l[NC];
   v4f acc[NC][4];
-  float* sp = &sacc[wave][0][0];  // the second way's weights, [key][column]
-  static_assert(TREE_KEYS * COLS <= COLS * QS, "weights of a tile in the wave's part of sacc");
-  auto pass = [&](auto slow_tag) {
-    constexpr bool SLOW = decltype(slow_tag)::value;
+  float* sp = (float*)&lds[QBYTES + wave * PBYTES];  // the second way's weights, [key][column]
+  auto start = [&] {
 #pragma unroll
     for (int ct = 0; ct < NC; ++ct) {
       m[ct] = ATTN_LOWEST;
@@ -222,94 +324,114 @@ __global__ __launch_bounds__(64 * TREE_NW) void tree_attn_kernel(TreeArgs a) {
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt) acc[ct][dt] = v4f{0.f, 0.f, 0.f, 0.f};
     }
-    for (int tile = t0 + wave; tile < t1; tile += TREE_NW) {
-      const bool own = tile >= pt;  // the nodes' rows
-      const int r0 = own ? (tile - pt) * TREE_KEYS : lo + tile * TREE_KEYS, last = (own ? a.nodes : P) - 1;
-      const int64_t base = ((int64_t)g * (own ? a.max_nodes : a.ctx_max)) * (ATTN_D * (int64_t)sizeof(KT));
-      const char* kb = (const char*)(own ? a.dk : a.kc) + base;
-      const char* vb = (const char*)(own ? a.dv : a.vc) + base;
-      auto row = [&](int k) { return (int64_t)min(r0 + k, last) * (ATTN_D * (int64_t)sizeof(KT)); };
-      typename R::K8 kr[2][2];
-      typename R::V4 vr[8];
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) kr[kt][j] = R::k8(kb + row(16 * kt + i16), j, kq);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) vr[e] = R::v4(vb + row(16 * (e >> 2) + 4 * kq + (e & 3)), i16);
-      const bool masked = own || r0 + TREE_KEYS > P || r0 < deepest;
+  };
+  // scores in powers of two -> weights; what a column does not see has none
+  auto weights = [&](int tile, v4f (&s)[NC][2]) {
+    const bool own = tile >= pt;
+    const int r0 = own ? (tile - pt) * TREE_KEYS : lo + tile * TREE_KEYS;
+    if (own || r0 + TREE_KEYS > P || r0 < deepest) {
 #pragma unroll
       for (int ct = 0; ct < NC; ++ct) {
-        v4f s[2] = {};
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float qv[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) qv[e] = qs[16 * ct + i16][R::dim(j, kq, e)];
-#pragma unroll
-          for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              s[kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(R::k(kr[kt][j], e), qv[e], s[kt], 0, 0, 0);
-        }
-        float p[8], mx = ATTN_LOWEST;
+        const int node = node_of(ct);
+        const int from = a.window > 0 ? P + sdep[node] + 1 - a.window : 0;
+        const uint64_t all = own ? svis[node] : ~0ull;
+        const int lo_k = own ? 0 : from - r0, hi_k = (own ? a.nodes : P) - r0;
+        const uint32_t bits = (uint32_t)(own ? all >> r0 : all);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          p[e] = s[e >> 2][e & 3] * a.scale2;
-          if (masked) {
-            const int k = r0 + 16 * (e >> 2) + 4 * kq + (e & 3);
-            const bool on = own ? k < a.nodes && (vis[ct] >> k & 1) : k < P && k >= from[ct];
-            p[e] = on ? p[e] : -INFINITY;
-          }
-          mx = fmaxf(mx, p[e]);
-        }
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        const float mn = fmaxf(m[ct], fmaxf(mx, __shfl_xor(mx, 32, 64)));
-        const float corr = __builtin_amdgcn_exp2f(m[ct] - mn);  // (first tile: of nothing)
-        m[ct] = mn;
-        float ls = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          p[e] = __builtin_amdgcn_exp2f(p[e] - mn);
-          ls += p[e];
-        }
-        l[ct] = fmaf(l[ct], corr, ls);  // this lane group's keys; the groups are added at the end
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt) acc[ct][dt] *= corr;
-        if constexpr (!SLOW) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-#pragma unroll
-            for (int dt = 0; dt < 4; ++dt)
-              acc[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(R::v(vr[e], dt), p[e], acc[ct][dt], 0, 0, 0);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) sp[(16 * (e >> 2) + 4 * kq + (e & 3)) * COLS + 16 * ct + i16] = p[e];
-        }
-      }
-      if constexpr (SLOW) {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll 1
-        for (int k = 0; k < TREE_KEYS; ++k) {
-          const char* vrow = vb + row(k);
-          typename R::V4 v[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = R::v4(vrow, 4 * kq + r);
-#pragma unroll
-          for (int ct = 0; ct < NC; ++ct) {
-            const float w = sp[k * COLS + 16 * ct + i16];
-            if (w != 0.f) {
-#pragma unroll
-              for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) acc[ct][dt][r] = fmaf(w, R::v(v[r], dt), acc[ct][dt][r]);
-            }
-          }
+          const int k = 16 * (e >> 2) + 4 * kq + (e & 3);
+          const bool on = k >= lo_k && k < hi_k && (bits >> k & 1);
+          s[ct][e >> 2][e & 3] = on ? s[ct][e >> 2][e & 3] : -INFINITY;
         }
       }
     }
+    float mx[NC];
+    bool move = false;
+#pragma unroll
+    for (int ct = 0; ct < NC; ++ct) {
+      mx[ct] = fmaxf(s[ct][0][0], s[ct][0][1]);
+#pragma unroll
+      for (int e = 2; e < 8; ++e) mx[ct] = fmaxf(mx[ct], s[ct][e >> 2][e & 3]);
+      move = move || mx[ct] > m[ct] + 8.f;
+    }
+    if (__any(move)) {
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct) {
+        float mn = fmaxf(mx[ct], __shfl_xor(mx[ct], 16, 64));
+        mn = fmaxf(m[ct], fmaxf(mn, __shfl_xor(mn, 32, 64)));
+        const float corr = __builtin_amdgcn_exp2f(m[ct] - mn);  // (first tile: of nothing)
+        m[ct] = mn;
+        l[ct] *= corr;
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) acc[ct][dt] *= corr;
+      }
+    }
+#pragma unroll
+    for (int ct = 0; ct < NC; ++ct) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float w = __builtin_amdgcn_exp2f(s[ct][e >> 2][e & 3] - m[ct]);
+        s[ct][e >> 2][e & 3] = w;
+        l[ct] += w;  // this lane group's keys; the groups are added at the end
+      }
+    }
   };
-  pass(std::false_type{});
+
+  start();
+  for (int tile = first; tile < t1; tile += TREE_NW) {
+    const int next = min(tile + TREE_NW, last);
+    if constexpr (NC > 2) asm volatile("" : "+v"(q0));  // 96 registers of query terms are read anew for each tile
+    v4f s[NC][2] = {};
+    {
+      v4u kt_[2][2][KTN];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) key_terms<KT>(kr[kt][j], kt_[kt][j]);
+      load_k(next);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int ct = 0; ct < NC; ++ct) {
+          v4u q[3];
+#pragma unroll
+          for (int k = 0; k < 3; ++k) q[k] = query(k, ct, j);
+#pragma unroll
+          for (int o = 2; o >= 0; --o)  // (the small products first)
+#pragma unroll
+            for (int k = 0; k <= o; ++k)
+              if (o - k < KTN) {
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+                  s[ct][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(kt_[kt][j][o - k]), as_b8(q[k]), s[ct][kt], 0, 0, 0);
+              }
+        }
+    }
+    weights(tile, s);
+    v4u pw[NC][3];
+#pragma unroll
+    for (int ct = 0; ct < NC; ++ct) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = s[ct][e >> 2][e & 3];
+      split8(x, pw[ct]);
+    }
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) {
+      v4u vt[KTN];
+      value_terms<KT>(vr, dt, vt);
+      if (dt == 3) load_v(next);
+#pragma unroll
+      for (int o = 2; o >= 0; --o)
+#pragma unroll
+        for (int k = 0; k <= o; ++k)
+          if (o - k < KTN) {
+#pragma unroll
+            for (int ct = 0; ct < NC; ++ct)
+              acc[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(vt[o - k]), as_b8(pw[ct][k]), acc[ct][dt], 0, 0, 0);
+          }
+    }
+  }
   bool ok = true;
 #pragma unroll
   for (int ct = 0; ct < NC; ++ct)
@@ -317,8 +439,56 @@ __global__ __launch_bounds__(64 * TREE_NW) void tree_attn_kernel(TreeArgs a) {
     for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
       for (int r = 0; r < 4; ++r) ok = ok && finite(acc[ct][dt][r]);
-  if (!__all(ok)) pass(std::true_type{});
+  if (!__all(ok)) {
+    start();
+#pragma unroll 1
+    for (int tile = first; tile < t1; tile += TREE_NW) {
+      load_k(tile);
+      v4f s[NC][2] = {};
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const v4u qa = query(0, ct, j), qb = query(1, ct, j), qc = query(2, ct, j);
+          auto term = [](const v4u& x, int e) {
+            return __builtin_bit_cast(float, e & 1 ? x[e >> 1] & 0xffff0000u : x[e >> 1] << 16);
+          };
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float q = term(qa, e) + (term(qb, e) + term(qc, e));
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+              s[ct][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(R::k(kr[kt][j], e), q, s[ct][kt], 0, 0, 0);
+          }
+        }
+      weights(tile, s);
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sp[(16 * (e >> 2) + 4 * kq + (e & 3)) * COLS + 16 * ct + i16] = s[ct][e >> 2][e & 3];
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      const auto r = rsrc(tile, true);
+#pragma unroll 1
+      for (int k = 0; k < TREE_KEYS; ++k) {
+        typename R::V4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = R::v4(r, k, 4 * kq + u);
+#pragma unroll
+        for (int ct = 0; ct < NC; ++ct) {
+          const float w = sp[k * COLS + 16 * ct + i16];
+          if (w != 0.f) {
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+              for (int u = 0; u < 4; ++u) acc[ct][dt][u] = fmaf(w, R::v(v[u], dt), acc[ct][dt][u]);
+          }
+        }
+      }
+    }
+  }
 
+  lds_barrier();  // (the sums take the query terms' place)
+  float(*sacc)[COLS][OROW] = (float(*)[COLS][OROW])lds;
 #pragma unroll
   for (int ct = 0; ct < NC; ++ct) {
     l[ct] += __shfl_xor(l[ct], 16, 64);
