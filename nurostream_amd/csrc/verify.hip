@@ -12,20 +12,27 @@
 // at which the running sum of the weights exceeds node 0's random number times their total. Temperature 0: p is one
 // at the largest logit, the lowest index of equals.
 //
-// Exponentials, sums and comparisons in 64 bits: a vocabulary's running sum is compared with a random number. A NaN
-// logit counts as -infinity; of +infinity in a row, its tokens share the row's whole weight; a row without any weight
-// gives the token -1. Sequences with no nodes (length 0) give count 0 and token -1.
+// Sums and comparisons in 64 bits, weights to 2^-35 of themselves: a vocabulary's running sum is compared with a random
+// number, and with 32-bit weights the answer would be another one in about one draw of a million. A NaN logit counts
+// as -infinity; of +infinity in a row, its tokens share the row's whole weight; a row without any weight gives the
+// token -1. Sequences with no nodes (length 0) give count 0 and token -1.
+//
+// Launches: the rows' chunk sums (all logits once: the bytes, 5 TB/s, and some 11 64-bit operations per logit bound
+// it), the walk with the draw of one workgroup per sequence, and only for drafts from q, whose residual needs the last
+// row's whole sum first, that row's chunk sums of max(p - q, 0) and the draw from them.
 #include "nsx_common.h"
 
 #include <algorithm>
+#include <type_traits>
 #include <math.h>
 
 namespace {
 
-constexpr int VF_CHUNK = 4096;  // logits per workgroup of the row passes
-constexpr int VF_THREADS = 256;
-constexpr int VF_PER = VF_CHUNK / VF_THREADS;
-constexpr int VF_MAX_CHUNKS = 1024;  // chunks of a row that one workgroup's threads hold four each
+constexpr int VF_CHUNK = 4096;       // logits per workgroup of the row passes
+constexpr int VF_THREADS = 256;      // of the row passes
+constexpr int VF_WALK = 1024;        // of the walk and the draw
+constexpr int VF_MAX_CHUNKS = 1024;
+constexpr int VF_VEC = 8;            // chunks begin where the row's address is a multiple of this many elements
 
 // A chunk's largest logit, its (lowest) index and the weights' sum relative to it.
 struct Part {
@@ -33,80 +40,144 @@ struct Part {
   int32_t at;
   double s;
 };
+// The node that the draw is from (-1: nothing left to draw), its row's largest logit and sum.
+struct Last {
+  int32_t node;
+  float M;
+  double Z;
+};
 
 struct VerifyArgs {
   const void* logits;
-  int dtype;
   int64_t row_stride;  // elements
   int B, n;
   int64_t V;
   const int32_t *tokens, *parents, *lengths;
   int64_t parents_stride;  // 0: one tree for all sequences
   const float *u, *q;
-  double inv_temp;  // 0: greedy
+  double scale2;  // log2(e) / temperature; 0: greedy
   int32_t *count, *path, *token;
   int nchunk;
-  Part* part;      // [B * n][nchunk]
-  double* resid;   // q: [B][nchunk], the sums of max(p - q, 0) at the last node
-  int32_t* state;  // q: [B], the last node reached where a child was refused there, else -1
+  Part* part;     // [B * n][nchunk]
+  double* resid;  // q: [B][nchunk], the sums of max(p - q, 0) at the last node
+  Last* last;     // q: [B]
 };
 
-__device__ __forceinline__ float vf_logit(const VerifyArgs& a, int64_t row, int64_t i) {
-  const float x = nsx_load_act(a.logits, a.dtype, row * a.row_stride + i);
-  return x == x ? x : -INFINITY;
+template <typename LT>  // float, _Float16, or uint16_t for bf16
+struct Row {
+  const LT* p;
+  int off;  // elements that the row's start lies behind a multiple of VF_VEC
+  __device__ __forceinline__ Row(const VerifyArgs& a, int64_t row)
+      : p((const LT*)a.logits + row * a.row_stride), off((int)((uintptr_t)p / sizeof(LT) % VF_VEC)) {}
+  static __device__ __forceinline__ float value(LT x) {
+    float f;
+    if constexpr (sizeof(LT) == 4) f = x;
+    else if constexpr (std::is_same_v<LT, _Float16>) f = (float)x;
+    else f = nsx_bf2f(x);
+    return f == f ? f : -INFINITY;
+  }
+  __device__ __forceinline__ float at(int64_t i) const { return value(p[i]); }
+  // The N elements from place v (a multiple of N) of the row's chunks on; -infinity where the row has none.
+  template <int N>
+  __device__ __forceinline__ void run(int64_t v, int64_t V, float (&x)[N]) const {
+    const int64_t i = v - off;
+    if (i >= 0 && i + N <= V) {
+      struct alignas(N * sizeof(LT)) Vec {
+        LT e[N];
+      };
+      const Vec w = *(const Vec*)(p + i);
+#pragma unroll
+      for (int k = 0; k < N; ++k) x[k] = value(w.e[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k) x[k] = i + k >= 0 && i + k < V ? at(i + k) : -INFINITY;
+    }
+  }
+};
+
+// 2^(j / 16) in LDS: sixteen entries on banks of their own.
+struct Pow2 {
+  double t[16];
+  __device__ __forceinline__ void fill() {
+    if (threadIdx.x < 16) t[threadIdx.x] = exp2((double)threadIdx.x / 16);
+  }
+};
+
+// The weight 2^(scale2 (x - M)) of logit x beside the largest, M > -infinity. y = n + j / 16 + r with |r| <= 1 / 32 by
+// adding 1.5 * 2^48; 2^r - 1 = r ln2 + r^2 (..), the last part (below 2.4e-4) in 32 bits: an error of 2^-35. Below
+// 2^-1020 it is zero.
+__device__ __forceinline__ double vf_weight(float x, float M, double scale2, const Pow2& tab) {
+  if (M == INFINITY) return x == M ? 1.0 : 0.0;
+  const double y = ((double)x - (double)M) * scale2;
+  const double t = y + 0x1.8p48;
+  const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
+  const double r = y - (t - 0x1.8p48);
+  const float f = (float)r;
+  // ln2^2 / 2, ln2^3 / 6, ln2^4 / 24, ln2^5 / 120
+  const float q = f * f * fmaf(f, fmaf(f, fmaf(f, 0.0013333558f, 0.0096181291f), 0.055504109f), 0.24022651f);
+  const double c = tab.t[k & 15], w = fma(fma(r, 0.69314718055994530942, (double)q), c, c);
+  const uint64_t bits = __builtin_bit_cast(uint64_t, w) + ((uint64_t)(uint32_t)(k >> 4) << 52);
+  return y < -1020.0 ? 0.0 : __builtin_bit_cast(double, bits);
 }
 
-// The weight of logit x beside the largest, M > -infinity.
-__device__ __forceinline__ double vf_weight(float x, float M, double inv_temp) {
-  return x == M ? 1.0 : exp(((double)x - (double)M) * inv_temp);  // (equals first: their difference may be of infinities)
-}
-
-template <typename T, typename Op>
-__device__ __forceinline__ T vf_block_reduce(T v, T* red, Op op) {  // over 256 threads, the same order in each
+template <int WAVES, typename T, typename Op>
+__device__ __forceinline__ T vf_block_reduce(T v, T* red, Op op) {  // the same order in every thread
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
-  __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  return op(op(red[0], red[1]), op(red[2], red[3]));
+  v = red[0];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) v = op(v, red[w]);
+  return v;
 }
 
-// Elements of chunk c of a row: element c * VF_CHUNK + 256 u + thread.
+template <typename LT, bool GREEDY>
 __global__ __launch_bounds__(VF_THREADS) void verify_stats_kernel(VerifyArgs a) {
+  constexpr int W = 16 / sizeof(LT), RUNS = VF_CHUNK / VF_THREADS / W;  // elements of a 16-byte load, loads
   __shared__ float redf[4];
   __shared__ int redi[4];
   __shared__ double redd[4];
+  __shared__ Pow2 tab;
   const int64_t row = blockIdx.y;
-  const int c = blockIdx.x;
-  const int64_t i0 = (int64_t)c * VF_CHUNK;
-  float x[VF_PER], m = -INFINITY;
+  const int c = blockIdx.x, t = threadIdx.x;
+  const Row<LT> r(a, row);
+  float x[RUNS][W], m = -INFINITY;
 #pragma unroll
-  for (int u = 0; u < VF_PER; ++u) {
-    const int64_t i = i0 + VF_THREADS * u + threadIdx.x;
-    x[u] = i < a.V ? vf_logit(a, row, i) : -INFINITY;
-    m = fmaxf(m, x[u]);
-  }
-  m = vf_block_reduce(m, redf, [](float p, float q) { return fmaxf(p, q); });
+  for (int u = 0; u < RUNS; ++u) r.run((int64_t)c * VF_CHUNK + (u * VF_THREADS + t) * W, a.V, x[u]);
+  if (!GREEDY) tab.fill();
+#pragma unroll
+  for (int u = 0; u < RUNS; ++u)
+#pragma unroll
+    for (int k = 0; k < W; ++k) m = fmaxf(m, x[u][k]);
+  m = vf_block_reduce<4>(m, redf, [](float p, float q) { return fmaxf(p, q); });
   int at = 0x7fffffff;
-  double s = 0.0;
 #pragma unroll
-  for (int u = VF_PER - 1; u >= 0; --u) {
-    const int64_t i = i0 + VF_THREADS * u + threadIdx.x;
-    if (x[u] == m && i < a.V) at = (int)i;
-    if (a.inv_temp != 0.0 && m > -INFINITY) s += vf_weight(x[u], m, a.inv_temp);
+  for (int u = RUNS - 1; u >= 0; --u)
+#pragma unroll
+    for (int k = W - 1; k >= 0; --k)
+      if (x[u][k] == m) at = (int)((int64_t)c * VF_CHUNK + (u * VF_THREADS + t) * W + k - r.off);
+  double s = 0.0;
+  if (!GREEDY && m > -INFINITY) {
+#pragma unroll
+    for (int u = 0; u < RUNS; ++u)
+#pragma unroll
+      for (int k = 0; k < W; ++k) s += vf_weight(x[u][k], m, a.scale2, tab);
   }
-  at = vf_block_reduce(at, redi, [](int p, int q) { return min(p, q); });
-  s = vf_block_reduce(s, redd, [](double p, double q) { return p + q; });
-  if (threadIdx.x == 0) a.part[row * a.nchunk + c] = Part{m, at, s};
+  at = vf_block_reduce<4>(at, redi, [](int p, int q) { return min(p, q); });
+  if (!GREEDY) s = vf_block_reduce<4>(s, redd, [](double p, double q) { return p + q; });
+  if (t == 0) a.part[row * a.nchunk + c] = Part{m, at, s};
 }
 
 // The row's largest logit, its index and the weights' sum, from its chunks: one wave.
-__device__ __forceinline__ Part vf_row(const VerifyArgs& a, int64_t row, int lane) {
+__device__ __forceinline__ Part vf_row(const VerifyArgs& a, int64_t row, int lane, const Pow2& tab) {
   const Part* p = a.part + row * a.nchunk;
-  float M = -INFINITY;
-  int at = 0x7fffffff;
-  for (int c = lane; c < a.nchunk; c += 64)
-    if (p[c].m > M || at == 0x7fffffff) M = p[c].m, at = p[c].at;
+  const Part none{-INFINITY, 0x7fffffff, 0.0};
+  const Part p0 = lane < a.nchunk ? p[lane] : none;  // (most vocabularies: the only ones)
+  float M = p0.m;
+  int at = p0.at;
+  for (int c = lane + 64; c < a.nchunk; c += 64)
+    if (p[c].m > M) M = p[c].m, at = p[c].at;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     const float m2 = __shfl_xor(M, o, 64);
@@ -114,242 +185,298 @@ __device__ __forceinline__ Part vf_row(const VerifyArgs& a, int64_t row, int lan
     if (m2 > M || (m2 == M && a2 < at)) M = m2, at = a2;
   }
   double s = 0.0;
-  if (a.inv_temp != 0.0 && M > -INFINITY)
-    for (int c = lane; c < a.nchunk; c += 64)
-      if (p[c].m > -INFINITY) s += p[c].s * vf_weight(p[c].m, M, a.inv_temp);
+  if (a.scale2 != 0.0 && M > -INFINITY) {
+    if (p0.m > -INFINITY) s = p0.s * vf_weight(p0.m, M, a.scale2, tab);
+    for (int c = lane + 64; c < a.nchunk; c += 64)
+      if (p[c].m > -INFINITY) s += p[c].s * vf_weight(p[c].m, M, a.scale2, tab);
+  }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
   return Part{M, at, s};
 }
 
-// What the draw needs of the last node.
-struct Last {
-  int node;
-  float M;
-  double Z;
-  bool refused;
-};
-
-// The weight of token i at the last node; refused: the refused tokens (drafts without probabilities).
-__device__ __forceinline__ double vf_left(const VerifyArgs& a, int b, const Last& z, const int* refused, int nref,
-                                          int64_t i) {
-  double w = vf_weight(vf_logit(a, (int64_t)b * a.n + z.node, i), z.M, a.inv_temp);
-  if (a.q && z.refused) return fmax(w / z.Z - (double)a.q[((int64_t)b * (a.n - 1) + z.node) * a.V + i], 0.0);
-  for (int r = 0; r < nref; ++r) w = refused[r] == i ? 0.0 : w;
-  return w;
+// max(p - q, 0) of token i at the last node.
+template <typename LT>
+__device__ __forceinline__ double vf_resid(const VerifyArgs& a, int b, const Last& z, double inv_z, const Row<LT>& r,
+                                           int64_t i, const Pow2& tab) {
+  const double q = a.q[((int64_t)b * (a.n - 1) + z.node) * a.V + i];
+  return fmax(vf_weight(r.at(i), z.M, a.scale2, tab) * inv_z - q, 0.0);
 }
 
-// The first token whose running sum exceeds u times the total, from the chunks' sums (in LDS): 256 threads.
-__device__ int vf_pick(const VerifyArgs& a, int b, const Last& z, const int* refused, int nref, double u,
-                       const double* sums, double* red) {
-  __shared__ int s_chunk;
-  __shared__ double s_before, s_target;
-  __shared__ int s_at, s_last;
-  const int t = threadIdx.x;
-  if (t == 0) {
-    double total = 0.0;
-    for (int c = 0; c < a.nchunk; ++c) total += sums[c];
-    const double target = u * total;
-    double run = 0.0, before = 0.0;
-    int pick = -1;
-    for (int c = 0; c < a.nchunk; ++c) {
-      if (!(sums[c] > 0.0)) continue;
-      if (pick >= 0 && !(run <= target)) break;
-      pick = c;  // (rounding may leave the target past the last weight: then the last chunk)
-      before = run;
-      run += sums[c];
+__device__ __forceinline__ double vf_wave_scan(double v) {  // inclusive
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double w = __shfl_up(v, o, 64);
+    if (lane >= o) v += w;
+  }
+  return v;
+}
+
+struct PickLds {
+  double sums[VF_MAX_CHUNKS + 1];  // the chunks' sums
+  double wave[VF_WALK / 64];
+  double before, target;
+  int chunk, at, last;
+};
+
+// The first token whose running sum exceeds u times the total, from the chunks' sums; weight(i): token i's. -1: no sum
+// is above zero. (A sum that is only rounding, all its chunk's tokens refused, is struck out and the draw made again.)
+template <typename F>
+__device__ int vf_pick(const VerifyArgs& a, PickLds& s, double u, int off, F weight) {
+  constexpr int PER = VF_CHUNK / VF_WALK;
+  const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+  for (;;) {
+    __syncthreads();
+    if (wv == 0) {
+      double total = 0.0;
+      for (int c0 = 0; c0 < a.nchunk; c0 += 64)
+        total += __shfl(vf_wave_scan(c0 + lane < a.nchunk ? s.sums[c0 + lane] : 0.0), 63, 64);
+      const double target = u * total;
+      double run = 0.0, before = 0.0;
+      int pick = -1;
+      for (int c0 = 0; c0 < a.nchunk; c0 += 64) {
+        const double v = c0 + lane < a.nchunk ? s.sums[c0 + lane] : 0.0;
+        const double up = vf_wave_scan(v), prev = __shfl_up(up, 1, 64);
+        const uint64_t some = __ballot(v > 0.0), hit = __ballot(v > 0.0 && run + up > target);
+        if (some) {  // (rounding may leave the target past the last weight: then the last chunk that has one)
+          const int at = hit ? __ffsll((unsigned long long)hit) - 1 : 63 - __clzll((long long)some);
+          const double pr = __shfl(prev, at, 64);
+          pick = c0 + at;
+          before = at ? run + pr : run;
+        }
+        if (hit) break;
+        run += __shfl(up, 63, 64);
+      }
+      if (lane == 0) {
+        s.chunk = pick;
+        s.before = before;
+        s.target = target;
+        s.at = 0x7fffffff;
+        s.last = -1;
+      }
     }
-    s_chunk = pick;
-    s_before = before;
-    s_target = target;
-    s_at = 0x7fffffff;
-    s_last = -1;
+    __syncthreads();
+    const int c = s.chunk;
+    if (c < 0) return -1;
+    const int64_t i0 = (int64_t)c * VF_CHUNK + t * PER - off;
+    double w[PER], mine = 0.0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      w[k] = i0 + k >= 0 && i0 + k < a.V ? weight(i0 + k) : 0.0;
+      mine += w[k];
+    }
+    const double up = vf_wave_scan(mine), prev = __shfl_up(up, 1, 64);
+    if (lane == 63) s.wave[wv] = up;
+    __syncthreads();
+    double base = s.before;
+    for (int k = 0; k < wv; ++k) base += s.wave[k];
+    const double end = base + up;  // the next thread's start, to the bit
+    double run = lane ? base + prev : base;
+    int found = -1, last = -1;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      run += w[k];
+      if (w[k] > 0.0) last = (int)(i0 + k);
+      if (found < 0 && w[k] > 0.0 && run > s.target) found = last;
+    }
+    if (found < 0 && end > s.target) found = last;
+    if (found >= 0) atomicMin(&s.at, found);
+    if (last >= 0) atomicMax(&s.last, last);  // (rounding may leave the target past the chunk's last weight)
+    __syncthreads();
+    const int got = s.at != 0x7fffffff ? s.at : s.last;
+    if (got >= 0) return got;
+    if (t == 0) s.sums[c] = 0.0;
   }
-  __syncthreads();
-  const int c = s_chunk;
-  if (c < 0) return -1;
-  // thread t: VF_PER elements in a row
-  const int64_t i0 = (int64_t)c * VF_CHUNK + t * VF_PER;
-  double w[VF_PER], mine = 0.0;
-  for (int k = 0; k < VF_PER; ++k) {
-    w[k] = i0 + k < a.V ? vf_left(a, b, z, refused, nref, i0 + k) : 0.0;
-    mine += w[k];
-  }
-  red[t] = mine;
-  __syncthreads();
-  double run = s_before;
-  for (int k = 0; k < t; ++k) run += red[k];
-  const double end = run + mine;  // the next thread's start, to the bit
-  int found = -1, last = -1;
-  for (int k = 0; k < VF_PER; ++k) {
-    run += w[k];
-    if (w[k] > 0.0) last = (int)(i0 + k);
-    if (found < 0 && w[k] > 0.0 && run > s_target) found = last;
-  }
-  if (found < 0 && end > s_target) found = last;
-  if (found >= 0) atomicMin(&s_at, found);
-  if (last >= 0) atomicMax(&s_last, last);  // (rounding may leave the target past the chunk's last weight)
-  __syncthreads();
-  return s_at != 0x7fffffff ? s_at : s_last;
 }
 
 // One workgroup per sequence: the rows' statistics, the walk and, unless a q is to be taken off, the draw.
-__global__ __launch_bounds__(VF_THREADS) void verify_walk_kernel(VerifyArgs a) {
+template <typename LT>
+__global__ __launch_bounds__(VF_WALK) void verify_walk_kernel(VerifyArgs a) {
   __shared__ float sM[64];
   __shared__ int sat[64], sref[64];
-  __shared__ double sZ[64];
-  __shared__ double sums[VF_MAX_CHUNKS], red[VF_THREADS];
+  __shared__ double sZ[64], swref[64];
+  __shared__ PickLds pick;
+  __shared__ Pow2 tab;
   __shared__ int s_node, s_nref;
   const int b = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6, n = a.n;
   const int len = a.lengths ? min(a.lengths[b], n) : n;
-  for (int r = wave; r < n; r += 4) {
-    const Part p = vf_row(a, (int64_t)b * n + r, lane);
+  // the nodes' own loads ahead of the rows' sums
+  int par = -1, tok = -1;
+  float u = 0.f, x = -INFINITY, q = 1.f;
+  if (wave == 0 && lane < len) {
+    tok = a.tokens[(int64_t)b * n + lane];
+    par = a.parents ? a.parents[(int64_t)b * a.parents_stride + lane] : lane - 1;
+    if (par >= lane) par = -1;
+    if (par >= 0 && tok >= 0 && tok < a.V && a.scale2 != 0.0) {
+      u = a.u[(int64_t)b * n + lane];
+      x = Row<LT>(a, (int64_t)b * n + par).at(tok);
+      if (a.q) q = a.q[((int64_t)b * (n - 1) + par) * a.V + tok];
+    }
+  }
+  tab.fill();
+  __syncthreads();
+  for (int r = wave; r < n; r += VF_WALK / 64) {
+    const Part p = vf_row(a, (int64_t)b * n + r, lane, tab);
     if (lane == 0) sM[r] = p.m, sat[r] = p.at, sZ[r] = p.s;
   }
   __syncthreads();
   if (len <= 0) {
     if (t < n) a.path[(int64_t)b * n + t] = -1;
-    if (t == 0) a.count[b] = 0, a.token[b] = -1;
-    if (t == 0 && a.state) a.state[b] = -1;
+    if (t == 0) {
+      a.count[b] = 0;
+      a.token[b] = -1;
+      if (a.last) a.last[b].node = -1;
+    }
     return;
   }
   if (wave == 0) {
-    const bool live = lane < len;
-    int par = -1, tok = -1;
-    if (live) {
-      tok = a.tokens[(int64_t)b * n + lane];
-      par = a.parents ? a.parents[(int64_t)b * a.parents_stride + lane] : lane - 1;
-      if (par < 0 || par >= lane) par = -1;
-    }
-    const bool can = live && par >= 0 && tok >= 0 && tok < a.V;
-    double p = 0.0, q = 1.0, u = 0.0;
-    if (can) {
-      if (a.inv_temp == 0.0) {
-        p = sM[par] > -INFINITY && sat[par] == tok ? 1.0 : 0.0;
+    double w = 0.0, p = 0.0;
+    if (par >= 0 && tok >= 0 && tok < a.V && sM[par] > -INFINITY) {
+      if (a.scale2 == 0.0) {
+        p = sat[par] == tok ? 1.0 : 0.0;
       } else {
-        if (sM[par] > -INFINITY) p = vf_weight(vf_logit(a, (int64_t)b * n + par, tok), sM[par], a.inv_temp) / sZ[par];
-        u = a.u[(int64_t)b * n + lane];
-        if (a.q) q = a.q[((int64_t)b * (n - 1) + par) * a.V + tok];
+        w = vf_weight(x, sM[par], a.scale2, tab);
+        p = w / sZ[par];
       }
     }
     int cur = 0, last = 0, got = 1;
     double left = 1.0;
-    uint64_t refused = 0, taken = 1;
+    uint64_t refused = 0, taken = 1, again = 0;
     while (true) {
-      const uint64_t cand = __ballot(live && par == cur && lane > last);
+      const uint64_t cand = __ballot(lane < len && par == cur && lane > last);
       if (!cand) break;
       const int i = __ffsll((unsigned long long)cand) - 1;
       const int ti = __shfl(tok, i, 64);
-      const bool again = __ballot((refused >> lane & 1) && tok == ti) != 0;
-      const double pi = again ? 0.0 : __shfl(p, i, 64), ui = __shfl(u, i, 64);
-      const bool ok = a.q && a.inv_temp != 0.0 ? ui * __shfl(q, i, 64) < pi : ui * left < pi;
+      const bool dup = __ballot((refused >> lane & 1) && tok == ti) != 0;
+      const double pi = dup ? 0.0 : __shfl(p, i, 64), ui = __shfl(u, i, 64);
+      const bool ok = a.q ? ui * (double)__shfl(q, i, 64) < pi : ui * left < pi;
       last = i;
       if (ok) {
         cur = i;
         taken |= 1ull << i;
         ++got;
-        refused = 0;
+        refused = again = 0;
         left = 1.0;
       } else {
         refused |= 1ull << i;
+        again |= (uint64_t)dup << i;
         left -= pi;
       }
     }
     const int slot = __popcll(taken & ((1ull << lane) - 1));
     if (lane < n && (taken >> lane & 1)) a.path[(int64_t)b * n + slot] = lane;
     if (lane < n && lane >= got) a.path[(int64_t)b * n + lane] = -1;
-    if (refused >> lane & 1) sref[__popcll(refused & ((1ull << lane) - 1))] = tok;
+    if (refused >> lane & 1) {
+      const int k = __popcll(refused & ((1ull << lane) - 1));
+      sref[k] = tok;
+      swref[k] = again >> lane & 1 ? 0.0 : w;  // (zero too where the token is no token)
+    }
     if (lane == 0) {
       a.count[b] = got;
       s_node = cur;
       s_nref = __popcll(refused);
-      if (a.state) a.state[b] = refused ? cur : -1;
     }
   }
   __syncthreads();
-  const Last z{s_node, sM[s_node], sZ[s_node], s_nref > 0};
-  if (!(z.M > -INFINITY)) {
-    if (t == 0) a.token[b] = -1;
-    if (t == 0 && a.state) a.state[b] = -1;
+  const int node = s_node, nref = s_nref;
+  const float M = sM[node];
+  if (!(M > -INFINITY) || a.scale2 == 0.0) {
+    if (t == 0) {
+      a.token[b] = M > -INFINITY ? sat[node] : -1;
+      if (a.last) a.last[b].node = -1;
+    }
     return;
   }
-  if (a.inv_temp == 0.0) {
-    if (t == 0) a.token[b] = sat[z.node];
-    return;
-  }
-  if (a.q && z.refused) return;
+  if (a.last && t == 0) a.last[b] = Last{nref ? node : -1, M, sZ[node]};
+  if (a.q && nref) return;
   // the chunks' sums, without the refused tokens
-  const Part* pr = a.part + ((int64_t)b * n + z.node) * a.nchunk;
-  for (int c = t; c < a.nchunk; c += VF_THREADS) {
-    double s = pr[c].m > -INFINITY ? pr[c].s * vf_weight(pr[c].m, z.M, a.inv_temp) : 0.0;
-    for (int r = 0; r < s_nref; ++r) {
-      bool dup = sref[r] < 0 || sref[r] >= a.V || sref[r] / VF_CHUNK != c;
-      for (int k = 0; k < r; ++k) dup = dup || sref[k] == sref[r];
-      if (!dup) s -= vf_weight(vf_logit(a, (int64_t)b * n + z.node, sref[r]), z.M, a.inv_temp);
-    }
-    sums[c] = fmax(s, 0.0);
+  const Row<LT> row(a, (int64_t)b * n + node);
+  const Part* pr = a.part + ((int64_t)b * n + node) * a.nchunk;
+  for (int c = t; c < a.nchunk; c += VF_WALK) {
+    double s = pr[c].m > -INFINITY ? pr[c].s * vf_weight(pr[c].m, M, a.scale2, tab) : 0.0;
+    for (int r = 0; r < nref; ++r)
+      if (swref[r] > 0.0 && (sref[r] + row.off) / VF_CHUNK == c) s -= swref[r];
+    pick.sums[c] = fmax(s, 0.0);
   }
-  __syncthreads();
-  const int tok = vf_pick(a, b, z, sref, s_nref, (double)a.u[(int64_t)b * n], sums, red);
-  if (t == 0) a.token[b] = tok;
+  const int got = vf_pick(a, pick, (double)a.u[(int64_t)b * n], row.off, [&](int64_t i) {
+    double w = vf_weight(row.at(i), M, a.scale2, tab);
+    for (int r = 0; r < nref; ++r) w = sref[r] == i ? 0.0 : w;
+    return w;
+  });
+  if (t == 0) a.token[b] = got;
 }
 
 // q: chunk sums of max(p - q, 0) at the last node, where a child was refused.
+template <typename LT>
 __global__ __launch_bounds__(VF_THREADS) void verify_resid_kernel(VerifyArgs a) {
+  constexpr int PER = VF_CHUNK / VF_THREADS;
   __shared__ double redd[4];
-  __shared__ float sM;
-  __shared__ double sZ;
-  const int b = blockIdx.y, c = blockIdx.x, node = a.state[b];
-  if (node < 0) return;
-  if (threadIdx.x < 64) {
-    const Part p = vf_row(a, (int64_t)b * a.n + node, threadIdx.x);
-    if (threadIdx.x == 0) sM = p.m, sZ = p.s;
-  }
+  __shared__ Pow2 tab;
+  const int b = blockIdx.y, c = blockIdx.x;
+  const Last z = a.last[b];
+  if (z.node < 0) return;
+  tab.fill();
   __syncthreads();
-  const Last z{node, sM, sZ, true};
+  const Row<LT> row(a, (int64_t)b * a.n + z.node);
+  const double inv_z = 1.0 / z.Z;
   double s = 0.0;
-  for (int k = 0; k < VF_PER; ++k) {
-    const int64_t i = (int64_t)c * VF_CHUNK + VF_THREADS * k + threadIdx.x;
-    if (i < a.V) s += vf_left(a, b, z, nullptr, 0, i);
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int64_t i = (int64_t)c * VF_CHUNK + VF_THREADS * k + threadIdx.x - row.off;
+    if (i >= 0 && i < a.V) s += vf_resid(a, b, z, inv_z, row, i, tab);
   }
-  s = vf_block_reduce(s, redd, [](double p, double q) { return p + q; });
+  s = vf_block_reduce<4>(s, redd, [](double p, double q) { return p + q; });
   if (threadIdx.x == 0) a.resid[(int64_t)b * a.nchunk + c] = s;
 }
 
-__global__ __launch_bounds__(VF_THREADS) void verify_draw_kernel(VerifyArgs a) {
-  __shared__ double sums[VF_MAX_CHUNKS], red[VF_THREADS];
-  __shared__ float sM;
-  __shared__ double sZ;
-  const int b = blockIdx.x, node = a.state[b];
-  if (node < 0) return;
-  if (threadIdx.x < 64) {
-    const Part p = vf_row(a, (int64_t)b * a.n + node, threadIdx.x);
-    if (threadIdx.x == 0) sM = p.m, sZ = p.s;
+template <typename LT>
+__global__ __launch_bounds__(VF_WALK) void verify_draw_kernel(VerifyArgs a) {
+  __shared__ PickLds pick;
+  __shared__ Pow2 tab;
+  const int b = blockIdx.x;
+  const Last z = a.last[b];
+  if (z.node < 0) return;
+  tab.fill();
+  const double u = a.u[(int64_t)b * a.n], inv_z = 1.0 / z.Z;
+  const Row<LT> row(a, (int64_t)b * a.n + z.node);
+  for (int c = threadIdx.x; c < a.nchunk; c += VF_WALK) pick.sums[c] = a.resid[(int64_t)b * a.nchunk + c];
+  int got = vf_pick(a, pick, u, row.off, [&](int64_t i) { return vf_resid(a, b, z, inv_z, row, i, tab); });
+  if (got < 0) {  // p nowhere above q (to rounding): drawn from p
+    const Part* pr = a.part + ((int64_t)b * a.n + z.node) * a.nchunk;
+    for (int c = threadIdx.x; c < a.nchunk; c += VF_WALK)
+      pick.sums[c] = pr[c].m > -INFINITY ? pr[c].s * vf_weight(pr[c].m, z.M, a.scale2, tab) : 0.0;
+    got = vf_pick(a, pick, u, row.off, [&](int64_t i) { return vf_weight(row.at(i), z.M, a.scale2, tab); });
   }
-  double any = 0.0;
-  for (int c = threadIdx.x; c < a.nchunk; c += VF_THREADS) any += sums[c] = a.resid[(int64_t)b * a.nchunk + c];
-  any = vf_block_reduce(any, red, [](double p, double q) { return p + q; });
-  __syncthreads();
-  Last z{node, sM, sZ, true};
-  if (!(any > 0.0)) {  // p nowhere above q (to rounding): drawn from p
-    z.refused = false;
-    const Part* pr = a.part + ((int64_t)b * a.n + node) * a.nchunk;
-    for (int c = threadIdx.x; c < a.nchunk; c += VF_THREADS)
-      sums[c] = pr[c].m > -INFINITY ? pr[c].s * vf_weight(pr[c].m, z.M, a.inv_temp) : 0.0;
-    __syncthreads();
-  }
-  const int tok = vf_pick(a, b, z, nullptr, 0, (double)a.u[(int64_t)b * a.n], sums, red);
-  if (threadIdx.x == 0) a.token[b] = tok;
+  if (threadIdx.x == 0) a.token[b] = got;
 }
 
 int64_t up16(int64_t v) { return (v + 15) & ~15ll; }
+int64_t chunks(int64_t vocab) { return nsx_cdiv(vocab + VF_VEC - 1, VF_CHUNK); }
+
+template <typename LT>
+int verify_launch(const VerifyArgs& a, hipStream_t st) {
+  const dim3 rows(a.nchunk, a.B * a.n), seqs(a.nchunk, a.B);
+  if (a.scale2 == 0.0) hipLaunchKernelGGL((verify_stats_kernel<LT, true>), rows, dim3(VF_THREADS), 0, st, a);
+  else hipLaunchKernelGGL((verify_stats_kernel<LT, false>), rows, dim3(VF_THREADS), 0, st, a);
+  NSX_LAUNCHED();
+  hipLaunchKernelGGL(verify_walk_kernel<LT>, dim3(a.B), dim3(VF_WALK), 0, st, a);
+  NSX_LAUNCHED();
+  if (a.q) {
+    hipLaunchKernelGGL(verify_resid_kernel<LT>, seqs, dim3(VF_THREADS), 0, st, a);
+    NSX_LAUNCHED();
+    hipLaunchKernelGGL(verify_draw_kernel<LT>, dim3(a.B), dim3(VF_WALK), 0, st, a);
+    NSX_LAUNCHED();
+  }
+  return NSX_OK;
+}
 
 }  // namespace
 
 extern "C" int64_t nsx_verify_workspace_bytes(int64_t batch, int n_nodes, int64_t vocab) {
   if (batch <= 0 || n_nodes <= 0 || vocab <= 0) return -1;
-  const int64_t nchunk = nsx_cdiv(vocab, VF_CHUNK);
-  return batch * n_nodes * nchunk * (int64_t)sizeof(Part) + up16(batch * nchunk * 8) + up16(batch * 4);
+  return batch * n_nodes * chunks(vocab) * (int64_t)sizeof(Part) + up16(batch * chunks(vocab) * 8) +
+         batch * (int64_t)sizeof(Last);
 }
 
 extern "C" int nsx_verify(const void* logits, int logits_dtype, int64_t row_stride, int64_t batch, int n_nodes,
@@ -363,7 +490,7 @@ extern "C" int nsx_verify(const void* logits, int logits_dtype, int64_t row_stri
               NSX_TREE_MAX_NODES);
   NSX_REQUIRE(batch >= 0 && batch * n_nodes < 65536, NSX_EINVAL, "%lld sequences of %d nodes: fewer than 65536 rows",
               (long long)batch, n_nodes);
-  NSX_REQUIRE(vocab > 0 && vocab <= (int64_t)VF_CHUNK * VF_MAX_CHUNKS, NSX_EINVAL, "vocabulary of %lld (1 to %lld)",
+  NSX_REQUIRE(vocab > 0 && chunks(vocab) <= VF_MAX_CHUNKS + 1 && vocab <= (int64_t)VF_CHUNK * VF_MAX_CHUNKS, NSX_EINVAL, "vocabulary of %lld (1 to %lld)",
               (long long)vocab, (long long)VF_CHUNK * VF_MAX_CHUNKS);
   NSX_REQUIRE(row_stride >= vocab, NSX_EINVAL, "rows %lld elements apart for %lld logits", (long long)row_stride,
               (long long)vocab);
@@ -378,26 +505,18 @@ extern "C" int nsx_verify(const void* logits, int logits_dtype, int64_t row_stri
   const int64_t need = nsx_verify_workspace_bytes(batch, n_nodes, vocab);
   NSX_REQUIRE(workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0, NSX_EINVAL,
               "workspace of %lld bytes, %lld needed, 16-byte aligned", (long long)workspace_bytes, (long long)need);
-  const int nchunk = (int)nsx_cdiv(vocab, VF_CHUNK);
   const bool residual = draft_probs && temperature > 0.0 && n_nodes > 1;
+  const int nchunk = (int)chunks(vocab);
   uint8_t* w = (uint8_t*)workspace;
   Part* part = (Part*)w;
   w += batch * n_nodes * nchunk * (int64_t)sizeof(Part);
   double* resid = (double*)w;
   w += up16(batch * nchunk * 8);
-  VerifyArgs a{logits, logits_dtype, row_stride, (int)batch, n_nodes, vocab, tokens, parents, lengths, parents_stride,
-               uniforms, residual ? draft_probs : nullptr, temperature > 0.0 ? 1.0 / temperature : 0.0, count, path,
-               token, nchunk, part, resid, residual ? (int32_t*)w : nullptr};
+  const VerifyArgs a{logits, row_stride, (int)batch, n_nodes, vocab, tokens, parents, lengths, parents_stride, uniforms,
+                     residual ? draft_probs : nullptr, temperature > 0.0 ? 1.44269504088896340736 / temperature : 0.0,
+                     count, path, token, nchunk, part, resid, residual ? (Last*)w : nullptr};
   hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(verify_stats_kernel, dim3(nchunk, (unsigned)(batch * n_nodes)), dim3(VF_THREADS), 0, st, a);
-  NSX_LAUNCHED();
-  hipLaunchKernelGGL(verify_walk_kernel, dim3((unsigned)batch), dim3(VF_THREADS), 0, st, a);
-  NSX_LAUNCHED();
-  if (residual) {
-    hipLaunchKernelGGL(verify_resid_kernel, dim3(nchunk, (unsigned)batch), dim3(VF_THREADS), 0, st, a);
-    NSX_LAUNCHED();
-    hipLaunchKernelGGL(verify_draw_kernel, dim3((unsigned)batch), dim3(VF_THREADS), 0, st, a);
-    NSX_LAUNCHED();
-  }
-  return NSX_OK;
+  if (logits_dtype == NSX_DT_F32) return verify_launch<float>(a, st);
+  if (logits_dtype == NSX_DT_F16) return verify_launch<_Float16>(a, st);
+  return verify_launch<uint16_t>(a, st);
 }
