@@ -28,11 +28,24 @@ struct TreeArgs {
   const void *kc, *vc, *dk, *dv;
   const int32_t *parents, *pos;
   int64_t ctx_max;
-  int window, n_rep, n_kv, n_head, nodes, max_nodes, nsplit, ncb;
+  int window, n_rep, n_kv, n_head, nodes, max_nodes;
+  int nsplit, ncb;   // splits of the keys, blocks of columns
+  int keys, round;   // keys of a tile; a split is a multiple of so many tiles
   float scale2;  // scale * log2(e): the softmax is taken in powers of two
   float* part;
   const float* sinks;
   float* out;
+};
+
+// Which tiles a split takes: the cache's rows from the first that any node sees, then the nodes' own rows.
+struct Tiles {
+  int lo, cache, all, per;  // first row; tiles of the cache's rows; with the nodes'; of a split
+  __device__ __forceinline__ Tiles(const TreeArgs& a, int P, int keys, int round) {
+    lo = a.window > 0 ? max(0, P + 1 - a.window) : 0;
+    cache = (P - lo + keys - 1) / keys;
+    all = cache + (a.nodes + keys - 1) / keys;
+    per = ((all + a.nsplit - 1) / a.nsplit + round - 1) / round * round;
+  }
 };
 
 // Lane i's node: its ancestors and itself as bits, from the parent list, each round doubling the path's length.
@@ -244,10 +257,8 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
   const int g = blockIdx.x % a.n_kv, cb = blockIdx.x / a.n_kv, c = blockIdx.y;
   const int P = *a.pos;
   if (P < 0 || P > a.ctx_max) return;
-  const int lo = a.window > 0 ? max(0, P + 1 - a.window) : 0;
-  const int pt = (P - lo + TREE_KEYS - 1) / TREE_KEYS, nt = pt + (a.nodes + TREE_KEYS - 1) / TREE_KEYS;
-  const int per = ((nt + a.nsplit - 1) / a.nsplit + TREE_NW - 1) / TREE_NW * TREE_NW;
-  const int t0 = c * per, t1 = min(nt, t0 + per);
+  const Tiles tl(a, P, TREE_KEYS, TREE_NW);
+  const int lo = tl.lo, pt = tl.cache, t0 = c * tl.per, t1 = min(tl.all, t0 + tl.per);
   if (t0 >= t1) return;
   const int ncol = a.nodes * a.n_rep, col0 = cb * COLS;
 
@@ -300,7 +311,7 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
     for (int k = 0; k < 3; ++k) *(v4u*)&lds[(k * COLS + cc) * QROW + (4 * j + gg) * 16] = tm[k];
   }
   lds_barrier();
-  int q0 = i16 * QROW + kq * 16;
+  const int q0 = i16 * QROW + kq * 16;
   auto query = [&](int k, int ct, int j) { return *(const v4u*)&lds[q0 + (k * COLS + 16 * ct) * QROW + 64 * j]; };
   // a column's node: what it sees of the nodes, its first visible row of the cache
   auto node_of = [&](int ct) { return min(col0 + 16 * ct + i16, ncol - 1) / a.n_rep; };
@@ -380,7 +391,6 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
   start();
   for (int tile = first; tile < t1; tile += TREE_NW) {
     const int next = min(tile + TREE_NW, last);
-    if constexpr (NC > 2) asm volatile("" : "+v"(q0));  // 96 registers of query terms are read anew for each tile
     v4f s[NC][2] = {};
     {
       v4u kt_[2][2][KTN];
@@ -531,21 +541,442 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
   }
 }
 
-// One workgroup per (node, query head): merge the live splits with the sink. Every wave forms all the splits' weights
-// (lane = split), then wave w sums the values of splits w, w + 4, ... (lane = dimension) and the four sums meet in LDS.
-__global__ __launch_bounds__(256) void tree_combine_kernel(TreeArgs a) {
-  constexpr int LPS = TREE_MAX_SPLIT / 64;  // splits per lane
-  __shared__ float ws[TREE_MAX_SPLIT];
-  __shared__ float red[4][ATTN_D];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t row = blockIdx.x;
+// Two bf16 terms of a pair of weights, each rounded to nearest: 2^-17 of a weight, the rounding of an fp32 score of 64.
+__device__ __forceinline__ void split_weights(float a, float b, uint32_t& hi, uint32_t& lo) {
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  hi = __builtin_bit_cast(uint32_t, b2{(__bf16)a, (__bf16)b});
+  lo = __builtin_bit_cast(uint32_t, b2{(__bf16)(a - __builtin_bit_cast(float, hi << 16)),
+                                       (__bf16)(b - __builtin_bit_cast(float, hi & 0xffff0000u))});
+}
+
+// The same attention for many columns: a workgroup of 8 waves takes 128 columns and a split of the keys. Four waves (32
+// columns each) make a group, the two groups share the split's tiles of KEYS keys, and a tile's rows become terms once
+// for the group: each wave loads a part of them, splits it and leaves it in LDS as the operands that every wave of the
+// group then reads.
+//
+// A tile takes two phases: products (the scores of tile i, the values of tile i - 1) and the rest (the weights of
+// tile i, the terms of keys i + 1 and values i). Waves w and w + 4 share a SIMD, and their groups are one phase apart, kept
+// so by the barrier between phases: the matrix cores have one group's products while the VALU has the other's weights.
+template <typename KT>
+__global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
+  using R = Rows<KT>;
+  constexpr int KTN = R::NT, NC = 2, CW = 4, NG = 2, COLS = 16 * NC * CW;
+  constexpr int TPP = KTN == 1 ? 2 : 1, KEYS = 32 * TPP;  // 16-bit rows: two tiles a phase, as their phases are short
+  constexpr int KF = TPP * 4 * KTN, VF = TPP * 4 * KTN;   // operands (64 lanes x 16 bytes) of a tile's keys and values
+  constexpr int GROUP = (KF + VF) * 1024, OROW = ATTN_D + 4;
+  constexpr int PBYTES = 32 * 16 * NC * 4;  // a wave's weights of 32 keys (the second way)
+  constexpr int LDS = std::max(std::max(NG * GROUP, 8 * PBYTES), CW * 16 * NC * OROW * 4);
+  __shared__ __align__(16) uint8_t lds[LDS];
+  __shared__ float sm[CW][16 * NC], sl[CW][16 * NC];
+  __shared__ uint64_t svis[64];
+  __shared__ int sdep[64];
+  const int t = threadIdx.x, lane = t & 63, i16 = lane & 15, kq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int group = wave / CW, cw = wave % CW;  // waves w and w + 4 lie on one SIMD
+  const int g = blockIdx.x % a.n_kv, cb = blockIdx.x / a.n_kv, c = blockIdx.y;
   const int P = *a.pos;
   if (P < 0 || P > a.ctx_max) return;
-  const int lo = a.window > 0 ? max(0, P + 1 - a.window) : 0;
-  const int nt = (P - lo + TREE_KEYS - 1) / TREE_KEYS + (a.nodes + TREE_KEYS - 1) / TREE_KEYS;
-  const int per = ((nt + a.nsplit - 1) / a.nsplit + TREE_NW - 1) / TREE_NW * TREE_NW;
-  const int nc = (nt + per - 1) / per;  // 1 <= nc <= nsplit
-  const float* ml = a.part + ((int64_t)a.nodes * a.n_head * ATTN_D + row * 2) * a.nsplit;
+  const Tiles tl(a, P, KEYS, 1);
+  const int lo = tl.lo, pt = tl.cache, t0 = c * tl.per, t1 = min(tl.all, t0 + tl.per);
+  if (t0 >= t1) return;
+  const int ncol = a.nodes * a.n_rep, col0 = cb * COLS + 16 * NC * cw;
+  const int phases = (t1 - t0 + 1) / 2;               // tiles of the first group, the most
+  const int mine = (t1 - t0 + 1 - group) / 2;  // of this one: t0 + group, + 2, ..
+
+  uint8_t* kl = lds + group * GROUP;
+  uint8_t* vl = kl + KF * 1024;
+  auto rsrc = [&](int i, bool values) {  // rows past the last, and tiles past the group's, read as zero
+    const int tile = t0 + group + 2 * i;
+    const bool own = tile >= pt;
+    const int r0 = own ? (tile - pt) * KEYS : lo + tile * KEYS;
+    const int rows = i < mine ? min((own ? a.nodes : P) - r0, KEYS) : 0;
+    const char* base = (const char*)(own ? (values ? a.dv : a.dk) : (values ? a.vc : a.kc));
+    return nsx_rsrc(base + ((int64_t)g * (own ? a.max_nodes : a.ctx_max) + (i < mine ? r0 : 0)) * R::BYTES,
+                    (uint32_t)rows * R::BYTES);
+  };
+  // This wave's part of a tile: items cw, cw + CW, .. of 4 a subtile. Of the keys an item is 16 rows x 32 dimensions; of the
+  // values 16 rows x 32 dimensions too, a lane holding rows 4 kq .. + 3 of dimensions 2 i16, 2 i16 + 1.
+  constexpr int ITEMS = TPP * 4 / CW;
+  using V2 = std::conditional_t<std::is_same_v<KT, float>, v2u, uint32_t>;
+  typename R::K8 kr[ITEMS];
+  V2 vr[ITEMS][4];
+  auto load_k = [&](int i) {
+    const auto r = rsrc(i, false);
+#pragma unroll
+    for (int it = 0; it < ITEMS; ++it) {
+      const int n = cw + CW * it;  // [subtile][kt][j]
+      kr[it] = R::k8(r, 16 * (n >> 1) + i16, n & 1, kq);
+    }
+  };
+  auto load_v = [&](int i) {
+    const auto r = rsrc(i, true);
+#pragma unroll
+    for (int it = 0; it < ITEMS; ++it) {
+      const int n = cw + CW * it;  // [subtile][kt][half of the dimensions]
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int o = (16 * (n >> 1) + 4 * kq + k) * R::BYTES + (n & 1) * (R::BYTES / 2) + i16 * (R::BYTES / 32);
+        if constexpr (std::is_same_v<KT, float>) vr[it][k] = __builtin_bit_cast(v2u, __builtin_amdgcn_raw_buffer_load_b64(r, o, 0, 0));
+        else vr[it][k] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, o, 0, 0);
+      }
+    }
+  };
+  auto store_k = [&] {
+#pragma unroll
+    for (int it = 0; it < ITEMS; ++it) {
+      v4u x[KTN];
+      key_terms<KT>(kr[it], x);
+#pragma unroll
+      for (int k = 0; k < KTN; ++k) *(v4u*)(kl + ((cw + CW * it) * KTN + k) * 1024 + lane * 16) = x[k];
+    }
+  };
+  auto store_v = [&] {  // operand [subtile][half][dimension's parity]: the kt'th 8 bytes of a lane
+#pragma unroll
+    for (int it = 0; it < ITEMS; ++it) {
+      const int n = cw + CW * it, sub = n >> 2, kt = (n >> 1) & 1, half = n & 1;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        v2u x[KTN];
+        if constexpr (KTN == 1) {
+          const uint32_t sel = b ? 0x07060302u : 0x05040100u;
+          x[0] = v2u{__builtin_amdgcn_perm(vr[it][1], vr[it][0], sel), __builtin_amdgcn_perm(vr[it][3], vr[it][2], sel)};
+        } else {
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            float f[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              if constexpr (std::is_same_v<KT, float>) f[q] = __builtin_bit_cast(float, (uint32_t)vr[it][2 * p + q][b]);
+              else f[q] = nsx_h2f(b ? vr[it][2 * p + q] >> 16 : vr[it][2 * p + q] & 0xffffu);
+            }
+#pragma unroll
+            for (int k = 0; k < KTN; ++k) {
+              x[k][p] = top2(f[0], f[1]);
+              if (k + 1 < KTN) f[0] = below(f[0]), f[1] = below(f[1]);
+            }
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < KTN; ++k)
+          *(v2u*)(vl + (((sub * 2 + half) * 2 + b) * KTN + k) * 1024 + lane * 16 + kt * 8) = x[k];
+      }
+    }
+  };
+  load_k(0);
+  load_v(0);
+
+  if (wave == 0) {
+    uint64_t line = tree_lineage(a.parents, a.nodes, lane);
+    const int dep = __popcll(line) - 1;
+    if (a.window > 0 && a.window < a.nodes) {  // ancestors out of the window
+      for (int j = 0; j < a.nodes; ++j)
+        if (dep - __shfl(dep, j, 64) >= a.window) line &= ~(1ull << j);
+    }
+    svis[lane] = line;
+    sdep[lane] = dep;
+  }
+  v4u q[NC][2][3];
+#pragma unroll
+  for (int ct = 0; ct < NC; ++ct) {
+    const int col = min(col0 + 16 * ct + i16, ncol - 1), node = col / a.n_rep, h = g * a.n_rep + col % a.n_rep;
+    const float* qp = a.q + ((int64_t)node * a.n_head + h) * ATTN_D;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const v4f x0 = *(const v4f*)(qp + R::dim(j, kq, 0)), x1 = *(const v4f*)(qp + R::dim(j, kq, 4));
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = (e < 4 ? x0[e & 3] : x1[e & 3]) * a.scale2;
+      split8(x, q[ct][j]);
+    }
+  }
+  lds_barrier();
+  uint64_t vis[NC];
+  int from[NC], deepest = 0;  // the columns' first visible cache rows, and the last of them
+#pragma unroll
+  for (int ct = 0; ct < NC; ++ct) {
+    const int node = min(col0 + 16 * ct + i16, ncol - 1) / a.n_rep;
+    vis[ct] = svis[node];
+    from[ct] = a.window > 0 ? P + sdep[node] + 1 - a.window : 0;
+    deepest = max(deepest, from[ct]);
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) deepest = max(deepest, __shfl_xor(deepest, o, 64));
+  deepest = __builtin_amdgcn_readfirstlane(deepest);
+
+  float m[NC], l[NC];
+  v4f acc[NC][4];  // [dimension's half, parity]
+  v4f s[NC][2 * TPP];
+  v4u pw[NC][TPP][2];
+  auto start = [&] {
+#pragma unroll
+    for (int ct = 0; ct < NC; ++ct) {
+      m[ct] = ATTN_LOWEST;
+      l[ct] = 0.f;
+#pragma unroll
+      for (int f = 0; f < 4; ++f) acc[ct][f] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+  };
+  // scores in powers of two -> weights, 16 keys each of N; r0: the first key's row (own: of the nodes)
+  auto weights = [&](auto& x, auto n_tag, bool own, int r0) {
+    constexpr int N = decltype(n_tag)::value;
+    if (own || r0 + 16 * N > P || r0 < deepest) {
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct) {
+        const int lo_k = own ? 0 : from[ct] - r0, hi_k = (own ? a.nodes : P) - r0;
+        const uint64_t bits = own ? vis[ct] >> r0 : ~0ull;
+#pragma unroll
+        for (int e = 0; e < 4 * N; ++e) {
+          const int k = 16 * (e >> 2) + 4 * kq + (e & 3);
+          const bool on = k >= lo_k && k < hi_k && (bits >> k & 1);
+          x[ct][e >> 2][e & 3] = on ? x[ct][e >> 2][e & 3] : -INFINITY;
+        }
+      }
+    }
+    float mx[NC];
+    bool move = false;
+#pragma unroll
+    for (int ct = 0; ct < NC; ++ct) {
+      mx[ct] = fmaxf(x[ct][0][0], x[ct][0][1]);
+#pragma unroll
+      for (int e = 2; e < 4 * N; ++e) mx[ct] = fmaxf(mx[ct], x[ct][e >> 2][e & 3]);
+      move = move || mx[ct] > m[ct] + 8.f;
+    }
+    if (__any(move)) {
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct) {
+        float mn = fmaxf(mx[ct], __shfl_xor(mx[ct], 16, 64));
+        mn = fmaxf(m[ct], fmaxf(mn, __shfl_xor(mn, 32, 64)));
+        const float corr = __builtin_amdgcn_exp2f(m[ct] - mn);  // (first tile: of nothing)
+        m[ct] = mn;
+        l[ct] *= corr;
+#pragma unroll
+        for (int f = 0; f < 4; ++f) acc[ct][f] *= corr;
+      }
+    }
+#pragma unroll
+    for (int ct = 0; ct < NC; ++ct) {
+#pragma unroll
+      for (int e = 0; e < 4 * N; ++e) {
+        const float w = __builtin_amdgcn_exp2f(x[ct][e >> 2][e & 3] - m[ct]);
+        x[ct][e >> 2][e & 3] = w;
+        l[ct] += w;  // this lane group's keys; the groups are added at the end
+      }
+    }
+  };
+  auto phase = [] {
+    __builtin_amdgcn_sched_barrier(0);
+    lds_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  start();
+  store_k();
+  load_k(1);
+  if (group) phase();
+  phase();
+#pragma unroll 1
+  for (int i = 0; i <= phases; ++i) {
+    __builtin_amdgcn_s_setprio(1);
+    if (i > 0 && i <= mine) {
+#pragma unroll
+      for (int u = 0; u < TPP; ++u)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          v4u x[KTN];
+#pragma unroll
+          for (int k = 0; k < KTN; ++k) x[k] = *(const v4u*)(vl + ((u * 4 + f) * KTN + k) * 1024 + lane * 16);
+#pragma unroll
+          for (int o = 2; o >= 0; --o)  // (the small products first)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              if (o - k >= 0 && o - k < KTN) {
+#pragma unroll
+                for (int ct = 0; ct < NC; ++ct)
+                  acc[ct][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(x[o - k]), as_b8(pw[ct][u][k]), acc[ct][f], 0, 0, 0);
+              }
+        }
+    }
+    if (i < mine) {
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+        for (int n = 0; n < 2 * TPP; ++n) s[ct][n] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int n = 0; n < 2 * TPP; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          v4u x[KTN];
+#pragma unroll
+          for (int k = 0; k < KTN; ++k) x[k] = *(const v4u*)(kl + ((n * 2 + j) * KTN + k) * 1024 + lane * 16);
+#pragma unroll
+          for (int o = 2; o >= 0; --o)
+#pragma unroll
+            for (int k = 0; k <= o; ++k)
+              if (o - k < KTN) {
+#pragma unroll
+                for (int ct = 0; ct < NC; ++ct)
+                  s[ct][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(x[o - k]), as_b8(q[ct][j][k]), s[ct][n], 0, 0, 0);
+              }
+        }
+    }
+    __builtin_amdgcn_s_setprio(0);
+    phase();
+    if (i < mine) {
+      const int tile = t0 + group + 2 * i;
+      const bool own = tile >= pt;
+      store_v();
+      store_k();
+      load_v(i + 1);
+      load_k(i + 2);
+      weights(s, std::integral_constant<int, 2 * TPP>{}, own, own ? (tile - pt) * KEYS : lo + tile * KEYS);
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+        for (int u = 0; u < TPP; ++u)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const v4f& y = s[ct][2 * u + (w >> 1)];
+            uint32_t hi, low;
+            split_weights(y[2 * (w & 1)], y[2 * (w & 1) + 1], hi, low);
+            pw[ct][u][0][w] = hi;
+            pw[ct][u][1][w] = low;
+          }
+    }
+    phase();
+  }
+  if (!group) phase();
+
+  bool ok = true;
+#pragma unroll
+  for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+    for (int f = 0; f < 4; ++f)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) ok = ok && finite(acc[ct][f][r]);
+  if (!__all(ok)) {  // the second way, by this wave alone
+    float* sp = (float*)&lds[wave * PBYTES];
+    start();
+#pragma unroll 1
+    for (int i = 0; i < mine * TPP; ++i) {
+      const int tile = t0 + group + 2 * (i / TPP);
+      const bool own = tile >= pt;
+      const auto rk = rsrc(i / TPP, false), rv = rsrc(i / TPP, true);
+      const int sub = 32 * (i % TPP), r0 = (own ? (tile - pt) * KEYS : lo + tile * KEYS) + sub;
+      v4f x[NC][2] = {};
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const auto kk = R::k8(rk, sub + 16 * kt + i16, j, kq);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int ct = 0; ct < NC; ++ct) {
+              auto term = [&](int k) {
+                const uint32_t w = q[ct][j][k][e >> 1];
+                return __builtin_bit_cast(float, e & 1 ? w & 0xffff0000u : w << 16);
+              };
+              x[ct][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(R::k(kk, e), term(0) + (term(1) + term(2)), x[ct][kt], 0, 0, 0);
+            }
+        }
+      weights(x, std::integral_constant<int, 2>{}, own, r0);
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sp[(16 * (e >> 2) + 4 * kq + (e & 3)) * (16 * NC) + 16 * ct + i16] = x[ct][e >> 2][e & 3];
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll 1
+      for (int k = 0; k < 32; ++k) {
+        typename R::V4 v[2][2];  // dimensions 32 h + 8 kq ..
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) v[h][u] = R::v4(rv, sub + k, 8 * h + 2 * kq + u);
+#pragma unroll
+        for (int ct = 0; ct < NC; ++ct) {
+          const float w = sp[k * (16 * NC) + 16 * ct + i16];
+          if (w != 0.f) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int d = 0; d < 8; ++d)
+                acc[ct][2 * h + (d & 1)][d >> 1] = fmaf(w, R::v(v[h][d >> 2], d & 3), acc[ct][2 * h + (d & 1)][d >> 1]);
+          }
+        }
+      }
+    }
+  }
+
+  // the second group's sums join the first's
+#pragma unroll
+  for (int ct = 0; ct < NC; ++ct) {
+    l[ct] += __shfl_xor(l[ct], 16, 64);
+    l[ct] += __shfl_xor(l[ct], 32, 64);
+  }
+  float(*so)[16 * NC][OROW] = (float(*)[16 * NC][OROW])lds;
+  lds_barrier();
+  if (group) {
+#pragma unroll
+    for (int ct = 0; ct < NC; ++ct) {
+      if (kq == 0) sm[cw][16 * ct + i16] = m[ct], sl[cw][16 * ct + i16] = l[ct];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          *(v4f*)&so[cw][16 * ct + i16][32 * h + 8 * kq + 4 * u] =
+              v4f{acc[ct][2 * h][2 * u], acc[ct][2 * h + 1][2 * u], acc[ct][2 * h][2 * u + 1], acc[ct][2 * h + 1][2 * u + 1]};
+    }
+  }
+  lds_barrier();
+  if (group) return;
+  const bool whole = a.nsplit == 1;
+#pragma unroll
+  for (int ct = 0; ct < NC; ++ct) {
+    const int cc = 16 * ct + i16, col = col0 + cc;
+    if (col >= ncol) continue;
+    const int h = g * a.n_rep + col % a.n_rep;
+    const int64_t row = (int64_t)(col / a.n_rep) * a.n_head + h;
+    const float sink = whole && a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
+    const float M = fmaxf(sink, fmaxf(m[ct], sm[cw][cc]));
+    const float e0 = __builtin_amdgcn_exp2f(m[ct] - M), e1 = __builtin_amdgcn_exp2f(sm[cw][cc] - M);  // (no tile: 0)
+    const float Z = (whole && a.sinks ? __builtin_amdgcn_exp2f(sink - M) : 0.f) + fmaf(e0, l[ct], e1 * sl[cw][cc]);
+    float* to = whole ? a.out + row * ATTN_D : a.part + (row * a.nsplit + c) * ATTN_D;
+    const float div = whole ? Z : 1.f;
+#pragma unroll
+    for (int d = 0; d < 16; d += 4) {
+      const int at = 32 * (d >> 3) + 8 * kq + (d & 7);
+      const v4f x = *(const v4f*)&so[cw][cc][at];
+      v4f v;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int dd = d + k;
+        v[k] = fmaf(e1, x[k], e0 * acc[ct][2 * (dd >> 3) + (dd & 1)][(dd & 7) >> 1]) / div;
+      }
+      *(v4f*)(to + at) = v;
+    }
+    if (!whole && kq == 0) {
+      float* ml = a.part + ((int64_t)a.nodes * a.n_head * ATTN_D + row * 2) * a.nsplit + 2 * c;
+      ml[0] = M;
+      ml[1] = Z;
+    }
+  }
+}
+
+// WPR waves per (node, query head): merge the live splits with the sink. Every wave forms all the splits' weights (lane =
+// split); then 16 lanes take a split's 64 values, so a wave adds four splits a load, WPR waves 4 WPR, and the lanes' and
+// waves' sums meet. Bound by its two rounds of loads and the launch.
+template <int WPR>
+__global__ __launch_bounds__(256) void tree_combine_kernel(TreeArgs a) {
+  constexpr int LPS = TREE_MAX_SPLIT / 64;  // splits per lane
+  __shared__ float ws[4][TREE_MAX_SPLIT];
+  __shared__ v4f red[4][16];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, part = wave % WPR, i16 = lane & 15, kq = lane >> 4;
+  const int64_t rows = (int64_t)a.nodes * a.n_head, row = min((int64_t)blockIdx.x * (4 / WPR) + wave / WPR, rows - 1);
+  const int P = *a.pos;
+  if (P < 0 || P > a.ctx_max) return;
+  const Tiles tl(a, P, a.keys, a.round);
+  const int nc = (tl.all + tl.per - 1) / tl.per;  // 1 <= nc <= nsplit
+  const float* ml = a.part + (rows * ATTN_D + row * 2) * a.nsplit;
   const float sink = a.sinks ? a.sinks[row % a.n_head] * LOG2E : -INFINITY;
   float mv[LPS], lv[LPS], M = sink;
 #pragma unroll
@@ -560,19 +991,37 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(TreeArgs a) {
   float z = 0.f;
 #pragma unroll
   for (int i = 0; i < LPS; ++i) {
-    const bool on = lane + 64 * i < nc;
-    const float e = on ? __builtin_amdgcn_exp2f(mv[i] - M) : 0.f;
-    if (wave == 0) ws[lane + 64 * i] = e;
-    z = on ? fmaf(e, lv[i], z) : z;
+    const float e = lane + 64 * i < nc ? __builtin_amdgcn_exp2f(mv[i] - M) : 0.f;
+    ws[wave][lane + 64 * i] = e;  // (splits past the last: weight 0)
+    z = fmaf(e, lv[i], z);
   }
   const float Z = nsx_wave_sum(z) + (a.sinks ? __builtin_amdgcn_exp2f(sink - M) : 0.f);
-  __syncthreads();
-  const float* pv = a.part + row * a.nsplit * ATTN_D + lane;
-  float v = 0.f;
-  for (int c0 = wave; c0 < nc; c0 += 4) v = fmaf(ws[c0], pv[(int64_t)c0 * ATTN_D], v);
-  red[wave][lane] = v;
-  __syncthreads();
-  if (wave == 0) a.out[row * ATTN_D + lane] = ((red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane])) / Z;
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own weights
+  const float* pv = a.part + row * a.nsplit * ATTN_D + 4 * i16;
+  v4f v = {0.f, 0.f, 0.f, 0.f};
+  for (int c0 = 4 * part + kq; c0 < nc; c0 += 16 * WPR) {
+    v4f x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[u] = *(const v4f*)(pv + (int64_t)min(c0 + 4 * WPR * u, nc - 1) * ATTN_D);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int s = c0 + 4 * WPR * u;
+      const float e = s < nc ? ws[wave][s] : 0.f;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) v[d] = fmaf(e, x[u][d], v[d]);
+    }
+  }
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    v[d] += __shfl_xor(v[d], 16, 64);
+    v[d] += __shfl_xor(v[d], 32, 64);
+  }
+  if constexpr (WPR > 1) {
+    if (kq == 0) red[wave][i16] = v;
+    __syncthreads();
+    v = (red[0][i16] + red[1][i16]) + (red[2][i16] + red[3][i16]);
+  }
+  if (part == 0 && kq == 0) *(v4f*)(a.out + row * ATTN_D + 4 * i16) = v / Z;
 }
 
 // Accepted nodes' rows into the caches: path[j] to row pos + j for j < count. One 16-byte piece of one row per thread
@@ -604,22 +1053,43 @@ __global__ void tree_advance_kernel(int32_t* pos, const int32_t* count, int node
 
 // ---------------------------------------------------------------------------
 
-// Column tiles of 16 per workgroup.
-int tree_nc(int64_t cols) { return cols <= 16 ? 1 : cols <= 32 ? 2 : 4; }
+enum { TREE_16, TREE_32, TREE_WIDE };  // kernel by the columns of its workgroups: 16, 32, 128
 
-// Splits per kv head and column block for a cache of ctx_max rows.
-int tree_splits(int n_kv, int n_rep, int nodes, int64_t ctx_max, int window) {
-  const int64_t cols = (int64_t)nodes * n_rep, ncb = nsx_cdiv(cols, 16 * tree_nc(cols));
-  const int64_t keys = window > 0 ? std::min<int64_t>(ctx_max, window) : ctx_max;
-  const int64_t tiles = nsx_cdiv(keys, TREE_KEYS) + nsx_cdiv(nodes, TREE_KEYS);
-  if (tiles <= 2 * TREE_NW) return 1;
-  return (int)std::min<int64_t>({nsx_cdiv(tiles, TREE_NW), nsx_cdiv(TREE_GRID, n_kv * ncb), TREE_MAX_SPLIT});
+// Which kernel a call runs, and its grid.
+struct TreePlan {
+  int kind, ncb, nsplit, keys, round;
+};
+
+// `work` counts pieces of 32 keys x 16 columns. Below 8192, eight for each SIMD of the chip, the kernel of 16 columns has
+// the most workgroups and the shortest way through one (us for 16 / 32 / 128 columns at 64 / 8 heads, fp32: 16 nodes,
+// 1000 keys 14.9 / 17.7 / 18.3; 8 nodes, 8000 keys 23.6 / 23.4 / 25.7; 48 nodes, 1500 keys 31.1 / 26.9 / 25.7). Past it,
+// more than 64 columns go to the wide kernel once its sharing of terms outweighs its longer way: three terms a
+// element from 11000 pieces on (16 nodes, 6000 keys 27.0 / 24.6 / 25.1; 32 nodes, 8000 keys 50.7 / 38.7 / 34.5), one
+// term from 32768 (bf16, 32 nodes, 4000 keys 23.5 / 21.6 / 23.8; 16 nodes, 16384 keys 34.5 / 27.1 / 26.6).
+TreePlan tree_plan(int n_kv, int n_rep, int nodes, int64_t ctx_max, int window, int kv_dtype) {
+  const int64_t cols = (int64_t)nodes * n_rep, rows = window > 0 ? std::min<int64_t>(ctx_max, window) : ctx_max;
+  const int64_t work = n_kv * nsx_cdiv(cols, 16) * nsx_cdiv(rows, 32);
+  const int terms = kv_dtype == NSX_DT_F32 ? 3 : kv_dtype == NSX_DT_F16 ? 2 : 1;
+  TreePlan p;
+  p.kind = work < 8192 ? TREE_16 : cols > 64 && work * terms >= 32768 ? TREE_WIDE : TREE_32;
+  const bool wide = p.kind == TREE_WIDE;
+  p.keys = wide && terms == 1 ? 2 * TREE_KEYS : TREE_KEYS;
+  p.round = wide ? 1 : TREE_NW;
+  p.ncb = (int)nsx_cdiv(cols, p.kind == TREE_16 ? 16 : p.kind == TREE_32 ? 32 : 128);
+  const int64_t tiles = nsx_cdiv(rows, p.keys) + nsx_cdiv(nodes, p.keys);
+  const int64_t step = wide ? 2 : TREE_NW;  // tiles that a workgroup takes at a time
+  // workgroups that the chip holds at once: two of four waves a CU, or one of eight
+  const int64_t fill = wide ? TREE_GRID / 2 : TREE_GRID;
+  p.nsplit = tiles <= 2 * step ? 1
+      : (int)std::min<int64_t>({nsx_cdiv(tiles, step), nsx_cdiv(fill, n_kv * (int64_t)p.ncb), TREE_MAX_SPLIT});
+  return p;
 }
 
-int64_t tree_bytes(int n_head, int n_kv, int nodes, int64_t ctx_max, int window) {
+int64_t tree_bytes(int n_head, int n_kv, int nodes, int64_t ctx_max, int window, int kv_dtype) {
   const int64_t rows = (int64_t)nodes * n_head;
   // the rotated queries, then a split's values and (maximum, sum) per row
-  return rows * ATTN_D * 4 + rows * tree_splits(n_kv, n_head / n_kv, nodes, ctx_max, window) * (ATTN_D + 2) * 4;
+  return rows * ATTN_D * 4 +
+         rows * tree_plan(n_kv, n_head / n_kv, nodes, ctx_max, window, kv_dtype).nsplit * (ATTN_D + 2) * 4;
 }
 
 int tree_shapes(int n_head, int n_kv, int head_dim, int nodes, int max_nodes, int64_t ctx_max, int window) {
@@ -636,25 +1106,31 @@ int tree_shapes(int n_head, int n_kv, int head_dim, int nodes, int max_nodes, in
 }
 
 template <typename KT>
-int tree_attn_typed(TreeArgs& a, hipStream_t st) {
-  const int nc = tree_nc((int64_t)a.nodes * a.n_rep);
-  a.ncb = (int)nsx_cdiv((int64_t)a.nodes * a.n_rep, 16 * nc);
-  const dim3 grid(a.n_kv * a.ncb, a.nsplit), block(64 * TREE_NW);
-  if (nc == 1) hipLaunchKernelGGL((tree_attn_kernel<KT, 1>), grid, block, 0, st, a);
-  else if (nc == 2) hipLaunchKernelGGL((tree_attn_kernel<KT, 2>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((tree_attn_kernel<KT, 4>), grid, block, 0, st, a);
+int tree_attn_typed(TreeArgs& a, const TreePlan& p, hipStream_t st) {
+  a.nsplit = p.nsplit;
+  a.ncb = p.ncb;
+  a.keys = p.keys;
+  a.round = p.round;
+  const dim3 grid(a.n_kv * a.ncb, a.nsplit);
+  if (p.kind == TREE_16) hipLaunchKernelGGL((tree_attn_kernel<KT, 1>), grid, dim3(64 * TREE_NW), 0, st, a);
+  else if (p.kind == TREE_32) hipLaunchKernelGGL((tree_attn_kernel<KT, 2>), grid, dim3(64 * TREE_NW), 0, st, a);
+  else hipLaunchKernelGGL((tree_wide_kernel<KT>), grid, dim3(512), 0, st, a);
   NSX_LAUNCHED();
   if (a.nsplit > 1) {
-    hipLaunchKernelGGL(tree_combine_kernel, dim3(a.nodes * a.n_head), dim3(256), 0, st, a);
+    // a wave per row, or four where the rows are few and their splits many
+    const int rows = a.nodes * a.n_head;
+    if (a.nsplit > 32) hipLaunchKernelGGL(tree_combine_kernel<4>, dim3(rows), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(tree_combine_kernel<1>, dim3((rows + 3) / 4), dim3(256), 0, st, a);
     NSX_LAUNCHED();
   }
   return NSX_OK;
 }
 
 int tree_attn_launch(TreeArgs& a, int kv_dtype, hipStream_t st) {
-  if (kv_dtype == NSX_DT_F32) return tree_attn_typed<float>(a, st);
-  if (kv_dtype == NSX_DT_F16) return tree_attn_typed<_Float16>(a, st);
-  return tree_attn_typed<Bf16>(a, st);
+  const TreePlan p = tree_plan(a.n_kv, a.n_rep, a.nodes, a.ctx_max, a.window, kv_dtype);
+  if (kv_dtype == NSX_DT_F32) return tree_attn_typed<float>(a, p, st);
+  if (kv_dtype == NSX_DT_F16) return tree_attn_typed<_Float16>(a, p, st);
+  return tree_attn_typed<Bf16>(a, p, st);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -665,7 +1141,9 @@ int64_t kv_elem(int dt) { return dt == NSX_DT_F32 ? 4 : 2; }
 extern "C" int64_t nsx_tree_workspace_bytes(int n_head, int n_kv, int head_dim, int max_nodes, int64_t ctx_max) {
   if (tree_shapes(n_head, n_kv, head_dim, max_nodes, max_nodes, ctx_max, 0) != NSX_OK) return -1;
   int64_t most = 0;  // fewer nodes or a window may take more splits, never more than the cache's rows do
-  for (int n = 1; n <= max_nodes; ++n) most = std::max(most, tree_bytes(n_head, n_kv, n, ctx_max, 0));
+  for (int n = 1; n <= max_nodes; ++n)
+    for (const int dt : {NSX_DT_F32, NSX_DT_F16, NSX_DT_BF16})
+      most = std::max(most, tree_bytes(n_head, n_kv, n, ctx_max, 0, dt));
   return most;
 }
 
@@ -677,7 +1155,7 @@ static int tree_checks(const void* kc, const void* vc, int kv_dtype, const void*
   NSX_REQUIRE(kc && vc && dk && dv && pos && workspace && out, NSX_EINVAL, "null buffer");
   NSX_REQUIRE(aligned16(kc) && aligned16(vc) && aligned16(dk) && aligned16(dv) && aligned16(workspace) && aligned16(out),
               NSX_EINVAL, "the caches, the nodes' rows, the workspace and out must be 16-byte aligned");
-  const int64_t need = tree_bytes(n_head, n_kv, nodes, ctx_max, window);
+  const int64_t need = tree_bytes(n_head, n_kv, nodes, ctx_max, window, kv_dtype);
   NSX_REQUIRE(workspace_bytes >= need, NSX_EINVAL, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
               (long long)need);
   return NSX_OK;
@@ -693,9 +1171,8 @@ extern "C" int nsx_tree_attn(const float* q, const void* k_cache, const void* v_
   if (const int rc = tree_checks(k_cache, v_cache, kv_dtype, node_k, node_v, pos, workspace, workspace_bytes, out,
                                  n_head, n_kv, n_nodes, ctx_max, window))
     return rc;
-  const int nsplit = tree_splits(n_kv, n_head / n_kv, n_nodes, ctx_max, window);
   TreeArgs a{q, k_cache, v_cache, node_k, node_v, parents, pos, ctx_max, window, n_head / n_kv, n_kv, n_head, n_nodes,
-             max_nodes, nsplit, 0, scale * LOG2E, (float*)workspace + (int64_t)n_nodes * n_head * ATTN_D, sinks, out};
+             max_nodes, 0, 0, 0, 0, scale * LOG2E, (float*)workspace + (int64_t)n_nodes * n_head * ATTN_D, sinks, out};
   return tree_attn_launch(a, kv_dtype, (hipStream_t)stream);
 }
 
@@ -721,9 +1198,8 @@ extern "C" int nsx_tree_attn_qkv(const float* qkv, const float* q_bias, const fl
   else if (kv_dtype == NSX_DT_F16) rope(_Float16{});
   else rope(Bf16{});
   NSX_LAUNCHED();
-  const int nsplit = tree_splits(n_kv, n_head / n_kv, n_nodes, ctx_max, window);
   TreeArgs a{q, k_cache, v_cache, node_k, node_v, parents, pos, ctx_max, window, n_head / n_kv, n_kv, n_head, n_nodes,
-             max_nodes, nsplit, 0, scale * LOG2E, q + (int64_t)n_nodes * n_head * ATTN_D, sinks, out};
+             max_nodes, 0, 0, 0, 0, scale * LOG2E, q + (int64_t)n_nodes * n_head * ATTN_D, sinks, out};
   return tree_attn_launch(a, kv_dtype, st);
 }
 
