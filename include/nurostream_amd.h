@@ -441,10 +441,12 @@ int nsx_tree_attn_qkv(const float *qkv, const float *q_bias, const float *k_bias
  * *pos, *pos + 1, ..., for all layers ([n_layer][n_kv][ctx_max][64] caches,
  * [n_layer][n_kv][max_nodes][64] nodes), then *pos += *count, at most to
  * ctx_max. Rows past ctx_max and entries of path outside [0, max_nodes) are
- * not copied; other rows stay as they are. */
+ * not copied; other rows stay as they are. counter: one device word, zero
+ * before the first call and after every call. */
 int nsx_tree_commit(void *k_caches, void *v_caches, const void *node_k, const void *node_v, int kv_dtype,
                     int n_layer, int n_kv, int head_dim, int n_nodes, int max_nodes, const int32_t *path,
-                    const int32_t *count, int32_t *pos, int64_t ctx_max, void *stream);
+                    const int32_t *count, int32_t *pos, int64_t ctx_max, uint32_t *counter,
+                    void *stream);
 /* Which drafted tokens the target model accepts, and the token that follows
  * them, for `batch` sequences of n_nodes nodes each. Node 0 is the sequence's
  * last known token, every other one a draft under its parent; row i of a

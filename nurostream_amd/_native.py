@@ -100,7 +100,7 @@ _SIGS = {
                            _p]),
     "nsx_tree_attn_qkv": (_i, [_p, _p, _p, _p, _p, C.c_float, _p, _p, _i, _p, _p, _p, _i, _i, _p, _i, _i, _i, _p, _i64,
                                _i, C.c_float, _p, _i64, _p, _p]),
-    "nsx_tree_commit": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p, _p, _p, _i64, _p]),
+    "nsx_tree_commit": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p, _p, _p, _i64, _p, _p]),
     "nsx_verify_workspace_bytes": (_i64, [_i64, _i, _i64]),
     "nsx_verify": (_i, [_p, _i, _i64, _i64, _i, _i64, _p, _p, _i64, _p, _p, _p, C.c_double, _p, _p, _p, _p, _i64, _p]),
     "nsx_reader_open": (_i, [C.c_char_p, _i, _i, _i, _i64, _i, _p, C.POINTER(_p)]),

@@ -340,19 +340,26 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
   auto weights = [&](int tile, v4f (&s)[NC][2]) {
     const bool own = tile >= pt;
     const int r0 = own ? (tile - pt) * TREE_KEYS : lo + tile * TREE_KEYS;
-    if (own || r0 + TREE_KEYS > P || r0 < deepest) {
+    if (own) {
 #pragma unroll
       for (int ct = 0; ct < NC; ++ct) {
-        const int node = node_of(ct);
-        const int from = a.window > 0 ? P + sdep[node] + 1 - a.window : 0;
-        const uint64_t all = own ? svis[node] : ~0ull;
-        const int lo_k = own ? 0 : from - r0, hi_k = (own ? a.nodes : P) - r0;
-        const uint32_t bits = (uint32_t)(own ? all >> r0 : all);
+        const uint64_t vis = svis[node_of(ct)];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const uint32_t bits = (uint32_t)(vis >> (r0 + 16 * n + 4 * kq));
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[ct][n][r] = bits & (1u << r) ? s[ct][n][r] : -INFINITY;
+        }
+      }
+    } else if (r0 + TREE_KEYS > P || r0 < deepest) {
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct) {
+        const int from = a.window > 0 ? P + sdep[node_of(ct)] + 1 - a.window : 0;
+        const int lo_k = from - r0 - 4 * kq, hi_k = P - r0 - 4 * kq;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int k = 16 * (e >> 2) + 4 * kq + (e & 3);
-          const bool on = k >= lo_k && k < hi_k && (bits >> k & 1);
-          s[ct][e >> 2][e & 3] = on ? s[ct][e >> 2][e & 3] : -INFINITY;
+          const int k = 16 * (e >> 2) + (e & 3);
+          s[ct][e >> 2][e & 3] = k >= lo_k && k < hi_k ? s[ct][e >> 2][e & 3] : -INFINITY;
         }
       }
     }
@@ -585,14 +592,21 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
 
   uint8_t* kl = lds + group * GROUP;
   uint8_t* vl = kl + KF * 1024;
-  auto rsrc = [&](int i, bool values) {  // rows past the last, and tiles past the group's, read as zero
+  // where tile i of the group lies; rows past the last, and tiles past the group's, read as zero
+  struct Source {
+    int64_t at;  // bytes from the start of the rows
+    uint32_t bytes;
+    bool own;
+  };
+  auto source = [&](int i) {
     const int tile = t0 + group + 2 * i;
     const bool own = tile >= pt;
-    const int r0 = own ? (tile - pt) * KEYS : lo + tile * KEYS;
-    const int rows = i < mine ? min((own ? a.nodes : P) - r0, KEYS) : 0;
-    const char* base = (const char*)(own ? (values ? a.dv : a.dk) : (values ? a.vc : a.kc));
-    return nsx_rsrc(base + ((int64_t)g * (own ? a.max_nodes : a.ctx_max) + (i < mine ? r0 : 0)) * R::BYTES,
-                    (uint32_t)rows * R::BYTES);
+    const int r0 = own ? (tile - pt) * KEYS : lo + tile * KEYS, rows = min((own ? a.nodes : P) - r0, KEYS);
+    const int64_t head = (int64_t)g * (own ? a.max_nodes : a.ctx_max);
+    return i < mine ? Source{(head + r0) * R::BYTES, (uint32_t)(rows * R::BYTES), own} : Source{0, 0, false};
+  };
+  auto rsrc = [&](const Source& x, bool values) {
+    return nsx_rsrc((const char*)(x.own ? (values ? a.dv : a.dk) : (values ? a.vc : a.kc)) + x.at, x.bytes);
   };
   // This wave's part of a tile: items cw, cw + CW, .. of 4 a subtile. Of the keys an item is 16 rows x 32 dimensions; of the
   // values 16 rows x 32 dimensions too, a lane holding rows 4 kq .. + 3 of dimensions 2 i16, 2 i16 + 1.
@@ -600,16 +614,16 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
   using V2 = std::conditional_t<std::is_same_v<KT, float>, v2u, uint32_t>;
   typename R::K8 kr[ITEMS];
   V2 vr[ITEMS][4];
-  auto load_k = [&](int i) {
-    const auto r = rsrc(i, false);
+  auto load_k = [&](const Source& x) {
+    const auto r = rsrc(x, false);
 #pragma unroll
     for (int it = 0; it < ITEMS; ++it) {
       const int n = cw + CW * it;  // [subtile][kt][j]
       kr[it] = R::k8(r, 16 * (n >> 1) + i16, n & 1, kq);
     }
   };
-  auto load_v = [&](int i) {
-    const auto r = rsrc(i, true);
+  auto load_v = [&](const Source& x) {
+    const auto r = rsrc(x, true);
 #pragma unroll
     for (int it = 0; it < ITEMS; ++it) {
       const int n = cw + CW * it;  // [subtile][kt][half of the dimensions]
@@ -662,8 +676,9 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
       }
     }
   };
-  load_k(0);
-  load_v(0);
+  Source src = source(0);
+  load_k(src);
+  load_v(src);
 
   if (wave == 0) {
     uint64_t line = tree_lineage(a.parents, a.nodes, lane);
@@ -719,16 +734,23 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
   // scores in powers of two -> weights, 16 keys each of N; r0: the first key's row (own: of the nodes)
   auto weights = [&](auto& x, auto n_tag, bool own, int r0) {
     constexpr int N = decltype(n_tag)::value;
-    if (own || r0 + 16 * N > P || r0 < deepest) {
+    if (own) {
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          const uint32_t bits = (uint32_t)(vis[ct] >> (r0 + 16 * n + 4 * kq));
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[ct][n][r] = bits & (1u << r) ? x[ct][n][r] : -INFINITY;
+        }
+    } else if (r0 + 16 * N > P || r0 < deepest) {
 #pragma unroll
       for (int ct = 0; ct < NC; ++ct) {
-        const int lo_k = own ? 0 : from[ct] - r0, hi_k = (own ? a.nodes : P) - r0;
-        const uint64_t bits = own ? vis[ct] >> r0 : ~0ull;
+        const int lo_k = from[ct] - r0 - 4 * kq, hi_k = P - r0 - 4 * kq;
 #pragma unroll
         for (int e = 0; e < 4 * N; ++e) {
-          const int k = 16 * (e >> 2) + 4 * kq + (e & 3);
-          const bool on = k >= lo_k && k < hi_k && (bits >> k & 1);
-          x[ct][e >> 2][e & 3] = on ? x[ct][e >> 2][e & 3] : -INFINITY;
+          const int k = 16 * (e >> 2) + (e & 3);
+          x[ct][e >> 2][e & 3] = k >= lo_k && k < hi_k ? x[ct][e >> 2][e & 3] : -INFINITY;
         }
       }
     }
@@ -769,65 +791,90 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
     __builtin_amdgcn_sched_barrier(0);
   };
 
+  // The products of a tile step by step, an operand set each: the values of tile i - 1 (the first time: zeros under no
+  // weights), then the keys of tile i (the last time: what is there, unused). A step's operands are read AHEAD steps early.
+  constexpr int STEPS = 8 * TPP, AHEAD = KTN == 1 ? 4 : KTN == 2 ? 2 : 1;
+  auto products = [&] {
+    v4u x[AHEAD + 1][KTN];
+    auto read = [&](int n) {
+#pragma unroll
+      for (int k = 0; k < KTN; ++k)
+        x[n % (AHEAD + 1)][k] =
+            *(const v4u*)((n < 4 * TPP ? vl + n * KTN * 1024 : kl + (n - 4 * TPP) * KTN * 1024) + k * 1024 + lane * 16);
+    };
+    auto dot = [](const v4u& x, const v4u& y, const v4f& c) {
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(x), as_b8(y), c, 0, 0, 0);
+    };
+#pragma unroll
+    for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+      for (int n = 0; n < 2 * TPP; ++n) s[ct][n] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) read(n);
+#pragma unroll
+    for (int n = 0; n < STEPS; ++n) {
+      if (n + AHEAD < STEPS) read(n + AHEAD);
+      const v4u(&y)[KTN] = x[n % (AHEAD + 1)];
+      if (n < 4 * TPP) {
+#pragma unroll
+        for (int o = 2; o >= 0; --o)  // (the small products first)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            if (o - k >= 0 && o - k < KTN) {
+#pragma unroll
+              for (int ct = 0; ct < NC; ++ct) acc[ct][n % 4] = dot(y[o - k], pw[ct][n / 4][k], acc[ct][n % 4]);
+            }
+      } else {
+        const int kn = n - 4 * TPP;
+#pragma unroll
+        for (int o = 2; o >= 0; --o)
+#pragma unroll
+          for (int k = 0; k <= o; ++k)
+            if (o - k < KTN) {
+#pragma unroll
+              for (int ct = 0; ct < NC; ++ct) s[ct][kn / 2] = dot(y[o - k], q[ct][kn % 2][k], s[ct][kn / 2]);
+            }
+      }
+    }
+    // the order above, kept by the scheduler: LDS reads (0x100) ahead of the products (0x8)
+    constexpr int PV = NC * (KTN == 3 ? 5 : 2 * KTN), QK = NC * (KTN == 3 ? 6 : KTN == 2 ? 5 : 3);
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * KTN, 0);
+#pragma unroll
+    for (int n = 0; n < STEPS; ++n) {
+      if (n + AHEAD < STEPS) __builtin_amdgcn_sched_group_barrier(0x100, KTN, 0);
+      if (n < 4 * TPP) __builtin_amdgcn_sched_group_barrier(0x8, PV, 0);
+      else __builtin_amdgcn_sched_group_barrier(0x8, QK, 0);
+    }
+  };
+
   start();
+#pragma unroll
+  for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+    for (int u = 0; u < TPP; ++u) pw[ct][u][0] = pw[ct][u][1] = v4u{0, 0, 0, 0};
+#pragma unroll
+  for (int n = 0; n < VF / CW; ++n) *(v4u*)(vl + (cw + CW * n) * 1024 + lane * 16) = v4u{0, 0, 0, 0};
   store_k();
-  load_k(1);
+  src = source(1);  // the tile whose keys are in registers and whose values are next
+  load_k(src);
   if (group) phase();
   phase();
 #pragma unroll 1
   for (int i = 0; i <= phases; ++i) {
-    __builtin_amdgcn_s_setprio(1);
-    if (i > 0 && i <= mine) {
-#pragma unroll
-      for (int u = 0; u < TPP; ++u)
-#pragma unroll
-        for (int f = 0; f < 4; ++f) {
-          v4u x[KTN];
-#pragma unroll
-          for (int k = 0; k < KTN; ++k) x[k] = *(const v4u*)(vl + ((u * 4 + f) * KTN + k) * 1024 + lane * 16);
-#pragma unroll
-          for (int o = 2; o >= 0; --o)  // (the small products first)
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-              if (o - k >= 0 && o - k < KTN) {
-#pragma unroll
-                for (int ct = 0; ct < NC; ++ct)
-                  acc[ct][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(x[o - k]), as_b8(pw[ct][u][k]), acc[ct][f], 0, 0, 0);
-              }
-        }
+    if (i <= mine) {
+      __builtin_amdgcn_s_setprio(1);
+      products();
+      __builtin_amdgcn_s_setprio(0);
     }
-    if (i < mine) {
-#pragma unroll
-      for (int ct = 0; ct < NC; ++ct)
-#pragma unroll
-        for (int n = 0; n < 2 * TPP; ++n) s[ct][n] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int n = 0; n < 2 * TPP; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          v4u x[KTN];
-#pragma unroll
-          for (int k = 0; k < KTN; ++k) x[k] = *(const v4u*)(kl + ((n * 2 + j) * KTN + k) * 1024 + lane * 16);
-#pragma unroll
-          for (int o = 2; o >= 0; --o)
-#pragma unroll
-            for (int k = 0; k <= o; ++k)
-              if (o - k < KTN) {
-#pragma unroll
-                for (int ct = 0; ct < NC; ++ct)
-                  s[ct][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(x[o - k]), as_b8(q[ct][j][k]), s[ct][n], 0, 0, 0);
-              }
-        }
-    }
-    __builtin_amdgcn_s_setprio(0);
     phase();
     if (i < mine) {
       const int tile = t0 + group + 2 * i;
       const bool own = tile >= pt;
       store_v();
       store_k();
-      load_v(i + 1);
-      load_k(i + 2);
+      load_v(src);
+      src = source(i + 2);
+      load_k(src);
       weights(s, std::integral_constant<int, 2 * TPP>{}, own, own ? (tile - pt) * KEYS : lo + tile * KEYS);
 #pragma unroll
       for (int ct = 0; ct < NC; ++ct)
@@ -860,7 +907,8 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
     for (int i = 0; i < mine * TPP; ++i) {
       const int tile = t0 + group + 2 * (i / TPP);
       const bool own = tile >= pt;
-      const auto rk = rsrc(i / TPP, false), rv = rsrc(i / TPP, true);
+      const Source tile_at = source(i / TPP);
+      const auto rk = rsrc(tile_at, false), rv = rsrc(tile_at, true);
       const int sub = 32 * (i % TPP), r0 = (own ? (tile - pt) * KEYS : lo + tile * KEYS) + sub;
       v4f x[NC][2] = {};
 #pragma unroll
@@ -1024,31 +1072,32 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(TreeArgs a) {
   if (part == 0 && kq == 0) *(v4f*)(a.out + row * ATTN_D + 4 * i16) = v / Z;
 }
 
-// Accepted nodes' rows into the caches: path[j] to row pos + j for j < count. One 16-byte piece of one row per thread
-// over (layer, kv head, j, piece), keys and values.
+// Accepted nodes' rows into the caches: path[j] to row pos + j for j < count, then pos moves on. A thread takes one
+// 16-byte piece of a key row and the same of the value row, over (layer and kv head, j, piece). Every workgroup reads pos
+// and counts itself out; the last one moves it and leaves the counter at zero for the next call. (Nothing else passes
+// between workgroups, so no fence: what the last one knows is that all others have pos.) Latency: two rounds of loads.
 __global__ __launch_bounds__(256) void tree_commit_kernel(char* __restrict__ kc, char* __restrict__ vc,
                                                           const char* __restrict__ dk, const char* __restrict__ dv,
                                                           int row_bytes, int heads, int nodes, int max_nodes,
                                                           const int32_t* __restrict__ path,
-                                                          const int32_t* __restrict__ count,
-                                                          const int32_t* __restrict__ pos, int64_t ctx_max) {
+                                                          const int32_t* __restrict__ count, int32_t* pos,
+                                                          int64_t ctx_max, uint32_t* out) {
   const int pieces = row_bytes / 16;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int p = *pos, n = min(*count, nodes);
   const int c = (int)(i % pieces), j = (int)(i / pieces % nodes);
   const int64_t h = i / pieces / nodes;
-  if (h >= heads || j >= n || p < 0 || (int64_t)p + j >= ctx_max) return;
-  const int src = path[j];
-  if (src < 0 || src >= max_nodes) return;
-  const int64_t from = (h * max_nodes + src) * row_bytes + 16 * c, to = (h * ctx_max + p + j) * row_bytes + 16 * c;
-  const v4u k = *(const v4u*)(dk + from), v = *(const v4u*)(dv + from);
-  *(v4u*)(kc + to) = k;
-  *(v4u*)(vc + to) = v;
-}
-
-__global__ void tree_advance_kernel(int32_t* pos, const int32_t* count, int nodes, int64_t ctx_max) {
-  if (threadIdx.x == 0 && *pos >= 0 && *pos <= ctx_max)
-    *pos = (int32_t)min((int64_t)*pos + max(0, min(*count, nodes)), ctx_max);
+  const int src = path[j], p = *pos, n = max(0, min(*count, nodes));
+  if (h < heads && j < n && p >= 0 && (int64_t)p + j < ctx_max && src >= 0 && src < max_nodes) {
+    const int64_t from = (h * max_nodes + src) * row_bytes + 16 * c, to = (h * ctx_max + p + j) * row_bytes + 16 * c;
+    const v4u k = *(const v4u*)(dk + from), v = *(const v4u*)(dv + from);
+    *(v4u*)(kc + to) = k;
+    *(v4u*)(vc + to) = v;
+  }
+  __syncthreads();  // every wave of the workgroup has pos
+  if (threadIdx.x == 0 && atomicAdd(out, 1u) == gridDim.x - 1) {
+    *out = 0;
+    if (p >= 0 && p <= ctx_max) *pos = (int32_t)min((int64_t)p + n, ctx_max);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1205,12 +1254,13 @@ extern "C" int nsx_tree_attn_qkv(const float* qkv, const float* q_bias, const fl
 
 extern "C" int nsx_tree_commit(void* k_caches, void* v_caches, const void* node_k, const void* node_v, int kv_dtype,
                                int n_layer, int n_kv, int head_dim, int n_nodes, int max_nodes, const int32_t* path,
-                               const int32_t* count, int32_t* pos, int64_t ctx_max, void* stream) {
+                               const int32_t* count, int32_t* pos, int64_t ctx_max, uint32_t* counter,
+                               void* stream) {
   if (const int rc = tree_shapes(n_kv, n_kv, head_dim, n_nodes, max_nodes, ctx_max, 0)) return rc;
   NSX_REQUIRE(n_layer > 0 && (int64_t)n_layer * n_kv < (1 << 24), NSX_EINVAL, "n_layer=%d", n_layer);
   NSX_REQUIRE(kv_dtype == NSX_DT_F32 || kv_dtype == NSX_DT_F16 || kv_dtype == NSX_DT_BF16, NSX_ETYPE,
               "cache element type %d", kv_dtype);
-  NSX_REQUIRE(k_caches && v_caches && node_k && node_v && path && count && pos, NSX_EINVAL, "null buffer");
+  NSX_REQUIRE(k_caches && v_caches && node_k && node_v && path && count && pos && counter, NSX_EINVAL, "null buffer");
   NSX_REQUIRE(aligned16(k_caches) && aligned16(v_caches) && aligned16(node_k) && aligned16(node_v), NSX_EINVAL,
               "the caches and the nodes' rows must be 16-byte aligned");
   hipStream_t st = (hipStream_t)stream;
@@ -1218,9 +1268,7 @@ extern "C" int nsx_tree_commit(void* k_caches, void* v_caches, const void* node_
   const int64_t work = (int64_t)heads * n_nodes * (row / 16);
   hipLaunchKernelGGL(tree_commit_kernel, dim3((unsigned)nsx_cdiv(work, 256)), dim3(256), 0, st, (char*)k_caches,
                      (char*)v_caches, (const char*)node_k, (const char*)node_v, row, heads, n_nodes, max_nodes, path,
-                     count, pos, ctx_max);
-  NSX_LAUNCHED();
-  hipLaunchKernelGGL(tree_advance_kernel, dim3(1), dim3(64), 0, st, pos, count, n_nodes, ctx_max);
+                     count, pos, ctx_max, counter);
   NSX_LAUNCHED();
   return NSX_OK;
 }

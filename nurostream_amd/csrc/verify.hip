@@ -106,8 +106,7 @@ struct Pow2 {
 // The weight 2^(scale2 (x - M)) of logit x beside the largest, M > -infinity. y = n + j / 16 + r with |r| <= 1 / 32 by
 // adding 1.5 * 2^48; 2^r - 1 = r ln2 + r^2 (..), the last part (below 2.4e-4) in 32 bits: an error of 2^-35. Below
 // 2^-1020 it is zero.
-__device__ __forceinline__ double vf_weight(float x, float M, double scale2, const Pow2& tab) {
-  if (M == INFINITY) return x == M ? 1.0 : 0.0;
+__device__ __forceinline__ double vf_weight_finite(float x, float M, double scale2, const Pow2& tab) {
   const double y = ((double)x - (double)M) * scale2;
   const double t = y + 0x1.8p48;
   const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
@@ -118,6 +117,10 @@ __device__ __forceinline__ double vf_weight(float x, float M, double scale2, con
   const double c = tab.t[k & 15], w = fma(fma(r, 0.69314718055994530942, (double)q), c, c);
   const uint64_t bits = __builtin_bit_cast(uint64_t, w) + ((uint64_t)(uint32_t)(k >> 4) << 52);
   return y < -1020.0 ? 0.0 : __builtin_bit_cast(double, bits);
+}
+__device__ __forceinline__ double vf_weight(float x, float M, double scale2, const Pow2& tab) {
+  if (M == INFINITY) return x == M ? 1.0 : 0.0;
+  return vf_weight_finite(x, M, scale2, tab);
 }
 
 template <int WAVES, typename T, typename Op>
@@ -152,20 +155,28 @@ __global__ __launch_bounds__(VF_THREADS) void verify_stats_kernel(VerifyArgs a) 
     for (int k = 0; k < W; ++k) m = fmaxf(m, x[u][k]);
   m = vf_block_reduce<4>(m, redf, [](float p, float q) { return fmaxf(p, q); });
   int at = 0x7fffffff;
-#pragma unroll
-  for (int u = RUNS - 1; u >= 0; --u)
-#pragma unroll
-    for (int k = W - 1; k >= 0; --k)
-      if (x[u][k] == m) at = (int)((int64_t)c * VF_CHUNK + (u * VF_THREADS + t) * W + k - r.off);
   double s = 0.0;
-  if (!GREEDY && m > -INFINITY) {
+  if constexpr (GREEDY) {
 #pragma unroll
-    for (int u = 0; u < RUNS; ++u)
+    for (int u = RUNS - 1; u >= 0; --u)
 #pragma unroll
-      for (int k = 0; k < W; ++k) s += vf_weight(x[u][k], m, a.scale2, tab);
+      for (int k = W - 1; k >= 0; --k)
+        if (x[u][k] == m) at = (int)((int64_t)c * VF_CHUNK + (u * VF_THREADS + t) * W + k - r.off);
+    at = vf_block_reduce<4>(at, redi, [](int p, int q) { return min(p, q); });
+  } else {
+    if (m == INFINITY) {
+#pragma unroll
+      for (int u = 0; u < RUNS; ++u)
+#pragma unroll
+        for (int k = 0; k < W; ++k) s += x[u][k] == m ? 1.0 : 0.0;
+    } else if (m > -INFINITY) {
+#pragma unroll
+      for (int u = 0; u < RUNS; ++u)
+#pragma unroll
+        for (int k = 0; k < W; ++k) s += vf_weight_finite(x[u][k], m, a.scale2, tab);
+    }
+    s = vf_block_reduce<4>(s, redd, [](double p, double q) { return p + q; });
   }
-  at = vf_block_reduce<4>(at, redi, [](int p, int q) { return min(p, q); });
-  if (!GREEDY) s = vf_block_reduce<4>(s, redd, [](double p, double q) { return p + q; });
   if (t == 0) a.part[row * a.nchunk + c] = Part{m, at, s};
 }
 

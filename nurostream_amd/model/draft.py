@@ -43,6 +43,7 @@ class DraftKV:
         self.v_stack = torch.zeros(shape, dtype=kv.dtype, device=kv.device)
         self.k, self.v = list(self.k_stack.unbind(0)), list(self.v_stack.unbind(0))
         self.workspace = torch.empty(nb, dtype=torch.uint8, device=kv.device)
+        self._taken = torch.zeros(1, dtype=torch.int32, device=kv.device)  # commit's workgroups count themselves out here
         self._dt = N.act_dtype_code(kv.dtype)
 
 
@@ -60,6 +61,17 @@ def _check(name: str, t, dtype, device, numel: int | None = None) -> None:
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def _call(what: str, fn, device: torch.device, *args) -> None:
+    """fn(*args, the device's current stream), with the device current."""
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if rc:
+        N.check(rc, what)
 
 
 def _tree(x: torch.Tensor, row: int, name: str, draft: DraftKV, layer: int, cfg: AttnConfig, sinks, parents, out):
@@ -89,13 +101,10 @@ def tree_attn(q: torch.Tensor, cfg: AttnConfig, draft: DraftKV, layer: int, sink
     window > 0 -> (n, n_head, head_dim) fp32."""
     n, y = _tree(q, cfg.n_head * cfg.head_dim, "q", draft, layer, cfg, sinks, parents, out)
     kv = draft.kv
-    with torch.cuda.device(q.device):
-        N.check(N.load().nsx_tree_attn(q.data_ptr(), kv.k[layer].data_ptr(), kv.v[layer].data_ptr(), draft._dt,
-                                       draft.k[layer].data_ptr(), draft.v[layer].data_ptr(), _ptr(parents), n,
-                                       draft.max_nodes, _ptr(sinks), cfg.n_head, cfg.n_head_kv, cfg.head_dim,
-                                       kv.pos.data_ptr(), kv.ctx_max, int(window), 1.0 / math.sqrt(cfg.head_dim),
-                                       draft.workspace.data_ptr(), draft.workspace.numel(), y.data_ptr(),
-                                       N.stream_ptr(q.device)), "tree_attn")
+    _call("tree_attn", N.load().nsx_tree_attn, q.device, q.data_ptr(), kv.k[layer].data_ptr(), kv.v[layer].data_ptr(),
+          draft._dt, draft.k[layer].data_ptr(), draft.v[layer].data_ptr(), _ptr(parents), n, draft.max_nodes,
+          _ptr(sinks), cfg.n_head, cfg.n_head_kv, cfg.head_dim, kv.pos.data_ptr(), kv.ctx_max, int(window),
+          1.0 / math.sqrt(cfg.head_dim), draft.workspace.data_ptr(), draft.workspace.numel(), y.data_ptr())
     return y
 
 
@@ -110,14 +119,11 @@ def tree_attn_qkv(qkv: torch.Tensor, bq, bk, bv, cfg: AttnConfig, inv_freq: torc
                        ("inv_freq", inv_freq, d // 2)):
         _check(name, t, torch.float32, dev, m)
     kv = draft.kv
-    with torch.cuda.device(dev):
-        N.check(N.load().nsx_tree_attn_qkv(qkv.data_ptr(), _ptr(bq), _ptr(bk), _ptr(bv), inv_freq.data_ptr(),
-                                           float(amp), kv.k[layer].data_ptr(), kv.v[layer].data_ptr(), draft._dt,
-                                           draft.k[layer].data_ptr(), draft.v[layer].data_ptr(), _ptr(parents), n,
-                                           draft.max_nodes, _ptr(sinks), cfg.n_head, cfg.n_head_kv, d,
-                                           kv.pos.data_ptr(), kv.ctx_max, int(window), 1.0 / math.sqrt(d),
-                                           draft.workspace.data_ptr(), draft.workspace.numel(), y.data_ptr(),
-                                           N.stream_ptr(dev)), "tree_attn_qkv")
+    _call("tree_attn_qkv", N.load().nsx_tree_attn_qkv, dev, qkv.data_ptr(), _ptr(bq), _ptr(bk), _ptr(bv),
+          inv_freq.data_ptr(), float(amp), kv.k[layer].data_ptr(), kv.v[layer].data_ptr(), draft._dt,
+          draft.k[layer].data_ptr(), draft.v[layer].data_ptr(), _ptr(parents), n, draft.max_nodes, _ptr(sinks),
+          cfg.n_head, cfg.n_head_kv, d, kv.pos.data_ptr(), kv.ctx_max, int(window), 1.0 / math.sqrt(d),
+          draft.workspace.data_ptr(), draft.workspace.numel(), y.data_ptr())
     return y
 
 
@@ -132,11 +138,9 @@ def commit(draft: DraftKV, path: torch.Tensor, count: torch.Tensor) -> None:
     n_layer, n_kv, m, d = draft.k_stack.shape
     if not 1 <= path.numel() <= m:
         raise ValueError(f"a path of {path.numel()} nodes: 1 to {m}")
-    with torch.cuda.device(path.device):
-        N.check(N.load().nsx_tree_commit(kv.k_stack.data_ptr(), kv.v_stack.data_ptr(), draft.k_stack.data_ptr(),
-                                         draft.v_stack.data_ptr(), draft._dt, n_layer, n_kv, d, path.numel(), m,
-                                         path.data_ptr(), count.data_ptr(), kv.pos.data_ptr(), kv.ctx_max,
-                                         N.stream_ptr(path.device)), "commit")
+    _call("commit", N.load().nsx_tree_commit, path.device, kv.k_stack.data_ptr(), kv.v_stack.data_ptr(),
+          draft.k_stack.data_ptr(), draft.v_stack.data_ptr(), draft._dt, n_layer, n_kv, d, path.numel(), m,
+          path.data_ptr(), count.data_ptr(), kv.pos.data_ptr(), kv.ctx_max, draft._taken.data_ptr())
 
 
 def verify(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tensor | None = None, *,
@@ -182,10 +186,9 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tensor | 
     lib = N.load()
     nb = max(0, lib.nsx_verify_workspace_bytes(B, n, V))
     ws = torch.empty(max(nb, 16), dtype=torch.uint8, device=dev)  # stream-ordered scratch, as the outputs
-    with torch.cuda.device(dev):
-        N.check(lib.nsx_verify(x.data_ptr(), dt, ld, B, n, V, tokens.data_ptr(), _ptr(parents), stride, _ptr(lengths),
-                               _ptr(uniforms), _ptr(draft_probs), temperature, count.data_ptr(), path.data_ptr(),
-                               token.data_ptr(), ws.data_ptr(), ws.numel(), N.stream_ptr(dev)), "verify")
+    _call("verify", lib.nsx_verify, dev, x.data_ptr(), dt, ld, B, n, V, tokens.data_ptr(), _ptr(parents), stride,
+          _ptr(lengths), _ptr(uniforms), _ptr(draft_probs), temperature, count.data_ptr(), path.data_ptr(),
+          token.data_ptr(), ws.data_ptr(), max(nb, 16))
     return count, path, token
 
 

@@ -67,16 +67,16 @@ def test_tree_workspace_serves_every_call(lib):
 
 
 def _commit(lib, **kw):
-    a = dict(k=A, v=A, dk=A, dv=A, dt=N.DT_F16, L=2, G=2, d=64, n=4, m=4, path=A, count=A, pos=A, ctx=10)
+    a = dict(k=A, v=A, dk=A, dv=A, dt=N.DT_F16, L=2, G=2, d=64, n=4, m=4, path=A, count=A, pos=A, ctx=10, counter=A)
     a.update(kw)
     return lib.nsx_tree_commit(a["k"], a["v"], a["dk"], a["dv"], a["dt"], a["L"], a["G"], a["d"], a["n"], a["m"],
-                               a["path"], a["count"], a["pos"], a["ctx"], None)
+                               a["path"], a["count"], a["pos"], a["ctx"], a["counter"], None)
 
 
 @pytest.mark.parametrize("kw,code", [
     (dict(L=0), N.EINVAL), (dict(L=1 << 23), N.EINVAL), (dict(G=0), N.EINVAL), (dict(d=32), N.ENOTIMPL),
     (dict(n=5), N.EINVAL), (dict(n=0), N.EINVAL), (dict(dt=3), N.ETYPE), (dict(path=None), N.EINVAL),
-    (dict(count=None), N.EINVAL), (dict(pos=None), N.EINVAL), (dict(k=A + 2), N.EINVAL), (dict(ctx=0), N.EINVAL)])
+    (dict(count=None), N.EINVAL), (dict(pos=None), N.EINVAL), (dict(counter=None), N.EINVAL), (dict(k=A + 2), N.EINVAL), (dict(ctx=0), N.EINVAL)])
 def test_commit_refusals(lib, kw, code):
     assert _commit(lib, **kw) == code
 

@@ -120,6 +120,109 @@ def test_tree_attention_long_cache(dev, heads, n, pos):
         assert rel_max(to_np(out), to_np(ref)) < TOL, ctx
 
 
+WIDE = dict(ctx=70000)  # a capacity from which many columns go to the kernel of 128 columns, however few the rows
+
+
+def _gpu_ref(c, kv, draft, q, parents, sinks, window, pos):
+    """oracle.draft.tree_attention in float64 on the device (tests/test_oracle_draft.py pins the restatement)."""
+    n, G, R = q.shape[0], c.n_head_kv, c.n_head // c.n_head_kv
+    k = torch.cat([kv.k[0][:, :pos], draft.k[0][:, :n]], 1).double()
+    v = torch.cat([kv.v[0][:, :pos], draft.v[0][:, :n]], 1).double()
+    depth, anc = OD.lineage(parents)
+    at = torch.cat([torch.arange(pos), pos + torch.from_numpy(depth)])
+    seen = torch.cat([torch.ones(n, pos, dtype=torch.bool), torch.from_numpy(anc)], 1)
+    if window:
+        seen &= (pos + torch.from_numpy(depth))[:, None] - at[None] < window
+    seen = seen.to(q.device)
+    qd = q.double().reshape(n, G, R, 64)
+    s = torch.stack([qd[:, g].reshape(n * R, 64) @ k[g].T.contiguous() for g in range(G)], 1) / 8.0
+    s = s.reshape(n, R, G, -1).transpose(1, 2).masked_fill(~seen[:, None, None], -math.inf)
+    z = sinks.double().reshape(1, G, R, 1).expand(n, G, R, 1) if sinks is not None else torch.full_like(s[..., :1], -math.inf)
+    w = torch.softmax(torch.cat([s, z], -1), -1)[..., :-1]
+    return to_np(torch.stack([w[:, g].reshape(n * R, -1) @ v[g] for g in range(G)], 1).reshape(n, R, G, 64).transpose(1, 2)
+                 .reshape(n, -1, 64))
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("heads,n,kind", [((32, 2), 64, "tree"), ((16, 1), 33, "chain"), ((24, 8), 50, "tree"),
+                                          ((64, 8), 17, "roots"), ((15, 3), 64, "tree")])
+def test_many_columns(dev, dtype, heads, n, kind):
+    """More columns than 64 over caches whose length lies around the tiles (32 and 64 keys), pairs of them and splits;
+    blocks of 128 columns that end inside."""
+    from nurostream_amd.model.draft import tree_attn
+    for pos in (0, 1, 31, 32, 33, 63, 64, 65, 127, 128, 129, 191, 255, 257, 1000, 5003):
+        c, kv, draft, q, sinks = _state(dev, *heads, n, pos, dtype, seed=pos + n, **WIDE)
+        parents = _parents(n, kind, seed=pos)
+        s = sinks if pos % 2 else None
+        out = tree_attn(q, c, draft, 0, s, 0, parents=_ids(parents, dev) if kind != "chain" else None)
+        assert rel_max(to_np(out), _gpu_ref(c, kv, draft, q, parents, s, 0, pos)) < TOL, pos
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_many_columns_in_a_window(dev, dtype):
+    """Windows that end inside the cache, the nodes' first rows a few apart; rows before every window hold NaN."""
+    from nurostream_amd.model.draft import tree_attn
+    for window, pos, n, kind in ((33000, 33500, 64, "chain"), (33001, 33010, 40, "tree"), (40000, 39990, 64, "chain")):
+        c, kv, draft, q, sinks = _state(dev, 16, 1, n, pos, dtype, seed=n, **WIDE)
+        parents = _parents(n, kind, seed=window)
+        ref = _gpu_ref(c, kv, draft, q, parents, sinks, window, pos)
+        gone = max(0, pos + 1 - window)
+        kv.k[0][:, :gone] = float("nan")
+        kv.v[0][:, :gone] = float("nan")
+        out = tree_attn(q, c, draft, 0, sinks, window, parents=_ids(parents, dev))
+        assert rel_max(to_np(out), ref) < TOL, (window, pos)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_many_columns_beside_rows_of_anything(dev, bad, dtype):
+    """As test_masked_rows_may_hold_anything, in the kernel of 128 columns; and a visible value row of infinities is
+    infinite in its dimensions' outputs and leaves the others as they were."""
+    from nurostream_amd.model.draft import tree_attn
+    n, pos = 64, 700
+    parents = _parents(n, "tree", seed=5)
+    _, anc = OD.lineage(parents)
+    leaf = [j for j in range(1, n) if anc[:, j].sum() == 1][:3]
+    c, kv, draft, q, sinks = _state(dev, 32, 2, n, pos, dtype, seed=9, **WIDE)
+    ref = _gpu_ref(c, kv, draft, q, parents, sinks, 0, pos)
+    for j in leaf:
+        draft.k[0][:, j] = bad
+        draft.v[0][:, j] = bad
+    others = [i for i in range(n) if i not in leaf]
+    out = to_np(tree_attn(q, c, draft, 0, sinks, 0, parents=_ids(parents, dev)))
+    assert rel_max(out[others], ref[others]) < TOL
+    kv.v[0][:, 55, 3::7] = bad
+    out = to_np(tree_attn(q, c, draft, 0, sinks, 0, parents=_ids(parents, dev)))
+    hit = np.zeros(64, bool)
+    hit[3::7] = True
+    assert rel_max(out[others][..., ~hit], ref[others][..., ~hit]) < TOL
+    if math.isnan(bad):
+        assert np.isnan(out[others][..., hit]).all()
+    else:
+        assert (out[others][..., hit] == bad).all()
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_many_columns_keys_of_minus_infinity(dev, dtype):
+    """Keys whose scores overflow to -infinity, whole tiles, pairs of tiles and splits of them (bf16 and fp32; fp16
+    holds keys of -infinity themselves)."""
+    from nurostream_amd.model.draft import tree_attn
+    n = 64
+    parents = _parents(n, "tree", seed=6)
+    for pos, dead in ((64, range(0, 64)), (700, range(0, 640)), (700, range(3, 700, 2))):
+        c, kv, draft, q, sinks = _state(dev, 16, 1, n, pos, dtype, seed=pos, **WIDE)
+        q.reshape(n, 16, 64)[:, :, 0] = 1e20 if dtype != "f16" else 1.0
+        kv.k[0][:, :pos, 0] = 0
+        draft.k[0][:, :n, 0] = 0
+        live = [r for r in range(pos) if r not in set(dead)]
+        ref = OD.tree_attention(to_np(q).reshape(n, 16, 64), to_np(kv.k[0][:, live].double()),
+                                to_np(kv.v[0][:, live].double()), to_np(draft.k[0].double()),
+                                to_np(draft.v[0].double()), parents, to_np(sinks))
+        kv.k[0][:, list(dead), 0] = -1e20 if dtype != "f16" else -math.inf
+        out = tree_attn(q, c, draft, 0, sinks, 0, parents=_ids(parents, dev))
+        assert rel_max(to_np(out), ref) < TOL, pos
+
+
 def test_tree_attention_one_node_is_the_decode_attention(dev):
     """A tree of one node equals the one-token attention with that token's row already in the cache."""
     from nurostream_amd.model.decode import attn_decode
