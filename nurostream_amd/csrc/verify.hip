@@ -123,16 +123,60 @@ __device__ __forceinline__ double vf_weight(float x, float M, double scale2, con
   return vf_weight_finite(x, M, scale2, tab);
 }
 
-template <int WAVES, typename T, typename Op>
-__device__ __forceinline__ T vf_block_reduce(T v, T* red, Op op) {  // the same order in every thread
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
+// Wave-wide operations on DPP moves and readlanes: no trip through LDS.
+template <int CTRL>
+__device__ __forceinline__ double vf_dpp(double v) {  // lanes without a source get 0
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xf, 0xf, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ float vf_lane(float v, int i) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i));
+}
+__device__ __forceinline__ double vf_lane(double v, int i) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), i) << 32 |
+                                        (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, i));
+}
+__device__ __forceinline__ float vf_wave_max(float v) {
+  v = nsx_row_fmax(v);
+  return fmaxf(fmaxf(vf_lane(v, 0), vf_lane(v, 16)), fmaxf(vf_lane(v, 32), vf_lane(v, 48)));
+}
+__device__ __forceinline__ double vf_wave_sum(double v) {
+  v += vf_dpp<NSX_DPP_ROR(8)>(v);
+  v += vf_dpp<NSX_DPP_ROR(4)>(v);
+  v += vf_dpp<NSX_DPP_ROR(2)>(v);
+  v += vf_dpp<NSX_DPP_ROR(1)>(v);
+  return (vf_lane(v, 0) + vf_lane(v, 16)) + (vf_lane(v, 32) + vf_lane(v, 48));
+}
+__device__ __forceinline__ double vf_wave_scan(double v) {  // inclusive: rows of 16 by shifts, then the rows before
+  v += vf_dpp<0x111>(v);
+  v += vf_dpp<0x112>(v);
+  v += vf_dpp<0x114>(v);
+  v += vf_dpp<0x118>(v);
+  const int row = (threadIdx.x & 63) >> 4;
+  const double r0 = vf_lane(v, 15), r1 = r0 + vf_lane(v, 31), r2 = r1 + vf_lane(v, 47);
+  return row == 0 ? v : (row == 1 ? r0 : row == 2 ? r1 : r2) + v;
+}
+// Over 256 threads, the same order in every one.
+__device__ __forceinline__ float vf_block_max(float v, float* red) {
+  v = vf_wave_max(v);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = red[0];
-#pragma unroll
-  for (int w = 1; w < WAVES; ++w) v = op(v, red[w]);
-  return v;
+  return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+__device__ __forceinline__ int vf_block_min(int v, int* red) {  // of values >= 0
+  v = (int)nsx_wave_min_u32((uint32_t)v);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return min(min(red[0], red[1]), min(red[2], red[3]));
+}
+__device__ __forceinline__ double vf_block_sum(double v, double* red) {
+  v = vf_wave_sum(v);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 template <typename LT, bool GREEDY>
@@ -153,7 +197,7 @@ __global__ __launch_bounds__(VF_THREADS) void verify_stats_kernel(VerifyArgs a) 
   for (int u = 0; u < RUNS; ++u)
 #pragma unroll
     for (int k = 0; k < W; ++k) m = fmaxf(m, x[u][k]);
-  m = vf_block_reduce<4>(m, redf, [](float p, float q) { return fmaxf(p, q); });
+  m = vf_block_max(m, redf);
   int at = 0x7fffffff;
   double s = 0.0;
   if constexpr (GREEDY) {
@@ -161,8 +205,8 @@ __global__ __launch_bounds__(VF_THREADS) void verify_stats_kernel(VerifyArgs a) 
     for (int u = RUNS - 1; u >= 0; --u)
 #pragma unroll
       for (int k = W - 1; k >= 0; --k)
-        if (x[u][k] == m) at = (int)((int64_t)c * VF_CHUNK + (u * VF_THREADS + t) * W + k - r.off);
-    at = vf_block_reduce<4>(at, redi, [](int p, int q) { return min(p, q); });
+        if (x[u][k] == m) at = max(0, (int)((int64_t)c * VF_CHUNK + (u * VF_THREADS + t) * W + k - r.off));
+    at = vf_block_min(at, redi);
   } else {
     if (m == INFINITY) {
 #pragma unroll
@@ -175,7 +219,7 @@ __global__ __launch_bounds__(VF_THREADS) void verify_stats_kernel(VerifyArgs a) 
 #pragma unroll
         for (int k = 0; k < W; ++k) s += vf_weight_finite(x[u][k], m, a.scale2, tab);
     }
-    s = vf_block_reduce<4>(s, redd, [](double p, double q) { return p + q; });
+    s = vf_block_sum(s, redd);
   }
   if (t == 0) a.part[row * a.nchunk + c] = Part{m, at, s};
 }
@@ -185,43 +229,19 @@ __device__ __forceinline__ Part vf_row(const VerifyArgs& a, int64_t row, int lan
   const Part* p = a.part + row * a.nchunk;
   const Part none{-INFINITY, 0x7fffffff, 0.0};
   const Part p0 = lane < a.nchunk ? p[lane] : none;  // (most vocabularies: the only ones)
-  float M = p0.m;
+  float mx = p0.m;
   int at = p0.at;
   for (int c = lane + 64; c < a.nchunk; c += 64)
-    if (p[c].m > M) M = p[c].m, at = p[c].at;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor(M, o, 64);
-    const int a2 = __shfl_xor(at, o, 64);
-    if (m2 > M || (m2 == M && a2 < at)) M = m2, at = a2;
-  }
+    if (p[c].m > mx) mx = p[c].m, at = p[c].at;
+  const float M = vf_wave_max(mx);
+  if (a.scale2 == 0.0) return Part{M, (int)nsx_wave_min_u32(mx == M ? (uint32_t)at : 0x7fffffffu), 0.0};
   double s = 0.0;
-  if (a.scale2 != 0.0 && M > -INFINITY) {
+  if (M > -INFINITY) {
     if (p0.m > -INFINITY) s = p0.s * vf_weight(p0.m, M, a.scale2, tab);
     for (int c = lane + 64; c < a.nchunk; c += 64)
       if (p[c].m > -INFINITY) s += p[c].s * vf_weight(p[c].m, M, a.scale2, tab);
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-  return Part{M, at, s};
-}
-
-// max(p - q, 0) of token i at the last node.
-template <typename LT>
-__device__ __forceinline__ double vf_resid(const VerifyArgs& a, int b, const Last& z, double inv_z, const Row<LT>& r,
-                                           int64_t i, const Pow2& tab) {
-  const double q = a.q[((int64_t)b * (a.n - 1) + z.node) * a.V + i];
-  return fmax(vf_weight(r.at(i), z.M, a.scale2, tab) * inv_z - q, 0.0);
-}
-
-__device__ __forceinline__ double vf_wave_scan(double v) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double w = __shfl_up(v, o, 64);
-    if (lane >= o) v += w;
-  }
-  return v;
+  return Part{M, 0, vf_wave_sum(s)};
 }
 
 struct PickLds {
@@ -231,10 +251,10 @@ struct PickLds {
   int chunk, at, last;
 };
 
-// The first token whose running sum exceeds u times the total, from the chunks' sums; weight(i): token i's. -1: no sum
-// is above zero. (A sum that is only rounding, all its chunk's tokens refused, is struck out and the draw made again.)
-template <typename F>
-__device__ int vf_pick(const VerifyArgs& a, PickLds& s, double u, int off, F weight) {
+// The first token whose running sum exceeds u times the total, from the chunks' sums; weight(i, load(i)): token i's. -1:
+// no sum is above zero. (A sum that is only rounding, all its chunk's tokens refused, is struck out and the draw made again.)
+template <typename L, typename F>
+__device__ int vf_pick(const VerifyArgs& a, PickLds& s, double u, int off, L load, F weight) {
   constexpr int PER = VF_CHUNK / VF_WALK;
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
   for (;;) {
@@ -242,7 +262,7 @@ __device__ int vf_pick(const VerifyArgs& a, PickLds& s, double u, int off, F wei
     if (wv == 0) {
       double total = 0.0;
       for (int c0 = 0; c0 < a.nchunk; c0 += 64)
-        total += __shfl(vf_wave_scan(c0 + lane < a.nchunk ? s.sums[c0 + lane] : 0.0), 63, 64);
+        total += vf_lane(vf_wave_scan(c0 + lane < a.nchunk ? s.sums[c0 + lane] : 0.0), 63);
       const double target = u * total;
       double run = 0.0, before = 0.0;
       int pick = -1;
@@ -252,12 +272,12 @@ __device__ int vf_pick(const VerifyArgs& a, PickLds& s, double u, int off, F wei
         const uint64_t some = __ballot(v > 0.0), hit = __ballot(v > 0.0 && run + up > target);
         if (some) {  // (rounding may leave the target past the last weight: then the last chunk that has one)
           const int at = hit ? __ffsll((unsigned long long)hit) - 1 : 63 - __clzll((long long)some);
-          const double pr = __shfl(prev, at, 64);
+          const double pr = vf_lane(prev, at);
           pick = c0 + at;
           before = at ? run + pr : run;
         }
         if (hit) break;
-        run += __shfl(up, 63, 64);
+        run += vf_lane(up, 63);
       }
       if (lane == 0) {
         s.chunk = pick;
@@ -271,10 +291,14 @@ __device__ int vf_pick(const VerifyArgs& a, PickLds& s, double u, int off, F wei
     const int c = s.chunk;
     if (c < 0) return -1;
     const int64_t i0 = (int64_t)c * VF_CHUNK + t * PER - off;
+    decltype(load(0)) raw[PER];  // all loads on their way, then the weights
     double w[PER], mine = 0.0;
 #pragma unroll
+    for (int k = 0; k < PER; ++k) raw[k] = load(min(max(i0 + k, (int64_t)0), a.V - 1));
+#pragma unroll
     for (int k = 0; k < PER; ++k) {
-      w[k] = i0 + k >= 0 && i0 + k < a.V ? weight(i0 + k) : 0.0;
+      w[k] = weight(i0 + k, raw[k]);
+      w[k] = i0 + k >= 0 && i0 + k < a.V ? w[k] : 0.0;
       mine += w[k];
     }
     const double up = vf_wave_scan(mine), prev = __shfl_up(up, 1, 64);
@@ -312,6 +336,7 @@ __global__ __launch_bounds__(VF_WALK) void verify_walk_kernel(VerifyArgs a) {
   __shared__ int s_node, s_nref;
   const int b = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6, n = a.n;
   const int len = a.lengths ? min(a.lengths[b], n) : n;
+  const double u0 = a.u ? a.u[(int64_t)b * n] : 0.f;
   // the nodes' own loads ahead of the rows' sums
   int par = -1, tok = -1;
   float u = 0.f, x = -INFINITY, q = 1.f;
@@ -358,10 +383,10 @@ __global__ __launch_bounds__(VF_WALK) void verify_walk_kernel(VerifyArgs a) {
       const uint64_t cand = __ballot(lane < len && par == cur && lane > last);
       if (!cand) break;
       const int i = __ffsll((unsigned long long)cand) - 1;
-      const int ti = __shfl(tok, i, 64);
+      const int ti = __builtin_amdgcn_readlane(tok, i);
       const bool dup = __ballot((refused >> lane & 1) && tok == ti) != 0;
-      const double pi = dup ? 0.0 : __shfl(p, i, 64), ui = __shfl(u, i, 64);
-      const bool ok = a.q ? ui * (double)__shfl(q, i, 64) < pi : ui * left < pi;
+      const double pi = dup ? 0.0 : vf_lane(p, i), ui = vf_lane(u, i);
+      const bool ok = a.q ? ui * (double)vf_lane(q, i) < pi : ui * left < pi;
       last = i;
       if (ok) {
         cur = i;
@@ -410,13 +435,32 @@ __global__ __launch_bounds__(VF_WALK) void verify_walk_kernel(VerifyArgs a) {
       if (swref[r] > 0.0 && (sref[r] + row.off) / VF_CHUNK == c) s -= swref[r];
     pick.sums[c] = fmax(s, 0.0);
   }
-  const int got = vf_pick(a, pick, (double)a.u[(int64_t)b * n], row.off, [&](int64_t i) {
-    double w = vf_weight(row.at(i), M, a.scale2, tab);
+  const int got = vf_pick(a, pick, u0, row.off, [&](int64_t i) { return row.at(i); }, [&](int64_t i, float x) {
+    double w = vf_weight(x, M, a.scale2, tab);
     for (int r = 0; r < nref; ++r) w = sref[r] == i ? 0.0 : w;
     return w;
   });
   if (t == 0) a.token[b] = got;
 }
+
+// max(p - q, 0) at the last node.
+template <typename LT>
+struct Resid {
+  const Row<LT> row;
+  const float* q;
+  const Last z;
+  const double scale2, inv_z;
+  struct Raw {
+    float x, q;
+  };
+  __device__ __forceinline__ Resid(const VerifyArgs& a, int b, const Last& z)
+      : row(a, (int64_t)b * a.n + z.node), q(a.q + ((int64_t)b * (a.n - 1) + z.node) * a.V), z(z), scale2(a.scale2),
+        inv_z(1.0 / z.Z) {}
+  __device__ __forceinline__ Raw load(int64_t i) const { return Raw{row.at(i), q[i]}; }
+  __device__ __forceinline__ double weight(const Raw& r, const Pow2& tab) const {
+    return fmax(vf_weight(r.x, z.M, scale2, tab) * inv_z - (double)r.q, 0.0);
+  }
+};
 
 // q: chunk sums of max(p - q, 0) at the last node, where a child was refused.
 template <typename LT>
@@ -429,15 +473,19 @@ __global__ __launch_bounds__(VF_THREADS) void verify_resid_kernel(VerifyArgs a) 
   if (z.node < 0) return;
   tab.fill();
   __syncthreads();
-  const Row<LT> row(a, (int64_t)b * a.n + z.node);
-  const double inv_z = 1.0 / z.Z;
+  const Resid<LT> r(a, b, z);
+  typename Resid<LT>::Raw raw[PER];
+  const int64_t i0 = (int64_t)c * VF_CHUNK + threadIdx.x - r.row.off;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) raw[k] = r.load(min(max(i0 + VF_THREADS * k, (int64_t)0), a.V - 1));
   double s = 0.0;
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    const int64_t i = (int64_t)c * VF_CHUNK + VF_THREADS * k + threadIdx.x - row.off;
-    if (i >= 0 && i < a.V) s += vf_resid(a, b, z, inv_z, row, i, tab);
+    const int64_t i = i0 + VF_THREADS * k;
+    const double w = r.weight(raw[k], tab);
+    s += i >= 0 && i < a.V ? w : 0.0;
   }
-  s = vf_block_reduce<4>(s, redd, [](double p, double q) { return p + q; });
+  s = vf_block_sum(s, redd);
   if (threadIdx.x == 0) a.resid[(int64_t)b * a.nchunk + c] = s;
 }
 
@@ -449,15 +497,17 @@ __global__ __launch_bounds__(VF_WALK) void verify_draw_kernel(VerifyArgs a) {
   const Last z = a.last[b];
   if (z.node < 0) return;
   tab.fill();
-  const double u = a.u[(int64_t)b * a.n], inv_z = 1.0 / z.Z;
-  const Row<LT> row(a, (int64_t)b * a.n + z.node);
+  const double u = a.u[(int64_t)b * a.n];
+  const Resid<LT> r(a, b, z);
   for (int c = threadIdx.x; c < a.nchunk; c += VF_WALK) pick.sums[c] = a.resid[(int64_t)b * a.nchunk + c];
-  int got = vf_pick(a, pick, u, row.off, [&](int64_t i) { return vf_resid(a, b, z, inv_z, row, i, tab); });
+  int got = vf_pick(a, pick, u, r.row.off, [&](int64_t i) { return r.load(i); },
+                    [&](int64_t, const typename Resid<LT>::Raw& x) { return r.weight(x, tab); });
   if (got < 0) {  // p nowhere above q (to rounding): drawn from p
     const Part* pr = a.part + ((int64_t)b * a.n + z.node) * a.nchunk;
     for (int c = threadIdx.x; c < a.nchunk; c += VF_WALK)
       pick.sums[c] = pr[c].m > -INFINITY ? pr[c].s * vf_weight(pr[c].m, z.M, a.scale2, tab) : 0.0;
-    got = vf_pick(a, pick, u, row.off, [&](int64_t i) { return vf_weight(row.at(i), z.M, a.scale2, tab); });
+    got = vf_pick(a, pick, u, r.row.off, [&](int64_t i) { return r.row.at(i); },
+                  [&](int64_t, float x) { return vf_weight(x, z.M, a.scale2, tab); });
   }
   if (threadIdx.x == 0) a.token[b] = got;
 }
