@@ -35,6 +35,10 @@ struct TreeArgs {
   float* part;
   const float* sinks;
   float* out;
+  // from raw projections: q is [nodes][n_head + 2 n_kv][64], and the nodes' rows are written to wk, wv (dk, dv)
+  const float *bq, *bk, *bv, *inv_freq;
+  float amp;
+  void *wk, *wv;
 };
 
 // Which tiles a split takes: the cache's rows from the first that any node sees, then the nodes' own rows.
@@ -74,7 +78,10 @@ __device__ __forceinline__ uint64_t tree_lineage(const int32_t* __restrict__ par
 template <typename KT>
 __device__ __forceinline__ void store_kv(void* p, int64_t i, float v) {
   if constexpr (std::is_same_v<KT, float>) ((float*)p)[i] = v;
-  else if constexpr (std::is_same_v<KT, _Float16>) ((_Float16*)p)[i] = (_Float16)v;
+  else if constexpr (std::is_same_v<KT, _Float16>) {
+    asm("" : "+v"(v));  // the fp32 value, rounded: not one instruction with what made it, rounding once
+    ((_Float16*)p)[i] = (_Float16)v;
+  }
   else ((uint16_t*)p)[i] = (uint16_t)nsx_f2bf(v);
 }
 struct Bf16 {
@@ -160,6 +167,10 @@ struct Rows<float> {
   static __device__ __forceinline__ V4 v4(__amdgpu_buffer_rsrc_t r, int row, int i) {
     return __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(r, row * BYTES + 16 * i, 0, 0));
   }
+  static __device__ __forceinline__ K8 k8(const uint8_t* row, int j, int g) {
+    return K8{*(const v4u*)(row + 128 * j + 16 * g), *(const v4u*)(row + 128 * j + 16 * g + 64)};
+  }
+  static __device__ __forceinline__ V4 v4(const uint8_t* row, int i) { return *(const v4u*)(row + 16 * i); }
   static __device__ __forceinline__ float k(const K8& x, int e) {
     return __builtin_bit_cast(float, e < 4 ? x.a[e & 3] : x.b[e & 3]);
   }
@@ -177,6 +188,8 @@ struct Rows16 {  // dimensions 32 j + 8 g .. + 7
   static __device__ __forceinline__ V4 v4(__amdgpu_buffer_rsrc_t r, int row, int i) {
     return __builtin_bit_cast(v2u, __builtin_amdgcn_raw_buffer_load_b64(r, row * BYTES + 8 * i, 0, 0));
   }
+  static __device__ __forceinline__ K8 k8(const uint8_t* row, int j, int g) { return *(const v4u*)(row + 64 * j + 16 * g); }
+  static __device__ __forceinline__ V4 v4(const uint8_t* row, int i) { return *(const v2u*)(row + 8 * i); }
   static __device__ __forceinline__ float one(uint32_t w, int hi) {
     if constexpr (std::is_same_v<KT, Bf16>) return __builtin_bit_cast(float, hi ? w & 0xffff0000u : w << 16);
     else return nsx_h2f(hi ? w >> 16 : w & 0xffffu);
@@ -239,15 +252,22 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028235e3
 // A key with weight zero takes no part whatever its value row holds (0 * NaN would be NaN): a wave whose sums are not
 // finite at the end goes through its tiles again, with products in fp32 and values added one key at a time under their
 // weights. (That is also what infinite keys and values take: of their terms the second is NaN.)
-template <typename KT, int NC>
+//
+// ROPE: q is the nodes' raw projections. A workgroup forms the sines and cosines of its columns' nodes (of all nodes where
+// its split has some of theirs) once, as a table in LDS, and rotates its queries by it; a split with node tiles also
+// makes those tiles' rows, for its own use in LDS and, the first block of columns, for the cache's keeper in wk and wv.
+template <typename KT, int NC, bool ROPE>
 __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) {
   using R = Rows<KT>;
   constexpr int NT = 64 * TREE_NW, COLS = 16 * NC, KTN = R::NT;
   constexpr int QROW = 2 * ATTN_D + 16, OROW = ATTN_D + 4;  // bytes of a column's term, floats of a column's sums
   constexpr int QBYTES = 3 * COLS * QROW, PBYTES = TREE_KEYS * COLS * 4;
-  constexpr int LDS = std::max(QBYTES + TREE_NW * PBYTES, TREE_NW * COLS * OROW * 4);
-  // first the columns' query terms [term][column] and behind them each wave's weights of a tile (the second way); in the
-  // end each wave's sums
+  constexpr int HALF = ATTN_D / 2, NROW = R::BYTES + 16, NBYTES = NSX_TREE_MAX_NODES * NROW;
+  constexpr int TABLE = ROPE ? NSX_TREE_MAX_NODES * HALF * (int)sizeof(float2) : 0;
+  constexpr int NODES_AT = QBYTES + std::max(TREE_NW * PBYTES, TABLE);
+  constexpr int LDS = std::max(NODES_AT + (ROPE ? 2 * NBYTES : 0), TREE_NW * COLS * OROW * 4);
+  // first the columns' query terms [term][column]; behind them the table, then each wave's weights of a tile (the second
+  // way); behind those the node tiles' keys and values; in the end each wave's sums
   __shared__ __align__(16) uint8_t lds[LDS];
   __shared__ float sm[TREE_NW][COLS], sl[TREE_NW][COLS];
   __shared__ uint64_t svis[64];
@@ -261,15 +281,18 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
   const int lo = tl.lo, pt = tl.cache, t0 = c * tl.per, t1 = min(tl.all, t0 + tl.per);
   if (t0 >= t1) return;
   const int ncol = a.nodes * a.n_rep, col0 = cb * COLS;
+  // ROPE: the node tiles come after the loop, from LDS
+  const int first = t0 + wave, end = ROPE ? min(t1, pt) : t1, last = end - 1, nodes0 = max(t0, pt);
 
   typename R::K8 kr[2][2];
   typename R::V4 vr[8];
-  auto rsrc = [&](int tile, bool values) {  // rows past the last read as zero
-    const bool own = tile >= pt;
-    const int r0 = own ? (tile - pt) * TREE_KEYS : lo + tile * TREE_KEYS, rows = (own ? a.nodes : P) - r0;
+  auto rsrc = [&](int tile, bool values) {  // rows past the last read as zero, as does a tile before the split's first
+    const bool own = !ROPE && tile >= pt;
+    const int r0 = own ? (tile - pt) * TREE_KEYS : lo + tile * TREE_KEYS;
+    const int rows = tile < t0 ? 0 : min((own ? a.nodes : P) - r0, TREE_KEYS);
     const char* base = (const char*)(own ? (values ? a.dv : a.dk) : (values ? a.vc : a.kc));
-    return nsx_rsrc(base + ((int64_t)g * (own ? a.max_nodes : a.ctx_max) + r0) * R::BYTES,
-                    (uint32_t)min(rows, TREE_KEYS) * R::BYTES);
+    return nsx_rsrc(base + ((int64_t)g * (own ? a.max_nodes : a.ctx_max) + (tile < t0 ? 0 : r0)) * R::BYTES,
+                    (uint32_t)(rows * R::BYTES));
   };
   auto load_k = [&](int tile) {
     const auto r = rsrc(tile, false);
@@ -283,7 +306,21 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
 #pragma unroll
     for (int e = 0; e < 8; ++e) vr[e] = R::v4(r, 16 * (e >> 2) + 4 * kq + (e & 3), i16);
   };
-  const int first = t0 + wave, last = t1 - 1;
+  // key (or value) row k of a node tile in LDS, the last row for those past it
+  auto node_row = [&](int tile, int k, bool values) {
+    const int row = min((tile - pt) * TREE_KEYS + k, a.nodes - 1) - (nodes0 - pt) * TREE_KEYS;
+    return (const uint8_t*)&lds[NODES_AT + (values ? NBYTES : 0) + row * NROW];
+  };
+  auto node_k = [&](int tile) {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) kr[kt][j] = R::k8(node_row(tile, 16 * kt + i16, false), j, kq);
+  };
+  auto node_v = [&](int tile) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) vr[e] = R::v4(node_row(tile, 16 * (e >> 2) + 4 * kq + (e & 3), true), i16);
+  };
   load_k(min(first, last));
   load_v(min(first, last));
 
@@ -297,14 +334,62 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
     svis[lane] = line;
     sdep[lane] = dep;
   }
+  const int heads = ROPE ? a.n_head + 2 * a.n_kv : a.n_head;  // rows of a node in q
+  float2* turn = (float2*)&lds[QBYTES];                       // amplitude times (cosine, sine)
+  if constexpr (ROPE) {
+    lds_barrier();
+    const int na = t1 > pt ? 0 : col0 / a.n_rep, nb = t1 > pt ? a.nodes : min(col0 + COLS - 1, ncol - 1) / a.n_rep + 1;
+    for (int i = na * HALF + t; i < nb * HALF; i += NT) {
+      float s, co;
+      sincosf((float)(P + sdep[i / HALF]) * a.inv_freq[i % HALF], &s, &co);
+      turn[i] = float2{co * a.amp, s * a.amp};
+    }
+    lds_barrier();
+    const int r0 = (nodes0 - pt) * TREE_KEYS, rows = min((t1 - pt) * TREE_KEYS, a.nodes) - r0;
+    for (int i = t; i < rows * HALF; i += NT) {
+      const int row = r0 + i / HALF, d = i % HALF;
+      const float* x = a.q + ((int64_t)row * heads + a.n_head + g) * ATTN_D + d;
+      const float* y = x + (int64_t)a.n_kv * ATTN_D;
+      float k0 = x[0], k1 = x[HALF], v0 = y[0], v1 = y[HALF];
+      if (a.bk) k0 += a.bk[g * ATTN_D + d], k1 += a.bk[g * ATTN_D + d + HALF];
+      if (a.bv) v0 += a.bv[g * ATTN_D + d], v1 += a.bv[g * ATTN_D + d + HALF];
+      const float2 w = turn[row * HALF + d];
+      const float z0 = fmaf(k0, w.x, -(k1 * w.y)), z1 = fmaf(k1, w.x, k0 * w.y);  // (as rope_elem)
+      uint8_t* to = &lds[NODES_AT + (row - r0) * NROW];
+      store_kv<KT>(to, d, z0), store_kv<KT>(to, d + HALF, z1);
+      store_kv<KT>(to + NBYTES, d, v0), store_kv<KT>(to + NBYTES, d + HALF, v1);
+      if (cb == 0) {
+        const int64_t at = ((int64_t)g * a.max_nodes + row) * ATTN_D + d;
+        store_kv<KT>(a.wk, at, z0), store_kv<KT>(a.wk, at + HALF, z1);
+        store_kv<KT>(a.wv, at, v0), store_kv<KT>(a.wv, at + HALF, v1);
+      }
+    }
+  }
   for (int i = t; i < COLS * (ATTN_D / 8); i += NT) {
     const int cc = i / (ATTN_D / 8), col = min(col0 + cc, ncol - 1), j = i / 4 % 2, gg = i % 4;
     const int node = col / a.n_rep, h = g * a.n_rep + col % a.n_rep;
-    const float* qp = a.q + ((int64_t)node * a.n_head + h) * ATTN_D;
-    const v4f x0 = *(const v4f*)(qp + R::dim(j, gg, 0)), x1 = *(const v4f*)(qp + R::dim(j, gg, 4));
-    float x[8];
+    const float* qp = a.q + ((int64_t)node * heads + h) * ATTN_D;
+    auto eight = [&](const float* p, int jj, float (&x)[8]) {
+      const v4f x0 = *(const v4f*)(p + R::dim(jj, gg, 0)), x1 = *(const v4f*)(p + R::dim(jj, gg, 4));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = (e < 4 ? x0[e & 3] : x1[e & 3]) * a.scale2;
+      for (int e = 0; e < 8; ++e) x[e] = e < 4 ? x0[e & 3] : x1[e & 3];
+    };
+    float x[8];
+    eight(qp, j, x);
+    if constexpr (ROPE) {
+      float other[8];
+      eight(qp, j ^ 1, other);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int d = R::dim(0, gg, e);
+        if (a.bq) x[e] += a.bq[h * ATTN_D + HALF * j + d], other[e] += a.bq[h * ATTN_D + HALF * (j ^ 1) + d];
+        const float2 w = turn[node * HALF + d];
+        const float ps = other[e] * w.y;
+        x[e] = fmaf(x[e], w.x, j ? ps : -ps);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= a.scale2;
     v4u tm[3];
     split8(x, tm);
 #pragma unroll
@@ -395,9 +480,8 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
     }
   };
 
-  start();
-  for (int tile = first; tile < t1; tile += TREE_NW) {
-    const int next = min(tile + TREE_NW, last);
+  // a tile whose rows are in kr and vr, the next one's loads on their way as soon as they are free
+  auto take = [&](int tile, auto next_k, auto next_v) {
     v4f s[NC][2] = {};
     {
       v4u kt_[2][2][KTN];
@@ -405,7 +489,7 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int j = 0; j < 2; ++j) key_terms<KT>(kr[kt][j], kt_[kt][j]);
-      load_k(next);
+      next_k();
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -437,7 +521,7 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
     for (int dt = 0; dt < 4; ++dt) {
       v4u vt[KTN];
       value_terms<KT>(vr, dt, vt);
-      if (dt == 3) load_v(next);
+      if (dt == 3) next_v();
 #pragma unroll
       for (int o = 2; o >= 0; --o)
 #pragma unroll
@@ -447,6 +531,21 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
             for (int ct = 0; ct < NC; ++ct)
               acc[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(vt[o - k]), as_b8(pw[ct][k]), acc[ct][dt], 0, 0, 0);
           }
+    }
+  };
+
+  start();
+  int tile = first;
+  for (; tile < end; tile += TREE_NW) {
+    const int next = min(tile + TREE_NW, last);
+    take(tile, [&] { load_k(next); }, [&] { load_v(next); });
+  }
+  if constexpr (ROPE) {
+#pragma unroll 1
+    for (; tile < t1; tile += TREE_NW) {
+      node_k(tile);
+      node_v(tile);
+      take(tile, [] {}, [] {});
     }
   }
   bool ok = true;
@@ -460,7 +559,9 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
     start();
 #pragma unroll 1
     for (int tile = first; tile < t1; tile += TREE_NW) {
-      load_k(tile);
+      const bool in_lds = ROPE && tile >= pt;
+      if (in_lds) node_k(tile);
+      else load_k(tile);
       v4f s[NC][2] = {};
 #pragma unroll
       for (int ct = 0; ct < NC; ++ct)
@@ -484,12 +585,12 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
 #pragma unroll
         for (int e = 0; e < 8; ++e) sp[(16 * (e >> 2) + 4 * kq + (e & 3)) * COLS + 16 * ct + i16] = s[ct][e >> 2][e & 3];
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      const auto r = rsrc(tile, true);
+      const auto r = rsrc(in_lds ? t0 - 1 : tile, true);
 #pragma unroll 1
       for (int k = 0; k < TREE_KEYS; ++k) {
         typename R::V4 v[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = R::v4(r, k, 4 * kq + u);
+        for (int u = 0; u < 4; ++u) v[u] = in_lds ? R::v4(node_row(tile, k, true), 4 * kq + u) : R::v4(r, k, 4 * kq + u);
 #pragma unroll
         for (int ct = 0; ct < NC; ++ct) {
           const float w = sp[k * COLS + 16 * ct + i16];
@@ -546,14 +647,6 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
       }
     }
   }
-}
-
-// Two bf16 terms of a pair of weights, each rounded to nearest: 2^-17 of a weight, the rounding of an fp32 score of 64.
-__device__ __forceinline__ void split_weights(float a, float b, uint32_t& hi, uint32_t& lo) {
-  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-  hi = __builtin_bit_cast(uint32_t, b2{(__bf16)a, (__bf16)b});
-  lo = __builtin_bit_cast(uint32_t, b2{(__bf16)(a - __builtin_bit_cast(float, hi << 16)),
-                                       (__bf16)(b - __builtin_bit_cast(float, hi & 0xffff0000u))});
 }
 
 // The same attention for many columns: a workgroup of 8 waves takes 128 columns and a split of the keys. Four waves (32
@@ -721,7 +814,7 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
   float m[NC], l[NC];
   v4f acc[NC][4];  // [dimension's half, parity]
   v4f s[NC][2 * TPP];
-  v4u pw[NC][TPP][2];
+  v4u pw[NC][TPP][3];
   auto start = [&] {
 #pragma unroll
     for (int ct = 0; ct < NC; ++ct) {
@@ -819,8 +912,8 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
 #pragma unroll
         for (int o = 2; o >= 0; --o)  // (the small products first)
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
-            if (o - k >= 0 && o - k < KTN) {
+          for (int k = 0; k <= o; ++k)
+            if (o - k < KTN) {
 #pragma unroll
               for (int ct = 0; ct < NC; ++ct) acc[ct][n % 4] = dot(y[o - k], pw[ct][n / 4][k], acc[ct][n % 4]);
             }
@@ -837,13 +930,12 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
       }
     }
     // the order above, kept by the scheduler: LDS reads (0x100) ahead of the products (0x8)
-    constexpr int PV = NC * (KTN == 3 ? 5 : 2 * KTN), QK = NC * (KTN == 3 ? 6 : KTN == 2 ? 5 : 3);
+    constexpr int PRODUCTS = NC * (KTN == 3 ? 6 : KTN == 2 ? 5 : 3);
     __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * KTN, 0);
 #pragma unroll
     for (int n = 0; n < STEPS; ++n) {
       if (n + AHEAD < STEPS) __builtin_amdgcn_sched_group_barrier(0x100, KTN, 0);
-      if (n < 4 * TPP) __builtin_amdgcn_sched_group_barrier(0x8, PV, 0);
-      else __builtin_amdgcn_sched_group_barrier(0x8, QK, 0);
+      __builtin_amdgcn_sched_group_barrier(0x8, PRODUCTS, 0);
     }
   };
 
@@ -851,7 +943,7 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
 #pragma unroll
   for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
-    for (int u = 0; u < TPP; ++u) pw[ct][u][0] = pw[ct][u][1] = v4u{0, 0, 0, 0};
+    for (int u = 0; u < TPP; ++u) pw[ct][u][0] = pw[ct][u][1] = pw[ct][u][2] = v4u{0, 0, 0, 0};
 #pragma unroll
   for (int n = 0; n < VF / CW; ++n) *(v4u*)(vl + (cw + CW * n) * 1024 + lane * 16) = v4u{0, 0, 0, 0};
   store_k();
@@ -879,15 +971,12 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
 #pragma unroll
       for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
-        for (int u = 0; u < TPP; ++u)
+        for (int u = 0; u < TPP; ++u) {
+          float x[8];
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const v4f& y = s[ct][2 * u + (w >> 1)];
-            uint32_t hi, low;
-            split_weights(y[2 * (w & 1)], y[2 * (w & 1) + 1], hi, low);
-            pw[ct][u][0][w] = hi;
-            pw[ct][u][1][w] = low;
-          }
+          for (int e = 0; e < 8; ++e) x[e] = s[ct][2 * u + (e >> 2)][e & 3];
+          split8(x, pw[ct][u]);
+        }
     }
     phase();
   }
@@ -1154,16 +1243,28 @@ int tree_shapes(int n_head, int n_kv, int head_dim, int nodes, int max_nodes, in
   return NSX_OK;
 }
 
-template <typename KT>
+template <typename KT, bool ROPE>
 int tree_attn_typed(TreeArgs& a, const TreePlan& p, hipStream_t st) {
   a.nsplit = p.nsplit;
   a.ncb = p.ncb;
   a.keys = p.keys;
   a.round = p.round;
   const dim3 grid(a.n_kv * a.ncb, a.nsplit);
-  if (p.kind == TREE_16) hipLaunchKernelGGL((tree_attn_kernel<KT, 1>), grid, dim3(64 * TREE_NW), 0, st, a);
-  else if (p.kind == TREE_32) hipLaunchKernelGGL((tree_attn_kernel<KT, 2>), grid, dim3(64 * TREE_NW), 0, st, a);
-  else hipLaunchKernelGGL((tree_wide_kernel<KT>), grid, dim3(512), 0, st, a);
+  if (p.kind == TREE_16) {
+    hipLaunchKernelGGL((tree_attn_kernel<KT, 1, ROPE>), grid, dim3(64 * TREE_NW), 0, st, a);
+  } else if (p.kind == TREE_32) {
+    hipLaunchKernelGGL((tree_attn_kernel<KT, 2, ROPE>), grid, dim3(64 * TREE_NW), 0, st, a);
+  } else {
+    if constexpr (ROPE) {  // a launch of its own: little beside this kernel's time
+      float* q = a.part - (int64_t)a.nodes * a.n_head * ATTN_D;
+      const dim3 rows((unsigned)nsx_cdiv((int64_t)a.nodes * (a.n_head + 2 * a.n_kv), 4));
+      hipLaunchKernelGGL((tree_rope_kernel<KT>), rows, dim3(256), 0, st, a.q, a.bq, a.bk, a.bv, a.inv_freq, a.amp,
+                         a.n_head, a.n_kv, a.parents, a.pos, a.ctx_max, a.nodes, a.max_nodes, q, a.wk, a.wv);
+      NSX_LAUNCHED();
+      a.q = q;
+    }
+    hipLaunchKernelGGL((tree_wide_kernel<KT>), grid, dim3(512), 0, st, a);
+  }
   NSX_LAUNCHED();
   if (a.nsplit > 1) {
     // a wave per row, or four where the rows are few and their splits many
@@ -1175,11 +1276,12 @@ int tree_attn_typed(TreeArgs& a, const TreePlan& p, hipStream_t st) {
   return NSX_OK;
 }
 
+template <bool ROPE>
 int tree_attn_launch(TreeArgs& a, int kv_dtype, hipStream_t st) {
   const TreePlan p = tree_plan(a.n_kv, a.n_rep, a.nodes, a.ctx_max, a.window, kv_dtype);
-  if (kv_dtype == NSX_DT_F32) return tree_attn_typed<float>(a, p, st);
-  if (kv_dtype == NSX_DT_F16) return tree_attn_typed<_Float16>(a, p, st);
-  return tree_attn_typed<Bf16>(a, p, st);
+  if (kv_dtype == NSX_DT_F32) return tree_attn_typed<float, ROPE>(a, p, st);
+  if (kv_dtype == NSX_DT_F16) return tree_attn_typed<_Float16, ROPE>(a, p, st);
+  return tree_attn_typed<Bf16, ROPE>(a, p, st);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -1221,8 +1323,9 @@ extern "C" int nsx_tree_attn(const float* q, const void* k_cache, const void* v_
                                  n_head, n_kv, n_nodes, ctx_max, window))
     return rc;
   TreeArgs a{q, k_cache, v_cache, node_k, node_v, parents, pos, ctx_max, window, n_head / n_kv, n_kv, n_head, n_nodes,
-             max_nodes, 0, 0, 0, 0, scale * LOG2E, (float*)workspace + (int64_t)n_nodes * n_head * ATTN_D, sinks, out};
-  return tree_attn_launch(a, kv_dtype, (hipStream_t)stream);
+             max_nodes, 0, 0, 0, 0, scale * LOG2E, (float*)workspace + (int64_t)n_nodes * n_head * ATTN_D, sinks, out, nullptr, nullptr, nullptr, nullptr, 0.f,
+             nullptr, nullptr};
+  return tree_attn_launch<false>(a, kv_dtype, (hipStream_t)stream);
 }
 
 extern "C" int nsx_tree_attn_qkv(const float* qkv, const float* q_bias, const float* k_bias, const float* v_bias,
@@ -1232,24 +1335,14 @@ extern "C" int nsx_tree_attn_qkv(const float* qkv, const float* q_bias, const fl
                                  const int32_t* pos, int64_t ctx_max, int window, float scale, void* workspace,
                                  int64_t workspace_bytes, float* out, void* stream) {
   if (const int rc = tree_shapes(n_head, n_kv, head_dim, n_nodes, max_nodes, ctx_max, window)) return rc;
-  NSX_REQUIRE(qkv && inv_freq, NSX_EINVAL, "null buffer");
+  NSX_REQUIRE(qkv && aligned16(qkv) && inv_freq, NSX_EINVAL, "qkv must be a 16-byte aligned buffer, inv_freq not null");
   if (const int rc = tree_checks(k_cache, v_cache, kv_dtype, node_k, node_v, pos, workspace, workspace_bytes, out,
                                  n_head, n_kv, n_nodes, ctx_max, window))
     return rc;
-  hipStream_t st = (hipStream_t)stream;
-  float* q = (float*)workspace;
-  const dim3 grid((unsigned)nsx_cdiv((int64_t)n_nodes * (n_head + 2 * n_kv), 4)), block(256);
-  auto rope = [&](auto tag) {
-    hipLaunchKernelGGL((tree_rope_kernel<decltype(tag)>), grid, block, 0, st, qkv, q_bias, k_bias, v_bias, inv_freq,
-                       amplitude, n_head, n_kv, parents, pos, ctx_max, n_nodes, max_nodes, q, node_k, node_v);
-  };
-  if (kv_dtype == NSX_DT_F32) rope(float{});
-  else if (kv_dtype == NSX_DT_F16) rope(_Float16{});
-  else rope(Bf16{});
-  NSX_LAUNCHED();
-  TreeArgs a{q, k_cache, v_cache, node_k, node_v, parents, pos, ctx_max, window, n_head / n_kv, n_kv, n_head, n_nodes,
-             max_nodes, 0, 0, 0, 0, scale * LOG2E, q + (int64_t)n_nodes * n_head * ATTN_D, sinks, out};
-  return tree_attn_launch(a, kv_dtype, st);
+  TreeArgs a{qkv, k_cache, v_cache, node_k, node_v, parents, pos, ctx_max, window, n_head / n_kv, n_kv, n_head, n_nodes,
+             max_nodes, 0, 0, 0, 0, scale * LOG2E, (float*)workspace + (int64_t)n_nodes * n_head * ATTN_D, sinks, out, q_bias,
+             k_bias, v_bias, inv_freq, amplitude, node_k, node_v};
+  return tree_attn_launch<true>(a, kv_dtype, (hipStream_t)stream);
 }
 
 extern "C" int nsx_tree_commit(void* k_caches, void* v_caches, const void* node_k, const void* node_v, int kv_dtype,

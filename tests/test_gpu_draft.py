@@ -340,6 +340,39 @@ def test_tree_attention_qkv(dev, heads, window, dtype):
         assert rel_max(to_np(out), _ref(c, kv, draft, q, parents, sinks, window, pos)) < TOL
 
 
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("heads,n,kind,ctx", [((16, 2), 64, "tree", None), ((8, 8), 33, "chain", None),
+                                              ((3, 1), 1, "chain", None), ((64, 8), 40, "tree", 9000),
+                                              ((32, 2), 64, "tree", 70000), ((16, 16), 7, "roots", 70000)])
+def test_tree_attention_qkv_equals_rotated_rows(dev, dtype, heads, n, kind, ctx):
+    """From raw projections and from what it left of them (queries rotated on the host's orders, rows beside the
+    cache): the same bits, over positions around tiles and splits, in every kernel (the capacity chooses it)."""
+    from nurostream_amd.model.decode import DeviceKV, rope_kv_append, yarn_inv_freq
+    from nurostream_amd.model.draft import tree_attn, tree_attn_qkv
+    H, G = heads
+    for pos, window in ((0, 0), (1, 0), (31, 0), (32, 9), (33, 0), (127, 70), (128, 0), (500, 0), (500, 128), (1500, 0)):
+        c, kv, draft, _, sinks = _state(dev, H, G, n, pos, dtype, seed=pos, ctx=ctx)
+        inv, amp = yarn_inv_freq(c, dev)
+        g = torch.Generator().manual_seed(pos)
+        qkv = torch.randn(n, (H + 2 * G) * 64, generator=g).to(dev)
+        b = [torch.randn(m * 64, generator=g).to(dev) for m in (H, G, G)]
+        draft.k[0].fill_(float("nan")), draft.v[0].fill_(float("nan"))
+        parents = _parents(n, kind, seed=pos)
+        par = None if kind == "chain" else _ids(parents, dev)
+        out = tree_attn_qkv(qkv, *b, c, inv, amp, draft, 0, sinks, window, parents=par)
+        depth, _ = OD.lineage(parents)
+        one = DeviceKV(1, c, pos + 65, dev)
+        q = qkv.clone()
+        for i in range(n):
+            one.pos.fill_(pos + int(depth[i]))
+            rope_kv_append(q[i], *b, c, inv, amp, one, 0)
+            at = pos + int(depth[i])
+            assert torch.equal(draft.k[0][:, i], one.k[0][:, at].to(kv.dtype)), (pos, i)
+            assert torch.equal(draft.v[0][:, i], one.v[0][:, at].to(kv.dtype)), (pos, i)
+        again = tree_attn(q[:, :H * 64].contiguous(), c, draft, 0, sinks, window, parents=par)
+        assert torch.equal(out, again), pos
+
+
 def test_position_outside_the_cache_writes_nothing(dev):
     from nurostream_amd.model.decode import yarn_inv_freq
     from nurostream_amd.model.draft import commit, tree_attn, tree_attn_qkv
