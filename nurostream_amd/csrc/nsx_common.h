@@ -150,6 +150,9 @@ __device__ __forceinline__ uint32_t nsx_wave_max_u32(uint32_t v) {
   return mx(mx(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
             mx(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
 }
+// A workgroup's barrier behind LDS writes, with global loads left in flight (__syncthreads waits for those too).
+__device__ __forceinline__ void nsx_lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 __device__ __forceinline__ uint32_t nsx_wave_min_u32(uint32_t v) {
   auto mn = [](uint32_t a, uint32_t b) { return a < b ? a : b; };
   v = nsx_row_reduce_u32(v, mn);

@@ -228,10 +228,6 @@ __device__ __forceinline__ void value_terms(const typename Rows<KT>::V4 (&x)[8],
   }
 }
 
-__device__ __forceinline__ void lds_barrier() {  // LDS writes visible; global loads stay in flight
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-}
-
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028235e38f; }
 
 // Workgroup (kv head g, block cb of 16 NC query columns, split c of the keys). A column is a (node, query head of the
@@ -337,14 +333,14 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
   const int heads = ROPE ? a.n_head + 2 * a.n_kv : a.n_head;  // rows of a node in q
   float2* turn = (float2*)&lds[QBYTES];                       // amplitude times (cosine, sine)
   if constexpr (ROPE) {
-    lds_barrier();
+    nsx_lds_barrier();
     const int na = t1 > pt ? 0 : col0 / a.n_rep, nb = t1 > pt ? a.nodes : min(col0 + COLS - 1, ncol - 1) / a.n_rep + 1;
     for (int i = na * HALF + t; i < nb * HALF; i += NT) {
       float s, co;
       sincosf((float)(P + sdep[i / HALF]) * a.inv_freq[i % HALF], &s, &co);
       turn[i] = float2{co * a.amp, s * a.amp};
     }
-    lds_barrier();
+    nsx_lds_barrier();
     const int r0 = (nodes0 - pt) * TREE_KEYS, rows = min((t1 - pt) * TREE_KEYS, a.nodes) - r0;
     for (int i = t; i < rows * HALF; i += NT) {
       const int row = r0 + i / HALF, d = i % HALF;
@@ -395,7 +391,7 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
 #pragma unroll
     for (int k = 0; k < 3; ++k) *(v4u*)&lds[(k * COLS + cc) * QROW + (4 * j + gg) * 16] = tm[k];
   }
-  lds_barrier();
+  nsx_lds_barrier();
   const int q0 = i16 * QROW + kq * 16;
   auto query = [&](int k, int ct, int j) { return *(const v4u*)&lds[q0 + (k * COLS + 16 * ct) * QROW + 64 * j]; };
   // a column's node: what it sees of the nodes, its first visible row of the cache
@@ -605,7 +601,7 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
     }
   }
 
-  lds_barrier();  // (the sums take the query terms' place)
+  nsx_lds_barrier();  // (the sums take the query terms' place)
   float(*sacc)[COLS][OROW] = (float(*)[COLS][OROW])lds;
 #pragma unroll
   for (int ct = 0; ct < NC; ++ct) {
@@ -619,7 +615,7 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
     for (int r = 0; r < 4; ++r)
       *(v4f*)&sacc[wave][16 * ct + i16][16 * kq + 4 * r] = v4f{acc[ct][0][r], acc[ct][1][r], acc[ct][2][r], acc[ct][3][r]};
   }
-  lds_barrier();
+  nsx_lds_barrier();
   const bool whole = a.nsplit == 1;
   for (int i = t; i < min(COLS, ncol - col0) * ATTN_D; i += NT) {
     const int cc = i / ATTN_D, d = i % ATTN_D, col = col0 + cc;
@@ -797,7 +793,7 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
       split8(x, q[ct][j]);
     }
   }
-  lds_barrier();
+  nsx_lds_barrier();
   uint64_t vis[NC];
   int from[NC], deepest = 0;  // the columns' first visible cache rows, and the last of them
 #pragma unroll
@@ -880,7 +876,7 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
   };
   auto phase = [] {
     __builtin_amdgcn_sched_barrier(0);
-    lds_barrier();
+    nsx_lds_barrier();
     __builtin_amdgcn_sched_barrier(0);
   };
 
@@ -1051,7 +1047,7 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
     l[ct] += __shfl_xor(l[ct], 32, 64);
   }
   float(*so)[16 * NC][OROW] = (float(*)[16 * NC][OROW])lds;
-  lds_barrier();
+  nsx_lds_barrier();
   if (group) {
 #pragma unroll
     for (int ct = 0; ct < NC; ++ct) {
@@ -1064,7 +1060,7 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
               v4f{acc[ct][2 * h][2 * u], acc[ct][2 * h + 1][2 * u], acc[ct][2 * h][2 * u + 1], acc[ct][2 * h + 1][2 * u + 1]};
     }
   }
-  lds_barrier();
+  nsx_lds_barrier();
   if (group) return;
   const bool whole = a.nsplit == 1;
 #pragma unroll

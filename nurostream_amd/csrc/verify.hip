@@ -12,14 +12,14 @@
 // at which the running sum of the weights exceeds node 0's random number times their total. Temperature 0: p is one
 // at the largest logit, the lowest index of equals.
 //
-// Sums and comparisons in 64 bits, weights to 2^-35 of themselves: a vocabulary's running sum is compared with a random
+// Sums and comparisons in 64 bits, weights to 2^-39 of themselves: a vocabulary's running sum is compared with a random
 // number, and with 32-bit weights the answer would be another one in about one draw of a million. A NaN logit counts
 // as -infinity; of +infinity in a row, its tokens share the row's whole weight; a row without any weight gives the
-// token -1. Sequences with no nodes (length 0) give count 0 and token -1.
+// token -1. Sequences with no nodes (length 0) give count 0 and token -1, and rows behind a length are not read.
 //
-// Launches: the rows' chunk sums (all logits once: the bytes, 5 TB/s, and some 11 64-bit operations per logit bound
-// it), the walk with the draw of one workgroup per sequence, and only for drafts from q, whose residual needs the last
-// row's whole sum first, that row's chunk sums of max(p - q, 0) and the draw from them.
+// Two launches. The rows' chunk sums read all logits once: 32 rows of 201088 fp32 logits 11 us, of which the bytes (2.3
+// TB/s with the launch; 8 us without weights) and then some 16 64-bit operations per logit; 120 rows of 151936 in bf16 14.
+// The walk with the draw is five dependent round trips to memory: 10 us, 3.5 where nothing is drawn (temperature 0).
 #include "nsx_common.h"
 
 #include <algorithm>
@@ -31,6 +31,7 @@ namespace {
 constexpr int VF_CHUNK = 4096;       // logits per workgroup of the row passes
 constexpr int VF_THREADS = 256;      // of the row passes
 constexpr int VF_WALK = 1024;        // of the walk and the draw
+constexpr int VF_WALK_Q = 512;       // of the same, a workgroup per chunk
 constexpr int VF_MAX_CHUNKS = 1024;
 constexpr int VF_VEC = 8;            // chunks begin where the row's address is a multiple of this many elements
 
@@ -39,12 +40,6 @@ struct Part {
   float m;
   int32_t at;
   double s;
-};
-// The node that the draw is from (-1: nothing left to draw), its row's largest logit and sum.
-struct Last {
-  int32_t node;
-  float M;
-  double Z;
 };
 
 struct VerifyArgs {
@@ -56,11 +51,12 @@ struct VerifyArgs {
   int64_t parents_stride;  // 0: one tree for all sequences
   const float *u, *q;
   double scale2;  // log2(e) / temperature; 0: greedy
+  double least;   // -1000 / scale2
   int32_t *count, *path, *token;
   int nchunk;
   Part* part;     // [B * n][nchunk]
-  double* resid;  // q: [B][nchunk], the sums of max(p - q, 0) at the last node
-  Last* last;     // q: [B]
+  double* resid;    // q: [B][nchunk], the sums of max(p - q, 0) at the last node
+  uint32_t* ticket;  // q: [B], how many of a sequence's workgroups have written theirs
 };
 
 template <typename LT>  // float, _Float16, or uint16_t for bf16
@@ -95,32 +91,33 @@ struct Row {
   }
 };
 
-// 2^(j / 16) in LDS: sixteen entries on banks of their own.
+// 2^(j / 32) in LDS: 32 entries, one on each pair of the 64 banks.
 struct Pow2 {
-  double t[16];
+  double t[32];
   __device__ __forceinline__ void fill() {
-    if (threadIdx.x < 16) t[threadIdx.x] = exp2((double)threadIdx.x / 16);
+    if (threadIdx.x < 32) t[threadIdx.x] = exp2((double)threadIdx.x / 32);
   }
 };
 
-// The weight 2^(scale2 (x - M)) of logit x beside the largest, M > -infinity. y = n + j / 16 + r with |r| <= 1 / 32 by
-// adding 1.5 * 2^48; 2^r - 1 = r ln2 + r^2 (..), the last part (below 2.4e-4) in 32 bits: an error of 2^-35. Below
-// 2^-1020 it is zero.
-__device__ __forceinline__ double vf_weight_finite(float x, float M, double scale2, const Pow2& tab) {
-  const double y = ((double)x - (double)M) * scale2;
-  const double t = y + 0x1.8p48;
-  const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
-  const double r = y - (t - 0x1.8p48);
-  const float f = (float)r;
-  // ln2^2 / 2, ln2^3 / 6, ln2^4 / 24, ln2^5 / 120
-  const float q = f * f * fmaf(f, fmaf(f, fmaf(f, 0.0013333558f, 0.0096181291f), 0.055504109f), 0.24022651f);
-  const double c = tab.t[k & 15], w = fma(fma(r, 0.69314718055994530942, (double)q), c, c);
-  const uint64_t bits = __builtin_bit_cast(uint64_t, w) + ((uint64_t)(uint32_t)(k >> 4) << 52);
-  return y < -1020.0 ? 0.0 : __builtin_bit_cast(double, bits);
+// The weight 2^(scale2 (x - M)) of logit x beside the largest, M > -infinity. The exponent is n + j / 32 + r with
+// |r| <= 1 / 64 by adding 1.5 * 2^47; 2^r - 1 = r (ln2 + ..) to the fourth power of r: an error of 2^-39. No weight is
+// below 2^-1000, `least` being the least difference: beside the largest one's 1 that is nothing.
+__device__ __forceinline__ double vf_weight_finite(float x, float M, const VerifyArgs& a, const Pow2& tab) {
+  const double d = fmax((double)x - (double)M, a.least);
+  const double t = fma(d, a.scale2, 0x1.8p47);
+  const uint32_t k = (uint32_t)__builtin_bit_cast(uint64_t, t);
+  const double r = fma(d, a.scale2, -(t - 0x1.8p47));
+  // ln2, ln2^2 / 2, ln2^3 / 6, ln2^4 / 24
+  const double h = fma(r, fma(r, fma(r, 0.0096181291076284772, 0.055504108664821580), 0.24022650695910071), 0.69314718055994531);
+  const double c = tab.t[k & 31], w = fma(r * h, c, c);
+  const uint64_t bits = __builtin_bit_cast(uint64_t, w) + ((uint64_t)(k >> 5) << 52);
+  return __builtin_bit_cast(double, bits);
 }
-__device__ __forceinline__ double vf_weight(float x, float M, double scale2, const Pow2& tab) {
+// With zero for what is below 2^-1000, and for M = +infinity.
+__device__ __forceinline__ double vf_weight(float x, float M, const VerifyArgs& a, const Pow2& tab) {
   if (M == INFINITY) return x == M ? 1.0 : 0.0;
-  return vf_weight_finite(x, M, scale2, tab);
+  const double w = vf_weight_finite(x, M, a, tab);
+  return (double)x - (double)M < a.least ? 0.0 : w;
 }
 
 // Wave-wide operations on DPP moves and readlanes: no trip through LDS.
@@ -172,11 +169,15 @@ __device__ __forceinline__ int vf_block_min(int v, int* red) {  // of values >= 
   __syncthreads();
   return min(min(red[0], red[1]), min(red[2], red[3]));
 }
+template <int NW = 4>
 __device__ __forceinline__ double vf_block_sum(double v, double* red) {
   v = vf_wave_sum(v);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  return (red[0] + red[1]) + (red[2] + red[3]);
+  v = red[0];
+#pragma unroll
+  for (int k = 1; k < NW; ++k) v += red[k];
+  return v;
 }
 
 template <typename LT, bool GREEDY>
@@ -188,6 +189,8 @@ __global__ __launch_bounds__(VF_THREADS) void verify_stats_kernel(VerifyArgs a) 
   __shared__ Pow2 tab;
   const int64_t row = blockIdx.y;
   const int c = blockIdx.x, t = threadIdx.x;
+  if (a.ticket && row % a.n == 0 && c == 0 && t == 0) a.ticket[row / a.n] = 0;
+  if (a.lengths && row % a.n >= a.lengths[row / a.n]) return;
   const Row<LT> r(a, row);
   float x[RUNS][W], m = -INFINITY;
 #pragma unroll
@@ -217,18 +220,20 @@ __global__ __launch_bounds__(VF_THREADS) void verify_stats_kernel(VerifyArgs a) 
 #pragma unroll
       for (int u = 0; u < RUNS; ++u)
 #pragma unroll
-        for (int k = 0; k < W; ++k) s += vf_weight_finite(x[u][k], m, a.scale2, tab);
+        for (int k = 0; k < W; ++k) s += vf_weight_finite(x[u][k], m, a, tab);
     }
     s = vf_block_sum(s, redd);
   }
   if (t == 0) a.part[row * a.nchunk + c] = Part{m, at, s};
 }
 
+// A lane's first chunk of a row (with most vocabularies its only one).
+__device__ __forceinline__ Part vf_part(const VerifyArgs& a, int64_t row, int lane) {
+  return lane < a.nchunk ? a.part[row * a.nchunk + lane] : Part{-INFINITY, 0x7fffffff, 0.0};
+}
 // The row's largest logit, its index and the weights' sum, from its chunks: one wave.
-__device__ __forceinline__ Part vf_row(const VerifyArgs& a, int64_t row, int lane, const Pow2& tab) {
+__device__ __forceinline__ Part vf_row(const VerifyArgs& a, int64_t row, int lane, const Part& p0, const Pow2& tab) {
   const Part* p = a.part + row * a.nchunk;
-  const Part none{-INFINITY, 0x7fffffff, 0.0};
-  const Part p0 = lane < a.nchunk ? p[lane] : none;  // (most vocabularies: the only ones)
   float mx = p0.m;
   int at = p0.at;
   for (int c = lane + 64; c < a.nchunk; c += 64)
@@ -237,25 +242,26 @@ __device__ __forceinline__ Part vf_row(const VerifyArgs& a, int64_t row, int lan
   if (a.scale2 == 0.0) return Part{M, (int)nsx_wave_min_u32(mx == M ? (uint32_t)at : 0x7fffffffu), 0.0};
   double s = 0.0;
   if (M > -INFINITY) {
-    if (p0.m > -INFINITY) s = p0.s * vf_weight(p0.m, M, a.scale2, tab);
+    if (p0.m > -INFINITY) s = p0.s * vf_weight(p0.m, M, a, tab);
     for (int c = lane + 64; c < a.nchunk; c += 64)
-      if (p[c].m > -INFINITY) s += p[c].s * vf_weight(p[c].m, M, a.scale2, tab);
+      if (p[c].m > -INFINITY) s += p[c].s * vf_weight(p[c].m, M, a, tab);
   }
   return Part{M, 0, vf_wave_sum(s)};
 }
 
+template <int T>
 struct PickLds {
   double sums[VF_MAX_CHUNKS + 1];  // the chunks' sums
-  double wave[VF_WALK / 64];
+  double wave[T / 64];
   double before, target;
   int chunk, at, last;
 };
 
 // The first token whose running sum exceeds u times the total, from the chunks' sums; weight(i, load(i)): token i's. -1:
 // no sum is above zero. (A sum that is only rounding, all its chunk's tokens refused, is struck out and the draw made again.)
-template <typename L, typename F>
-__device__ int vf_pick(const VerifyArgs& a, PickLds& s, double u, int off, L load, F weight) {
-  constexpr int PER = VF_CHUNK / VF_WALK;
+template <int T, typename L, typename F>
+__device__ int vf_pick(const VerifyArgs& a, PickLds<T>& s, double u, int off, L load, F weight) {
+  constexpr int PER = VF_CHUNK / T;
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
   for (;;) {
     __syncthreads();
@@ -325,16 +331,41 @@ __device__ int vf_pick(const VerifyArgs& a, PickLds& s, double u, int off, L loa
   }
 }
 
-// One workgroup per sequence: the rows' statistics, the walk and, unless a q is to be taken off, the draw.
+// max(p - q, 0) at the last node.
 template <typename LT>
-__global__ __launch_bounds__(VF_WALK) void verify_walk_kernel(VerifyArgs a) {
+struct Resid {
+  const VerifyArgs& a;
+  const Row<LT> row;
+  const float* q;
+  const float M;
+  const double inv_z;
+  struct Raw {
+    float x, q;
+  };
+  __device__ __forceinline__ Resid(const VerifyArgs& a, int b, int node, float M, double Z)
+      : a(a), row(a, (int64_t)b * a.n + node), q(a.q + ((int64_t)b * (a.n - 1) + node) * a.V), M(M), inv_z(1.0 / Z) {}
+  __device__ __forceinline__ Raw load(int64_t i) const { return Raw{row.at(i), q[i]}; }
+  __device__ __forceinline__ double weight(const Raw& r, const Pow2& tab) const {
+    return fmax(vf_weight(r.x, M, a, tab) * inv_z - (double)r.q, 0.0);
+  }
+};
+
+// The rows' statistics, the walk and the draw: one workgroup per sequence. With q there is one per chunk and sequence, as
+// a draw from max(p - q, 0) needs all of that row's sums: each makes the same walk, the first alone writes it, and each
+// sums its chunk, the last to do so drawing. (The walks are made side by side, where a launch each for the residual's sums
+// and their draw came one after the other: 24 sequences of 5 rows of 151936 bf16 logits 42 us in four launches, 28 in two.
+// 512 threads: with 1024 31 us, and a workgroup of 256 spills.)
+template <typename LT, bool Q, int T>
+__global__ __launch_bounds__(T) void verify_walk_kernel(VerifyArgs a) {
   __shared__ float sM[64];
   __shared__ int sat[64], sref[64];
   __shared__ double sZ[64], swref[64];
-  __shared__ PickLds pick;
+  __shared__ PickLds<T> pick;
   __shared__ Pow2 tab;
-  __shared__ int s_node, s_nref;
-  const int b = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6, n = a.n;
+  __shared__ int s_node, s_nref, s_last;
+  const int c = Q ? blockIdx.x : 0, b = Q ? blockIdx.y : blockIdx.x;
+  const bool first = c == 0;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, n = a.n;
   const int len = a.lengths ? min(a.lengths[b], n) : n;
   const double u0 = a.u ? a.u[(int64_t)b * n] : 0.f;
   // the nodes' own loads ahead of the rows' sums
@@ -347,22 +378,30 @@ __global__ __launch_bounds__(VF_WALK) void verify_walk_kernel(VerifyArgs a) {
     if (par >= 0 && tok >= 0 && tok < a.V && a.scale2 != 0.0) {
       u = a.u[(int64_t)b * n + lane];
       x = Row<LT>(a, (int64_t)b * n + par).at(tok);
-      if (a.q) q = a.q[((int64_t)b * (n - 1) + par) * a.V + tok];
+      if (Q) q = a.q[((int64_t)b * (n - 1) + par) * a.V + tok];
     }
   }
+  constexpr int AHEAD = 4, NW = T / 64;  // the rows' chunks too, of a wave's first rows
+  Part ahead[AHEAD];
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k)
+    if (wave + k * NW < len) ahead[k] = vf_part(a, (int64_t)b * n + wave + k * NW, lane);
   tab.fill();
-  __syncthreads();
-  for (int r = wave; r < n; r += VF_WALK / 64) {
-    const Part p = vf_row(a, (int64_t)b * n + r, lane, tab);
+  nsx_lds_barrier();
+  auto row_of = [&](int r, const Part& p0) {
+    const Part p = vf_row(a, (int64_t)b * n + r, lane, p0, tab);
     if (lane == 0) sM[r] = p.m, sat[r] = p.at, sZ[r] = p.s;
-  }
+  };
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k)
+    if (wave + k * NW < len) row_of(wave + k * NW, ahead[k]);
+  for (int r = wave + AHEAD * NW; r < len; r += NW) row_of(r, vf_part(a, (int64_t)b * n + r, lane));
   __syncthreads();
   if (len <= 0) {
-    if (t < n) a.path[(int64_t)b * n + t] = -1;
-    if (t == 0) {
+    if (first && t < n) a.path[(int64_t)b * n + t] = -1;
+    if (first && t == 0) {
       a.count[b] = 0;
       a.token[b] = -1;
-      if (a.last) a.last[b].node = -1;
     }
     return;
   }
@@ -372,7 +411,7 @@ __global__ __launch_bounds__(VF_WALK) void verify_walk_kernel(VerifyArgs a) {
       if (a.scale2 == 0.0) {
         p = sat[par] == tok ? 1.0 : 0.0;
       } else {
-        w = vf_weight(x, sM[par], a.scale2, tab);
+        w = vf_weight(x, sM[par], a, tab);
         p = w / sZ[par];
       }
     }
@@ -401,15 +440,15 @@ __global__ __launch_bounds__(VF_WALK) void verify_walk_kernel(VerifyArgs a) {
       }
     }
     const int slot = __popcll(taken & ((1ull << lane) - 1));
-    if (lane < n && (taken >> lane & 1)) a.path[(int64_t)b * n + slot] = lane;
-    if (lane < n && lane >= got) a.path[(int64_t)b * n + lane] = -1;
+    if (first && lane < n && (taken >> lane & 1)) a.path[(int64_t)b * n + slot] = lane;
+    if (first && lane < n && lane >= got) a.path[(int64_t)b * n + lane] = -1;
     if (refused >> lane & 1) {
       const int k = __popcll(refused & ((1ull << lane) - 1));
       sref[k] = tok;
       swref[k] = again >> lane & 1 ? 0.0 : w;  // (zero too where the token is no token)
     }
     if (lane == 0) {
-      a.count[b] = got;
+      if (first) a.count[b] = got;
       s_node = cur;
       s_nref = __popcll(refused);
     }
@@ -418,98 +457,60 @@ __global__ __launch_bounds__(VF_WALK) void verify_walk_kernel(VerifyArgs a) {
   const int node = s_node, nref = s_nref;
   const float M = sM[node];
   if (!(M > -INFINITY) || a.scale2 == 0.0) {
-    if (t == 0) {
-      a.token[b] = M > -INFINITY ? sat[node] : -1;
-      if (a.last) a.last[b].node = -1;
-    }
+    if (first && t == 0) a.token[b] = M > -INFINITY ? sat[node] : -1;
     return;
   }
-  if (a.last && t == 0) a.last[b] = Last{nref ? node : -1, M, sZ[node]};
-  if (a.q && nref) return;
-  // the chunks' sums, without the refused tokens
-  const Row<LT> row(a, (int64_t)b * n + node);
   const Part* pr = a.part + ((int64_t)b * n + node) * a.nchunk;
-  for (int c = t; c < a.nchunk; c += VF_WALK) {
-    double s = pr[c].m > -INFINITY ? pr[c].s * vf_weight(pr[c].m, M, a.scale2, tab) : 0.0;
-    for (int r = 0; r < nref; ++r)
-      if (swref[r] > 0.0 && (sref[r] + row.off) / VF_CHUNK == c) s -= swref[r];
-    pick.sums[c] = fmax(s, 0.0);
-  }
-  const int got = vf_pick(a, pick, u0, row.off, [&](int64_t i) { return row.at(i); }, [&](int64_t i, float x) {
-    double w = vf_weight(x, M, a.scale2, tab);
-    for (int r = 0; r < nref; ++r) w = sref[r] == i ? 0.0 : w;
-    return w;
-  });
-  if (t == 0) a.token[b] = got;
-}
-
-// max(p - q, 0) at the last node.
-template <typename LT>
-struct Resid {
-  const Row<LT> row;
-  const float* q;
-  const Last z;
-  const double scale2, inv_z;
-  struct Raw {
-    float x, q;
-  };
-  __device__ __forceinline__ Resid(const VerifyArgs& a, int b, const Last& z)
-      : row(a, (int64_t)b * a.n + z.node), q(a.q + ((int64_t)b * (a.n - 1) + z.node) * a.V), z(z), scale2(a.scale2),
-        inv_z(1.0 / z.Z) {}
-  __device__ __forceinline__ Raw load(int64_t i) const { return Raw{row.at(i), q[i]}; }
-  __device__ __forceinline__ double weight(const Raw& r, const Pow2& tab) const {
-    return fmax(vf_weight(r.x, z.M, scale2, tab) * inv_z - (double)r.q, 0.0);
-  }
-};
-
-// q: chunk sums of max(p - q, 0) at the last node, where a child was refused.
-template <typename LT>
-__global__ __launch_bounds__(VF_THREADS) void verify_resid_kernel(VerifyArgs a) {
-  constexpr int PER = VF_CHUNK / VF_THREADS;
-  __shared__ double redd[4];
-  __shared__ Pow2 tab;
-  const int b = blockIdx.y, c = blockIdx.x;
-  const Last z = a.last[b];
-  if (z.node < 0) return;
-  tab.fill();
-  __syncthreads();
-  const Resid<LT> r(a, b, z);
-  typename Resid<LT>::Raw raw[PER];
-  const int64_t i0 = (int64_t)c * VF_CHUNK + threadIdx.x - r.row.off;
+  const bool residual = Q && nref;
+  int got = -1;
+  if constexpr (Q) {
+    if (residual) {
+      constexpr int PER = VF_CHUNK / T;
+      const Resid<LT> r(a, b, node, M, sZ[node]);
+      typename Resid<LT>::Raw raw[PER];
+      const int64_t i0 = (int64_t)c * VF_CHUNK + t - r.row.off;
 #pragma unroll
-  for (int k = 0; k < PER; ++k) raw[k] = r.load(min(max(i0 + VF_THREADS * k, (int64_t)0), a.V - 1));
-  double s = 0.0;
+      for (int k = 0; k < PER; ++k) raw[k] = r.load(min(max(i0 + T * k, (int64_t)0), a.V - 1));
+      double s = 0.0;
 #pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const int64_t i = i0 + VF_THREADS * k;
-    const double w = r.weight(raw[k], tab);
-    s += i >= 0 && i < a.V ? w : 0.0;
-  }
-  s = vf_block_sum(s, redd);
-  if (threadIdx.x == 0) a.resid[(int64_t)b * a.nchunk + c] = s;
-}
-
-template <typename LT>
-__global__ __launch_bounds__(VF_WALK) void verify_draw_kernel(VerifyArgs a) {
-  __shared__ PickLds pick;
-  __shared__ Pow2 tab;
-  const int b = blockIdx.x;
-  const Last z = a.last[b];
-  if (z.node < 0) return;
-  tab.fill();
-  const double u = a.u[(int64_t)b * a.n];
-  const Resid<LT> r(a, b, z);
-  for (int c = threadIdx.x; c < a.nchunk; c += VF_WALK) pick.sums[c] = a.resid[(int64_t)b * a.nchunk + c];
-  int got = vf_pick(a, pick, u, r.row.off, [&](int64_t i) { return r.load(i); },
+      for (int k = 0; k < PER; ++k) {
+        const int64_t i = i0 + T * k;
+        const double w = r.weight(raw[k], tab);
+        s += i >= 0 && i < a.V ? w : 0.0;
+      }
+      s = vf_block_sum<T / 64>(s, pick.wave);
+      double* sums = a.resid + (int64_t)b * a.nchunk;
+      if (t == 0) {  // the sum first, then the count, as every workgroup on the device sees them
+        __hip_atomic_store(sums + c, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        s_last = __hip_atomic_fetch_add(a.ticket + b, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == a.nchunk - 1u;
+      }
+      __syncthreads();
+      if (!s_last) return;
+      for (int k = t; k < a.nchunk; k += T)
+        pick.sums[k] = __hip_atomic_load(sums + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      got = vf_pick(a, pick, u0, r.row.off, [&](int64_t i) { return r.load(i); },
                     [&](int64_t, const typename Resid<LT>::Raw& x) { return r.weight(x, tab); });
-  if (got < 0) {  // p nowhere above q (to rounding): drawn from p
-    const Part* pr = a.part + ((int64_t)b * a.n + z.node) * a.nchunk;
-    for (int c = threadIdx.x; c < a.nchunk; c += VF_WALK)
-      pick.sums[c] = pr[c].m > -INFINITY ? pr[c].s * vf_weight(pr[c].m, z.M, a.scale2, tab) : 0.0;
-    got = vf_pick(a, pick, u, r.row.off, [&](int64_t i) { return r.row.at(i); },
-                  [&](int64_t, float x) { return vf_weight(x, z.M, a.scale2, tab); });
+    } else if (!first) {
+      return;
+    }
   }
-  if (threadIdx.x == 0) a.token[b] = got;
+  if (got < 0) {  // (from the residual: p is nowhere above q, to rounding, and the draw is from p)
+    // the chunks' sums, without the refused tokens
+    const int out = residual ? 0 : nref;
+    const Row<LT> row(a, (int64_t)b * n + node);
+    for (int k = t; k < a.nchunk; k += T) {
+      double s = pr[k].m > -INFINITY ? pr[k].s * vf_weight(pr[k].m, M, a, tab) : 0.0;
+      for (int r = 0; r < out; ++r)
+        if (swref[r] > 0.0 && (sref[r] + row.off) / VF_CHUNK == k) s -= swref[r];
+      pick.sums[k] = fmax(s, 0.0);
+    }
+    got = vf_pick(a, pick, u0, row.off, [&](int64_t i) { return row.at(i); }, [&](int64_t i, float x) {
+      double w = vf_weight(x, M, a, tab);
+      for (int r = 0; r < out; ++r) w = sref[r] == i ? 0.0 : w;
+      return w;
+    });
+  }
+  if (t == 0) a.token[b] = got;
 }
 
 int64_t up16(int64_t v) { return (v + 15) & ~15ll; }
@@ -521,14 +522,9 @@ int verify_launch(const VerifyArgs& a, hipStream_t st) {
   if (a.scale2 == 0.0) hipLaunchKernelGGL((verify_stats_kernel<LT, true>), rows, dim3(VF_THREADS), 0, st, a);
   else hipLaunchKernelGGL((verify_stats_kernel<LT, false>), rows, dim3(VF_THREADS), 0, st, a);
   NSX_LAUNCHED();
-  hipLaunchKernelGGL(verify_walk_kernel<LT>, dim3(a.B), dim3(VF_WALK), 0, st, a);
+  if (a.q) hipLaunchKernelGGL((verify_walk_kernel<LT, true, VF_WALK_Q>), seqs, dim3(VF_WALK_Q), 0, st, a);
+  else hipLaunchKernelGGL((verify_walk_kernel<LT, false, VF_WALK>), dim3(a.B), dim3(VF_WALK), 0, st, a);
   NSX_LAUNCHED();
-  if (a.q) {
-    hipLaunchKernelGGL(verify_resid_kernel<LT>, seqs, dim3(VF_THREADS), 0, st, a);
-    NSX_LAUNCHED();
-    hipLaunchKernelGGL(verify_draw_kernel<LT>, dim3(a.B), dim3(VF_WALK), 0, st, a);
-    NSX_LAUNCHED();
-  }
   return NSX_OK;
 }
 
@@ -537,7 +533,7 @@ int verify_launch(const VerifyArgs& a, hipStream_t st) {
 extern "C" int64_t nsx_verify_workspace_bytes(int64_t batch, int n_nodes, int64_t vocab) {
   if (batch <= 0 || n_nodes <= 0 || vocab <= 0) return -1;
   return batch * n_nodes * chunks(vocab) * (int64_t)sizeof(Part) + up16(batch * chunks(vocab) * 8) +
-         batch * (int64_t)sizeof(Last);
+         batch * (int64_t)sizeof(uint32_t);
 }
 
 extern "C" int nsx_verify(const void* logits, int logits_dtype, int64_t row_stride, int64_t batch, int n_nodes,
@@ -573,9 +569,10 @@ extern "C" int nsx_verify(const void* logits, int logits_dtype, int64_t row_stri
   w += batch * n_nodes * nchunk * (int64_t)sizeof(Part);
   double* resid = (double*)w;
   w += up16(batch * nchunk * 8);
+  const double scale2 = temperature > 0.0 ? 1.44269504088896340736 / temperature : 0.0;
   const VerifyArgs a{logits, row_stride, (int)batch, n_nodes, vocab, tokens, parents, lengths, parents_stride, uniforms,
-                     residual ? draft_probs : nullptr, temperature > 0.0 ? 1.44269504088896340736 / temperature : 0.0,
-                     count, path, token, nchunk, part, resid, residual ? (Last*)w : nullptr};
+                     residual ? draft_probs : nullptr, scale2, scale2 > 0.0 ? -1000.0 / scale2 : 0.0,
+                     count, path, token, nchunk, part, resid, residual ? (uint32_t*)w : nullptr};
   hipStream_t st = (hipStream_t)stream;
   if (logits_dtype == NSX_DT_F32) return verify_launch<float>(a, st);
   if (logits_dtype == NSX_DT_F16) return verify_launch<_Float16>(a, st);

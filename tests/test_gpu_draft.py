@@ -501,6 +501,75 @@ def test_verify_lengths(dev):
         _check_verify(dev, logits, tokens, parents, u, probs, T, lengths=[5, 0, 1, 3, 9, -2], par=None)
 
 
+def test_verify_reads_no_row_behind_a_length(dev):
+    """Rows, probabilities and uniforms behind the lengths hold NaN: the same answers as with numbers there."""
+    from nurostream_amd.model.draft import verify
+    lengths = [5, 0, 1, 3, 9, -2]
+    for q, T in ((False, 0.0), (False, 0.8), (True, 0.8)):
+        logits, tokens, _, u, probs = _verify_case(5, 6, 5, 9001, "chain", q, "f32", T, dev)
+        i32 = lambda a: torch.as_tensor(np.asarray(a), dtype=torch.int32, device=dev)  # noqa: E731
+        run = lambda: verify(logits.to(dev), i32(tokens), torch.from_numpy(u).to(dev), temperature=T,  # noqa: E731
+                             lengths=i32(lengths), draft_probs=None if probs is None else torch.from_numpy(probs).to(dev))
+        want = run()
+        for b, k in enumerate(lengths):
+            k = max(0, min(k, 5))
+            logits[b, k:], u[b, max(k, 1):] = math.nan, math.nan
+            if probs is not None:
+                probs[b, max(k - 1, 0):] = math.nan
+        assert all(torch.equal(x, y) for x, y in zip(run(), want))
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_verify_residuals_captured(dev, dtype):
+    """Drafts that q made too likely, refused over many chunks and sequences at once: each replay of a captured call,
+    with eager calls between, gives the oracle's answers."""
+    from nurostream_amd.model.draft import verify
+    B, n, V, T = 9, 4, 50021, 0.9
+    cases = [_verify_case(40 + i, B, n, V, "chain", True, dtype, T, dev) for i in range(3)]
+    for logits, tokens, _, u, probs in cases:
+        for b in range(B):
+            for i in range(n - 1):  # q at the draft ten times what p has there
+                if (b + i) % 2:
+                    row = OD.target_probs(logits[b, i].double().numpy(), T)
+                    probs[b, i, tokens[b, i + 1]] = 10 * row[tokens[b, i + 1]] + 0.01
+                    u[b, i + 1] = 0.5
+    dev_of = lambda c: [c[0].to(dev), torch.from_numpy(c[1]).to(torch.int32).to(dev),  # noqa: E731
+                        torch.from_numpy(c[3]).to(dev), torch.from_numpy(c[4]).to(dev)]
+    bufs = dev_of(cases[0])
+    call = lambda x: verify(x[0], x[1], x[2], draft_probs=x[3], temperature=T)  # noqa: E731
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        call(bufs)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        got = call(bufs)
+    refused = 0
+    for i in (1, 2, 0, 1):
+        for a, b in zip(bufs, dev_of(cases[i])):
+            a.copy_(b)
+        graph.replay()
+        eager = call(bufs)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, eager)), i
+        logits, tokens, parents, u, probs = cases[i]
+        for b in range(B):
+            path, t = OD.verify_one(logits[b].double().numpy(), tokens[b], parents, u[b], T, probs[b])
+            assert (int(got[0][b]), got[1][b].tolist(), int(got[2][b])) == (len(path), path + [-1] * (n - len(path)), t), b
+            refused += len(path) < n
+    assert refused >= 12
+
+
+def test_verify_nothing_left_of_p(dev):
+    """q twice p everywhere: what is refused leaves no residual, and the token is drawn from p."""
+    V, T = 9001, 1.0
+    logits, tokens, parents, u, _ = _verify_case(8, 3, 2, V, "chain", False, "f32", T, dev)
+    probs = np.stack([[OD.target_probs(logits[b, 0].double().numpy(), T) * 2] for b in range(3)]).astype(np.float32)
+    u[:, 1] = 0.75
+    _check_verify(dev, logits, tokens, parents, u, probs, T, par=None)
+
+
 def test_verify_refused_and_repeated_siblings(dev):
     """Uniforms near one refuse every child; the same token twice under a node, tokens outside the vocabulary, and a
     row whose mass the drafts hold between them."""
