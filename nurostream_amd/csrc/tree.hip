@@ -8,7 +8,8 @@
 // The nodes' key and value rows live beside the cache ([n_kv][max_nodes][64], the cache's type), so that refused
 // drafts never touch it; tree_commit_kernel moves the accepted ones in.
 //
-// Cache and node rows: fp32, fp16 or bf16; queries, sums and outputs fp32.
+// Cache and node rows: fp32, fp16 or bf16; queries, sums and outputs fp32. A call is one launch where a kv head's keys are
+// one split, with the merge of the splits two.
 #include "nsx_common.h"
 #include "rope.h"
 
@@ -52,15 +53,13 @@ struct Tiles {
   }
 };
 
-// Lane i's node: its ancestors and itself as bits, from the parent list, each round doubling the path's length.
-// Every lane of the wave takes part; lanes past `nodes` hold only their own bit.
-__device__ __forceinline__ uint64_t tree_lineage(const int32_t* __restrict__ parents, int nodes, int lane) {
-  int up = -1;
-  if (lane < nodes) {
-    up = parents ? parents[lane] : lane - 1;
-    if (up >= lane) up = -1;
-  }
-  up = up < 0 ? -1 : up;
+// Lane i's node: its ancestors and itself as bits, from the nodes' parents (-1 in lanes past the last node, which hold only
+// their own bit), each round doubling the path's length. Every lane of the wave takes part.
+__device__ __forceinline__ int tree_parent(const int32_t* __restrict__ parents, int nodes, int lane) {
+  return lane >= nodes ? -1 : parents ? parents[lane] : lane - 1;
+}
+__device__ __forceinline__ uint64_t tree_lineage(int up, int lane) {
+  up = up < 0 || up >= lane ? -1 : up;
   uint64_t bits = 1ull << lane;
 #pragma unroll
   for (int r = 0; r < 6; ++r) {
@@ -87,38 +86,6 @@ __device__ __forceinline__ void store_kv(void* p, int64_t i, float v) {
 struct Bf16 {
   uint16_t bits;
 };
-
-// One wave per row of the nodes' q | k | v blocks: bias, rotary at the node's position for q and k; q rows into
-// q_out, k and v rows beside the cache.
-template <typename KT>
-__global__ __launch_bounds__(256) void tree_rope_kernel(const float* __restrict__ qkv, const float* __restrict__ bq,
-                                                        const float* __restrict__ bk, const float* __restrict__ bv,
-                                                        const float* __restrict__ inv_freq, float amp, int n_head,
-                                                        int n_kv, const int32_t* __restrict__ parents,
-                                                        const int32_t* __restrict__ pos_ptr, int64_t ctx_max,
-                                                        int nodes, int max_nodes, float* __restrict__ q_out,
-                                                        void* __restrict__ dk, void* __restrict__ dv) {
-  const int lane = threadIdx.x & 63, rows = n_head + 2 * n_kv;
-  const int w = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (w >= nodes * rows) return;
-  const int node = w / rows, r = w % rows;
-  const int p = *pos_ptr;
-  const uint64_t line = tree_lineage(parents, nodes, lane);
-  if (p < 0 || p > ctx_max) return;
-  const uint64_t mine = (uint64_t)__shfl((uint32_t)(line >> 32), node, 64) << 32 | __shfl((uint32_t)line, node, 64);
-  const int at = p + __popcll(mine) - 1;
-  float x = qkv[((int64_t)node * rows + r) * ATTN_D + lane];
-  const float* b = r < n_head ? bq : r < n_head + n_kv ? bk : bv;
-  const int rb = r < n_head ? r : r < n_head + n_kv ? r - n_head : r - n_head - n_kv;
-  if (b) x += b[rb * ATTN_D + lane];
-  if (r >= n_head + n_kv) {
-    store_kv<KT>(dv, ((int64_t)rb * max_nodes + node) * ATTN_D + lane, x);
-    return;
-  }
-  const float y = rope_elem(x, __shfl_xor(x, ATTN_D / 2, 64), lane, at, inv_freq, amp);
-  if (r < n_head) q_out[((int64_t)node * n_head + r) * ATTN_D + lane] = y;
-  else store_kv<KT>(dk, ((int64_t)rb * max_nodes + node) * ATTN_D + lane, y);
-}
 
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ b8 as_b8(v4u x) { return __builtin_bit_cast(b8, x); }
@@ -228,6 +195,63 @@ __device__ __forceinline__ void value_terms(const typename Rows<KT>::V4 (&x)[8],
   }
 }
 
+// The sines and cosines of nodes na .. nb - 1, times the amplitude: turn[node][pair of dimensions], by NT threads, a
+// thread keeping its dimension, whose frequency is `freq`.
+template <int NT>
+__device__ __forceinline__ void tree_turns(float freq, float amp, int P, const int* depth, int na, int nb, float2* turn) {
+  constexpr int HALF = ATTN_D / 2;
+  for (int i = na * HALF + threadIdx.x; i < nb * HALF; i += NT) {
+    float s, co;
+    sincosf((float)(P + depth[i / HALF]) * freq, &s, &co);
+    turn[i] = float2{co * amp, s * amp};
+  }
+}
+// The key and value rows of nodes r0 .. r0 + rows - 1 of kv head g from the raw projections, by NT threads, a thread taking
+// dimensions d and d + 32 of every NT / 32'th row: all loads at once, ahead of the sines.
+template <typename KT, int NT>
+struct NodeRows {
+  static constexpr int HALF = ATTN_D / 2, N = NSX_TREE_MAX_NODES * HALF / NT;
+  float k[N][2], v[N][2];
+  __device__ __forceinline__ NodeRows(const TreeArgs& a, int g, int r0, int rows) {
+    const int d = threadIdx.x % HALF, first = threadIdx.x / HALF;
+    const float* x = a.q + ((int64_t)r0 * (a.n_head + 2 * a.n_kv) + a.n_head + g) * ATTN_D + d;
+    float b[4];
+    if (a.bk) b[0] = a.bk[g * ATTN_D + d], b[1] = a.bk[g * ATTN_D + d + HALF];
+    if (a.bv) b[2] = a.bv[g * ATTN_D + d], b[3] = a.bv[g * ATTN_D + d + HALF];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int row = min(first + n * (NT / HALF), max(rows, 1) - 1);
+      const float *kp = x + (int64_t)row * (a.n_head + 2 * a.n_kv) * ATTN_D, *vp = kp + (int64_t)a.n_kv * ATTN_D;
+      k[n][0] = kp[0], k[n][1] = kp[HALF], v[n][0] = vp[0], v[n][1] = vp[HALF];
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      if (a.bk) k[n][0] += b[0], k[n][1] += b[1];
+      if (a.bv) v[n][0] += b[2], v[n][1] += b[3];
+    }
+  }
+  // f(row, d, key's two elements, value's), rotated by turn (of the node)
+  template <typename F>
+  __device__ __forceinline__ void each(int r0, int rows, const float2* turn, F f) const {
+    const int d = threadIdx.x % HALF, first = threadIdx.x / HALF;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int row = first + n * (NT / HALF);
+      if (row < rows) {
+        const float2 w = turn[(r0 + row) * HALF + d];
+        const float z0 = fmaf(k[n][0], w.x, -(k[n][1] * w.y)), z1 = fmaf(k[n][1], w.x, k[n][0] * w.y);  // (as rope_elem)
+        f(row, d, z0, z1, v[n][0], v[n][1]);
+      }
+    }
+  }
+};
+template <typename KT>
+__device__ __forceinline__ void store_row(void* k, void* v, int64_t row, int d, float k0, float k1, float v0, float v1) {
+  const int64_t at = row * ATTN_D + d;
+  store_kv<KT>(k, at, k0), store_kv<KT>(k, at + ATTN_D / 2, k1);
+  store_kv<KT>(v, at, v0), store_kv<KT>(v, at + ATTN_D / 2, v1);
+}
+
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028235e38f; }
 
 // Workgroup (kv head g, block cb of 16 NC query columns, split c of the keys). A column is a (node, query head of the
@@ -251,7 +275,13 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028235e3
 //
 // ROPE: q is the nodes' raw projections. A workgroup forms the sines and cosines of its columns' nodes (of all nodes where
 // its split has some of theirs) once, as a table in LDS, and rotates its queries by it; a split with node tiles also
-// makes those tiles' rows, for its own use in LDS and, the first block of columns, for the cache's keeper in wk and wv.
+// makes those tiles' rows, for its own use in LDS and, the first block of columns, for the cache's keeper in wk and wv. What
+// does not depend on the position is loaded ahead of it, and the first tiles ahead of the sines (a launch of its own for the
+// rows, and their loads where they were used, took 23 nodes 17.7 us and 13.2; now 11.4).
+//
+// Bounds: few keys, the chain of dependent loads (position, parents, rows) and the launch -- one node over 203 bf16 rows 6
+// us; many keys and few columns, their bytes -- 7 nodes over 131000 fp16 rows, 268 MB, 52 us, what a copy reaches; many
+// columns, the terms' VALU work beside the products, which the wide kernel below shares among four waves.
 template <typename KT, int NC, bool ROPE>
 __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) {
   using R = Rows<KT>;
@@ -271,12 +301,38 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
   const int t = threadIdx.x, lane = t & 63, i16 = lane & 15, kq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int g = blockIdx.x % a.n_kv, cb = blockIdx.x / a.n_kv, c = blockIdx.y;
+  // what does not wait for the position: the wave's parents, a thread's frequency, its eight elements of a query and
+  // those that they turn with
+  const int heads = ROPE ? a.n_head + 2 * a.n_kv : a.n_head;  // rows of a node in q
+  const int ncol = a.nodes * a.n_rep, col0 = cb * COLS;
+  const int up = wave == 0 ? tree_parent(a.parents, a.nodes, lane) : -1;
+  const float freq = ROPE ? a.inv_freq[t % HALF] : 0.f;
+  const int qc = t / (ATTN_D / 8), qcol = min(col0 + qc, ncol - 1), qj = t / 4 % 2, qg = t % 4;
+  const int qnode = qcol / a.n_rep, qh = g * a.n_rep + qcol % a.n_rep;
+  auto eight = [&](const float* p, int j, float (&x)[8]) {
+    const v4f x0 = *(const v4f*)(p + R::dim(j, qg, 0)), x1 = *(const v4f*)(p + R::dim(j, qg, 4));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = e < 4 ? x0[e & 3] : x1[e & 3];
+  };
+  float qx[8], qy[8], bx[8], by[8];
+  static_assert(COLS * (ATTN_D / 8) <= NT);
+  if (qc < COLS) {
+    const float* p = a.q + ((int64_t)qnode * heads + qh) * ATTN_D;
+    eight(p, qj, qx);
+    if constexpr (ROPE) {
+      eight(p, qj ^ 1, qy);
+      if (a.bq) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          bx[e] = a.bq[qh * ATTN_D + R::dim(qj, qg, e)], by[e] = a.bq[qh * ATTN_D + R::dim(qj ^ 1, qg, e)];
+      }
+    }
+  }
   const int P = *a.pos;
   if (P < 0 || P > a.ctx_max) return;
   const Tiles tl(a, P, TREE_KEYS, TREE_NW);
   const int lo = tl.lo, pt = tl.cache, t0 = c * tl.per, t1 = min(tl.all, t0 + tl.per);
   if (t0 >= t1) return;
-  const int ncol = a.nodes * a.n_rep, col0 = cb * COLS;
   // ROPE: the node tiles come after the loop, from LDS
   const int first = t0 + wave, end = ROPE ? min(t1, pt) : t1, last = end - 1, nodes0 = max(t0, pt);
 
@@ -321,7 +377,7 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
   load_v(min(first, last));
 
   if (wave == 0) {
-    uint64_t line = tree_lineage(a.parents, a.nodes, lane);
+    uint64_t line = tree_lineage(up, lane);
     const int dep = __popcll(line) - 1;
     if (a.window > 0 && a.window < a.nodes) {  // ancestors out of the window
       for (int j = 0; j < a.nodes; ++j)
@@ -330,66 +386,43 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
     svis[lane] = line;
     sdep[lane] = dep;
   }
-  const int heads = ROPE ? a.n_head + 2 * a.n_kv : a.n_head;  // rows of a node in q
-  float2* turn = (float2*)&lds[QBYTES];                       // amplitude times (cosine, sine)
+  float2* turn = (float2*)&lds[QBYTES];  // amplitude times (cosine, sine)
   if constexpr (ROPE) {
-    nsx_lds_barrier();
-    const int na = t1 > pt ? 0 : col0 / a.n_rep, nb = t1 > pt ? a.nodes : min(col0 + COLS - 1, ncol - 1) / a.n_rep + 1;
-    for (int i = na * HALF + t; i < nb * HALF; i += NT) {
-      float s, co;
-      sincosf((float)(P + sdep[i / HALF]) * a.inv_freq[i % HALF], &s, &co);
-      turn[i] = float2{co * a.amp, s * a.amp};
-    }
-    nsx_lds_barrier();
-    const int r0 = (nodes0 - pt) * TREE_KEYS, rows = min((t1 - pt) * TREE_KEYS, a.nodes) - r0;
-    for (int i = t; i < rows * HALF; i += NT) {
-      const int row = r0 + i / HALF, d = i % HALF;
-      const float* x = a.q + ((int64_t)row * heads + a.n_head + g) * ATTN_D + d;
-      const float* y = x + (int64_t)a.n_kv * ATTN_D;
-      float k0 = x[0], k1 = x[HALF], v0 = y[0], v1 = y[HALF];
-      if (a.bk) k0 += a.bk[g * ATTN_D + d], k1 += a.bk[g * ATTN_D + d + HALF];
-      if (a.bv) v0 += a.bv[g * ATTN_D + d], v1 += a.bv[g * ATTN_D + d + HALF];
-      const float2 w = turn[row * HALF + d];
-      const float z0 = fmaf(k0, w.x, -(k1 * w.y)), z1 = fmaf(k1, w.x, k0 * w.y);  // (as rope_elem)
-      uint8_t* to = &lds[NODES_AT + (row - r0) * NROW];
-      store_kv<KT>(to, d, z0), store_kv<KT>(to, d + HALF, z1);
-      store_kv<KT>(to + NBYTES, d, v0), store_kv<KT>(to + NBYTES, d + HALF, v1);
-      if (cb == 0) {
-        const int64_t at = ((int64_t)g * a.max_nodes + row) * ATTN_D + d;
-        store_kv<KT>(a.wk, at, z0), store_kv<KT>(a.wk, at + HALF, z1);
-        store_kv<KT>(a.wv, at, v0), store_kv<KT>(a.wv, at + HALF, v1);
-      }
+    const bool makes = t1 > pt;  // this split has nodes' rows: all nodes' sines, as the rows it makes are
+    const int na = makes ? 0 : col0 / a.n_rep, nb = makes ? a.nodes : min(col0 + COLS - 1, ncol - 1) / a.n_rep + 1;
+    if (makes) {
+      const int r0 = (nodes0 - pt) * TREE_KEYS, rows = min((t1 - pt) * TREE_KEYS, a.nodes) - r0;
+      const NodeRows<KT, NT> x(a, g, r0, rows);
+      nsx_lds_barrier();
+      tree_turns<NT>(freq, a.amp, P, sdep, na, nb, turn);
+      nsx_lds_barrier();
+      x.each(r0, rows, turn, [&](int row, int d, float k0, float k1, float v0, float v1) {
+        uint8_t* to = &lds[NODES_AT + row * NROW];
+        store_row<KT>(to, to + NBYTES, 0, d, k0, k1, v0, v1);
+        if (cb == 0) store_row<KT>(a.wk, a.wv, (int64_t)g * a.max_nodes + r0 + row, d, k0, k1, v0, v1);
+      });
+    } else {
+      nsx_lds_barrier();
+      tree_turns<NT>(freq, a.amp, P, sdep, na, nb, turn);
+      nsx_lds_barrier();
     }
   }
-  for (int i = t; i < COLS * (ATTN_D / 8); i += NT) {
-    const int cc = i / (ATTN_D / 8), col = min(col0 + cc, ncol - 1), j = i / 4 % 2, gg = i % 4;
-    const int node = col / a.n_rep, h = g * a.n_rep + col % a.n_rep;
-    const float* qp = a.q + ((int64_t)node * heads + h) * ATTN_D;
-    auto eight = [&](const float* p, int jj, float (&x)[8]) {
-      const v4f x0 = *(const v4f*)(p + R::dim(jj, gg, 0)), x1 = *(const v4f*)(p + R::dim(jj, gg, 4));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = e < 4 ? x0[e & 3] : x1[e & 3];
-    };
-    float x[8];
-    eight(qp, j, x);
+  if (qc < COLS) {
     if constexpr (ROPE) {
-      float other[8];
-      eight(qp, j ^ 1, other);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int d = R::dim(0, gg, e);
-        if (a.bq) x[e] += a.bq[h * ATTN_D + HALF * j + d], other[e] += a.bq[h * ATTN_D + HALF * (j ^ 1) + d];
-        const float2 w = turn[node * HALF + d];
-        const float ps = other[e] * w.y;
-        x[e] = fmaf(x[e], w.x, j ? ps : -ps);
+        if (a.bq) qx[e] += bx[e], qy[e] += by[e];
+        const float2 w = turn[qnode * HALF + R::dim(0, qg, e)];
+        const float ps = qy[e] * w.y;
+        qx[e] = fmaf(qx[e], w.x, qj ? ps : -ps);
       }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] *= a.scale2;
+    for (int e = 0; e < 8; ++e) qx[e] *= a.scale2;
     v4u tm[3];
-    split8(x, tm);
+    split8(qx, tm);
 #pragma unroll
-    for (int k = 0; k < 3; ++k) *(v4u*)&lds[(k * COLS + cc) * QROW + (4 * j + gg) * 16] = tm[k];
+    for (int k = 0; k < 3; ++k) *(v4u*)&lds[(k * COLS + qc) * QROW + (4 * qj + qg) * 16] = tm[k];
   }
   nsx_lds_barrier();
   const int q0 = i16 * QROW + kq * 16;
@@ -653,7 +686,15 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
 // A tile takes two phases: products (the scores of tile i, the values of tile i - 1) and the rest (the weights of
 // tile i, the terms of keys i + 1 and values i). Waves w and w + 4 share a SIMD, and their groups are one phase apart, kept
 // so by the barrier between phases: the matrix cores have one group's products while the VALU has the other's weights.
-template <typename KT>
+//
+// Bound by the phases' shared issue: 64 nodes over 65536 bf16 keys (64 / 8 heads, three products a term pair: 206 GFLOP of
+// bf16) 184 us, 1120 TFLOP/s, what a large library product reaches here (1108); 64 nodes over 6000 fp32 keys (six products)
+// 48 us, 16 over 16384 37. Both groups in one phase 188 for an earlier 160, no offset between them 184; scheduler groups,
+// one barrier a tile, 32 x 32 products, two workgroups of four waves: all within 5 % or slower.
+//
+// ROPE as above, the table where the first tiles come afterwards; a split with nodes' rows writes them beside the cache
+// and loads them back as it does the cache's.
+template <typename KT, bool ROPE>
 __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
   using R = Rows<KT>;
   constexpr int KTN = R::NT, NC = 2, CW = 4, NG = 2, COLS = 16 * NC * CW;
@@ -670,12 +711,35 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int group = wave / CW, cw = wave % CW;  // waves w and w + 4 lie on one SIMD
   const int g = blockIdx.x % a.n_kv, cb = blockIdx.x / a.n_kv, c = blockIdx.y;
+  // what does not wait for the position: the wave's parents, a thread's frequency, its queries
+  constexpr int HALF = ATTN_D / 2;
+  const int heads = ROPE ? a.n_head + 2 * a.n_kv : a.n_head;  // rows of a node in q
+  const int ncol = a.nodes * a.n_rep, col0 = cb * COLS + 16 * NC * cw;
+  const int up = wave == 0 ? tree_parent(a.parents, a.nodes, lane) : -1;
+  const float freq = ROPE ? a.inv_freq[t % HALF] : 0.f;
+  float qx[NC][2][8], qb[NC][2][8];
+#pragma unroll
+  for (int ct = 0; ct < NC; ++ct) {
+    const int col = min(col0 + 16 * ct + i16, ncol - 1), h = g * a.n_rep + col % a.n_rep;
+    const float* qp = a.q + ((int64_t)(col / a.n_rep) * heads + h) * ATTN_D;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const v4f x0 = *(const v4f*)(qp + R::dim(j, kq, 0)), x1 = *(const v4f*)(qp + R::dim(j, kq, 4));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) qx[ct][j][e] = e < 4 ? x0[e & 3] : x1[e & 3];
+    }
+    if (ROPE && a.bq) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) qb[ct][j][e] = a.bq[h * ATTN_D + R::dim(j, kq, e)];
+    }
+  }
   const int P = *a.pos;
   if (P < 0 || P > a.ctx_max) return;
   const Tiles tl(a, P, KEYS, 1);
   const int lo = tl.lo, pt = tl.cache, t0 = c * tl.per, t1 = min(tl.all, t0 + tl.per);
   if (t0 >= t1) return;
-  const int ncol = a.nodes * a.n_rep, col0 = cb * COLS + 16 * NC * cw;
   const int phases = (t1 - t0 + 1) / 2;               // tiles of the first group, the most
   const int mine = (t1 - t0 + 1 - group) / 2;  // of this one: t0 + group, + 2, ..
 
@@ -765,12 +829,15 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
       }
     }
   };
+  // ROPE: a split with nodes' rows makes them first
+  const bool makes = ROPE && t1 > pt;
   Source src = source(0);
-  load_k(src);
-  load_v(src);
-
+  if (!makes || !src.own) {
+    load_k(src);
+    load_v(src);
+  }
   if (wave == 0) {
-    uint64_t line = tree_lineage(a.parents, a.nodes, lane);
+    uint64_t line = tree_lineage(up, lane);
     const int dep = __popcll(line) - 1;
     if (a.window > 0 && a.window < a.nodes) {  // ancestors out of the window
       for (int j = 0; j < a.nodes; ++j)
@@ -779,18 +846,48 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
     svis[lane] = line;
     sdep[lane] = dep;
   }
+  static_assert(!ROPE || NSX_TREE_MAX_NODES * HALF * (int)sizeof(float2) <= LDS);
+  float2* turn = (float2*)lds;  // amplitude times (cosine, sine); the first tiles come over it, a barrier later
+  if constexpr (ROPE) {
+    const int na = makes ? 0 : cb * COLS / a.n_rep, nb = makes ? a.nodes : min(cb * COLS + COLS - 1, ncol - 1) / a.n_rep + 1;
+    if (makes) {
+      const int r0 = (max(t0, pt) - pt) * KEYS, rows = min((t1 - pt) * KEYS, a.nodes) - r0;
+      const NodeRows<KT, 512> x(a, g, r0, rows);
+      nsx_lds_barrier();
+      tree_turns<512>(freq, a.amp, P, sdep, na, nb, turn);
+      nsx_lds_barrier();
+      x.each(r0, rows, turn, [&](int row, int d, float k0, float k1, float v0, float v1) {
+        store_row<KT>(a.wk, a.wv, (int64_t)g * a.max_nodes + r0 + row, d, k0, k1, v0, v1);  // (every block the same)
+      });
+      __syncthreads();  // this workgroup's stores, ahead of its loads
+      if (src.own) {
+        load_k(src);
+        load_v(src);
+      }
+    } else {
+      nsx_lds_barrier();
+      tree_turns<512>(freq, a.amp, P, sdep, na, nb, turn);
+      nsx_lds_barrier();
+    }
+  }
   v4u q[NC][2][3];
 #pragma unroll
   for (int ct = 0; ct < NC; ++ct) {
-    const int col = min(col0 + 16 * ct + i16, ncol - 1), node = col / a.n_rep, h = g * a.n_rep + col % a.n_rep;
-    const float* qp = a.q + ((int64_t)node * a.n_head + h) * ATTN_D;
+    if constexpr (ROPE) {
+      const int node = min(col0 + 16 * ct + i16, ncol - 1) / a.n_rep;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (a.bq) qx[ct][0][e] += qb[ct][0][e], qx[ct][1][e] += qb[ct][1][e];
+        const float2 w = turn[node * HALF + R::dim(0, kq, e)];
+        const float x0 = qx[ct][0][e], x1 = qx[ct][1][e];
+        qx[ct][0][e] = fmaf(x0, w.x, -(x1 * w.y)), qx[ct][1][e] = fmaf(x1, w.x, x0 * w.y);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const v4f x0 = *(const v4f*)(qp + R::dim(j, kq, 0)), x1 = *(const v4f*)(qp + R::dim(j, kq, 4));
-      float x[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = (e < 4 ? x0[e & 3] : x1[e & 3]) * a.scale2;
-      split8(x, q[ct][j]);
+      for (int e = 0; e < 8; ++e) qx[ct][j][e] *= a.scale2;
+      split8(qx[ct][j], q[ct][j]);
     }
   }
   nsx_lds_barrier();
@@ -1194,18 +1291,19 @@ struct TreePlan {
   int kind, ncb, nsplit, keys, round;
 };
 
-// `work` counts pieces of 32 keys x 16 columns. Below 8192, eight for each SIMD of the chip, the kernel of 16 columns has
-// the most workgroups and the shortest way through one (us for 16 / 32 / 128 columns at 64 / 8 heads, fp32: 16 nodes,
-// 1000 keys 14.9 / 17.7 / 18.3; 8 nodes, 8000 keys 23.6 / 23.4 / 25.7; 48 nodes, 1500 keys 31.1 / 26.9 / 25.7). Past it,
-// more than 64 columns go to the wide kernel once its sharing of terms outweighs its longer way: three terms a
-// element from 11000 pieces on (16 nodes, 6000 keys 27.0 / 24.6 / 25.1; 32 nodes, 8000 keys 50.7 / 38.7 / 34.5), one
-// term from 32768 (bf16, 32 nodes, 4000 keys 23.5 / 21.6 / 23.8; 16 nodes, 16384 keys 34.5 / 27.1 / 26.6).
+// `work` counts pieces of 32 keys x 16 columns. Below 12288, twelve for each SIMD of the chip, the kernel of 16 columns has
+// the most workgroups and the shortest way through one (us for 16 / 32 / 128 columns at 64 / 8 heads, fp32, 4000 keys:
+// 16 nodes 22.9 / 23.7 / 26.3, 32 nodes 30.1 / 27.6 / 31.0; bf16 17.6 / 20.2 / 24.6 and 21.7 / 21.2 / 27.5). Past it, more
+// than 64 columns go to the wide kernel once its sharing of terms outweighs its longer way, the sooner the more terms an
+// element has: three from 32768 pieces on (fp32, 64 nodes, 4000 keys 52.3 / 41.3 / 42.6, 8000 keys 86.4 / 64.8 / 60.0), two
+// from 49152 (8000 keys 63.1 / 52.8 / 52.6), one from 98304 (bf16, 64 nodes, 16000 keys 95.4 / 62.1 / 62.5, 32000 keys
+// 178 / 110 / 104).
 TreePlan tree_plan(int n_kv, int n_rep, int nodes, int64_t ctx_max, int window, int kv_dtype) {
   const int64_t cols = (int64_t)nodes * n_rep, rows = window > 0 ? std::min<int64_t>(ctx_max, window) : ctx_max;
   const int64_t work = n_kv * nsx_cdiv(cols, 16) * nsx_cdiv(rows, 32);
   const int terms = kv_dtype == NSX_DT_F32 ? 3 : kv_dtype == NSX_DT_F16 ? 2 : 1;
   TreePlan p;
-  p.kind = work < 8192 ? TREE_16 : cols > 64 && work * terms >= 32768 ? TREE_WIDE : TREE_32;
+  p.kind = work < 12288 ? TREE_16 : cols > 64 && work * terms >= 98304 ? TREE_WIDE : TREE_32;
   const bool wide = p.kind == TREE_WIDE;
   p.keys = wide && terms == 1 ? 2 * TREE_KEYS : TREE_KEYS;
   p.round = wide ? 1 : TREE_NW;
@@ -1220,10 +1318,8 @@ TreePlan tree_plan(int n_kv, int n_rep, int nodes, int64_t ctx_max, int window, 
 }
 
 int64_t tree_bytes(int n_head, int n_kv, int nodes, int64_t ctx_max, int window, int kv_dtype) {
-  const int64_t rows = (int64_t)nodes * n_head;
-  // the rotated queries, then a split's values and (maximum, sum) per row
-  return rows * ATTN_D * 4 +
-         rows * tree_plan(n_kv, n_head / n_kv, nodes, ctx_max, window, kv_dtype).nsplit * (ATTN_D + 2) * 4;
+  // a split's values and (maximum, sum) per row
+  return (int64_t)nodes * n_head * tree_plan(n_kv, n_head / n_kv, nodes, ctx_max, window, kv_dtype).nsplit * (ATTN_D + 2) * 4;
 }
 
 int tree_shapes(int n_head, int n_kv, int head_dim, int nodes, int max_nodes, int64_t ctx_max, int window) {
@@ -1251,15 +1347,7 @@ int tree_attn_typed(TreeArgs& a, const TreePlan& p, hipStream_t st) {
   } else if (p.kind == TREE_32) {
     hipLaunchKernelGGL((tree_attn_kernel<KT, 2, ROPE>), grid, dim3(64 * TREE_NW), 0, st, a);
   } else {
-    if constexpr (ROPE) {  // a launch of its own: little beside this kernel's time
-      float* q = a.part - (int64_t)a.nodes * a.n_head * ATTN_D;
-      const dim3 rows((unsigned)nsx_cdiv((int64_t)a.nodes * (a.n_head + 2 * a.n_kv), 4));
-      hipLaunchKernelGGL((tree_rope_kernel<KT>), rows, dim3(256), 0, st, a.q, a.bq, a.bk, a.bv, a.inv_freq, a.amp,
-                         a.n_head, a.n_kv, a.parents, a.pos, a.ctx_max, a.nodes, a.max_nodes, q, a.wk, a.wv);
-      NSX_LAUNCHED();
-      a.q = q;
-    }
-    hipLaunchKernelGGL((tree_wide_kernel<KT>), grid, dim3(512), 0, st, a);
+    hipLaunchKernelGGL((tree_wide_kernel<KT, ROPE>), grid, dim3(512), 0, st, a);
   }
   NSX_LAUNCHED();
   if (a.nsplit > 1) {
@@ -1319,8 +1407,8 @@ extern "C" int nsx_tree_attn(const float* q, const void* k_cache, const void* v_
                                  n_head, n_kv, n_nodes, ctx_max, window))
     return rc;
   TreeArgs a{q, k_cache, v_cache, node_k, node_v, parents, pos, ctx_max, window, n_head / n_kv, n_kv, n_head, n_nodes,
-             max_nodes, 0, 0, 0, 0, scale * LOG2E, (float*)workspace + (int64_t)n_nodes * n_head * ATTN_D, sinks, out, nullptr, nullptr, nullptr, nullptr, 0.f,
-             nullptr, nullptr};
+             max_nodes, 0, 0, 0, 0, scale * LOG2E, (float*)workspace, sinks, out, nullptr,
+             nullptr, nullptr, nullptr, 0.f, nullptr, nullptr};
   return tree_attn_launch<false>(a, kv_dtype, (hipStream_t)stream);
 }
 
@@ -1336,7 +1424,7 @@ extern "C" int nsx_tree_attn_qkv(const float* qkv, const float* q_bias, const fl
                                  n_head, n_kv, n_nodes, ctx_max, window))
     return rc;
   TreeArgs a{qkv, k_cache, v_cache, node_k, node_v, parents, pos, ctx_max, window, n_head / n_kv, n_kv, n_head, n_nodes,
-             max_nodes, 0, 0, 0, 0, scale * LOG2E, (float*)workspace + (int64_t)n_nodes * n_head * ATTN_D, sinks, out, q_bias,
+             max_nodes, 0, 0, 0, 0, scale * LOG2E, (float*)workspace, sinks, out, q_bias,
              k_bias, v_bias, inv_freq, amplitude, node_k, node_v};
   return tree_attn_launch<true>(a, kv_dtype, (hipStream_t)stream);
 }

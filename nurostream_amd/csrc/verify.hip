@@ -108,7 +108,8 @@ __device__ __forceinline__ double vf_weight_finite(float x, float M, const Verif
   const uint32_t k = (uint32_t)__builtin_bit_cast(uint64_t, t);
   const double r = fma(d, a.scale2, -(t - 0x1.8p47));
   // ln2, ln2^2 / 2, ln2^3 / 6, ln2^4 / 24
-  const double h = fma(r, fma(r, fma(r, 0.0096181291076284772, 0.055504108664821580), 0.24022650695910071), 0.69314718055994531);
+  const double h =
+      fma(r, fma(r, fma(r, 0.0096181291076284772, 0.055504108664821580), 0.24022650695910071), 0.69314718055994531);
   const double c = tab.t[k & 31], w = fma(r * h, c, c);
   const uint64_t bits = __builtin_bit_cast(uint64_t, w) + ((uint64_t)(k >> 5) << 52);
   return __builtin_bit_cast(double, bits);
@@ -547,12 +548,12 @@ extern "C" int nsx_verify(const void* logits, int logits_dtype, int64_t row_stri
               NSX_TREE_MAX_NODES);
   NSX_REQUIRE(batch >= 0 && batch * n_nodes < 65536, NSX_EINVAL, "%lld sequences of %d nodes: fewer than 65536 rows",
               (long long)batch, n_nodes);
-  NSX_REQUIRE(vocab > 0 && chunks(vocab) <= VF_MAX_CHUNKS + 1 && vocab <= (int64_t)VF_CHUNK * VF_MAX_CHUNKS, NSX_EINVAL, "vocabulary of %lld (1 to %lld)",
-              (long long)vocab, (long long)VF_CHUNK * VF_MAX_CHUNKS);
+  NSX_REQUIRE(vocab > 0 && vocab <= (int64_t)VF_CHUNK * VF_MAX_CHUNKS, NSX_EINVAL, "vocabulary of %lld (1 to %lld)",
+              (long long)vocab, (long long)VF_CHUNK * VF_MAX_CHUNKS);  // (then at most VF_MAX_CHUNKS + 1 chunks)
   NSX_REQUIRE(row_stride >= vocab, NSX_EINVAL, "rows %lld elements apart for %lld logits", (long long)row_stride,
               (long long)vocab);
-  NSX_REQUIRE(temperature == 0.0 || (temperature >= 1e-30 && temperature <= 1e30), NSX_EINVAL, "temperature %g (0, or 1e-30 to 1e30)",
-              temperature);
+  NSX_REQUIRE(temperature == 0.0 || (temperature >= 1e-30 && temperature <= 1e30), NSX_EINVAL,
+              "temperature %g (0, or 1e-30 to 1e30)", temperature);
   NSX_REQUIRE(parents_stride == 0 || parents_stride >= n_nodes, NSX_EINVAL, "parents_stride=%lld",
               (long long)parents_stride);
   NSX_REQUIRE(!(draft_probs && parents), NSX_EINVAL, "draft probabilities go with chains (no parents)");

@@ -158,12 +158,13 @@ def test_many_columns(dev, dtype, heads, n, kind):
         assert rel_max(to_np(out), _gpu_ref(c, kv, draft, q, parents, s, 0, pos)) < TOL, pos
 
 
+@pytest.mark.parametrize("heads", [(16, 1), (32, 2)], ids=lambda h: f"{h[0]}q{h[1]}kv")
 @pytest.mark.parametrize("dtype", sorted(TYPES))
-def test_many_columns_in_a_window(dev, dtype):
+def test_many_columns_in_a_window(dev, dtype, heads):
     """Windows that end inside the cache, the nodes' first rows a few apart; rows before every window hold NaN."""
     from nurostream_amd.model.draft import tree_attn
     for window, pos, n, kind in ((33000, 33500, 64, "chain"), (33001, 33010, 40, "tree"), (40000, 39990, 64, "chain")):
-        c, kv, draft, q, sinks = _state(dev, 16, 1, n, pos, dtype, seed=n, **WIDE)
+        c, kv, draft, q, sinks = _state(dev, *heads, n, pos, dtype, seed=n, **WIDE)
         parents = _parents(n, kind, seed=window)
         ref = _gpu_ref(c, kv, draft, q, parents, sinks, window, pos)
         gone = max(0, pos + 1 - window)
@@ -350,7 +351,8 @@ def test_tree_attention_qkv_equals_rotated_rows(dev, dtype, heads, n, kind, ctx)
     from nurostream_amd.model.decode import DeviceKV, rope_kv_append, yarn_inv_freq
     from nurostream_amd.model.draft import tree_attn, tree_attn_qkv
     H, G = heads
-    for pos, window in ((0, 0), (1, 0), (31, 0), (32, 9), (33, 0), (127, 70), (128, 0), (500, 0), (500, 128), (1500, 0)):
+    for pos, window in ((0, 0), (1, 0), (31, 0), (32, 9), (33, 0), (127, 70), (128, 0), (500, 0), (500, 128), (1500, 0),
+                        *(((33500, 33001),) if ctx == 70000 else ())):
         c, kv, draft, _, sinks = _state(dev, H, G, n, pos, dtype, seed=pos, ctx=ctx)
         inv, amp = yarn_inv_freq(c, dev)
         g = torch.Generator().manual_seed(pos)
