@@ -439,8 +439,8 @@ int nsx_tree_attn_qkv(const float *qkv, const float *q_bias, const float *k_bias
                       int64_t workspace_bytes, float *out, void *stream);
 /* Rows path[0 .. min(*count, n_nodes) - 1] of the nodes into the caches' rows
  * *pos, *pos + 1, ..., for all layers ([n_layer][n_kv][ctx_max][64] caches,
- * [n_layer][n_kv][max_nodes][64] nodes), then *pos += *count, at most to
- * ctx_max. Rows past ctx_max and entries of path outside [0, max_nodes) are
+ * [n_layer][n_kv][max_nodes][64] nodes), then *pos moves on by as many, at most
+ * to ctx_max. Rows past ctx_max and entries of path outside [0, max_nodes) are
  * not copied; other rows stay as they are. counter: one device word, zero
  * before the first call and after every call. */
 int nsx_tree_commit(void *k_caches, void *v_caches, const void *node_k, const void *node_v, int kv_dtype,

@@ -37,7 +37,7 @@ class DraftKV:
         nb = N.load().nsx_tree_workspace_bytes(cfg.n_head, n_kv, head_dim, int(max_nodes), kv.ctx_max)
         if nb < 0:
             raise NotImplementedError(N.load().nsx_last_error().decode(errors="replace"))
-        self.kv, self.max_nodes, self.n_head = kv, int(max_nodes), cfg.n_head
+        self.kv, self.max_nodes, self.heads = kv, int(max_nodes), (cfg.n_head, n_kv, head_dim)
         shape = (n_layer, n_kv, self.max_nodes, head_dim)
         self.k_stack = torch.zeros(shape, dtype=kv.dtype, device=kv.device)
         self.v_stack = torch.zeros(shape, dtype=kv.dtype, device=kv.device)
@@ -82,8 +82,9 @@ def _tree(x: torch.Tensor, row: int, name: str, draft: DraftKV, layer: int, cfg:
     _check(name, x, torch.float32, kv.k_stack.device, n * row)
     if not 1 <= n <= draft.max_nodes:
         raise ValueError(f"{n} nodes: this DraftKV holds 1 to {draft.max_nodes}")
-    if cfg.n_head != draft.n_head:
-        raise ValueError(f"{cfg.n_head} query heads; the DraftKV was made for {draft.n_head}")
+    if (cfg.n_head, cfg.n_head_kv, cfg.head_dim) != draft.heads:
+        raise ValueError(f"{cfg.n_head} query heads over {cfg.n_head_kv} of {cfg.head_dim}; the DraftKV was made for "
+                         "{} over {} of {}".format(*draft.heads))
     if not 0 <= layer < len(draft.k):
         raise IndexError(f"layer {layer} of {len(draft.k)}")
     _check("parents", parents, torch.int32, x.device, n)

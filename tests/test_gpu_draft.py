@@ -433,6 +433,55 @@ def test_commit_skips_bad_entries(dev):
     assert torch.equal(kv.k[0].nan_to_num(5.0), k.nan_to_num(5.0)) and int(kv.pos) == 7
 
 
+def test_refusals_of_tensors(dev):
+    """Wrong types, sizes, layouts and another model's heads are refused before any launch."""
+    from nurostream_amd.model.decode import yarn_inv_freq
+    from nurostream_amd.model.draft import commit, tree_attn, tree_attn_qkv, verify
+    n, H, G = 4, 8, 2
+    c, kv, draft, q, sinks = _state(dev, H, G, n, 5, ctx=20)
+    inv, amp = yarn_inv_freq(c, dev)
+    par, qkv = _ids([-1, 0, 0, 1], dev), torch.zeros(n, (H + 2 * G) * 64, device=dev)
+    attn = lambda **kw: tree_attn(**{**dict(q=q, cfg=c, draft=draft, layer=0, sinks=sinks, window=0, parents=par), **kw})  # noqa: E731
+    raw = lambda **kw: tree_attn_qkv(**{**dict(qkv=qkv, bq=None, bk=None, bv=None, cfg=c, inv_freq=inv, amp=amp,  # noqa: E731
+                                               draft=draft, layer=0, sinks=sinks, window=0, parents=par), **kw})
+    wide = torch.zeros(n, 2 * H * 64, device=dev)
+    z = lambda *s: torch.zeros(*s, device=dev)  # noqa: E731
+    for kw in (dict(cfg=_cfg(H, 4)), dict(cfg=_cfg(H, 1)), dict(cfg=_cfg(16, G), q=z(n, 16 * 64)), dict(q=z(5, H * 64)),
+               dict(q=wide[:, ::2]), dict(q=z(n, H * 64 - 1)), dict(sinks=z(H + 1)), dict(parents=par[:3]),
+               dict(out=z(n, H, 63)), dict(window=-1), dict(q=z(0, H * 64)), dict(sinks=sinks.cpu())):
+        with pytest.raises(ValueError):
+            attn(**kw)
+    for kw in (dict(q=q.half()), dict(parents=par.long()), dict(sinks=sinks.double()), dict(out=z(n, H, 64).half())):
+        with pytest.raises(TypeError):
+            attn(**kw)
+    for layer in (-1, 1):
+        with pytest.raises(IndexError):
+            attn(layer=layer)
+    for kw in (dict(qkv=q), dict(bq=z(H * 64 - 64)), dict(bk=z(H * 64)), dict(bv=z(1)), dict(inv_freq=z(64)),
+               dict(cfg=_cfg(H, 4), qkv=z(n, 16 * 64))):
+        with pytest.raises(ValueError):
+            raw(**kw)
+    path, count = _ids([0, 1], dev), _ids([2], dev)
+    for args in ((path.long(), count), (path, count.long())):
+        with pytest.raises(TypeError):
+            commit(draft, *args)
+    for args in ((_ids([0] * 5, dev), count), (path, path), (_ids([0] * 4, dev)[::2], count)):
+        with pytest.raises(ValueError):
+            commit(draft, *args)
+    x, tok, u = z(2, 3, 50), _ids([[0, 1, 2]] * 2, dev), z(2, 3)
+    ver = lambda **kw: verify(**{**dict(logits=x, tokens=tok, uniforms=u, temperature=1.0), **kw})  # noqa: E731
+    for kw in (dict(tokens=tok[:1]), dict(uniforms=None), dict(uniforms=u[:1]), dict(parents=_ids([-1, 0], dev)),
+               dict(parents=_ids([-1, 0, 0], dev), draft_probs=z(2, 2, 50)), dict(draft_probs=z(2, 3, 50)),
+               dict(lengths=_ids([1], dev)), dict(temperature=-1.0), dict(temperature=float("nan")), dict(logits=z(50)),
+               dict(logits=z(1, 65, 50), tokens=_ids([0] * 65, dev), uniforms=z(65)), dict(logits=z(2, 3, 0))):
+        with pytest.raises(ValueError):
+            ver(**kw)
+    for kw in (dict(logits=x.double()), dict(tokens=tok.long()), dict(uniforms=u.double()), dict(draft_probs=z(2, 2, 50).half())):
+        with pytest.raises(TypeError):
+            ver(**kw)
+    assert int(kv.pos) == 5 and ver(logits=z(0, 3, 50), tokens=tok[:0], uniforms=u[:0])[0].shape == (0,)
+
+
 # -- verification ---------------------------------------------------------------
 
 
