@@ -111,8 +111,9 @@ __device__ __forceinline__ double vf_weight_finite(float x, float M, const Verif
   const double h =
       fma(r, fma(r, fma(r, 0.0096181291076284772, 0.055504108664821580), 0.24022650695910071), 0.69314718055994531);
   const double c = tab.t[k & 31], w = fma(r * h, c, c);
-  const uint64_t bits = __builtin_bit_cast(uint64_t, w) + ((uint64_t)(k >> 5) << 52);
-  return __builtin_bit_cast(double, bits);
+  const uint64_t bits = __builtin_bit_cast(uint64_t, w);
+  const uint32_t high = (uint32_t)(bits >> 32) + ((k & ~31u) << 15);  // 2^n into the exponent
+  return __builtin_bit_cast(double, (uint64_t)high << 32 | (uint32_t)bits);
 }
 // With zero for what is below 2^-1000, and for M = +infinity.
 __device__ __forceinline__ double vf_weight(float x, float M, const VerifyArgs& a, const Pow2& tab) {
@@ -188,10 +189,10 @@ __global__ __launch_bounds__(VF_THREADS) void verify_stats_kernel(VerifyArgs a) 
   __shared__ int redi[4];
   __shared__ double redd[4];
   __shared__ Pow2 tab;
-  const int64_t row = blockIdx.y;
-  const int c = blockIdx.x, t = threadIdx.x;
-  if (a.ticket && row % a.n == 0 && c == 0 && t == 0) a.ticket[row / a.n] = 0;
-  if (a.lengths && row % a.n >= a.lengths[row / a.n]) return;
+  const int c = blockIdx.x, i = blockIdx.y, b = blockIdx.z, t = threadIdx.x;
+  if (a.ticket && i == 0 && c == 0 && t == 0) a.ticket[b] = 0;
+  if (a.lengths && i >= a.lengths[b]) return;
+  const int64_t row = (int64_t)b * a.n + i;
   const Row<LT> r(a, row);
   float x[RUNS][W], m = -INFINITY;
 #pragma unroll
@@ -519,7 +520,7 @@ int64_t chunks(int64_t vocab) { return nsx_cdiv(vocab + VF_VEC - 1, VF_CHUNK); }
 
 template <typename LT>
 int verify_launch(const VerifyArgs& a, hipStream_t st) {
-  const dim3 rows(a.nchunk, a.B * a.n), seqs(a.nchunk, a.B);
+  const dim3 rows(a.nchunk, a.n, a.B), seqs(a.nchunk, a.B);
   if (a.scale2 == 0.0) hipLaunchKernelGGL((verify_stats_kernel<LT, true>), rows, dim3(VF_THREADS), 0, st, a);
   else hipLaunchKernelGGL((verify_stats_kernel<LT, false>), rows, dim3(VF_THREADS), 0, st, a);
   NSX_LAUNCHED();
