@@ -19,7 +19,7 @@
 namespace {
 
 constexpr int TREE_KEYS = 32;       // keys per wave and step
-constexpr int TREE_NW = 4;          // waves of a workgroup
+constexpr int TREE_NW = 4;          // waves of a workgroup, 8 where it takes all keys
 constexpr int TREE_MAX_SPLIT = 128;  // splits of a kv head's keys: the combine kernel's lanes hold two each
 constexpr int TREE_GRID = 512;      // workgroups to fill the chip with: two on each of 256 CUs
 constexpr float LOG2E = 1.44269504088896340736f;
@@ -256,7 +256,7 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028235e3
 
 // Workgroup (kv head g, block cb of 16 NC query columns, split c of the keys). A column is a (node, query head of the
 // kv head) pair, node-major. The keys are the cache's rows from the first that any node sees, in tiles of 32, then the
-// nodes' own rows in tiles of their own; a split is a run of tiles and wave w takes every TREE_NW'th of them. Splits
+// nodes' own rows in tiles of their own; a split is a run of tiles and wave w takes every NW'th of them. Splits
 // past the present length return at once: the grid goes by ctx_max, so that it does not depend on the position.
 //
 // A tile: scores by v_mfma_f32_16x16x32_bf16, A = 16 keys x 32 dimensions, B = 32 dimensions x 16 columns, an element
@@ -277,25 +277,25 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028235e3
 // its split has some of theirs) once, as a table in LDS, and rotates its queries by it; a split with node tiles also
 // makes those tiles' rows, for its own use in LDS and, the first block of columns, for the cache's keeper in wk and wv. What
 // does not depend on the position is loaded ahead of it, and the first tiles ahead of the sines (a launch of its own for the
-// rows, and their loads where they were used, took 23 nodes 17.7 us and 13.2; now 11.4).
+// rows, and their loads where they were used, took 23 nodes 17.7 us and 13.2; ahead 11.4, with eight waves 10.7).
 //
-// Bounds: few keys, the chain of dependent loads (position, parents, rows) and the launch -- one node over 203 bf16 rows 6
+// Bounds: few keys, the chain of dependent loads (position, parents, rows) and the launch -- one node over 203 bf16 rows 5.5
 // us; many keys and few columns, their bytes -- 7 nodes over 131000 fp16 rows, 268 MB, 52 us, what a copy reaches; many
 // columns, the terms' VALU work beside the products, which the wide kernel below shares among four waves.
-template <typename KT, int NC, bool ROPE>
-__global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) {
+template <typename KT, int NC, int NW, bool ROPE>
+__global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
   using R = Rows<KT>;
-  constexpr int NT = 64 * TREE_NW, COLS = 16 * NC, KTN = R::NT;
+  constexpr int NT = 64 * NW, COLS = 16 * NC, KTN = R::NT;
   constexpr int QROW = 2 * ATTN_D + 16, OROW = ATTN_D + 4;  // bytes of a column's term, floats of a column's sums
   constexpr int QBYTES = 3 * COLS * QROW, PBYTES = TREE_KEYS * COLS * 4;
   constexpr int HALF = ATTN_D / 2, NROW = R::BYTES + 16, NBYTES = NSX_TREE_MAX_NODES * NROW;
   constexpr int TABLE = ROPE ? NSX_TREE_MAX_NODES * HALF * (int)sizeof(float2) : 0;
-  constexpr int NODES_AT = QBYTES + std::max(TREE_NW * PBYTES, TABLE);
-  constexpr int LDS = std::max(NODES_AT + (ROPE ? 2 * NBYTES : 0), TREE_NW * COLS * OROW * 4);
+  constexpr int NODES_AT = QBYTES + std::max(NW * PBYTES, TABLE);
+  constexpr int LDS = std::max(NODES_AT + (ROPE ? 2 * NBYTES : 0), NW * COLS * OROW * 4);
   // first the columns' query terms [term][column]; behind them the table, then each wave's weights of a tile (the second
   // way); behind those the node tiles' keys and values; in the end each wave's sums
   __shared__ __align__(16) uint8_t lds[LDS];
-  __shared__ float sm[TREE_NW][COLS], sl[TREE_NW][COLS];
+  __shared__ float sm[NW][COLS], sl[NW][COLS];
   __shared__ uint64_t svis[64];
   __shared__ int sdep[64];
   const int t = threadIdx.x, lane = t & 63, i16 = lane & 15, kq = lane >> 4;
@@ -330,7 +330,7 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
   }
   const int P = *a.pos;
   if (P < 0 || P > a.ctx_max) return;
-  const Tiles tl(a, P, TREE_KEYS, TREE_NW);
+  const Tiles tl(a, P, TREE_KEYS, NW);
   const int lo = tl.lo, pt = tl.cache, t0 = c * tl.per, t1 = min(tl.all, t0 + tl.per);
   if (t0 >= t1) return;
   // ROPE: the node tiles come after the loop, from LDS
@@ -565,13 +565,13 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
 
   start();
   int tile = first;
-  for (; tile < end; tile += TREE_NW) {
-    const int next = min(tile + TREE_NW, last);
+  for (; tile < end; tile += NW) {
+    const int next = min(tile + NW, last);
     take(tile, [&] { load_k(next); }, [&] { load_v(next); });
   }
   if constexpr (ROPE) {
 #pragma unroll 1
-    for (; tile < t1; tile += TREE_NW) {
+    for (; tile < t1; tile += NW) {
       node_k(tile);
       node_v(tile);
       take(tile, [] {}, [] {});
@@ -587,7 +587,7 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
   if (!__all(ok)) {
     start();
 #pragma unroll 1
-    for (int tile = first; tile < t1; tile += TREE_NW) {
+    for (int tile = first; tile < t1; tile += NW) {
       const bool in_lds = ROPE && tile >= pt;
       if (in_lds) node_k(tile);
       else load_k(tile);
@@ -657,10 +657,10 @@ __global__ __launch_bounds__(64 * TREE_NW, 2) void tree_attn_kernel(TreeArgs a) 
     const float sink = whole && a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
     float M = sink;
 #pragma unroll
-    for (int w = 0; w < TREE_NW; ++w) M = fmaxf(M, sm[w][cc]);
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, sm[w][cc]);
     float Z = whole && a.sinks ? __builtin_amdgcn_exp2f(sink - M) : 0.f, v = 0.f;
 #pragma unroll
-    for (int w = 0; w < TREE_NW; ++w) {  // (a wave without a tile has weight 0)
+    for (int w = 0; w < NW; ++w) {  // (a wave without a tile has weight 0)
       const float e = __builtin_amdgcn_exp2f(sm[w][cc] - M);
       Z = fmaf(e, sl[w][cc], Z);
       v = fmaf(e, sacc[w][cc][d], v);
@@ -1291,6 +1291,7 @@ enum { TREE_16, TREE_32, TREE_WIDE };  // kernel by the columns of its workgroup
 // Which kernel a call runs, and its grid.
 struct TreePlan {
   int kind, ncb, nsplit, keys, round;
+  bool alone;  // 16 columns, all keys: eight waves
 };
 
 // `work` counts pieces of 32 keys x 16 columns. Below 12288, twelve for each SIMD of the chip, the kernel of 16 columns has
@@ -1300,6 +1301,11 @@ struct TreePlan {
 // element has: three from 32768 pieces on (fp32, 64 nodes, 4000 keys 52.3 / 41.3 / 42.6, 8000 keys 86.4 / 64.8 / 60.0), two
 // from 49152 (8000 keys 63.1 / 52.8 / 52.6), one from 98304 (bf16, 64 nodes, 16000 keys 95.4 / 62.1 / 62.5, 32000 keys
 // 178 / 110 / 104).
+//
+// Few tiles are one workgroup's, of eight waves, rather than splits with a merge behind them: with up to 96 KB of keys, where
+// the merge costs as much as the longer way, and some more where the grid is large (us alone / split: one node of 64 / 8
+// heads, bf16, 17 tiles 9.1 / 10.0, 33 tiles 11.2 / 10.0; fp32, 11 tiles 10.6 / 10.9, 17 tiles 12.9 / 10.8; 40 nodes, fp32, 15
+// tiles 13.0 / 20.7, 21 tiles 15.5 / 18.2). Four waves do for four tiles (one node, 3 tiles, fp32 8.2, with eight 8.8).
 TreePlan tree_plan(int n_kv, int n_rep, int nodes, int64_t ctx_max, int window, int kv_dtype) {
   const int64_t cols = (int64_t)nodes * n_rep, rows = window > 0 ? std::min<int64_t>(ctx_max, window) : ctx_max;
   const int64_t work = n_kv * nsx_cdiv(cols, 16) * nsx_cdiv(rows, 32);
@@ -1314,7 +1320,8 @@ TreePlan tree_plan(int n_kv, int n_rep, int nodes, int64_t ctx_max, int window, 
   const int64_t step = wide ? 2 : TREE_NW;  // tiles that a workgroup takes at a time
   // workgroups that the chip holds at once: two of four waves a CU, or one of eight
   const int64_t fill = wide ? TREE_GRID / 2 : TREE_GRID;
-  p.nsplit = tiles <= 2 * step ? 1
+  p.alone = p.kind == TREE_16 && tiles > TREE_NW && tiles <= (terms == 3 ? 12 : 24) + (n_kv * p.ncb >= 64 ? 8 : 0);
+  p.nsplit = tiles <= 2 * step || p.alone ? 1
       : (int)std::min<int64_t>({nsx_cdiv(tiles, step), nsx_cdiv(fill, n_kv * (int64_t)p.ncb), TREE_MAX_SPLIT});
   return p;
 }
@@ -1344,10 +1351,12 @@ int tree_attn_typed(TreeArgs& a, const TreePlan& p, hipStream_t st) {
   a.keys = p.keys;
   a.round = p.round;
   const dim3 grid(a.n_kv * a.ncb, a.nsplit);
-  if (p.kind == TREE_16) {
-    hipLaunchKernelGGL((tree_attn_kernel<KT, 1, ROPE>), grid, dim3(64 * TREE_NW), 0, st, a);
+  if (p.alone) {
+    hipLaunchKernelGGL((tree_attn_kernel<KT, 1, 2 * TREE_NW, ROPE>), grid, dim3(128 * TREE_NW), 0, st, a);
+  } else if (p.kind == TREE_16) {
+    hipLaunchKernelGGL((tree_attn_kernel<KT, 1, TREE_NW, ROPE>), grid, dim3(64 * TREE_NW), 0, st, a);
   } else if (p.kind == TREE_32) {
-    hipLaunchKernelGGL((tree_attn_kernel<KT, 2, ROPE>), grid, dim3(64 * TREE_NW), 0, st, a);
+    hipLaunchKernelGGL((tree_attn_kernel<KT, 2, TREE_NW, ROPE>), grid, dim3(64 * TREE_NW), 0, st, a);
   } else {
     hipLaunchKernelGGL((tree_wide_kernel<KT, ROPE>), grid, dim3(512), 0, st, a);
   }

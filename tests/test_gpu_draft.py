@@ -69,12 +69,13 @@ def _ids(parents, dev):
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("heads", [(16, 2), (3, 3), (5, 1), (32, 2), (64, 8)], ids=lambda h: f"{h[0]}q{h[1]}kv")
 @pytest.mark.parametrize("n,kind", [(1, "chain"), (2, "tree"), (9, "tree"), (33, "tree"), (64, "chain"), (7, "roots")])
-def test_tree_attention_matches_oracle(dev, dtype, heads, n, kind):
+@pytest.mark.parametrize("ctx", [None, 9000])
+def test_tree_attention_matches_oracle(dev, dtype, heads, n, kind, ctx):
     """One to 64 nodes over caches whose length lies on, before and behind the edges of tiles (32 keys), waves (128)
-    and splits; 1 to 16 query heads per kv head."""
+    and splits; 1 to 16 query heads per kv head. The cache's capacity, little more or 9000, chooses the kernel."""
     from nurostream_amd.model.draft import tree_attn
     for pos in (0, 1, 31, 32, 33, 127, 128, 129, 300, 1025):
-        c, kv, draft, q, sinks = _state(dev, *heads, n, pos, dtype, seed=pos + n)
+        c, kv, draft, q, sinks = _state(dev, *heads, n, pos, dtype, seed=pos + n, ctx=ctx)
         parents = _parents(n, kind, seed=pos)
         s = sinks if pos % 2 else None
         out = tree_attn(q, c, draft, 0, s, 0, parents=_ids(parents, dev) if kind != "chain" else None)
@@ -238,16 +239,17 @@ def test_tree_attention_one_node_is_the_decode_attention(dev):
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-def test_masked_rows_may_hold_anything(dev, bad, dtype):
+@pytest.mark.parametrize("ctx,pos,window", [(None, 200, 40), (6000, 2000, 1500)])
+def test_masked_rows_may_hold_anything(dev, bad, dtype, ctx, pos, window):
     """NaN or infinite key and value rows of nodes that are nobody's ancestors, and of cache rows that only the
     shallower nodes' windows reach: the nodes that do not see them are as without them."""
     from nurostream_amd.model.draft import tree_attn
-    n, pos, window = 24, 200, 40
+    n = 24
     parents = _parents(n, "tree", seed=3)
     parents[1:4] = [0, 0, 0]
     _, anc = OD.lineage(parents)
     leaf = [j for j in range(1, n) if anc[:, j].sum() == 1][:3]  # leaves: only they see themselves
-    c, kv, draft, q, sinks = _state(dev, 16, 2, n, pos, dtype, seed=9)
+    c, kv, draft, q, sinks = _state(dev, 16, 2, n, pos, dtype, seed=9, ctx=ctx)
     ref = _ref(c, kv, draft, q, parents, sinks, window, pos)
     for j in leaf:
         draft.k[0][:, j] = bad
@@ -265,13 +267,14 @@ def test_masked_rows_may_hold_anything(dev, bad, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-def test_keys_of_minus_infinity_have_no_weight(dev, dtype):
+@pytest.mark.parametrize("ctx", [None, 6000])
+def test_keys_of_minus_infinity_have_no_weight(dev, dtype, ctx):
     """Keys whose scores overflow to -infinity, single ones and whole tiles and splits of them, beside others."""
     from nurostream_amd.model.draft import tree_attn
     n = 5
     parents = [-1, 0, 0, 1, 2]
     for pos, dead in ((10, range(10)), (64, range(0, 32)), (700, range(0, 640)), (700, range(3, 700, 2))):
-        c, kv, draft, q, sinks = _state(dev, 8, 2, n, pos, dtype, seed=pos)
+        c, kv, draft, q, sinks = _state(dev, 8, 2, n, pos, dtype, seed=pos, ctx=ctx)
         qr = q.reshape(n, 8, 64)
         qr[:, :, 0] = 1e20
         kv.k[0][:, :pos, 0] = 0
