@@ -88,6 +88,7 @@ struct Bf16 {
 };
 
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ b8 as_b8(v4u x) { return __builtin_bit_cast(b8, x); }
 
 // Two bf16 from the upper halves of two fp32.
@@ -110,6 +111,52 @@ __device__ __forceinline__ void split8(const float (&x)[8], v4u (&t)[NT]) {
       if (k + 1 < NT) a = below(a), b = below(b);
     }
   }
+}
+
+// Two fp16 terms of 8 fp32, each rounded to nearest: 2^-24 of an element that is at least 2^-1, 2^-25 of smaller ones.
+__device__ __forceinline__ void halves8(const float (&x)[8], v4u (&t)[2]) {
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  typedef float f2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const h2 a = __builtin_convertvector((f2{x[2 * i], x[2 * i + 1]}), h2);
+    t[0][i] = __builtin_bit_cast(uint32_t, a);
+    asm("" : "+v"(t[0][i]));  // (both halves from here, not from conversions of their own)
+    const h2 c = __builtin_bit_cast(h2, (uint32_t)t[0][i]);
+    t[1][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{x[2 * i] - (float)c[0], x[2 * i + 1] - (float)c[1]}), h2));
+  }
+}
+
+// How queries and weights meet rows of a type. fp32 and bf16 rows: three bf16 terms of each. fp16 rows, one fp16 term as
+// they are: two fp16 terms, of queries scaled by a power of two so that a column's largest lies in 2^13 .. 2^14 (its scores
+// scaled back), and of weights up to 2^15: what is 2^-14 of the largest still keeps 24 bits.
+template <typename KT>
+struct Meets {
+  static constexpr int QT = 3;
+  static constexpr float LIFT = 0.f;  // by how much the softmax's reference stays below the largest score
+  static constexpr bool SCALED = false;
+  static __device__ __forceinline__ void split(const float (&x)[8], v4u (&t)[QT]) { split8(x, t); }
+  static __device__ __forceinline__ v4f dot(const v4u& a, const v4u& b, const v4f& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(a), as_b8(b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float term(const v4u& x, int e) {
+    return __builtin_bit_cast(float, e & 1 ? x[e >> 1] & 0xffff0000u : x[e >> 1] << 16);
+  }
+};
+template <>
+struct Meets<_Float16> {
+  static constexpr int QT = 2;
+  static constexpr float LIFT = 7.f;
+  static constexpr bool SCALED = true;
+  static __device__ __forceinline__ void split(const float (&x)[8], v4u (&t)[QT]) { halves8(x, t); }
+  static __device__ __forceinline__ v4f dot(const v4u& a, const v4u& b, const v4f& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float term(const v4u& x, int e) { return nsx_h2f(e & 1 ? x[e >> 1] >> 16 : x[e >> 1] & 0xffffu); }
+};
+// The exponent that brings `most`, a column's largest |query|, into 2^13 .. 2^14.
+__device__ __forceinline__ int query_shift(float most) {
+  return most > 0.f && most < INFINITY ? 14 - max(__builtin_amdgcn_frexp_expf(most), -100) : 0;
 }
 
 // How a wave holds 32 rows of a type: K8, 8 dimensions of a key row; V4, 4 dimensions of a value row; NT, the bf16
@@ -145,7 +192,7 @@ struct Rows<float> {
 };
 template <typename KT>
 struct Rows16 {  // dimensions 32 j + 8 g .. + 7
-  static constexpr int NT = std::is_same_v<KT, Bf16> ? 1 : 2, BYTES = 2 * ATTN_D;
+  static constexpr int NT = 1, BYTES = 2 * ATTN_D;
   static __device__ __forceinline__ int dim(int j, int g, int e) { return 32 * j + 8 * g + e; }
   using K8 = v4u;
   using V4 = v2u;
@@ -259,15 +306,16 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028235e3
 // nodes' own rows in tiles of their own; a split is a run of tiles and wave w takes every NW'th of them. Splits
 // past the present length return at once: the grid goes by ctx_max, so that it does not depend on the position.
 //
-// A tile: scores by v_mfma_f32_16x16x32_bf16, A = 16 keys x 32 dimensions, B = 32 dimensions x 16 columns, an element
-// being the sum of its bf16 terms (three of an fp32 value, two of an fp16 one, exactly; of their products those of
-// 2^-22 and less are left out). Lane l's results are column l % 16 and keys 4 (l / 16) .. + 3 of each 16: the B operand
+// A tile: scores by v_mfma_f32_16x16x32_bf16 (_f16), A = 16 keys x 32 dimensions, B = 32 dimensions x 16 columns, an element
+// being the sum of its terms (`Meets`; three bf16 terms of an fp32 value, exactly; of their products those of 2^-22 and less
+// are left out). Lane l's results are column l % 16 and keys 4 (l / 16) .. + 3 of each 16: the B operand
 // of the second product as they stand, when A's lane l holds of each value row the keys of its group and dimensions
 // 4 (l % 16) ..; D then has column l % 16, dimensions 16 (l / 16) + 4 r + dt. So every row is read once by one wave, in
 // pieces of 8 or 16 bytes, and turned into terms once for the wave's 16 NC columns, whose own terms lie in LDS.
 //
 // The softmax's reference m only moves (and the sums are only rescaled) when a tile has a score beyond 2^8 times it:
-// weights stay below 2^8, a sum of 2^31 of them below 2^39. So a tile mostly needs no exchange between lanes.
+// weights stay below 2^8 (2^15 over fp16 rows, whose reference lies 2^7 below), a sum of 2^31 of them below 2^46. So a tile
+// mostly needs no exchange between lanes.
 //
 // A key with weight zero takes no part whatever its value row holds (0 * NaN would be NaN): a wave whose sums are not
 // finite at the end goes through its tiles again, with products in fp32 and values added one key at a time under their
@@ -280,14 +328,15 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028235e3
 // rows, and their loads where they were used, took 23 nodes 17.7 us and 13.2; ahead 11.4, with eight waves 10.7).
 //
 // Bounds: few keys, the chain of dependent loads (position, parents, rows) and the launch -- one node over 203 bf16 rows 5.5
-// us; many keys and few columns, their bytes -- 7 nodes over 131000 fp16 rows, 268 MB, 52 us, what a copy reaches; many
+// us; many keys and few columns, their bytes -- 7 nodes over 131000 fp16 rows, 268 MB, 49 us, 5.4 TB/s; many
 // columns, the terms' VALU work beside the products, which the wide kernel below shares among four waves.
 template <typename KT, int NC, int NW, bool ROPE>
 __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
   using R = Rows<KT>;
-  constexpr int NT = 64 * NW, COLS = 16 * NC, KTN = R::NT;
+  using Q = Meets<KT>;
+  constexpr int NT = 64 * NW, COLS = 16 * NC, KTN = R::NT, QT = Q::QT;
   constexpr int QROW = 2 * ATTN_D + 16, OROW = ATTN_D + 4;  // bytes of a column's term, floats of a column's sums
-  constexpr int QBYTES = 3 * COLS * QROW, PBYTES = TREE_KEYS * COLS * 4;
+  constexpr int QBYTES = QT * COLS * QROW, PBYTES = TREE_KEYS * COLS * 4;
   constexpr int HALF = ATTN_D / 2, NROW = R::BYTES + 16, NBYTES = NSX_TREE_MAX_NODES * NROW;
   constexpr int TABLE = ROPE ? NSX_TREE_MAX_NODES * HALF * (int)sizeof(float2) : 0;
   constexpr int NODES_AT = QBYTES + std::max(NW * PBYTES, TABLE);
@@ -296,6 +345,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
   // way); behind those the node tiles' keys and values; in the end each wave's sums
   __shared__ __align__(16) uint8_t lds[LDS];
   __shared__ float sm[NW][COLS], sl[NW][COLS];
+  __shared__ float sunit[COLS];  // scaled queries: what a column's scores are in units of
   __shared__ uint64_t svis[64];
   __shared__ int sdep[64];
   const int t = threadIdx.x, lane = t & 63, i16 = lane & 15, kq = lane >> 4;
@@ -419,16 +469,32 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) qx[e] *= a.scale2;
-    v4u tm[3];
-    split8(qx, tm);
+    if constexpr (Q::SCALED) {
+      float most = 0.f;
 #pragma unroll
-    for (int k = 0; k < 3; ++k) *(v4u*)&lds[(k * COLS + qc) * QROW + (4 * qj + qg) * 16] = tm[k];
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(qx[e]));
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor(most, o, 64));  // (a column's eight threads)
+      const int up = query_shift(most);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) qx[e] = ldexpf(qx[e], up);
+      if (t % 8 == 0) sunit[qc] = ldexpf(1.f, -up);
+    }
+    v4u tm[QT];
+    Q::split(qx, tm);
+#pragma unroll
+    for (int k = 0; k < QT; ++k) *(v4u*)&lds[(k * COLS + qc) * QROW + (4 * qj + qg) * 16] = tm[k];
   }
   nsx_lds_barrier();
   const int q0 = i16 * QROW + kq * 16;
   auto query = [&](int k, int ct, int j) { return *(const v4u*)&lds[q0 + (k * COLS + 16 * ct) * QROW + 64 * j]; };
   // a column's node: what it sees of the nodes, its first visible row of the cache
   auto node_of = [&](int ct) { return min(col0 + 16 * ct + i16, ncol - 1) / a.n_rep; };
+  float unit[NC];
+  if constexpr (Q::SCALED) {
+#pragma unroll
+    for (int ct = 0; ct < NC; ++ct) unit[ct] = sunit[16 * ct + i16];
+  }
   int deepest = 0;  // the last of the columns' first rows
   if (a.window > 0) {
 #pragma unroll
@@ -452,6 +518,12 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
   };
   // scores in powers of two -> weights; what a column does not see has none
   auto weights = [&](int tile, v4f (&s)[NC][2]) {
+    if constexpr (Q::SCALED) {
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) s[ct][n] *= unit[ct];
+    }
     const bool own = tile >= pt;
     const int r0 = own ? (tile - pt) * TREE_KEYS : lo + tile * TREE_KEYS;
     if (own) {
@@ -484,13 +556,13 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
       mx[ct] = fmaxf(s[ct][0][0], s[ct][0][1]);
 #pragma unroll
       for (int e = 2; e < 8; ++e) mx[ct] = fmaxf(mx[ct], s[ct][e >> 2][e & 3]);
-      move = move || mx[ct] > m[ct] + 8.f;
+      move = move || mx[ct] > m[ct] + (8.f + Q::LIFT);
     }
     if (__any(move)) {
 #pragma unroll
       for (int ct = 0; ct < NC; ++ct) {
         float mn = fmaxf(mx[ct], __shfl_xor(mx[ct], 16, 64));
-        mn = fmaxf(m[ct], fmaxf(mn, __shfl_xor(mn, 32, 64)));
+        mn = fmaxf(m[ct], fmaxf(mn, __shfl_xor(mn, 32, 64)) - Q::LIFT);
         const float corr = __builtin_amdgcn_exp2f(m[ct] - mn);  // (first tile: of nothing)
         m[ct] = mn;
         l[ct] *= corr;
@@ -523,28 +595,28 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int ct = 0; ct < NC; ++ct) {
-          v4u q[3];
+          v4u q[QT];
 #pragma unroll
-          for (int k = 0; k < 3; ++k) q[k] = query(k, ct, j);
+          for (int k = 0; k < QT; ++k) q[k] = query(k, ct, j);
 #pragma unroll
-          for (int o = 2; o >= 0; --o)  // (the small products first)
+          for (int o = QT - 1; o >= 0; --o)  // (the small products first)
 #pragma unroll
             for (int k = 0; k <= o; ++k)
               if (o - k < KTN) {
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
-                  s[ct][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(kt_[kt][j][o - k]), as_b8(q[k]), s[ct][kt], 0, 0, 0);
+                  s[ct][kt] = Q::dot(kt_[kt][j][o - k], q[k], s[ct][kt]);
               }
         }
     }
     weights(tile, s);
-    v4u pw[NC][3];
+    v4u pw[NC][QT];
 #pragma unroll
     for (int ct = 0; ct < NC; ++ct) {
       float x[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = s[ct][e >> 2][e & 3];
-      split8(x, pw[ct]);
+      Q::split(x, pw[ct]);
     }
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) {
@@ -552,13 +624,12 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
       value_terms<KT>(vr, dt, vt);
       if (dt == 3) next_v();
 #pragma unroll
-      for (int o = 2; o >= 0; --o)
+      for (int o = QT - 1; o >= 0; --o)
 #pragma unroll
         for (int k = 0; k <= o; ++k)
           if (o - k < KTN) {
 #pragma unroll
-            for (int ct = 0; ct < NC; ++ct)
-              acc[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(vt[o - k]), as_b8(pw[ct][k]), acc[ct][dt], 0, 0, 0);
+            for (int ct = 0; ct < NC; ++ct) acc[ct][dt] = Q::dot(vt[o - k], pw[ct][k], acc[ct][dt]);
           }
     }
   };
@@ -596,13 +667,14 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
       for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const v4u qa = query(0, ct, j), qb = query(1, ct, j), qc = query(2, ct, j);
-          auto term = [](const v4u& x, int e) {
-            return __builtin_bit_cast(float, e & 1 ? x[e >> 1] & 0xffff0000u : x[e >> 1] << 16);
-          };
+          v4u qt[QT];
+#pragma unroll
+          for (int k = 0; k < QT; ++k) qt[k] = query(k, ct, j);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float q = term(qa, e) + (term(qb, e) + term(qc, e));
+            float q = Q::term(qt[QT - 1], e);
+#pragma unroll
+            for (int k = QT - 2; k >= 0; --k) q += Q::term(qt[k], e);
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
               s[ct][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(R::k(kr[kt][j], e), q, s[ct][kt], 0, 0, 0);
@@ -697,7 +769,8 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
 template <typename KT, bool ROPE>
 __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
   using R = Rows<KT>;
-  constexpr int KTN = R::NT, NC = 2, CW = 4, NG = 2, COLS = 16 * NC * CW;
+  using Q = Meets<KT>;
+  constexpr int KTN = R::NT, QT = Q::QT, NC = 2, CW = 4, NG = 2, COLS = 16 * NC * CW;
   constexpr int TPP = KTN == 1 ? 2 : 1, KEYS = 32 * TPP;  // 16-bit rows: two tiles a phase, as their phases are short
   constexpr int KF = TPP * 4 * KTN, VF = TPP * 4 * KTN;   // operands (64 lanes x 16 bytes) of a tile's keys and values
   constexpr int GROUP = (KF + VF) * 1024, OROW = ATTN_D + 4;
@@ -812,10 +885,7 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
           for (int p = 0; p < 2; ++p) {
             float f[2];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              if constexpr (std::is_same_v<KT, float>) f[q] = __builtin_bit_cast(float, (uint32_t)vr[it][2 * p + q][b]);
-              else f[q] = nsx_h2f(b ? vr[it][2 * p + q] >> 16 : vr[it][2 * p + q] & 0xffffu);
-            }
+            for (int q = 0; q < 2; ++q) f[q] = __builtin_bit_cast(float, (uint32_t)vr[it][2 * p + q][b]);
 #pragma unroll
             for (int k = 0; k < KTN; ++k) {
               x[k][p] = top2(f[0], f[1]);
@@ -870,7 +940,8 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
       nsx_lds_barrier();
     }
   }
-  v4u q[NC][2][3];
+  v4u q[NC][2][QT];
+  float unit[NC];  // scaled queries: what a column's scores are in units of
 #pragma unroll
   for (int ct = 0; ct < NC; ++ct) {
     if constexpr (ROPE) {
@@ -883,11 +954,28 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
         qx[ct][0][e] = fmaf(x0, w.x, -(x1 * w.y)), qx[ct][1][e] = fmaf(x1, w.x, x0 * w.y);
       }
     }
+    int up = 0;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int e = 0; e < 8; ++e) qx[ct][j][e] *= a.scale2;
-      split8(qx[ct][j], q[ct][j]);
+    if constexpr (Q::SCALED) {
+      float most = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(qx[ct][j][e]));
+      most = fmaxf(most, __shfl_xor(most, 16, 64));
+      up = query_shift(fmaxf(most, __shfl_xor(most, 32, 64)));
+      unit[ct] = ldexpf(1.f, -up);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if constexpr (Q::SCALED) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) qx[ct][j][e] = ldexpf(qx[ct][j][e], up);
+      }
+      Q::split(qx[ct][j], q[ct][j]);
     }
   }
   nsx_lds_barrier();
@@ -907,7 +995,7 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
   float m[NC], l[NC];
   v4f acc[NC][4];  // [dimension's half, parity]
   v4f s[NC][2 * TPP];
-  v4u pw[NC][TPP][3];
+  v4u pw[NC][TPP][QT];
   auto start = [&] {
 #pragma unroll
     for (int ct = 0; ct < NC; ++ct) {
@@ -920,6 +1008,12 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
   // scores in powers of two -> weights, 16 keys each of N; r0: the first key's row (own: of the nodes)
   auto weights = [&](auto& x, auto n_tag, bool own, int r0) {
     constexpr int N = decltype(n_tag)::value;
+    if constexpr (Q::SCALED) {
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+        for (int n = 0; n < N; ++n) x[ct][n] *= unit[ct];
+    }
     if (own) {
 #pragma unroll
       for (int ct = 0; ct < NC; ++ct)
@@ -947,13 +1041,13 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
       mx[ct] = fmaxf(x[ct][0][0], x[ct][0][1]);
 #pragma unroll
       for (int e = 2; e < 4 * N; ++e) mx[ct] = fmaxf(mx[ct], x[ct][e >> 2][e & 3]);
-      move = move || mx[ct] > m[ct] + 8.f;
+      move = move || mx[ct] > m[ct] + (8.f + Q::LIFT);
     }
     if (__any(move)) {
 #pragma unroll
       for (int ct = 0; ct < NC; ++ct) {
         float mn = fmaxf(mx[ct], __shfl_xor(mx[ct], 16, 64));
-        mn = fmaxf(m[ct], fmaxf(mn, __shfl_xor(mn, 32, 64)));
+        mn = fmaxf(m[ct], fmaxf(mn, __shfl_xor(mn, 32, 64)) - Q::LIFT);
         const float corr = __builtin_amdgcn_exp2f(m[ct] - mn);  // (first tile: of nothing)
         m[ct] = mn;
         l[ct] *= corr;
@@ -979,7 +1073,7 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
 
   // The products of a tile step by step, an operand set each: the values of tile i - 1 (the first time: zeros under no
   // weights), then the keys of tile i (the last time: what is there, unused). A step's operands are read AHEAD steps early.
-  constexpr int STEPS = 8 * TPP, AHEAD = KTN == 1 ? 4 : KTN == 2 ? 2 : 1;
+  constexpr int STEPS = 8 * TPP, AHEAD = KTN == 1 ? 4 : 1;
   auto products = [&] {
     v4u x[AHEAD + 1][KTN];
     auto read = [&](int n) {
@@ -987,9 +1081,6 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
       for (int k = 0; k < KTN; ++k)
         x[n % (AHEAD + 1)][k] =
             *(const v4u*)((n < 4 * TPP ? vl + n * KTN * 1024 : kl + (n - 4 * TPP) * KTN * 1024) + k * 1024 + lane * 16);
-    };
-    auto dot = [](const v4u& x, const v4u& y, const v4f& c) {
-      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(x), as_b8(y), c, 0, 0, 0);
     };
 #pragma unroll
     for (int ct = 0; ct < NC; ++ct)
@@ -1003,27 +1094,27 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
       const v4u(&y)[KTN] = x[n % (AHEAD + 1)];
       if (n < 4 * TPP) {
 #pragma unroll
-        for (int o = 2; o >= 0; --o)  // (the small products first)
+        for (int o = QT - 1; o >= 0; --o)  // (the small products first)
 #pragma unroll
           for (int k = 0; k <= o; ++k)
             if (o - k < KTN) {
 #pragma unroll
-              for (int ct = 0; ct < NC; ++ct) acc[ct][n % 4] = dot(y[o - k], pw[ct][n / 4][k], acc[ct][n % 4]);
+              for (int ct = 0; ct < NC; ++ct) acc[ct][n % 4] = Q::dot(y[o - k], pw[ct][n / 4][k], acc[ct][n % 4]);
             }
       } else {
         const int kn = n - 4 * TPP;
 #pragma unroll
-        for (int o = 2; o >= 0; --o)
+        for (int o = QT - 1; o >= 0; --o)
 #pragma unroll
           for (int k = 0; k <= o; ++k)
             if (o - k < KTN) {
 #pragma unroll
-              for (int ct = 0; ct < NC; ++ct) s[ct][kn / 2] = dot(y[o - k], q[ct][kn % 2][k], s[ct][kn / 2]);
+              for (int ct = 0; ct < NC; ++ct) s[ct][kn / 2] = Q::dot(y[o - k], q[ct][kn % 2][k], s[ct][kn / 2]);
             }
       }
     }
     // the order above, kept by the scheduler: LDS reads (0x100) ahead of the products (0x8)
-    constexpr int PRODUCTS = NC * (KTN == 3 ? 6 : KTN == 2 ? 5 : 3);
+    constexpr int PRODUCTS = NC * (KTN == 3 ? 6 : QT);
     __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * KTN, 0);
 #pragma unroll
     for (int n = 0; n < STEPS; ++n) {
@@ -1036,7 +1127,10 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
 #pragma unroll
   for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
-    for (int u = 0; u < TPP; ++u) pw[ct][u][0] = pw[ct][u][1] = pw[ct][u][2] = v4u{0, 0, 0, 0};
+    for (int u = 0; u < TPP; ++u) {
+#pragma unroll
+      for (int k = 0; k < QT; ++k) pw[ct][u][k] = v4u{0, 0, 0, 0};
+    }
 #pragma unroll
   for (int n = 0; n < VF / CW; ++n) *(v4u*)(vl + (cw + CW * n) * 1024 + lane * 16) = v4u{0, 0, 0, 0};
   store_k();
@@ -1068,7 +1162,7 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
           float x[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = s[ct][2 * u + (e >> 2)][e & 3];
-          split8(x, pw[ct][u]);
+          Q::split(x, pw[ct][u]);
         }
     }
     phase();
@@ -1102,11 +1196,10 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
           for (int e = 0; e < 8; ++e)
 #pragma unroll
             for (int ct = 0; ct < NC; ++ct) {
-              auto term = [&](int k) {
-                const uint32_t w = q[ct][j][k][e >> 1];
-                return __builtin_bit_cast(float, e & 1 ? w & 0xffff0000u : w << 16);
-              };
-              x[ct][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(R::k(kk, e), term(0) + (term(1) + term(2)), x[ct][kt], 0, 0, 0);
+              float qe = Q::term(q[ct][j][QT - 1], e);
+#pragma unroll
+              for (int k = QT - 2; k >= 0; --k) qe += Q::term(q[ct][j][k], e);
+              x[ct][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(R::k(kk, e), qe, x[ct][kt], 0, 0, 0);
             }
         }
       weights(x, std::integral_constant<int, 2>{}, own, r0);
@@ -1298,9 +1391,9 @@ struct TreePlan {
 // the most workgroups and the shortest way through one (us for 16 / 32 / 128 columns at 64 / 8 heads, fp32, 4000 keys:
 // 16 nodes 22.9 / 23.7 / 26.3, 32 nodes 30.1 / 27.6 / 31.0; bf16 17.6 / 20.2 / 24.6 and 21.7 / 21.2 / 27.5). Past it, more
 // than 64 columns go to the wide kernel once its sharing of terms outweighs its longer way, the sooner the more terms an
-// element has: three from 32768 pieces on (fp32, 64 nodes, 4000 keys 52.3 / 41.3 / 42.6, 8000 keys 86.4 / 64.8 / 60.0), two
-// from 49152 (8000 keys 63.1 / 52.8 / 52.6), one from 98304 (bf16, 64 nodes, 16000 keys 95.4 / 62.1 / 62.5, 32000 keys
-// 178 / 110 / 104).
+// element has: three from 32768 pieces on (fp32, 64 nodes, 4000 keys 52.3 / 41.3 / 42.6, 8000 keys 86.4 / 64.8 / 60.0), one
+// from 98304 (64 nodes, 16000 keys: bf16 95.0 / 59.8 / 60.6, fp16 94.9 / 57.2 / 54.8; 32000 keys 177 / 104 / 101 and 177 / 98 /
+// 88; 8000 keys 52.7 / 36.8 / 42.5 and 53.2 / 36.0 / 40.2).
 //
 // Few tiles are one workgroup's, of eight waves, rather than splits with a merge behind them: with up to 96 KB of keys, where
 // the merge costs as much as the longer way, and some more where the grid is large (us alone / split: one node of 64 / 8
@@ -1309,7 +1402,7 @@ struct TreePlan {
 TreePlan tree_plan(int n_kv, int n_rep, int nodes, int64_t ctx_max, int window, int kv_dtype) {
   const int64_t cols = (int64_t)nodes * n_rep, rows = window > 0 ? std::min<int64_t>(ctx_max, window) : ctx_max;
   const int64_t work = n_kv * nsx_cdiv(cols, 16) * nsx_cdiv(rows, 32);
-  const int terms = kv_dtype == NSX_DT_F32 ? 3 : kv_dtype == NSX_DT_F16 ? 2 : 1;
+  const int terms = kv_dtype == NSX_DT_F32 ? 3 : 1;
   TreePlan p;
   p.kind = work < 12288 ? TREE_16 : cols > 64 && work * terms >= 98304 ? TREE_WIDE : TREE_32;
   const bool wide = p.kind == TREE_WIDE;

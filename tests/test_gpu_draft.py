@@ -287,6 +287,29 @@ def test_keys_of_minus_infinity_have_no_weight(dev, dtype, ctx):
         assert rel_max(to_np(out), ref) < TOL, pos
 
 
+@pytest.mark.parametrize("ctx", [None, 6000, 70000])
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_queries_of_any_size(dev, dtype, ctx):
+    """Small queries over large keys, large ones over small keys (subnormal ones in fp16), a node's queries of zeros, of
+    differing sizes by head, and values of any size: each output beside its own largest value."""
+    from nurostream_amd.model.draft import tree_attn
+    n, pos, heads = 40, 150, (32, 2)
+    for up in (-20, 18):
+        c, kv, draft, q, sinks = _state(dev, *heads, n, pos, dtype, seed=up + 50, ctx=ctx)
+        parents = _parents(n, "tree", seed=2)
+        size = 2.0 ** torch.arange(32, device=dev).remainder(7).neg()  # heads by 2^0 .. 2^-6
+        q = (q.reshape(n, 32, 64) * size[:, None] * 2.0 ** up).reshape(n, -1).contiguous()
+        q[3] = 0
+        for t, m in ((kv.k[0], pos), (draft.k[0], n)):
+            t[:, :m] = (t[:, :m].float() * 2.0 ** (-18 if up > 0 else 12)).to(t.dtype)
+        for t, m in ((kv.v[0], pos), (draft.v[0], n)):
+            t[:, :m] = (t[:, :m].float() * 2.0 ** (-up // 2)).to(t.dtype)
+        ref = _ref(c, kv, draft, q, parents, sinks, 0, pos)
+        out = to_np(tree_attn(q, c, draft, 0, sinks, 0, parents=_ids(parents, dev)))
+        for h in range(32):
+            assert rel_max(out[:, h], ref[:, h]) < TOL, (up, h)
+
+
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 def test_wide_ranges_in_one_row(dev, dtype):
     """Value rows with elements 2^20 times their others (2^10 in fp16) and keys whose large element meets a query's
