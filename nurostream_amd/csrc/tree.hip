@@ -761,8 +761,10 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
 //
 // Bound by the phases' shared issue: 64 nodes over 65536 bf16 keys (64 / 8 heads, three products a term pair: 206 GFLOP of
 // bf16) 184 us, 1120 TFLOP/s, what a large library product reaches here (1108); 64 nodes over 6000 fp32 keys (six products)
-// 48 us, 16 over 16384 37. Both groups in one phase 188 for an earlier 160, no offset between them 184; scheduler groups,
-// one barrier a tile, 32 x 32 products, two workgroups of four waves: all within 5 % or slower.
+// 48 us, 16 over 16384 38; 64 over 32000 fp16 keys (two) 83. Of an iteration's 5450 cycles over fp32 rows the products take
+// 1870 and the rest 2530, the VALU issuing an instruction in 8 beside the other group's products. Both groups in one phase
+// 188 for an earlier 160, no offset between them 184; scheduler groups, one barrier a tile, 32 x 32 products, two workgroups of
+// four waves: all within 5 % or slower.
 //
 // ROPE as above, the table where the first tiles come afterwards; a split with nodes' rows writes them beside the cache
 // and loads them back as it does the cache's.
