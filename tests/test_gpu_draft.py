@@ -873,6 +873,22 @@ def test_generate_with_drafts_is_generate(dev, tmp_path):
         list(ns.generate([1], drafts=64))
 
 
+def test_generate_ends_with_the_context(dev, tmp_path, monkeypatch):
+    """A context that ends before max_tokens, in the middle of a pass, at the prompt's end and before it."""
+    import dataclasses
+    ns, _ = _tiny(tmp_path, dev)
+    small = dataclasses.replace(ns.model.attn_config(), context_length=20)
+    monkeypatch.setattr(ns.model, "attn_config", lambda: small)
+    for prompt in ([5, 6, 7] * 3, [5, 6] * 10, [9]):
+        want = list(ns.generate(prompt, max_tokens=50))
+        assert len(want) == 21 - len(prompt)
+        for drafts in (1, 7, 40):
+            assert list(ns.generate(prompt, max_tokens=50, drafts=drafts)) == want
+    for kw in ({}, dict(drafts=3)):
+        with pytest.raises(ValueError):
+            list(ns.generate([5] * 21, max_tokens=2, **kw))
+
+
 def test_generate_sampled_and_16_bit(dev, tmp_path):
     """Sampling with drafts and 16-bit caches runs to its end, the same for the same seed."""
     ns, _ = _tiny(tmp_path, dev)
