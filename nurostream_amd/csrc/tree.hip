@@ -113,7 +113,8 @@ __device__ __forceinline__ void split8(const float (&x)[8], v4u (&t)[NT]) {
   }
 }
 
-// Two fp16 terms of 8 fp32, each rounded to nearest: 2^-24 of an element that is at least 2^-1, 2^-25 of smaller ones.
+// Two fp16 terms of 8 fp32, each rounded to nearest. They miss an element of at least 2^-2 by 2^-23 of itself (half a step
+// of 2^-24 at 2^-1 .. 1), a smaller one by 2^-25 whatever its size: half of fp16's least number.
 __device__ __forceinline__ void halves8(const float (&x)[8], v4u (&t)[2]) {
   typedef _Float16 h2 __attribute__((ext_vector_type(2)));
   typedef float f2 __attribute__((ext_vector_type(2)));
@@ -128,8 +129,12 @@ __device__ __forceinline__ void halves8(const float (&x)[8], v4u (&t)[2]) {
 }
 
 // How queries and weights meet rows of a type. fp32 and bf16 rows: three bf16 terms of each. fp16 rows, one fp16 term as
-// they are: two fp16 terms, of queries scaled by a power of two so that a column's largest lies in 2^13 .. 2^14 (its scores
-// scaled back), and of weights up to 2^15: what is 2^-14 of the largest still keeps 24 bits.
+// they are: two fp16 terms, of weights up to 2^15 and of queries, scaled by a power of two so that a column's largest lies in
+// 2^13 .. 2^14 (its scores scaled back). Elements down to 2^-16 of the largest keep 23 bits, smaller ones lose some. What a
+// column loses that way may change a score by no more than 2^-20, a weight by 2^-20.5 of itself, over any fp16 keys
+// (`query_lost`: a column whose largest is below 8 does not lose it by one small element, and one element in 27000 of normal
+// ones is that small); where it could, the scores are fp32 products of the queries as they are, a workgroup's (the wide
+// kernel: a wave's) columns at a time.
 template <typename KT>
 struct Meets {
   static constexpr int QT = 3;
@@ -158,6 +163,19 @@ struct Meets<_Float16> {
 __device__ __forceinline__ int query_shift(float most) {
   return most > 0.f && most < INFINITY ? 14 - max(__builtin_amdgcn_frexp_expf(most), -100) : 0;
 }
+// What two fp16 terms miss of 8 scaled queries beyond 2^-23 of each (infinite and NaN ones: NaN).
+__device__ __forceinline__ float query_lost(const float (&x)[8], const v4u (&t)[2]) {
+  float lost = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float r = fabsf((x[e] - Meets<_Float16>::term(t[0], e)) - Meets<_Float16>::term(t[1], e));
+    lost += r <= 0x1p-23f * fabsf(x[e]) ? 0.f : r;
+  }
+  return lost;
+}
+// Whether a column's queries, having lost so much when scaled by 2^up, need fp32 products: over keys up to 65504 < 2^16 a
+// score is off by up to 2^16 times that, of which 2^-20 is let pass.
+__device__ __forceinline__ bool query_spread(float lost, int up) { return !(ldexpf(lost, -up) <= 0x1p-36f); }
 
 // How a wave holds 32 rows of a type: K8, 8 dimensions of a key row; V4, 4 dimensions of a value row; NT, the bf16
 // terms that an element takes exactly.
@@ -346,6 +364,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
   __shared__ __align__(16) uint8_t lds[LDS];
   __shared__ float sm[NW][COLS], sl[NW][COLS];
   __shared__ float sunit[COLS];  // scaled queries: what a column's scores are in units of
+  __shared__ int sspread[NW];    // and whether a wave's columns need fp32 products
   __shared__ uint64_t svis[64];
   __shared__ int sdep[64];
   const int t = threadIdx.x, lane = t & 63, i16 = lane & 15, kq = lane >> 4;
@@ -457,6 +476,11 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
       nsx_lds_barrier();
     }
   }
+  bool spread = false;
+  auto leave = [&](const v4u (&tm)[QT]) {
+#pragma unroll
+    for (int k = 0; k < QT; ++k) *(v4u*)&lds[(k * COLS + qc) * QROW + (4 * qj + qg) * 16] = tm[k];
+  };
   if (qc < COLS) {
     if constexpr (ROPE) {
 #pragma unroll
@@ -469,23 +493,49 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) qx[e] *= a.scale2;
+    v4u tm[QT];
     if constexpr (Q::SCALED) {
-      float most = 0.f;
+      float most = 0.f, x[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(qx[e]));
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor(most, o, 64));  // (a column's eight threads)
       const int up = query_shift(most);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) qx[e] = ldexpf(qx[e], up);
+      for (int e = 0; e < 8; ++e) x[e] = ldexpf(qx[e], up);
       if (t % 8 == 0) sunit[qc] = ldexpf(1.f, -up);
-    }
-    v4u tm[QT];
-    Q::split(qx, tm);
+      Q::split(x, tm);
+      float lost = query_lost(x, tm);
 #pragma unroll
-    for (int k = 0; k < QT; ++k) *(v4u*)&lds[(k * COLS + qc) * QROW + (4 * qj + qg) * 16] = tm[k];
+      for (int o = 1; o < 8; o <<= 1) lost += __shfl_xor(lost, o, 64);
+      spread = query_spread(lost, up);
+    } else {
+      Q::split(qx, tm);
+    }
+    leave(tm);
+  }
+  if constexpr (Q::SCALED) {
+    const int any = __any(spread);
+    if (lane == 0) sspread[wave] = any;
   }
   nsx_lds_barrier();
+  bool exact = false;  // the queries are in LDS as fp32 values, four in place of each term
+  if constexpr (Q::SCALED) {
+    int some = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) some |= sspread[w];
+    exact = __builtin_amdgcn_readfirstlane(some) != 0;
+    if (exact) {
+      if (qc < COLS) {
+        v4u x[QT];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e >> 2][e & 3] = __builtin_bit_cast(uint32_t, qx[e]);
+        leave(x);
+        if (t % 8 == 0) sunit[qc] = 1.f;
+      }
+      nsx_lds_barrier();
+    }
+  }
   const int q0 = i16 * QROW + kq * 16;
   auto query = [&](int k, int ct, int j) { return *(const v4u*)&lds[q0 + (k * COLS + 16 * ct) * QROW + 64 * j]; };
   // a column's node: what it sees of the nodes, its first visible row of the cache
@@ -581,10 +631,34 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
     }
   };
 
+  // scores of the keys in kr by fp32 products
+  auto scores32 = [&](v4f (&s)[NC][2]) {
+#pragma unroll
+    for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        v4u qt[QT];
+#pragma unroll
+        for (int k = 0; k < QT; ++k) qt[k] = query(k, ct, j);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float q = Q::term(qt[QT - 1], e);
+#pragma unroll
+          for (int k = QT - 2; k >= 0; --k) q += Q::term(qt[k], e);
+          if (exact) q = __builtin_bit_cast(float, (uint32_t)qt[e >> 2][e & 3]);
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt)
+            s[ct][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(R::k(kr[kt][j], e), q, s[ct][kt], 0, 0, 0);
+        }
+      }
+  };
   // a tile whose rows are in kr and vr, the next one's loads on their way as soon as they are free
   auto take = [&](int tile, auto next_k, auto next_v) {
     v4f s[NC][2] = {};
-    {
+    if (Q::SCALED && exact) {
+      scores32(s);
+      next_k();
+    } else {
       v4u kt_[2][2][KTN];
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
@@ -663,23 +737,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
       if (in_lds) node_k(tile);
       else load_k(tile);
       v4f s[NC][2] = {};
-#pragma unroll
-      for (int ct = 0; ct < NC; ++ct)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          v4u qt[QT];
-#pragma unroll
-          for (int k = 0; k < QT; ++k) qt[k] = query(k, ct, j);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float q = Q::term(qt[QT - 1], e);
-#pragma unroll
-            for (int k = QT - 2; k >= 0; --k) q += Q::term(qt[k], e);
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
-              s[ct][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(R::k(kr[kt][j], e), q, s[ct][kt], 0, 0, 0);
-          }
-        }
+      scores32(s);
       weights(tile, s);
 #pragma unroll
       for (int ct = 0; ct < NC; ++ct)
@@ -944,6 +1002,7 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
   }
   v4u q[NC][2][QT];
   float unit[NC];  // scaled queries: what a column's scores are in units of
+  bool exact = false;  // q holds the queries as fp32 values, four in place of each term
 #pragma unroll
   for (int ct = 0; ct < NC; ++ct) {
     if constexpr (ROPE) {
@@ -956,28 +1015,46 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
         qx[ct][0][e] = fmaf(x0, w.x, -(x1 * w.y)), qx[ct][1][e] = fmaf(x1, w.x, x0 * w.y);
       }
     }
-    int up = 0;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int e = 0; e < 8; ++e) qx[ct][j][e] *= a.scale2;
     if constexpr (Q::SCALED) {
-      float most = 0.f;
+      float most = 0.f, lost = 0.f;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(qx[ct][j][e]));
       most = fmaxf(most, __shfl_xor(most, 16, 64));
-      up = query_shift(fmaxf(most, __shfl_xor(most, 32, 64)));
+      const int up = query_shift(fmaxf(most, __shfl_xor(most, 32, 64)));
       unit[ct] = ldexpf(1.f, -up);
-    }
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      if constexpr (Q::SCALED) {
+      for (int j = 0; j < 2; ++j) {
+        float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) qx[ct][j][e] = ldexpf(qx[ct][j][e], up);
+        for (int e = 0; e < 8; ++e) x[e] = ldexpf(qx[ct][j][e], up);
+        Q::split(x, q[ct][j]);
+        lost += query_lost(x, q[ct][j]);
       }
-      Q::split(qx[ct][j], q[ct][j]);
+      lost += __shfl_xor(lost, 16, 64);
+      lost += __shfl_xor(lost, 32, 64);
+      exact = exact || query_spread(lost, up);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) Q::split(qx[ct][j], q[ct][j]);
+    }
+  }
+  if constexpr (Q::SCALED) {
+    exact = __any(exact);
+    if (exact) {
+#pragma unroll
+      for (int ct = 0; ct < NC; ++ct) {
+        unit[ct] = 1.f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) q[ct][j][e >> 2][e & 3] = __builtin_bit_cast(uint32_t, qx[ct][j][e]);
+      }
     }
   }
   nsx_lds_barrier();
@@ -1067,6 +1144,13 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
       }
     }
   };
+  // query e of 8, for fp32 products
+  auto query32 = [&](int ct, int j, int e) {
+    float x = Q::term(q[ct][j][QT - 1], e);
+#pragma unroll
+    for (int k = QT - 2; k >= 0; --k) x += Q::term(q[ct][j][k], e);
+    return exact ? __builtin_bit_cast(float, (uint32_t)q[ct][j][e >> 2][e & 3]) : x;
+  };
   auto phase = [] {
     __builtin_amdgcn_sched_barrier(0);
     nsx_lds_barrier();
@@ -1125,6 +1209,23 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
     }
   };
 
+  // the scores of the tile in LDS by fp32 products, in place of those above
+  auto scores32 = [&] {
+    if constexpr (Q::SCALED) {
+#pragma unroll
+      for (int n = 0; n < 4 * TPP; ++n) {
+        const auto x = __builtin_bit_cast(typename R::K8, *(const v4u*)(kl + n * 1024 + lane * 16));
+#pragma unroll
+        for (int ct = 0; ct < NC; ++ct) {
+          if (n % 2 == 0) s[ct][n / 2] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            s[ct][n / 2] = __builtin_amdgcn_mfma_f32_16x16x4f32(R::k(x, e), query32(ct, n % 2, e), s[ct][n / 2], 0, 0, 0);
+        }
+      }
+    }
+  };
+
   start();
 #pragma unroll
   for (int ct = 0; ct < NC; ++ct)
@@ -1146,6 +1247,7 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
       __builtin_amdgcn_s_setprio(1);
       products();
       __builtin_amdgcn_s_setprio(0);
+      if (Q::SCALED && exact) scores32();
     }
     phase();
     if (i < mine) {
@@ -1197,12 +1299,8 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
 #pragma unroll
-            for (int ct = 0; ct < NC; ++ct) {
-              float qe = Q::term(q[ct][j][QT - 1], e);
-#pragma unroll
-              for (int k = QT - 2; k >= 0; --k) qe += Q::term(q[ct][j][k], e);
-              x[ct][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(R::k(kk, e), qe, x[ct][kt], 0, 0, 0);
-            }
+            for (int ct = 0; ct < NC; ++ct)
+              x[ct][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(R::k(kk, e), query32(ct, j, e), x[ct][kt], 0, 0, 0);
         }
       weights(x, std::integral_constant<int, 2>{}, own, r0);
 #pragma unroll

@@ -1,0 +1,79 @@
+"""GPU parity of the drafted tokens' attention where a row's elements lie far apart: what is large meets zeros, and what is
+left must keep its bits."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from helpers import rel_max, to_np
+from test_gpu_draft import TOL, TYPES, _gpu_ref, _ids, _parents, _state
+
+pytestmark = pytest.mark.gpu
+
+# Capacities by which the kernels of 16 columns (one workgroup's keys, splits of them), 32 and 128 columns run: 40 nodes of 16
+# query heads over 2 kv heads are 320 columns a kv head.
+CTX = [None, 2000, 6000, 24000, 70000]
+
+
+def _zero_keys(kv, draft, dims):
+    for t in (kv.k[0], draft.k[0]):
+        t[:, :, dims] = 0
+
+
+@pytest.mark.parametrize("ctx", CTX)
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_large_query_elements_over_zero_keys(dev, dtype, ctx):
+    """A query element of 2^24 to 2^100 that every key meets with zero leaves the score to the others: they keep their
+    bits. Every third node has one, in one head or all; the rest are as they were."""
+    from nurostream_amd.model.draft import tree_attn
+    n, pos = 40, 300
+    parents = _parents(n, "tree", seed=3)
+    for e in (24, 30, 40, 60, 100):
+        c, kv, draft, q, sinks = _state(dev, 32, 2, n, pos, dtype, seed=e, ctx=ctx)
+        _zero_keys(kv, draft, [7])
+        ref = _gpu_ref(c, kv, draft, q, parents, sinks, 0, pos)  # (the element adds zero to every score)
+        x = q.reshape(n, 32, 64)
+        x[::3, :, 7] = 2.0 ** e
+        x[1::3, 5, 7] = -(2.0 ** e)
+        out = to_np(tree_attn(q, c, draft, 0, sinks, 0, parents=_ids(parents, dev)))
+        assert rel_max(out, ref) < TOL, e
+
+
+@pytest.mark.parametrize("ctx", CTX)
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_small_query_elements_over_large_keys(dev, dtype, ctx):
+    """The scores come from query elements 2^-16 to 2^-26 of the head's largest, over keys of 2^15, beside a large element
+    over zero keys."""
+    from nurostream_amd.model.draft import tree_attn
+    n, pos = 40, 300
+    parents = _parents(n, "tree", seed=4)
+    for e in (16, 21, 26):
+        c, kv, draft, q, sinks = _state(dev, 32, 2, n, pos, dtype, seed=e, ctx=ctx)
+        _zero_keys(kv, draft, [0])
+        for t, m in ((kv.k[0], pos), (draft.k[0], n)):
+            t[:, :m] *= 2.0 ** 13  # |k| < 2^13 * 5.5 < 65504
+        q *= 2.0 ** -13
+        q.reshape(n, 32, 64)[..., 0] = 2.0 ** (e - 13)
+        ref = _gpu_ref(c, kv, draft, q, parents, sinks, 0, pos)
+        out = to_np(tree_attn(q, c, draft, 0, sinks, 0, parents=_ids(parents, dev)))
+        assert rel_max(out, ref) < TOL, e
+
+
+@pytest.mark.parametrize("ctx", CTX)
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_large_projections_over_zero_keys(dev, dtype, ctx):
+    """The same from raw projections: a large bias in a rotated pair of dimensions whose keys are zero, in one head."""
+    from nurostream_amd.model.decode import yarn_inv_freq
+    from nurostream_amd.model.draft import tree_attn_qkv
+    n, pos, H, G = 40, 300, 32, 2
+    parents = _parents(n, "tree", seed=5)
+    c, kv, draft, _, sinks = _state(dev, H, G, n, pos, dtype, seed=2, ctx=ctx)
+    inv, amp = yarn_inv_freq(c, dev)
+    _zero_keys(kv, draft, [7, 39])
+    qkv = torch.randn(n, (H + 2 * G) * 64, generator=torch.Generator().manual_seed(8)).to(dev)
+    qkv.reshape(n, H + 2 * G, 64)[:, H:H + G, [7, 39]] = 0
+    bq = torch.zeros(H * 64, device=dev)
+    want = tree_attn_qkv(qkv, bq, None, None, c, inv, amp, draft, 0, sinks, 0, parents=_ids(parents, dev)).clone()
+    bq.reshape(H, 64)[3, 7] = 2.0 ** 40
+    got = tree_attn_qkv(qkv, bq, None, None, c, inv, amp, draft, 0, sinks, 0, parents=_ids(parents, dev))
+    assert rel_max(to_np(got), to_np(want)) < 2 * TOL
