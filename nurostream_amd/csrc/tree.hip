@@ -128,17 +128,16 @@ __device__ __forceinline__ void halves8(const float (&x)[8], v4u (&t)[2]) {
   }
 }
 
-// How queries and weights meet rows of a type. fp32 and bf16 rows: three bf16 terms of each. fp16 rows, one fp16 term as
-// they are: two fp16 terms, of weights up to 2^15 and of queries, scaled by a power of two so that a column's largest lies in
-// 2^13 .. 2^14 (its scores scaled back). Elements down to 2^-16 of the largest keep 23 bits, smaller ones lose some. What a
-// column loses that way may change a score by no more than 2^-20, a weight by 2^-20.5 of itself, over any fp16 keys
-// (`query_lost`: a column whose largest is below 8 does not lose it by one small element, and one element in 27000 of normal
-// ones is that small); where it could, the scores are fp32 products of the queries as they are, a workgroup's (the wide
-// kernel: a wave's) columns at a time.
+// How queries meet keys of a type. fp32 and bf16 keys: three bf16 terms of a query, all its 24 bits. fp16 keys, one fp16 term
+// as they are: two fp16 terms of the queries, scaled by a power of two so that a column's largest lies in 2^13 .. 2^14 (its
+// scores scaled back). Elements down to 2^-16 of the largest keep 23 bits, smaller ones lose some. What a column loses that
+// way may change a score by no more than 2^-20, a weight by 2^-20.5 of itself, over any fp16 keys (`query_lost`: a column
+// whose largest is below 8 does not lose it by one small element, and one element in 27000 of normal ones is that small);
+// where it could, the scores are fp32 products of the queries as they are, a workgroup's (the wide kernel: a wave's) columns
+// at a time.
 template <typename KT>
 struct Meets {
   static constexpr int QT = 3;
-  static constexpr float LIFT = 0.f;  // by how much the softmax's reference stays below the largest score
   static constexpr bool SCALED = false;
   static __device__ __forceinline__ void split(const float (&x)[8], v4u (&t)[QT]) { split8(x, t); }
   static __device__ __forceinline__ v4f dot(const v4u& a, const v4u& b, const v4f& c) {
@@ -151,7 +150,6 @@ struct Meets {
 template <>
 struct Meets<_Float16> {
   static constexpr int QT = 2;
-  static constexpr float LIFT = 7.f;
   static constexpr bool SCALED = true;
   static __device__ __forceinline__ void split(const float (&x)[8], v4u (&t)[QT]) { halves8(x, t); }
   static __device__ __forceinline__ v4f dot(const v4u& a, const v4u& b, const v4f& c) {
@@ -177,13 +175,17 @@ __device__ __forceinline__ float query_lost(const float (&x)[8], const v4u (&t)[
 // score is off by up to 2^16 times that, of which 2^-20 is let pass.
 __device__ __forceinline__ bool query_spread(float lost, int up) { return !(ldexpf(lost, -up) <= 0x1p-36f); }
 
-// How a wave holds 32 rows of a type: K8, 8 dimensions of a key row; V4, 4 dimensions of a value row; NT, the bf16
-// terms that an element takes exactly.
+// How a wave holds 32 rows of a type: K8, 8 dimensions of a key row; V4, 4 dimensions of a value row; NT, the terms that a
+// key's element takes exactly (`Meets`); VT, the bf16 terms that a value's does.
+//
+// Weights are three bf16 terms over every type, as a light key's must keep its bits beside a heavy key whose value is zero.
+// (Two fp16 terms, for fp16 values as they are, end at 2^-25: 300 keys of 2^-20 the largest weight erred by 1.6e-4 of what
+// they left with the largest at 2^7, and a larger one moves that by 8 bits at most.)
 template <typename KT>
 struct Rows;
 template <>
 struct Rows<float> {
-  static constexpr int NT = 3, BYTES = 4 * ATTN_D;
+  static constexpr int NT = 3, VT = 3, BYTES = 4 * ATTN_D;
   // The 8 dimensions that lane group g of a product holds of dimensions 32 j ..: 4 g .. + 3 and the same 16 further on, so
   // that a load instruction takes 64 contiguous bytes of each row.
   static __device__ __forceinline__ int dim(int j, int g, int e) { return 32 * j + 16 * (e >> 2) + 4 * g + (e & 3); }
@@ -210,7 +212,7 @@ struct Rows<float> {
 };
 template <typename KT>
 struct Rows16 {  // dimensions 32 j + 8 g .. + 7
-  static constexpr int NT = 1, BYTES = 2 * ATTN_D;
+  static constexpr int NT = 1, VT = std::is_same_v<KT, Bf16> ? 1 : 2, BYTES = 2 * ATTN_D;
   static __device__ __forceinline__ int dim(int j, int g, int e) { return 32 * j + 8 * g + e; }
   using K8 = v4u;
   using V4 = v2u;
@@ -245,10 +247,13 @@ __device__ __forceinline__ void key_terms(const typename Rows<KT>::K8& x, v4u (&
     split8(f, t);
   }
 }
+__device__ __forceinline__ v4f dot_bf16(const v4u& a, const v4u& b, const v4f& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(a), as_b8(b), c, 0, 0, 0);
+}
 // Dimension d of a lane's 8 value rows.
 template <typename KT>
-__device__ __forceinline__ void value_terms(const typename Rows<KT>::V4 (&x)[8], int d, v4u (&t)[Rows<KT>::NT]) {
-  if constexpr (Rows<KT>::NT == 1) {
+__device__ __forceinline__ void value_terms(const typename Rows<KT>::V4 (&x)[8], int d, v4u (&t)[Rows<KT>::VT]) {
+  if constexpr (Rows<KT>::VT == 1) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       t[0][i] = __builtin_amdgcn_perm(x[2 * i + 1][d >> 1], x[2 * i][d >> 1], d & 1 ? 0x07060302u : 0x05040100u);
@@ -325,15 +330,15 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028235e3
 // past the present length return at once: the grid goes by ctx_max, so that it does not depend on the position.
 //
 // A tile: scores by v_mfma_f32_16x16x32_bf16 (_f16), A = 16 keys x 32 dimensions, B = 32 dimensions x 16 columns, an element
-// being the sum of its terms (`Meets`; three bf16 terms of an fp32 value, exactly; of their products those of 2^-22 and less
-// are left out). Lane l's results are column l % 16 and keys 4 (l / 16) .. + 3 of each 16: the B operand
+// being the sum of its terms (`Meets`, `Rows`; three bf16 terms of an fp32 value, exactly). Left out are the products of two
+// terms from 2^-22 of the whole product on: the terms being cut toward zero, a product is short by 2^-21 of itself at the most,
+// 2^-24 in the mean, whatever its sign. Lane l's results are column l % 16 and keys 4 (l / 16) .. + 3 of each 16: the B operand
 // of the second product as they stand, when A's lane l holds of each value row the keys of its group and dimensions
 // 4 (l % 16) ..; D then has column l % 16, dimensions 16 (l / 16) + 4 r + dt. So every row is read once by one wave, in
 // pieces of 8 or 16 bytes, and turned into terms once for the wave's 16 NC columns, whose own terms lie in LDS.
 //
 // The softmax's reference m only moves (and the sums are only rescaled) when a tile has a score beyond 2^8 times it:
-// weights stay below 2^8 (2^15 over fp16 rows, whose reference lies 2^7 below), a sum of 2^31 of them below 2^46. So a tile
-// mostly needs no exchange between lanes.
+// weights stay below 2^8, a sum of 2^31 of them below 2^39. So a tile mostly needs no exchange between lanes.
 //
 // A key with weight zero takes no part whatever its value row holds (0 * NaN would be NaN): a wave whose sums are not
 // finite at the end goes through its tiles again, with products in fp32 and values added one key at a time under their
@@ -346,13 +351,13 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028235e3
 // rows, and their loads where they were used, took 23 nodes 17.7 us and 13.2; ahead 11.4, with eight waves 10.7).
 //
 // Bounds: few keys, the chain of dependent loads (position, parents, rows) and the launch -- one node over 203 bf16 rows 5.5
-// us; many keys and few columns, their bytes -- 7 nodes over 131000 fp16 rows, 268 MB, 49 us, 5.4 TB/s; many
+// us; many keys and few columns, their bytes -- 7 nodes over 131000 fp16 rows, 268 MB, 53 us, 5.1 TB/s; many
 // columns, the terms' VALU work beside the products, which the wide kernel below shares among four waves.
 template <typename KT, int NC, int NW, bool ROPE>
 __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
   using R = Rows<KT>;
   using Q = Meets<KT>;
-  constexpr int NT = 64 * NW, COLS = 16 * NC, KTN = R::NT, QT = Q::QT;
+  constexpr int NT = 64 * NW, COLS = 16 * NC, KTN = R::NT, VT = R::VT, QT = Q::QT, PT = 3;
   constexpr int QROW = 2 * ATTN_D + 16, OROW = ATTN_D + 4;  // bytes of a column's term, floats of a column's sums
   constexpr int QBYTES = QT * COLS * QROW, PBYTES = TREE_KEYS * COLS * 4;
   constexpr int HALF = ATTN_D / 2, NROW = R::BYTES + 16, NBYTES = NSX_TREE_MAX_NODES * NROW;
@@ -606,13 +611,13 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
       mx[ct] = fmaxf(s[ct][0][0], s[ct][0][1]);
 #pragma unroll
       for (int e = 2; e < 8; ++e) mx[ct] = fmaxf(mx[ct], s[ct][e >> 2][e & 3]);
-      move = move || mx[ct] > m[ct] + (8.f + Q::LIFT);
+      move = move || mx[ct] > m[ct] + 8.f;
     }
     if (__any(move)) {
 #pragma unroll
       for (int ct = 0; ct < NC; ++ct) {
         float mn = fmaxf(mx[ct], __shfl_xor(mx[ct], 16, 64));
-        mn = fmaxf(m[ct], fmaxf(mn, __shfl_xor(mn, 32, 64)) - Q::LIFT);
+        mn = fmaxf(m[ct], fmaxf(mn, __shfl_xor(mn, 32, 64)));
         const float corr = __builtin_amdgcn_exp2f(m[ct] - mn);  // (first tile: of nothing)
         m[ct] = mn;
         l[ct] *= corr;
@@ -684,26 +689,26 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
         }
     }
     weights(tile, s);
-    v4u pw[NC][QT];
+    v4u pw[NC][PT];
 #pragma unroll
     for (int ct = 0; ct < NC; ++ct) {
       float x[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = s[ct][e >> 2][e & 3];
-      Q::split(x, pw[ct]);
+      split8(x, pw[ct]);
     }
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) {
-      v4u vt[KTN];
+      v4u vt[VT];
       value_terms<KT>(vr, dt, vt);
       if (dt == 3) next_v();
 #pragma unroll
-      for (int o = QT - 1; o >= 0; --o)
+      for (int o = PT - 1; o >= 0; --o)
 #pragma unroll
         for (int k = 0; k <= o; ++k)
-          if (o - k < KTN) {
+          if (o - k < VT) {
 #pragma unroll
-            for (int ct = 0; ct < NC; ++ct) acc[ct][dt] = Q::dot(vt[o - k], pw[ct][k], acc[ct][dt]);
+            for (int ct = 0; ct < NC; ++ct) acc[ct][dt] = dot_bf16(vt[o - k], pw[ct][k], acc[ct][dt]);
           }
     }
   };
@@ -819,7 +824,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
 //
 // Bound by the phases' shared issue: 64 nodes over 65536 bf16 keys (64 / 8 heads, three products a term pair: 206 GFLOP of
 // bf16) 184 us, 1120 TFLOP/s, what a large library product reaches here (1108); 64 nodes over 6000 fp32 keys (six products)
-// 48 us, 16 over 16384 38; 64 over 32000 fp16 keys (two) 83. Of an iteration's 5450 cycles over fp32 rows the products take
+// 48 us, 16 over 16384 38; 64 over 32000 fp16 keys (two of the scores, five of the values) 116. Of an iteration's 5450 cycles over fp32 rows the products take
 // 1870 and the rest 2530, the VALU issuing an instruction in 8 beside the other group's products. Both groups in one phase
 // 188 for an earlier 160, no offset between them 184; scheduler groups, one barrier a tile, 32 x 32 products, two workgroups of
 // four waves: all within 5 % or slower.
@@ -830,9 +835,9 @@ template <typename KT, bool ROPE>
 __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
   using R = Rows<KT>;
   using Q = Meets<KT>;
-  constexpr int KTN = R::NT, QT = Q::QT, NC = 2, CW = 4, NG = 2, COLS = 16 * NC * CW;
+  constexpr int KTN = R::NT, VT = R::VT, QT = Q::QT, PT = 3, NC = 2, CW = 4, NG = 2, COLS = 16 * NC * CW;
   constexpr int TPP = KTN == 1 ? 2 : 1, KEYS = 32 * TPP;  // 16-bit rows: two tiles a phase, as their phases are short
-  constexpr int KF = TPP * 4 * KTN, VF = TPP * 4 * KTN;   // operands (64 lanes x 16 bytes) of a tile's keys and values
+  constexpr int KF = TPP * 4 * KTN, VF = TPP * 4 * VT;    // operands (64 lanes x 16 bytes) of a tile's keys and values
   constexpr int GROUP = (KF + VF) * 1024, OROW = ATTN_D + 4;
   constexpr int PBYTES = 32 * 16 * NC * 4;  // a wave's weights of 32 keys (the second way)
   constexpr int LDS = std::max(std::max(NG * GROUP, 8 * PBYTES), CW * 16 * NC * OROW * 4);
@@ -936,8 +941,8 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
       const int n = cw + CW * it, sub = n >> 2, kt = (n >> 1) & 1, half = n & 1;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        v2u x[KTN];
-        if constexpr (KTN == 1) {
+        v2u x[VT];
+        if constexpr (VT == 1) {
           const uint32_t sel = b ? 0x07060302u : 0x05040100u;
           x[0] = v2u{__builtin_amdgcn_perm(vr[it][1], vr[it][0], sel), __builtin_amdgcn_perm(vr[it][3], vr[it][2], sel)};
         } else {
@@ -945,17 +950,20 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
           for (int p = 0; p < 2; ++p) {
             float f[2];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) f[q] = __builtin_bit_cast(float, (uint32_t)vr[it][2 * p + q][b]);
+            for (int q = 0; q < 2; ++q) {
+              if constexpr (std::is_same_v<KT, float>) f[q] = __builtin_bit_cast(float, (uint32_t)vr[it][2 * p + q][b]);
+              else f[q] = nsx_h2f(b ? vr[it][2 * p + q] >> 16 : vr[it][2 * p + q] & 0xffffu);
+            }
 #pragma unroll
-            for (int k = 0; k < KTN; ++k) {
+            for (int k = 0; k < VT; ++k) {
               x[k][p] = top2(f[0], f[1]);
-              if (k + 1 < KTN) f[0] = below(f[0]), f[1] = below(f[1]);
+              if (k + 1 < VT) f[0] = below(f[0]), f[1] = below(f[1]);
             }
           }
         }
 #pragma unroll
-        for (int k = 0; k < KTN; ++k)
-          *(v2u*)(vl + (((sub * 2 + half) * 2 + b) * KTN + k) * 1024 + lane * 16 + kt * 8) = x[k];
+        for (int k = 0; k < VT; ++k)
+          *(v2u*)(vl + (((sub * 2 + half) * 2 + b) * VT + k) * 1024 + lane * 16 + kt * 8) = x[k];
       }
     }
   };
@@ -1074,7 +1082,7 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
   float m[NC], l[NC];
   v4f acc[NC][4];  // [dimension's half, parity]
   v4f s[NC][2 * TPP];
-  v4u pw[NC][TPP][QT];
+  v4u pw[NC][TPP][PT];
   auto start = [&] {
 #pragma unroll
     for (int ct = 0; ct < NC; ++ct) {
@@ -1120,13 +1128,13 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
       mx[ct] = fmaxf(x[ct][0][0], x[ct][0][1]);
 #pragma unroll
       for (int e = 2; e < 4 * N; ++e) mx[ct] = fmaxf(mx[ct], x[ct][e >> 2][e & 3]);
-      move = move || mx[ct] > m[ct] + (8.f + Q::LIFT);
+      move = move || mx[ct] > m[ct] + 8.f;
     }
     if (__any(move)) {
 #pragma unroll
       for (int ct = 0; ct < NC; ++ct) {
         float mn = fmaxf(mx[ct], __shfl_xor(mx[ct], 16, 64));
-        mn = fmaxf(m[ct], fmaxf(mn, __shfl_xor(mn, 32, 64)) - Q::LIFT);
+        mn = fmaxf(m[ct], fmaxf(mn, __shfl_xor(mn, 32, 64)));
         const float corr = __builtin_amdgcn_exp2f(m[ct] - mn);  // (first tile: of nothing)
         m[ct] = mn;
         l[ct] *= corr;
@@ -1159,14 +1167,13 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
 
   // The products of a tile step by step, an operand set each: the values of tile i - 1 (the first time: zeros under no
   // weights), then the keys of tile i (the last time: what is there, unused). A step's operands are read AHEAD steps early.
-  constexpr int STEPS = 8 * TPP, AHEAD = KTN == 1 ? 4 : 1;
+  constexpr int STEPS = 8 * TPP, VSTEPS = 4 * TPP, AHEAD = VT == 1 ? 4 : 1, MOST = VT > KTN ? VT : KTN;
   auto products = [&] {
-    v4u x[AHEAD + 1][KTN];
+    v4u x[AHEAD + 1][MOST];
     auto read = [&](int n) {
+      const uint8_t* at = n < VSTEPS ? vl + n * VT * 1024 : kl + (n - VSTEPS) * KTN * 1024;
 #pragma unroll
-      for (int k = 0; k < KTN; ++k)
-        x[n % (AHEAD + 1)][k] =
-            *(const v4u*)((n < 4 * TPP ? vl + n * KTN * 1024 : kl + (n - 4 * TPP) * KTN * 1024) + k * 1024 + lane * 16);
+      for (int k = 0; k < (n < VSTEPS ? VT : KTN); ++k) x[n % (AHEAD + 1)][k] = *(const v4u*)(at + k * 1024 + lane * 16);
     };
 #pragma unroll
     for (int ct = 0; ct < NC; ++ct)
@@ -1177,18 +1184,18 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
 #pragma unroll
     for (int n = 0; n < STEPS; ++n) {
       if (n + AHEAD < STEPS) read(n + AHEAD);
-      const v4u(&y)[KTN] = x[n % (AHEAD + 1)];
-      if (n < 4 * TPP) {
+      const v4u(&y)[MOST] = x[n % (AHEAD + 1)];
+      if (n < VSTEPS) {
 #pragma unroll
-        for (int o = QT - 1; o >= 0; --o)  // (the small products first)
+        for (int o = PT - 1; o >= 0; --o)  // (the small products first)
 #pragma unroll
           for (int k = 0; k <= o; ++k)
-            if (o - k < KTN) {
+            if (o - k < VT) {
 #pragma unroll
-              for (int ct = 0; ct < NC; ++ct) acc[ct][n % 4] = Q::dot(y[o - k], pw[ct][n / 4][k], acc[ct][n % 4]);
+              for (int ct = 0; ct < NC; ++ct) acc[ct][n % 4] = dot_bf16(y[o - k], pw[ct][n / 4][k], acc[ct][n % 4]);
             }
       } else {
-        const int kn = n - 4 * TPP;
+        const int kn = n - VSTEPS;
 #pragma unroll
         for (int o = QT - 1; o >= 0; --o)
 #pragma unroll
@@ -1199,13 +1206,15 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
             }
       }
     }
-    // the order above, kept by the scheduler: LDS reads (0x100) ahead of the products (0x8)
-    constexpr int PRODUCTS = NC * (KTN == 3 ? 6 : QT);
-    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * KTN, 0);
+    // the order above, kept by the scheduler: LDS reads (0x100) ahead of the products (0x8); of the first and second kind
+    constexpr int VPRODUCTS = NC * (VT == 3 ? 6 : VT == 2 ? 5 : 3), KPRODUCTS = NC * (KTN == 3 ? 6 : QT);
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * VT, 0);
 #pragma unroll
     for (int n = 0; n < STEPS; ++n) {
-      if (n + AHEAD < STEPS) __builtin_amdgcn_sched_group_barrier(0x100, KTN, 0);
-      __builtin_amdgcn_sched_group_barrier(0x8, PRODUCTS, 0);
+      if (n + AHEAD < VSTEPS) __builtin_amdgcn_sched_group_barrier(0x100, VT, 0);
+      else if (n + AHEAD < STEPS) __builtin_amdgcn_sched_group_barrier(0x100, KTN, 0);
+      if (n < VSTEPS) __builtin_amdgcn_sched_group_barrier(0x8, VPRODUCTS, 0);
+      else __builtin_amdgcn_sched_group_barrier(0x8, KPRODUCTS, 0);
     }
   };
 
@@ -1232,7 +1241,7 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
 #pragma unroll
     for (int u = 0; u < TPP; ++u) {
 #pragma unroll
-      for (int k = 0; k < QT; ++k) pw[ct][u][k] = v4u{0, 0, 0, 0};
+      for (int k = 0; k < PT; ++k) pw[ct][u][k] = v4u{0, 0, 0, 0};
     }
 #pragma unroll
   for (int n = 0; n < VF / CW; ++n) *(v4u*)(vl + (cw + CW * n) * 1024 + lane * 16) = v4u{0, 0, 0, 0};
@@ -1266,7 +1275,7 @@ __global__ __launch_bounds__(512, 2) void tree_wide_kernel(TreeArgs a) {
           float x[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = s[ct][2 * u + (e >> 2)][e & 3];
-          Q::split(x, pw[ct][u]);
+          split8(x, pw[ct][u]);
         }
     }
     phase();
@@ -1491,9 +1500,10 @@ struct TreePlan {
 // the most workgroups and the shortest way through one (us for 16 / 32 / 128 columns at 64 / 8 heads, fp32, 4000 keys:
 // 16 nodes 22.9 / 23.7 / 26.3, 32 nodes 30.1 / 27.6 / 31.0; bf16 17.6 / 20.2 / 24.6 and 21.7 / 21.2 / 27.5). Past it, more
 // than 64 columns go to the wide kernel once its sharing of terms outweighs its longer way, the sooner the more terms an
-// element has: three from 32768 pieces on (fp32, 64 nodes, 4000 keys 52.3 / 41.3 / 42.6, 8000 keys 86.4 / 64.8 / 60.0), one
-// from 98304 (64 nodes, 16000 keys: bf16 95.0 / 59.8 / 60.6, fp16 94.9 / 57.2 / 54.8; 32000 keys 177 / 104 / 101 and 177 / 98 /
-// 88; 8000 keys 52.7 / 36.8 / 42.5 and 53.2 / 36.0 / 40.2).
+// element has: three from 32768 pieces on (fp32, 64 nodes, 4000 keys 52.3 / 41.3 / 42.6, 8000 keys 86.4 / 64.8 / 60.0), two from
+// 49152 (fp16 values; 64 nodes, 8000 keys 54.8 / 44.9 / 43.5; 16 nodes, 32000 keys 54.7 / 44.5 / 41.8, 16000 keys 33.3 / 28.6 /
+// 29.1), one from 98304 (bf16, 64 nodes, 16000 keys 95.0 / 59.8 / 60.6, 32000 keys 177 / 104 / 101, 8000 keys 52.7 / 36.8 /
+// 42.5).
 //
 // Few tiles are one workgroup's, of eight waves, rather than splits with a merge behind them: with up to 96 KB of keys, where
 // the merge costs as much as the longer way, and some more where the grid is large (us alone / split: one node of 64 / 8
@@ -1502,11 +1512,11 @@ struct TreePlan {
 TreePlan tree_plan(int n_kv, int n_rep, int nodes, int64_t ctx_max, int window, int kv_dtype) {
   const int64_t cols = (int64_t)nodes * n_rep, rows = window > 0 ? std::min<int64_t>(ctx_max, window) : ctx_max;
   const int64_t work = n_kv * nsx_cdiv(cols, 16) * nsx_cdiv(rows, 32);
-  const int terms = kv_dtype == NSX_DT_F32 ? 3 : 1;
+  const int terms = kv_dtype == NSX_DT_F32 ? 3 : kv_dtype == NSX_DT_F16 ? 2 : 1;  // of a value
   TreePlan p;
   p.kind = work < 12288 ? TREE_16 : cols > 64 && work * terms >= 98304 ? TREE_WIDE : TREE_32;
   const bool wide = p.kind == TREE_WIDE;
-  p.keys = wide && terms == 1 ? 2 * TREE_KEYS : TREE_KEYS;
+  p.keys = wide && terms < 3 ? 2 * TREE_KEYS : TREE_KEYS;
   p.round = wide ? 1 : TREE_NW;
   p.ncb = (int)nsx_cdiv(cols, p.kind == TREE_16 ? 16 : p.kind == TREE_32 ? 32 : 128);
   const int64_t tiles = nsx_cdiv(rows, p.keys) + nsx_cdiv(nodes, p.keys);

@@ -1,5 +1,5 @@
-"""GPU parity of the drafted tokens' attention where a row's elements lie far apart: what is large meets zeros, and what is
-left must keep its bits."""
+"""GPU parity of the drafted tokens' attention where a row's elements, or the softmax's weights, lie far apart: what is large
+meets zeros, and what is left must keep its bits."""
 from __future__ import annotations
 
 import pytest
@@ -77,3 +77,24 @@ def test_large_projections_over_zero_keys(dev, dtype, ctx):
     bq.reshape(H, 64)[3, 7] = 2.0 ** 40
     got = tree_attn_qkv(qkv, bq, None, None, c, inv, amp, draft, 0, sinks, 0, parents=_ids(parents, dev))
     assert rel_max(to_np(got), to_np(want)) < 2 * TOL
+
+
+@pytest.mark.parametrize("ctx", CTX)
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("at", [0, 171, 299])
+def test_light_keys_under_a_heavy_one(dev, dtype, ctx, at):
+    """One key has 2^20, 2^58 or 2^87 times the weight of every other and a value of zero: what the others leave is right
+    beside itself."""
+    from nurostream_amd.model.draft import tree_attn
+    n, pos = 40, 300
+    parents = _parents(n, "tree", seed=6)
+    for above in (14.0, 40.0, 60.0):
+        c, kv, draft, q, _ = _state(dev, 32, 2, n, pos, dtype, seed=9, ctx=ctx)
+        _zero_keys(kv, draft, [7])
+        q *= 0.05  # scores of deviation 0.1 beside each other
+        q.reshape(n, 32, 64)[..., 7] = 8.0
+        kv.k[0][:, at, 7] = above
+        kv.v[0][:, at] = 0
+        ref = _gpu_ref(c, kv, draft, q, parents, None, 0, pos)
+        out = to_np(tree_attn(q, c, draft, 0, None, 0, parents=_ids(parents, dev)))
+        assert rel_max(out, ref) < TOL, above
