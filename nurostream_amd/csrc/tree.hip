@@ -139,7 +139,13 @@ template <typename KT>
 struct Meets {
   static constexpr int QT = 3;
   static constexpr bool SCALED = false;
-  static __device__ __forceinline__ void split(const float (&x)[8], v4u (&t)[QT]) { split8(x, t); }
+  static __device__ __forceinline__ void split(const float (&x)[8], v4u (&t)[QT]) {
+    split8(x, t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)  // an infinite query: one infinite term, not infinity - infinity beside it
+#pragma unroll
+      for (int k = 1; k < QT; ++k) t[k][e >> 1] &= fabsf(x[e]) == INFINITY ? (e & 1 ? 0xffffu : 0xffff0000u) : ~0u;
+  }
   static __device__ __forceinline__ v4f dot(const v4u& a, const v4u& b, const v4f& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(a), as_b8(b), c, 0, 0, 0);
   }
@@ -342,7 +348,8 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028235e3
 //
 // A key with weight zero takes no part whatever its value row holds (0 * NaN would be NaN): a wave whose sums are not
 // finite at the end goes through its tiles again, with products in fp32 and values added one key at a time under their
-// weights. (That is also what infinite keys and values take: of their terms the second is NaN.)
+// weights. (That is also what infinite keys and values take: of their terms the second is NaN. Infinite queries keep one
+// term; where it meets a key's zero term, the second way has the score.)
 //
 // ROPE: q is the nodes' raw projections. A workgroup forms the sines and cosines of its columns' nodes (of all nodes where
 // its split has some of theirs) once, as a table in LDS, and rotates its queries by it; a split with node tiles also

@@ -98,3 +98,28 @@ def test_light_keys_under_a_heavy_one(dev, dtype, ctx, at):
         ref = _gpu_ref(c, kv, draft, q, parents, None, 0, pos)
         out = to_np(tree_attn(q, c, draft, 0, None, 0, parents=_ids(parents, dev)))
         assert rel_max(out, ref) < TOL, above
+
+
+@pytest.mark.parametrize("ctx", CTX)
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_infinite_queries(dev, dtype, ctx):
+    """A query element of infinity whose keys all have the other sign: every score is -infinity and the sink has all the
+    weight, as in the one-token attention. The other nodes and heads are as they were."""
+    from nurostream_amd.model.decode import attn_decode
+    from nurostream_amd.model.draft import tree_attn
+    n, pos = 40, 300
+    parents = _parents(n, "tree", seed=3)
+    c, kv, draft, q, sinks = _state(dev, 32, 2, n, pos, dtype, seed=11, ctx=ctx)
+    for t, m in ((kv.k[0], pos), (draft.k[0], n)):
+        t[:, :m, 7] = t[:, :m, 7].abs() + 0.25
+    ref = _gpu_ref(c, kv, draft, q, parents, sinks, 0, pos)
+    x = q.reshape(n, 32, 64)
+    x[5, :, 7] = -float("inf")
+    x[9, 20, 7] = -float("inf")
+    ref[5], ref[9, 20] = 0, 0
+    out = to_np(tree_attn(q, c, draft, 0, sinks, 0, parents=_ids(parents, dev)))
+    assert (out[5] == 0).all() and (out[9, 20] == 0).all()
+    assert rel_max(out, ref) < TOL
+    if dtype == "f32":
+        kv.k[0][:, pos], kv.v[0][:, pos] = draft.k[0][:, 0], draft.v[0][:, 0]
+        assert bool((attn_decode(q[5].contiguous(), kv, 0, sinks, 0, c) == 0).all())
