@@ -12,13 +12,14 @@
 // at which the running sum of the weights exceeds node 0's random number times their total. Temperature 0: p is one
 // at the largest logit, the lowest index of equals.
 //
-// Sums and comparisons in 64 bits, weights to 2^-39 of themselves: a vocabulary's running sum is compared with a random
-// number, and with 32-bit weights the answer would be another one in about one draw of a million. A NaN logit counts
-// as -infinity; of +infinity in a row, its tokens share the row's whole weight; a row without any weight gives the
-// token -1. Sequences with no nodes (length 0) give count 0 and token -1, and rows behind a length are not read.
+// Weights, sums and comparisons in 64 bits: a vocabulary's running sum is compared with a random number, and with 32-bit
+// weights the answer would be another one in about one draw of a million; and what refused tokens leave of a row is a
+// difference, which a weight's error outgrows where they had nearly all of it. A NaN logit counts as -infinity; of
+// +infinity in a row, its tokens share the row's whole weight; a row without any weight gives the token -1. Sequences with
+// no nodes (length 0) give count 0 and token -1, and rows behind a length are not read.
 //
 // Two launches. The rows' chunk sums read all logits once: 32 rows of 201088 fp32 logits 11 us, of which the bytes (2.3
-// TB/s with the launch; 8 us without weights) and then some 16 64-bit operations per logit; 120 rows of 151936 in bf16 14.
+// TB/s with the launch; 8 us without weights) and then some 18 64-bit operations per logit; 120 rows of 151936 in bf16 14.
 // The walk with the draw is five dependent round trips to memory: 10 us, 3.1 where nothing is drawn (temperature 0).
 #include "nsx_common.h"
 
@@ -100,16 +101,20 @@ struct Pow2 {
 };
 
 // The weight 2^(scale2 (x - M)) of logit x beside the largest, M > -infinity. The exponent is n + j / 32 + r with
-// |r| <= 1 / 64 by adding 1.5 * 2^47; 2^r - 1 = r (ln2 + ..) to the fourth power of r: an error of 2^-39. No weight is
-// below 2^-1000, `least` being the least difference: beside the largest one's 1 that is nothing.
+// |r| <= 1 / 64 by adding 1.5 * 2^47; 2^r - 1 = r (ln2 + ..) to the sixth power of r leaves out 2^-58: with the roundings
+// 2^-51 of the weight (to the fourth power 2^-39), beside what the product with scale2 loses, as any exp(x / T) does. No
+// weight is below 2^-1000, `least` being the least difference: beside the largest one's 1 that is nothing.
 __device__ __forceinline__ double vf_weight_finite(float x, float M, const VerifyArgs& a, const Pow2& tab) {
   const double d = fmax((double)x - (double)M, a.least);
   const double t = fma(d, a.scale2, 0x1.8p47);
   const uint32_t k = (uint32_t)__builtin_bit_cast(uint64_t, t);
   const double r = fma(d, a.scale2, -(t - 0x1.8p47));
-  // ln2, ln2^2 / 2, ln2^3 / 6, ln2^4 / 24
-  const double h =
-      fma(r, fma(r, fma(r, 0.0096181291076284772, 0.055504108664821580), 0.24022650695910071), 0.69314718055994531);
+  double h = 0.00015403530393381609;  // ln2^6 / 720, ln2^5 / 120, ..
+  h = fma(r, h, 0.0013333558146428443);
+  h = fma(r, h, 0.0096181291076284772);
+  h = fma(r, h, 0.055504108664821580);
+  h = fma(r, h, 0.24022650695910071);
+  h = fma(r, h, 0.69314718055994531);
   const double c = tab.t[k & 31], w = fma(r * h, c, c);
   const uint64_t bits = __builtin_bit_cast(uint64_t, w);
   const uint32_t high = (uint32_t)(bits >> 32) + ((k & ~31u) << 15);  // 2^n into the exponent
