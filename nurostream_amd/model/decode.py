@@ -75,11 +75,38 @@ def yarn_inv_freq(cfg: AttnConfig, device) -> tuple[torch.Tensor, float]:
     return inv.to(device), float(amplitude)
 
 
+class LayerViews(list):
+    """A stack's layers, a view each. A list that something is put into or taken out of is no longer the stack's
+    (`stack` is None): calls that move rows by the stack refuse it."""
+
+    def __init__(self, stack: torch.Tensor) -> None:
+        super().__init__(stack.unbind(0))
+        self.stack: torch.Tensor | None = stack
+
+    def __reduce__(self):  # a copy is its own copied stack's
+        return (list, (list(self),)) if self.stack is None else (LayerViews, (self.stack,))
+
+
+def _detaching(name: str):
+    change = getattr(list, name)
+
+    def method(self, *args, **kwargs):
+        self.stack = None
+        return change(self, *args, **kwargs)
+    return method
+
+
+for _name in ("__setitem__", "__delitem__", "__iadd__", "__imul__", "append", "extend", "insert", "pop", "remove", "clear",
+              "reverse", "sort"):
+    setattr(LayerViews, _name, _detaching(_name))
+
+
 class DeviceKV:
     """Per-layer K/V history in HBM, [n_kv][ctx_max][head_dim] each, and the
     next token's position as a device int32 (`pos`) with a host mirror
     (`length`). The layers' caches `k` and `v` are views of one tensor each
-    (`k_stack`, `v_stack`). dtype: fp32; or float16 / bfloat16, half the bytes,
+    (`k_stack`, `v_stack`); model.draft.commit refuses others put in their
+    place. dtype: fp32; or float16 / bfloat16, half the bytes,
     for model.draft's attention (one token being a tree of one node) -- the
     one-token calls below take fp32 caches."""
 
@@ -93,7 +120,7 @@ class DeviceKV:
         shape = (n_layer, cfg.n_head_kv, self.ctx_max, cfg.head_dim)
         self.k_stack = torch.zeros(shape, dtype=dtype, device=self.device)
         self.v_stack = torch.zeros(shape, dtype=dtype, device=self.device)
-        self.k, self.v = list(self.k_stack.unbind(0)), list(self.v_stack.unbind(0))
+        self.k, self.v = LayerViews(self.k_stack), LayerViews(self.v_stack)
         self.pos = torch.zeros(1, dtype=torch.int32, device=self.device)
         nb = N.load().nsx_attn_workspace_bytes(cfg.n_head, cfg.head_dim, self.ctx_max)
         if nb < 0:

@@ -19,7 +19,7 @@ import math
 import torch
 
 from .. import _native as N
-from .decode import AttnConfig, DeviceKV
+from .decode import AttnConfig, DeviceKV, LayerViews
 
 MAX_NODES = N.TREE_MAX_NODES
 
@@ -41,7 +41,7 @@ class DraftKV:
         shape = (n_layer, n_kv, self.max_nodes, head_dim)
         self.k_stack = torch.zeros(shape, dtype=kv.dtype, device=kv.device)
         self.v_stack = torch.zeros(shape, dtype=kv.dtype, device=kv.device)
-        self.k, self.v = list(self.k_stack.unbind(0)), list(self.v_stack.unbind(0))
+        self.k, self.v = LayerViews(self.k_stack), LayerViews(self.v_stack)
         self.workspace = torch.empty(nb, dtype=torch.uint8, device=kv.device)
         self._taken = torch.zeros(1, dtype=torch.int32, device=kv.device)  # commit's workgroups count themselves out here
         self._dt = N.act_dtype_code(kv.dtype)
@@ -78,6 +78,15 @@ def _call(what: str, fn, device: torch.device, *args) -> None:
         N.check(rc, what)
 
 
+def _stacked(kv: DeviceKV, draft: DraftKV) -> bool:
+    """Whether the layers are still the views of the stacks that they were made as."""
+    try:
+        return (kv.k.stack is kv.k_stack and kv.v.stack is kv.v_stack and draft.k.stack is draft.k_stack
+                and draft.v.stack is draft.v_stack)
+    except AttributeError:  # lists of the caller's
+        return False
+
+
 def _tree(x: torch.Tensor, row: int, name: str, draft: DraftKV, layer: int, cfg: AttnConfig, sinks, parents, out):
     """Checks shared by both attention calls -> (nodes, out)."""
     kv = draft.kv
@@ -91,6 +100,10 @@ def _tree(x: torch.Tensor, row: int, name: str, draft: DraftKV, layer: int, cfg:
                          "{} over {} of {}".format(*draft.heads))
     if not 0 <= layer < len(draft.k):
         raise IndexError(f"layer {layer} of {len(draft.k)}")
+    if not _stacked(kv, draft):  # a layer of the caller's: the kernels take its shape and type for granted
+        for name, t, like in (("kv.k", kv.k, kv.k_stack), ("kv.v", kv.v, kv.v_stack), ("draft.k", draft.k, draft.k_stack),
+                              ("draft.v", draft.v, draft.v_stack)):
+            _check(f"{name}[{layer}]", t[layer], kv.dtype, x.device, like[layer].numel())
     _check("parents", parents, torch.int32, x.device, n)
     _check("sinks", sinks, torch.float32, x.device, cfg.n_head)
     _check("out", out, torch.float32, x.device, n * cfg.n_head * cfg.head_dim)
@@ -135,8 +148,12 @@ def tree_attn_qkv(qkv: torch.Tensor, bq, bk, bv, cfg: AttnConfig, inv_freq: torc
 def commit(draft: DraftKV, path: torch.Tensor, count: torch.Tensor) -> None:
     """Rows path[0 .. count - 1] of every layer's nodes into the caches' rows kv.pos, kv.pos + 1, ..., then kv.pos +=
     count on the device (path, count: device int32, as `verify` returns them for one sequence). The host's kv.length
-    is the caller's to move on, by the count once it is known there."""
+    is the caller's to move on, by the count once it is known there. Layers that were replaced in kv.k, kv.v, draft.k or
+    draft.v are refused: the rows move from stack to stack."""
     kv = draft.kv
+    if not _stacked(kv, draft):
+        raise ValueError("a layer of kv.k, kv.v, draft.k or draft.v was replaced: commit moves the rows of the stacks "
+                         "that they were made as")
     N.require_device(path, count)
     _check("path", path, torch.int32, kv.k_stack.device)
     _check("count", count, torch.int32, path.device, 1)

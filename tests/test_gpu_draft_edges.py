@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_draft import _ids
+from test_gpu_draft import _ids, _state
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +30,22 @@ def test_verify_accepts_to_the_late_bits(dev, T):
     us[:, 1] = torch.from_numpy(u[pick])
     count, _, _ = verify(logits.to(dev), _ids([[0, 1]] * B, dev), us.to(dev), temperature=T)
     assert (count.cpu().numpy() - 1 == (gap[pick] > 0)).all()
+
+
+def test_attention_over_replaced_layers(dev):
+    """A layer that the caller put in place of a view is read if it has the view's layout, and refused otherwise; commit
+    refuses it either way."""
+    from nurostream_amd.model.draft import commit, tree_attn
+    c, kv, draft, q, sinks = _state(dev, 16, 2, 4, 50, "f32", seed=1)
+    want = tree_attn(q, c, draft, 0, sinks, 0).clone()
+    rows = kv.k[0]
+    kv.k[0] = rows.clone()
+    assert torch.equal(tree_attn(q, c, draft, 0, sinks, 0), want)
+    with pytest.raises(ValueError):
+        commit(draft, _ids([0], dev), _ids([1], dev))
+    for bad, error in ((rows[:, :60].contiguous(), ValueError), (rows.half(), TypeError), (rows.cpu(), ValueError),
+                       (rows.transpose(0, 1).contiguous().transpose(0, 1), ValueError)):
+        kv.k[0] = bad
+        with pytest.raises(error):
+            tree_attn(q, c, draft, 0, sinks, 0)
+    assert int(kv.pos) == 50
