@@ -90,6 +90,8 @@ def _stacked(kv: DeviceKV, draft: DraftKV) -> bool:
 def _tree(x: torch.Tensor, row: int, name: str, draft: DraftKV, layer: int, cfg: AttnConfig, sinks, parents, out):
     """Checks shared by both attention calls -> (nodes, out)."""
     kv = draft.kv
+    if kv.length > kv.ctx_max:
+        raise ValueError(f"kv.length {kv.length} lies past the cache's {kv.ctx_max} rows")
     N.require_device(x)
     n = x.numel() // row if x.dim() > 1 else 1
     _check(name, x, torch.float32, kv.k_stack.device, n * row)
@@ -116,7 +118,8 @@ def tree_attn(q: torch.Tensor, cfg: AttnConfig, draft: DraftKV, layer: int, sink
               parents: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Sink attention of the nodes' rotated queries (n, n_head * head_dim) over the layer's cache (kv.pos rows) and the
     rows that draft.k / draft.v hold of their ancestors and themselves, the last `window` positions of those when
-    window > 0 -> (n, n_head, head_dim) fp32."""
+    window > 0 -> (n, n_head, head_dim) fp32. A device position outside 0 .. kv.ctx_max leaves the output unwritten; the
+    host's mirror kv.length is checked."""
     n, y = _tree(q, cfg.n_head * cfg.head_dim, "q", draft, layer, cfg, sinks, parents, out)
     kv = draft.kv
     _call("tree_attn", N.load().nsx_tree_attn, q.device, q.data_ptr(), kv.k[layer].data_ptr(), kv.v[layer].data_ptr(),
@@ -148,12 +151,15 @@ def tree_attn_qkv(qkv: torch.Tensor, bq, bk, bv, cfg: AttnConfig, inv_freq: torc
 def commit(draft: DraftKV, path: torch.Tensor, count: torch.Tensor) -> None:
     """Rows path[0 .. count - 1] of every layer's nodes into the caches' rows kv.pos, kv.pos + 1, ..., then kv.pos +=
     count on the device (path, count: device int32, as `verify` returns them for one sequence). The host's kv.length
-    is the caller's to move on, by the count once it is known there. Layers that were replaced in kv.k, kv.v, draft.k or
+    is the caller's to move on, by the count once it is known there; a full cache by that mirror is refused, and rows past
+    the cache's end by the device's position are not written (kv.pos then stops at the end). Layers that were replaced in kv.k, kv.v, draft.k or
     draft.v are refused: the rows move from stack to stack."""
     kv = draft.kv
     if not _stacked(kv, draft):
         raise ValueError("a layer of kv.k, kv.v, draft.k or draft.v was replaced: commit moves the rows of the stacks "
                          "that they were made as")
+    if kv.length >= kv.ctx_max:
+        raise ValueError(f"the cache's {kv.ctx_max} rows are taken (kv.length {kv.length})")
     N.require_device(path, count)
     _check("path", path, torch.int32, kv.k_stack.device)
     _check("count", count, torch.int32, path.device, 1)

@@ -39,3 +39,20 @@ def test_replaced_layers(lib):  # noqa: F811
         assert kv.k[1].data_ptr() == kv.k_stack[1].data_ptr() and d.k[2].data_ptr() == d.k_stack[2].data_ptr()
         with pytest.raises(N.NativeError):  # on to the check for tensors on the GPU
             commit(d, path, count)
+
+
+def test_lengths_past_the_cache(lib):  # noqa: F811
+    """The host's mirror of the position says where rows would be dropped: a commit into a full cache, and attention or a
+    commit behind its end, are refused before anything else."""
+    from nurostream_amd.model.draft import tree_attn, tree_attn_qkv
+    c = _cfg()
+    kv = DeviceKV(1, c, 50, "cpu")
+    d = DraftKV(kv, c, max_nodes=4)
+    path, count = torch.zeros(4, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    calls = {"commit": lambda: commit(d, path, count), "attn": lambda: tree_attn(torch.zeros(4, 16 * 64), c, d, 0, None, 0),
+             "qkv": lambda: tree_attn_qkv(torch.zeros(4, 20 * 64), None, None, None, c, torch.zeros(32), 1.0, d, 0, None, 0)}
+    for length, refused in ((0, ()), (49, ()), (50, ("commit",)), (51, ("commit", "attn", "qkv"))):
+        kv.length = length
+        for name, call in calls.items():
+            with pytest.raises(ValueError if name in refused else N.NativeError):
+                call()
