@@ -259,8 +259,10 @@ class NeuroStream:
         t0 = time.perf_counter()
         while True:
             for tok in ready:
-                if tok in eos or tok < 0 or self.stats.generated_tokens >= max_tokens:
+                if tok in eos or self.stats.generated_tokens >= max_tokens:
                     break
+                if tok < 0:  # (verify's answer to a row without any weight)
+                    raise FloatingPointError("the model's logits hold no number to choose a token by")
                 self.stats.generated_tokens += 1
                 yield self._piece(tok)
             else:

@@ -49,3 +49,27 @@ def test_attention_over_replaced_layers(dev):
         with pytest.raises(error):
             tree_attn(q, c, draft, 0, sinks, 0)
     assert int(kv.pos) == 50
+
+
+@pytest.mark.parametrize("kw", [dict(drafts=4), dict(drafts=0, kv_dtype=torch.bfloat16),
+                                dict(drafts=4, temperature=0.8, top_p=1.0)])
+def test_generate_without_a_number(dev, tmp_path, monkeypatch, kw):
+    """Logits that are all NaN end the generation with an error, behind the tokens before them: of the prompt's last pass,
+    or of a later one."""
+    from test_gpu_decode import _tiny_model
+    ns, _ = _tiny_model(tmp_path, dev)
+    whole = ns.model.forward_tree
+    for good in (0, 3):
+        calls = []
+
+        def pass_(*args, **kwargs):
+            calls.append(0)
+            x = whole(*args, **kwargs)
+            return x if len(calls) <= good else torch.full_like(x, float("nan"))
+
+        monkeypatch.setattr(ns.model, "forward_tree", pass_)
+        got = []
+        with pytest.raises(FloatingPointError):
+            for piece in ns.generate([11, 200, 37], max_tokens=30, **kw):
+                got.append(piece)
+        assert len(got) >= good and len(calls) == good + 1
