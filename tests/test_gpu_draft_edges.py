@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_draft import _ids, _state
+from test_gpu_draft import TYPES, _cfg, _ids, _parents, _state, _step_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +73,112 @@ def test_generate_without_a_number(dev, tmp_path, monkeypatch, kw):
             for piece in ns.generate([11, 200, 37], max_tokens=30, **kw):
                 got.append(piece)
         assert len(got) >= good and len(calls) == good + 1
+
+
+@pytest.mark.parametrize("ctx", [None, 50])
+def test_generate_with_drafts_that_are_accepted(dev, tmp_path, monkeypatch, ctx):
+    """Drafts that hold the tokens to come, each level a wrong one beside the right one: paths of several nodes are
+    accepted, pass after pass, also up to the context's end; the tokens are those without drafts."""
+    import dataclasses
+    from test_gpu_decode import _tiny_model
+    import nurostream_amd.model.draft as draft_calls
+    ns, _ = _tiny_model(tmp_path, dev)
+    if ctx:
+        small = dataclasses.replace(ns.model.attn_config(), context_length=ctx)
+        monkeypatch.setattr(ns.model, "attn_config", lambda: small)
+    prompt = [11, 200, 37]
+    want = list(ns.generate(prompt, max_tokens=60))
+    known = prompt + [int(p[1:-1]) for p in want]
+
+    class Known:
+        def __init__(self, tokens):
+            self.n = len(tokens)
+
+        def extend(self, tokens):
+            self.n += len(tokens)
+
+        def propose(self, n_drafts, depth=None):
+            nodes, parents, tip = [known[self.n - 1]], [-1], 0
+            for level, t in enumerate(known[self.n:]):
+                if level >= min(n_drafts, depth) or len(nodes) + 2 > n_drafts + 1:
+                    break
+                nodes += [(t + 1) % 300, t]
+                parents += [tip, tip]
+                tip = len(nodes) - 1
+            return nodes, parents
+
+    monkeypatch.setattr(draft_calls, "LookupDrafts", Known)
+    for drafts in (2, 7, 12, 63):
+        assert list(ns.generate(prompt, max_tokens=60, drafts=drafts)) == want
+        s = ns.stats
+        a_pass = drafts // 2 + 1  # tokens of a pass: the accepted drafts and the one that follows
+        assert s.passes <= -(-(len(want) - 1) // a_pass) + 1
+        assert s.accepted_tokens >= len(want) - 1 - s.passes and s.drafted_tokens <= drafts * s.passes
+
+
+@pytest.mark.parametrize("T", [0.0, 0.8])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_whole_step_captured_with_accepted_paths(dev, T, dtype):
+    """The captured step of test_gpu_draft.py with drafts that the target gives nearly all its weight: every replay commits
+    a path of several nodes, whose rows and positions are the eager step's and are read by the next replay."""
+    from nurostream_amd.model.decode import DeviceKV, yarn_inv_freq
+    from nurostream_amd.model.draft import DraftKV, commit, tree_attn_qkv, verify
+    H, G, V, n, L, ctx = 16, 2, 6001, 11, 2, 400
+    c = _cfg(H, G)
+    inv, amp = yarn_inv_freq(c, dev)
+    tree = _parents(n, "tree", 4)
+    parents = _ids(tree, dev)
+
+    def inputs(seed):
+        x = _step_inputs(dev, n, L, H, G, V, seed)
+        g = torch.Generator().manual_seed(seed)
+        for i in range(1, n):  # a child in two has the parent's heavy token
+            if torch.rand(1, generator=g) < 0.5 or i == 1:
+                x["logits"][tree[i], x["tokens"][0, i]] = 60.0
+        return x
+
+    def make():
+        kv = DeviceKV(L, c, ctx, dev, dtype=TYPES[dtype])
+        g = torch.Generator().manual_seed(1)
+        for t in (kv.k_stack, kv.v_stack):
+            t.copy_(torch.randn(t.shape, generator=g))
+        kv.pos.fill_(300)
+        return kv, DraftKV(kv, c, max_nodes=n)
+
+    def step(x, draft):
+        att = [tree_attn_qkv(x["qkv"][li], None, None, None, c, inv, amp, draft, li, None, 128 if li % 2 else 0,
+                             parents=parents) for li in range(L)]
+        count, path, token = verify(x["logits"], x["tokens"], x["u"], parents=parents, temperature=T)
+        commit(draft, path[0], count)
+        return (*att, count, path, token)
+
+    (kv_g, dg), (kv_e, de) = make(), make()
+    bufs = inputs(0)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(bufs, dg)
+    torch.cuda.synchronize()
+    kv_g.k_stack.copy_(kv_e.k_stack), kv_g.v_stack.copy_(kv_e.v_stack), kv_g.pos.fill_(300)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        got = step(bufs, dg)
+    counts = []
+    for i in range(6):
+        x = inputs(10 + i)
+        for key in bufs:
+            for a, b in zip(bufs[key], x[key]):
+                a.copy_(b)
+        before = int(kv_e.pos)
+        graph.replay()
+        want = step(x, de)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+        assert torch.equal(kv_g.k_stack, kv_e.k_stack) and torch.equal(kv_g.v_stack, kv_e.v_stack)
+        counts.append(int(want[-3]))
+        assert int(kv_g.pos) == int(kv_e.pos) == before + counts[-1]
+        path = want[-2][0, :counts[-1]].tolist()
+        for j, node in enumerate(path):
+            assert torch.equal(kv_e.k_stack[:, :, before + j], de.k_stack[:, :, node])
+            assert node == 0 or tree[node] == path[j - 1]
+    assert min(counts) >= 2 and max(counts) >= 3
