@@ -418,7 +418,10 @@ int64_t nsx_tree_workspace_bytes(int n_head, int n_kv, int head_dim, int max_nod
  * fp32, rotated. Caches [n_kv][ctx_max][64] and the nodes' own rows
  * [n_kv][max_nodes][64], all of kv_dtype (NSX_DT_*). sinks, scale, n_head and
  * n_kv as nsx_attn_decode. out: [n_nodes][n_head][64] fp32. A key of weight
- * zero takes no part, whatever its value row holds. Nothing is written unless
+ * zero takes no part, whatever its value row holds. Scores take all of the
+ * queries' bits (over fp16 caches a score may be off by 2^-18 more where a
+ * query's elements lie 2^16 and more apart), weights all of theirs, whatever
+ * lies beside them. Nothing is written unless
  * 0 <= *pos <= ctx_max. The buffers are 16-byte aligned; the workspace need
  * not be cleared and is free for other use once the call's work on the stream
  * is done. */

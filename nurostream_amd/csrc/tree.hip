@@ -131,10 +131,11 @@ __device__ __forceinline__ void halves8(const float (&x)[8], v4u (&t)[2]) {
 // How queries meet keys of a type. fp32 and bf16 keys: three bf16 terms of a query, all its 24 bits. fp16 keys, one fp16 term
 // as they are: two fp16 terms of the queries, scaled by a power of two so that a column's largest lies in 2^13 .. 2^14 (its
 // scores scaled back). Elements down to 2^-16 of the largest keep 23 bits, smaller ones lose some. What a column loses that
-// way may change a score by no more than 2^-20, a weight by 2^-20.5 of itself, over any fp16 keys (`query_lost`: a column
-// whose largest is below 8 does not lose it by one small element, and one element in 27000 of normal ones is that small);
-// where it could, the scores are fp32 products of the queries as they are, a workgroup's (the wide kernel: a wave's) columns
-// at a time.
+// way may change a score by no more than 2^-18 over any fp16 keys, by 2^-20 over keys below 2^14 (`query_lost`); where it
+// could, the scores are fp32 products of the queries as they are, a workgroup's (the wide kernel: a wave's) columns at a time.
+// A column whose scaled largest is below 32 (a query of 177) does not lose as much by one small element, and one of 27000
+// normal elements is that small. All columns so: 7 nodes over 131000 rows 59 us for 53, 64 over 32000 243 for 116. (With 2^-20
+// over any keys queries of 71 made the latter 200.)
 template <typename KT>
 struct Meets {
   static constexpr int QT = 3;
@@ -178,8 +179,8 @@ __device__ __forceinline__ float query_lost(const float (&x)[8], const v4u (&t)[
   return lost;
 }
 // Whether a column's queries, having lost so much when scaled by 2^up, need fp32 products: over keys up to 65504 < 2^16 a
-// score is off by up to 2^16 times that, of which 2^-20 is let pass.
-__device__ __forceinline__ bool query_spread(float lost, int up) { return !(ldexpf(lost, -up) <= 0x1p-36f); }
+// score is off by up to 2^16 times that, of which 2^-18 is let pass.
+__device__ __forceinline__ bool query_spread(float lost, int up) { return !(ldexpf(lost, -up) <= 0x1p-34f); }
 
 // How a wave holds 32 rows of a type: K8, 8 dimensions of a key row; V4, 4 dimensions of a value row; NT, the terms that a
 // key's element takes exactly (`Meets`); VT, the bf16 terms that a value's does.
@@ -357,8 +358,8 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028235e3
 // does not depend on the position is loaded ahead of it, and the first tiles ahead of the sines (a launch of its own for the
 // rows, and their loads where they were used, took 23 nodes 17.7 us and 13.2; ahead 11.4, with eight waves 10.7).
 //
-// Bounds: few keys, the chain of dependent loads (position, parents, rows) and the launch -- one node over 203 bf16 rows 5.5
-// us; many keys and few columns, their bytes -- 7 nodes over 131000 fp16 rows, 268 MB, 53 us, 5.1 TB/s; many
+// Bounds: few keys, the chain of dependent loads (position, parents, rows) and the launch -- one node over 203 bf16 rows 5.6
+// us; many keys and few columns, their bytes -- 7 nodes over 131000 fp16 rows, 268 MB, 52 us, 5.2 TB/s; many
 // columns, the terms' VALU work beside the products, which the wide kernel below shares among four waves.
 template <typename KT, int NC, int NW, bool ROPE>
 __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
@@ -830,7 +831,8 @@ __global__ __launch_bounds__(64 * NW, 2) void tree_attn_kernel(TreeArgs a) {
 // so by the barrier between phases: the matrix cores have one group's products while the VALU has the other's weights.
 //
 // Bound by the phases' shared issue: 64 nodes over 65536 bf16 keys (64 / 8 heads, three products a term pair: 206 GFLOP of
-// bf16) 184 us, 1120 TFLOP/s, what a large library product reaches here (1108); 64 nodes over 6000 fp32 keys (six products)
+// bf16) 184 us back to back, 1120 TFLOP/s, what a large library product reaches here (1108; a call at a time under a profiler
+// took 206 to 250); 64 nodes over 6000 fp32 keys (six products)
 // 48 us, 16 over 16384 38; 64 over 32000 fp16 keys (two of the scores, five of the values) 116. Of an iteration's 5450 cycles over fp32 rows the products take
 // 1870 and the rest 2530, the VALU issuing an instruction in 8 beside the other group's products. Both groups in one phase
 // 188 for an earlier 160, no offset between them 184; scheduler groups, one barrier a tile, 32 x 32 products, two workgroups of
@@ -1511,6 +1513,13 @@ struct TreePlan {
 // 49152 (fp16 values; 64 nodes, 8000 keys 54.8 / 44.9 / 43.5; 16 nodes, 32000 keys 54.7 / 44.5 / 41.8, 16000 keys 33.3 / 28.6 /
 // 29.1), one from 98304 (bf16, 64 nodes, 16000 keys 95.0 / 59.8 / 60.6, 32000 keys 177 / 104 / 101, 8000 keys 52.7 / 36.8 /
 // 42.5).
+//
+// The columns themselves do not enter below that: with 16 or fewer the kernel of 16 stays ahead past 12288 pieces too (8
+// columns over 32000 rows: by 7 % over fp32, 16 over 16-bit rows), which takes 8 kv heads and 49152 rows to reach. And the
+// choice goes by the capacity, so that a captured call serves every position: a cache a tenth full costs up to half as much
+// again (us full / a tenth full of the capacity's choice, from projections: one node, 13107 rows, fp32 18.0 / 19.6, bf16 13.3 /
+// 14.4; 16 nodes, 1638 rows 17.2 / 23.2 and 13.8 / 16.7; 64 nodes, 600 rows 22.0 / 26.8 and 12.4 / 20.4, 6000 rows 49.3 / 49.2 and
+// 33.4 / 38.0).
 //
 // Few tiles are one workgroup's, of eight waves, rather than splits with a merge behind them: with up to 96 KB of keys, where
 // the merge costs as much as the longer way, and some more where the grid is large (us alone / split: one node of 64 / 8

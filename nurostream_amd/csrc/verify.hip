@@ -18,7 +18,7 @@
 // +infinity in a row, its tokens share the row's whole weight; a row without any weight gives the token -1. Sequences with
 // no nodes (length 0) give count 0 and token -1, and rows behind a length are not read.
 //
-// Two launches. The rows' chunk sums read all logits once: 32 rows of 201088 fp32 logits 11 us, of which the bytes (2.3
+// Two launches. The rows' chunk sums read all logits once: 32 rows of 201088 fp32 logits 11.7 us, of which the bytes (2.2
 // TB/s with the launch; 8 us without weights) and then some 18 64-bit operations per logit; 120 rows of 151936 in bf16 14.
 // The walk with the draw is five dependent round trips to memory: 10 us, 3.1 where nothing is drawn (temperature 0).
 #include "nsx_common.h"
