@@ -113,8 +113,8 @@ __device__ __forceinline__ void split8(const float (&x)[8], v4u (&t)[NT]) {
   }
 }
 
-// Two fp16 terms of 8 fp32, each rounded to nearest. They miss an element of at least 2^-2 by 2^-23 of itself (half a step
-// of 2^-24 at 2^-1 .. 1), a smaller one by 2^-25 whatever its size: half of fp16's least number.
+// Two fp16 terms of 8 fp32, each rounded to nearest. They miss an element of at least 2^-2 by up to 2^-23 of
+// itself (2^-24 at 2^-1 .. 1), a smaller one by up to 2^-25 whatever its size: half of fp16's least number.
 __device__ __forceinline__ void halves8(const float (&x)[8], v4u (&t)[2]) {
   typedef _Float16 h2 __attribute__((ext_vector_type(2)));
   typedef float f2 __attribute__((ext_vector_type(2)));
