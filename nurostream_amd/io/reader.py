@@ -28,6 +28,24 @@ from .. import _native as N
 DEFAULT_WORKERS = 8
 SLOT_BYTES = 8 << 20  # one staging buffer; larger reads are split across buffers and workers
 
+# Readers and reads dropped while the thread was capturing a graph, which freeing pinned memory and waiting for copies
+# would end: they are closed with the next reader that is opened or closed, or the next read.
+_dropped: list = []
+
+
+def _capturing(device: torch.device) -> bool:
+    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
+
+def _close_dropped() -> None:
+    if not _dropped:
+        return
+    if torch.cuda.is_current_stream_capturing():
+        return
+    items, _dropped[:] = list(_dropped), []
+    for x in sorted(items, key=lambda x: isinstance(x, DiskReader)):  # reads first
+        x.close() if isinstance(x, DiskReader) else x.cancel()
+
 
 @dataclass
 class IOStats:
@@ -99,6 +117,9 @@ class ReadFuture:
     def __del__(self) -> None:  # never free a destination a copy may still write
         if not self.retired and self.reader is not None and self.reader._handle is not None:
             try:
+                if _capturing(self.reader.device):
+                    _dropped.append(self)
+                    return
                 self.reader._retire(self)
             except Exception:
                 pass
@@ -119,6 +140,7 @@ class DiskReader:
         self.device = torch.device(device) if device is not None else torch.device("cpu")
         self._lib = N.load()
         self._handle = None
+        _close_dropped()
         cuda = self.device.type == "cuda"
         if cuda and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
@@ -147,6 +169,7 @@ class DiskReader:
     def _submit(self, offset: int, nbytes: int, dst: torch.Tensor) -> ReadFuture:
         if self._handle is None:
             raise RuntimeError("reader is closed")
+        _close_dropped()
         on_dev = dst.is_cuda
         t = C.c_uint64()
         N.check(self._lib.nsx_reader_submit(self._handle, int(offset), int(nbytes), dst.data_ptr() if nbytes else None,
@@ -221,6 +244,7 @@ class DiskReader:
         return bool(c.direct)
 
     def close(self) -> None:
+        _close_dropped()
         if self._handle is None:
             return
         _ = self.stats  # keep the final counters
@@ -235,6 +259,9 @@ class DiskReader:
 
     def __del__(self) -> None:
         try:
+            if self._handle is not None and _capturing(self.device):
+                _dropped.append(self)
+                return
             self.close()
         except Exception:
             pass
