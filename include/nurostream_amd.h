@@ -483,6 +483,87 @@ int nsx_verify(const void *logits, int logits_dtype, int64_t row_stride, int64_t
                int32_t *count, int32_t *path, int32_t *token, void *workspace, int64_t workspace_bytes,
                void *stream);
 
+/* ---- several sequences at once ----
+ * No reference counterpart (the reference decodes one sequence). A batch of
+ * sequences, each with key and value rows of its own, behind rows that all of
+ * them share (one prompt's), in bf16 or quantised to 8 bits: the new tokens'
+ * rows into the cache, attention over it, and the next tokens by sampling.
+ * Row types: bf16 (NSX_DT_BF16), or 8 bits with an fp32 scale for each row of
+ * a key or value head: NSX_KV_INT8, value = code * scale, scale = max|x| /
+ * 127, code = x / scale to the nearest; NSX_KV_E4M3 (OCP), scale = max|x| /
+ * 448, the same. A row of zeros has scale 0, and one that holds an infinity or
+ * a NaN gets scale NaN: all of it reads back as NaN. head_dim: 64 or 128. */
+enum { NSX_KV_INT8 = 3, NSX_KV_E4M3 = 4 };
+typedef struct {
+  void *k, *v;              /* [n_seq][n_kv][ctx_max][head_dim] of the row type */
+  float *k_scale, *v_scale; /* [n_seq][n_kv][ctx_max]; NULL for bf16 */
+  const int32_t *pos;       /* [n_seq]: how many rows each sequence holds */
+  int64_t n_seq, ctx_max;
+} nsx_kv_rows;
+/* n new tokens of every sequence, counts[b] <= n of them in earnest (NULL: all)
+ * from their raw projections qkv, [n_seq][n][n_head + 2 n_kv][head_dim] of
+ * x_dtype (NSX_DT_*): plus bias (NULL: none), query and key heads times
+ * 1 / sqrt(mean(x^2) + eps) and the norm's weights of head_dim (NULL: no
+ * norm), then rotated: pairs (i, i + head_dim / 2) by the angle position *
+ * inv_freq[i] (taken in 64 bits), times amplitude. Token j of sequence b stands
+ * at position *prefix_pos (NULL: 0) + kv->pos[b] + j; its key and value rows go
+ * to row kv->pos[b] + j, its queries to q_out, [n_seq][n][n_head][head_dim] of
+ * x_dtype. kv->pos is not moved. Tokens from counts[b] on: queries zero, no
+ * rows; rows at or past ctx_max, or before 0, are not written. q_out may not
+ * overlap qkv. */
+int nsx_append_qkv(const void *qkv, int x_dtype, const float *q_bias, const float *k_bias, const float *v_bias,
+                   const float *q_norm, const float *k_norm, float eps, const float *inv_freq, float amplitude,
+                   int n_head, int n_kv, int head_dim, int64_t n, const int32_t *counts, const nsx_kv_rows *kv,
+                   int kv_type, const int32_t *prefix_pos, void *q_out, void *stream);
+/* Finished rows k and v, [n_seq][n_kv][n][head_dim] of x_dtype, into rows first
+ * .. first + n - 1 of every sequence, first being start[b] (device) or, with
+ * start NULL, start0. Rows outside 0 .. ctx_max - 1 are not written. */
+int nsx_store_rows(const void *k, const void *v, int x_dtype, int64_t n, const int32_t *start, int64_t start0,
+                   int n_kv, int head_dim, const nsx_kv_rows *kv, int kv_type, void *stream);
+/* The values of those rows, as x_dtype; rows outside 0 .. ctx_max - 1 give
+ * zeros. */
+int nsx_load_rows(const nsx_kv_rows *kv, int kv_type, int n_kv, int head_dim, const int32_t *start, int64_t start0,
+                  int64_t n, void *k, void *v, int x_dtype, void *stream);
+/* Attention of the tokens that nsx_append_qkv wrote rows for: token j of
+ * sequence b sees the prefix's rows 0 .. prefix->pos[0] - 1 (prefix NULL:
+ * none; n_seq 1, the same row type) and rows 0 .. kv->pos[b] + j of its own
+ * sequence, of these together the last `window` positions when window > 0. q
+ * and out: [n_seq][n][n_head][head_dim] of x_dtype; sinks, scale, n_head and
+ * n_kv as nsx_attn_decode. Products take all bits of the queries; fp32 queries
+ * meet weights of all 24 bits, fp16 ones of 16, bf16 ones of 8. Rows past the
+ * ones seen take no part, whatever they hold. Tokens from counts[b] on, and
+ * tokens that see nothing, give zeros. The rows, q, out and the workspace are
+ * 16-byte aligned; the workspace is scratch of the call. */
+int64_t nsx_batch_attn_workspace_bytes(int n_head, int n_kv, int head_dim, int64_t n_seq, int64_t n,
+                                       int64_t ctx_max, int64_t prefix_max, int window);
+int nsx_batch_attn(const void *q, int x_dtype, const nsx_kv_rows *kv, const nsx_kv_rows *prefix, int kv_type,
+                   int n_head, int n_kv, int head_dim, int64_t n, const int32_t *counts, const float *sinks,
+                   int window, float scale, void *workspace, int64_t workspace_bytes, void *out, void *stream);
+/* A token for each of `batch` rows of logits (row_stride elements apart, vocab
+ * of them): weights e^((x - max) / temperature); of the tokens in descending
+ * order (equal logits by their index) the first top_k (0: all); of those, each
+ * before which less than top_p of their whole weight lies (1: all); of those,
+ * the ones of at least min_p of the largest weight; then the first token in
+ * index order at which the running sum of the weights exceeds uniforms[row]
+ * times their total. temperature <= 0: the largest logit, the lowest index of
+ * equals. A NaN logit counts as -infinity; of +infinity in a row, its tokens
+ * share the row's whole weight; a row without any weight gives -1.
+ * Weights are computed in 64 bits and summed as whole multiples of 2^-(62 -
+ * ceil(log2 vocab)) of the largest, so that no order of summing matters.
+ * Settings: one value for all rows, or with the array not NULL (device) one
+ * each. uniforms (device fp32, in [0, 1)) may be NULL if temperatures is NULL
+ * and temperature 0. vocab up to 4194304, batch below 65536. */
+typedef struct {
+  double temperature, top_p, min_p;
+  int64_t top_k;
+  const float *temperatures, *top_ps, *min_ps; /* NULL, or [batch] */
+  const int32_t *top_ks;
+} nsx_sampling;
+int64_t nsx_sample_workspace_bytes(int64_t batch, int64_t vocab);
+int nsx_sample(const void *logits, int logits_dtype, int64_t row_stride, int64_t batch, int64_t vocab,
+               const float *uniforms, const nsx_sampling *settings, int32_t *token, void *workspace,
+               int64_t workspace_bytes, void *stream);
+
 /* ---- disk reader: GGUF bytes from a file into device (or host) memory ----
  * Replaces the reference's thread-pool reader and the disk side of its
  * streaming source (io/reader.py AsyncReader, io/stream.py StreamingSource):

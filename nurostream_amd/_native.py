@@ -19,6 +19,7 @@ HEADER = Path(__file__).resolve().parents[1] / "include" / "nurostream_amd.h"
 OK, EINVAL, ETYPE, ENOTIMPL, EHIP, EKERNEL, EIO, ETIMEDOUT = 0, 1, 2, 3, 4, 5, 6, 7
 READ_DIRECT = 1
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
+KV_INT8, KV_E4M3 = 3, 4  # rows of a batch's cache, beside DT_BF16
 LAYOUT_GGUF, LAYOUT_T64 = 0, 1
 ROUTE_GPTOSS, ROUTE_QWEN3 = 0, 1
 DISPATCH_AUTO, DISPATCH_PAIRS, DISPATCH_GROUPED, DISPATCH_MFMA = 0, 1, 2, 3
@@ -45,6 +46,20 @@ class MoeLayerC(C.Structure):
         ("gate_stride", C.c_int64), ("up_stride", C.c_int64), ("down_stride", C.c_int64),
         ("gate_tiles", _p), ("up_tiles", _p), ("down_tiles", _p),
     ]
+
+
+class KvRowsC(C.Structure):
+    """nsx_kv_rows."""
+
+    _fields_ = [("k", _p), ("v", _p), ("k_scale", _p), ("v_scale", _p), ("pos", _p), ("n_seq", C.c_int64),
+                ("ctx_max", C.c_int64)]
+
+
+class SamplingC(C.Structure):
+    """nsx_sampling."""
+
+    _fields_ = [("temperature", C.c_double), ("top_p", C.c_double), ("min_p", C.c_double), ("top_k", C.c_int64),
+                ("temperatures", _p), ("top_ps", _p), ("min_ps", _p), ("top_ks", _p)]
 
 
 class ReaderStatsC(C.Structure):
@@ -103,6 +118,15 @@ _SIGS = {
     "nsx_tree_commit": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p, _p, _p, _i64, _p, _p]),
     "nsx_verify_workspace_bytes": (_i64, [_i64, _i, _i64]),
     "nsx_verify": (_i, [_p, _i, _i64, _i64, _i, _i64, _p, _p, _i64, _p, _p, _p, C.c_double, _p, _p, _p, _p, _i64, _p]),
+    "nsx_append_qkv": (_i, [_p, _i, _p, _p, _p, _p, _p, C.c_float, _p, C.c_float, _i, _i, _i, _i64, _p,
+                            C.POINTER(KvRowsC), _i, _p, _p, _p]),
+    "nsx_store_rows": (_i, [_p, _p, _i, _i64, _p, _i64, _i, _i, C.POINTER(KvRowsC), _i, _p]),
+    "nsx_load_rows": (_i, [C.POINTER(KvRowsC), _i, _i, _i, _p, _i64, _i64, _p, _p, _i, _p]),
+    "nsx_batch_attn_workspace_bytes": (_i64, [_i, _i, _i, _i64, _i64, _i64, _i64, _i]),
+    "nsx_batch_attn": (_i, [_p, _i, C.POINTER(KvRowsC), C.POINTER(KvRowsC), _i, _i, _i, _i, _i64, _p, _p, _i, C.c_float,
+                            _p, _i64, _p, _p]),
+    "nsx_sample_workspace_bytes": (_i64, [_i64, _i64]),
+    "nsx_sample": (_i, [_p, _i, _i64, _i64, _i64, _p, C.POINTER(SamplingC), _p, _p, _i64, _p]),
     "nsx_reader_open": (_i, [C.c_char_p, _i, _i, _i, _i64, _i, _p, C.POINTER(_p)]),
     "nsx_reader_submit": (_i, [_p, _i64, _i64, _p, _i, _p, C.POINTER(C.c_uint64)]),
     "nsx_reader_poll": (_i, [_p, C.c_uint64]),

@@ -16,7 +16,8 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libnsx.so"
-SOURCES = ("quant.hip", "gemv_mm.hip", "moe.hip", "attn.hip", "tree.hip", "verify.hip", "reader.hip")
+SOURCES = ("quant.hip", "gemv_mm.hip", "moe.hip", "attn.hip", "tree.hip", "verify.hip", "batch.hip", "sample.hip",
+           "reader.hip")
 HEADERS = ("nsx_common.h", "raw_dot.h", "gemv_mm.h", "rope.h", "launch_cache.h")
 
 HIPCC_FLAGS = [
