@@ -281,6 +281,15 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
 
 // --- attention ---------------------------------------------------------------
 
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+#define LDS_AS __attribute__((address_space(3)))
+
+constexpr int AT_ROWS = 32;   // rows (tokens x heads of a kv head) of a wave
+constexpr int AT_NW = 4;      // waves of a workgroup
+constexpr int AT_MAX_SPLIT = 64;
+
 struct AttnArgs {
   const void* q;
   KvRows kv, pre;  // pre.n_seq 0: none
@@ -288,77 +297,610 @@ struct AttnArgs {
   const float* sinks;
   int H, G, rep, window;
   int64_t n;
-  float scale;
-  float* part;
+  float scale2;  // scale * log2(e): the softmax is taken in powers of two
+  float* part;   // [token][head][splits][D], then [token][head][splits] of (maximum, sum)
   void* out;
+  // what a segment's rows are cut into: row tiles, splits of the keys, whether a workgroup's waves share keys
+  struct Cut {
+    int tiles, splits, shared;
+  } pcut, ocut;
+  int pblocks, splits;  // workgroups of the prefix; splits of both
 };
 
-// A wave per (token, head).
-template <typename XT, int KV, int D>
-__global__ __launch_bounds__(64) void attn_kernel(AttnArgs a) {
-  const int64_t tok = blockIdx.x, b = tok / a.n, j = tok - b * a.n;
-  const int h = blockIdx.y, g = h / a.rep, lane = threadIdx.x;
-  __shared__ float qs[D];
-  __shared__ float ps[64];
-  XT* out = (XT*)a.out + (tok * a.H + h) * D;
-  const bool live = !a.counts || j < a.counts[b];
-  const int64_t P = a.pre.n_seq ? min((int64_t)max(*a.pre.pos, 0), a.pre.ctx_max) : 0;
-  const int64_t L = live ? min((int64_t)a.kv.pos[b] + j + 1, a.kv.ctx_max) : 0;
-  float acc[D / 64] = {};
-  float m = LOWEST, l = 0.f;
-  if (live) {
-    const XT* q = (const XT*)a.q + (tok * a.H + h) * D;
-    for (int i = lane; i < D; i += 64) qs[i] = to_f(q[i]);
-    __syncthreads();
-    const int64_t at = P + a.kv.pos[b] + j, first = a.window > 0 ? max((int64_t)0, at + 1 - a.window) : 0;
-    for (int seg = 0; seg < 2; ++seg) {
-      const KvRows& kv = seg ? a.kv : a.pre;
-      const int64_t lo = seg ? max((int64_t)0, first - P) : first, hi = seg ? L : P;
-      const int64_t base = (seg ? b * a.G + g : g) * kv.ctx_max;
-      for (int64_t t0 = lo; t0 < hi; t0 += 64) {
-        float s = -INFINITY;
-        if (t0 + lane < hi) {
-          s = 0.f;
-          for (int c = 0; c < D / 8; ++c) {
-            float x[8];
-            get_row<KV, D>(kv.k, kv.ks, base + t0 + lane, c, x);
-            for (int i = 0; i < 4; ++i) s += qs[4 * c + i] * x[i] + qs[D / 2 + 4 * c + i] * x[4 + i];
-          }
-          s *= a.scale * LOG2E;
+// A cache row's elements as bf16, which holds all of their bits, 16 bytes of the row at a time.
+template <int KV>
+struct Codes {
+  static constexpr int BYTES = KV == NSX_DT_BF16 ? 2 : 1, PER = 16 / BYTES;  // of an element; elements of 16 bytes
+  static __device__ __forceinline__ void put(uint8_t* lds, v4u x) {
+    if constexpr (KV == NSX_DT_BF16) {
+      *(v4u*)lds = x;
+    } else {
+      v4u y[2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t a, b;
+        if constexpr (KV == NSX_KV_E4M3) {
+          a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[i], 1.f, false));
+          b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[i], 1.f, true));
+        } else {
+          float f[4];
+          codes4<KV>(x[i], f);
+          a = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, f[1]), __builtin_bit_cast(uint32_t, f[0]), 0x07060302u);
+          b = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, f[3]), __builtin_bit_cast(uint32_t, f[2]), 0x07060302u);
         }
-        float mx = s;
-        for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-        mx = fmaxf(mx, m);
-        const float p = t0 + lane < hi ? exp2f(s - mx) : 0.f, f = exp2f(m - mx);
-        float z = p;
-        for (int o = 32; o; o >>= 1) z += __shfl_xor(z, o, 64);
-        l = l * f + z;
-        m = mx;
-        ps[lane] = p;
-        __syncthreads();
-        for (int i = 0; i < D / 64; ++i) acc[i] *= f;
-        for (int64_t t = t0; t < min(hi, t0 + 64); ++t)
-          for (int i = 0; i < D / 64; ++i) {
-            const int64_t e = (base + t) * D + lane + 64 * i;
-            float x;
-            if constexpr (KV == NSX_DT_BF16) x = to_f(((const Bf16*)kv.v)[e]);
-            else {
-              float c[4];
-              codes4<KV>(((const uint8_t*)kv.v)[e], c);
-              x = c[0] * kv.vs[base + t];
-            }
-            acc[i] = fmaf(ps[t - t0], x, acc[i]);
-          }
-        __syncthreads();
+        y[i >> 1][2 * (i & 1)] = a;
+        y[i >> 1][2 * (i & 1) + 1] = b;
       }
-    }
-    if (a.sinks) {
-      const float sink = a.sinks[h] * LOG2E, mx = fmaxf(m, sink), f = exp2f(m - mx);
-      l = l * f + exp2f(sink - mx);
-      for (int i = 0; i < D / 64; ++i) acc[i] *= f;
+      *(v4u*)lds = y[0];
+      *(v4u*)(lds + 16) = y[1];
     }
   }
-  for (int i = 0; i < D / 64; ++i) from_f(out[lane + 64 * i], l == 0.f ? 0.f : acc[i] / l);
+};
+
+// Two bf16 from the upper halves of two fp32; what they leave.
+__device__ __forceinline__ uint32_t top2(float lo, float hi) {
+  return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo), 0x07060302u);
+}
+__device__ __forceinline__ float below(float x) {
+  return x - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & 0xffff0000u);
+}
+__device__ __forceinline__ uint32_t near2(float lo, float hi) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{lo, hi}), b2));
+}
+// 8 fp32 as NT bf16 terms: the first ones 8 bits each toward zero, the last one to the nearest (of three: exact).
+template <int NT>
+__device__ __forceinline__ void terms8(const float (&x)[8], v4u (&t)[NT]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+    for (int k = 0; k < NT; ++k) {
+      if (k + 1 < NT) {
+        t[k][i] = top2(a, b);
+        a = below(a), b = below(b);
+      } else {
+        t[k][i] = near2(a, b);
+      }
+    }
+  }
+}
+__device__ __forceinline__ f16v dot(const v4u& a, const v4u& b, const f16v& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ float other_half_max(float x) {  // the larger of lane and lane ^ 32
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+__device__ __forceinline__ float other_half_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+}
+
+// Where a workgroup stands: a segment (the prefix, or a sequence's own rows) of a kv head, its rows r0 .. and its split.
+struct Place {
+  const uint8_t *k, *v;
+  const float *ks, *vs;
+  bool own;
+  int g, split, slot;     // kv head; split of the segment, of both segments
+  int64_t b, r0, rows;    // sequence (own); first row of the workgroup, rows of the segment
+  int P;                  // the prefix's length
+};
+// Row r of a place's segment: its token and head, and the keys [lo, hi) of the segment that it sees.
+struct Row {
+  int64_t tok;
+  int h, lo, hi;
+  bool live;
+  __device__ __forceinline__ Row(const AttnArgs& a, const Place& p, int64_t r) {
+    r = r < p.rows ? r : p.rows - 1;
+    const int64_t t = r / a.rep;
+    tok = p.own ? p.b * a.n + t : t;
+    h = p.g * a.rep + (int)(r - t * a.rep);
+    const int64_t b = p.own ? p.b : tok / a.n, j = tok - b * a.n, row = (int64_t)a.kv.pos[b] + j;
+    live = !a.counts || j < a.counts[b];
+    const int64_t first = a.window > 0 ? p.P + row + 1 - a.window : 0;
+    const int64_t end = p.own ? (row + 1 < a.kv.ctx_max ? row + 1 : a.kv.ctx_max) : p.P;
+    const int64_t from = p.own ? first - p.P : first;
+    hi = (int)(end > 0 ? end : 0);
+    lo = (int)(from < 0 ? 0 : from < hi ? from : hi);
+  }
+};
+
+// A row's (or split's) end: its maximum (of scores in powers of two), sum and D values over the sum's weights.
+template <typename XT, int D>
+struct End {
+  const AttnArgs& a;
+  const Place& p;
+  __device__ __forceinline__ float* part(const Row& r) const {
+    return a.part + ((r.tok * a.H + r.h) * a.splits + p.slot) * D;
+  }
+  // The factor that values are stored with: 1 for a part, what divides by the whole sum for the answer.
+  __device__ __forceinline__ float factor(const Row& r, float m, float l, bool first) const {
+    if (a.splits > 1) {
+      if (first) {
+        float2* ml = (float2*)(a.part + (int64_t)(a.kv.n_seq * a.n * a.H) * a.splits * D);
+        ml[(r.tok * a.H + r.h) * a.splits + p.slot] = float2{m, l};
+      }
+      return 1.f;
+    }
+    if (!r.live) return 0.f;
+    float f = 1.f;
+    if (a.sinks) {
+      const float sink = a.sinks[r.h] * LOG2E, M = fmaxf(m, sink);
+      f = __builtin_amdgcn_exp2f(m - M);
+      l = fmaf(l, f, __builtin_amdgcn_exp2f(sink - M));
+    }
+    return l == 0.f ? 0.f : f / l;
+  }
+  // Values d .. d + 3
+  __device__ __forceinline__ void store(const Row& r, int d, float f, const float (&x)[4]) const {
+    if (a.splits > 1) {
+      *(v4f*)(part(r) + d) = v4f{x[0], x[1], x[2], x[3]};
+    } else {
+      float y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = f == 0.f ? 0.f : x[i] * f;  // (a token that is not there: zero whatever x is)
+      store4((XT*)a.out + (r.tok * a.H + r.h) * D + d, y);
+    }
+  }
+};
+
+// A row once more, key by key and none that it does not see: for rows whose sums are not finite, as an infinity or a NaN
+// beside a weight of zero makes them in a product of matrices. A wave's work.
+template <typename XT, int KV, int D>
+__device__ __forceinline__ void row_alone(const AttnArgs& a, const Place& p, int64_t r, int t0, int t1) {
+  const int lane = threadIdx.x & 63;
+  const Row row(a, p, r);
+  const XT* q = (const XT*)a.q + (row.tok * a.H + row.h) * D;
+  const int lo = max(row.lo, t0), hi = min(row.hi, t1);
+  float m = LOWEST, l = 0.f, acc[D / 64] = {};
+  for (int t = lo; t < hi; t += 64) {
+    const int key = t + lane;
+    float s = -INFINITY;
+    if (key < hi) {
+      s = 0.f;
+      for (int c = 0; c < D / 8; ++c) {
+        float x[8], lo4[4], hi4[4];
+        get_row<KV, D>(p.k, p.ks, key, c, x);
+        load4(q + 4 * c, lo4);
+        load4(q + D / 2 + 4 * c, hi4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s = fmaf(lo4[i], x[i], fmaf(hi4[i], x[4 + i], s));
+      }
+      s *= a.scale2;
+    }
+    float M = s;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    M = fmaxf(M, m);
+    const float w = key < hi ? __builtin_amdgcn_exp2f(s - M) : 0.f, f = __builtin_amdgcn_exp2f(m - M);
+    l = l * f + nsx_wave_sum(w);
+    m = M;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) acc[i] *= f;
+    for (int u = 0; u < min(64, hi - t); ++u) {
+      const float wu = __shfl(w, u, 64);
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) {
+        const int64_t e = (int64_t)(t + u) * D + lane + 64 * i;
+        float x;
+        if constexpr (KV == NSX_DT_BF16) {
+          x = to_f(((const Bf16*)p.v)[e]);
+        } else {
+          float c[4];
+          codes4<KV>(p.v[e], c);
+          x = c[0] * p.vs[t + u];
+        }
+        acc[i] = fmaf(wu, x, acc[i]);
+      }
+    }
+  }
+  const End<XT, D> end{a, p};
+  const float f = end.factor(row, m, l, lane == 0);
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) {
+    if (a.splits > 1) end.part(row)[lane + 64 * i] = acc[i];
+    else from_f(((XT*)a.out + (row.tok * a.H + row.h) * D)[lane + 64 * i], f == 0.f ? 0.f : acc[i] * f);
+  }
+}
+
+// A wave's 32 rows over its keys. Scores are K Q^T, so that a lane holds 16 of 32 keys' scores of one row (lane % 32; the other
+// lane of the row holds the others), and its weights are at once the second operand of V^T W^T, of which it holds D / 2 values
+// of the same row. The operand's order of keys is the scores' own, and V's rows are read from LDS in it, transposed.
+template <int KV, int D, int NT, int NB>
+struct Wave {
+  static constexpr int PITCH = 2 * D + 16;  // of a row in LDS: reads of 8 rows at once fall on different banks
+  v4u q[NT][D / 16];
+  f16v acc[D / 32];
+  float m, l;
+
+  template <typename XT>
+  __device__ __forceinline__ void start(const XT* row) {
+    const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      if constexpr (NT == 1) {
+        q[0][ks] = *(const v4u*)(row + 16 * ks + 8 * h);
+      } else {
+        float a[4], b[4];
+        load4(row + 16 * ks + 8 * h, a);
+        load4(row + 16 * ks + 8 * h + 4, b);
+        const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        v4u t[NT];
+        terms8<NT>(x, t);
+#pragma unroll
+        for (int k = 0; k < NT; ++k) q[k][ks] = t[k];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] = f16v{};
+    m = LOWEST;
+    l = 0.f;
+  }
+
+  // NB blocks of 32 keys in LDS, the first of them key `key0` of the segment; the row sees [lo, hi).
+  __device__ __forceinline__ void step(const uint8_t* kl, const uint8_t* vl, const float* sk, const float* sv, float c, bool all,
+                                       int key0, int lo, int hi) {
+    const int lane = threadIdx.x & 63, i32 = lane & 31, h = lane >> 5;
+    f16v s[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      s[nb] = f16v{};
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const v4u k = *(const v4u*)(kl + (32 * nb + i32) * PITCH + 32 * ks + 16 * h);
+#pragma unroll
+        for (int t = NT - 1; t >= 0; --t) s[nb] = dot(k, q[t][ks], s[nb]);
+      }
+    }
+    // scores in powers of two, from here on; what the row does not see: -infinity
+    float most = -INFINITY;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        if constexpr (KV == NSX_DT_BF16) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) s[nb][e + k] *= c;
+        } else {
+          const v4f f = *(const v4f*)(sk + 32 * nb + 2 * e + 4 * h);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) s[nb][e + k] *= f[k];
+        }
+        if (!all) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int key = key0 + 32 * nb + 2 * e + 4 * h + k;
+            s[nb][e + k] = key >= lo && key < hi ? s[nb][e + k] : -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) most = fmaxf(most, s[nb][e + k]);
+      }
+    most = other_half_max(most);
+    // The reference moves only when a score is 2^8 above it: weights stay below 2^8, and the sums are seldom rescaled.
+    if (__any(most > m + 8.f)) {
+      const float to = most > m + 8.f ? most : m, f = __builtin_amdgcn_exp2f(m - to);
+      m = to;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][e] *= f;
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      v4u w[2][NT];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = __builtin_amdgcn_exp2f(s[nb][8 * kb + e] - m);
+          l += x[e];
+        }
+        if constexpr (KV != NSX_DT_BF16) {
+#pragma unroll
+          for (int e = 0; e < 8; e += 4) {
+            const v4f f = *(const v4f*)(sv + 32 * nb + 16 * kb + 2 * e + 4 * h);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[e + k] *= f[k];
+          }
+        }
+        terms8<NT>(x, w[kb]);
+      }
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          // values of dimension 32 i + lane % 32, keys 16 kb + 4 h .. + 3 and 8 behind them
+          const uint8_t* at = vl + (32 * nb + 16 * kb + 4 * h + ((lane & 15) >> 2)) * PITCH +
+                              2 * (32 * i + 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
+          const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s4*)at);
+          const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s4*)(at + 8 * PITCH));
+          const v2u a2 = __builtin_bit_cast(v2u, a), b2 = __builtin_bit_cast(v2u, b);
+          const v4u v = {a2[0], a2[1], b2[0], b2[1]};
+#pragma unroll
+          for (int t = NT - 1; t >= 0; --t) acc[i] = dot(v, w[kb][t], acc[i]);
+        }
+    }
+  }
+  __device__ __forceinline__ bool finite() const {
+    float z = l * 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) z += acc[i][e] * 0.f;
+    return z == 0.f;
+  }
+};
+
+// 16-byte pieces of KEYS rows of k and v (and their scales) by THREADS threads: from memory to registers, then to LDS as bf16.
+template <int KV, int D, int KEYS, int THREADS>
+struct Stage {
+  static constexpr int PIECES = D / Codes<KV>::PER, N = KEYS * PIECES / THREADS, PITCH = 2 * D + 16;
+  v4u k[N], v[N];
+  float s;
+  __device__ __forceinline__ void load(const Place& p, int t0, int last, int t) {  // rows t0 .., none past `last`
+    const uint8_t *kp = p.k + (int64_t)t0 * (D * Codes<KV>::BYTES), *vp = p.v + (int64_t)t0 * (D * Codes<KV>::BYTES);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int x = t + THREADS * i, at = min(x / PIECES, last - t0) * (D * Codes<KV>::BYTES) + x % PIECES * 16;
+      k[i] = *(const v4u*)(kp + at);
+      v[i] = *(const v4u*)(vp + at);
+    }
+    if constexpr (KV != NSX_DT_BF16) {
+      static_assert(THREADS >= 2 * KEYS, "a thread per scale");
+      if (t < 2 * KEYS) s = (t < KEYS ? p.ks : p.vs)[t0 + min(t % KEYS, last - t0)];
+    }
+  }
+  __device__ __forceinline__ void store(uint8_t* kl, uint8_t* vl, float* sc, float c, int t) const {  // sc: KEYS of k, KEYS of v
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int x = t + THREADS * i, at = x / PIECES * PITCH + x % PIECES * (2 * Codes<KV>::PER);
+      Codes<KV>::put(kl + at, k[i]);
+      Codes<KV>::put(vl + at, v[i]);
+    }
+    if constexpr (KV != NSX_DT_BF16) {
+      if (t < 2 * KEYS) sc[t] = t < KEYS ? s * c : s;
+    }
+  }
+};
+
+template <int D>
+constexpr int attn_lds() {
+  return 2 * 2 * 64 * (2 * D + 16) + 2048;  // two stages of 64 keys (or four waves' of 32), scales; then sums to be joined
+}
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
+// A workgroup's rows over its split of a segment. SHARED: its four waves take 32 rows each of 128 and share every stage of 64
+// keys; else all of them take the same 32 rows, each every fourth stage of 32 keys, and their sums are joined in LDS.
+template <typename XT, int KV, int D, int NT, bool SHARED>
+__device__ __forceinline__ void attend(const AttnArgs& a, const Place& p, int nsplit, uint8_t* lds) {
+  constexpr int KEYS = SHARED ? 64 : 32, THREADS = SHARED ? 256 : 64, PITCH = 2 * D + 16, TILE = KEYS * PITCH;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i32 = lane & 31, h = lane >> 5;
+  const int64_t r = p.r0 + (SHARED ? AT_ROWS * wave : 0) + i32;
+  const Row row(a, p, r);
+  const bool mine = r < p.rows;
+  // keys that all live rows of the wave see, [lo1, hi0), and that any of the workgroup's does, [w0, w1)
+  const int lo0 = wave_min(row.live ? row.lo : 0x7fffffff), lo1 = -wave_min(row.live ? -row.lo : 0);
+  const int hi0 = wave_min(row.live ? row.hi : 0x7fffffff), hi1 = -wave_min(row.live ? -row.hi : 0);
+  int w0 = lo0, w1 = hi1;
+  if constexpr (SHARED) {
+    int2* range = (int2*)lds;
+    if (lane == 0) range[wave] = int2{lo0, hi1};
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < AT_NW; ++i) w0 = min(w0, range[i].x), w1 = max(w1, range[i].y);
+    __syncthreads();
+  }
+  const int tiles = w1 > w0 ? (w1 - w0 + KEYS - 1) / KEYS : 0;
+  int per = (tiles + nsplit - 1) / nsplit;
+  if (!SHARED) per = (per + AT_NW - 1) / AT_NW * AT_NW;
+  const int first = min(p.split * per, tiles), end = min(first + per, tiles);
+  const int t0 = w0 + first * KEYS, t1 = min(w1, w0 + end * KEYS);
+
+  Wave<KV, D, NT, KEYS / 32> w;
+  w.start((const XT*)a.q + (row.tok * a.H + row.h) * D);
+  Stage<KV, D, KEYS, THREADS> st;
+  uint8_t* tile = lds + (SHARED ? 0 : 2 * TILE * wave);
+  float* scales = (float*)(lds + 2 * 2 * 64 * PITCH) + (SHARED ? 0 : 2 * KEYS * wave);
+  const int t = SHARED ? threadIdx.x : lane, step = SHARED ? 1 : AT_NW;
+  int i = first + (SHARED ? 0 : wave), buf = 0;
+  if (i < end) st.load(p, w0 + i * KEYS, w1 - 1, t);
+  for (; i < end; i += step) {
+    uint8_t* kl = tile + (SHARED ? buf * 2 * TILE : 0);
+    float* sc = scales + (SHARED ? buf * 2 * KEYS : 0);
+    st.store(kl, kl + TILE, sc, a.scale2, t);
+    if (i + step < end) st.load(p, w0 + (i + step) * KEYS, w1 - 1, t);
+    if constexpr (SHARED) nsx_lds_barrier();
+    else __builtin_amdgcn_wave_barrier();
+    const int key0 = w0 + i * KEYS;
+    w.step(kl, kl + TILE, sc, sc + KEYS, a.scale2, key0 >= lo1 && key0 + KEYS <= hi0, key0, row.lo, row.hi);
+    buf ^= 1;
+    if constexpr (!SHARED) __builtin_amdgcn_wave_barrier();
+  }
+  const bool fine = w.finite();
+  w.l = other_half_sum(w.l);
+  const uint64_t odd = __ballot(!fine && mine && row.live);
+  uint32_t bad = (uint32_t)odd | (uint32_t)(odd >> 32);
+  const End<XT, D> fin{a, p};
+  if constexpr (SHARED) {
+    if (mine && !(bad >> i32 & 1)) {
+      const float f = fin.factor(row, w.m, w.l, h == 0);
+#pragma unroll
+      for (int blk = 0; blk < D / 32; ++blk)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const float x[4] = {w.acc[blk][e], w.acc[blk][e + 1], w.acc[blk][e + 2], w.acc[blk][e + 3]};
+          fin.store(row, 32 * blk + 2 * e + 4 * h, f, x);
+        }
+    }
+    for (; bad; bad &= bad - 1) row_alone<XT, KV, D>(a, p, p.r0 + AT_ROWS * wave + __builtin_ctz(bad), t0, t1);
+  } else {
+    // the waves' sums, on the largest of their references
+    constexpr int OP = D + 4;
+    float* sums = (float*)lds;                                  // [wave][row][OP]
+    float2* ml = (float2*)(lds + 2 * 2 * 64 * PITCH);           // [wave][row]
+    uint32_t* odds = (uint32_t*)(ml + AT_NW * AT_ROWS);
+    static_assert(AT_NW * AT_ROWS * OP * 4 <= 2 * 2 * 64 * PITCH && AT_NW * (AT_ROWS * 8 + 4) <= 2048, "LDS");
+    __syncthreads();
+    if (h == 0) ml[wave * AT_ROWS + i32] = float2{w.m, w.l};
+    if (lane == 0) odds[wave] = bad;
+    __syncthreads();
+    bad = odds[0] | odds[1] | odds[2] | odds[3];
+    float M = LOWEST, L = 0.f;
+#pragma unroll
+    for (int k = 0; k < AT_NW; ++k) M = fmaxf(M, ml[k * AT_ROWS + i32].x);
+#pragma unroll
+    for (int k = 0; k < AT_NW; ++k) {
+      const float2 x = ml[k * AT_ROWS + i32];
+      L = fmaf(x.y, __builtin_amdgcn_exp2f(x.x - M), L);
+    }
+    const float f = __builtin_amdgcn_exp2f(w.m - M);
+#pragma unroll
+    for (int blk = 0; blk < D / 32; ++blk)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *(v4f*)(sums + (wave * AT_ROWS + i32) * OP + 32 * blk + 2 * e + 4 * h) =
+            v4f{w.acc[blk][e] * f, w.acc[blk][e + 1] * f, w.acc[blk][e + 2] * f, w.acc[blk][e + 3] * f};
+    __syncthreads();
+    // a wave a quarter of the dimensions of every row, two lanes a row
+    if (mine && !(bad >> i32 & 1)) {
+      const float y = fin.factor(row, M, L, threadIdx.x < 32);
+#pragma unroll
+      for (int e = 0; e < D / 8; e += 4) {
+        const int d = D / 4 * wave + D / 8 * h + e;
+        float x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          x[k] = (sums[i32 * OP + d + k] + sums[(AT_ROWS + i32) * OP + d + k]) +
+                 (sums[(2 * AT_ROWS + i32) * OP + d + k] + sums[(3 * AT_ROWS + i32) * OP + d + k]);
+        fin.store(row, d, y, x);
+      }
+    }
+    for (int k = 0; bad; bad &= bad - 1, ++k)
+      if (k % AT_NW == wave) row_alone<XT, KV, D>(a, p, p.r0 + __builtin_ctz(bad), t0, t1);
+  }
+}
+
+template <typename XT>
+constexpr int attn_terms() {
+  // bf16 rows and codes of 8 bits are bf16's own; queries and weights are as many bf16 terms as their type has bytes of bits
+  return std::is_same_v<XT, float> ? 3 : std::is_same_v<XT, Half> ? 2 : 1;
+}
+
+template <typename XT, int KV, int D>
+__global__ __launch_bounds__(256, (attn_terms<XT>() == 3 && D == 128 ? 1 : 2)) void attn_kernel(AttnArgs a) {
+  extern __shared__ __align__(16) uint8_t lds[];
+  constexpr int NT = attn_terms<XT>();
+  Place p;
+  const bool own = (int)blockIdx.x >= a.pblocks;
+  const AttnArgs::Cut cut = own ? a.ocut : a.pcut;
+  const KvRows& kv = own ? a.kv : a.pre;
+  // Workgroups go to the chip's eight parts (a cache each) in turn: those of one run of keys to the same one.
+  const int id = own ? blockIdx.x - a.pblocks : blockIdx.x;
+  const int units = (own ? (int)a.kv.n_seq : 1) * a.G * cut.splits;
+  const int eight = id / (8 * cut.tiles), left = min(8, units - 8 * eight), in = id - eight * 8 * cut.tiles;
+  const int unit = 8 * eight + in % left, tile = in / left;
+  p.own = own;
+  p.split = unit % cut.splits;
+  p.slot = p.split + (own ? a.pcut.splits : 0);
+  p.g = unit / cut.splits % a.G;
+  p.b = unit / cut.splits / a.G;
+  p.rows = (own ? a.n : a.kv.n_seq * a.n) * a.rep;
+  p.r0 = (int64_t)tile * (cut.shared ? AT_NW * AT_ROWS : AT_ROWS);
+  p.P = a.pre.n_seq ? (int)min((int64_t)max(*a.pre.pos, 0), a.pre.ctx_max) : 0;
+  const int64_t base = (own ? p.b * a.G + p.g : p.g) * kv.ctx_max;
+  p.k = (const uint8_t*)kv.k + base * (D * Codes<KV>::BYTES);
+  p.v = (const uint8_t*)kv.v + base * (D * Codes<KV>::BYTES);
+  p.ks = kv.ks + (KV == NSX_DT_BF16 ? 0 : base);
+  p.vs = kv.vs + (KV == NSX_DT_BF16 ? 0 : base);
+  if (cut.shared) attend<XT, KV, D, NT, true>(a, p, cut.splits, lds);
+  else attend<XT, KV, D, NT, false>(a, p, cut.splits, lds);
+}
+
+// The splits' sums of a (token, head) and its sink: a wave each, D / 4 lanes a split.
+template <typename XT, int D>
+__global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
+  constexpr int LPR = D / 4, AT_ONCE = 64 / LPR;
+  const int lane = threadIdx.x & 63;
+  const int64_t rows = a.kv.n_seq * a.n * a.H, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int64_t tok = row / a.H, b = tok / a.n;
+  const int h = (int)(row - tok * a.H);
+  const bool live = !a.counts || tok - b * a.n < a.counts[b];
+  const float2* ml = (const float2*)(a.part + rows * a.splits * D) + row * a.splits;
+  float m = LOWEST, l = 0.f;
+  if (lane < a.splits) {
+    const float2 x = ml[lane];
+    m = x.x;
+    l = x.y;
+  }
+  const float sink = a.sinks ? a.sinks[h] * LOG2E : LOWEST;
+  float M = fmaxf(m, sink);
+#pragma unroll
+  for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+  const float w = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - M);
+  const float Z = nsx_wave_sum(w == 0.f ? 0.f : w * l) + (a.sinks ? __builtin_amdgcn_exp2f(sink - M) : 0.f);
+  const float* part = a.part + row * a.splits * D + 4 * (lane % LPR);
+  float x[4] = {};
+  for (int s0 = 0; s0 < a.splits; s0 += AT_ONCE) {
+    const int s = s0 + lane / LPR;
+    const float ws = __shfl(w, min(s, 63), 64);
+    if (s < a.splits && ws != 0.f) {
+      const v4f y = *(const v4f*)(part + (int64_t)s * D);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = fmaf(ws, y[k], x[k]);
+    }
+  }
+#pragma unroll
+  for (int o = LPR; o < 64; o *= 2)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] += __shfl_xor(x[k], o, 64);
+  const float f = !live || Z == 0.f ? 0.f : 1.f / Z;
+  if (lane < LPR) {
+    float y[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y[k] = f == 0.f ? 0.f : x[k] * f;
+    store4((XT*)a.out + row * D + 4 * lane, y);
+  }
+}
+
+// How a call's rows and keys are cut into workgroups: by the caches' sizes, not their lengths, so that a captured call serves
+// every length.
+struct Plan {
+  AttnArgs::Cut pre, own;
+  int64_t pblocks, oblocks;
+  int splits;
+};
+Plan attn_plan(int G, int rep, int64_t B, int64_t n, int64_t ctx_max, int64_t prefix_max, int window) {
+  Plan p;
+  const int64_t prows = B * n * rep, orows = n * rep;
+  const int64_t pk = window > 0 ? std::min<int64_t>(prefix_max, window + n) : prefix_max;
+  const int64_t ok = window > 0 ? std::min<int64_t>(ctx_max, window + n) : ctx_max;
+  // pieces of 32 rows x 32 keys, and how many of them a wave takes where the chip's 2048 waves share them
+  const int64_t pw = prefix_max ? G * nsx_cdiv(prows, AT_ROWS) * nsx_cdiv(pk, 32) : 0;
+  const int64_t ow = B * G * nsx_cdiv(orows, AT_ROWS) * nsx_cdiv(ok, 32);
+  const int64_t each = std::max<int64_t>(8, nsx_cdiv(pw + ow, 2048));
+  auto cut = [&](int64_t rows, int64_t keys) {
+    AttnArgs::Cut c;
+    c.shared = rows > 2 * AT_ROWS;
+    c.tiles = (int)nsx_cdiv(rows, c.shared ? AT_NW * AT_ROWS : AT_ROWS);
+    c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(AT_MAX_SPLIT / 2, nsx_cdiv(nsx_cdiv(keys, 32), c.shared ? each : AT_NW * each)));
+    return c;
+  };
+  p.own = cut(orows, ok);
+  p.pre = prefix_max ? cut(prows, pk) : AttnArgs::Cut{0, 0, 0};
+  p.pblocks = (int64_t)G * p.pre.tiles * p.pre.splits;
+  p.oblocks = B * G * p.own.tiles * p.own.splits;
+  p.splits = p.pre.splits + p.own.splits;
+  return p;
 }
 
 // ---------------------------------------------------------------------------
@@ -473,7 +1015,11 @@ extern "C" int nsx_load_rows(const nsx_kv_rows* kv, int kv_type, int n_kv, int h
 
 extern "C" int64_t nsx_batch_attn_workspace_bytes(int n_head, int n_kv, int head_dim, int64_t n_seq, int64_t n,
                                                   int64_t ctx_max, int64_t prefix_max, int window) {
-  return 16;
+  if (batch_heads(n_head, n_kv, head_dim) != NSX_OK || n_seq <= 0 || n_seq >= 65536 || n <= 0 || n >= (1ll << 24) ||
+      n_seq * n >= (1ll << 24) || ctx_max <= 0 || ctx_max >= (1ll << 30) || prefix_max < 0 || prefix_max >= (1ll << 30) || window < 0)
+    return -1;
+  const Plan p = attn_plan(n_kv, n_head / n_kv, n_seq, n, ctx_max, prefix_max, window);
+  return p.splits > 1 ? n_seq * n * n_head * p.splits * (head_dim + 2) * 4 : 16;
 }
 
 extern "C" int nsx_batch_attn(const void* q, int x_dtype, const nsx_kv_rows* kv, const nsx_kv_rows* prefix, int kv_type,
@@ -496,10 +1042,19 @@ extern "C" int nsx_batch_attn(const void* q, int x_dtype, const nsx_kv_rows* kv,
                                                       prefix ? prefix->ctx_max : 0, window);
   NSX_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, NSX_EINVAL,
               "workspace of %lld bytes, %lld needed, 16-byte aligned", (long long)workspace_bytes, (long long)need);
+  const Plan plan = attn_plan(n_kv, n_head / n_kv, kv->n_seq, n, kv->ctx_max, prefix ? prefix->ctx_max : 0, window);
+  NSX_REQUIRE(plan.pblocks + plan.oblocks < (1ll << 24) && kv->n_seq * n * n_head < (1ll << 26), NSX_EINVAL,
+              "%lld tokens of %d heads: too many for one call", (long long)(kv->n_seq * n), n_head);
   const AttnArgs a{q, kv_rows(kv), prefix ? kv_rows(prefix) : KvRows{}, counts, sinks, n_head, n_kv, n_head / n_kv, window, n,
-                   scale, (float*)workspace, out};
+                   scale * LOG2E, (float*)workspace, out, plan.pre, plan.own, (int)plan.pblocks, plan.splits};
   return with_types(x_dtype, kv_type, head_dim, [&](auto x, auto t, auto d) {
-    return nsx_launch(attn_kernel<decltype(x), t(), d()>, dim3((unsigned)(kv->n_seq * n), n_head), dim3(64), 0,
-                      (hipStream_t)stream, a);
+    using XT = decltype(x);
+    constexpr int LDS = attn_lds<d()>();
+    auto* kernel = attn_kernel<XT, t(), d()>;
+    if (const int rc = nsx_allow_lds((const void*)kernel, LDS)) return rc;
+    if (const int rc = nsx_launch(kernel, dim3((unsigned)(plan.pblocks + plan.oblocks)), dim3(256), LDS, (hipStream_t)stream, a))
+      return rc;
+    if (plan.splits == 1) return (int)NSX_OK;
+    return nsx_launch(join_kernel<XT, d()>, dim3((unsigned)nsx_cdiv(kv->n_seq * n * n_head, 4)), dim3(256), 0, (hipStream_t)stream, a);
   });
 }
