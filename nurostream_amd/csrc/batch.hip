@@ -300,11 +300,11 @@ struct AttnArgs {
   float scale2;  // scale * log2(e): the softmax is taken in powers of two
   float* part;   // [token][head][splits][D], then [token][head][splits] of (maximum, sum)
   void* out;
-  // what a segment's rows are cut into: row tiles, splits of the keys, whether a workgroup's waves share keys
+  // what rows are cut into: tiles of so many rows, splits of their keys
   struct Cut {
-    int tiles, splits, shared;
+    int rows, tiles, splits;
   } pcut, ocut;
-  int pblocks, splits;  // workgroups of the prefix; splits of both
+  int pblocks, splits;  // workgroups that take the prefix's keys alone; splits of all of a row's keys
 };
 
 // A cache row's elements as bf16, which holds all of their bits, 16 bytes of the row at a time.
@@ -378,33 +378,44 @@ __device__ __forceinline__ float other_half_sum(float x) {
   return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
 }
 
-// Where a workgroup stands: a segment (the prefix, or a sequence's own rows) of a kv head, its rows r0 .. and its split.
-struct Place {
+// Rows that a workgroup's keys come from: the prefix's, or a sequence's own, of a kv head.
+struct Source {
   const uint8_t *k, *v;
   const float *ks, *vs;
-  bool own;
-  int g, split, slot;     // kv head; split of the segment, of both segments
-  int64_t b, r0, rows;    // sequence (own); first row of the workgroup, rows of the segment
-  int P;                  // the prefix's length
 };
-// Row r of a place's segment: its token and head, and the keys [lo, hi) of the segment that it sees.
+// Where a workgroup stands: rows r0 .. of a kv head's rows (all sequences' or, with `own`, sequence b's), which see keys of the
+// prefix (source 0), of their sequence (1), or both, one after the other; its split of those keys.
+struct Place {
+  Source src[2];
+  bool own, with[2];
+  int g, split, splits, slot;  // kv head; split of so many; which of the splits of all of a row's keys
+  int b, r0, rows;
+  int P;  // the prefix's length
+};
+// Row r of a place (the last one's in place of those behind it): its token and head, and the keys [lo, hi) that it sees of
+// each source.
 struct Row {
-  int64_t tok;
-  int h, lo, hi;
+  int tok, h, lo[2], hi[2];
   bool live;
-  __device__ __forceinline__ Row(const AttnArgs& a, const Place& p, int64_t r) {
-    r = r < p.rows ? r : p.rows - 1;
-    const int64_t t = r / a.rep;
-    tok = p.own ? p.b * a.n + t : t;
-    h = p.g * a.rep + (int)(r - t * a.rep);
-    const int64_t b = p.own ? p.b : tok / a.n, j = tok - b * a.n, row = (int64_t)a.kv.pos[b] + j;
-    live = !a.counts || j < a.counts[b];
+  __device__ __forceinline__ Row(const AttnArgs& a, const Place& p, int r) {
+    const uint32_t x = (uint32_t)min(r, p.rows - 1), t = x / (uint32_t)a.rep;
+    tok = p.own ? p.b * (int)a.n + (int)t : (int)t;
+    h = p.g * a.rep + (int)(x - t * (uint32_t)a.rep);
+    const uint32_t b = p.own ? p.b : a.n == 1 ? t : t / (uint32_t)a.n, j = p.own ? t : a.n == 1 ? 0 : t - b * (uint32_t)a.n;
+    const int64_t row = (int64_t)a.kv.pos[b] + j;
+    live = !a.counts || (int)j < a.counts[b];
     const int64_t first = a.window > 0 ? p.P + row + 1 - a.window : 0;
-    const int64_t end = p.own ? (row + 1 < a.kv.ctx_max ? row + 1 : a.kv.ctx_max) : p.P;
-    const int64_t from = p.own ? first - p.P : first;
-    hi = (int)(end > 0 ? end : 0);
-    lo = (int)(from < 0 ? 0 : from < hi ? from : hi);
+    const int64_t end = row + 1 < 0 ? 0 : row + 1 < a.kv.ctx_max ? row + 1 : a.kv.ctx_max;
+    hi[0] = p.with[0] ? p.P : 0;
+    hi[1] = p.with[1] ? (int)end : 0;
+    lo[0] = (int)(first < 0 ? 0 : first < hi[0] ? first : hi[0]);
+    lo[1] = (int)(first < p.P ? 0 : first - p.P < hi[1] ? first - p.P : hi[1]);
   }
+};
+
+struct At {
+  int tok, h;
+  bool live;
 };
 
 // A row's (or split's) end: its maximum (of scores in powers of two), sum and D values over the sum's weights.
@@ -412,15 +423,15 @@ template <typename XT, int D>
 struct End {
   const AttnArgs& a;
   const Place& p;
-  __device__ __forceinline__ float* part(const Row& r) const {
-    return a.part + ((r.tok * a.H + r.h) * a.splits + p.slot) * D;
+  __device__ __forceinline__ float* part(const At& r) const {
+    return a.part + ((int64_t)(r.tok * a.H + r.h) * a.splits + p.slot) * D;
   }
   // The factor that values are stored with: 1 for a part, what divides by the whole sum for the answer.
-  __device__ __forceinline__ float factor(const Row& r, float m, float l, bool first) const {
+  __device__ __forceinline__ float factor(const At& r, float m, float l, bool first) const {
     if (a.splits > 1) {
       if (first) {
         float2* ml = (float2*)(a.part + (int64_t)(a.kv.n_seq * a.n * a.H) * a.splits * D);
-        ml[(r.tok * a.H + r.h) * a.splits + p.slot] = float2{m, l};
+        ml[(int64_t)(r.tok * a.H + r.h) * a.splits + p.slot] = float2{m, l};
       }
       return 1.f;
     }
@@ -434,94 +445,117 @@ struct End {
     return l == 0.f ? 0.f : f / l;
   }
   // Values d .. d + 3
-  __device__ __forceinline__ void store(const Row& r, int d, float f, const float (&x)[4]) const {
+  __device__ __forceinline__ void store(const At& r, int d, float f, const float (&x)[4]) const {
     if (a.splits > 1) {
       *(v4f*)(part(r) + d) = v4f{x[0], x[1], x[2], x[3]};
     } else {
       float y[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[i] = f == 0.f ? 0.f : x[i] * f;  // (a token that is not there: zero whatever x is)
-      store4((XT*)a.out + (r.tok * a.H + r.h) * D + d, y);
+      store4((XT*)a.out + (int64_t)(r.tok * a.H + r.h) * D + d, y);
     }
+  }
+};
+
+// The keys of a workgroup: of each source's rows [from, to), those that any of its rows sees, in tiles, the tiles from `first`
+// to `end` of both.
+struct Range {
+  int from[2], to[2], tiles[2], first, end;
+  template <int KEYS>
+  __device__ __forceinline__ void split(const Place& p, int round) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) tiles[i] = to[i] > from[i] ? (to[i] - from[i] + KEYS - 1) / KEYS : 0;
+    const int all = tiles[0] + tiles[1], per = ((all + p.splits - 1) / p.splits + round - 1) / round * round;
+    first = min(p.split * per, all);
+    end = min(first + per, all);
   }
 };
 
 // A row once more, key by key and none that it does not see: for rows whose sums are not finite, as an infinity or a NaN
 // beside a weight of zero makes them in a product of matrices. A wave's work.
-template <typename XT, int KV, int D>
-__device__ __forceinline__ void row_alone(const AttnArgs& a, const Place& p, int64_t r, int t0, int t1) {
+template <typename XT, int KV, int D, int KEYS>
+__device__ __forceinline__ void row_alone(const AttnArgs& a, const Place& p, const Range& w, int r) {
   const int lane = threadIdx.x & 63;
   const Row row(a, p, r);
-  const XT* q = (const XT*)a.q + (row.tok * a.H + row.h) * D;
-  const int lo = max(row.lo, t0), hi = min(row.hi, t1);
+  const XT* q = (const XT*)a.q + (int64_t)(row.tok * a.H + row.h) * D;
   float m = LOWEST, l = 0.f, acc[D / 64] = {};
-  for (int t = lo; t < hi; t += 64) {
-    const int key = t + lane;
-    float s = -INFINITY;
-    if (key < hi) {
-      s = 0.f;
-      for (int c = 0; c < D / 8; ++c) {
-        float x[8], lo4[4], hi4[4];
-        get_row<KV, D>(p.k, p.ks, key, c, x);
-        load4(q + 4 * c, lo4);
-        load4(q + D / 2 + 4 * c, hi4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s = fmaf(lo4[i], x[i], fmaf(hi4[i], x[4 + i], s));
-      }
-      s *= a.scale2;
-    }
-    float M = s;
+  for (int i = 0; i < 2; ++i) {
+    const Source src = p.src[i];
+    const int t0 = i ? max(w.first - w.tiles[0], 0) : min(w.first, w.tiles[0]), t1 = i ? max(w.end - w.tiles[0], 0) : min(w.end, w.tiles[0]);
+    const int lo = max(row.lo[i], w.from[i] + t0 * KEYS), hi = t1 > t0 ? min(row.hi[i], w.from[i] + t1 * KEYS) : 0;
+#pragma unroll 1
+    for (int t = lo; t < hi; t += 64) {
+      const int key = t + lane;
+      float s = -INFINITY;
+      if (key < hi) {
+        s = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < D / 8; ++c) {
+          float x[8], lo4[4], hi4[4];
+          get_row<KV, D>(src.k, src.ks, key, c, x);
+          load4(q + 4 * c, lo4);
+          load4(q + D / 2 + 4 * c, hi4);
 #pragma unroll
-    for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-    M = fmaxf(M, m);
-    const float w = key < hi ? __builtin_amdgcn_exp2f(s - M) : 0.f, f = __builtin_amdgcn_exp2f(m - M);
-    l = l * f + nsx_wave_sum(w);
-    m = M;
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) acc[i] *= f;
-    for (int u = 0; u < min(64, hi - t); ++u) {
-      const float wu = __shfl(w, u, 64);
-#pragma unroll
-      for (int i = 0; i < D / 64; ++i) {
-        const int64_t e = (int64_t)(t + u) * D + lane + 64 * i;
-        float x;
-        if constexpr (KV == NSX_DT_BF16) {
-          x = to_f(((const Bf16*)p.v)[e]);
-        } else {
-          float c[4];
-          codes4<KV>(p.v[e], c);
-          x = c[0] * p.vs[t + u];
+          for (int k = 0; k < 4; ++k) s = fmaf(lo4[k], x[k], fmaf(hi4[k], x[4 + k], s));
         }
-        acc[i] = fmaf(wu, x, acc[i]);
+        s *= a.scale2;
+      }
+      float M = s;
+#pragma unroll
+      for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+      M = fmaxf(M, m);
+      const float e = key < hi ? __builtin_amdgcn_exp2f(s - M) : 0.f, f = __builtin_amdgcn_exp2f(m - M);
+      l = l * f + nsx_wave_sum(e);
+      m = M;
+#pragma unroll
+      for (int k = 0; k < D / 64; ++k) acc[k] *= f;
+#pragma unroll 1
+      for (int u = 0; u < min(64, hi - t); ++u) {
+        const float eu = __shfl(e, u, 64);
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k) {
+          const int64_t at = (int64_t)(t + u) * D + lane + 64 * k;
+          float x;
+          if constexpr (KV == NSX_DT_BF16) {
+            x = to_f(((const Bf16*)src.v)[at]);
+          } else {
+            float c[4];
+            codes4<KV>(src.v[at], c);
+            x = c[0] * src.vs[t + u];
+          }
+          acc[k] = fmaf(eu, x, acc[k]);
+        }
       }
     }
   }
   const End<XT, D> end{a, p};
-  const float f = end.factor(row, m, l, lane == 0);
+  const At at{row.tok, row.h, row.live};
+  const float f = end.factor(at, m, l, lane == 0);
 #pragma unroll
   for (int i = 0; i < D / 64; ++i) {
-    if (a.splits > 1) end.part(row)[lane + 64 * i] = acc[i];
-    else from_f(((XT*)a.out + (row.tok * a.H + row.h) * D)[lane + 64 * i], f == 0.f ? 0.f : acc[i] * f);
+    if (a.splits > 1) end.part(at)[lane + 64 * i] = acc[i];
+    else from_f(((XT*)a.out + (int64_t)(row.tok * a.H + row.h) * D)[lane + 64 * i], f == 0.f ? 0.f : acc[i] * f);
   }
 }
 
-// A wave's 32 rows over its keys. Scores are K Q^T, so that a lane holds 16 of 32 keys' scores of one row (lane % 32; the other
-// lane of the row holds the others), and its weights are at once the second operand of V^T W^T, of which it holds D / 2 values
-// of the same row. The operand's order of keys is the scores' own, and V's rows are read from LDS in it, transposed.
-template <int KV, int D, int NT, int NB>
+// A wave's RB x 32 rows over its keys. Scores are K Q^T, so that a lane holds 16 of 32 keys' scores of one row (lane % 32; the
+// other lane of the row holds the others), and its weights are at once the second operand of V^T W^T, of which it holds D / 2
+// values of the same row. The operand's order of keys is the scores' own, and V's rows are read from LDS in it, transposed.
+template <int KV, int D, int NT, int NB, int RB>
 struct Wave {
   static constexpr int PITCH = 2 * D + 16;  // of a row in LDS: reads of 8 rows at once fall on different banks
-  v4u q[NT][D / 16];
-  f16v acc[D / 32];
-  float m, l;
+  v4u q[RB][NT][D / 16];
+  f16v acc[RB][D / 32];
+  float m[RB], l[RB];
 
   template <typename XT>
-  __device__ __forceinline__ void start(const XT* row) {
+  __device__ __forceinline__ void start(int rb, const XT* row) {
     const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
       if constexpr (NT == 1) {
-        q[0][ks] = *(const v4u*)(row + 16 * ks + 8 * h);
+        q[rb][0][ks] = *(const v4u*)(row + 16 * ks + 8 * h);
       } else {
         float a[4], b[4];
         load4(row + 16 * ks + 8 * h, a);
@@ -530,85 +564,93 @@ struct Wave {
         v4u t[NT];
         terms8<NT>(x, t);
 #pragma unroll
-        for (int k = 0; k < NT; ++k) q[k][ks] = t[k];
+        for (int k = 0; k < NT; ++k) q[rb][k][ks] = t[k];
       }
     }
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] = f16v{};
-    m = LOWEST;
-    l = 0.f;
+    for (int i = 0; i < D / 32; ++i) acc[rb][i] = f16v{};
+    m[rb] = LOWEST;
+    l[rb] = 0.f;
   }
 
-  // NB blocks of 32 keys in LDS, the first of them key `key0` of the segment; the row sees [lo, hi).
+  // NB blocks of 32 keys in LDS, the first of them key `key0` of its source; row rb of the lane sees [lo, hi) (`all`: these
+  // keys at least).
   __device__ __forceinline__ void step(const uint8_t* kl, const uint8_t* vl, const float* sk, const float* sv, float c, bool all,
-                                       int key0, int lo, int hi) {
+                                       int key0, const int (&lo)[RB], const int (&hi)[RB]) {
     const int lane = threadIdx.x & 63, i32 = lane & 31, h = lane >> 5;
-    f16v s[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      s[nb] = f16v{};
+      f16v s[RB];
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) s[rb] = f16v{};
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
         const v4u k = *(const v4u*)(kl + (32 * nb + i32) * PITCH + 32 * ks + 16 * h);
 #pragma unroll
-        for (int t = NT - 1; t >= 0; --t) s[nb] = dot(k, q[t][ks], s[nb]);
+        for (int t = NT - 1; t >= 0; --t)
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) s[rb] = dot(k, q[rb][t][ks], s[rb]);
       }
-    }
-    // scores in powers of two, from here on; what the row does not see: -infinity
-    float most = -INFINITY;
+      if constexpr (KV != NSX_DT_BF16) {  // (a score's factor is its key's scale, which has the one of all in it)
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        if constexpr (KV == NSX_DT_BF16) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) s[nb][e + k] *= c;
-        } else {
+        for (int e = 0; e < 16; e += 4) {
           const v4f f = *(const v4f*)(sk + 32 * nb + 2 * e + 4 * h);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) s[nb][e + k] *= f[k];
-        }
-        if (!all) {
+          for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int key = key0 + 32 * nb + 2 * e + 4 * h + k;
-            s[nb][e + k] = key >= lo && key < hi ? s[nb][e + k] : -INFINITY;
-          }
+            for (int k = 0; k < 4; ++k) s[rb][e + k] *= f[k];
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) most = fmaxf(most, s[nb][e + k]);
       }
-    most = other_half_max(most);
-    // The reference moves only when a score is 2^8 above it: weights stay below 2^8, and the sums are seldom rescaled.
-    if (__any(most > m + 8.f)) {
-      const float to = most > m + 8.f ? most : m, f = __builtin_amdgcn_exp2f(m - to);
-      m = to;
-      l *= f;
+      if (!all) {
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i)
+        for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][e] *= f;
-    }
+          for (int e = 0; e < 16; ++e) {
+            const int key = key0 + 32 * nb + 8 * (e >> 2) + 4 * h + (e & 3);
+            float x = key >= lo[rb] && key < hi[rb] ? s[rb][e] : -INFINITY;
+            asm volatile("" : "+v"(x));  // (a branch, not selects: few tiles take it)
+            s[rb][e] = x;
+          }
+      }
+      // The reference is an earlier maximum, moved only when a score is 8 above it: weights stay below 2^8, and the sums are
+      // seldom rescaled.
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      v4u w[2][NT];
+      for (int rb = 0; rb < RB; ++rb) {
+        float most = s[rb][0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) most = fmaxf(most, s[rb][e]);
+        most = other_half_max(most);
+        if (KV == NSX_DT_BF16) most *= c;
+        if (__any(most > m[rb] + 8.f)) {
+          const float to = fmaxf(most, m[rb]), by = __builtin_amdgcn_exp2f(m[rb] - to);
+          m[rb] = to;
+          l[rb] *= by;
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[rb][i][e] *= by;
+        }
+      }
+      v4u w[RB][2][NT];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] = __builtin_amdgcn_exp2f(s[nb][8 * kb + e] - m);
-          l += x[e];
-        }
+        v4f g[2];  // the values' scales
         if constexpr (KV != NSX_DT_BF16) {
 #pragma unroll
-          for (int e = 0; e < 8; e += 4) {
-            const v4f f = *(const v4f*)(sv + 32 * nb + 16 * kb + 2 * e + 4 * h);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) x[e + k] *= f[k];
-          }
+          for (int e = 0; e < 2; ++e) g[e] = *(const v4f*)(sv + 32 * nb + 16 * kb + 8 * e + 4 * h);
         }
-        terms8<NT>(x, w[kb]);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float y = s[rb][8 * kb + e];
+            x[e] = __builtin_amdgcn_exp2f(KV == NSX_DT_BF16 ? fmaf(y, c, -m[rb]) : y - m[rb]);
+            l[rb] += x[e];
+            if constexpr (KV != NSX_DT_BF16) x[e] *= g[e >> 2][e & 3];
+          }
+          terms8<NT>(x, w[rb][kb]);
+        }
       }
 #pragma unroll
       for (int i = 0; i < D / 32; ++i)
@@ -622,16 +664,18 @@ struct Wave {
           const v2u a2 = __builtin_bit_cast(v2u, a), b2 = __builtin_bit_cast(v2u, b);
           const v4u v = {a2[0], a2[1], b2[0], b2[1]};
 #pragma unroll
-          for (int t = NT - 1; t >= 0; --t) acc[i] = dot(v, w[kb][t], acc[i]);
+          for (int t = NT - 1; t >= 0; --t)
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) acc[rb][i] = dot(v, w[rb][kb][t], acc[rb][i]);
         }
     }
   }
-  __device__ __forceinline__ bool finite() const {
-    float z = l * 0.f;
+  __device__ __forceinline__ bool finite(int rb) const {
+    float z = l[rb] * 0.f;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) z += acc[i][e] * 0.f;
+      for (int e = 0; e < 16; ++e) z = fmaf(acc[rb][i][e], 0.f, z);
     return z == 0.f;
   }
 };
@@ -642,7 +686,7 @@ struct Stage {
   static constexpr int PIECES = D / Codes<KV>::PER, N = KEYS * PIECES / THREADS, PITCH = 2 * D + 16;
   v4u k[N], v[N];
   float s;
-  __device__ __forceinline__ void load(const Place& p, int t0, int last, int t) {  // rows t0 .., none past `last`
+  __device__ __forceinline__ void load(const Source& p, int t0, int last, int t) {  // rows t0 .., none past `last`
     const uint8_t *kp = p.k + (int64_t)t0 * (D * Codes<KV>::BYTES), *vp = p.v + (int64_t)t0 * (D * Codes<KV>::BYTES);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -672,85 +716,127 @@ template <int D>
 constexpr int attn_lds() {
   return 2 * 2 * 64 * (2 * D + 16) + 2048;  // two stages of 64 keys (or four waves' of 32), scales; then sums to be joined
 }
-__device__ __forceinline__ int wave_min(int v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
-  return v;
-}
-
-// A workgroup's rows over its split of a segment. SHARED: its four waves take 32 rows each of 128 and share every stage of 64
-// keys; else all of them take the same 32 rows, each every fourth stage of 32 keys, and their sums are joined in LDS.
-template <typename XT, int KV, int D, int NT, bool SHARED>
-__device__ __forceinline__ void attend(const AttnArgs& a, const Place& p, int nsplit, uint8_t* lds) {
+// A workgroup's rows over its keys. SHARED: its four waves take RB x 32 rows each and share every stage of 64 keys; else all
+// of them take the same 32 rows, each every fourth stage of 32 keys, and their sums are joined in LDS.
+template <typename XT, int KV, int D, int NT, bool SHARED, int RB>
+__device__ __forceinline__ void attend(const AttnArgs& a, const Place& p, uint8_t* lds) {
   constexpr int KEYS = SHARED ? 64 : 32, THREADS = SHARED ? 256 : 64, PITCH = 2 * D + 16, TILE = KEYS * PITCH;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i32 = lane & 31, h = lane >> 5;
-  const int64_t r = p.r0 + (SHARED ? AT_ROWS * wave : 0) + i32;
-  const Row row(a, p, r);
-  const bool mine = r < p.rows;
-  // keys that all live rows of the wave see, [lo1, hi0), and that any of the workgroup's does, [w0, w1)
-  const int lo0 = wave_min(row.live ? row.lo : 0x7fffffff), lo1 = -wave_min(row.live ? -row.lo : 0);
-  const int hi0 = wave_min(row.live ? row.hi : 0x7fffffff), hi1 = -wave_min(row.live ? -row.hi : 0);
-  int w0 = lo0, w1 = hi1;
+  const int r = p.r0 + (SHARED ? RB * AT_ROWS * wave : 0) + i32;
+  Wave<KV, D, NT, KEYS / 32, RB> w;
+  Stage<KV, D, KEYS, THREADS> st;
+  // of each source, the keys that any live row of the workgroup sees, and those that all of the wave's do
+  Range range;
+  int all0[2], all1[2], lo[2][RB], hi[2][RB], tok[RB], head[RB];
+  uint32_t least[2] = {~0u, ~0u}, most[2] = {0, 0}, latest[2] = {0, 0}, soonest[2] = {~0u, ~0u};
+  bool live[RB];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const Row row(a, p, r + AT_ROWS * rb);
+    tok[rb] = row.tok, head[rb] = row.h, live[rb] = row.live;
+    w.start(rb, (const XT*)a.q + (int64_t)(row.tok * a.H + row.h) * D);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      lo[i][rb] = row.lo[i], hi[i][rb] = row.hi[i];
+      if (row.live) {
+        least[i] = min(least[i], (uint32_t)row.lo[i]), latest[i] = max(latest[i], (uint32_t)row.lo[i]);
+        soonest[i] = min(soonest[i], (uint32_t)row.hi[i]), most[i] = max(most[i], (uint32_t)row.hi[i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    range.from[i] = 0, range.to[i] = 0, all0[i] = 0, all1[i] = 0;
+    if (p.with[i]) {
+      range.from[i] = (int)min(nsx_wave_min_u32(least[i]), 0x7fffffffu), range.to[i] = (int)nsx_wave_max_u32(most[i]);
+      all0[i] = (int)nsx_wave_max_u32(latest[i]), all1[i] = (int)min(nsx_wave_min_u32(soonest[i]), 0x7fffffffu);
+    }
+  }
   if constexpr (SHARED) {
-    int2* range = (int2*)lds;
-    if (lane == 0) range[wave] = int2{lo0, hi1};
+    int4* each = (int4*)lds;
+    if (lane == 0) each[wave] = int4{range.from[0], range.to[0], range.from[1], range.to[1]};
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < AT_NW; ++i) w0 = min(w0, range[i].x), w1 = max(w1, range[i].y);
+    for (int i = 0; i < AT_NW; ++i) {
+      const int4 x = each[i];
+      range.from[0] = min(range.from[0], __builtin_amdgcn_readfirstlane(x.x));
+      range.to[0] = max(range.to[0], __builtin_amdgcn_readfirstlane(x.y));
+      range.from[1] = min(range.from[1], __builtin_amdgcn_readfirstlane(x.z));
+      range.to[1] = max(range.to[1], __builtin_amdgcn_readfirstlane(x.w));
+    }
     __syncthreads();
   }
-  const int tiles = w1 > w0 ? (w1 - w0 + KEYS - 1) / KEYS : 0;
-  int per = (tiles + nsplit - 1) / nsplit;
-  if (!SHARED) per = (per + AT_NW - 1) / AT_NW * AT_NW;
-  const int first = min(p.split * per, tiles), end = min(first + per, tiles);
-  const int t0 = w0 + first * KEYS, t1 = min(w1, w0 + end * KEYS);
+  range.split<KEYS>(p, SHARED ? 1 : AT_NW);
 
-  Wave<KV, D, NT, KEYS / 32> w;
-  w.start((const XT*)a.q + (row.tok * a.H + row.h) * D);
-  Stage<KV, D, KEYS, THREADS> st;
   uint8_t* tile = lds + (SHARED ? 0 : 2 * TILE * wave);
   float* scales = (float*)(lds + 2 * 2 * 64 * PITCH) + (SHARED ? 0 : 2 * KEYS * wave);
   const int t = SHARED ? threadIdx.x : lane, step = SHARED ? 1 : AT_NW;
-  int i = first + (SHARED ? 0 : wave), buf = 0;
-  if (i < end) st.load(p, w0 + i * KEYS, w1 - 1, t);
-  for (; i < end; i += step) {
+  const int w0 = __builtin_amdgcn_readfirstlane(wave);
+  auto first_key = [&](int i) {  // of tile i, in its source
+    return i >= range.tiles[0] ? range.from[1] + (i - range.tiles[0]) * KEYS : range.from[0] + i * KEYS;
+  };
+  auto load = [&](int i) {
+    const bool o = i >= range.tiles[0];
+    const Source src{o ? p.src[1].k : p.src[0].k, o ? p.src[1].v : p.src[0].v, o ? p.src[1].ks : p.src[0].ks,
+                     o ? p.src[1].vs : p.src[0].vs};
+    st.load(src, first_key(i), (o ? range.to[1] : range.to[0]) - 1, t);
+  };
+  int i = range.first + (SHARED ? 0 : w0), buf = 0;
+  if (i < range.end) load(i);
+  for (; i < range.end; i += step) {
     uint8_t* kl = tile + (SHARED ? buf * 2 * TILE : 0);
     float* sc = scales + (SHARED ? buf * 2 * KEYS : 0);
     st.store(kl, kl + TILE, sc, a.scale2, t);
-    if (i + step < end) st.load(p, w0 + (i + step) * KEYS, w1 - 1, t);
+    if (i + step < range.end) load(i + step);
     if constexpr (SHARED) nsx_lds_barrier();
     else __builtin_amdgcn_wave_barrier();
-    const int key0 = w0 + i * KEYS;
-    w.step(kl, kl + TILE, sc, sc + KEYS, a.scale2, key0 >= lo1 && key0 + KEYS <= hi0, key0, row.lo, row.hi);
+    const bool o = i >= range.tiles[0];
+    const int key0 = first_key(i);
+    int from[RB], to[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) from[rb] = o ? lo[1][rb] : lo[0][rb], to[rb] = o ? hi[1][rb] : hi[0][rb];
+    const bool all = key0 >= (o ? all0[1] : all0[0]) && key0 + KEYS <= (o ? all1[1] : all1[0]);
+    w.step(kl, kl + TILE, sc, sc + KEYS, a.scale2, all, key0, from, to);
     buf ^= 1;
     if constexpr (!SHARED) __builtin_amdgcn_wave_barrier();
   }
-  const bool fine = w.finite();
-  w.l = other_half_sum(w.l);
-  const uint64_t odd = __ballot(!fine && mine && row.live);
-  uint32_t bad = (uint32_t)odd | (uint32_t)(odd >> 32);
   const End<XT, D> fin{a, p};
   if constexpr (SHARED) {
-    if (mine && !(bad >> i32 & 1)) {
-      const float f = fin.factor(row, w.m, w.l, h == 0);
 #pragma unroll
-      for (int blk = 0; blk < D / 32; ++blk)
+    for (int rb = 0; rb < RB; ++rb) {
+      const At row{tok[rb], head[rb], live[rb]};
+      const bool mine = r + AT_ROWS * rb < p.rows;
+      const uint64_t odd = __ballot(!w.finite(rb) && mine && live[rb]);
+      uint32_t bad = (uint32_t)odd | (uint32_t)(odd >> 32);
+      w.l[rb] = other_half_sum(w.l[rb]);
+      if (mine && !(bad >> i32 & 1)) {
+        const float f = fin.factor(row, w.m[rb], w.l[rb], h == 0);
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const float x[4] = {w.acc[blk][e], w.acc[blk][e + 1], w.acc[blk][e + 2], w.acc[blk][e + 3]};
-          fin.store(row, 32 * blk + 2 * e + 4 * h, f, x);
-        }
+        for (int blk = 0; blk < D / 32; ++blk)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            const f16v& y = w.acc[rb][blk];
+            const float x[4] = {y[e], y[e + 1], y[e + 2], y[e + 3]};
+            fin.store(row, 32 * blk + 2 * e + 4 * h, f, x);
+          }
+      }
+      for (; bad; bad &= bad - 1)
+        row_alone<XT, KV, D, KEYS>(a, p, range, p.r0 + AT_ROWS * (RB * wave + rb) + __builtin_ctz(bad));
     }
-    for (; bad; bad &= bad - 1) row_alone<XT, KV, D>(a, p, p.r0 + AT_ROWS * wave + __builtin_ctz(bad), t0, t1);
   } else {
+    const At row{tok[0], head[0], live[0]};
+    const bool mine = r < p.rows;
+    const uint64_t odd = __ballot(!w.finite(0) && mine && live[0]);
+    uint32_t bad = (uint32_t)odd | (uint32_t)(odd >> 32);
+    const float l = other_half_sum(w.l[0]), m = w.m[0];
     // the waves' sums, on the largest of their references
     constexpr int OP = D + 4;
-    float* sums = (float*)lds;                                  // [wave][row][OP]
-    float2* ml = (float2*)(lds + 2 * 2 * 64 * PITCH);           // [wave][row]
+    float* sums = (float*)lds;                         // [wave][row][OP]
+    float2* ml = (float2*)(lds + 2 * 2 * 64 * PITCH);  // [wave][row]
     uint32_t* odds = (uint32_t*)(ml + AT_NW * AT_ROWS);
     static_assert(AT_NW * AT_ROWS * OP * 4 <= 2 * 2 * 64 * PITCH && AT_NW * (AT_ROWS * 8 + 4) <= 2048, "LDS");
     __syncthreads();
-    if (h == 0) ml[wave * AT_ROWS + i32] = float2{w.m, w.l};
+    if (h == 0) ml[wave * AT_ROWS + i32] = float2{m, l};
     if (lane == 0) odds[wave] = bad;
     __syncthreads();
     bad = odds[0] | odds[1] | odds[2] | odds[3];
@@ -762,13 +848,14 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Place& p, int ns
       const float2 x = ml[k * AT_ROWS + i32];
       L = fmaf(x.y, __builtin_amdgcn_exp2f(x.x - M), L);
     }
-    const float f = __builtin_amdgcn_exp2f(w.m - M);
+    const float f = __builtin_amdgcn_exp2f(m - M);
 #pragma unroll
     for (int blk = 0; blk < D / 32; ++blk)
 #pragma unroll
-      for (int e = 0; e < 16; e += 4)
-        *(v4f*)(sums + (wave * AT_ROWS + i32) * OP + 32 * blk + 2 * e + 4 * h) =
-            v4f{w.acc[blk][e] * f, w.acc[blk][e + 1] * f, w.acc[blk][e + 2] * f, w.acc[blk][e + 3] * f};
+      for (int e = 0; e < 16; e += 4) {
+        const f16v& y = w.acc[0][blk];
+        *(v4f*)(sums + (wave * AT_ROWS + i32) * OP + 32 * blk + 2 * e + 4 * h) = v4f{y[e] * f, y[e + 1] * f, y[e + 2] * f, y[e + 3] * f};
+      }
     __syncthreads();
     // a wave a quarter of the dimensions of every row, two lanes a row
     if (mine && !(bad >> i32 & 1)) {
@@ -785,7 +872,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Place& p, int ns
       }
     }
     for (int k = 0; bad; bad &= bad - 1, ++k)
-      if (k % AT_NW == wave) row_alone<XT, KV, D>(a, p, p.r0 + __builtin_ctz(bad), t0, t1);
+      if (k % AT_NW == wave) row_alone<XT, KV, D, KEYS>(a, p, range, p.r0 + __builtin_ctz(bad));
   }
 }
 
@@ -794,35 +881,45 @@ constexpr int attn_terms() {
   // bf16 rows and codes of 8 bits are bf16's own; queries and weights are as many bf16 terms as their type has bytes of bits
   return std::is_same_v<XT, float> ? 3 : std::is_same_v<XT, Half> ? 2 : 1;
 }
+// Whether a kernel has waves of 64 rows: where their registers leave two waves to a SIMD.
+template <typename XT, int D>
+constexpr bool attn_wide() {
+  return attn_terms<XT>() == 1 && D == 64;
+}
 
-template <typename XT, int KV, int D>
+template <typename XT, int KV, int D, int RB>
 __global__ __launch_bounds__(256, (attn_terms<XT>() == 3 && D == 128 ? 1 : 2)) void attn_kernel(AttnArgs a) {
   extern __shared__ __align__(16) uint8_t lds[];
   constexpr int NT = attn_terms<XT>();
   Place p;
-  const bool own = (int)blockIdx.x >= a.pblocks;
-  const AttnArgs::Cut cut = own ? a.ocut : a.pcut;
-  const KvRows& kv = own ? a.kv : a.pre;
+  p.own = (int)blockIdx.x >= a.pblocks;
+  const AttnArgs::Cut cut = p.own ? a.ocut : a.pcut;
   // Workgroups go to the chip's eight parts (a cache each) in turn: those of one run of keys to the same one.
-  const int id = own ? blockIdx.x - a.pblocks : blockIdx.x;
-  const int units = (own ? (int)a.kv.n_seq : 1) * a.G * cut.splits;
+  const int id = p.own ? blockIdx.x - a.pblocks : blockIdx.x;
+  const int units = (p.own ? (int)a.kv.n_seq : 1) * a.G * cut.splits;
   const int eight = id / (8 * cut.tiles), left = min(8, units - 8 * eight), in = id - eight * 8 * cut.tiles;
-  const int unit = 8 * eight + in % left, tile = in / left;
-  p.own = own;
+  const int unit = 8 * eight + (int)((uint32_t)in % (uint32_t)left), tile = (int)((uint32_t)in / (uint32_t)left);
   p.split = unit % cut.splits;
-  p.slot = p.split + (own ? a.pcut.splits : 0);
+  p.splits = cut.splits;
+  p.slot = p.split + (p.own ? a.pcut.splits : 0);
   p.g = unit / cut.splits % a.G;
   p.b = unit / cut.splits / a.G;
-  p.rows = (own ? a.n : a.kv.n_seq * a.n) * a.rep;
-  p.r0 = (int64_t)tile * (cut.shared ? AT_NW * AT_ROWS : AT_ROWS);
+  p.rows = (int)(p.own ? a.n : a.kv.n_seq * a.n) * a.rep;
+  p.r0 = tile * cut.rows;
   p.P = a.pre.n_seq ? (int)min((int64_t)max(*a.pre.pos, 0), a.pre.ctx_max) : 0;
-  const int64_t base = (own ? p.b * a.G + p.g : p.g) * kv.ctx_max;
-  p.k = (const uint8_t*)kv.k + base * (D * Codes<KV>::BYTES);
-  p.v = (const uint8_t*)kv.v + base * (D * Codes<KV>::BYTES);
-  p.ks = kv.ks + (KV == NSX_DT_BF16 ? 0 : base);
-  p.vs = kv.vs + (KV == NSX_DT_BF16 ? 0 : base);
-  if (cut.shared) attend<XT, KV, D, NT, true>(a, p, cut.splits, lds);
-  else attend<XT, KV, D, NT, false>(a, p, cut.splits, lds);
+  p.with[0] = !p.own || a.pblocks == 0;
+  p.with[1] = p.own;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const KvRows& kv = i ? a.kv : a.pre;
+    const int64_t base = (int64_t)(i ? p.b * a.G + p.g : p.g) * kv.ctx_max;
+    p.src[i].k = (const uint8_t*)kv.k + base * (D * Codes<KV>::BYTES);
+    p.src[i].v = (const uint8_t*)kv.v + base * (D * Codes<KV>::BYTES);
+    p.src[i].ks = kv.ks + (KV == NSX_DT_BF16 ? 0 : base);
+    p.src[i].vs = kv.vs + (KV == NSX_DT_BF16 ? 0 : base);
+  }
+  if (cut.rows == AT_ROWS) attend<XT, KV, D, NT, false, 1>(a, p, lds);
+  else attend<XT, KV, D, NT, true, RB>(a, p, lds);
 }
 
 // The splits' sums of a (token, head) and its sink: a wave each, D / 4 lanes a split.
@@ -873,35 +970,41 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
 }
 
 // How a call's rows and keys are cut into workgroups: by the caches' sizes, not their lengths, so that a captured call serves
-// every length.
+// every length. Sequences of few rows each (a step of decoding) meet the prefix together, in workgroups of its own; those of
+// more than 64 meet it in their own workgroups, ahead of their own keys.
 struct Plan {
   AttnArgs::Cut pre, own;
   int64_t pblocks, oblocks;
   int splits;
 };
-Plan attn_plan(int G, int rep, int64_t B, int64_t n, int64_t ctx_max, int64_t prefix_max, int window) {
-  Plan p;
+Plan attn_plan(int G, int rep, int64_t B, int64_t n, int64_t ctx_max, int64_t prefix_max, int window, bool wide) {
+  Plan p{};
   const int64_t prows = B * n * rep, orows = n * rep;
   const int64_t pk = window > 0 ? std::min<int64_t>(prefix_max, window + n) : prefix_max;
   const int64_t ok = window > 0 ? std::min<int64_t>(ctx_max, window + n) : ctx_max;
-  // pieces of 32 rows x 32 keys, and how many of them a wave takes where the chip's 2048 waves share them
-  const int64_t pw = prefix_max ? G * nsx_cdiv(prows, AT_ROWS) * nsx_cdiv(pk, 32) : 0;
-  const int64_t ow = B * G * nsx_cdiv(orows, AT_ROWS) * nsx_cdiv(ok, 32);
+  // pieces of 32 rows x 32 keys, and how many of them a wave takes where the chip's 2048 waves share them; a wave that has
+  // few keys takes as long as for some 16 pieces more
+  const int64_t pw = G * nsx_cdiv(prows, AT_ROWS) * nsx_cdiv(pk, 32);
+  const int64_t ow = B * G * nsx_cdiv(orows, AT_ROWS) * (nsx_cdiv(ok, 32) + (orows <= 2 * AT_ROWS ? 8 : 0));
   const int64_t each = std::max<int64_t>(8, nsx_cdiv(pw + ow, 2048));
   auto cut = [&](int64_t rows, int64_t keys) {
     AttnArgs::Cut c;
-    c.shared = rows > 2 * AT_ROWS;
-    c.tiles = (int)nsx_cdiv(rows, c.shared ? AT_NW * AT_ROWS : AT_ROWS);
-    c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(AT_MAX_SPLIT / 2, nsx_cdiv(nsx_cdiv(keys, 32), c.shared ? each : AT_NW * each)));
+    const int waves = rows > 2 * AT_ROWS ? 1 : AT_NW;  // that share a row's keys
+    c.rows = waves > 1 ? AT_ROWS : wide && rows > AT_NW * AT_ROWS ? 2 * AT_NW * AT_ROWS : AT_NW * AT_ROWS;
+    c.tiles = (int)nsx_cdiv(rows, c.rows);
+    const int64_t share = c.rows == 2 * AT_NW * AT_ROWS ? std::max<int64_t>(4, each / 2) : waves * each;
+    c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(AT_MAX_SPLIT / 2, nsx_cdiv(nsx_cdiv(keys, 32), share)));
     return c;
   };
-  p.own = cut(orows, ok);
-  p.pre = prefix_max ? cut(prows, pk) : AttnArgs::Cut{0, 0, 0};
+  const bool apart = prefix_max && orows <= 2 * AT_ROWS;
+  p.own = cut(orows, ok + (apart ? 0 : pk));
+  if (apart) p.pre = cut(prows, pk);
   p.pblocks = (int64_t)G * p.pre.tiles * p.pre.splits;
   p.oblocks = B * G * p.own.tiles * p.own.splits;
   p.splits = p.pre.splits + p.own.splits;
   return p;
 }
+bool attn_wide(int x_dtype, int head_dim) { return x_dtype == NSX_DT_BF16 && head_dim == 64; }
 
 // ---------------------------------------------------------------------------
 
@@ -1018,8 +1121,9 @@ extern "C" int64_t nsx_batch_attn_workspace_bytes(int n_head, int n_kv, int head
   if (batch_heads(n_head, n_kv, head_dim) != NSX_OK || n_seq <= 0 || n_seq >= 65536 || n <= 0 || n >= (1ll << 24) ||
       n_seq * n >= (1ll << 24) || ctx_max <= 0 || ctx_max >= (1ll << 30) || prefix_max < 0 || prefix_max >= (1ll << 30) || window < 0)
     return -1;
-  const Plan p = attn_plan(n_kv, n_head / n_kv, n_seq, n, ctx_max, prefix_max, window);
-  return p.splits > 1 ? n_seq * n * n_head * p.splits * (head_dim + 2) * 4 : 16;
+  int splits = 1;  // (whatever the type)
+  for (const bool wide : {false, true}) splits = std::max(splits, attn_plan(n_kv, n_head / n_kv, n_seq, n, ctx_max, prefix_max, window, wide).splits);
+  return splits > 1 ? n_seq * n * n_head * splits * (head_dim + 2) * 4 : 16;
 }
 
 extern "C" int nsx_batch_attn(const void* q, int x_dtype, const nsx_kv_rows* kv, const nsx_kv_rows* prefix, int kv_type,
@@ -1034,6 +1138,7 @@ extern "C" int nsx_batch_attn(const void* q, int x_dtype, const nsx_kv_rows* kv,
     NSX_REQUIRE(prefix->n_seq == 1 && prefix->pos, NSX_EINVAL, "the prefix is one sequence's rows (got %lld) with a length",
                 (long long)prefix->n_seq);
   }
+  NSX_REQUIRE(scale > 0.f && scale < INFINITY, NSX_EINVAL, "scale %g", scale);
   NSX_REQUIRE(n >= 0 && n < (1ll << 24) && window >= 0 && kv->n_seq * n < (1ll << 24), NSX_EINVAL, "n=%lld window=%d: fewer than 2^24 tokens",
               (long long)n, window);
   if (n == 0) return NSX_OK;
@@ -1042,7 +1147,8 @@ extern "C" int nsx_batch_attn(const void* q, int x_dtype, const nsx_kv_rows* kv,
                                                       prefix ? prefix->ctx_max : 0, window);
   NSX_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, NSX_EINVAL,
               "workspace of %lld bytes, %lld needed, 16-byte aligned", (long long)workspace_bytes, (long long)need);
-  const Plan plan = attn_plan(n_kv, n_head / n_kv, kv->n_seq, n, kv->ctx_max, prefix ? prefix->ctx_max : 0, window);
+  const Plan plan = attn_plan(n_kv, n_head / n_kv, kv->n_seq, n, kv->ctx_max, prefix ? prefix->ctx_max : 0, window,
+                              attn_wide(x_dtype, head_dim));
   NSX_REQUIRE(plan.pblocks + plan.oblocks < (1ll << 24) && kv->n_seq * n * n_head < (1ll << 26), NSX_EINVAL,
               "%lld tokens of %d heads: too many for one call", (long long)(kv->n_seq * n), n_head);
   const AttnArgs a{q, kv_rows(kv), prefix ? kv_rows(prefix) : KvRows{}, counts, sinks, n_head, n_kv, n_head / n_kv, window, n,
@@ -1050,7 +1156,9 @@ extern "C" int nsx_batch_attn(const void* q, int x_dtype, const nsx_kv_rows* kv,
   return with_types(x_dtype, kv_type, head_dim, [&](auto x, auto t, auto d) {
     using XT = decltype(x);
     constexpr int LDS = attn_lds<d()>();
-    auto* kernel = attn_kernel<XT, t(), d()>;
+    auto* kernel = attn_kernel<XT, t(), d(), 1>;
+    if constexpr (attn_wide<XT, d()>())
+      if (std::max(plan.pre.rows, plan.own.rows) == 2 * AT_NW * AT_ROWS) kernel = attn_kernel<XT, t(), d(), 2>;
     if (const int rc = nsx_allow_lds((const void*)kernel, LDS)) return rc;
     if (const int rc = nsx_launch(kernel, dim3((unsigned)(plan.pblocks + plan.oblocks)), dim3(256), LDS, (hipStream_t)stream, a))
       return rc;
