@@ -18,7 +18,7 @@ CSRC = PKG / "csrc"
 LIB = PKG / "libnsx.so"
 SOURCES = ("quant.hip", "gemv_mm.hip", "moe.hip", "attn.hip", "tree.hip", "verify.hip", "batch.hip", "sample.hip",
            "reader.hip")
-HEADERS = ("nsx_common.h", "raw_dot.h", "gemv_mm.h", "rope.h", "launch_cache.h")
+HEADERS = ("nsx_common.h", "raw_dot.h", "gemv_mm.h", "rope.h", "pow2.h", "launch_cache.h")
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

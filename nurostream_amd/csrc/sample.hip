@@ -1,10 +1,34 @@
 // A token for each row of logits by temperature, top-k, top-p and min-p from given random numbers (gfx950).
+//
+// A token's weight is 2^(log2(e) (x - M) / T), M the row's largest logit, computed in 64 bits and rounded to a whole multiple of
+// 2^-bits: sums of weights are sums of whole numbers, the same in any order, so that the row may be split over workgroups and
+// added up by atomics. A token's order is its logit's bits, made to order as numbers do, over its index's complement: every
+// token has another one, larger for larger logits and among equals for lower indices; a filter keeps the tokens from some
+// order on.
+//
+// Four launches, each over all rows:
+//  1. every part's largest order (the row's largest is known behind it); the row's histogram is cleared;
+//  2. the histogram: weight and number of the tokens in each 16th of an octave below M;
+//  3. every part reads the histogram: the bin in which top-k ends, the bins in which top-p may (it counts from what top-k
+//     leaves of its last bin); the weight of its tokens above those, and the list of the tokens in them;
+//  4. a workgroup per row: where the filters end among the listed tokens, by digits; the parts' sums with what is kept of
+//     those; the part in which the random number falls, and in that part the token.
 #include "nsx_common.h"
+#include "pow2.h"
 
+#include <algorithm>
 #include <type_traits>
 #include <math.h>
 
 namespace {
+
+constexpr int THREADS = 512;
+constexpr int VEC = 8;                  // logits of a thread, consecutive
+constexpr int PART = THREADS * VEC;     // logits of a part
+constexpr int MAX_PARTS = 1 + (1 << 22) / PART;
+constexpr int BINS = 1024;              // 64 octaves of 16: no weight lies lower
+constexpr int LIST = 8192;             // listed tokens; a row with more in its last bins is read again instead
+constexpr int GRID = 512;               // workgroups of a pass over all rows: two on each of 256 CUs
 
 struct SampleArgs {
   const void* logits;
@@ -16,179 +40,485 @@ struct SampleArgs {
   const int32_t* top_ks;
   int32_t* token;
   int bits;  // of a weight behind the point
+  int parts;
+  uint64_t* best;       // [batch][parts]
+  uint64_t* sums;       // [batch][parts]
+  uint64_t* mass;       // [batch][BINS]
+  uint32_t* many;       // [batch][BINS]
+  uint32_t* listed;     // [batch]
+  uint32_t* list;       // [batch][LIST]
 };
 
-constexpr int THREADS = 1024;
-
+// A row's logits and settings.
 template <typename LT>  // float, _Float16, or uint16_t for bf16
-__device__ __forceinline__ float logit(const LT* p, int64_t i) {
-  float f;
-  if constexpr (std::is_same_v<LT, uint16_t>) f = nsx_bf2f(p[i]);
-  else f = (float)p[i];
-  return f == f ? f + 0.f : -INFINITY;  // (no -0)
+struct Row {
+  const LT* p;
+  int64_t V;
+  int off;  // elements that the row's start lies behind a multiple of VEC
+  double T, top_p, min_p, scale2, least, unit;
+  int64_t top_k;
+  float M = 0.f, scale32 = 0.f;
+  __device__ __forceinline__ Row(const SampleArgs& a, int64_t row)
+      : p((const LT*)a.logits + row * a.row_stride), V(a.V), off((int)((uintptr_t)p / sizeof(LT) % VEC)) {
+    T = a.temperatures ? (double)a.temperatures[row] : a.temperature;
+    top_p = a.top_ps ? (double)a.top_ps[row] : a.top_p;
+    min_p = a.min_ps ? (double)a.min_ps[row] : a.min_p;
+    min_p = min_p > 0.0 ? fmin(min_p, 1.0) : 0.0;
+    top_k = a.top_ks ? a.top_ks[row] : a.top_k;
+    if (top_k <= 0 || top_k >= V) top_k = 0;
+    scale2 = 1.44269504088896340736 / T;
+    least = -1000.0 / scale2;
+    unit = __builtin_bit_cast(double, (uint64_t)(1023 + a.bits) << 52);
+  }
+  // What top-p's tokens, of `whole` in all, are the first to reach: each of them has less than that before it.
+  __device__ __forceinline__ uint64_t target(uint64_t whole) const {
+    const uint64_t t = (uint64_t)ceil(fmax(top_p, 0.0) * (double)whole);
+    return t < 1 ? 1 : t < whole || whole < 1 ? t : whole;
+  }
+  __device__ __forceinline__ bool drawn() const { return T > 0.0 && M > -INFINITY; }  // not the largest, not none
+  __device__ __forceinline__ bool cut() const { return top_k || top_p < 1.0; }
+  __device__ __forceinline__ void largest(uint64_t order) {
+    const uint32_t u = (uint32_t)(order >> 32);
+    M = __builtin_bit_cast(float, u ^ ((int32_t)u < 0 ? 0x80000000u : 0xffffffffu));
+    scale32 = (float)fmin(16.0 * scale2, 3e38);  // (times a difference of zero: zero)
+  }
+  static __device__ __forceinline__ float value(LT x) {
+    float f;
+    if constexpr (std::is_same_v<LT, uint16_t>) f = nsx_bf2f(x);
+    else f = (float)x;
+    return f == f ? f + 0.f : -INFINITY;  // (no -0)
+  }
+  __device__ __forceinline__ float at(int64_t i) const { return value(p[i]); }
+  // The elements from place v (a multiple of VEC) of the row's parts on, element k being token v - off + k; -infinity where
+  // there is none.
+  __device__ __forceinline__ void run(int64_t v, float (&x)[VEC]) const {
+    const int64_t i = v - off;
+    if (i >= 0 && i + VEC <= V) {
+      struct alignas(VEC * sizeof(LT) > 16 ? 16 : VEC * sizeof(LT)) Vec {
+        LT e[VEC];
+      };
+      const Vec w = *(const Vec*)(p + i);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) x[k] = value(w.e[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) x[k] = i + k >= 0 && i + k < V ? at(i + k) : -INFINITY;
+    }
+  }
+  static __device__ __forceinline__ uint64_t order(float x, int64_t i) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    return (uint64_t)(u ^ ((int32_t)u < 0 ? 0xffffffffu : 0x80000000u)) << 32 | (uint32_t)~(uint32_t)i;
+  }
+  __device__ __forceinline__ double real(float x, const Pow2& tab) const {
+    const double d = (double)x - (double)M;
+    if (M == INFINITY) return x == M ? 1.0 : 0.0;
+    return d < least ? 0.0 : nsx_pow2(fmax(d, least), scale2, tab);
+  }
+  __device__ __forceinline__ uint64_t whole(double w) const {  // in units, to the nearest
+    const double y = rint(w * unit), hi = floor(y * 0x1p-32);
+    return (uint64_t)(uint32_t)hi << 32 | (uint32_t)fma(hi, -0x1p32, y);
+  }
+  __device__ __forceinline__ uint64_t weight(float x, const Pow2& tab) const { return whole(real(x, tab)); }
+  // The bin of a logit of weight above zero: 16ths of an octave below M. 32-bit operations that never fall as x rises.
+  __device__ __forceinline__ int bin(float x) const {
+    if (M == INFINITY) return 0;
+    const float e = (M - x) * scale32;
+    return e < BINS - 1 ? (int)e : BINS - 1;
+  }
+};
+
+__device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) {
+  return (uint64_t)__shfl_xor((uint32_t)(v >> 32), o, 64) << 32 | __shfl_xor((uint32_t)v, o, 64);
 }
-__device__ __forceinline__ uint32_t order_of(float x) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, x);
-  return u ^ ((int32_t)u < 0 ? 0xffffffffu : 0x80000000u);
+__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int o) {
+  return (uint64_t)__shfl_up((uint32_t)(v >> 32), o, 64) << 32 | __shfl_up((uint32_t)v, o, 64);
+}
+constexpr int NW = THREADS / 64;
+// The workgroup's largest v / v's sum / the sum of the threads before this one with the whole sum; s: NW words of LDS, free
+// again behind the call.
+__device__ __forceinline__ uint64_t block_max(uint64_t v, uint64_t* s) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v = max64(v, shfl_xor64(v, o));
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) v = max64(v, s[i]);
+  __syncthreads();
+  return v;
+}
+__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* s, uint64_t& all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint64_t x = v;
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const uint64_t y = shfl_up64(x, o);
+    x += lane >= o ? y : 0;
+  }
+  if (lane == 63) s[wave] = x;
+  __syncthreads();
+  uint64_t before = 0;
+  all = 0;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    before += i < wave ? s[i] : 0;
+    all += s[i];
+  }
+  __syncthreads();
+  return before + x - v;
+}
+
+// The row's largest order, of its parts' ones.
+template <typename LT>
+__device__ __forceinline__ uint64_t row_best(const SampleArgs& a, int64_t row, uint64_t* s) {
+  uint64_t v = 0;
+  for (int i = threadIdx.x; i < a.parts; i += THREADS) v = max64(v, a.best[row * a.parts + i]);
+  return block_max(v, s);
 }
 
 template <typename LT>
-__global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
-  __shared__ uint64_t mass[256];
-  __shared__ uint32_t many[256];
-  __shared__ uint64_t s64[THREADS];
-  __shared__ uint32_t s32[THREADS];
-  const int t = threadIdx.x;
-  const int64_t row = blockIdx.x;
-  const LT* p = (const LT*)a.logits + row * a.row_stride;
-  const double T = a.temperatures ? (double)a.temperatures[row] : a.temperature;
-  const double top_p = a.top_ps ? (double)a.top_ps[row] : a.top_p, min_p = fmin(a.min_ps ? (double)a.min_ps[row] : a.min_p, 1.0);
-  const int64_t top_k = a.top_ks ? a.top_ks[row] : a.top_k;
-  // the largest and its lowest index
-  uint64_t best = 0;
-  for (int64_t i = t; i < a.V; i += THREADS) {
-    const uint64_t v = (uint64_t)order_of(logit(p, i)) << 32 | (uint32_t)~(uint32_t)i;
-    best = v > best ? v : best;
+__global__ __launch_bounds__(THREADS) void best_kernel(SampleArgs a) {
+  __shared__ uint64_t s[NW];
+  const int64_t row = blockIdx.y;
+  const Row<LT> r(a, row);
+  if (a.mass)
+    for (int i = blockIdx.x * THREADS + threadIdx.x; i < BINS; i += gridDim.x * THREADS) {
+      a.mass[row * BINS + i] = 0;
+      a.many[row * BINS + i] = 0;
+      if (i == 0) a.listed[row] = 0;
+    }
+  for (int part = blockIdx.x; part < a.parts; part += gridDim.x) {
+    const int64_t v = (int64_t)part * PART + threadIdx.x * VEC;
+    float x[VEC];
+    r.run(v, x);
+    uint64_t best = 0;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) best = max64(best, v - r.off + k >= 0 && v - r.off + k < a.V ? Row<LT>::order(x[k], v - r.off + k) : 0);
+    best = block_max(best, s);
+    if (threadIdx.x == 0) a.best[row * a.parts + part] = best;
   }
-  s64[t] = best;
+}
+
+template <typename LT>
+__global__ __launch_bounds__(THREADS) void bins_kernel(SampleArgs a) {
+  __shared__ uint64_t s[NW], mass[BINS];
+  __shared__ uint32_t many[BINS];
+  __shared__ Pow2 tab;
+  const int64_t row = blockIdx.y;
+  Row<LT> r(a, row);
+  if (!r.cut()) return;
+  tab.fill();
+  for (int i = threadIdx.x; i < BINS; i += THREADS) mass[i] = 0, many[i] = 0;
+  r.largest(row_best<LT>(a, row, s));  // (its barriers order the clearing as well)
+  if (!r.drawn()) return;
+  for (int part = blockIdx.x; part < a.parts; part += gridDim.x) {
+    const int64_t v = (int64_t)part * PART + threadIdx.x * VEC;
+    float x[VEC];
+    r.run(v, x);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const uint64_t w = r.weight(x[k], tab);
+      if (w) {
+        const int b = r.bin(x[k]);
+        atomicAdd((unsigned long long*)&mass[b], (unsigned long long)w);
+        if (r.top_k) atomicAdd(&many[b], 1u);
+      }
+    }
+  }
   __syncthreads();
-  for (int o = THREADS / 2; o; o >>= 1) {
-    if (t < o) s64[t] = s64[t + o] > s64[t] ? s64[t + o] : s64[t];
+  for (int i = threadIdx.x; i < BINS; i += THREADS) {
+    if (mass[i]) atomicAdd((unsigned long long*)&a.mass[row * BINS + i], (unsigned long long)mass[i]);
+    if (many[i]) atomicAdd(&a.many[row * BINS + i], many[i]);
+  }
+}
+
+// Where a row's filters end, as far as its histogram tells.
+struct Ends {
+  int kbin, plo, phi;         // top-k's last bin; the bins that top-p's may be; BINS: no such filter
+  uint64_t above_k, above_p;  // the weight above kbin, above plo
+  uint32_t before_k;          // the number of tokens above kbin
+  uint64_t all;               // the whole weight
+  template <typename LT>
+  __device__ __forceinline__ void find(const SampleArgs& a, const Row<LT>& r, int64_t row, uint64_t* s, Ends* shared) {
+    if (threadIdx.x == 0) *shared = Ends{BINS, BINS, BINS, 0, 0, 0, 0};
+    constexpr int PER = BINS / THREADS;
+    uint64_t m[PER], n[PER], sm = 0, sn = 0, am, an;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      m[i] = a.mass[row * BINS + threadIdx.x * PER + i];
+      n[i] = a.many[row * BINS + threadIdx.x * PER + i];
+      sm += m[i], sn += n[i];
+    }
+    const uint64_t bm = block_scan(sm, s, am), bn = block_scan(sn, s, an);
+    uint64_t cm = bm, cn = bn;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {  // (one thread finds it, if any)
+      if (r.top_k && cn < (uint64_t)r.top_k && cn + n[i] >= (uint64_t)r.top_k) {
+        shared->kbin = threadIdx.x * PER + i;
+        shared->above_k = cm;
+        shared->before_k = (uint32_t)cn;
+        shared->all = cm + m[i];
+      }
+      cm += m[i], cn += n[i];
+    }
     __syncthreads();
+    Ends e = *shared;
+    __syncthreads();
+    if (e.kbin == BINS) e.above_k = e.all = am;
+    if (r.top_p < 1.0) {
+      // (what top-k leaves lies between above_k and all)
+      const uint64_t lo = r.target(e.kbin == BINS ? e.all : e.above_k), hi = r.target(e.all);
+      cm = bm;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (cm < lo && cm + m[i] >= lo) shared->plo = threadIdx.x * PER + i, shared->above_p = cm;
+        if (cm < hi && cm + m[i] >= hi) shared->phi = threadIdx.x * PER + i;
+        cm += m[i];
+      }
+    }
+    __syncthreads();
+    e.plo = shared->plo, e.phi = shared->phi, e.above_p = shared->above_p;
+    e.all = e.kbin == BINS ? am : 0;
+    *this = e;
   }
-  best = s64[0];
-  __syncthreads();
-  const int32_t at = (int32_t)~(uint32_t)best;
-  const float M = logit(p, at);
-  if (!(M > -INFINITY) || !(T > 0.0)) {
-    if (t == 0) a.token[row] = M > -INFINITY ? at : -1;
+  __device__ __forceinline__ bool sure(int bin) const { return bin < kbin && bin < plo; }
+  __device__ __forceinline__ bool open(int bin) const { return bin == kbin || (bin >= plo && bin <= phi && bin <= kbin); }
+};
+
+template <typename LT>
+__global__ __launch_bounds__(THREADS) void sums_kernel(SampleArgs a) {
+  __shared__ uint64_t s[NW];
+  __shared__ Ends shared;
+  __shared__ Pow2 tab;
+  const int64_t row = blockIdx.y;
+  Row<LT> r(a, row);
+  tab.fill();
+  r.largest(row_best<LT>(a, row, s));
+  if (!r.drawn()) return;
+  const bool cut = r.cut();
+  Ends e{BINS, BINS, BINS, 0, 0, 0, 0};
+  if (cut) e.find(a, r, row, s, &shared);
+  for (int part = blockIdx.x; part < a.parts; part += gridDim.x) {
+    const int64_t v = (int64_t)part * PART + threadIdx.x * VEC;
+    float x[VEC];
+    r.run(v, x);
+    uint64_t sum = 0, all;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const double w = r.real(x[k], tab);
+      const uint64_t y = r.whole(w);
+      const int b = cut ? r.bin(x[k]) : 0;
+      if (!cut || e.sure(b)) sum += w < r.min_p ? 0 : y;
+      else if (y && e.open(b)) {
+        const uint32_t at = atomicAdd(&a.listed[row], 1u);
+        if (at < LIST) a.list[row * LIST + at] = (uint32_t)(v - r.off + k);
+      }
+    }
+    block_scan(sum, s, all);
+    if (threadIdx.x == 0) a.sums[row * a.parts + part] = all;
+  }
+}
+
+// The order c among tokens of which those above it together weigh less than `want` and those from it on at least that; `above`: the weight above
+// it. each(f): f(order, weight) for every token, by whichever threads. By digits of 10 bits from the first one that differs,
+// until the digits are all or one token is left.
+constexpr int DIGIT = 10;
+struct Pick {
+  uint64_t s[NW], mass[1 << DIGIT], order, above;
+  uint32_t many[1 << DIGIT];
+  int digit;
+};
+template <typename Each>
+__device__ __forceinline__ uint64_t pick_order(Pick& p, uint64_t want, uint64_t& above, Each each) {
+  uint64_t lo = 0, hi = 0;  // the largest of the complements, the largest
+  each([&](uint64_t o, uint64_t) { hi = max64(hi, o), lo = max64(lo, ~o); });
+  hi = block_max(hi, p.s);
+  lo = ~block_max(lo, p.s);
+  above = 0;
+  if (hi == lo) return hi;
+  int shift = 64 - __clzll((long long)(hi ^ lo));  // bits of an order below those that all share
+  while (true) {
+    const int width = shift < DIGIT ? shift : DIGIT, low = shift - width;
+    const uint64_t same = shift == 64 ? 0 : hi >> shift;
+    for (int i = threadIdx.x; i < 1 << DIGIT; i += THREADS) p.mass[i] = 0, p.many[i] = 0;
+    if (threadIdx.x == 0) p.digit = 0;
+    __syncthreads();
+    each([&](uint64_t o, uint64_t w) {
+      if ((shift == 64 ? 0 : o >> shift) != same) return;
+      const int d = (int)(o >> low) & ((1 << width) - 1);
+      atomicAdd((unsigned long long*)&p.mass[d], (unsigned long long)w);
+      atomicAdd(&p.many[d], 1u);
+    });
+    __syncthreads();
+    // from the largest digit down: the first at which the running sum reaches what is wanted
+    constexpr int PER = (1 << DIGIT) / THREADS;
+    uint64_t m[PER], sum = 0, all;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sum += m[i] = p.mass[(1 << DIGIT) - 1 - threadIdx.x * PER - i];
+    uint64_t run = above + block_scan(sum, p.s, all);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (run < want && run + m[i] >= want) {
+        p.digit = (1 << DIGIT) - 1 - threadIdx.x * PER - i;
+        p.above = run;
+      }
+      run += m[i];
+    }
+    __syncthreads();
+    above = p.above;
+    const int d = p.digit;
+    const uint32_t n = p.many[d];
+    hi = (shift == 64 ? 0 : hi >> shift << shift) | (uint64_t)d << low;
+    shift = low;
+    __syncthreads();
+    if (n == 1) {
+      each([&](uint64_t o, uint64_t) {
+        if (o >> shift == hi >> shift) p.order = o;
+      });
+      __syncthreads();
+      return p.order;
+    }
+    if (shift == 0) return hi;
+  }
+}
+
+template <typename LT>
+__global__ __launch_bounds__(THREADS) void draw_kernel(SampleArgs a) {
+  __shared__ Pick p;
+  __shared__ Ends shared;
+  __shared__ Pow2 tab;
+  __shared__ uint64_t sums[MAX_PARTS];
+  __shared__ int found;
+  const int64_t row = blockIdx.x;
+  Row<LT> r(a, row);
+  tab.fill();
+  const uint64_t best = row_best<LT>(a, row, p.s);
+  r.largest(best);
+  if (!r.drawn()) {
+    if (threadIdx.x == 0) a.token[row] = r.M > -INFINITY ? (int32_t)~(uint32_t)best : -1;
     return;
   }
-  auto real = [&](float x) { return M == INFINITY ? (x == M ? 1.0 : 0.0) : exp(((double)x - (double)M) / T); };
-  auto weight = [&](float x) { return (uint64_t)rint(ldexp(real(x), a.bits)); };
-  // the border: tokens above key are kept, and `ties` of those at it, by their index
-  uint32_t key = 0, ties = 0xffffffffu;
-  uint64_t whole = 0;
-  for (int mode = 0; mode < 2; ++mode) {  // 0: by their number, 1: by their weight
-    if (mode == 0 ? !(top_k > 0 && top_k < a.V) : !(top_p < 1.0)) continue;
-    if (mode == 1) {
-      // the whole weight of what top_k left
-      uint64_t s = 0;
-      for (int64_t i = t; i < a.V; i += THREADS) {
-        const float x = logit(p, i);
-        if (order_of(x) > key) s += weight(x);
-        else if (order_of(x) == key && ties == 0xffffffffu) s += weight(x);
-      }
-      s64[t] = s;
-      __syncthreads();
-      for (int o = THREADS / 2; o; o >>= 1) {
-        if (t < o) s64[t] += s64[t + o];
-        __syncthreads();
-      }
-      whole = s64[0];
-      __syncthreads();
-      if (ties != 0xffffffffu) {
-        const uint32_t u = key ^ ((int32_t)key < 0 ? 0x80000000u : 0xffffffffu);
-        whole += ties * weight(__builtin_bit_cast(float, u));
-      }
-    }
-    const uint64_t want = mode == 0 ? (uint64_t)top_k : (uint64_t)ceil(fmax(top_p, 0.0) * (double)whole);
-    uint64_t above = 0;
-    uint32_t found = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = t; i < 256; i += THREADS) mass[i] = 0, many[i] = 0;
-      __syncthreads();
-      for (int64_t i = t; i < a.V; i += THREADS) {
-        const float x = logit(p, i);
-        const uint32_t o = order_of(x);
-        if (shift == 24 || (o >> (shift + 8)) == (found >> (shift + 8))) {
-          atomicAdd(&many[o >> shift & 255], 1u);
-          if (mode) atomicAdd((unsigned long long*)&mass[o >> shift & 255], (unsigned long long)weight(x));
+  for (int i = threadIdx.x; i < a.parts; i += THREADS) sums[i] = a.sums[row * a.parts + i];
+  if (threadIdx.x == 0) found = 0x7fffffff;
+  __syncthreads();
+  const bool cut = r.cut();
+  Ends e{BINS, BINS, BINS, 0, 0, 0, 0};
+  uint64_t last = 0;  // the order of the last token that the filters keep
+  if (cut) {
+    e.find(a, r, row, p.s, &shared);
+    const uint32_t n = a.listed[row];
+    const uint32_t* list = a.list + row * LIST;
+    // the listed tokens, or where they are too many all of the row's in those bins
+    auto tokens = [&](auto f) {
+      if (n <= LIST) {
+        for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+          const uint32_t t = list[i];
+          const float x = r.at(t);
+          f(t, x, r.bin(x));
+        }
+      } else {
+        for (int64_t t = threadIdx.x; t < a.V; t += THREADS) {
+          const float x = r.at(t);
+          const int b = r.bin(x);
+          if (e.open(b) && r.weight(x, tab)) f((uint32_t)t, x, b);
         }
       }
-      __syncthreads();
-      if (t == 0) {
-        int d = 255;
-        uint64_t sum = above;
-        for (;; --d) {
-          const uint64_t m = mode ? mass[d] : many[d];
-          if (sum + m >= want && many[d]) break;
-          if (d == 0) break;
-          sum += m;
-        }
-        s64[0] = sum;
-        s32[0] = d;
+    };
+    uint64_t whole = e.all;
+    if (e.kbin < BINS) {
+      uint64_t dummy;
+      last = pick_order(p, (uint64_t)r.top_k - e.before_k, dummy, [&](auto f) {
+        tokens([&](uint32_t t, float x, int b) {
+          if (b == e.kbin) f(Row<LT>::order(x, t), 1);
+        });
+      });
+      uint64_t in = 0;
+      tokens([&](uint32_t t, float x, int b) {
+        if (b == e.kbin && Row<LT>::order(x, t) >= last) in += r.weight(x, tab);
+      });
+      block_scan(in, p.s, whole);
+      whole += e.above_k;
+    }
+    if (r.top_p < 1.0) {
+      uint64_t dummy;
+      last = max64(last, pick_order(p, r.target(whole) - e.above_p, dummy, [&](auto f) {
+        tokens([&](uint32_t t, float x, int b) {
+          const uint64_t o = Row<LT>::order(x, t);
+          if (b >= e.plo && b <= e.phi && o >= last) f(o, r.weight(x, tab));
+        });
+      }));
+    }
+    tokens([&](uint32_t t, float x, int) {
+      if (Row<LT>::order(x, t) >= last) {
+        const double w = r.real(x, tab);
+        if (!(w < r.min_p)) atomicAdd((unsigned long long*)&sums[(t + r.off) / PART], (unsigned long long)r.whole(w));
       }
-      __syncthreads();
-      above = s64[0];
-      found |= s32[0] << shift;
-      __syncthreads();
-    }
-    const uint32_t u = found ^ ((int32_t)found < 0 ? 0x80000000u : 0xffffffffu);
-    const uint64_t w = mode ? weight(__builtin_bit_cast(float, u)) : 1;
-    uint64_t r = want > above ? (w ? (want - above + w - 1) / w : 0xffffffffu) : 0;
-    if (mode && found == order_of(M) && r == 0) r = 1;  // (the likeliest token stays)
-    if (found > key) key = found, ties = (uint32_t)(r < 0xffffffffu ? r : 0xffffffffu);
-    else if (found == key) ties = (uint32_t)(r < ties ? r : ties);
+    });
+    __syncthreads();
   }
-  // the draw: passes over the row in index order, a thread a run of tokens
-  const int64_t per = (a.V + THREADS - 1) / THREADS, i0 = t * per, i1 = i0 + per < a.V ? i0 + per : a.V;
-  uint32_t mine = 0;
-  for (int64_t i = i0; i < i1; ++i) mine += order_of(logit(p, i)) == key;
-  s32[t] = mine;
-  __syncthreads();
-  if (t == 0) {
-    uint32_t s = 0;
-    for (int i = 0; i < THREADS; ++i) {
-      const uint32_t v = s32[i];
-      s32[i] = s;
-      s += v;
+  // the part in which the random number falls
+  constexpr int PER = (MAX_PARTS + THREADS - 1) / THREADS;
+  uint64_t sum = 0, total;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) sum += threadIdx.x * PER + i < a.parts ? sums[threadIdx.x * PER + i] : 0;
+  uint64_t run = block_scan(sum, p.s, total);
+  const double want = fmin(fmax((double)a.u[row] * (double)total, 0.0), (double)total);
+  const uint64_t target = (uint64_t)want < total ? (uint64_t)want : total - 1;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int part = threadIdx.x * PER + i;
+    const uint64_t m = part < a.parts ? sums[part] : 0;
+    if (run <= target && run + m > target) {
+      found = part;
+      p.above = run;
     }
+    run += m;
   }
   __syncthreads();
-  const uint32_t before = s32[t];
-  auto kept = [&](float x, uint32_t& tie) -> uint64_t {
-    const uint32_t o = order_of(x);
-    if (o < key) return 0;
-    if (o == key && tie++ >= ties) return 0;
-    return real(x) < min_p ? 0 : weight(x);
-  };
-  uint64_t sum = 0;
-  uint32_t tie = before;
-  for (int64_t i = i0; i < i1; ++i) sum += kept(logit(p, i), tie);
-  s64[t] = sum;
-  __syncthreads();
-  if (t == 0) {
-    uint64_t s = 0;
-    for (int i = 0; i < THREADS; ++i) {
-      const uint64_t v = s64[i];
-      s64[i] = s;
-      s += v;
-    }
-    mass[0] = s;
+  const int part = found;
+  if (part >= a.parts) return;  // (no weight is a number: does not happen)
+  // and the token in it
+  const int64_t v = (int64_t)part * PART + threadIdx.x * VEC;
+  float x[VEC];
+  r.run(v, x);
+  uint64_t w[VEC];
+  sum = 0;
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) {
+    const double y = r.real(x[k], tab);
+    w[k] = y < r.min_p || (cut && Row<LT>::order(x[k], v - r.off + k) < last) ? 0 : r.whole(y);
+    sum += w[k];
   }
-  __syncthreads();
-  const uint64_t total = mass[0];
-  const double x = fmin(fmax((double)a.u[row] * (double)total, 0.0), (double)total);
-  const uint64_t target = (uint64_t)x < total ? (uint64_t)x : total - 1;
-  uint64_t run = s64[t];
-  if (run <= target && run + sum > target) {
-    tie = before;
-    for (int64_t i = i0; i < i1; ++i) {
-      run += kept(logit(p, i), tie);
-      if (run > target) {
-        a.token[row] = (int32_t)i;
-        break;
-      }
-    }
+  run = p.above;
+  run += block_scan(sum, p.s, total);
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) {
+    if (run <= target && run + w[k] > target) a.token[row] = (int32_t)(v - r.off + k);
+    run += w[k];
   }
+}
+
+int parts_of(int64_t vocab) { return (int)nsx_cdiv(vocab + VEC - 1, PART); }
+int64_t up16(int64_t v) { return (v + 15) & ~15ll; }
+
+template <typename LT>
+int sample_launch(const SampleArgs& a, int64_t batch, bool cut, bool greedy, hipStream_t st) {
+  const int per_row = (int)std::min<int64_t>(a.parts, nsx_cdiv(GRID, batch));
+  const dim3 grid(per_row, (unsigned)batch);
+  if (const int rc = nsx_launch(best_kernel<LT>, grid, dim3(THREADS), 0, st, a)) return rc;
+  if (cut)
+    if (const int rc = nsx_launch(bins_kernel<LT>, grid, dim3(THREADS), 0, st, a)) return rc;
+  if (!greedy)
+    if (const int rc = nsx_launch(sums_kernel<LT>, grid, dim3(THREADS), 0, st, a)) return rc;
+  return nsx_launch(draw_kernel<LT>, dim3((unsigned)batch), dim3(THREADS), 0, st, a);
 }
 
 }  // namespace
 
 extern "C" int64_t nsx_sample_workspace_bytes(int64_t batch, int64_t vocab) {
-  if (batch <= 0 || vocab <= 0) return -1;
-  return 16;
+  if (batch <= 0 || vocab <= 0 || vocab > (1 << 22)) return -1;
+  return batch * ((int64_t)parts_of(vocab) * 16 + BINS * 12 + LIST * 4) + up16(batch * 4);
 }
 
 extern "C" int nsx_sample(const void* logits, int logits_dtype, int64_t row_stride, int64_t batch, int64_t vocab,
@@ -215,11 +545,14 @@ extern "C" int nsx_sample(const void* logits, int logits_dtype, int64_t row_stri
               "workspace of %lld bytes, %lld needed, 16-byte aligned", (long long)workspace_bytes, (long long)need);
   int bits = 62;
   while (bits > 0 && (1ll << (62 - bits)) < vocab) --bits;
+  const bool cut = s.top_ks || s.top_ps || s.top_k > 0 || s.top_p < 1.0, greedy = !s.temperatures && s.temperature == 0.0;
+  const int parts = parts_of(vocab);
+  uint64_t *best = (uint64_t*)workspace, *sums = best + batch * parts, *mass = sums + batch * parts;
+  uint32_t *many = (uint32_t*)(mass + batch * BINS), *list = many + batch * BINS, *listed = list + batch * LIST;
   const SampleArgs a{logits, row_stride, vocab, uniforms, s.temperature, s.top_p, s.min_p, s.top_k, s.temperatures,
-                     s.top_ps, s.min_ps, s.top_ks, token, bits};
+                     s.top_ps, s.min_ps, s.top_ks, token, bits, parts, best, sums, cut && !greedy ? mass : nullptr, many, listed, list};
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)batch);
-  if (logits_dtype == NSX_DT_F32) return nsx_launch(sample_kernel<float>, grid, dim3(THREADS), 0, st, a);
-  if (logits_dtype == NSX_DT_F16) return nsx_launch(sample_kernel<_Float16>, grid, dim3(THREADS), 0, st, a);
-  return nsx_launch(sample_kernel<uint16_t>, grid, dim3(THREADS), 0, st, a);
+  if (logits_dtype == NSX_DT_F32) return sample_launch<float>(a, batch, cut && !greedy, greedy, st);
+  if (logits_dtype == NSX_DT_F16) return sample_launch<_Float16>(a, batch, cut && !greedy, greedy, st);
+  return sample_launch<uint16_t>(a, batch, cut && !greedy, greedy, st);
 }
