@@ -7,7 +7,7 @@
 // order on.
 //
 // Four launches, each over all rows:
-//  1. every part's largest order (the row's largest is known behind it); the row's histogram is cleared;
+//  1. the largest order of each workgroup's parts (the row's is known behind it); the row's histogram is cleared;
 //  2. the histogram: weight and number of the tokens in each 16th of an octave below M;
 //  3. every part reads the histogram: the bin in which top-k ends, the bins in which top-p may (it counts from what top-k
 //     leaves of its last bin); the weight of its tokens above those, and the list of the tokens in them;
@@ -41,7 +41,8 @@ struct SampleArgs {
   int32_t* token;
   int bits;  // of a weight behind the point
   int parts;
-  uint64_t* best;       // [batch][parts]
+  int groups;           // workgroups of a row in the passes over all rows
+  uint64_t* best;       // [batch][groups]
   uint64_t* sums;       // [batch][parts]
   uint64_t* mass;       // [batch][BINS]
   uint32_t* many;       // [batch][BINS]
@@ -90,21 +91,31 @@ struct Row {
   }
   __device__ __forceinline__ float at(int64_t i) const { return value(p[i]); }
   // The elements from place v (a multiple of VEC) of the row's parts on, element k being token v - off + k; -infinity where
-  // there is none.
-  __device__ __forceinline__ void run(int64_t v, float (&x)[VEC]) const {
+  // there is none. Loaded as they lie, a vector, or one by one at the row's ends.
+  struct alignas(16) Raw {
+    LT e[VEC];
+  };
+  __device__ __forceinline__ Raw load(int64_t v) const {
     const int64_t i = v - off;
+    Raw w;
     if (i >= 0 && i + VEC <= V) {
-      struct alignas(VEC * sizeof(LT) > 16 ? 16 : VEC * sizeof(LT)) Vec {
-        LT e[VEC];
-      };
-      const Vec w = *(const Vec*)(p + i);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) x[k] = value(w.e[k]);
+      w = *(const Raw*)(p + i);
     } else {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) x[k] = i + k >= 0 && i + k < V ? at(i + k) : -INFINITY;
+      for (int k = 0; k < VEC; ++k) w.e[k] = i + k >= 0 && i + k < V ? p[i + k] : LT(0);
+    }
+    return w;
+  }
+  __device__ __forceinline__ void values(int64_t v, const Raw& w, float (&x)[VEC]) const {
+    const int64_t i = v - off;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) x[k] = value(w.e[k]);
+    if (i < 0 || i + VEC > V) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) x[k] = i + k >= 0 && i + k < V ? x[k] : -INFINITY;
     }
   }
+  __device__ __forceinline__ void run(int64_t v, float (&x)[VEC]) const { values(v, load(v), x); }
   static __device__ __forceinline__ uint64_t order(float x, int64_t i) {
     const uint32_t u = __builtin_bit_cast(uint32_t, x);
     return (uint64_t)(u ^ ((int32_t)u < 0 ? 0xffffffffu : 0x80000000u)) << 32 | (uint32_t)~(uint32_t)i;
@@ -128,18 +139,36 @@ struct Row {
 };
 
 __device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) {
-  return (uint64_t)__shfl_xor((uint32_t)(v >> 32), o, 64) << 32 | __shfl_xor((uint32_t)v, o, 64);
+// Wave-wide operations on DPP moves and readlanes: no trip through LDS.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp64(uint64_t v) {  // lanes without a source, or outside ROWS, get 0
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+  return (uint64_t)hi << 32 | lo;
 }
-__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int o) {
-  return (uint64_t)__shfl_up((uint32_t)(v >> 32), o, 64) << 32 | __shfl_up((uint32_t)v, o, 64);
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {  // of the lanes up to this one
+  v += dpp64<0x111, 0xf>(v);  // row_shr
+  v += dpp64<0x112, 0xf>(v);
+  v += dpp64<0x114, 0xf>(v);
+  v += dpp64<0x118, 0xf>(v);
+  v += dpp64<0x142, 0xa>(v);  // row_bcast:15 into the odd rows
+  v += dpp64<0x143, 0xc>(v);  // row_bcast:31 into the upper half
+  return v;
+}
+__device__ __forceinline__ uint64_t lane64(uint64_t v, int i) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), i) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, i);
+}
+__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) { return lane64(wave_scan(v), 63); }
+__device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
+  const uint32_t hi = nsx_wave_max_u32((uint32_t)(v >> 32));
+  return (uint64_t)hi << 32 | nsx_wave_max_u32((uint32_t)(v >> 32) == hi ? (uint32_t)v : 0);
 }
 constexpr int NW = THREADS / 64;
-// The workgroup's largest v / v's sum / the sum of the threads before this one with the whole sum; s: NW words of LDS, free
-// again behind the call.
+// The workgroup's largest v / the sum of the threads before this one with the whole sum; s: NW words of LDS, free again behind
+// the call.
 __device__ __forceinline__ uint64_t block_max(uint64_t v, uint64_t* s) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v = max64(v, shfl_xor64(v, o));
+  v = wave_max64(v);
   if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
   __syncthreads();
   v = 0;
@@ -150,12 +179,7 @@ __device__ __forceinline__ uint64_t block_max(uint64_t v, uint64_t* s) {
 }
 __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* s, uint64_t& all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint64_t x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const uint64_t y = shfl_up64(x, o);
-    x += lane >= o ? y : 0;
-  }
+  const uint64_t x = wave_scan(v);
   if (lane == 63) s[wave] = x;
   __syncthreads();
   uint64_t before = 0;
@@ -169,12 +193,27 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* s, uint64_t
   return before + x - v;
 }
 
-// The row's largest order, of its parts' ones.
+// The row's largest order, of its workgroups' ones.
 template <typename LT>
 __device__ __forceinline__ uint64_t row_best(const SampleArgs& a, int64_t row, uint64_t* s) {
   uint64_t v = 0;
-  for (int i = threadIdx.x; i < a.parts; i += THREADS) v = max64(v, a.best[row * a.parts + i]);
+  for (int i = threadIdx.x; i < a.groups; i += THREADS) v = max64(v, a.best[row * a.groups + i]);
   return block_max(v, s);
+}
+
+// f(part, index of the first, logits) for the workgroup's share of a row's parts, a thread VEC logits of each, the next part's
+// on their way meanwhile.
+template <typename LT, typename F>
+__device__ __forceinline__ void each_part(const SampleArgs& a, const Row<LT>& r, F f) {
+  typename Row<LT>::Raw next = r.load((int64_t)blockIdx.x * PART + threadIdx.x * VEC);
+  for (int part = blockIdx.x; part < a.parts; part += gridDim.x) {
+    const int64_t v = (int64_t)part * PART + threadIdx.x * VEC;
+    const typename Row<LT>::Raw now = next;
+    if (part + (int)gridDim.x < a.parts) next = r.load(v + (int64_t)gridDim.x * PART);
+    float x[VEC];
+    r.values(v, now, x);
+    f(part, v - r.off, x);
+  }
 }
 
 template <typename LT>
@@ -188,16 +227,18 @@ __global__ __launch_bounds__(THREADS) void best_kernel(SampleArgs a) {
       a.many[row * BINS + i] = 0;
       if (i == 0) a.listed[row] = 0;
     }
-  for (int part = blockIdx.x; part < a.parts; part += gridDim.x) {
-    const int64_t v = (int64_t)part * PART + threadIdx.x * VEC;
-    float x[VEC];
-    r.run(v, x);
-    uint64_t best = 0;
+  uint64_t best = 0;
+  each_part(a, r, [&](int, int64_t i, const float (&x)[VEC]) {
+    // (of its own logits a thread looks for the largest first: the order of one token, not of eight)
+    float top = x[0];
+    int at = 0;
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) best = max64(best, v - r.off + k >= 0 && v - r.off + k < a.V ? Row<LT>::order(x[k], v - r.off + k) : 0);
-    best = block_max(best, s);
-    if (threadIdx.x == 0) a.best[row * a.parts + part] = best;
-  }
+    for (int k = 1; k < VEC; ++k) at = x[k] > top ? k : at, top = fmaxf(top, x[k]);
+    i += at;
+    best = max64(best, i < 0 ? Row<LT>::order(top, 0) : i < a.V ? Row<LT>::order(top, i) : 0);
+  });
+  best = block_max(best, s);
+  if (threadIdx.x == 0) a.best[row * a.groups + blockIdx.x] = best;
 }
 
 template <typename LT>
@@ -212,10 +253,7 @@ __global__ __launch_bounds__(THREADS) void bins_kernel(SampleArgs a) {
   for (int i = threadIdx.x; i < BINS; i += THREADS) mass[i] = 0, many[i] = 0;
   r.largest(row_best<LT>(a, row, s));  // (its barriers order the clearing as well)
   if (!r.drawn()) return;
-  for (int part = blockIdx.x; part < a.parts; part += gridDim.x) {
-    const int64_t v = (int64_t)part * PART + threadIdx.x * VEC;
-    float x[VEC];
-    r.run(v, x);
+  each_part(a, r, [&](int, int64_t, const float (&x)[VEC]) {
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
       const uint64_t w = r.weight(x[k], tab);
@@ -225,7 +263,7 @@ __global__ __launch_bounds__(THREADS) void bins_kernel(SampleArgs a) {
         if (r.top_k) atomicAdd(&many[b], 1u);
       }
     }
-  }
+  });
   __syncthreads();
   for (int i = threadIdx.x; i < BINS; i += THREADS) {
     if (mass[i]) atomicAdd((unsigned long long*)&a.mass[row * BINS + i], (unsigned long long)mass[i]);
@@ -288,36 +326,48 @@ struct Ends {
 
 template <typename LT>
 __global__ __launch_bounds__(THREADS) void sums_kernel(SampleArgs a) {
-  __shared__ uint64_t s[NW];
+  constexpr int OPEN = 2048;  // listed tokens of a workgroup; where they are more, the row is read again
+  __shared__ uint64_t s[NW], sums[MAX_PARTS];
+  __shared__ uint32_t list[OPEN], n, base;
   __shared__ Ends shared;
   __shared__ Pow2 tab;
   const int64_t row = blockIdx.y;
   Row<LT> r(a, row);
   tab.fill();
+  if (threadIdx.x == 0) n = 0;
+  for (int i = threadIdx.x; i < (a.parts - 1) / a.groups + 1; i += THREADS) sums[i] = 0;
   r.largest(row_best<LT>(a, row, s));
   if (!r.drawn()) return;
   const bool cut = r.cut();
   Ends e{BINS, BINS, BINS, 0, 0, 0, 0};
   if (cut) e.find(a, r, row, s, &shared);
-  for (int part = blockIdx.x; part < a.parts; part += gridDim.x) {
-    const int64_t v = (int64_t)part * PART + threadIdx.x * VEC;
-    float x[VEC];
-    r.run(v, x);
-    uint64_t sum = 0, all;
+  each_part(a, r, [&](int part, int64_t i, const float (&x)[VEC]) {
+    uint64_t sum = 0;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
-      const double w = r.real(x[k], tab);
-      const uint64_t y = r.whole(w);
       const int b = cut ? r.bin(x[k]) : 0;
-      if (!cut || e.sure(b)) sum += w < r.min_p ? 0 : y;
-      else if (y && e.open(b)) {
-        const uint32_t at = atomicAdd(&a.listed[row], 1u);
-        if (at < LIST) a.list[row * LIST + at] = (uint32_t)(v - r.off + k);
+      if (!cut || e.sure(b)) {
+        const double w = r.real(x[k], tab);
+        sum += w < r.min_p ? 0 : r.whole(w);
+      } else if (e.open(b) && x[k] > -INFINITY) {
+        const uint32_t at = atomicAdd(&n, 1u);
+        if (at < OPEN) list[at] = (uint32_t)(i + k);
       }
     }
-    block_scan(sum, s, all);
-    if (threadIdx.x == 0) a.sums[row * a.parts + part] = all;
-  }
+    if (__any(sum != 0)) {
+      sum = wave_sum64(sum);
+      if ((threadIdx.x & 63) == 0) atomicAdd((unsigned long long*)&sums[part / a.groups], (unsigned long long)sum);
+    }
+  });
+  __syncthreads();
+  const uint32_t mine = n;
+  if (mine && threadIdx.x == 0) base = atomicAdd(&a.listed[row], mine <= OPEN ? mine : LIST + 1);
+  for (int part = blockIdx.x + threadIdx.x * a.groups; part < a.parts; part += THREADS * a.groups)
+    a.sums[row * a.parts + part] = sums[part / a.groups];
+  if (!mine) return;
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < mine && i < OPEN; i += THREADS)
+    if (base + i < LIST) a.list[row * LIST + base + i] = list[i];
 }
 
 // The order c among tokens of which those above it together weigh less than `want` and those from it on at least that; `above`: the weight above
@@ -409,19 +459,36 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(SampleArgs a) {
     e.find(a, r, row, p.s, &shared);
     const uint32_t n = a.listed[row];
     const uint32_t* list = a.list + row * LIST;
-    // the listed tokens, or where they are too many all of the row's in those bins
+    // f(order, weight, bin, whether min-p keeps it) for the listed tokens: held in registers; or where they are more, taken
+    // from the list, or from all of the row's in those bins
+    constexpr int HELD = 4;
+    uint64_t ho[HELD] = {}, hw[HELD] = {};
+    int hb[HELD];
+    bool hk[HELD];
+    auto look = [&](uint32_t t, uint64_t& o, uint64_t& w, int& b, bool& keep) {
+      const float x = r.at(t);
+      const double y = r.real(x, tab);
+      o = Row<LT>::order(x, t), w = r.whole(y), b = r.bin(x), keep = !(y < r.min_p);
+    };
+    if (n <= HELD * THREADS) {
+#pragma unroll
+      for (int i = 0; i < HELD; ++i)
+        if (threadIdx.x + i * THREADS < n) look(list[threadIdx.x + i * THREADS], ho[i], hw[i], hb[i], hk[i]);
+    }
     auto tokens = [&](auto f) {
-      if (n <= LIST) {
-        for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-          const uint32_t t = list[i];
-          const float x = r.at(t);
-          f(t, x, r.bin(x));
-        }
+      if (n <= HELD * THREADS) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+          if (hw[i]) f(ho[i], hw[i], hb[i], hk[i]);
       } else {
-        for (int64_t t = threadIdx.x; t < a.V; t += THREADS) {
-          const float x = r.at(t);
-          const int b = r.bin(x);
-          if (e.open(b) && r.weight(x, tab)) f((uint32_t)t, x, b);
+        const int64_t end = n <= LIST ? n : a.V;
+#pragma unroll 1
+        for (int64_t i = threadIdx.x; i < end; i += THREADS) {
+          uint64_t o, w;
+          int b;
+          bool keep;
+          look(n <= LIST ? list[i] : (uint32_t)i, o, w, b, keep);
+          if (w && e.open(b)) f(o, w, b, keep);
         }
       }
     };
@@ -429,13 +496,13 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(SampleArgs a) {
     if (e.kbin < BINS) {
       uint64_t dummy;
       last = pick_order(p, (uint64_t)r.top_k - e.before_k, dummy, [&](auto f) {
-        tokens([&](uint32_t t, float x, int b) {
-          if (b == e.kbin) f(Row<LT>::order(x, t), 1);
+        tokens([&](uint64_t o, uint64_t, int b, bool) {
+          if (b == e.kbin) f(o, 1);
         });
       });
       uint64_t in = 0;
-      tokens([&](uint32_t t, float x, int b) {
-        if (b == e.kbin && Row<LT>::order(x, t) >= last) in += r.weight(x, tab);
+      tokens([&](uint64_t o, uint64_t w, int b, bool) {
+        if (b == e.kbin && o >= last) in += w;
       });
       block_scan(in, p.s, whole);
       whole += e.above_k;
@@ -443,17 +510,13 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(SampleArgs a) {
     if (r.top_p < 1.0) {
       uint64_t dummy;
       last = max64(last, pick_order(p, r.target(whole) - e.above_p, dummy, [&](auto f) {
-        tokens([&](uint32_t t, float x, int b) {
-          const uint64_t o = Row<LT>::order(x, t);
-          if (b >= e.plo && b <= e.phi && o >= last) f(o, r.weight(x, tab));
+        tokens([&](uint64_t o, uint64_t w, int b, bool) {
+          if (b >= e.plo && b <= e.phi && o >= last) f(o, w);
         });
       }));
     }
-    tokens([&](uint32_t t, float x, int) {
-      if (Row<LT>::order(x, t) >= last) {
-        const double w = r.real(x, tab);
-        if (!(w < r.min_p)) atomicAdd((unsigned long long*)&sums[(t + r.off) / PART], (unsigned long long)r.whole(w));
-      }
+    tokens([&](uint64_t o, uint64_t w, int, bool keep) {
+      if (o >= last && keep) atomicAdd((unsigned long long*)&sums[((uint32_t)~(uint32_t)o + r.off) / PART], (unsigned long long)w);
     });
     __syncthreads();
   }
@@ -504,8 +567,7 @@ int64_t up16(int64_t v) { return (v + 15) & ~15ll; }
 
 template <typename LT>
 int sample_launch(const SampleArgs& a, int64_t batch, bool cut, bool greedy, hipStream_t st) {
-  const int per_row = (int)std::min<int64_t>(a.parts, nsx_cdiv(GRID, batch));
-  const dim3 grid(per_row, (unsigned)batch);
+  const dim3 grid(a.groups, (unsigned)batch);
   if (const int rc = nsx_launch(best_kernel<LT>, grid, dim3(THREADS), 0, st, a)) return rc;
   if (cut)
     if (const int rc = nsx_launch(bins_kernel<LT>, grid, dim3(THREADS), 0, st, a)) return rc;
@@ -550,7 +612,7 @@ extern "C" int nsx_sample(const void* logits, int logits_dtype, int64_t row_stri
   uint64_t *best = (uint64_t*)workspace, *sums = best + batch * parts, *mass = sums + batch * parts;
   uint32_t *many = (uint32_t*)(mass + batch * BINS), *list = many + batch * BINS, *listed = list + batch * LIST;
   const SampleArgs a{logits, row_stride, vocab, uniforms, s.temperature, s.top_p, s.min_p, s.top_k, s.temperatures,
-                     s.top_ps, s.min_ps, s.top_ks, token, bits, parts, best, sums, cut && !greedy ? mass : nullptr, many, listed, list};
+                     s.top_ps, s.min_ps, s.top_ks, token, bits, parts, (int)std::min<int64_t>(parts, nsx_cdiv(GRID, batch)), best, sums, cut && !greedy ? mass : nullptr, many, listed, list};
   hipStream_t st = (hipStream_t)stream;
   if (logits_dtype == NSX_DT_F32) return sample_launch<float>(a, batch, cut && !greedy, greedy, st);
   if (logits_dtype == NSX_DT_F16) return sample_launch<_Float16>(a, batch, cut && !greedy, greedy, st);
