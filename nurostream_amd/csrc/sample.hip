@@ -28,6 +28,8 @@ constexpr int PART = THREADS * VEC;     // logits of a part
 constexpr int MAX_PARTS = 1 + (1 << 22) / PART;
 constexpr int BINS = 1024;              // 64 octaves of 16: no weight lies lower
 constexpr int LIST = 8192;             // listed tokens; a row with more in its last bins is read again instead
+constexpr int HELD = 4;                 // listed tokens that a thread holds in registers
+constexpr int FEW = HELD * THREADS / 2;
 constexpr int GRID = 512;               // workgroups of a pass over all rows: two on each of 256 CUs
 
 struct SampleArgs {
@@ -78,6 +80,9 @@ struct Row {
   }
   __device__ __forceinline__ bool drawn() const { return T > 0.0 && M > -INFINITY; }  // not the largest, not none
   __device__ __forceinline__ bool cut() const { return top_k || top_p < 1.0; }
+  // Few tokens of the highest are wanted: counting finds their last bin, and all of them are listed, so that no other token's
+  // weight is computed.
+  __device__ __forceinline__ bool few() const { return top_k && top_k <= FEW; }
   __device__ __forceinline__ void largest(uint64_t order) {
     const uint32_t u = (uint32_t)(order >> 32);
     M = __builtin_bit_cast(float, u ^ ((int32_t)u < 0 ? 0x80000000u : 0xffffffffu));
@@ -130,12 +135,13 @@ struct Row {
     return (uint64_t)(uint32_t)hi << 32 | (uint32_t)fma(hi, -0x1p32, y);
   }
   __device__ __forceinline__ uint64_t weight(float x, const Pow2& tab) const { return whole(real(x, tab)); }
-  // The bin of a logit of weight above zero: 16ths of an octave below M. 32-bit operations that never fall as x rises.
-  __device__ __forceinline__ int bin(float x) const {
-    if (M == INFINITY) return 0;
-    const float e = (M - x) * scale32;
-    return e < BINS - 1 ? (int)e : BINS - 1;
+  // How many 16ths of an octave below M a logit lies: 32-bit operations that never fall as x does; and the bin that it is in.
+  __device__ __forceinline__ float depth(float x) const {
+    if (M == INFINITY) return x == M ? 0.f : INFINITY;
+    return (M - x) * scale32;
   }
+  static __device__ __forceinline__ int bin_at(float depth) { return depth < BINS - 1 ? (int)depth : BINS - 1; }
+  __device__ __forceinline__ int bin(float x) const { return bin_at(depth(x)); }
 };
 
 __device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
@@ -193,13 +199,23 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* s, uint64_t
   return before + x - v;
 }
 
-// The row's largest order, of its workgroups' ones.
-template <typename LT>
-__device__ __forceinline__ uint64_t row_best(const SampleArgs& a, int64_t row, uint64_t* s) {
-  uint64_t v = 0;
-  for (int i = threadIdx.x; i < a.groups; i += THREADS) v = max64(v, a.best[row * a.groups + i]);
-  return block_max(v, s);
-}
+// What a workgroup reads of the passes before, all of it on its way before the first of it is waited for: the row's largest
+// orders, one per workgroup, and the histogram.
+struct Known {
+  static constexpr int PER = BINS / THREADS;
+  uint64_t best = 0, mass[PER];
+  uint32_t many[PER];
+  __device__ __forceinline__ Known(const SampleArgs& a, int64_t row, bool cut) {
+    for (int i = threadIdx.x; i < a.groups; i += THREADS) best = max64(best, a.best[row * a.groups + i]);
+    if (cut) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        mass[i] = a.mass[row * BINS + threadIdx.x * PER + i];
+        many[i] = a.many[row * BINS + threadIdx.x * PER + i];
+      }
+    }
+  }
+};
 
 // f(part, index of the first, logits) for the workgroup's share of a row's parts, a thread VEC logits of each, the next part's
 // on their way meanwhile.
@@ -249,11 +265,19 @@ __global__ __launch_bounds__(THREADS) void bins_kernel(SampleArgs a) {
   const int64_t row = blockIdx.y;
   Row<LT> r(a, row);
   if (!r.cut()) return;
+  const Known known(a, row, false);
   tab.fill();
   for (int i = threadIdx.x; i < BINS; i += THREADS) mass[i] = 0, many[i] = 0;
-  r.largest(row_best<LT>(a, row, s));  // (its barriers order the clearing as well)
+  r.largest(block_max(known.best, s));  // (its barriers order the clearing as well)
   if (!r.drawn()) return;
+  const bool few = r.few();
   each_part(a, r, [&](int, int64_t, const float (&x)[VEC]) {
+    if (few) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        if (x[k] > -INFINITY) atomicAdd(&many[r.bin(x[k])], 1u);
+      return;
+    }
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
       const uint64_t w = r.weight(x[k], tab);
@@ -278,30 +302,40 @@ struct Ends {
   uint32_t before_k;          // the number of tokens above kbin
   uint64_t all;               // the whole weight
   template <typename LT>
-  __device__ __forceinline__ void find(const SampleArgs& a, const Row<LT>& r, int64_t row, uint64_t* s, Ends* shared) {
+  __device__ __forceinline__ void find(const Row<LT>& r, const Known& known, uint64_t* s, Ends* shared) {
+    constexpr int PER = Known::PER;
     if (threadIdx.x == 0) *shared = Ends{BINS, BINS, BINS, 0, 0, 0, 0};
-    constexpr int PER = BINS / THREADS;
-    uint64_t m[PER], n[PER], sm = 0, sn = 0, am, an;
+    uint64_t am = 0, cm = 0, bm = 0;
+    if (!r.few()) {
+      uint64_t sum = 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      m[i] = a.mass[row * BINS + threadIdx.x * PER + i];
-      n[i] = a.many[row * BINS + threadIdx.x * PER + i];
-      sm += m[i], sn += n[i];
+      for (int i = 0; i < PER; ++i) sum += known.mass[i];
+      cm = bm = block_scan(sum, s, am);
     }
-    const uint64_t bm = block_scan(sm, s, am), bn = block_scan(sn, s, an);
-    uint64_t cm = bm, cn = bn;
+    if (r.top_k) {
+      uint64_t sum = 0, all;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {  // (one thread finds it, if any)
-      if (r.top_k && cn < (uint64_t)r.top_k && cn + n[i] >= (uint64_t)r.top_k) {
-        shared->kbin = threadIdx.x * PER + i;
-        shared->above_k = cm;
-        shared->before_k = (uint32_t)cn;
-        shared->all = cm + m[i];
+      for (int i = 0; i < PER; ++i) sum += known.many[i];
+      uint64_t cn = block_scan(sum, s, all);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {  // (one thread finds it, if any)
+        const uint64_t m = r.few() ? 0 : known.mass[i];
+        if (cn < (uint64_t)r.top_k && cn + known.many[i] >= (uint64_t)r.top_k) {
+          shared->kbin = threadIdx.x * PER + i;
+          shared->above_k = cm;
+          shared->before_k = (uint32_t)cn;
+          shared->all = cm + m;
+        }
+        cm += m, cn += known.many[i];
       }
-      cm += m[i], cn += n[i];
     }
     __syncthreads();
     Ends e = *shared;
+    if (r.few()) {  // (no weights are known: every token down to kbin is open)
+      const int kbin = e.kbin < BINS ? e.kbin : BINS - 1;
+      *this = Ends{kbin, 0, kbin, 0, 0, 0, 0};
+      return;
+    }
     __syncthreads();
     if (e.kbin == BINS) e.above_k = e.all = am;
     if (r.top_p < 1.0) {
@@ -310,16 +344,18 @@ struct Ends {
       cm = bm;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        if (cm < lo && cm + m[i] >= lo) shared->plo = threadIdx.x * PER + i, shared->above_p = cm;
-        if (cm < hi && cm + m[i] >= hi) shared->phi = threadIdx.x * PER + i;
-        cm += m[i];
+        const uint64_t m = known.mass[i];
+        if (cm < lo && cm + m >= lo) shared->plo = threadIdx.x * PER + i, shared->above_p = cm;
+        if (cm < hi && cm + m >= hi) shared->phi = threadIdx.x * PER + i;
+        cm += m;
       }
+      __syncthreads();
+      e.plo = shared->plo, e.phi = shared->phi, e.above_p = shared->above_p;
     }
-    __syncthreads();
-    e.plo = shared->plo, e.phi = shared->phi, e.above_p = shared->above_p;
     e.all = e.kbin == BINS ? am : 0;
     *this = e;
   }
+  __device__ __forceinline__ int last() const { return kbin < BINS ? kbin : phi; }  // bin that is sure or open
   __device__ __forceinline__ bool sure(int bin) const { return bin < kbin && bin < plo; }
   __device__ __forceinline__ bool open(int bin) const { return bin == kbin || (bin >= plo && bin <= phi && bin <= kbin); }
 };
@@ -333,25 +369,38 @@ __global__ __launch_bounds__(THREADS) void sums_kernel(SampleArgs a) {
   __shared__ Pow2 tab;
   const int64_t row = blockIdx.y;
   Row<LT> r(a, row);
+  const bool cut = a.mass && r.cut();
+  const Known known(a, row, cut);
   tab.fill();
   if (threadIdx.x == 0) n = 0;
   for (int i = threadIdx.x; i < (a.parts - 1) / a.groups + 1; i += THREADS) sums[i] = 0;
-  r.largest(row_best<LT>(a, row, s));
+  r.largest(block_max(known.best, s));
   if (!r.drawn()) return;
-  const bool cut = r.cut();
   Ends e{BINS, BINS, BINS, 0, 0, 0, 0};
-  if (cut) e.find(a, r, row, s, &shared);
+  if (cut) e.find(r, known, s, &shared);
+  const float deepest = e.last() < BINS - 1 ? (float)(e.last() + 1) : INFINITY;  // (one look tells most tokens from those kept)
   each_part(a, r, [&](int part, int64_t i, const float (&x)[VEC]) {
     uint64_t sum = 0;
+    if (!cut) {
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      const int b = cut ? r.bin(x[k]) : 0;
-      if (!cut || e.sure(b)) {
+      for (int k = 0; k < VEC; ++k) {
         const double w = r.real(x[k], tab);
         sum += w < r.min_p ? 0 : r.whole(w);
-      } else if (e.open(b) && x[k] > -INFINITY) {
-        const uint32_t at = atomicAdd(&n, 1u);
-        if (at < OPEN) list[at] = (uint32_t)(i + k);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const float depth = r.depth(x[k]);
+        if (depth < deepest) {
+          const int b = Row<LT>::bin_at(depth);
+          if (e.sure(b)) {
+            const double w = r.real(x[k], tab);
+            sum += w < r.min_p ? 0 : r.whole(w);
+          } else if (e.open(b)) {
+            const uint32_t at = atomicAdd(&n, 1u);
+            if (at < OPEN) list[at] = (uint32_t)(i + k);
+          }
+        }
       }
     }
     if (__any(sum != 0)) {
@@ -370,33 +419,39 @@ __global__ __launch_bounds__(THREADS) void sums_kernel(SampleArgs a) {
     if (base + i < LIST) a.list[row * LIST + base + i] = list[i];
 }
 
-// The order c among tokens of which those above it together weigh less than `want` and those from it on at least that; `above`: the weight above
-// it. each(f): f(order, weight) for every token, by whichever threads. By digits of 10 bits from the first one that differs,
-// until the digits are all or one token is left.
+// Among tokens, the order of the one with which their sum from the highest on reaches `want`; 0 where all of them do not.
+// each(f): f(order, weight) for every token, by whichever threads. By digits of 10 bits of what an order lies above the lowest,
+// from the highest bit that one has, until the digits are all or one token is left.
 constexpr int DIGIT = 10;
 struct Pick {
-  uint64_t s[NW], mass[1 << DIGIT], order, above;
+  uint64_t s[NW], t[NW], mass[1 << DIGIT], order, above;
   uint32_t many[1 << DIGIT];
   int digit;
 };
 template <typename Each>
-__device__ __forceinline__ uint64_t pick_order(Pick& p, uint64_t want, uint64_t& above, Each each) {
-  uint64_t lo = 0, hi = 0;  // the largest of the complements, the largest
+__device__ __forceinline__ uint64_t pick_order(Pick& p, uint64_t want, Each each) {
+  uint64_t above = 0, lo = 0, hi = 0;  // lo: the largest complement
   each([&](uint64_t o, uint64_t) { hi = max64(hi, o), lo = max64(lo, ~o); });
-  hi = block_max(hi, p.s);
-  lo = ~block_max(lo, p.s);
-  above = 0;
-  if (hi == lo) return hi;
-  int shift = 64 - __clzll((long long)(hi ^ lo));  // bits of an order below those that all share
-  while (true) {
-    const int width = shift < DIGIT ? shift : DIGIT, low = shift - width;
-    const uint64_t same = shift == 64 ? 0 : hi >> shift;
-    for (int i = threadIdx.x; i < 1 << DIGIT; i += THREADS) p.mass[i] = 0, p.many[i] = 0;
-    if (threadIdx.x == 0) p.digit = 0;
+  hi = wave_max64(hi), lo = wave_max64(lo);
+  if ((threadIdx.x & 63) == 0) p.s[threadIdx.x >> 6] = hi, p.t[threadIdx.x >> 6] = lo;
+  for (int i = threadIdx.x; i < 1 << DIGIT; i += THREADS) p.mass[i] = 0, p.many[i] = 0;
+  if (threadIdx.x == 0) p.digit = -1;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NW; ++i) hi = max64(hi, p.s[i]), lo = max64(lo, p.t[i]);
+  lo = ~lo;
+  if (hi == lo) {
     __syncthreads();
+    return hi;
+  }
+  int shift = hi < lo ? 0 : 64 - __clzll((long long)(hi - lo)), bits = 0;  // digits of orders in [lo, lo + 2^shift) (2^64: all)
+  while (true) {
+    const int width = shift < DIGIT ? shift : DIGIT;
+    shift -= width;
+    bits = width;
     each([&](uint64_t o, uint64_t w) {
-      if ((shift == 64 ? 0 : o >> shift) != same) return;
-      const int d = (int)(o >> low) & ((1 << width) - 1);
+      const uint64_t d = (o - lo) >> shift;
+      if (o < lo || d >> bits) return;
       atomicAdd((unsigned long long*)&p.mass[d], (unsigned long long)w);
       atomicAdd(&p.many[d], 1u);
     });
@@ -416,20 +471,23 @@ __device__ __forceinline__ uint64_t pick_order(Pick& p, uint64_t want, uint64_t&
       run += m[i];
     }
     __syncthreads();
-    above = p.above;
     const int d = p.digit;
+    if (d < 0) return 0;
+    above = p.above;
     const uint32_t n = p.many[d];
-    hi = (shift == 64 ? 0 : hi >> shift << shift) | (uint64_t)d << low;
-    shift = low;
-    __syncthreads();
+    lo += (uint64_t)d << shift;
     if (n == 1) {
       each([&](uint64_t o, uint64_t) {
-        if (o >> shift == hi >> shift) p.order = o;
+        if (o >= lo && (o - lo) >> shift == 0) p.order = o;
       });
       __syncthreads();
       return p.order;
     }
-    if (shift == 0) return hi;
+    if (shift == 0) return lo;
+    __syncthreads();
+    for (int i = threadIdx.x; i < 1 << DIGIT; i += THREADS) p.mass[i] = 0, p.many[i] = 0;
+    if (threadIdx.x == 0) p.digit = -1;
+    __syncthreads();
   }
 }
 
@@ -442,26 +500,30 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(SampleArgs a) {
   __shared__ int found;
   const int64_t row = blockIdx.x;
   Row<LT> r(a, row);
+  const bool cut = a.mass && r.cut();
+  const Known known(a, row, cut);
+  const uint32_t* list = a.list + row * LIST;
+  uint32_t first[HELD], n = 0;
+  if (cut) {
+    n = a.listed[row];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) first[i] = list[threadIdx.x + i * THREADS];  // (as many as there are count)
+  }
   tab.fill();
-  const uint64_t best = row_best<LT>(a, row, p.s);
+  for (int i = threadIdx.x; i < a.parts; i += THREADS) sums[i] = a.sums[row * a.parts + i];  // (of a drawn row)
+  if (threadIdx.x == 0) found = 0x7fffffff;
+  const uint64_t best = block_max(known.best, p.s);
   r.largest(best);
   if (!r.drawn()) {
     if (threadIdx.x == 0) a.token[row] = r.M > -INFINITY ? (int32_t)~(uint32_t)best : -1;
     return;
   }
-  for (int i = threadIdx.x; i < a.parts; i += THREADS) sums[i] = a.sums[row * a.parts + i];
-  if (threadIdx.x == 0) found = 0x7fffffff;
-  __syncthreads();
-  const bool cut = r.cut();
   Ends e{BINS, BINS, BINS, 0, 0, 0, 0};
   uint64_t last = 0;  // the order of the last token that the filters keep
   if (cut) {
-    e.find(a, r, row, p.s, &shared);
-    const uint32_t n = a.listed[row];
-    const uint32_t* list = a.list + row * LIST;
+    e.find(r, known, p.s, &shared);
     // f(order, weight, bin, whether min-p keeps it) for the listed tokens: held in registers; or where they are more, taken
     // from the list, or from all of the row's in those bins
-    constexpr int HELD = 4;
     uint64_t ho[HELD] = {}, hw[HELD] = {};
     int hb[HELD];
     bool hk[HELD];
@@ -473,7 +535,7 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(SampleArgs a) {
     if (n <= HELD * THREADS) {
 #pragma unroll
       for (int i = 0; i < HELD; ++i)
-        if (threadIdx.x + i * THREADS < n) look(list[threadIdx.x + i * THREADS], ho[i], hw[i], hb[i], hk[i]);
+        if (threadIdx.x + i * THREADS < n) look(first[i], ho[i], hw[i], hb[i], hk[i]);
     }
     auto tokens = [&](auto f) {
       if (n <= HELD * THREADS) {
@@ -494,22 +556,22 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(SampleArgs a) {
     };
     uint64_t whole = e.all;
     if (e.kbin < BINS) {
-      uint64_t dummy;
-      last = pick_order(p, (uint64_t)r.top_k - e.before_k, dummy, [&](auto f) {
+      // (of the few: all of them are listed, of others those of the last bin)
+      const int from = r.few() ? 0 : e.kbin;
+      last = pick_order(p, (uint64_t)r.top_k - e.before_k, [&](auto f) {
         tokens([&](uint64_t o, uint64_t, int b, bool) {
-          if (b == e.kbin) f(o, 1);
+          if (b >= from && b <= e.kbin) f(o, 1);
         });
       });
       uint64_t in = 0;
       tokens([&](uint64_t o, uint64_t w, int b, bool) {
-        if (b == e.kbin && o >= last) in += w;
+        if (b >= from && b <= e.kbin && o >= last) in += w;
       });
       block_scan(in, p.s, whole);
       whole += e.above_k;
     }
     if (r.top_p < 1.0) {
-      uint64_t dummy;
-      last = max64(last, pick_order(p, r.target(whole) - e.above_p, dummy, [&](auto f) {
+      last = max64(last, pick_order(p, r.target(whole) - e.above_p, [&](auto f) {
         tokens([&](uint64_t o, uint64_t w, int b, bool) {
           if (b >= e.plo && b <= e.phi && o >= last) f(o, w);
         });

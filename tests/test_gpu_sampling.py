@@ -104,6 +104,28 @@ def test_large_vocabularies(dev, x, B, V, kw):
         _check(logits, torch.rand(B, generator=g, device=dev), 0.8, **kw)
 
 
+@pytest.mark.parametrize("x", FLOATS)
+def test_fewer_tokens_than_asked_for(dev, x):
+    """Most tokens masked away: top-k finds fewer than it may keep, top-p fewer than its share needs."""
+    g = _gen(dev, 14)
+    logits = torch.full((30, 5000), -math.inf, device=dev)
+    logits[:, ::617] = torch.randn(30, 9, generator=g, device=dev)
+    logits[::3, 7] = -3000.0  # a weight of nothing
+    u = torch.rand(30, generator=g, device=dev)
+    for kw in (dict(top_k=20), dict(top_k=9), dict(top_k=3), dict(top_k=20, top_p=0.7), dict(top_k=2000, top_p=0.999), dict(top_p=0.4)):
+        _check(logits.to(x), u, 0.7, **kw)
+
+
+@pytest.mark.parametrize("top_k", [1023, 1024, 1025, 2049, 9000])
+def test_top_k_among_many_equals(dev, top_k):
+    """Borders of every way to hold the tokens of the last bin: in registers, in a list, or read again."""
+    g = _gen(dev, top_k)
+    for step in (1.0, 0.02, 1e-4):
+        logits = torch.round(torch.randn(3, 20000, generator=g, device=dev) / step) * step
+        _check(logits, torch.rand(3, generator=g, device=dev), 1.0, top_k, 0.9)
+        _check(logits * 0.01, torch.rand(3, generator=g, device=dev), 1.0, top_k)
+
+
 @pytest.mark.parametrize("V", [300000, 4194304])
 def test_flat_row(dev, V):
     """All tokens of equal weight: whole counts tell the answer."""
