@@ -539,12 +539,19 @@ __device__ __forceinline__ void row_alone(const AttnArgs& a, const Place& p, con
   }
 }
 
+// A stage of KEYS key rows and as many value rows in LDS, as bf16. Keys are read 16 bytes of each of 8 rows at once, values
+// (transposed) 64 bytes of each of 4: pitches of 4 and of 16 (or 48) of the 64 banks past a multiple of them keep those apart.
+template <int D>
+struct Pitch {
+  static constexpr int K = 2 * D + 16, V = D == 64 ? 192 : 320;
+  static constexpr int stage(int keys) { return keys * (K + V); }
+};
+
 // A wave's RB x 32 rows over its keys. Scores are K Q^T, so that a lane holds 16 of 32 keys' scores of one row (lane % 32; the
 // other lane of the row holds the others), and its weights are at once the second operand of V^T W^T, of which it holds D / 2
 // values of the same row. The operand's order of keys is the scores' own, and V's rows are read from LDS in it, transposed.
 template <int KV, int D, int NT, int NB, int RB>
 struct Wave {
-  static constexpr int PITCH = 2 * D + 16;  // of a row in LDS: reads of 8 rows at once fall on different banks
   v4u q[RB][NT][D / 16];
   f16v acc[RB][D / 32];
   float m[RB], l[RB];
@@ -585,7 +592,7 @@ struct Wave {
       for (int rb = 0; rb < RB; ++rb) s[rb] = f16v{};
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
-        const v4u k = *(const v4u*)(kl + (32 * nb + i32) * PITCH + 32 * ks + 16 * h);
+        const v4u k = *(const v4u*)(kl + (32 * nb + i32) * Pitch<D>::K + 32 * ks + 16 * h);
 #pragma unroll
         for (int t = NT - 1; t >= 0; --t)
 #pragma unroll
@@ -657,10 +664,10 @@ struct Wave {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
           // values of dimension 32 i + lane % 32, keys 16 kb + 4 h .. + 3 and 8 behind them
-          const uint8_t* at = vl + (32 * nb + 16 * kb + 4 * h + ((lane & 15) >> 2)) * PITCH +
+          const uint8_t* at = vl + (32 * nb + 16 * kb + 4 * h + ((lane & 15) >> 2)) * Pitch<D>::V +
                               2 * (32 * i + 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
           const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s4*)at);
-          const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s4*)(at + 8 * PITCH));
+          const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s4*)(at + 8 * Pitch<D>::V));
           const v2u a2 = __builtin_bit_cast(v2u, a), b2 = __builtin_bit_cast(v2u, b);
           const v4u v = {a2[0], a2[1], b2[0], b2[1]};
 #pragma unroll
@@ -683,7 +690,7 @@ struct Wave {
 // 16-byte pieces of KEYS rows of k and v (and their scales) by THREADS threads: from memory to registers, then to LDS as bf16.
 template <int KV, int D, int KEYS, int THREADS>
 struct Stage {
-  static constexpr int PIECES = D / Codes<KV>::PER, N = KEYS * PIECES / THREADS, PITCH = 2 * D + 16;
+  static constexpr int PIECES = D / Codes<KV>::PER, N = KEYS * PIECES / THREADS;
   v4u k[N], v[N];
   float s;
   __device__ __forceinline__ void load(const Source& p, int t0, int last, int t) {  // rows t0 .., none past `last`
@@ -702,9 +709,9 @@ struct Stage {
   __device__ __forceinline__ void store(uint8_t* kl, uint8_t* vl, float* sc, float c, int t) const {  // sc: KEYS of k, KEYS of v
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int x = t + THREADS * i, at = x / PIECES * PITCH + x % PIECES * (2 * Codes<KV>::PER);
-      Codes<KV>::put(kl + at, k[i]);
-      Codes<KV>::put(vl + at, v[i]);
+      const int x = t + THREADS * i, row = x / PIECES, at = x % PIECES * (2 * Codes<KV>::PER);
+      Codes<KV>::put(kl + row * Pitch<D>::K + at, k[i]);
+      Codes<KV>::put(vl + row * Pitch<D>::V + at, v[i]);
     }
     if constexpr (KV != NSX_DT_BF16) {
       if (t < 2 * KEYS) sc[t] = t < KEYS ? s * c : s;
@@ -714,13 +721,13 @@ struct Stage {
 
 template <int D>
 constexpr int attn_lds() {
-  return 2 * 2 * 64 * (2 * D + 16) + 2048;  // two stages of 64 keys (or four waves' of 32), scales; then sums to be joined
+  return 2 * Pitch<D>::stage(64) + 2048;  // two stages of 64 keys (or four waves' of 32), scales; then sums to be joined
 }
 // A workgroup's rows over its keys. SHARED: its four waves take RB x 32 rows each and share every stage of 64 keys; else all
 // of them take the same 32 rows, each every fourth stage of 32 keys, and their sums are joined in LDS.
 template <typename XT, int KV, int D, int NT, bool SHARED, int RB>
 __device__ __forceinline__ void attend(const AttnArgs& a, const Place& p, uint8_t* lds) {
-  constexpr int KEYS = SHARED ? 64 : 32, THREADS = SHARED ? 256 : 64, PITCH = 2 * D + 16, TILE = KEYS * PITCH;
+  constexpr int KEYS = SHARED ? 64 : 32, THREADS = SHARED ? 256 : 64, STAGE = Pitch<D>::stage(KEYS), SUMS = 2 * Pitch<D>::stage(64);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i32 = lane & 31, h = lane >> 5;
   const int r = p.r0 + (SHARED ? RB * AT_ROWS * wave : 0) + i32;
   Wave<KV, D, NT, KEYS / 32, RB> w;
@@ -768,8 +775,8 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Place& p, uint8_
   }
   range.split<KEYS>(p, SHARED ? 1 : AT_NW);
 
-  uint8_t* tile = lds + (SHARED ? 0 : 2 * TILE * wave);
-  float* scales = (float*)(lds + 2 * 2 * 64 * PITCH) + (SHARED ? 0 : 2 * KEYS * wave);
+  uint8_t* tile = lds + (SHARED ? 0 : STAGE * wave);
+  float* scales = (float*)(lds + SUMS) + (SHARED ? 0 : 2 * KEYS * wave);
   const int t = SHARED ? threadIdx.x : lane, step = SHARED ? 1 : AT_NW;
   const int w0 = __builtin_amdgcn_readfirstlane(wave);
   auto first_key = [&](int i) {  // of tile i, in its source
@@ -784,9 +791,9 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Place& p, uint8_
   int i = range.first + (SHARED ? 0 : w0), buf = 0;
   if (i < range.end) load(i);
   for (; i < range.end; i += step) {
-    uint8_t* kl = tile + (SHARED ? buf * 2 * TILE : 0);
+    uint8_t *kl = tile + (SHARED ? buf * STAGE : 0), *vl = kl + KEYS * Pitch<D>::K;
     float* sc = scales + (SHARED ? buf * 2 * KEYS : 0);
-    st.store(kl, kl + TILE, sc, a.scale2, t);
+    st.store(kl, vl, sc, a.scale2, t);
     if (i + step < range.end) load(i + step);
     if constexpr (SHARED) nsx_lds_barrier();
     else __builtin_amdgcn_wave_barrier();
@@ -796,7 +803,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Place& p, uint8_
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) from[rb] = o ? lo[1][rb] : lo[0][rb], to[rb] = o ? hi[1][rb] : hi[0][rb];
     const bool all = key0 >= (o ? all0[1] : all0[0]) && key0 + KEYS <= (o ? all1[1] : all1[0]);
-    w.step(kl, kl + TILE, sc, sc + KEYS, a.scale2, all, key0, from, to);
+    w.step(kl, vl, sc, sc + KEYS, a.scale2, all, key0, from, to);
     buf ^= 1;
     if constexpr (!SHARED) __builtin_amdgcn_wave_barrier();
   }
@@ -832,9 +839,9 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Place& p, uint8_
     // the waves' sums, on the largest of their references
     constexpr int OP = D + 4;
     float* sums = (float*)lds;                         // [wave][row][OP]
-    float2* ml = (float2*)(lds + 2 * 2 * 64 * PITCH);  // [wave][row]
+    float2* ml = (float2*)(lds + SUMS);             // [wave][row]
     uint32_t* odds = (uint32_t*)(ml + AT_NW * AT_ROWS);
-    static_assert(AT_NW * AT_ROWS * OP * 4 <= 2 * 2 * 64 * PITCH && AT_NW * (AT_ROWS * 8 + 4) <= 2048, "LDS");
+    static_assert(AT_NW * AT_ROWS * OP * 4 <= SUMS && AT_NW * (AT_ROWS * 8 + 4) <= 2048, "LDS");
     __syncthreads();
     if (h == 0) ml[wave * AT_ROWS + i32] = float2{m, l};
     if (lane == 0) odds[wave] = bad;
@@ -977,33 +984,38 @@ struct Plan {
   int64_t pblocks, oblocks;
   int splits;
 };
-Plan attn_plan(int G, int rep, int64_t B, int64_t n, int64_t ctx_max, int64_t prefix_max, int window, bool wide) {
+Plan attn_plan(int G, int rep, int64_t B, int64_t n, int64_t ctx_max, int64_t prefix_max, int window, bool wide, int occ) {
   Plan p{};
   const int64_t prows = B * n * rep, orows = n * rep;
   const int64_t pk = window > 0 ? std::min<int64_t>(prefix_max, window + n) : prefix_max;
   const int64_t ok = window > 0 ? std::min<int64_t>(ctx_max, window + n) : ctx_max;
-  // pieces of 32 rows x 32 keys, and how many of them a wave takes where the chip's 2048 waves share them; a wave that has
-  // few keys takes as long as for some 16 pieces more
-  const int64_t pw = G * nsx_cdiv(prows, AT_ROWS) * nsx_cdiv(pk, 32);
-  const int64_t ow = B * G * nsx_cdiv(orows, AT_ROWS) * (nsx_cdiv(ok, 32) + (orows <= 2 * AT_ROWS ? 8 : 0));
-  const int64_t each = std::max<int64_t>(8, nsx_cdiv(pw + ow, 2048));
-  auto cut = [&](int64_t rows, int64_t keys) {
+  // pieces of 32 rows x 32 keys, and how many of them a wave takes where the chip's share them
+  const int64_t slots = 256 * occ, pw = G * nsx_cdiv(prows, AT_ROWS) * nsx_cdiv(pk, 32), ow = B * G * nsx_cdiv(orows, AT_ROWS) * nsx_cdiv(ok, 32);
+  const bool many = nsx_cdiv(pw + ow, 2048) > 20;
+  auto cut = [&](int64_t rows, int64_t keys, int64_t units, int64_t room) {
     AttnArgs::Cut c;
-    const int waves = rows > 2 * AT_ROWS ? 1 : AT_NW;  // that share a row's keys
+    const int waves = rows > 2 * AT_ROWS && many ? 1 : AT_NW;  // that share a row's keys
     c.rows = waves > 1 ? AT_ROWS : wide && rows > AT_NW * AT_ROWS ? 2 * AT_NW * AT_ROWS : AT_NW * AT_ROWS;
     c.tiles = (int)nsx_cdiv(rows, c.rows);
-    const int64_t share = c.rows == 2 * AT_NW * AT_ROWS ? std::max<int64_t>(4, each / 2) : waves * each;
-    c.splits = (int)std::max<int64_t>(1, std::min<int64_t>(AT_MAX_SPLIT / 2, nsx_cdiv(nsx_cdiv(keys, 32), share)));
+    const int64_t most = nsx_cdiv(nsx_cdiv(keys, 32), 3 * waves);
+    c.splits = (int)std::max<int64_t>(1, std::min<int64_t>({AT_MAX_SPLIT / 2, most, room / (units * c.tiles)}));
     return c;
   };
-  const bool apart = prefix_max && orows <= 2 * AT_ROWS;
-  p.own = cut(orows, ok + (apart ? 0 : pk));
-  if (apart) p.pre = cut(prows, pk);
+  const bool apart = prefix_max && orows <= 2 * AT_ROWS && pk + ok > 512;
+  if (apart) {
+    p.own = cut(orows, ok, B * G, std::max<int64_t>(slots / 4, slots * ow / (pw + ow)));
+    const int64_t left = slots - B * G * p.own.tiles * p.own.splits;
+    p.pre = cut(prows, pk, G, many ? slots : std::max<int64_t>(slots / 2, left));
+  } else {
+    p.own = cut(orows, ok + pk, B * G, slots);
+  }
   p.pblocks = (int64_t)G * p.pre.tiles * p.pre.splits;
   p.oblocks = B * G * p.own.tiles * p.own.splits;
   p.splits = p.pre.splits + p.own.splits;
   return p;
 }
+// Workgroups of a kernel that a CU holds.
+int attn_occ(int x_dtype, int head_dim) { return x_dtype == NSX_DT_F32 && head_dim == 128 ? 1 : 2; }
 bool attn_wide(int x_dtype, int head_dim) { return x_dtype == NSX_DT_BF16 && head_dim == 64; }
 
 // ---------------------------------------------------------------------------
@@ -1122,7 +1134,8 @@ extern "C" int64_t nsx_batch_attn_workspace_bytes(int n_head, int n_kv, int head
       n_seq * n >= (1ll << 24) || ctx_max <= 0 || ctx_max >= (1ll << 30) || prefix_max < 0 || prefix_max >= (1ll << 30) || window < 0)
     return -1;
   int splits = 1;  // (whatever the type)
-  for (const bool wide : {false, true}) splits = std::max(splits, attn_plan(n_kv, n_head / n_kv, n_seq, n, ctx_max, prefix_max, window, wide).splits);
+  for (const int dt : {NSX_DT_F32, NSX_DT_F16, NSX_DT_BF16})
+    splits = std::max(splits, attn_plan(n_kv, n_head / n_kv, n_seq, n, ctx_max, prefix_max, window, attn_wide(dt, head_dim), attn_occ(dt, head_dim)).splits);
   return splits > 1 ? n_seq * n * n_head * splits * (head_dim + 2) * 4 : 16;
 }
 
@@ -1148,7 +1161,7 @@ extern "C" int nsx_batch_attn(const void* q, int x_dtype, const nsx_kv_rows* kv,
   NSX_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, NSX_EINVAL,
               "workspace of %lld bytes, %lld needed, 16-byte aligned", (long long)workspace_bytes, (long long)need);
   const Plan plan = attn_plan(n_kv, n_head / n_kv, kv->n_seq, n, kv->ctx_max, prefix ? prefix->ctx_max : 0, window,
-                              attn_wide(x_dtype, head_dim));
+                              attn_wide(x_dtype, head_dim), attn_occ(x_dtype, head_dim));
   NSX_REQUIRE(plan.pblocks + plan.oblocks < (1ll << 24) && kv->n_seq * n * n_head < (1ll << 26), NSX_EINVAL,
               "%lld tokens of %d heads: too many for one call", (long long)(kv->n_seq * n), n_head);
   const AttnArgs a{q, kv_rows(kv), prefix ? kv_rows(prefix) : KvRows{}, counts, sinks, n_head, n_kv, n_head / n_kv, window, n,
