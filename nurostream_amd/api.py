@@ -197,6 +197,14 @@ class NeuroStream:
         n_keep = min(int(torch.searchsorted(mass, torch.tensor([top_p], dtype=mass.dtype))) + 1, p_desc.numel())
         return int(order[torch.multinomial(p_desc[:n_keep], 1)])
 
+    def _draw(self, logits: torch.Tensor, temperature: float, top_p: float, top_k: int, min_p: float) -> torch.Tensor:
+        """A token for each row of logits on the device (model.sampling), with numbers of torch's generator."""
+        from .model.sampling import sample
+        greedy = temperature <= 0
+        u = None if greedy else torch.rand(logits.shape[0], device=logits.device)
+        return sample(logits, u, temperature=0.0 if greedy else float(temperature), top_k=int(top_k),
+                      top_p=float(top_p) if 0 < top_p < 1 else 1.0, min_p=float(min_p))
+
     def _piece(self, token: int) -> str:
         """The token's entry in the GGUF vocabulary (tokenizer.ggml.tokens), or <id> without one."""
         vocab = self.gguf.metadata.get("tokenizer.ggml.tokens")
@@ -205,18 +213,24 @@ class NeuroStream:
         return f"<{token}>"
 
     @staticmethod
-    def _nucleus(logits: torch.Tensor, temperature: float, top_p: float) -> torch.Tensor:
+    def _nucleus(logits: torch.Tensor, temperature: float, top_p: float, top_k: int = 0, min_p: float = 0.0) -> torch.Tensor:
         """Rows of logits with the tokens that `_sample` would not draw at -infinity: all but the smallest set of most
-        likely tokens whose mass reaches top_p (0 < top_p < 1, temperature > 0)."""
-        if temperature <= 0 or not 0 < top_p < 1:
+        likely tokens whose mass reaches top_p (0 < top_p < 1, temperature > 0); with top_k and min_p as
+        `model.sampling.sample` has them, too."""
+        if temperature <= 0 or not (0 < top_p < 1 or top_k > 0 or min_p > 0):
             return logits
-        p_desc, order = torch.sort(torch.softmax(logits.float() / temperature, dim=-1), descending=True, dim=-1)
-        before = torch.cumsum(p_desc, -1) - p_desc
-        return logits.masked_fill(torch.zeros_like(before, dtype=torch.bool).scatter_(-1, order, before >= top_p),
-                                  float("-inf"))
+        p_desc, order = torch.sort(torch.softmax(logits.float() / temperature, dim=-1), descending=True, dim=-1, stable=True)
+        gone = p_desc < min_p * p_desc[..., :1]
+        if top_k > 0:
+            gone[..., top_k:] = True
+            p_desc[..., top_k:] = 0
+        if 0 < top_p < 1:
+            before = torch.cumsum(p_desc, -1) - p_desc
+            gone |= before >= (top_p if top_k <= 0 else top_p * p_desc.sum(-1, keepdim=True))
+        return logits.masked_fill(torch.zeros_like(gone).scatter_(-1, order, gone), float("-inf"))
 
     def _generate_drafted(self, ids: list[int], max_tokens: int, temperature: float, top_p: float, stop_on_eos: bool,
-                          drafts: int, kv_dtype: torch.dtype):
+                          drafts: int, kv_dtype: torch.dtype, top_k: int = 0, min_p: float = 0.0):
         """generate() with several tokens per pass: the prompt in pieces of 64, then passes over the last token and up
         to `drafts` looked-up drafts of what follows it (model.draft)."""
         import time
@@ -234,7 +248,7 @@ class NeuroStream:
         def settle(logits, nodes, parents):
             """(accepted nodes, the token that follows) of a pass, the accepted rows in the cache."""
             u = torch.rand(1, len(nodes), device=self.device) if temperature > 0 else None
-            count, path, token = verify(self._nucleus(logits, temperature, top_p), i32([nodes]), u,
+            count, path, token = verify(self._nucleus(logits, temperature, top_p, top_k, min_p), i32([nodes]), u,
                                         parents=parents, temperature=temperature)
             commit(draft, path[0], count)
             n, nxt, *p = torch.cat([count, token, path[0]]).tolist()
@@ -249,7 +263,7 @@ class NeuroStream:
                 commit(draft, torch.arange(len(piece), dtype=torch.int32, device=self.device), i32([len(piece)]))
                 kv.length += len(piece)
             u = torch.rand(1, 1, device=self.device) if temperature > 0 else None
-            pending = int(verify(self._nucleus(logits, temperature, top_p), i32([ids[-1:]]), u,
+            pending = int(verify(self._nucleus(logits, temperature, top_p, top_k, min_p), i32([ids[-1:]]), u,
                                  temperature=temperature)[2])
         self.stats.prefill_seconds = time.perf_counter() - t0
         eos_id = self.gguf.metadata.get("tokenizer.ggml.eos_token_id")
@@ -284,7 +298,8 @@ class NeuroStream:
         self.stats.decode_seconds = time.perf_counter() - t0
 
     def generate(self, prompt, max_tokens: int = 128, temperature: float = 0.0, top_p: float = 0.95,
-                 stop_on_eos: bool = True, drafts: int = 0, kv_dtype: torch.dtype = torch.float32):
+                 stop_on_eos: bool = True, drafts: int = 0, kv_dtype: torch.dtype = torch.float32, top_k: int = 0,
+                 min_p: float = 0.0):
         """Yield one text piece per generated token (api.py:193-237).
 
         The prompt is a list of token ids: the GGUF tokenizer (text to ids) is
@@ -300,7 +315,9 @@ class NeuroStream:
         the prompt then goes through in pieces of 64 tokens. The tokens are
         distributed as without drafts (temperature 0: the same up to rounding
         between near-equal logits). kv_dtype: torch.float16 / bfloat16 for a
-        KV cache of half the bytes, on the same path."""
+        KV cache of half the bytes, on the same path. top_k > 0, min_p > 0:
+        filters of sampled tokens beside top_p, as model.sampling.sample has
+        them."""
         import time
         from .model.decode import DeviceKV
         if isinstance(prompt, str):
@@ -311,8 +328,11 @@ class NeuroStream:
             raise ValueError("empty prompt")
         if not 0 <= drafts <= 63:
             raise ValueError(f"drafts {drafts}: 0 to 63")
+        if top_k < 0 or not 0 <= min_p <= 1:
+            raise ValueError(f"top_k {top_k}, min_p {min_p}: at least 0, and 0 to 1")
         if drafts or kv_dtype != torch.float32:
-            yield from self._generate_drafted(ids, max_tokens, temperature, top_p, stop_on_eos, int(drafts), kv_dtype)
+            yield from self._generate_drafted(ids, max_tokens, temperature, top_p, stop_on_eos, int(drafts), kv_dtype,
+                                              int(top_k), float(min_p))
             return
         c = self.model.attn_config()
         kv = DeviceKV(self.cfg.n_layer, c, min(c.context_length, len(ids) + max_tokens), self.device)
@@ -326,7 +346,12 @@ class NeuroStream:
         pos = len(ids)
         t0 = time.perf_counter()
         for _ in range(max_tokens):
-            nxt = self._sample(logits[-1], temperature, top_p)
+            if temperature > 0 and (top_k or min_p):
+                nxt = int(self._draw(logits[-1:], temperature, top_p, top_k, min_p))
+                if nxt < 0:
+                    raise FloatingPointError("the model's logits hold no number to choose a token by")
+            else:
+                nxt = self._sample(logits[-1], temperature, top_p)
             if stop_on_eos and nxt in eos:
                 break
             self.stats.generated_tokens += 1
@@ -336,6 +361,75 @@ class NeuroStream:
             with torch.no_grad():
                 logits = self.model.forward([nxt], kv, start_pos=pos)
             pos += 1
+        self.stats.decode_seconds = time.perf_counter() - t0
+
+    def generate_batch(self, prompts, max_tokens: int = 128, temperature: float = 0.0, top_p: float = 0.95, top_k: int = 0,
+                       min_p: float = 0.0, stop_on_eos: bool = True, kv_dtype: torch.dtype = torch.bfloat16):
+        """Several sequences at once: yields, step by step, a list of a text piece per prompt, None for a sequence that has
+        ended (by the end-of-text token, which is not given out, or the context's end). The reference generates one
+        sequence (api.py:193-237).
+
+        prompts: lists of token ids (the same one several times: several answers to it). What all of them begin with is
+        run and kept once, the rest and the answers behind it, in a cache of kv_dtype (torch.bfloat16, int8 or
+        float8_e4m3fn; model.batch). Tokens are sampled as `generate` does, on the GPU (model.sampling)."""
+        import time
+        from .model.batch import BatchKV
+        if isinstance(prompts, str) or any(isinstance(p, str) for p in prompts):
+            raise NotImplementedError("text prompts need the GGUF tokenizer, which is outside this build; "
+                                      "pass lists of token ids")
+        ids = [[int(t) for t in p] for p in prompts]
+        if not ids or not all(ids):
+            raise ValueError("empty prompt")
+        if top_k < 0 or not 0 <= min_p <= 1:
+            raise ValueError(f"top_k {top_k}, min_p {min_p}: at least 0, and 0 to 1")
+        c, B = self.model.attn_config(), len(ids)
+        if max(map(len, ids)) > c.context_length:
+            raise ValueError("prompt and continuation exceed model context length")
+        shared = 0  # every sequence keeps a token of its own: its logits are the first that are wanted
+        while shared < min(map(len, ids)) - 1 and all(p[shared] == ids[0][shared] for p in ids):
+            shared += 1
+        own = [p[shared:] for p in ids]
+        longest, piece = max(map(len, own)), 256
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=self.device)  # noqa: E731
+        self.stats = GenerationStats(prompt_tokens=shared + sum(map(len, own)))
+        t0 = time.perf_counter()
+        with torch.no_grad():
+            prefix = None
+            if shared:
+                prefix = BatchKV(self.cfg.n_layer, c, 1, shared, self.device, dtype=kv_dtype)
+                for i in range(0, shared, piece):
+                    self.model.forward_batch(i32([ids[0][i:min(i + piece, shared)]]), prefix)
+            rows = min(c.context_length - shared, longest + max_tokens)
+            kv = BatchKV(self.cfg.n_layer, c, B, rows, self.device, dtype=kv_dtype, prefix=prefix)
+            step, logits = max(1, piece // B), None
+            for i in range(0, longest, step):
+                cut = [p[i:i + step] for p in own]
+                n = max(map(len, cut))
+                got = self.model.forward_batch(i32([p + [0] * (n - len(p)) for p in cut]), kv, counts=i32([len(p) for p in cut]))
+                ends = i32([i < len(p) <= i + step for p in own]).bool()[:, None]
+                logits = got if logits is None else torch.where(ends, got, logits)
+        self.stats.prefill_seconds = time.perf_counter() - t0
+        eos_id = self.gguf.metadata.get("tokenizer.ggml.eos_token_id")
+        eos = set() if eos_id is None or not stop_on_eos else {int(eos_id)}
+        taken, alive = [len(p) for p in own], [True] * B
+        t0 = time.perf_counter()
+        for given in range(1, max_tokens + 1):
+            tokens = self._draw(logits, temperature, top_p, top_k, min_p)
+            drawn = tokens.tolist()
+            if any(a and t < 0 for a, t in zip(alive, drawn)):
+                raise FloatingPointError("the model's logits hold no number to choose a token by")
+            alive = [a and t not in eos for a, t in zip(alive, drawn)]
+            if not any(alive):
+                break
+            self.stats.generated_tokens += sum(alive)
+            yield [self._piece(t) if a else None for a, t in zip(alive, drawn)]
+            alive = [a and n < c.context_length - shared for a, n in zip(alive, taken)]
+            if given == max_tokens or not any(alive):
+                break
+            kv.length = max(n for a, n in zip(alive, taken) if a)
+            with torch.no_grad():
+                logits = self.model.forward_batch(tokens.clamp(min=0)[:, None], kv, counts=i32([int(a) for a in alive]))
+            taken = [n + a for a, n in zip(alive, taken)]
         self.stats.decode_seconds = time.perf_counter() - t0
 
     # -- warm-up and introspection (api.py:336-341, 399-441) -------------------

@@ -991,7 +991,8 @@ Plan attn_plan(int G, int rep, int64_t B, int64_t n, int64_t ctx_max, int64_t pr
   const int64_t ok = window > 0 ? std::min<int64_t>(ctx_max, window + n) : ctx_max;
   // pieces of 32 rows x 32 keys, and how many of them a wave takes where the chip's share them
   const int64_t slots = 256 * occ, pw = G * nsx_cdiv(prows, AT_ROWS) * nsx_cdiv(pk, 32), ow = B * G * nsx_cdiv(orows, AT_ROWS) * nsx_cdiv(ok, 32);
-  const bool many = nsx_cdiv(pw + ow, 2048) > 20;
+  const int64_t each = nsx_cdiv(pw + ow, 2048);
+  const bool many = each > 20;
   auto cut = [&](int64_t rows, int64_t keys, int64_t units, int64_t room) {
     AttnArgs::Cut c;
     const int waves = rows > 2 * AT_ROWS && many ? 1 : AT_NW;  // that share a row's keys
@@ -1005,7 +1006,7 @@ Plan attn_plan(int G, int rep, int64_t B, int64_t n, int64_t ctx_max, int64_t pr
   if (apart) {
     p.own = cut(orows, ok, B * G, std::max<int64_t>(slots / 4, slots * ow / (pw + ow)));
     const int64_t left = slots - B * G * p.own.tiles * p.own.splits;
-    p.pre = cut(prows, pk, G, many ? slots : std::max<int64_t>(slots / 2, left));
+    p.pre = cut(prows, pk, G, each > 10 ? slots : std::max<int64_t>(slots / 2, left));
   } else {
     p.own = cut(orows, ok + pk, B * G, slots);
   }

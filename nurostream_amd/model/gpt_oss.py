@@ -1026,6 +1026,45 @@ class GptOssModel:
         return self._linear_nodes(name, add_rms_norm(x.contiguous(), None, self.w("output_norm.weight"),
                                                      self.cfg.rms_eps))
 
+    # -- several sequences at once ---------------------------------------------
+
+    def _attention_batch(self, x: torch.Tensor, layer: int, kv, counts) -> torch.Tensor:
+        """x + o_proj(attention) for the new tokens of a batch of sequences, their rows behind the batch's."""
+        from .batch import append_qkv, batch_attn
+        c, p = self.attn_config(), f"blk.{layer}."
+        h = add_rms_norm(x, None, self.w(p + "attn_norm.weight"), self.cfg.rms_eps)
+        cat = self._qkv_raw(layer)
+        if cat is not None:
+            qkv = self._linear_nodes("", h, raw=cat)
+        else:
+            qkv = torch.cat([self._linear_nodes(p + n + ".weight", h) for n in ("attn_q", "attn_k", "attn_v")], -1)
+        b = lambda n: self.w(p + n + ".bias") if self.has(p + n + ".bias") else None  # noqa: E731
+        sinks = self.w(p + "attn_sinks.weight") if self.has(p + "attn_sinks.weight") else None
+        q = append_qkv(qkv, b("attn_q"), b("attn_k"), b("attn_v"), c, self._inv_freq, self._amp, kv, layer, counts=counts)
+        att = batch_attn(q, c, kv, layer, sinks, c.sliding_window if layer % 2 == 0 else 0, counts=counts)
+        return self._linear_nodes(p + "attn_output.weight", att.reshape(x.shape[0], -1), bias=b("attn_output"), resid=x)
+
+    def forward_batch(self, tokens, kv, counts=None, last_only: bool = True) -> torch.Tensor:
+        """The next n tokens of every sequence of a model.batch.BatchKV -- tokens (n_seq, n) device int32, counts (n_seq,)
+        device int32 of them in earnest (None: all) -- through every layer, their rows into the cache, which is moved on.
+        Logits (n_seq, vocab) of each sequence's last token (of its first where it has none), or (n_seq, n, vocab) when
+        not last_only. A prefix is filled the same way, as a batch of one sequence."""
+        self.attn_config()
+        if tokens.dim() != 2 or tokens.shape[0] != kv.n_seq or tokens.dtype != torch.int32:
+            raise ValueError(f"tokens of shape {tuple(tokens.shape)}, {tokens.dtype}: int32 ({kv.n_seq}, n)")
+        B, n = tokens.shape
+        x = self.embed(tokens.reshape(-1)).reshape(B * n, self.cfg.n_embd).contiguous()
+        for layer in range(self.cfg.n_layer):
+            x = self._attention_batch(x, layer, kv, counts)
+            x = self._ffn_block(x, layer)
+        kv.advance(n, counts)
+        if last_only and n > 1:
+            at = torch.full((B,), n - 1, device=x.device) if counts is None else counts.long().clamp(1, n) - 1
+            x = x.reshape(B, n, -1)[torch.arange(B, device=x.device), at]
+        name = "output.weight" if self.has("output.weight") else "token_embd.weight"
+        y = self._linear_nodes(name, add_rms_norm(x.contiguous(), None, self.w("output_norm.weight"), self.cfg.rms_eps))
+        return y if last_only else y.reshape(B, n, -1)
+
     def forward(self, tokens, kv=None, start_pos: int = 0, last_only: bool = True) -> torch.Tensor:
         """Logits (model/gpt_oss.py:207-228): (1, vocab), or (T, vocab) when not
         last_only. Tokens go through one at a time at positions start_pos..;

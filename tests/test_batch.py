@@ -226,3 +226,20 @@ def test_copy_from_refusals():
     other.pos.fill_(10)
     with pytest.raises(ValueError):
         BatchKV(1, cfg, 3, 9, "cpu").copy_from(other)
+
+
+@pytest.mark.parametrize("top_k,top_p,min_p", [(5, 1.0, 0.0), (0, 0.7, 0.05), (12, 0.6, 0.01), (300, 0.95, 0.0), (1, 0.5, 0.9)])
+def test_nucleus_keeps_what_sampling_may_draw(top_k, top_p, min_p):
+    """generate's filter ahead of verification, against the definition written out."""
+    from batch_cases import sample_exact
+    from nurostream_amd.api import NeuroStream
+    g = torch.Generator().manual_seed(top_k)
+    lg = 3 * torch.randn(4, 200, generator=g)
+    kept = NeuroStream._nucleus(lg, 0.8, top_p, top_k, min_p) > float("-inf")
+    u = [(i + 0.5) / 4000 for i in range(4000)]
+    each = lambda x: [x] * 4000  # noqa: E731
+    for r in range(2):
+        drawn = set(sample_exact(lg[r:r + 1].expand(4000, -1), u, each(0.8), each(top_k), each(top_p), each(min_p)))
+        assert drawn <= set(kept[r].nonzero()[:, 0].tolist())
+        heavy = torch.softmax(lg[r].double() / 0.8, -1) * kept[r]
+        assert drawn >= set((heavy / heavy.sum() > 1 / 2000).nonzero()[:, 0].tolist())
