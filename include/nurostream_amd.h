@@ -533,7 +533,8 @@ int nsx_load_rows(const nsx_kv_rows *kv, int kv_type, int n_kv, int head_dim, co
  * meet weights of all 24 bits, fp16 ones of 16, bf16 ones of 8. Rows past the
  * ones seen take no part, whatever they hold. Tokens from counts[b] on, and
  * tokens that see nothing, give zeros. The rows, q, out and the workspace are
- * 16-byte aligned; the workspace is scratch of the call. */
+ * 16-byte aligned; the workspace is scratch of the call (NULL where its bytes
+ * are 0). */
 int64_t nsx_batch_attn_workspace_bytes(int n_head, int n_kv, int head_dim, int64_t n_seq, int64_t n,
                                        int64_t ctx_max, int64_t prefix_max, int window);
 int nsx_batch_attn(const void *q, int x_dtype, const nsx_kv_rows *kv, const nsx_kv_rows *prefix, int kv_type,

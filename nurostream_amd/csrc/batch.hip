@@ -82,48 +82,65 @@ __device__ __forceinline__ uint32_t row_max(uint32_t x) {
   return row_all<LANES>(x, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
 }
 
-// A row's 8 elements per lane into a cache: rounded to bf16, or as codes with the row's scale. The largest is taken of the
-// elements' bits, which order NaN above infinity above every number.
+__device__ __forceinline__ uint32_t near2(float lo, float hi) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{lo, hi}), b2));
+}
+// The codes of a lane's 8 elements of a row, and the row's scale. The largest is taken of the elements' bits, which order NaN
+// above infinity above every number. Elements meet the scale's reciprocal, 2^-23 of a code at most beside the quotient, so that
+// none passes the largest code; scales below 2^-100, whose reciprocals end, are divided by.
 template <int KV, int D>
-__device__ __forceinline__ void put_row(void* rows, float* scales, int64_t row, int l, const float (&x)[8]) {
-  const float a[4] = {x[0], x[1], x[2], x[3]}, b[4] = {x[4], x[5], x[6], x[7]};
-  if constexpr (KV == NSX_DT_BF16) {
-    Bf16* p = (Bf16*)rows + row * D + 4 * l;
-    store4(p, a);
-    store4(p + D / 2, b);
-  } else {
-    uint32_t m = 0;
+__device__ __forceinline__ void codes8(const float (&x)[8], uint32_t (&c)[2], float& scale) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu;
+    m = u > m ? u : m;
+  }
+  m = row_max<D / 8>(m);
+  constexpr float TOP = KV == NSX_KV_INT8 ? 127.f : 448.f;
+  const bool finite = m < 0x7f800000u;
+  const float s = __builtin_bit_cast(float, m) / TOP, r = 1.f / s;
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = x[i] * r;
+  if (!(s >= 0x1p-100f) || !finite) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint32_t u = __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu;
-      m = u > m ? u : m;
+      y[i] = finite && s > 0.f ? fminf(fmaxf(x[i] / s, -TOP), TOP) : 0.f;
+      asm volatile("" : "+v"(y[i]));  // (a branch: few rows take it)
     }
-    m = row_max<D / 8>(m);
-    const bool finite = m < 0x7f800000u;
-    const float s = __builtin_bit_cast(float, m) / (KV == NSX_KV_INT8 ? 127.f : 448.f);
-    uint32_t c[2] = {0, 0};
-    if (finite && s > 0.f) {
-      float y[8];
+  }
+  scale = finite ? s : __builtin_nanf("");
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = x[i] / s;
+  for (int h = 0; h < 2; ++h) {
+    if constexpr (KV == NSX_KV_INT8) {
+      uint32_t z[4];  // 1.5 * 2^23 more: the nearest whole number's low byte in the lowest one
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if constexpr (KV == NSX_KV_INT8) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            c[h] |= ((uint32_t)(int)rintf(fminf(fmaxf(y[4 * h + i], -127.f), 127.f)) & 0xffu) << (8 * i);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) y[4 * h + i] = fminf(fmaxf(y[4 * h + i], -448.f), 448.f);
-          int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], 0, false);
-          c[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], w, true);
-        }
-      }
+      for (int i = 0; i < 4; ++i) z[i] = __builtin_bit_cast(uint32_t, y[4 * h + i] + 12582912.f);
+      c[h] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(z[3], z[2], 0x0c0c0400u), __builtin_amdgcn_perm(z[1], z[0], 0x0c0c0400u), 0x05040100u);
+    } else {
+      const int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], 0, false);
+      c[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], w, true);
     }
+  }
+}
+// A row's 8 elements per lane (4 l .., D / 2 + 4 l ..) into a cache: rounded to bf16, or as codes with the row's scale.
+template <int KV, int D>
+__device__ __forceinline__ void put_row(void* rows, float* scales, int64_t row, int l, const float (&x)[8]) {
+  if constexpr (KV == NSX_DT_BF16) {
+    uint16_t* p = (uint16_t*)rows + row * D + 4 * l;
+    *(v2u*)p = v2u{near2(x[0], x[1]), near2(x[2], x[3])};
+    *(v2u*)(p + D / 2) = v2u{near2(x[4], x[5]), near2(x[6], x[7])};
+  } else {
+    uint32_t c[2];
+    float s;
+    codes8<KV, D>(x, c, s);
     uint8_t* p = (uint8_t*)rows + row * D + 4 * l;
     *(uint32_t*)p = c[0];
     *(uint32_t*)(p + D / 2) = c[1];
-    if (l == 0) scales[row] = finite ? s : __builtin_nanf("");
+    if (l == 0) scales[row] = s;
   }
 }
 // The values of 4 codes, without the scale.
@@ -138,6 +155,7 @@ __device__ __forceinline__ void codes4(uint32_t w, float (&x)[4]) {
     x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
   }
 }
+// Row `row` of a cache, elements 4 l .. and D / 2 + 4 l ..
 template <int KV, int D>
 __device__ __forceinline__ void get_row(const void* rows, const float* scales, int64_t row, int l, float (&x)[8]) {
   float a[4], b[4], s = 1.f;
@@ -250,32 +268,71 @@ struct RowsArgs {
   int G;
 };
 
-template <typename XT, int KV, int D, bool STORE>
+// 8 consecutive elements as they lie
+template <typename T>
+struct alignas(16) Eight {
+  T e[8];
+};
+// A lane 8 consecutive elements of a row, D / 8 lanes a row, a thread RPT rows: all of their loads at once.
+template <typename XT, int KV, int D, bool STORE, int RPT>
 __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
   constexpr int LANES = D / 8, ROWS = 256 / LANES;
   const int l = threadIdx.x % LANES;
-  const int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES;
-  if (r >= a.rows) return;
-  const int64_t bg = r / a.n, b = bg / a.G, at = (a.start ? a.start[b] : a.start0) + (r - bg * a.n);
-  const bool in = at >= 0 && at < a.kv.ctx_max;
-  const int64_t row = bg * a.kv.ctx_max + at;
   const bool v = blockIdx.y;
-  XT* p = (XT*)(v ? a.v : a.k) + r * D + 4 * l;
-  void* cache = v ? a.kv.v : a.kv.k;
-  float* scale = v ? a.kv.vs : a.kv.ks;
-  if constexpr (STORE) {
-    if (!in) return;
-    float lo[4], hi[4];
-    load4(p, lo);
-    load4(p + D / 2, hi);
-    const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    put_row<KV, D>(cache, scale, row, l, x);
-  } else {
-    float x[8] = {};
-    if (in) get_row<KV, D>(cache, scale, row, l, x);
-    const float lo[4] = {x[0], x[1], x[2], x[3]}, hi[4] = {x[4], x[5], x[6], x[7]};
-    store4(p, lo);
-    store4(p + D / 2, hi);
+  XT* x = (XT*)(v ? a.v : a.k);
+  uint8_t* cache = (uint8_t*)(v ? a.kv.v : a.kv.k);
+  float* scales = v ? a.kv.vs : a.kv.ks;
+  const uint32_t n = (uint32_t)a.n, first = blockIdx.x * (ROWS * RPT) + threadIdx.x / LANES, rows = (uint32_t)a.rows;
+  using Code = std::conditional_t<KV == NSX_DT_BF16, v4u, v2u>;
+  Eight<XT> in[RPT] = {};
+  Code code[RPT] = {};
+  float scale[RPT];
+  int64_t at[RPT];
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const uint32_t r = min(first + ROWS * i, rows - 1), bg = r / n, b = bg / (uint32_t)a.G;
+    const int64_t row = (a.start ? (int64_t)a.start[b] : a.start0) + (r - bg * n);
+    at[i] = first + ROWS * i < rows && row >= 0 && row < a.kv.ctx_max ? (int64_t)bg * a.kv.ctx_max + row : -1;
+    if constexpr (STORE) {
+      in[i] = *(const Eight<XT>*)(x + (int64_t)r * D + 8 * l);
+    } else if (at[i] >= 0) {
+      code[i] = *(const Code*)(cache + (at[i] * D + 8 * l) * (int)(sizeof(Code) / 8));
+      scale[i] = KV == NSX_DT_BF16 ? 1.f : scales[at[i]];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    float y[8];
+    if constexpr (STORE) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) y[k] = to_f(in[i].e[k]);
+      if constexpr (KV == NSX_DT_BF16) {
+        if (at[i] >= 0) *(Code*)(cache + (at[i] * D + 8 * l) * 2) = v4u{near2(y[0], y[1]), near2(y[2], y[3]), near2(y[4], y[5]), near2(y[6], y[7])};
+      } else {
+        uint32_t c[2];
+        float s;
+        codes8<KV, D>(y, c, s);  // (every lane of a row has the same `at`)
+        if (at[i] >= 0) {
+          *(Code*)(cache + at[i] * D + 8 * l) = v2u{c[0], c[1]};
+          if (l == 0) scales[at[i]] = s;
+        }
+      }
+    } else if (first + ROWS * i < rows) {
+      float lo[4], hi[4];
+      if constexpr (KV == NSX_DT_BF16) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[k] = nsx_bf2f(code[i][k >> 1] >> (16 * (k & 1)) & 0xffffu);
+      } else {
+        codes4<KV>(code[i][0], lo);
+        codes4<KV>(code[i][1], hi);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[k] = lo[k] * scale[i], y[4 + k] = hi[k] * scale[i];
+      }
+      Eight<XT> out;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) from_f(out.e[k], at[i] >= 0 ? y[k] : 0.f);
+      *(Eight<XT>*)(x + ((int64_t)first + ROWS * i) * D + 8 * l) = out;
+    }
   }
 }
 
@@ -343,11 +400,6 @@ __device__ __forceinline__ uint32_t top2(float lo, float hi) {
 }
 __device__ __forceinline__ float below(float x) {
   return x - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & 0xffff0000u);
-}
-__device__ __forceinline__ uint32_t near2(float lo, float hi) {
-  typedef float f2 __attribute__((ext_vector_type(2)));
-  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{lo, hi}), b2));
 }
 // 8 fp32 as NT bf16 terms: the first ones 8 bits each toward zero, the last one to the nearest (of three: exact).
 template <int NT>
@@ -1112,12 +1164,15 @@ static int move_rows(void* k, void* v, int x_dtype, int64_t n, const int32_t* st
   if (n == 0) return NSX_OK;
   NSX_REQUIRE(k && v && aligned16(k) && aligned16(v), NSX_EINVAL, "k and v must be 16-byte aligned buffers");
   const int64_t rows = kv->n_seq * n_kv * n;
-  const int64_t groups = nsx_cdiv(rows, 256 / (head_dim / 8));
-  NSX_REQUIRE(groups < (1ll << 24), NSX_EINVAL, "%lld rows", (long long)rows);
+  NSX_REQUIRE(rows < (1ll << 28), NSX_EINVAL, "%lld rows: fewer than 2^28", (long long)rows);
   const RowsArgs a{k, v, kv_rows(kv), start, start0, n, rows, n_kv};
   return with_types(x_dtype, kv_type, head_dim, [&](auto x, auto t, auto d) {
-    return nsx_launch(rows_kernel<decltype(x), t(), d(), STORE>, dim3((unsigned)groups, 2), dim3(256), 0,
-                      (hipStream_t)stream, a);
+    // four rows a thread where that leaves workgroups for every CU (4 x 16000 rows of 8 heads into int8: 38 us, with one 53;
+    // 2 rows back: 3.2 us, with one 2.2)
+    constexpr int ROWS = 256 / (d() / 8);
+    const bool four = rows >= 4 * ROWS * 512;
+    auto* kernel = four ? rows_kernel<decltype(x), t(), d(), STORE, 4> : rows_kernel<decltype(x), t(), d(), STORE, 1>;
+    return nsx_launch(kernel, dim3((unsigned)nsx_cdiv(rows, (four ? 4 : 1) * ROWS), 2), dim3(256), 0, (hipStream_t)stream, a);
   });
 }
 extern "C" int nsx_store_rows(const void* k, const void* v, int x_dtype, int64_t n, const int32_t* start, int64_t start0,
@@ -1137,7 +1192,7 @@ extern "C" int64_t nsx_batch_attn_workspace_bytes(int n_head, int n_kv, int head
   int splits = 1;  // (whatever the type)
   for (const int dt : {NSX_DT_F32, NSX_DT_F16, NSX_DT_BF16})
     splits = std::max(splits, attn_plan(n_kv, n_head / n_kv, n_seq, n, ctx_max, prefix_max, window, attn_wide(dt, head_dim), attn_occ(dt, head_dim)).splits);
-  return splits > 1 ? n_seq * n * n_head * splits * (head_dim + 2) * 4 : 16;
+  return splits > 1 ? n_seq * n * n_head * splits * (head_dim + 2) * 4 : 0;
 }
 
 extern "C" int nsx_batch_attn(const void* q, int x_dtype, const nsx_kv_rows* kv, const nsx_kv_rows* prefix, int kv_type,
@@ -1159,7 +1214,7 @@ extern "C" int nsx_batch_attn(const void* q, int x_dtype, const nsx_kv_rows* kv,
   NSX_REQUIRE(q && out && kv->pos && aligned16(q) && aligned16(out), NSX_EINVAL, "q and out must be 16-byte aligned buffers");
   const int64_t need = nsx_batch_attn_workspace_bytes(n_head, n_kv, head_dim, kv->n_seq, n, kv->ctx_max,
                                                       prefix ? prefix->ctx_max : 0, window);
-  NSX_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, NSX_EINVAL,
+  NSX_REQUIRE((workspace || !need) && aligned16(workspace) && workspace_bytes >= need, NSX_EINVAL,
               "workspace of %lld bytes, %lld needed, 16-byte aligned", (long long)workspace_bytes, (long long)need);
   const Plan plan = attn_plan(n_kv, n_head / n_kv, kv->n_seq, n, kv->ctx_max, prefix ? prefix->ctx_max : 0, window,
                               attn_wide(x_dtype, head_dim), attn_occ(x_dtype, head_dim));

@@ -23,6 +23,7 @@ from .. import _native as N
 from .decode import AttnConfig, DeviceKV
 from .draft import _call, _check, _ptr
 
+X_TYPES = {torch.float32: N.DT_F32, torch.float16: N.DT_F16, torch.bfloat16: N.DT_BF16}
 ROW_TYPES = {torch.bfloat16: N.DT_BF16, torch.int8: N.KV_INT8, torch.float8_e4m3fn: N.KV_E4M3}
 
 
@@ -59,19 +60,20 @@ class BatchKV:
                 raise ValueError("a prefix is one sequence without a prefix of its own")
             if (prefix.heads, prefix.dtype, prefix.device, prefix.k_stack.shape[0]) != (self.heads, dtype, self.device, n_layer):
                 raise ValueError("a prefix has its batch's layers, heads, row type and device")
-        self._kind = ROW_TYPES[dtype]
-        self._layers: dict[int, N.KvRowsC] = {}
+        self._kind, self._index = ROW_TYPES[dtype], self.k_stack.get_device()
+        self._scratch: dict[tuple, int] = {}  # bytes of the attention's workspace by sizes
+        self._layers: dict = {}
 
-    def rows(self, layer: int) -> N.KvRowsC:
-        """A layer as the kernels take it."""
+    def rows(self, layer: int):
+        """A layer as the kernels take it (a reference to its nsx_kv_rows)."""
         got = self._layers.get(layer)
         if got is None:
             if not 0 <= layer < self.k_stack.shape[0]:
                 raise IndexError(f"layer {layer} of {self.k_stack.shape[0]}")
-            got = N.KvRowsC(self.k_stack[layer].data_ptr(), self.v_stack[layer].data_ptr(),
+            got = C.byref(N.KvRowsC(self.k_stack[layer].data_ptr(), self.v_stack[layer].data_ptr(),
                             None if self.k_scale is None else self.k_scale[layer].data_ptr(),
                             None if self.v_scale is None else self.v_scale[layer].data_ptr(), self.pos.data_ptr(), self.n_seq,
-                            self.ctx_max)
+                            self.ctx_max))
             self._layers[layer] = got
         return got
 
@@ -84,7 +86,7 @@ class BatchKV:
         return {k: v for k, v in self.__dict__.items() if k != "_layers"}
 
     def __setstate__(self, state) -> None:
-        self.__dict__.update(state, _layers={})
+        self.__dict__.update(state, _layers={}, _index=state["k_stack"].get_device())
 
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.k_stack, self.v_stack, self.k_scale, self.v_scale)
@@ -133,18 +135,27 @@ class BatchKV:
         self.length = n
 
 
-def _tokens(x: torch.Tensor, row: int, name: str, kv: BatchKV, cfg: AttnConfig, counts) -> int:
+def _fits(t: torch.Tensor, dtype: torch.dtype, index: int, numel: int) -> bool:
+    """What `_check` looks for on the GPU, in the least of the host's time."""
+    return t.dtype is dtype and t.get_device() == index and t.numel() == numel and t.is_contiguous()
+
+
+def _tokens(x: torch.Tensor, heads: int, name: str, kv: BatchKV, cfg: AttnConfig, counts) -> int:
     """Checks shared by the calls on tokens -> tokens per sequence."""
     N.require_device(x)
-    N.act_dtype_code(x.dtype)
-    if (cfg.n_head_kv, cfg.head_dim) != kv.heads or cfg.n_head % cfg.n_head_kv:
-        raise ValueError("{} query heads over {} of {}; the cache was made for {} of {}".format(
-            cfg.n_head, cfg.n_head_kv, cfg.head_dim, *kv.heads))
-    n = x.numel() // (kv.n_seq * row) if row else 0
-    _check(name, x, x.dtype, kv.device, kv.n_seq * n * row)
-    if n < 1:
-        raise ValueError(f"{name} of shape {tuple(x.shape)} for {kv.n_seq} sequences and rows of {row}")
-    _check("counts", counts, torch.int32, kv.device, kv.n_seq)
+    if x.dtype not in X_TYPES:
+        N.act_dtype_code(x.dtype)
+    G, d = kv.heads
+    if cfg.n_head_kv != G or cfg.head_dim != d or cfg.n_head % G:
+        raise ValueError(f"{cfg.n_head} query heads over {cfg.n_head_kv} of {cfg.head_dim}; the cache was made for {G} of {d}")
+    numel, row = x.numel(), kv.n_seq * heads * d
+    n = numel // row
+    if n < 1 or n * row != numel:
+        raise ValueError(f"{name} of shape {tuple(x.shape)} for {kv.n_seq} sequences and rows of {heads * d}")
+    if not _fits(x, x.dtype, kv._index, numel):
+        _check(name, x, x.dtype, kv.device, numel)
+    if counts is not None and not _fits(counts, torch.int32, kv._index, kv.n_seq):
+        _check("counts", counts, torch.int32, kv.device, kv.n_seq)
     if kv.length + n > kv.ctx_max:
         raise ValueError(f"{n} tokens behind up to {kv.length} rows of a cache of {kv.ctx_max}")
     return n
@@ -162,16 +173,20 @@ def append_qkv(qkv: torch.Tensor, bq, bk, bv, cfg: AttnConfig, inv_freq: torch.T
     int32: how many of the n tokens a sequence has; the others' queries are zero, and they leave no rows. Rows past the
     cache's end by the device's position are not written; the host's kv.length is checked."""
     d, H, G = cfg.head_dim, cfg.n_head, cfg.n_head_kv
-    n = _tokens(qkv, (H + 2 * G) * d, "qkv", kv, cfg, counts)
-    dev = kv.device
+    n = _tokens(qkv, H + 2 * G, "qkv", kv, cfg, counts)
+    index = kv._index
     for name, t, m in (("bq", bq, H * d), ("bk", bk, G * d), ("bv", bv, G * d), ("inv_freq", inv_freq, d // 2),
                        ("q_norm", q_norm, d), ("k_norm", k_norm, d)):
-        _check(name, t, torch.float32, dev, m)
-    _check("out", out, qkv.dtype, dev, kv.n_seq * n * H * d)
-    q = torch.empty((kv.n_seq, n, H, d), dtype=qkv.dtype, device=dev) if out is None else out
-    _call("append_qkv", N.load().nsx_append_qkv, dev, qkv.data_ptr(), N.act_dtype_code(qkv.dtype), _ptr(bq), _ptr(bk),
-          _ptr(bv), _ptr(q_norm), _ptr(k_norm), float(eps), inv_freq.data_ptr(), float(amp), H, G, d, n, _ptr(counts),
-          C.byref(kv.rows(layer)), kv._kind, None if kv.prefix is None else kv.prefix.pos.data_ptr(), q.data_ptr())
+        if t is not None and not _fits(t, torch.float32, index, m):
+            _check(name, t, torch.float32, kv.device, m)
+    if out is None:
+        q = qkv.new_empty((kv.n_seq, n, H, d))
+    else:
+        _check("out", out, qkv.dtype, kv.device, kv.n_seq * n * H * d)
+        q = out
+    _call("append_qkv", N.load().nsx_append_qkv, kv.device, qkv.data_ptr(), X_TYPES[qkv.dtype], _ptr(bq), _ptr(bk), _ptr(bv),
+          _ptr(q_norm), _ptr(k_norm), eps, inv_freq.data_ptr(), amp, H, G, d, n, _ptr(counts), kv.rows(layer), kv._kind,
+          None if kv.prefix is None else kv.prefix.pos.data_ptr(), q.data_ptr())
     return q
 
 
@@ -183,25 +198,36 @@ def batch_attn(q: torch.Tensor, cfg: AttnConfig, kv: BatchKV, layer: int, sinks:
     of 24; weights are rounded to 16 bits beside fp16 queries, to 8 beside bf16 ones. Tokens that a sequence does not have
     (`counts`) give zeros."""
     d, H, G = cfg.head_dim, cfg.n_head, cfg.n_head_kv
-    n = _tokens(q, H * d, "q", kv, cfg, counts)
-    _check("sinks", sinks, torch.float32, kv.device, H)
-    _check("out", out, q.dtype, kv.device, q.numel())
+    n, window, prefix = _tokens(q, H, "q", kv, cfg, counts), int(window), kv.prefix
+    if sinks is not None and not _fits(sinks, torch.float32, kv._index, H):
+        _check("sinks", sinks, torch.float32, kv.device, H)
     if window < 0:
         raise ValueError(f"window {window}")
-    y = torch.empty((kv.n_seq, n, H, d), dtype=q.dtype, device=kv.device) if out is None else out
-    lib, prefix = N.load(), kv.prefix
-    nb = lib.nsx_batch_attn_workspace_bytes(H, G, d, kv.n_seq, n, kv.ctx_max, 0 if prefix is None else prefix.ctx_max, int(window))
-    ws = torch.empty(max(nb, 16), dtype=torch.uint8, device=kv.device)  # stream-ordered scratch, as the output
-    _call("batch_attn", lib.nsx_batch_attn, kv.device, q.data_ptr(), N.act_dtype_code(q.dtype), C.byref(kv.rows(layer)),
-          None if prefix is None else C.byref(prefix.rows(layer)), kv._kind, H, G, d, n, _ptr(counts), _ptr(sinks), int(window),
-          1.0 / math.sqrt(d), ws.data_ptr(), ws.numel(), y.data_ptr())
+    if out is None:
+        y = q.new_empty((kv.n_seq, n, H, d))
+    else:
+        _check("out", out, q.dtype, kv.device, q.numel())
+        y = out
+    lib = N.load()
+    nb = kv._scratch.get((H, n, window))  # (by sizes alone: the prefix is the one that the cache was made with)
+    if nb is None:
+        nb = lib.nsx_batch_attn_workspace_bytes(H, G, d, kv.n_seq, n, kv.ctx_max, 0 if prefix is None else prefix.ctx_max, window)
+        if nb < 0:
+            raise ValueError(f"{n} tokens of {kv.n_seq} sequences: too many for one call")
+        kv._scratch[H, n, window] = nb
+    # stream-ordered scratch, as the output
+    ws = None if nb == 0 else torch.empty(nb, dtype=torch.uint8, device=kv.device).data_ptr()
+    _call("batch_attn", lib.nsx_batch_attn, kv.device, q.data_ptr(), X_TYPES[q.dtype], kv.rows(layer),
+          None if prefix is None else prefix.rows(layer), kv._kind, H, G, d, n, _ptr(counts), _ptr(sinks), window,
+          1.0 / math.sqrt(d), ws, nb, y.data_ptr())
     return y
 
 
 def _first(start, kv: BatchKV, n: int) -> tuple[torch.Tensor | None, int]:
     """A run of rows' first one: (device array, 0) or (None, the host's number, checked)."""
     if isinstance(start, torch.Tensor):
-        _check("start", start, torch.int32, kv.device, kv.n_seq)
+        if not _fits(start, torch.int32, kv._index, kv.n_seq):
+            _check("start", start, torch.int32, kv.device, kv.n_seq)
         return start, 0
     start = int(start)
     if start < 0 or start + n > kv.ctx_max:
@@ -222,14 +248,14 @@ def store_rows(k: torch.Tensor, v: torch.Tensor, kv: BatchKV, layer: int, start:
     _check("v", v, k.dtype, kv.device)
     first, start0 = _first(start, kv, k.shape[2])
     _call("store_rows", N.load().nsx_store_rows, kv.device, k.data_ptr(), v.data_ptr(), code, k.shape[2], _ptr(first), start0,
-          G, d, C.byref(kv.rows(layer)), kv._kind)
+          G, d, kv.rows(layer), kv._kind)
 
 
 def load_rows(kv: BatchKV, layer: int, start: int | torch.Tensor, n: int,
               dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
     """(k, v): the values that rows start .. start + n - 1 of every sequence stand for, (n_seq, n_kv, n, head_dim) of dtype
     (fp32 / fp16 / bf16). start as in `store_rows`; rows outside the cache give zeros."""
-    code = N.act_dtype_code(dtype)
+    code = X_TYPES[dtype] if dtype in X_TYPES else N.act_dtype_code(dtype)
     G, d = kv.heads
     if n < 0:
         raise ValueError(f"{n} rows")
@@ -237,7 +263,7 @@ def load_rows(kv: BatchKV, layer: int, start: int | torch.Tensor, n: int,
     N.require_device(kv.k_stack)
     k = torch.empty((kv.n_seq, G, n, d), dtype=dtype, device=kv.device)
     v = torch.empty_like(k)
-    _call("load_rows", N.load().nsx_load_rows, kv.device, C.byref(kv.rows(layer)), kv._kind, G, d, _ptr(first), start0, n,
+    _call("load_rows", N.load().nsx_load_rows, kv.device, kv.rows(layer), kv._kind, G, d, _ptr(first), start0, n,
           k.data_ptr(), v.data_ptr(), code)
     return k, v
 

@@ -74,7 +74,7 @@ def _attn(lib, **kw):
     a = dict(q=A, dt=N.DT_F32, kv=None, prefix=None, kind=N.KV_INT8, H=16, G=2, d=64, n=5, counts=None, sinks=None, window=0,
              scale=0.125, ws=A, wsb=1 << 40, out=A)
     a.update(kw)
-    return lib.nsx_batch_attn(a["q"], a["dt"], C.byref(a["kv"] or _rows()), a["prefix"] and C.byref(a["prefix"]), a["kind"], a["H"],
+    return lib.nsx_batch_attn(a["q"], a["dt"], C.byref(a["kv"] or _rows(ctx_max=5000)), a["prefix"] and C.byref(a["prefix"]), a["kind"], a["H"],
                               a["G"], a["d"], a["n"], a["counts"], a["sinks"], a["window"], a["scale"], a["ws"], a["wsb"],
                               a["out"], None)
 
@@ -82,7 +82,8 @@ def _attn(lib, **kw):
 @pytest.mark.parametrize("kw,code", [
     (dict(dt=3), N.ETYPE), (dict(kind=0), N.ETYPE), (dict(d=32), N.ENOTIMPL), (dict(H=17), N.EINVAL), (dict(n=-2), N.EINVAL),
     (dict(n=1 << 23), N.EINVAL), (dict(window=-1), N.EINVAL), (dict(q=None), N.EINVAL), (dict(out=None), N.EINVAL),
-    (dict(q=A + 8), N.EINVAL), (dict(out=A + 4), N.EINVAL), (dict(ws=None), N.EINVAL), (dict(ws=A + 8), N.EINVAL),
+    (dict(q=A + 8), N.EINVAL), (dict(out=A + 4), N.EINVAL), (dict(ws=None), N.EINVAL), (dict(scale=0.0), N.EINVAL), (dict(scale=-1.0), N.EINVAL),
+    (dict(scale=float("nan")), N.EINVAL), (dict(scale=float("inf")), N.EINVAL), (dict(ws=A + 8), N.EINVAL),
     (dict(wsb=0), N.EINVAL), (dict(n=0), N.OK)])
 def test_attention_checks(lib, kw, code):
     assert _attn(lib, **kw) == code
@@ -145,7 +146,7 @@ def test_cache_object():
     with pytest.raises(IndexError):
         kv.rows(2)
     twin = copy.deepcopy(kv)  # tensors of its own, and their addresses
-    assert twin.rows(1).k == twin.k_stack[1].data_ptr() != kv.rows(1).k and twin.prefix.k_stack is not prefix.k_stack
+    assert twin.rows(1)._obj.k == twin.k_stack[1].data_ptr() != kv.rows(1)._obj.k and twin.prefix.k_stack is not prefix.k_stack
     assert kv.nbytes() == 2 * 2 * 3 * 2 * 10 * (64 + 4)
     kv.advance(4)
     kv.advance(5, counts=torch.tensor([0, 9, 2], dtype=torch.int32))
