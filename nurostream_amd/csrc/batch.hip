@@ -637,18 +637,18 @@ struct Wave {
   __device__ __forceinline__ void step(const uint8_t* kl, const uint8_t* vl, const float* sk, const float* sv, float c, bool all,
                                        int key0, const int (&lo)[RB], const int (&hi)[RB]) {
     const int lane = threadIdx.x & 63, i32 = lane & 31, h = lane >> 5;
+    f16v s[RB][NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      f16v s[RB];
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) s[rb] = f16v{};
+      for (int rb = 0; rb < RB; ++rb) s[rb][nb] = f16v{};
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
         const v4u k = *(const v4u*)(kl + (32 * nb + i32) * Pitch<D>::K + 32 * ks + 16 * h);
 #pragma unroll
         for (int t = NT - 1; t >= 0; --t)
 #pragma unroll
-          for (int rb = 0; rb < RB; ++rb) s[rb] = dot(k, q[rb][t][ks], s[rb]);
+          for (int rb = 0; rb < RB; ++rb) s[rb][nb] = dot(k, q[rb][t][ks], s[rb][nb]);
       }
       if constexpr (KV != NSX_DT_BF16) {  // (a score's factor is its key's scale, which has the one of all in it)
 #pragma unroll
@@ -657,40 +657,52 @@ struct Wave {
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s[rb][e + k] *= f[k];
+            for (int k = 0; k < 4; ++k) s[rb][nb][e + k] *= f[k];
         }
       }
-      if (!all) {
+    }
+    if (!all) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int key = key0 + 32 * nb + 8 * (e >> 2) + 4 * h + (e & 3);
-            float x = key >= lo[rb] && key < hi[rb] ? s[rb][e] : -INFINITY;
+            float x = key >= lo[rb] && key < hi[rb] ? s[rb][nb][e] : -INFINITY;
             asm volatile("" : "+v"(x));  // (a branch, not selects: few tiles take it)
-            s[rb][e] = x;
+            s[rb][nb][e] = x;
           }
-      }
-      // The reference is an earlier maximum, moved only when a score is 8 above it: weights stay below 2^8, and the sums are
-      // seldom rescaled.
+    }
+    // The reference is an earlier maximum, moved only when a score is 8 above it: weights stay below 2^8, and the sums are
+    // seldom rescaled.
+    float most[RB];
+    bool moved = false;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      most[rb] = s[rb][0][0];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) most[rb] = fmaxf(fmaxf(most[rb], s[rb][nb][e]), s[rb][nb][e + 1]);
+      most[rb] = other_half_max(most[rb]);
+      if (KV == NSX_DT_BF16) most[rb] *= c;
+      moved = moved || most[rb] > m[rb] + 8.f;
+    }
+    if (__any(moved)) {
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
-        float most = s[rb][0];
+        const float to = fmaxf(most[rb], m[rb]), by = __builtin_amdgcn_exp2f(m[rb] - to);
+        m[rb] = to;
+        l[rb] *= by;
 #pragma unroll
-        for (int e = 1; e < 16; ++e) most = fmaxf(most, s[rb][e]);
-        most = other_half_max(most);
-        if (KV == NSX_DT_BF16) most *= c;
-        if (__any(most > m[rb] + 8.f)) {
-          const float to = fmaxf(most, m[rb]), by = __builtin_amdgcn_exp2f(m[rb] - to);
-          m[rb] = to;
-          l[rb] *= by;
+        for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-          for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[rb][i][e] *= by;
-        }
+          for (int e = 0; e < 16; ++e) acc[rb][i][e] *= by;
       }
-      v4u w[RB][2][NT];
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
         v4f g[2];  // the values' scales
@@ -698,23 +710,21 @@ struct Wave {
 #pragma unroll
           for (int e = 0; e < 2; ++e) g[e] = *(const v4f*)(sv + 32 * nb + 16 * kb + 8 * e + 4 * h);
         }
+        v4u w[RB][NT];
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
           float x[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float y = s[rb][8 * kb + e];
+            const float y = s[rb][nb][8 * kb + e];
             x[e] = __builtin_amdgcn_exp2f(KV == NSX_DT_BF16 ? fmaf(y, c, -m[rb]) : y - m[rb]);
             l[rb] += x[e];
             if constexpr (KV != NSX_DT_BF16) x[e] *= g[e >> 2][e & 3];
           }
-          terms8<NT>(x, w[rb][kb]);
+          terms8<NT>(x, w[rb]);
         }
-      }
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
+        for (int i = 0; i < D / 32; ++i) {
           // values of dimension 32 i + lane % 32, keys 16 kb + 4 h .. + 3 and 8 behind them
           const uint8_t* at = vl + (32 * nb + 16 * kb + 4 * h + ((lane & 15) >> 2)) * Pitch<D>::V +
                               2 * (32 * i + 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
@@ -725,9 +735,9 @@ struct Wave {
 #pragma unroll
           for (int t = NT - 1; t >= 0; --t)
 #pragma unroll
-            for (int rb = 0; rb < RB; ++rb) acc[rb][i] = dot(v, w[rb][kb][t], acc[rb][i]);
+            for (int rb = 0; rb < RB; ++rb) acc[rb][i] = dot(v, w[rb][t], acc[rb][i]);
         }
-    }
+      }
   }
   __device__ __forceinline__ bool finite(int rb) const {
     float z = l[rb] * 0.f;
