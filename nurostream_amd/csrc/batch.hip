@@ -599,22 +599,22 @@ struct Pitch {
   static constexpr int stage(int keys) { return keys * (K + V); }
 };
 
-// A wave's RB x 32 rows over its keys. Scores are K Q^T, so that a lane holds 16 of 32 keys' scores of one row (lane % 32; the
+// A wave's 32 rows over its keys. Scores are K Q^T, so that a lane holds 16 of 32 keys' scores of one row (lane % 32; the
 // other lane of the row holds the others), and its weights are at once the second operand of V^T W^T, of which it holds D / 2
 // values of the same row. The operand's order of keys is the scores' own, and V's rows are read from LDS in it, transposed.
-template <int KV, int D, int NT, int NB, int RB>
+template <int KV, int D, int NT, int NB>
 struct Wave {
-  v4u q[RB][NT][D / 16];
-  f16v acc[RB][D / 32];
-  float m[RB], l[RB];
+  v4u q[NT][D / 16];
+  f16v acc[D / 32];
+  float m, l;
 
   template <typename XT>
-  __device__ __forceinline__ void start(int rb, const XT* row) {
+  __device__ __forceinline__ void start(const XT* row) {
     const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
       if constexpr (NT == 1) {
-        q[rb][0][ks] = *(const v4u*)(row + 16 * ks + 8 * h);
+        q[0][ks] = *(const v4u*)(row + 16 * ks + 8 * h);
       } else {
         float a[4], b[4];
         load4(row + 16 * ks + 8 * h, a);
@@ -623,41 +623,40 @@ struct Wave {
         v4u t[NT];
         terms8<NT>(x, t);
 #pragma unroll
-        for (int k = 0; k < NT; ++k) q[rb][k][ks] = t[k];
+        for (int k = 0; k < NT; ++k) q[k][ks] = t[k];
       }
     }
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[rb][i] = f16v{};
-    m[rb] = LOWEST;
-    l[rb] = 0.f;
+    for (int i = 0; i < D / 32; ++i) acc[i] = f16v{};
+    m = LOWEST;
+    l = 0.f;
   }
 
-  // NB blocks of 32 keys in LDS, the first of them key `key0` of its source; row rb of the lane sees [lo, hi) (`all`: these
-  // keys at least).
+  // NB blocks of 32 keys in LDS, the first of them key `key0` of its source; the lane's row sees [lo, hi) (`all`: these keys at
+  // least).
   __device__ __forceinline__ void step(const uint8_t* kl, const uint8_t* vl, const float* sk, const float* sv, float c, bool all,
-                                       int key0, const int (&lo)[RB], const int (&hi)[RB]) {
+                                       int key0, int lo, int hi) {
     const int lane = threadIdx.x & 63, i32 = lane & 31, h = lane >> 5;
-    f16v s[RB][NB];
+    f16v s[NB];
+    v4u k[D / 16];
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) k[ks] = *(const v4u*)(kl + i32 * Pitch<D>::K + 32 * ks + 16 * h);
+    if constexpr (D == 64) __builtin_amdgcn_sched_barrier(0);  // (all of them on their way before the first is waited for)
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) s[rb][nb] = f16v{};
+      s[nb] = f16v{};
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
-        const v4u k = *(const v4u*)(kl + (32 * nb + i32) * Pitch<D>::K + 32 * ks + 16 * h);
 #pragma unroll
-        for (int t = NT - 1; t >= 0; --t)
-#pragma unroll
-          for (int rb = 0; rb < RB; ++rb) s[rb][nb] = dot(k, q[rb][t][ks], s[rb][nb]);
+        for (int t = NT - 1; t >= 0; --t) s[nb] = dot(k[ks], q[t][ks], s[nb]);
+        if (nb + 1 < NB) k[ks] = *(const v4u*)(kl + (32 * (nb + 1) + i32) * Pitch<D>::K + 32 * ks + 16 * h);
       }
       if constexpr (KV != NSX_DT_BF16) {  // (a score's factor is its key's scale, which has the one of all in it)
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
           const v4f f = *(const v4f*)(sk + 32 * nb + 2 * e + 4 * h);
 #pragma unroll
-          for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) s[rb][nb][e + k] *= f[k];
+          for (int x = 0; x < 4; ++x) s[nb][e + x] *= f[x];
         }
       }
     }
@@ -665,86 +664,85 @@ struct Wave {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int key = key0 + 32 * nb + 8 * (e >> 2) + 4 * h + (e & 3);
-            float x = key >= lo[rb] && key < hi[rb] ? s[rb][nb][e] : -INFINITY;
-            asm volatile("" : "+v"(x));  // (a branch, not selects: few tiles take it)
-            s[rb][nb][e] = x;
-          }
+        for (int e = 0; e < 16; ++e) {
+          const int key = key0 + 32 * nb + 8 * (e >> 2) + 4 * h + (e & 3);
+          float x = key >= lo && key < hi ? s[nb][e] : -INFINITY;
+          asm volatile("" : "+v"(x));  // (a branch, not selects: few tiles take it)
+          s[nb][e] = x;
+        }
     }
     // The reference is an earlier maximum, moved only when a score is 8 above it: weights stay below 2^8, and the sums are
     // seldom rescaled.
-    float most[RB];
-    bool moved = false;
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      most[rb] = s[rb][0][0];
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) most[rb] = fmaxf(fmaxf(most[rb], s[rb][nb][e]), s[rb][nb][e + 1]);
-      most[rb] = other_half_max(most[rb]);
-      if (KV == NSX_DT_BF16) most[rb] *= c;
-      moved = moved || most[rb] > m[rb] + 8.f;
-    }
-    if (__any(moved)) {
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        const float to = fmaxf(most[rb], m[rb]), by = __builtin_amdgcn_exp2f(m[rb] - to);
-        m[rb] = to;
-        l[rb] *= by;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[rb][i][e] *= by;
-      }
-    }
+    float most = s[0][0];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        v4f g[2];  // the values' scales
-        if constexpr (KV != NSX_DT_BF16) {
+      for (int e = 0; e < 16; e += 2) most = fmaxf(fmaxf(most, s[nb][e]), s[nb][e + 1]);
+    most = other_half_max(most);
+    if (KV == NSX_DT_BF16) most *= c;
+    if (__any(most > m + 8.f)) {
+      const float to = fmaxf(most, m), by = __builtin_amdgcn_exp2f(m - to);
+      m = to;
+      l *= by;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) g[e] = *(const v4f*)(sv + 32 * nb + 16 * kb + 8 * e + 4 * h);
-        }
-        v4u w[RB][NT];
+      for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          float x[8];
+        for (int e = 0; e < 16; ++e) acc[i][e] *= by;
+    }
+    // 16 keys at a time: their products stand beside the next ones' exponentials
+    v4u v[D / 32], w[NT];
+    auto load = [&](int u, v4u (&to)[D / 32]) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float y = s[rb][nb][8 * kb + e];
-            x[e] = __builtin_amdgcn_exp2f(KV == NSX_DT_BF16 ? fmaf(y, c, -m[rb]) : y - m[rb]);
-            l[rb] += x[e];
-            if constexpr (KV != NSX_DT_BF16) x[e] *= g[e >> 2][e & 3];
-          }
-          terms8<NT>(x, w[rb]);
-        }
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          // values of dimension 32 i + lane % 32, keys 16 kb + 4 h .. + 3 and 8 behind them
-          const uint8_t* at = vl + (32 * nb + 16 * kb + 4 * h + ((lane & 15) >> 2)) * Pitch<D>::V +
-                              2 * (32 * i + 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
-          const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s4*)at);
-          const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s4*)(at + 8 * Pitch<D>::V));
-          const v2u a2 = __builtin_bit_cast(v2u, a), b2 = __builtin_bit_cast(v2u, b);
-          const v4u v = {a2[0], a2[1], b2[0], b2[1]};
-#pragma unroll
-          for (int t = NT - 1; t >= 0; --t)
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb) acc[rb][i] = dot(v, w[rb][t], acc[rb][i]);
-        }
+      for (int i = 0; i < D / 32; ++i) {
+        // values of dimension 32 i + lane % 32, keys 16 u + 4 h .. + 3 and 8 behind them
+        const uint8_t* at = vl + (16 * u + 4 * h + ((lane & 15) >> 2)) * Pitch<D>::V + 2 * (32 * i + 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
+        const v2u a = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s4*)at));
+        const v2u b = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s4*)(at + 8 * Pitch<D>::V)));
+        to[i] = v4u{a[0], a[1], b[0], b[1]};
       }
+    };
+    auto weigh = [&](int u, v4u (&to)[NT]) {
+      v4f g[2];  // the values' scales
+      if constexpr (KV != NSX_DT_BF16) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) g[e] = *(const v4f*)(sv + 16 * u + 8 * e + 4 * h);
+      }
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = s[u >> 1][8 * (u & 1) + e];
+        x[e] = __builtin_amdgcn_exp2f(KV == NSX_DT_BF16 ? fmaf(y, c, -m) : y - m);
+        l += x[e];
+        if constexpr (KV != NSX_DT_BF16) x[e] *= g[e >> 2][e & 3];
+      }
+      terms8<NT>(x, to);
+    };
+    load(0, v);
+    weigh(0, w);
+#pragma unroll
+    for (int u = 0; u < 2 * NB; ++u) {
+      v4u vn[D / 32], wn[NT];
+      if constexpr (D == 64) __builtin_amdgcn_sched_barrier(0);
+      if (u + 1 < 2 * NB) load(u + 1, vn);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int t = NT - 1; t >= 0; --t) acc[i] = dot(v[i], w[t], acc[i]);
+      if (u + 1 < 2 * NB) {
+        weigh(u + 1, wn);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) v[i] = vn[i];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) w[t] = wn[t];
+      }
+    }
   }
-  __device__ __forceinline__ bool finite(int rb) const {
-    float z = l[rb] * 0.f;
+  __device__ __forceinline__ bool finite() const {
+    float z = l * 0.f;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) z = fmaf(acc[rb][i][e], 0.f, z);
+      for (int e = 0; e < 16; ++e) z = fmaf(acc[i][e], 0.f, z);
     return z == 0.f;
   }
 };
@@ -785,40 +783,30 @@ template <int D>
 constexpr int attn_lds() {
   return 2 * Pitch<D>::stage(64) + 2048;  // two stages of 64 keys (or four waves' of 32), scales; then sums to be joined
 }
-// A workgroup's rows over its keys. SHARED: its four waves take RB x 32 rows each and share every stage of 64 keys; else all
+// A workgroup's rows over its keys. SHARED: its four waves take 32 rows each and share every stage of 64 keys; else all
 // of them take the same 32 rows, each every fourth stage of 32 keys, and their sums are joined in LDS.
-template <typename XT, int KV, int D, int NT, bool SHARED, int RB>
+template <typename XT, int KV, int D, int NT, bool SHARED>
 __device__ __forceinline__ void attend(const AttnArgs& a, const Place& p, uint8_t* lds) {
   constexpr int KEYS = SHARED ? 64 : 32, THREADS = SHARED ? 256 : 64, STAGE = Pitch<D>::stage(KEYS), SUMS = 2 * Pitch<D>::stage(64);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i32 = lane & 31, h = lane >> 5;
-  const int r = p.r0 + (SHARED ? RB * AT_ROWS * wave : 0) + i32;
-  Wave<KV, D, NT, KEYS / 32, RB> w;
+  const int r = p.r0 + (SHARED ? AT_ROWS * wave : 0) + i32;
+  Wave<KV, D, NT, KEYS / 32> w;
   Stage<KV, D, KEYS, THREADS> st;
   // of each source, the keys that any live row of the workgroup sees, and those that all of the wave's do
   Range range;
-  int all0[2], all1[2], lo[2][RB], hi[2][RB], tok[RB], head[RB];
-  uint32_t least[2] = {~0u, ~0u}, most[2] = {0, 0}, latest[2] = {0, 0}, soonest[2] = {~0u, ~0u};
-  bool live[RB];
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const Row row(a, p, r + AT_ROWS * rb);
-    tok[rb] = row.tok, head[rb] = row.h, live[rb] = row.live;
-    w.start(rb, (const XT*)a.q + (int64_t)(row.tok * a.H + row.h) * D);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      lo[i][rb] = row.lo[i], hi[i][rb] = row.hi[i];
-      if (row.live) {
-        least[i] = min(least[i], (uint32_t)row.lo[i]), latest[i] = max(latest[i], (uint32_t)row.lo[i]);
-        soonest[i] = min(soonest[i], (uint32_t)row.hi[i]), most[i] = max(most[i], (uint32_t)row.hi[i]);
-      }
-    }
-  }
+  const Row row(a, p, r);
+  const At at{row.tok, row.h, row.live};
+  w.start((const XT*)a.q + (int64_t)(row.tok * a.H + row.h) * D);
+  int all0[2], all1[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     range.from[i] = 0, range.to[i] = 0, all0[i] = 0, all1[i] = 0;
     if (p.with[i]) {
-      range.from[i] = (int)min(nsx_wave_min_u32(least[i]), 0x7fffffffu), range.to[i] = (int)nsx_wave_max_u32(most[i]);
-      all0[i] = (int)nsx_wave_max_u32(latest[i]), all1[i] = (int)min(nsx_wave_min_u32(soonest[i]), 0x7fffffffu);
+      const uint32_t lo = (uint32_t)row.lo[i], hi = (uint32_t)row.hi[i];
+      range.from[i] = (int)min(nsx_wave_min_u32(row.live ? lo : ~0u), 0x7fffffffu);
+      range.to[i] = (int)nsx_wave_max_u32(row.live ? hi : 0);
+      all0[i] = (int)nsx_wave_max_u32(row.live ? lo : 0);
+      all1[i] = (int)min(nsx_wave_min_u32(row.live ? hi : ~0u), 0x7fffffffu);
     }
   }
   if constexpr (SHARED) {
@@ -861,43 +849,29 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Place& p, uint8_
     else __builtin_amdgcn_wave_barrier();
     const bool o = i >= range.tiles[0];
     const int key0 = first_key(i);
-    int from[RB], to[RB];
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) from[rb] = o ? lo[1][rb] : lo[0][rb], to[rb] = o ? hi[1][rb] : hi[0][rb];
     const bool all = key0 >= (o ? all0[1] : all0[0]) && key0 + KEYS <= (o ? all1[1] : all1[0]);
-    w.step(kl, vl, sc, sc + KEYS, a.scale2, all, key0, from, to);
+    w.step(kl, vl, sc, sc + KEYS, a.scale2, all, key0, o ? row.lo[1] : row.lo[0], o ? row.hi[1] : row.hi[0]);
     buf ^= 1;
     if constexpr (!SHARED) __builtin_amdgcn_wave_barrier();
   }
   const End<XT, D> fin{a, p};
+  const bool mine = r < p.rows;
+  const uint64_t odd = __ballot(!w.finite() && mine && row.live);
+  uint32_t bad = (uint32_t)odd | (uint32_t)(odd >> 32);
+  w.l = other_half_sum(w.l);
   if constexpr (SHARED) {
+    if (mine && !(bad >> i32 & 1)) {
+      const float f = fin.factor(at, w.m, w.l, h == 0);
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      const At row{tok[rb], head[rb], live[rb]};
-      const bool mine = r + AT_ROWS * rb < p.rows;
-      const uint64_t odd = __ballot(!w.finite(rb) && mine && live[rb]);
-      uint32_t bad = (uint32_t)odd | (uint32_t)(odd >> 32);
-      w.l[rb] = other_half_sum(w.l[rb]);
-      if (mine && !(bad >> i32 & 1)) {
-        const float f = fin.factor(row, w.m[rb], w.l[rb], h == 0);
+      for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-        for (int blk = 0; blk < D / 32; ++blk)
-#pragma unroll
-          for (int e = 0; e < 16; e += 4) {
-            const f16v& y = w.acc[rb][blk];
-            const float x[4] = {y[e], y[e + 1], y[e + 2], y[e + 3]};
-            fin.store(row, 32 * blk + 2 * e + 4 * h, f, x);
-          }
-      }
-      for (; bad; bad &= bad - 1)
-        row_alone<XT, KV, D, KEYS>(a, p, range, p.r0 + AT_ROWS * (RB * wave + rb) + __builtin_ctz(bad));
+        for (int e = 0; e < 16; e += 4) {
+          const float x[4] = {w.acc[i][e], w.acc[i][e + 1], w.acc[i][e + 2], w.acc[i][e + 3]};
+          fin.store(at, 32 * i + 2 * e + 4 * h, f, x);
+        }
     }
+    for (; bad; bad &= bad - 1) row_alone<XT, KV, D, KEYS>(a, p, range, p.r0 + AT_ROWS * wave + __builtin_ctz(bad));
   } else {
-    const At row{tok[0], head[0], live[0]};
-    const bool mine = r < p.rows;
-    const uint64_t odd = __ballot(!w.finite(0) && mine && live[0]);
-    uint32_t bad = (uint32_t)odd | (uint32_t)(odd >> 32);
-    const float l = other_half_sum(w.l[0]), m = w.m[0];
     // the waves' sums, on the largest of their references
     constexpr int OP = D + 4;
     float* sums = (float*)lds;                         // [wave][row][OP]
@@ -905,7 +879,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Place& p, uint8_
     uint32_t* odds = (uint32_t*)(ml + AT_NW * AT_ROWS);
     static_assert(AT_NW * AT_ROWS * OP * 4 <= SUMS && AT_NW * (AT_ROWS * 8 + 4) <= 2048, "LDS");
     __syncthreads();
-    if (h == 0) ml[wave * AT_ROWS + i32] = float2{m, l};
+    if (h == 0) ml[wave * AT_ROWS + i32] = float2{w.m, w.l};
     if (lane == 0) odds[wave] = bad;
     __syncthreads();
     bad = odds[0] | odds[1] | odds[2] | odds[3];
@@ -917,18 +891,18 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Place& p, uint8_
       const float2 x = ml[k * AT_ROWS + i32];
       L = fmaf(x.y, __builtin_amdgcn_exp2f(x.x - M), L);
     }
-    const float f = __builtin_amdgcn_exp2f(m - M);
+    const float f = __builtin_amdgcn_exp2f(w.m - M);
 #pragma unroll
     for (int blk = 0; blk < D / 32; ++blk)
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
-        const f16v& y = w.acc[0][blk];
+        const f16v& y = w.acc[blk];
         *(v4f*)(sums + (wave * AT_ROWS + i32) * OP + 32 * blk + 2 * e + 4 * h) = v4f{y[e] * f, y[e + 1] * f, y[e + 2] * f, y[e + 3] * f};
       }
     __syncthreads();
     // a wave a quarter of the dimensions of every row, two lanes a row
     if (mine && !(bad >> i32 & 1)) {
-      const float y = fin.factor(row, M, L, threadIdx.x < 32);
+      const float y = fin.factor(at, M, L, threadIdx.x < 32);
 #pragma unroll
       for (int e = 0; e < D / 8; e += 4) {
         const int d = D / 4 * wave + D / 8 * h + e;
@@ -937,7 +911,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Place& p, uint8_
         for (int k = 0; k < 4; ++k)
           x[k] = (sums[i32 * OP + d + k] + sums[(AT_ROWS + i32) * OP + d + k]) +
                  (sums[(2 * AT_ROWS + i32) * OP + d + k] + sums[(3 * AT_ROWS + i32) * OP + d + k]);
-        fin.store(row, d, y, x);
+        fin.store(at, d, y, x);
       }
     }
     for (int k = 0; bad; bad &= bad - 1, ++k)
@@ -950,13 +924,7 @@ constexpr int attn_terms() {
   // bf16 rows and codes of 8 bits are bf16's own; queries and weights are as many bf16 terms as their type has bytes of bits
   return std::is_same_v<XT, float> ? 3 : std::is_same_v<XT, Half> ? 2 : 1;
 }
-// Whether a kernel has waves of 64 rows: where their registers leave two waves to a SIMD.
-template <typename XT, int D>
-constexpr bool attn_wide() {
-  return attn_terms<XT>() == 1 && D == 64;
-}
-
-template <typename XT, int KV, int D, int RB>
+template <typename XT, int KV, int D>
 __global__ __launch_bounds__(256, (attn_terms<XT>() == 3 && D == 128 ? 1 : 2)) void attn_kernel(AttnArgs a) {
   extern __shared__ __align__(16) uint8_t lds[];
   constexpr int NT = attn_terms<XT>();
@@ -987,8 +955,8 @@ __global__ __launch_bounds__(256, (attn_terms<XT>() == 3 && D == 128 ? 1 : 2)) v
     p.src[i].ks = kv.ks + (KV == NSX_DT_BF16 ? 0 : base);
     p.src[i].vs = kv.vs + (KV == NSX_DT_BF16 ? 0 : base);
   }
-  if (cut.rows == AT_ROWS) attend<XT, KV, D, NT, false, 1>(a, p, lds);
-  else attend<XT, KV, D, NT, true, RB>(a, p, lds);
+  if (cut.rows == AT_ROWS) attend<XT, KV, D, NT, false>(a, p, lds);
+  else attend<XT, KV, D, NT, true>(a, p, lds);
 }
 
 // The splits' sums of a (token, head) and its sink: a wave each, D / 4 lanes a split.
@@ -1046,19 +1014,20 @@ struct Plan {
   int64_t pblocks, oblocks;
   int splits;
 };
-Plan attn_plan(int G, int rep, int64_t B, int64_t n, int64_t ctx_max, int64_t prefix_max, int window, bool wide, int occ) {
+Plan attn_plan(int G, int rep, int64_t B, int64_t n, int64_t ctx_max, int64_t prefix_max, int window, int occ) {
   Plan p{};
   const int64_t prows = B * n * rep, orows = n * rep;
   const int64_t pk = window > 0 ? std::min<int64_t>(prefix_max, window + n) : prefix_max;
   const int64_t ok = window > 0 ? std::min<int64_t>(ctx_max, window + n) : ctx_max;
   // pieces of 32 rows x 32 keys, and how many of them a wave takes where the chip's share them
-  const int64_t slots = 256 * occ, pw = G * nsx_cdiv(prows, AT_ROWS) * nsx_cdiv(pk, 32), ow = B * G * nsx_cdiv(orows, AT_ROWS) * nsx_cdiv(ok, 32);
+  const int64_t pw = G * nsx_cdiv(prows, AT_ROWS) * nsx_cdiv(pk, 32), ow = B * G * nsx_cdiv(orows, AT_ROWS) * nsx_cdiv(ok, 32);
   const int64_t each = nsx_cdiv(pw + ow, 2048);
   const bool many = each > 20;
+  const int64_t slots = 256 * (many ? occ : std::min(occ, 2));
   auto cut = [&](int64_t rows, int64_t keys, int64_t units, int64_t room) {
     AttnArgs::Cut c;
     const int waves = rows > 2 * AT_ROWS && many ? 1 : AT_NW;  // that share a row's keys
-    c.rows = waves > 1 ? AT_ROWS : wide && rows > AT_NW * AT_ROWS ? 2 * AT_NW * AT_ROWS : AT_NW * AT_ROWS;
+    c.rows = waves > 1 ? AT_ROWS : AT_NW * AT_ROWS;
     c.tiles = (int)nsx_cdiv(rows, c.rows);
     const int64_t most = nsx_cdiv(nsx_cdiv(keys, 32), 3 * waves);
     c.splits = (int)std::max<int64_t>(1, std::min<int64_t>({AT_MAX_SPLIT / 2, most, room / (units * c.tiles)}));
@@ -1078,8 +1047,7 @@ Plan attn_plan(int G, int rep, int64_t B, int64_t n, int64_t ctx_max, int64_t pr
   return p;
 }
 // Workgroups of a kernel that a CU holds.
-int attn_occ(int x_dtype, int head_dim) { return x_dtype == NSX_DT_F32 && head_dim == 128 ? 1 : 2; }
-bool attn_wide(int x_dtype, int head_dim) { return x_dtype == NSX_DT_BF16 && head_dim == 64; }
+int attn_occ(int x_dtype, int head_dim) { return x_dtype == NSX_DT_F32 && head_dim == 128 ? 1 : x_dtype == NSX_DT_BF16 && head_dim == 64 ? 3 : 2; }
 
 // ---------------------------------------------------------------------------
 
@@ -1201,7 +1169,7 @@ extern "C" int64_t nsx_batch_attn_workspace_bytes(int n_head, int n_kv, int head
     return -1;
   int splits = 1;  // (whatever the type)
   for (const int dt : {NSX_DT_F32, NSX_DT_F16, NSX_DT_BF16})
-    splits = std::max(splits, attn_plan(n_kv, n_head / n_kv, n_seq, n, ctx_max, prefix_max, window, attn_wide(dt, head_dim), attn_occ(dt, head_dim)).splits);
+    splits = std::max(splits, attn_plan(n_kv, n_head / n_kv, n_seq, n, ctx_max, prefix_max, window, attn_occ(dt, head_dim)).splits);
   return splits > 1 ? n_seq * n * n_head * splits * (head_dim + 2) * 4 : 0;
 }
 
@@ -1227,7 +1195,7 @@ extern "C" int nsx_batch_attn(const void* q, int x_dtype, const nsx_kv_rows* kv,
   NSX_REQUIRE((workspace || !need) && aligned16(workspace) && workspace_bytes >= need, NSX_EINVAL,
               "workspace of %lld bytes, %lld needed, 16-byte aligned", (long long)workspace_bytes, (long long)need);
   const Plan plan = attn_plan(n_kv, n_head / n_kv, kv->n_seq, n, kv->ctx_max, prefix ? prefix->ctx_max : 0, window,
-                              attn_wide(x_dtype, head_dim), attn_occ(x_dtype, head_dim));
+                              attn_occ(x_dtype, head_dim));
   NSX_REQUIRE(plan.pblocks + plan.oblocks < (1ll << 24) && kv->n_seq * n * n_head < (1ll << 26), NSX_EINVAL,
               "%lld tokens of %d heads: too many for one call", (long long)(kv->n_seq * n), n_head);
   const AttnArgs a{q, kv_rows(kv), prefix ? kv_rows(prefix) : KvRows{}, counts, sinks, n_head, n_kv, n_head / n_kv, window, n,
@@ -1235,9 +1203,7 @@ extern "C" int nsx_batch_attn(const void* q, int x_dtype, const nsx_kv_rows* kv,
   return with_types(x_dtype, kv_type, head_dim, [&](auto x, auto t, auto d) {
     using XT = decltype(x);
     constexpr int LDS = attn_lds<d()>();
-    auto* kernel = attn_kernel<XT, t(), d(), 1>;
-    if constexpr (attn_wide<XT, d()>())
-      if (std::max(plan.pre.rows, plan.own.rows) == 2 * AT_NW * AT_ROWS) kernel = attn_kernel<XT, t(), d(), 2>;
+    auto* kernel = attn_kernel<XT, t(), d()>;
     if (const int rc = nsx_allow_lds((const void*)kernel, LDS)) return rc;
     if (const int rc = nsx_launch(kernel, dim3((unsigned)(plan.pblocks + plan.oblocks)), dim3(256), LDS, (hipStream_t)stream, a))
       return rc;
