@@ -976,21 +976,29 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
     m = x.x;
     l = x.y;
   }
-  const float sink = a.sinks ? a.sinks[h] * LOG2E : LOWEST;
-  float M = fmaxf(m, sink);
+  const float* part = a.part + row * a.splits * D + 4 * (lane % LPR);
+  constexpr int AHEAD = 4;  // rounds of loads in one go, before the weights are known
+  v4f y[AHEAD];
+  auto load = [&](int s0) {
 #pragma unroll
-  for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    for (int i = 0; i < AHEAD; ++i) y[i] = *(const v4f*)(part + (int64_t)min(s0 + AT_ONCE * i + lane / LPR, a.splits - 1) * D);
+  };
+  load(0);
+  const float sink = a.sinks ? a.sinks[h] * LOG2E : LOWEST;
+  float M = nsx_row_fmax(fmaxf(m, sink));
+  M = fmaxf(M, __shfl_xor(M, 16, 64));
+  M = other_half_max(M);
   const float w = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - M);
   const float Z = nsx_wave_sum(w == 0.f ? 0.f : w * l) + (a.sinks ? __builtin_amdgcn_exp2f(sink - M) : 0.f);
-  const float* part = a.part + row * a.splits * D + 4 * (lane % LPR);
   float x[4] = {};
-  for (int s0 = 0; s0 < a.splits; s0 += AT_ONCE) {
-    const int s = s0 + lane / LPR;
-    const float ws = __shfl(w, min(s, 63), 64);
-    if (s < a.splits && ws != 0.f) {
-      const v4f y = *(const v4f*)(part + (int64_t)s * D);
+  for (int s0 = 0; s0 < a.splits; s0 += AHEAD * AT_ONCE) {
+    if (s0) load(s0);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) x[k] = fmaf(ws, y[k], x[k]);
+    for (int i = 0; i < AHEAD; ++i) {
+      const int s = s0 + AT_ONCE * i + lane / LPR;
+      const float ws = __shfl(w, min(s, 63), 64);  // (0 in lanes past the last split)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = ws != 0.f ? fmaf(ws, y[i][k], x[k]) : x[k];
     }
   }
 #pragma unroll
@@ -999,10 +1007,9 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
     for (int k = 0; k < 4; ++k) x[k] += __shfl_xor(x[k], o, 64);
   const float f = !live || Z == 0.f ? 0.f : 1.f / Z;
   if (lane < LPR) {
-    float y[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) y[k] = f == 0.f ? 0.f : x[k] * f;
-    store4((XT*)a.out + row * D + 4 * lane, y);
+    for (int k = 0; k < 4; ++k) x[k] = f == 0.f ? 0.f : x[k] * f;
+    store4((XT*)a.out + row * D + 4 * lane, x);
   }
 }
 
