@@ -549,8 +549,8 @@ int nsx_batch_attn(const void *q, int x_dtype, const nsx_kv_rows *kv, const nsx_
  * times their total. temperature <= 0: the largest logit, the lowest index of
  * equals. A NaN logit counts as -infinity; of +infinity in a row, its tokens
  * share the row's whole weight; a row without any weight gives -1.
- * Weights are computed in 64 bits and summed as whole multiples of 2^-(62 -
- * ceil(log2 vocab)) of the largest, so that no order of summing matters.
+ * Weights are computed in 64 bits and summed as whole multiples of 2^-min(51,
+ * 62 - ceil(log2 vocab)) of the largest, so that no order of summing matters.
  * Settings: one value for all rows, or with the array not NULL (device) one
  * each. uniforms (device fp32, in [0, 1)) may be NULL if temperatures is NULL
  * and temperature 0. vocab up to 4194304, batch below 65536. */

@@ -25,12 +25,15 @@ namespace {
 constexpr int THREADS = 512;
 constexpr int VEC = 8;                  // logits of a thread, consecutive
 constexpr int PART = THREADS * VEC;     // logits of a part
-constexpr int MAX_PARTS = 1 + (1 << 22) / PART;
+constexpr int INDEX = 22;              // bits of an index
+constexpr uint32_t LAST_INDEX = (1u << INDEX) - 1;
+constexpr int MAX_PARTS = 1 + (1 << INDEX) / PART;
 constexpr int BINS = 1024;              // 64 octaves of 16: no weight lies lower
 constexpr int LIST = 8192;             // listed tokens; a row with more in its last bins is read again instead
 constexpr int HELD = 4;                 // listed tokens that a thread holds in registers
 constexpr int FEW = HELD * THREADS / 2;
-constexpr int GRID = 512;               // workgroups of a pass over all rows: two on each of 256 CUs
+constexpr int RANK = THREADS / 4;       // listed tokens up to which each is compared with each
+constexpr int GRID = 1024;               // workgroups of a pass over all rows: two on each of 256 CUs
 
 struct SampleArgs {
   const void* logits;
@@ -61,10 +64,12 @@ struct Row {
   double T, top_p, min_p, scale2, least, unit;
   int64_t top_k;
   float M = 0.f, scale32 = 0.f;
+  bool infinite = false;  // the largest logit is: its equals count as 0 from then on, the others as -infinity
   __device__ __forceinline__ Row(const SampleArgs& a, int64_t row)
       : p((const LT*)a.logits + row * a.row_stride), V(a.V), off((int)((uintptr_t)p / sizeof(LT) % VEC)) {
     T = a.temperatures ? (double)a.temperatures[row] : a.temperature;
     top_p = a.top_ps ? (double)a.top_ps[row] : a.top_p;
+    if (T > 0.0) T = fmin(fmax(T, 1e-30), 1e30);  // (a row's own is not looked at before)
     min_p = a.min_ps ? (double)a.min_ps[row] : a.min_p;
     min_p = min_p > 0.0 ? fmin(min_p, 1.0) : 0.0;
     top_k = a.top_ks ? a.top_ks[row] : a.top_k;
@@ -84,17 +89,21 @@ struct Row {
   // weight is computed.
   __device__ __forceinline__ bool few() const { return top_k && top_k <= FEW; }
   __device__ __forceinline__ void largest(uint64_t order) {
-    const uint32_t u = (uint32_t)(order >> 32);
-    M = __builtin_bit_cast(float, u ^ ((int32_t)u < 0 ? 0x80000000u : 0xffffffffu));
+    const uint32_t u = (uint32_t)(order >> INDEX) << SAME;
+    const uint32_t bits = (u ^ ((int32_t)u < 0 ? 0x80000000u : 0xffffffffu)) & (0xffffffffu << SAME);
+    M = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(bits));
+    infinite = M == INFINITY;
+    if (infinite) M = 0.f;
     scale32 = (float)fmin(16.0 * scale2, 3e38);  // (times a difference of zero: zero)
   }
   static __device__ __forceinline__ float value(LT x) {
     float f;
     if constexpr (std::is_same_v<LT, uint16_t>) f = nsx_bf2f(x);
     else f = (float)x;
-    return f == f ? f + 0.f : -INFINITY;  // (no -0)
+    return fmaxf(f + 0.f, -INFINITY);  // (no -0, no NaN)
   }
-  __device__ __forceinline__ float at(int64_t i) const { return value(p[i]); }
+  __device__ __forceinline__ float seen(float x) const { return !infinite ? x : x == INFINITY ? 0.f : -INFINITY; }
+  __device__ __forceinline__ float at(int64_t i) const { return seen(value(p[i])); }
   // The elements from place v (a multiple of VEC) of the row's parts on, element k being token v - off + k; -infinity where
   // there is none. Loaded as they lie, a vector, or one by one at the row's ends.
   struct alignas(16) Raw {
@@ -119,25 +128,27 @@ struct Row {
 #pragma unroll
       for (int k = 0; k < VEC; ++k) x[k] = i + k >= 0 && i + k < V ? x[k] : -INFINITY;
     }
+    if (infinite) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) x[k] = seen(x[k]);
+    }
   }
   __device__ __forceinline__ void run(int64_t v, float (&x)[VEC]) const { values(v, load(v), x); }
+  // (without the bits that are the same in all: few digits tell two orders apart)
+  static constexpr int SAME = std::is_same_v<LT, float> ? 0 : std::is_same_v<LT, uint16_t> ? 16 : 13;
   static __device__ __forceinline__ uint64_t order(float x, int64_t i) {
     const uint32_t u = __builtin_bit_cast(uint32_t, x);
-    return (uint64_t)(u ^ ((int32_t)u < 0 ? 0xffffffffu : 0x80000000u)) << 32 | (uint32_t)~(uint32_t)i;
+    return (uint64_t)((u ^ ((int32_t)u < 0 ? 0xffffffffu : 0x80000000u)) >> SAME) << INDEX | (~(uint32_t)i & LAST_INDEX);
   }
-  __device__ __forceinline__ double real(float x, const Pow2& tab) const {
-    const double d = (double)x - (double)M;
-    if (M == INFINITY) return x == M ? 1.0 : 0.0;
-    return d < least ? 0.0 : nsx_pow2(fmax(d, least), scale2, tab);
+  __device__ __forceinline__ double real(float x, const Pow2& tab) const {  // (2^-1000 for -infinity)
+    return nsx_pow2(fmax((double)x - (double)M, least), scale2, tab);
   }
-  __device__ __forceinline__ uint64_t whole(double w) const {  // in units, to the nearest
-    const double y = rint(w * unit), hi = floor(y * 0x1p-32);
-    return (uint64_t)(uint32_t)hi << 32 | (uint32_t)fma(hi, -0x1p32, y);
+  __device__ __forceinline__ uint64_t whole(double w) const {  // in units, to the nearest: the last bits of a sum with 2^52
+    return __builtin_bit_cast(uint64_t, fma(w, unit, 0x1p52)) & 0xfffffffffffffull;
   }
   __device__ __forceinline__ uint64_t weight(float x, const Pow2& tab) const { return whole(real(x, tab)); }
   // How many 16ths of an octave below M a logit lies: 32-bit operations that never fall as x does; and the bin that it is in.
   __device__ __forceinline__ float depth(float x) const {
-    if (M == INFINITY) return x == M ? 0.f : INFINITY;
     return (M - x) * scale32;
   }
   static __device__ __forceinline__ int bin_at(float depth) { return depth < BINS - 1 ? (int)depth : BINS - 1; }
@@ -243,16 +254,29 @@ __global__ __launch_bounds__(THREADS) void best_kernel(SampleArgs a) {
       a.many[row * BINS + i] = 0;
       if (i == 0) a.listed[row] = 0;
     }
+  // (a thread keeps the eight logits among which its largest is, and looks for that one's place behind the last)
+  typename Row<LT>::Raw next = r.load((int64_t)blockIdx.x * PART + threadIdx.x * VEC), held = next;
+  float most = -INFINITY;
+  int64_t from = 0;
+  for (int part = blockIdx.x; part < a.parts; part += gridDim.x) {
+    const int64_t v = (int64_t)part * PART + threadIdx.x * VEC;
+    const typename Row<LT>::Raw now = next;
+    if (part + (int)gridDim.x < a.parts) next = r.load(v + (int64_t)gridDim.x * PART);
+    float x[VEC], top = most;
+    r.values(v, now, x);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) top = fmaxf(top, x[k]);
+    if (top > most) most = top, from = v, held = now;
+  }
   uint64_t best = 0;
-  each_part(a, r, [&](int, int64_t i, const float (&x)[VEC]) {
-    // (of its own logits a thread looks for the largest first: the order of one token, not of eight)
-    float top = x[0];
+  if (most > -INFINITY) {
+    float x[VEC];
+    r.values(from, held, x);
     int at = 0;
 #pragma unroll
-    for (int k = 1; k < VEC; ++k) at = x[k] > top ? k : at, top = fmaxf(top, x[k]);
-    i += at;
-    best = max64(best, i < 0 ? Row<LT>::order(top, 0) : i < a.V ? Row<LT>::order(top, i) : 0);
-  });
+    for (int k = 1; k < VEC; ++k) at = x[k] > x[0] ? (x[0] = x[k], k) : at;
+    best = Row<LT>::order(most, from - r.off + at);
+  }
   best = block_max(best, s);
   if (threadIdx.x == 0) a.best[row * a.groups + blockIdx.x] = best;
 }
@@ -381,26 +405,23 @@ __global__ __launch_bounds__(THREADS) void sums_kernel(SampleArgs a) {
   const float deepest = e.last() < BINS - 1 ? (float)(e.last() + 1) : INFINITY;  // (one look tells most tokens from those kept)
   each_part(a, r, [&](int part, int64_t i, const float (&x)[VEC]) {
     uint64_t sum = 0;
-    if (!cut) {
+    bool sure[VEC], any = false;
 #pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const float depth = r.depth(x[k]);
+      const int b = Row<LT>::bin_at(depth);
+      sure[k] = depth < deepest && e.sure(b);
+      any |= sure[k];
+      if (depth < deepest && e.open(b)) {
+        const uint32_t at = atomicAdd(&n, 1u);
+        if (at < OPEN) list[at] = (uint32_t)(i + k);
+      }
+    }
+    if (__any(any)) {
+#pragma unroll 4
       for (int k = 0; k < VEC; ++k) {
         const double w = r.real(x[k], tab);
-        sum += w < r.min_p ? 0 : r.whole(w);
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        const float depth = r.depth(x[k]);
-        if (depth < deepest) {
-          const int b = Row<LT>::bin_at(depth);
-          if (e.sure(b)) {
-            const double w = r.real(x[k], tab);
-            sum += w < r.min_p ? 0 : r.whole(w);
-          } else if (e.open(b)) {
-            const uint32_t at = atomicAdd(&n, 1u);
-            if (at < OPEN) list[at] = (uint32_t)(i + k);
-          }
-        }
+        sum += sure[k] && !(w < r.min_p) ? r.whole(w) : 0;
       }
     }
     if (__any(sum != 0)) {
@@ -421,12 +442,16 @@ __global__ __launch_bounds__(THREADS) void sums_kernel(SampleArgs a) {
 
 // Among tokens, the order of the one with which their sum from the highest on reaches `want`; 0 where all of them do not.
 // each(f): f(order, weight) for every token, by whichever threads. By digits of 10 bits of what an order lies above the lowest,
-// from the highest bit that one has, until the digits are all or one token is left.
+// from the highest bit that one has, until the digits are all or few tokens are left.
 constexpr int DIGIT = 10;
 struct Pick {
-  uint64_t s[NW], t[NW], mass[1 << DIGIT], order, above;
-  uint32_t many[1 << DIGIT];
+  uint64_t s[NW], t[NW], mass[1 << DIGIT], above, order[64], weight[64];
+  uint32_t many[1 << DIGIT], n;
   int digit;
+};
+struct Rank {
+  uint64_t order[RANK], k_order[RANK], weight[RANK], before[RANK];
+  uint32_t many[RANK];
 };
 template <typename Each>
 __device__ __forceinline__ uint64_t pick_order(Pick& p, uint64_t want, Each each) {
@@ -435,7 +460,7 @@ __device__ __forceinline__ uint64_t pick_order(Pick& p, uint64_t want, Each each
   hi = wave_max64(hi), lo = wave_max64(lo);
   if ((threadIdx.x & 63) == 0) p.s[threadIdx.x >> 6] = hi, p.t[threadIdx.x >> 6] = lo;
   for (int i = threadIdx.x; i < 1 << DIGIT; i += THREADS) p.mass[i] = 0, p.many[i] = 0;
-  if (threadIdx.x == 0) p.digit = -1;
+  if (threadIdx.x == 0) p.digit = -1, p.n = 0;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < NW; ++i) hi = max64(hi, p.s[i]), lo = max64(lo, p.t[i]);
@@ -476,12 +501,18 @@ __device__ __forceinline__ uint64_t pick_order(Pick& p, uint64_t want, Each each
     above = p.above;
     const uint32_t n = p.many[d];
     lo += (uint64_t)d << shift;
-    if (n == 1) {
-      each([&](uint64_t o, uint64_t) {
-        if (o >= lo && (o - lo) >> shift == 0) p.order = o;
+    if (n <= 64) {  // few: each with each, a lane one token, the same in all waves
+      each([&](uint64_t o, uint64_t w) {
+        if (o < lo || (o - lo) >> shift) return;
+        const uint32_t i = atomicAdd(&p.n, 1u);
+        p.order[i] = o, p.weight[i] = w;
       });
       __syncthreads();
-      return p.order;
+      const uint32_t lane = threadIdx.x & 63;
+      const uint64_t o = lane < n ? p.order[lane] : 0, w = lane < n ? p.weight[lane] : 0;
+      uint64_t run = above;
+      for (uint32_t j = 0; j < n; ++j) run += p.order[j] > o ? p.weight[j] : 0;
+      return lane64(o, __builtin_amdgcn_readfirstlane(__ffsll(__ballot(w && run < want && run + w >= want)) - 1));
     }
     if (shift == 0) return lo;
     __syncthreads();
@@ -494,6 +525,7 @@ __device__ __forceinline__ uint64_t pick_order(Pick& p, uint64_t want, Each each
 template <typename LT>
 __global__ __launch_bounds__(THREADS) void draw_kernel(SampleArgs a) {
   __shared__ Pick p;
+  __shared__ Rank rank;
   __shared__ Ends shared;
   __shared__ Pow2 tab;
   __shared__ uint64_t sums[MAX_PARTS];
@@ -515,7 +547,7 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(SampleArgs a) {
   const uint64_t best = block_max(known.best, p.s);
   r.largest(best);
   if (!r.drawn()) {
-    if (threadIdx.x == 0) a.token[row] = r.M > -INFINITY ? (int32_t)~(uint32_t)best : -1;
+    if (threadIdx.x == 0) a.token[row] = r.M > -INFINITY ? (int32_t)(~(uint32_t)best & LAST_INDEX) : -1;
     return;
   }
   Ends e{BINS, BINS, BINS, 0, 0, 0, 0};
@@ -555,32 +587,75 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(SampleArgs a) {
       }
     };
     uint64_t whole = e.all;
-    if (e.kbin < BINS) {
-      // (of the few: all of them are listed, of others those of the last bin)
-      const int from = r.few() ? 0 : e.kbin;
-      last = pick_order(p, (uint64_t)r.top_k - e.before_k, [&](auto f) {
-        tokens([&](uint64_t o, uint64_t, int b, bool) {
-          if (b >= from && b <= e.kbin) f(o, 1);
+    // (of the few all are listed, of others those of the last bin)
+    const int from = r.few() ? 0 : e.kbin;
+    if (n <= RANK) {
+      const int i = threadIdx.x % RANK;
+      const bool mine = threadIdx.x < RANK && hw[0];
+      const bool in_k = mine && e.kbin < BINS && hb[0] >= from && hb[0] <= e.kbin;
+      const bool in_p = mine && hb[0] >= e.plo && hb[0] <= e.phi;
+      if (threadIdx.x < RANK) {
+        rank.order[i] = ho[0];
+        rank.k_order[i] = in_k ? ho[0] : 0;
+        rank.weight[i] = in_p ? hw[0] : 0;
+        rank.before[i] = 0;
+        rank.many[i] = 0;
+      }
+      __syncthreads();
+      const uint64_t o = rank.order[i];
+      uint64_t before = 0;
+      uint32_t more = 0;
+      if (o) {
+        constexpr int SHARE = RANK * RANK / THREADS;
+        const int from_j = threadIdx.x / RANK * SHARE;
+#pragma unroll 8
+        for (int j = from_j; j < from_j + SHARE; ++j) {  // (behind the last: order 0)
+          more += rank.k_order[j] > o;
+          before += rank.order[j] > o ? rank.weight[j] : 0;
+        }
+        if (more) atomicAdd(&rank.many[i], more);
+        if (before) atomicAdd((unsigned long long*)&rank.before[i], (unsigned long long)before);
+      }
+      __syncthreads();
+      more = rank.many[i], before = rank.before[i];
+      bool kept = mine && (!in_k || e.before_k + more < r.top_k);
+      if (e.kbin < BINS) {
+        block_scan(in_k && kept ? hw[0] : 0, p.s, whole);
+        whole += e.above_k;
+      }
+      if (r.top_p < 1.0) kept = kept && (!in_p || e.above_p + before < r.target(whole));
+      last = block_max(kept ? ~ho[0] : 0, p.s);
+      last = last ? ~last : 0;
+      if (kept && hk[0])
+        atomicAdd((unsigned long long*)&sums[((~(uint32_t)ho[0] & LAST_INDEX) + r.off) / PART], (unsigned long long)hw[0]);
+      __syncthreads();
+    } else {
+      if (e.kbin < BINS) {
+        last = pick_order(p, (uint64_t)r.top_k - e.before_k, [&](auto f) {
+          tokens([&](uint64_t o, uint64_t, int b, bool) {
+            if (b >= from && b <= e.kbin) f(o, 1);
+          });
         });
-      });
-      uint64_t in = 0;
-      tokens([&](uint64_t o, uint64_t w, int b, bool) {
-        if (b >= from && b <= e.kbin && o >= last) in += w;
-      });
-      block_scan(in, p.s, whole);
-      whole += e.above_k;
-    }
-    if (r.top_p < 1.0) {
-      last = max64(last, pick_order(p, r.target(whole) - e.above_p, [&](auto f) {
+        uint64_t in = 0;
         tokens([&](uint64_t o, uint64_t w, int b, bool) {
-          if (b >= e.plo && b <= e.phi && o >= last) f(o, w);
+          if (b >= from && b <= e.kbin && o >= last) in += w;
         });
-      }));
+        block_scan(in, p.s, whole);
+        whole += e.above_k;
+      }
+      if (r.top_p < 1.0) {
+        last = max64(last, pick_order(p, r.target(whole) - e.above_p, [&](auto f) {
+          tokens([&](uint64_t o, uint64_t w, int b, bool) {
+            if (b >= e.plo && b <= e.phi && o >= last) f(o, w);
+          });
+        }));
+      }
+      tokens([&](uint64_t o, uint64_t w, int, bool keep) {
+        if (o >= last && keep)
+          atomicAdd((unsigned long long*)&sums[((~(uint32_t)o & LAST_INDEX) + r.off) / PART], (unsigned long long)w);
+      });
+      __syncthreads();
     }
-    tokens([&](uint64_t o, uint64_t w, int, bool keep) {
-      if (o >= last && keep) atomicAdd((unsigned long long*)&sums[((uint32_t)~(uint32_t)o + r.off) / PART], (unsigned long long)w);
-    });
-    __syncthreads();
   }
   // the part in which the random number falls
   constexpr int PER = (MAX_PARTS + THREADS - 1) / THREADS;
@@ -611,8 +686,11 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(SampleArgs a) {
   sum = 0;
 #pragma unroll
   for (int k = 0; k < VEC; ++k) {
-    const double y = r.real(x[k], tab);
-    w[k] = y < r.min_p || (cut && Row<LT>::order(x[k], v - r.off + k) < last) ? 0 : r.whole(y);
+    w[k] = 0;
+    if (Row<LT>::order(x[k], v - r.off + k) >= last) {  // (of a row cut short, few waves have one)
+      const double y = r.real(x[k], tab);
+      w[k] = y < r.min_p ? 0 : r.whole(y);
+    }
     sum += w[k];
   }
   run = p.above;
@@ -641,7 +719,7 @@ int sample_launch(const SampleArgs& a, int64_t batch, bool cut, bool greedy, hip
 }  // namespace
 
 extern "C" int64_t nsx_sample_workspace_bytes(int64_t batch, int64_t vocab) {
-  if (batch <= 0 || vocab <= 0 || vocab > (1 << 22)) return -1;
+  if (batch <= 0 || vocab <= 0 || vocab > (1 << INDEX)) return -1;
   return batch * ((int64_t)parts_of(vocab) * 16 + BINS * 12 + LIST * 4) + up16(batch * 4);
 }
 
@@ -650,7 +728,7 @@ extern "C" int nsx_sample(const void* logits, int logits_dtype, int64_t row_stri
                           int64_t workspace_bytes, void* stream) {
   NSX_REQUIRE(logits_dtype == NSX_DT_F32 || logits_dtype == NSX_DT_F16 || logits_dtype == NSX_DT_BF16, NSX_ETYPE,
               "logits element type %d", logits_dtype);
-  NSX_REQUIRE(batch >= 0 && batch < 65536 && vocab > 0 && vocab <= (1 << 22), NSX_EINVAL,
+  NSX_REQUIRE(batch >= 0 && batch < 65536 && vocab > 0 && vocab <= (1 << INDEX), NSX_EINVAL,
               "%lld rows of %lld logits (fewer than 65536, 1 to 4194304)", (long long)batch, (long long)vocab);
   NSX_REQUIRE(row_stride >= vocab, NSX_EINVAL, "rows %lld elements apart for %lld logits", (long long)row_stride,
               (long long)vocab);
@@ -667,8 +745,9 @@ extern "C" int nsx_sample(const void* logits, int logits_dtype, int64_t row_stri
   const int64_t need = nsx_sample_workspace_bytes(batch, vocab);
   NSX_REQUIRE(workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0, NSX_EINVAL,
               "workspace of %lld bytes, %lld needed, 16-byte aligned", (long long)workspace_bytes, (long long)need);
-  int bits = 62;
+  int bits = 62;  // (sums below 2^63; a weight below 2^52)
   while (bits > 0 && (1ll << (62 - bits)) < vocab) --bits;
+  bits = std::min(bits, 51);
   const bool cut = s.top_ks || s.top_ps || s.top_k > 0 || s.top_p < 1.0, greedy = !s.temperatures && s.temperature == 0.0;
   const int parts = parts_of(vocab);
   uint64_t *best = (uint64_t*)workspace, *sums = best + batch * parts, *mass = sums + batch * parts;

@@ -112,7 +112,8 @@ def rounding(want: torch.Tensor, t: torch.dtype) -> torch.Tensor:
 
 
 def sample_exact(logits, u, T, top_k, top_p, min_p) -> list[int]:
-    """Row by row: weights in 64 bits, summed as whole multiples of 2^-(62 - ceil(log2 vocab)) of the largest."""
+    """Row by row: weights in 64 bits, summed as whole multiples of 2^-min(51, 62 - ceil(log2 vocab)) of the
+    largest."""
     got = []
     for r in range(logits.shape[0]):
         x = logits[r].double().cpu()
@@ -125,7 +126,7 @@ def sample_exact(logits, u, T, top_k, top_p, min_p) -> list[int]:
             got.append(int((x == top).nonzero()[0]))
             continue
         real = ((x == top).double() if top == math.inf else torch.exp((x - top) / T[r])).tolist()
-        unit = 2.0 ** (62 - (V - 1).bit_length())
+        unit = 2.0 ** min(51, 62 - (V - 1).bit_length())
         w = [round(a * unit) for a in real]
         x = x.tolist()
         order = sorted(range(V), key=lambda i: (-x[i], i))
