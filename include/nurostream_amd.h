@@ -521,7 +521,7 @@ int nsx_append_qkv(const void *qkv, int x_dtype, const float *q_bias, const floa
 int nsx_store_rows(const void *k, const void *v, int x_dtype, int64_t n, const int32_t *start, int64_t start0,
                    int n_kv, int head_dim, const nsx_kv_rows *kv, int kv_type, void *stream);
 /* The values of those rows, as x_dtype; rows outside 0 .. ctx_max - 1 give
- * zeros. */
+ * zeros. k and v do not overlap. */
 int nsx_load_rows(const nsx_kv_rows *kv, int kv_type, int n_kv, int head_dim, const int32_t *start, int64_t start0,
                   int64_t n, void *k, void *v, int x_dtype, void *stream);
 /* Attention of the tokens that nsx_append_qkv wrote rows for: token j of
@@ -533,8 +533,8 @@ int nsx_load_rows(const nsx_kv_rows *kv, int kv_type, int n_kv, int head_dim, co
  * meet weights of all 24 bits, fp16 ones of 16, bf16 ones of 8. Rows past the
  * ones seen take no part, whatever they hold. Tokens from counts[b] on, and
  * tokens that see nothing, give zeros. The rows, q, out and the workspace are
- * 16-byte aligned; the workspace is scratch of the call (NULL where its bytes
- * are 0). */
+ * 16-byte aligned, and out does not overlap q; the workspace is scratch of the
+ * call (NULL where its bytes are 0). */
 int64_t nsx_batch_attn_workspace_bytes(int n_head, int n_kv, int head_dim, int64_t n_seq, int64_t n,
                                        int64_t ctx_max, int64_t prefix_max, int window);
 int nsx_batch_attn(const void *q, int x_dtype, const nsx_kv_rows *kv, const nsx_kv_rows *prefix, int kv_type,

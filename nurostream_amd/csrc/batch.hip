@@ -1150,6 +1150,8 @@ static int move_rows(void* k, void* v, int x_dtype, int64_t n, const int32_t* st
   NSX_REQUIRE(k && v && aligned16(k) && aligned16(v), NSX_EINVAL, "k and v must be 16-byte aligned buffers");
   const int64_t rows = kv->n_seq * n_kv * n;
   NSX_REQUIRE(rows < (1ll << 28), NSX_EINVAL, "%lld rows: fewer than 2^28", (long long)rows);
+  const int64_t bytes = rows * head_dim * x_size(x_dtype);
+  NSX_REQUIRE(STORE || !overlap(k, bytes, v, bytes), NSX_EINVAL, "k overlaps v");
   const RowsArgs a{k, v, kv_rows(kv), start, start0, n, rows, n_kv};
   return with_types(x_dtype, kv_type, head_dim, [&](auto x, auto t, auto d) {
     // four rows a thread where that leaves workgroups for every CU (4 x 16000 rows of 8 heads into int8: 38 us, with one 53;
@@ -1201,9 +1203,11 @@ extern "C" int nsx_batch_attn(const void* q, int x_dtype, const nsx_kv_rows* kv,
                                                       prefix ? prefix->ctx_max : 0, window);
   NSX_REQUIRE((workspace || !need) && aligned16(workspace) && workspace_bytes >= need, NSX_EINVAL,
               "workspace of %lld bytes, %lld needed, 16-byte aligned", (long long)workspace_bytes, (long long)need);
+  const int64_t bytes = kv->n_seq * n * n_head * head_dim * x_size(x_dtype);
+  NSX_REQUIRE(!overlap(q, bytes, out, bytes), NSX_EINVAL, "out overlaps q");
   const Plan plan = attn_plan(n_kv, n_head / n_kv, kv->n_seq, n, kv->ctx_max, prefix ? prefix->ctx_max : 0, window,
                               attn_occ(x_dtype, head_dim));
-  NSX_REQUIRE(plan.pblocks + plan.oblocks < (1ll << 24) && kv->n_seq * n * n_head < (1ll << 26), NSX_EINVAL,
+  NSX_REQUIRE(plan.pblocks + plan.oblocks < (1ll << 24) && kv->n_seq * n * n_head <= (1ll << 26) - 4, NSX_EINVAL,
               "%lld tokens of %d heads: too many for one call", (long long)(kv->n_seq * n), n_head);
   const AttnArgs a{q, kv_rows(kv), prefix ? kv_rows(prefix) : KvRows{}, counts, sinks, n_head, n_kv, n_head / n_kv, window, n,
                    scale * LOG2E, (float*)workspace, out, plan.pre, plan.own, (int)plan.pblocks, plan.splits};

@@ -194,7 +194,7 @@ def batch_attn(q: torch.Tensor, cfg: AttnConfig, kv: BatchKV, layer: int, sinks:
                counts: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Sink attention of the new tokens' queries (n_seq, n, n_head, head_dim), as `append_qkv` gives them with their rows
     written -> the same shape and type: token j of a sequence sees the prefix, its sequence's rows and the new tokens up
-    to itself, the last `window` positions of those when window > 0. fp32 queries are taken with all their bits and weights
+    to itself, the last `window` positions of those when window > 0. out: not q's own memory. fp32 queries are taken with all their bits and weights
     of 24; weights are rounded to 16 bits beside fp16 queries, to 8 beside bf16 ones. Tokens that a sequence does not have
     (`counts`) give zeros."""
     d, H, G = cfg.head_dim, cfg.n_head, cfg.n_head_kv
@@ -216,10 +216,10 @@ def batch_attn(q: torch.Tensor, cfg: AttnConfig, kv: BatchKV, layer: int, sinks:
             raise ValueError(f"{n} tokens of {kv.n_seq} sequences: too many for one call")
         kv._scratch[H, n, window] = nb
     # stream-ordered scratch, as the output
-    ws = None if nb == 0 else torch.empty(nb, dtype=torch.uint8, device=kv.device).data_ptr()
+    ws = None if nb == 0 else torch.empty(nb, dtype=torch.uint8, device=kv.device)
     _call("batch_attn", lib.nsx_batch_attn, kv.device, q.data_ptr(), X_TYPES[q.dtype], kv.rows(layer),
           None if prefix is None else prefix.rows(layer), kv._kind, H, G, d, n, _ptr(counts), _ptr(sinks), window,
-          1.0 / math.sqrt(d), ws, nb, y.data_ptr())
+          1.0 / math.sqrt(d), _ptr(ws), nb, y.data_ptr())
     return y
 
 

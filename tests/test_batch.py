@@ -72,7 +72,7 @@ def test_cache_checks(lib, kw):
 
 def _attn(lib, **kw):
     a = dict(q=A, dt=N.DT_F32, kv=None, prefix=None, kind=N.KV_INT8, H=16, G=2, d=64, n=5, counts=None, sinks=None, window=0,
-             scale=0.125, ws=A, wsb=1 << 40, out=A)
+             scale=0.125, ws=A, wsb=1 << 40, out=A + (1 << 30))
     a.update(kw)
     return lib.nsx_batch_attn(a["q"], a["dt"], C.byref(a["kv"] or _rows(ctx_max=5000)), a["prefix"] and C.byref(a["prefix"]), a["kind"], a["H"],
                               a["G"], a["d"], a["n"], a["counts"], a["sinks"], a["window"], a["scale"], a["ws"], a["wsb"],
@@ -84,7 +84,7 @@ def _attn(lib, **kw):
     (dict(n=1 << 23), N.EINVAL), (dict(window=-1), N.EINVAL), (dict(q=None), N.EINVAL), (dict(out=None), N.EINVAL),
     (dict(q=A + 8), N.EINVAL), (dict(out=A + 4), N.EINVAL), (dict(ws=None), N.EINVAL), (dict(scale=0.0), N.EINVAL), (dict(scale=-1.0), N.EINVAL),
     (dict(scale=float("nan")), N.EINVAL), (dict(scale=float("inf")), N.EINVAL), (dict(ws=A + 8), N.EINVAL),
-    (dict(wsb=0), N.EINVAL), (dict(n=0), N.OK)])
+    (dict(wsb=0), N.EINVAL), (dict(out=A), N.EINVAL), (dict(out=A + 2 * 5 * 16 * 64 * 4 - 16), N.EINVAL), (dict(n=0), N.OK)])
 def test_attention_checks(lib, kw, code):
     assert _attn(lib, **kw) == code
     assert _attn(lib, prefix=_rows(n_seq=1), **kw) == code
@@ -102,6 +102,8 @@ def test_rows_checks(lib, kw, code):
     a = dict(k=A, v=A, dt=N.DT_F32, n=3, start0=0, G=2, d=64, kind=N.KV_INT8)
     a.update(kw)
     kv = _rows()
+    if code == N.OK:  # two outputs in one place
+        assert lib.nsx_load_rows(C.byref(kv), N.KV_INT8, 2, 64, None, 0, 3, A, A + 512, N.DT_F32, None) == N.EINVAL
     assert lib.nsx_store_rows(a["k"], a["v"], a["dt"], a["n"], None, a["start0"], a["G"], a["d"], C.byref(kv), a["kind"],
                               None) == code
     assert lib.nsx_load_rows(C.byref(kv), a["kind"], a["G"], a["d"], None, a["start0"], a["n"], a["k"], a["v"], a["dt"],

@@ -458,3 +458,105 @@ def test_copies(dev, t, dt):
     c.copy_from(b)
     for x, y in zip(load_rows(c, 2, 0, 23), load_rows(b, 2, 0, 23)):
         assert torch.equal(x, y.to(torch.bfloat16).float())
+
+
+def test_two_streams_at_once(dev):
+    """Two batches behind one prefix, each a step at a time on a stream of its own, as one after the other."""
+    cfg, normal = _cfg(32, 4, 128), _gen(dev, 51)
+    inv, amp = yarn_inv_freq(cfg, dev)
+    prefix = BatchKV(1, cfg, 1, 3000, dev, dtype=torch.float8_e4m3fn)
+    _pass(prefix, cfg, normal(1, 2900, 40 * 128), inv, amp, None)
+    prefix.advance(2900)
+    sizes, steps = (5, 33), 8
+    rows = [[normal(b, 1, 40 * 128) for _ in range(steps)] for b in sizes]
+    sinks = normal(32)
+
+    def make():
+        return [BatchKV(1, cfg, b, steps, dev, dtype=torch.float8_e4m3fn, prefix=prefix) for b in sizes]
+
+    want = [[], []]
+    for i, kv in enumerate(make()):
+        for x in rows[i]:
+            want[i].append(_pass(kv, cfg, x, inv, amp, sinks))
+            kv.advance()
+    torch.cuda.synchronize()
+    batches, streams, got = make(), [torch.cuda.Stream() for _ in sizes], [[], []]
+    torch.cuda.synchronize()
+    for step in range(steps):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(_pass(batches[i], cfg, rows[i][step], inv, amp, sinks))
+                batches[i].advance()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("x,t,d,window", [(torch.float16, torch.bfloat16, 128, 0), (torch.bfloat16, torch.int8, 64, 20),
+                                          (torch.float32, torch.float8_e4m3fn, 128, 37)])
+def test_captured_steps_of_several_tokens(dev, x, t, d, window):
+    """Ragged steps of several tokens, two graphs of two batches behind one prefix replayed in turn, eager work between."""
+    cfg, normal = _cfg(24, 3, d), _gen(dev, 61 + window)
+    inv, amp = yarn_inv_freq(cfg, dev)
+    prefix = BatchKV(1, cfg, 1, 700, dev, dtype=t)
+    _pass(prefix, cfg, normal(1, 650, 30 * d).to(x), inv, amp, None)
+    prefix.advance(650)
+    sides = []
+    for B, n in ((3, 5), (2, 18)):
+        eager, kept = (BatchKV(1, cfg, B, 6 * n, dev, dtype=t, prefix=prefix) for _ in "ab")
+        rows, counts = torch.zeros(B, n, 30 * d, device=dev, dtype=x), torch.zeros(B, dtype=torch.int32, device=dev)
+        _pass(kept, cfg, rows, inv, amp, None, counts, window)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = _pass(kept, cfg, rows, inv, amp, None, counts, window)
+            kept.advance(n, counts)
+        kept.reset()
+        sides.append((B, n, eager, kept, rows, counts, graph, out))
+    for step in range(5):
+        for B, n, eager, kept, rows, counts, graph, out in sides:
+            fresh = normal(B, n, 30 * d).to(x)
+            c = torch.tensor([(step * 3 + 2 * b) % (n + 1) for b in range(B)], dtype=torch.int32, device=dev)
+            want = _pass(eager, cfg, fresh, inv, amp, None, c, window)
+            eager.advance(n, c)
+            rows.copy_(fresh)
+            counts.copy_(c)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) and torch.equal(kept.pos, eager.pos), (step, B)
+            assert not any(want[b, int(c[b]):].any() for b in range(B))
+
+
+@pytest.mark.parametrize("t", ROWS)
+def test_far_rows(dev, t):
+    """A cache of more than 2^31 elements: rows at its end, as those of a small one."""
+    cfg, normal = _cfg(8, 2, 128), _gen(dev, 71)
+    far, near = BatchKV(1, cfg, 3, 3_000_001, dev, dtype=t), BatchKV(1, cfg, 3, 101, dev, dtype=t)
+    assert far.k_stack.numel() > 2 ** 31
+    start = torch.tensor([0, 2, 1], dtype=torch.int32, device=dev)  # of 90 rows
+    k, v, qkv = normal(3, 2, 90, 128), normal(3, 2, 90, 128), normal(3, 9, 12 * 128)
+    inv = torch.zeros(64, device=dev)  # (positions differ)
+    outs = []
+    for kv in (far, near):
+        first = start + (kv.ctx_max - 101)
+        store_rows(k, v, kv, 0, first)
+        kv.pos.copy_(first + 90)
+        q = append_qkv(qkv, None, None, None, cfg, inv, 1.0, kv, 0)
+        outs.append((q, batch_attn(q, cfg, kv, 0, None, 60), *load_rows(kv, 0, kv.pos - 90, 99)))
+    for a, b in zip(outs[0][2:], outs[1][2:]):
+        assert torch.equal(a, b)
+    assert torch.equal(outs[0][0], outs[1][0])
+    held = _held(near)
+    want, room = attn_exact(outs[1][0], None, None, *held, near.pos.tolist(), 0, None, None, 60, 1 / math.sqrt(128))
+    for q, out, *_ in outs:
+        _close(out, want, room + rounding(want, out.dtype))
+
+
+def test_empty_copies(dev):
+    """Nothing copied: lengths of zero."""
+    cfg = _cfg(8, 2, 64)
+    b = BatchKV(2, cfg, 2, 25, dev, dtype=torch.int8)
+    b.advance(3)
+    b.copy_from(DeviceKV(2, cfg, 30, dev, dtype=torch.float16))
+    assert b.pos.tolist() == [0, 0] and b.length == 0
+    assert all(t.shape == (2, 2, 0, 64) for t in load_rows(b, 0, 5, 0))

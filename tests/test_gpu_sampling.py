@@ -189,3 +189,34 @@ def test_captured(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(token, want)
+
+
+def test_extreme_temperatures_of_rows(dev):
+    """Temperatures past both ends count as the ends: all tokens alike, or the largest logits alone."""
+    g = _gen(dev, 13)
+    logits = torch.randn(4, 5000, generator=g, device=dev)
+    logits[:, 7] = -float("inf")
+    logits[2, 100] = logits[2, 4000] = 9.0
+    t = torch.tensor([float("inf"), 1e38, 1e-38, float("nan")], device=dev)
+    u = torch.tensor([0.3, 0.75, 0.6, 0.5], device=dev)
+    others = [i for i in range(5000) if i != 7]
+    got = sample(logits, u, temperature=t).tolist()
+    assert got == [others[int(float(u[0]) * 4999)], others[int(0.75 * 4999)], 4000, int(logits[3].argmax())]
+
+
+def test_two_streams_at_once(dev):
+    """Calls on two streams, each with scratch of its own, as one after the other."""
+    g = _gen(dev, 14)
+    kw = dict(temperature=0.8, top_k=300, top_p=0.9)
+    sides = [(torch.randn(b, 50000, generator=g, device=dev), torch.rand(b, generator=g, device=dev)) for b in (1, 40)]
+    want = [[sample(x + i, u, **kw) for i in range(6)] for x, u in sides]
+    shifted = [[x + i for i in range(6)] for x, u in sides]
+    streams, got = [torch.cuda.Stream() for _ in sides], [[], []]
+    torch.cuda.synchronize()
+    for i in range(6):
+        for s, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[s].append(sample(shifted[s][i], sides[s][1], **kw))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
