@@ -639,6 +639,8 @@ struct Wave {
     const int lane = threadIdx.x & 63, i32 = lane & 31, h = lane >> 5;
     f16v s[NB];
     v4u k[D / 16];
+    // what codes' scores are taken from at once: the reference, or 0 where there is none yet
+    const float from = KV == NSX_DT_BF16 || m == LOWEST ? 0.f : m;
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) k[ks] = *(const v4u*)(kl + i32 * Pitch<D>::K + 32 * ks + 16 * h);
     if constexpr (D == 64) __builtin_amdgcn_sched_barrier(0);  // (all of them on their way before the first is waited for)
@@ -656,7 +658,7 @@ struct Wave {
         for (int e = 0; e < 16; e += 4) {
           const v4f f = *(const v4f*)(sk + 32 * nb + 2 * e + 4 * h);
 #pragma unroll
-          for (int x = 0; x < 4; ++x) s[nb][e + x] *= f[x];
+          for (int x = 0; x < 4; ++x) s[nb][e + x] = fmaf(s[nb][e + x], f[x], -from);
         }
       }
     }
@@ -679,9 +681,15 @@ struct Wave {
 #pragma unroll
       for (int e = 0; e < 16; e += 2) most = fmaxf(fmaxf(most, s[nb][e]), s[nb][e + 1]);
     most = other_half_max(most);
-    if (KV == NSX_DT_BF16) most *= c;
+    most = KV == NSX_DT_BF16 ? most * c : most + from;
     if (__any(most > m + 8.f)) {
       const float to = fmaxf(most, m), by = __builtin_amdgcn_exp2f(m - to);
+      if constexpr (KV != NSX_DT_BF16) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[nb][e] -= to - from;
+      }
       m = to;
       l *= by;
 #pragma unroll
@@ -711,7 +719,7 @@ struct Wave {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float y = s[u >> 1][8 * (u & 1) + e];
-        x[e] = __builtin_amdgcn_exp2f(KV == NSX_DT_BF16 ? fmaf(y, c, -m) : y - m);
+        x[e] = __builtin_amdgcn_exp2f(KV == NSX_DT_BF16 ? fmaf(y, c, -m) : y);
         l += x[e];
         if constexpr (KV != NSX_DT_BF16) x[e] *= g[e >> 2][e & 3];
       }
