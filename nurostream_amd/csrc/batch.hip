@@ -1,5 +1,12 @@
-// Several sequences at once (gfx950): the new tokens' rows into a cache of 16 or 8 bits, and attention over a prefix that
-// all sequences share and the rows of their own.
+// Several sequences at once (gfx950): the new tokens' rows into a cache of 16 or 8 bits, finished rows into it and back, and
+// attention over a prefix that all sequences share and the rows of their own.
+//
+// A cache row of 8 bits is codes c with one fp32 scale: x ~ c s, s the row's largest magnitude over the type's (127 for int8,
+// 448 for e4m3). Codes of either type, and bf16 rows, are bf16 numbers exactly, so attention multiplies the codes themselves
+// on the matrix cores and puts a key's scale to its score, a value row's to its weight.
+//
+// Times below are kernels' own, of replayed graphs or traces, on one MI355X; a large copy reaches 5.08 TB/s there (read and
+// written), a large bf16 product 1375 TFLOP/s.
 #include "nsx_common.h"
 
 #include <algorithm>
@@ -119,7 +126,8 @@ __device__ __forceinline__ void codes8(const float (&x)[8], uint32_t (&c)[2], fl
       uint32_t z[4];  // 1.5 * 2^23 more: the nearest whole number's low byte in the lowest one
 #pragma unroll
       for (int i = 0; i < 4; ++i) z[i] = __builtin_bit_cast(uint32_t, y[4 * h + i] + 12582912.f);
-      c[h] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(z[3], z[2], 0x0c0c0400u), __builtin_amdgcn_perm(z[1], z[0], 0x0c0c0400u), 0x05040100u);
+      c[h] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(z[3], z[2], 0x0c0c0400u),
+                                   __builtin_amdgcn_perm(z[1], z[0], 0x0c0c0400u), 0x05040100u);
     } else {
       const int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], 0, false);
       c[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], w, true);
@@ -187,7 +195,15 @@ struct AppendArgs {
   void* q;
 };
 
-// A workgroup per token and 256 / (D / 8) x passes of its heads.
+// x + bias; of a query or key head, with norm weights w, x <- x w / sqrt(mean(x^2) + eps); then (a, b) <- (a cos - b sin, b cos
+// + a sin) of partners d / 2 apart, at position * inv_freq; queries out in the input's type, rows into the cache. All of a row
+// lies in one row of lanes' registers from the first load to the stores, in fp32: everything is read and written once.
+//
+// A workgroup takes a token and 256 / (D / 8) of its heads at a time, so that its angles are computed once: the sine of a
+// position's 64-bit angle costs what some hundred fp32 operations do. `passes` of such heads follow each other in a workgroup
+// where tokens alone fill the chip: bf16 tokens of 80 heads of 64 into int8, one pass / all of them in a workgroup: 64 tokens
+// 3.0 / 4.0 us, 512 4.6 / 4.7, 4001 16.7 / 14.9. Few tokens are bound by the launch (one: 2.6 us), many by memory: 4001 fp32
+// tokens 25.7 us, where a copy of their 152 MB takes 29.9 (part of them stays in the caches).
 template <typename XT, int KV, int D>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   constexpr int LANES = D / 8, ROWS = 256 / LANES;
@@ -273,7 +289,9 @@ template <typename T>
 struct alignas(16) Eight {
   T e[8];
 };
-// A lane 8 consecutive elements of a row, D / 8 lanes a row, a thread RPT rows: all of their loads at once.
+// A lane takes 8 consecutive elements of a row, D / 8 lanes a row, a thread RPT rows: all of their loads at once. Bound by
+// memory: 4 x 16000 rows of 8 heads of 64, k and v: bf16 into int8 37.6 us and back 33.2, of 32.7 that a copy of the same 166
+// MB takes (with a row a thread 53). 37 rows are launches: 2.5 and 2.7 us.
 template <typename XT, int KV, int D, bool STORE, int RPT>
 __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
   constexpr int LANES = D / 8, ROWS = 256 / LANES;
@@ -307,7 +325,8 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) y[k] = to_f(in[i].e[k]);
       if constexpr (KV == NSX_DT_BF16) {
-        if (at[i] >= 0) *(Code*)(cache + (at[i] * D + 8 * l) * 2) = v4u{near2(y[0], y[1]), near2(y[2], y[3]), near2(y[4], y[5]), near2(y[6], y[7])};
+        const v4u w{near2(y[0], y[1]), near2(y[2], y[3]), near2(y[4], y[5]), near2(y[6], y[7])};
+        if (at[i] >= 0) *(Code*)(cache + (at[i] * D + 8 * l) * 2) = w;
       } else {
         uint32_t c[2];
         float s;
@@ -337,6 +356,28 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
 }
 
 // --- attention ---------------------------------------------------------------
+//
+// out = sum_t 2^(s_t - m) v_t / (sum_t 2^(s_t - m) + 2^(sink - m)), s_t = q . k_t scale log2(e), in one pass over the keys with
+// a running reference m and sum, all in fp32.
+//
+// The heads of a kv head, times the tokens, times (for the shared prefix) the sequences are the rows of one product: 64
+// sequences of 8 heads each make 512 rows, for which a prefix's keys are read once. Operations bind where rows are many (64
+// tokens behind 32768 rows: 34.7 GFLOP, 25 us of the matrix cores' time against 12 us of the bytes'), launches and latency
+// where they are few.
+//
+// A wave takes 32 rows, on v_mfma_f32_32x32x16_bf16. S = K Q^T, not Q K^T: the 16 scores that a lane then holds are of one row,
+// so that maxima and sums need one exchange between lane halves, and the weights are at once the second operand of V^T W^T,
+// without a trip through LDS. K's and V's rows lie in LDS as bf16, V's read transposed on the way (ds_read_b64_tr_b16).
+//
+// Queries and weights are NT bf16 terms: bf16 queries are themselves and their weights are rounded to bf16 (2^-8 of one at
+// most, as the output is); fp16's 11 bits are two terms of 8 exactly, weights 16 bits of theirs; fp32's 24 bits are three,
+// exactly. More terms are more products, not more reads.
+//
+// What it runs at: 64 bf16 tokens of 64 heads of 64 behind 32768 e4m3 rows 64 us (540 TFLOP/s): of the CUs' busy cycles the
+// vector units work in 71 % (per score a scale, half a maximum, an exponential of 4 issue slots, a sum, a scale, half a
+// rounding), the matrix cores in 27 %: the two overlap in part only, with 3 waves a SIMD. 4 x 512 tokens of 32 heads of 128
+// behind 2000 bf16 rows 81 us (700 TFLOP/s): 40 % and 33 % of busy cycles, the CUs being busy 64 % of the time, since sequences
+// of fewer tokens than others leave workgroups without work.
 
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float f16v __attribute__((ext_vector_type(16)));
@@ -534,7 +575,8 @@ __device__ __forceinline__ void row_alone(const AttnArgs& a, const Place& p, con
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const Source src = p.src[i];
-    const int t0 = i ? max(w.first - w.tiles[0], 0) : min(w.first, w.tiles[0]), t1 = i ? max(w.end - w.tiles[0], 0) : min(w.end, w.tiles[0]);
+    const int t0 = i ? max(w.first - w.tiles[0], 0) : min(w.first, w.tiles[0]);
+    const int t1 = i ? max(w.end - w.tiles[0], 0) : min(w.end, w.tiles[0]);
     const int lo = max(row.lo[i], w.from[i] + t0 * KEYS), hi = t1 > t0 ? min(row.hi[i], w.from[i] + t1 * KEYS) : 0;
 #pragma unroll 1
     for (int t = lo; t < hi; t += 64) {
@@ -674,7 +716,7 @@ struct Wave {
         }
     }
     // The reference is an earlier maximum, moved only when a score is 8 above it: weights stay below 2^8, and the sums are
-    // seldom rescaled.
+    // seldom rescaled (one look a stage: 68 us became 66 for 64 tokens behind 32768 e4m3 rows, 87 81 for prompts of 512).
     float most = s[0][0];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
@@ -703,7 +745,8 @@ struct Wave {
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
         // values of dimension 32 i + lane % 32, keys 16 u + 4 h .. + 3 and 8 behind them
-        const uint8_t* at = vl + (16 * u + 4 * h + ((lane & 15) >> 2)) * Pitch<D>::V + 2 * (32 * i + 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
+        const uint8_t* at = vl + (16 * u + 4 * h + ((lane & 15) >> 2)) * Pitch<D>::V +
+                            2 * (32 * i + 16 * ((lane >> 4) & 1) + 4 * (lane & 3));
         const v2u a = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s4*)at));
         const v2u b = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s4*)(at + 8 * Pitch<D>::V)));
         to[i] = v4u{a[0], a[1], b[0], b[1]};
@@ -791,11 +834,14 @@ template <int D>
 constexpr int attn_lds() {
   return 2 * Pitch<D>::stage(64) + 2048;  // two stages of 64 keys (or four waves' of 32), scales; then sums to be joined
 }
-// A workgroup's rows over its keys. SHARED: its four waves take 32 rows each and share every stage of 64 keys; else all
-// of them take the same 32 rows, each every fourth stage of 32 keys, and their sums are joined in LDS.
+// A workgroup's rows over its keys. SHARED: its four waves take 32 rows each and share every stage of 64 keys, the next on its
+// way from memory meanwhile, the one behind it in the other half of LDS: a barrier a stage. Else all of them take the same 32
+// rows, each every fourth stage of 32 keys, without a barrier, and their sums are joined in LDS: more waves for few rows (64
+// tokens behind 8000 int8 rows 32 us so, SHARED 38; behind 32768 e4m3 rows 86 and 68).
 template <typename XT, int KV, int D, int NT, bool SHARED>
 __device__ __forceinline__ void attend(const AttnArgs& a, const Place& p, uint8_t* lds) {
-  constexpr int KEYS = SHARED ? 64 : 32, THREADS = SHARED ? 256 : 64, STAGE = Pitch<D>::stage(KEYS), SUMS = 2 * Pitch<D>::stage(64);
+  constexpr int KEYS = SHARED ? 64 : 32, THREADS = SHARED ? 256 : 64;
+  constexpr int STAGE = Pitch<D>::stage(KEYS), SUMS = 2 * Pitch<D>::stage(64);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i32 = lane & 31, h = lane >> 5;
   const int r = p.r0 + (SHARED ? AT_ROWS * wave : 0) + i32;
   Wave<KV, D, NT, KEYS / 32> w;
@@ -905,7 +951,8 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Place& p, uint8_
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
         const f16v& y = w.acc[blk];
-        *(v4f*)(sums + (wave * AT_ROWS + i32) * OP + 32 * blk + 2 * e + 4 * h) = v4f{y[e] * f, y[e + 1] * f, y[e + 2] * f, y[e + 3] * f};
+        *(v4f*)(sums + (wave * AT_ROWS + i32) * OP + 32 * blk + 2 * e + 4 * h) =
+            v4f{y[e] * f, y[e + 1] * f, y[e + 2] * f, y[e + 3] * f};
       }
     __syncthreads();
     // a wave a quarter of the dimensions of every row, two lanes a row
@@ -929,7 +976,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Place& p, uint8_
 
 template <typename XT>
 constexpr int attn_terms() {
-  // bf16 rows and codes of 8 bits are bf16's own; queries and weights are as many bf16 terms as their type has bytes of bits
+  // bf16 terms of a query (and of the weights beside it) that hold all of its 8, 11 or 24 bits
   return std::is_same_v<XT, float> ? 3 : std::is_same_v<XT, Half> ? 2 : 1;
 }
 template <typename XT, int KV, int D>
@@ -967,7 +1014,9 @@ __global__ __launch_bounds__(256, (attn_terms<XT>() == 3 && D == 128 ? 1 : 2)) v
   else attend<XT, KV, D, NT, true>(a, p, lds);
 }
 
-// The splits' sums of a (token, head) and its sink: a wave each, D / 4 lanes a split.
+// out = (sum_s 2^(m_s - M) y_s) / (sum_s 2^(m_s - M) l_s + 2^(sink - M)) over a (token, head)'s splits s: a wave each, D / 4
+// lanes a split, the splits in the same order in every call. The first rounds of y are loaded before the weights are known: 1
+// token of 64 heads over 30000 rows 10.7 us in all, so 8.8. Bound by latency: 4 us for 16 tokens of 64 heads, 6.4 for 64.
 template <typename XT, int D>
 __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
   constexpr int LPR = D / 4, AT_ONCE = 64 / LPR;
@@ -1022,8 +1071,18 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
 }
 
 // How a call's rows and keys are cut into workgroups: by the caches' sizes, not their lengths, so that a captured call serves
-// every length. Sequences of few rows each (a step of decoding) meet the prefix together, in workgroups of its own; those of
-// more than 64 meet it in their own workgroups, ahead of their own keys.
+// every length. Both sides of each rule in us, attention and join together:
+//  - sequences of up to 64 rows each (a step of decoding) meet the prefix together, in workgroups of its own, joined with their
+//    own keys; where all keys are 512 at most, or rows more, a sequence's workgroups meet the prefix ahead of their own keys,
+//    with no join for it (2 sequences behind 200 rows 6.7, apart 8.9; 32 sequences with a window of 128 7.5 and 11.2; but 64
+//    behind 1000 21.2, apart 12.4, 16 in fp32 14.8 and 11.6);
+//  - SHARED workgroups where a wave of 2048 has more than 20 pieces of 32 rows by 32 keys to do and there are more than 64 rows
+//    (19 pieces: 64 tokens behind 8000 int8 rows 38, else 32; 16: 16 in fp32 behind 32000 47 and 45; 37: 64 behind 16000 42 and
+//    53 to 64);
+//  - as many workgroups as the chip holds at once, but 3 pieces a wave in a split at least (16 sequences behind 1000 rows: 2
+//    10.9, 3 11.5, 4 12.9; 64: 4 best), of which a sequence's own keys take their share, a quarter at least, and the prefix
+//    what they leave, half at least; or, beyond 10 pieces a wave, all of them once more (64 behind 8000: 32, else 41; 64 behind
+//    16000 of 128 44 and 48; but 64 in fp32 behind 3000 31, else 27).
 struct Plan {
   AttnArgs::Cut pre, own;
   int64_t pblocks, oblocks;
@@ -1061,8 +1120,10 @@ Plan attn_plan(int G, int rep, int64_t B, int64_t n, int64_t ctx_max, int64_t pr
   p.splits = p.pre.splits + p.own.splits;
   return p;
 }
-// Workgroups of a kernel that a CU holds.
-int attn_occ(int x_dtype, int head_dim) { return x_dtype == NSX_DT_F32 && head_dim == 128 ? 1 : x_dtype == NSX_DT_BF16 && head_dim == 64 ? 3 : 2; }
+// Workgroups of a kernel that a CU holds, by its registers (up to 512, 256 or 168 a lane).
+int attn_occ(int x_dtype, int head_dim) {
+  return x_dtype == NSX_DT_F32 && head_dim == 128 ? 1 : x_dtype == NSX_DT_BF16 && head_dim == 64 ? 3 : 2;
+}
 
 // ---------------------------------------------------------------------------
 
@@ -1125,8 +1186,8 @@ extern "C" int nsx_append_qkv(const void* qkv, int x_dtype, const float* q_bias,
   if (const int rc = batch_types(x_dtype, kv_type)) return rc;
   if (const int rc = batch_heads(n_head, n_kv, head_dim)) return rc;
   if (const int rc = batch_cache(kv, kv_type, n_kv, "kv")) return rc;
-  NSX_REQUIRE(n >= 0 && n < (1ll << 24) && kv->n_seq * n < (1ll << 24), NSX_EINVAL, "%lld tokens of %lld sequences: fewer than 2^24",
-              (long long)n, (long long)kv->n_seq);
+  NSX_REQUIRE(n >= 0 && n < (1ll << 24) && kv->n_seq * n < (1ll << 24), NSX_EINVAL,
+              "%lld tokens of %lld sequences: fewer than 2^24", (long long)n, (long long)kv->n_seq);
   NSX_REQUIRE(eps >= 0.f, NSX_EINVAL, "eps %g", eps);
   if (n == 0) return NSX_OK;
   NSX_REQUIRE(qkv && q_out && inv_freq && kv->pos, NSX_EINVAL, "null buffer");
@@ -1137,7 +1198,7 @@ extern "C" int nsx_append_qkv(const void* qkv, int x_dtype, const float* q_bias,
   const int64_t tokens = kv->n_seq * n, e = x_size(x_dtype) * head_dim;
   NSX_REQUIRE(!overlap(qkv, tokens * heads * e, q_out, tokens * n_head * e), NSX_EINVAL, "q_out overlaps qkv");
   const int rows = 256 / (head_dim / 8), all = (int)nsx_cdiv(heads, rows);
-  const int passes = tokens >= 512 ? all : 1;
+  const int passes = tokens >= 512 ? all : 1;  // (both sides at append_kernel)
   const AppendArgs a{qkv, q_bias, k_bias, v_bias, q_norm, k_norm, inv_freq, eps, amplitude, n_head, n_kv, passes, n, counts,
                      prefix_pos, kv_rows(kv), q_out};
   return with_types(x_dtype, kv_type, head_dim, [&](auto x, auto t, auto d) {
@@ -1182,7 +1243,8 @@ extern "C" int nsx_load_rows(const nsx_kv_rows* kv, int kv_type, int n_kv, int h
 extern "C" int64_t nsx_batch_attn_workspace_bytes(int n_head, int n_kv, int head_dim, int64_t n_seq, int64_t n,
                                                   int64_t ctx_max, int64_t prefix_max, int window) {
   if (batch_heads(n_head, n_kv, head_dim) != NSX_OK || n_seq <= 0 || n_seq >= 65536 || n <= 0 || n >= (1ll << 24) ||
-      n_seq * n >= (1ll << 24) || ctx_max <= 0 || ctx_max >= (1ll << 30) || prefix_max < 0 || prefix_max >= (1ll << 30) || window < 0)
+      n_seq * n >= (1ll << 24) || ctx_max <= 0 || ctx_max >= (1ll << 30) || prefix_max < 0 || prefix_max >= (1ll << 30) ||
+      window < 0)
     return -1;
   int splits = 1;  // (whatever the type)
   for (const int dt : {NSX_DT_F32, NSX_DT_F16, NSX_DT_BF16})
@@ -1203,8 +1265,8 @@ extern "C" int nsx_batch_attn(const void* q, int x_dtype, const nsx_kv_rows* kv,
                 (long long)prefix->n_seq);
   }
   NSX_REQUIRE(scale > 0.f && scale < INFINITY, NSX_EINVAL, "scale %g", scale);
-  NSX_REQUIRE(n >= 0 && n < (1ll << 24) && window >= 0 && kv->n_seq * n < (1ll << 24), NSX_EINVAL, "n=%lld window=%d: fewer than 2^24 tokens",
-              (long long)n, window);
+  NSX_REQUIRE(n >= 0 && n < (1ll << 24) && window >= 0 && kv->n_seq * n < (1ll << 24), NSX_EINVAL,
+              "n=%lld window=%d: fewer than 2^24 tokens", (long long)n, window);
   if (n == 0) return NSX_OK;
   NSX_REQUIRE(q && out && kv->pos && aligned16(q) && aligned16(out), NSX_EINVAL, "q and out must be 16-byte aligned buffers");
   const int64_t need = nsx_batch_attn_workspace_bytes(n_head, n_kv, head_dim, kv->n_seq, n, kv->ctx_max,
@@ -1224,9 +1286,10 @@ extern "C" int nsx_batch_attn(const void* q, int x_dtype, const nsx_kv_rows* kv,
     constexpr int LDS = attn_lds<d()>();
     auto* kernel = attn_kernel<XT, t(), d()>;
     if (const int rc = nsx_allow_lds((const void*)kernel, LDS)) return rc;
-    if (const int rc = nsx_launch(kernel, dim3((unsigned)(plan.pblocks + plan.oblocks)), dim3(256), LDS, (hipStream_t)stream, a))
-      return rc;
+    const dim3 grid((unsigned)(plan.pblocks + plan.oblocks));
+    if (const int rc = nsx_launch(kernel, grid, dim3(256), LDS, (hipStream_t)stream, a)) return rc;
     if (plan.splits == 1) return (int)NSX_OK;
-    return nsx_launch(join_kernel<XT, d()>, dim3((unsigned)nsx_cdiv(kv->n_seq * n * n_head, 4)), dim3(256), 0, (hipStream_t)stream, a);
+    const dim3 join((unsigned)nsx_cdiv(kv->n_seq * n * n_head, 4));
+    return nsx_launch(join_kernel<XT, d()>, join, dim3(256), 0, (hipStream_t)stream, a);
   });
 }
