@@ -220,3 +220,14 @@ def test_two_streams_at_once(dev):
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("kw", [dict(top_p=0.9), dict(top_k=70), dict(top_k=3000, top_p=0.7), dict()])
+def test_a_row_alone(dev, kw):
+    """A row's token does not depend on the batch that it is in."""
+    g = _gen(dev, 15)
+    logits = 2 * torch.randn(130, 9000, generator=g, device=dev)
+    u = torch.rand(130, generator=g, device=dev)
+    want = sample(logits, u, temperature=0.9, **kw)
+    for rows in (slice(0, 1), slice(77, 78), slice(100, 130)):
+        assert torch.equal(sample(logits[rows], u[rows].clone(), temperature=0.9, **kw), want[rows])
