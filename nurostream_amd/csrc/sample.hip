@@ -65,6 +65,12 @@ struct SampleArgs {
   uint32_t* list;       // [batch][LIST]
 };
 
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ double uniform(double x) {  // (the same in all lanes: out of the vector registers)
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  return __builtin_bit_cast(double, (uint64_t)(uint32_t)uniform((int)(u >> 32)) << 32 | (uint32_t)uniform((int)(uint32_t)u));
+}
+
 // A row's logits and settings.
 template <typename LT>  // float, _Float16, or uint16_t for bf16
 struct Row {
@@ -84,8 +90,9 @@ struct Row {
     min_p = min_p > 0.0 ? fmin(min_p, 1.0) : 0.0;
     top_k = a.top_ks ? a.top_ks[row] : a.top_k;
     if (top_k <= 0 || top_k >= V) top_k = 0;
-    scale2 = 1.44269504088896340736 / T;
-    least = -1000.0 / scale2;
+    min_p = uniform(min_p);
+    scale2 = uniform(1.44269504088896340736 / T);
+    least = uniform(-1000.0 / scale2);
     unit = __builtin_bit_cast(double, (uint64_t)(1023 + a.bits) << 52);
   }
   // What top-p's tokens, of `whole` in all, are the first to reach: each of them has less than that before it.
@@ -104,7 +111,8 @@ struct Row {
     M = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(bits));
     infinite = M == INFINITY;
     if (infinite) M = 0.f;
-    scale32 = (float)fmin(16.0 * scale2, 3e38);  // (times a difference of zero: zero)
+    // (times a difference of zero: zero)
+    scale32 = __builtin_bit_cast(float, uniform(__builtin_bit_cast(int, (float)fmin(16.0 * scale2, 3e38))));
   }
   static __device__ __forceinline__ float value(LT x) {
     float f;
@@ -367,7 +375,7 @@ struct Ends {
     Ends e = *shared;
     if (r.few()) {  // (no weights are known: every token down to kbin is open)
       const int kbin = e.kbin < BINS ? e.kbin : BINS - 1;
-      *this = Ends{kbin, 0, kbin, 0, 0, 0, 0};
+      *this = Ends{uniform(kbin), 0, uniform(kbin), 0, 0, 0, 0};
       return;
     }
     __syncthreads();
@@ -388,6 +396,7 @@ struct Ends {
     }
     e.all = e.kbin == BINS ? am : 0;
     *this = e;
+    kbin = uniform(kbin), plo = uniform(plo), phi = uniform(phi);
   }
   __device__ __forceinline__ int last() const { return kbin < BINS ? kbin : phi; }  // bin that is sure or open
   __device__ __forceinline__ bool sure(int bin) const { return bin < kbin && bin < plo; }
