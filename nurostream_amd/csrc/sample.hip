@@ -13,12 +13,13 @@
 //     leaves of its last bin); the weight of its tokens above those, and the list of the tokens in them;
 //  4. a workgroup per row: where the filters end among the listed tokens; the parts' sums with what is kept of those; the part
 //     in which the random number falls, and in that part the token.
-// Greedy rows end behind the first, rows without top-k and top-p skip the second.
+// Where all rows are greedy the second and third are left out, without top-k and top-p the second; of few rows, the last of a
+// row's workgroups in the third does the fourth's work.
 //
-// Bytes bind nothing here: 48 rows of 151936 bf16 logits are 2.9 us of a copy's time. The launches take 2.9, 4.8, 6.0 and 9.0 us
-// for one row of 201088 with top-k 50 and top-p 0.95, where each is a chain of a few loads and barriers (the fourth some 20 000
-// cycles on one CU), and 6, 11, 17 and 16 us for 48 rows of settings of their own, where the second and third are
-// bound by the weights: some 30 vector instructions of a logit, most of 64 bits.
+// Bytes bind nothing here: 48 rows of 151936 bf16 logits are 2.9 us of a copy's time. The launches take 2.9, 4.8 and 13 us for
+// one row of 201088 with top-k 50 and top-p 0.95, each a chain of a few loads and barriers (the token's some 20 000 cycles on one
+// CU), and 6, 11, 15 and 16 us for 48 rows of settings of their own, where the second and third are bound by the weights: some 30
+// vector instructions of a logit, most of 64 bits.
 #include "nsx_common.h"
 #include "pow2.h"
 
@@ -31,19 +32,23 @@ namespace {
 constexpr int THREADS = 512;
 constexpr int VEC = 8;                  // logits of a thread, consecutive
 constexpr int PART = THREADS * VEC;     // logits of a part
-constexpr int INDEX = 22;              // bits of an index
+constexpr int INDEX = 22;               // bits of an index
 constexpr uint32_t LAST_INDEX = (1u << INDEX) - 1;
 constexpr int MAX_PARTS = 1 + (1 << INDEX) / PART;
 constexpr int BINS = 1024;              // 64 octaves of 16: no weight lies lower
 constexpr int LIST = 8192;              // listed tokens; a row with more in its last bins is read again instead
 constexpr int HELD = 4;                 // listed tokens that a thread holds in registers
-constexpr int FEW = HELD * THREADS / 2;  // a top-k below which all tokens that it may keep are listed (see few())
-// Listed tokens up to which each is compared with each, all threads at once, in place of digit after digit: the fourth launch
+constexpr int FEW = HELD * THREADS / 2;  // a top-k up to which all tokens that it may keep are listed (see few())
+// Listed tokens up to which each is compared with each, all threads at once, in place of digit after digit: the last step
 // takes 9.3 us so for 52 tokens, 11.6 by digits.
 constexpr int RANK = THREADS / 4;
-// Workgroups of a pass over all rows, four on each of 256 CUs: rows differ in work, and smaller shares of them level that (48 rows
-// of settings of their own 59 us in all with 512 and with 768, 55 with 1024, 57 with all parts apart).
+// Workgroups of a pass over all rows, four on each of 256 CUs: rows differ in work, and smaller shares of them level that
+// (48 rows of settings of their own 59 us in all with 512 and with 768, 55 with 1024, 57 with all parts apart).
 constexpr int GRID = 1024;
+// Workgroups up to which the last of a row's goes on to its token, a launch less (its registers leave two workgroups a CU):
+// rows of 151936 bf16 logits with top-p 0.9, so / by a launch of its own: 1 row 23.6 / 26.3 us, 4 25.7 / 27.2, 8 32.5 / 30.7,
+// 48 66 / 52; without filters 13.1 / 14.7, 15.4 / 14.9, 18.6 / 16.7, 38 / 31.
+constexpr int FUSED = 160;
 
 struct SampleArgs {
   const void* logits;
@@ -62,6 +67,7 @@ struct SampleArgs {
   uint64_t* mass;       // [batch][BINS]
   uint32_t* many;       // [batch][BINS]
   uint32_t* listed;     // [batch]
+  uint32_t* ended;      // [batch]: workgroups of a row that are through its parts
   uint32_t* list;       // [batch][LIST]
 };
 
@@ -272,6 +278,7 @@ __global__ __launch_bounds__(THREADS) void best_kernel(SampleArgs a) {
       a.many[row * BINS + i] = 0;
       if (i == 0) a.listed[row] = 0;
     }
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.ended[row] = 0;
   // (a thread keeps the eight logits among which its largest is, and looks for that one's place behind the last)
   typename Row<LT>::Raw next = r.load((int64_t)blockIdx.x * PART + threadIdx.x * VEC), held = next;
   float most = -INFINITY;
@@ -403,62 +410,6 @@ struct Ends {
   __device__ __forceinline__ bool open(int bin) const { return bin == kbin || (bin >= plo && bin <= phi && bin <= kbin); }
 };
 
-template <typename LT>
-__global__ __launch_bounds__(THREADS) void sums_kernel(SampleArgs a) {
-  constexpr int OPEN = 2048;  // listed tokens of a workgroup; where they are more, the row is read again
-  __shared__ uint64_t s[NW], sums[MAX_PARTS];
-  __shared__ uint32_t list[OPEN], n, base;
-  __shared__ Ends shared;
-  __shared__ Pow2 tab;
-  const int64_t row = blockIdx.y;
-  Row<LT> r(a, row);
-  const bool cut = a.mass && r.cut();
-  const Known known(a, row, cut);
-  tab.fill();
-  if (threadIdx.x == 0) n = 0;
-  for (int i = threadIdx.x; i < (a.parts - 1) / a.groups + 1; i += THREADS) sums[i] = 0;
-  r.largest(block_max(known.best, s));
-  if (!r.drawn()) return;
-  Ends e{BINS, BINS, BINS, 0, 0, 0, 0};
-  if (cut) e.find(r, known, s, &shared);
-  const float deepest = e.last() < BINS - 1 ? (float)(e.last() + 1) : INFINITY;  // (one look tells most tokens from those kept)
-  each_part(a, r, [&](int part, int64_t i, const float (&x)[VEC]) {
-    uint64_t sum = 0;
-    bool sure[VEC], any = false;
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      const float depth = r.depth(x[k]);
-      const int b = Row<LT>::bin_at(depth);
-      sure[k] = depth < deepest && e.sure(b);
-      any |= sure[k];
-      if (depth < deepest && e.open(b)) {
-        const uint32_t at = atomicAdd(&n, 1u);
-        if (at < OPEN) list[at] = (uint32_t)(i + k);
-      }
-    }
-    if (__any(any)) {
-#pragma unroll 4
-      for (int k = 0; k < VEC; ++k) {
-        const double w = r.real(x[k], tab);
-        sum += sure[k] && !(w < r.min_p) ? r.whole(w) : 0;
-      }
-    }
-    if (__any(sum != 0)) {
-      sum = wave_sum64(sum);
-      if ((threadIdx.x & 63) == 0) atomicAdd((unsigned long long*)&sums[part / a.groups], (unsigned long long)sum);
-    }
-  });
-  __syncthreads();
-  const uint32_t mine = n;
-  if (mine && threadIdx.x == 0) base = atomicAdd(&a.listed[row], mine <= OPEN ? mine : LIST + 1);
-  for (int part = blockIdx.x + threadIdx.x * a.groups; part < a.parts; part += THREADS * a.groups)
-    a.sums[row * a.parts + part] = sums[part / a.groups];
-  if (!mine) return;
-  __syncthreads();
-  for (uint32_t i = threadIdx.x; i < mine && i < OPEN; i += THREADS)
-    if (base + i < LIST) a.list[row * LIST + base + i] = list[i];
-}
-
 // Among tokens, the order of the one with which their sum from the highest on reaches `want`; 0 where all of them do not.
 // each(f): f(order, weight) for every token, by whichever threads. By digits of 10 bits of what an order lies above the lowest,
 // from the highest bit that one has, until the digits are all or few tokens are left.
@@ -541,38 +492,29 @@ __device__ __forceinline__ uint64_t pick_order(Pick& p, uint64_t want, Each each
   }
 }
 
-template <typename LT>
-__global__ __launch_bounds__(THREADS) void draw_kernel(SampleArgs a) {
-  __shared__ Pick p;
-  __shared__ Rank rank;
-  __shared__ Ends shared;
-  __shared__ Pow2 tab;
-  __shared__ uint64_t sums[MAX_PARTS];
-  __shared__ int found;
-  const int64_t row = blockIdx.x;
-  Row<LT> r(a, row);
-  const bool cut = a.mass && r.cut();
-  const Known known(a, row, cut);
+// What a row's last step holds in LDS.
+struct Draw {
+  Pick p;
+  Rank rank;
+  uint64_t sums[MAX_PARTS];
+  int found;
+};
+// What other workgroups of the same launch (SAME) or of the one before wrote.
+template <bool SAME, typename T>
+__device__ __forceinline__ T fetch(const T* p) {
+  return SAME ? __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : *p;
+}
+// A row's token, by one workgroup, from what its parts' workgroups found: their sums, in d.sums, and the n listed tokens, of which
+// `first` are this thread's.
+template <typename LT, bool SAME>
+__device__ __forceinline__ void draw(const SampleArgs& a, int64_t row, const Row<LT>& r, const Ends& e, bool cut, const Pow2& tab,
+                                     Draw& d, uint32_t n, const uint32_t (&first)[HELD]) {
+  Pick& p = d.p;
+  Rank& rank = d.rank;
+  uint64_t* sums = d.sums;
   const uint32_t* list = a.list + row * LIST;
-  uint32_t first[HELD], n = 0;
-  if (cut) {
-    n = a.listed[row];
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) first[i] = list[threadIdx.x + i * THREADS];  // (as many as there are count)
-  }
-  tab.fill();
-  for (int i = threadIdx.x; i < a.parts; i += THREADS) sums[i] = a.sums[row * a.parts + i];  // (of a drawn row)
-  if (threadIdx.x == 0) found = 0x7fffffff;
-  const uint64_t best = block_max(known.best, p.s);
-  r.largest(best);
-  if (!r.drawn()) {
-    if (threadIdx.x == 0) a.token[row] = r.M > -INFINITY ? (int32_t)(~(uint32_t)best & LAST_INDEX) : -1;
-    return;
-  }
-  Ends e{BINS, BINS, BINS, 0, 0, 0, 0};
   uint64_t last = 0;  // the order of the last token that the filters keep
   if (cut) {
-    e.find(r, known, p.s, &shared);
     // f(order, weight, bin, whether min-p keeps it) for the listed tokens: held in registers; or where they are more, taken
     // from the list, or from all of the row's in those bins
     uint64_t ho[HELD] = {}, hw[HELD] = {};
@@ -600,7 +542,7 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(SampleArgs a) {
           uint64_t o, w;
           int b;
           bool keep;
-          look(n <= LIST ? list[i] : (uint32_t)i, o, w, b, keep);
+          look(n <= LIST ? fetch<SAME>(list + i) : (uint32_t)i, o, w, b, keep);
           if (w && e.open(b)) f(o, w, b, keep);
         }
       }
@@ -689,13 +631,13 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(SampleArgs a) {
     const int part = threadIdx.x * PER + i;
     const uint64_t m = part < a.parts ? sums[part] : 0;
     if (run <= target && run + m > target) {
-      found = part;
+      d.found = part;
       p.above = run;
     }
     run += m;
   }
   __syncthreads();
-  const int part = found;
+  const int part = d.found;
   if (part >= a.parts) return;  // (no weight is a number: does not happen)
   // and the token in it
   const int64_t v = (int64_t)part * PART + threadIdx.x * VEC;
@@ -721,6 +663,125 @@ __global__ __launch_bounds__(THREADS) void draw_kernel(SampleArgs a) {
   }
 }
 
+// LAST: the last workgroup of a row goes on to its token. What it needs of the others they store past their caches, then count
+// themselves.
+template <typename LT, bool LAST>
+__global__ __launch_bounds__(THREADS) void sums_kernel(SampleArgs a) {
+  constexpr int OPEN = 2048;  // listed tokens of a workgroup; where they are more, the row is read again
+  __shared__ uint64_t s[NW], sums[MAX_PARTS];
+  __shared__ uint32_t list[OPEN], n, base;
+  __shared__ Ends shared;
+  __shared__ Pow2 tab;
+  const int64_t row = blockIdx.y;
+  Row<LT> r(a, row);
+  const bool cut = a.mass && r.cut();
+  const Known known(a, row, cut);
+  tab.fill();
+  if (threadIdx.x == 0) n = 0;
+  for (int i = threadIdx.x; i < (a.parts - 1) / a.groups + 1; i += THREADS) sums[i] = 0;
+  const uint64_t best = block_max(known.best, s);
+  r.largest(best);
+  if (!r.drawn()) {
+    if (LAST && blockIdx.x == 0 && threadIdx.x == 0)
+      a.token[row] = r.M > -INFINITY ? (int32_t)(~(uint32_t)best & LAST_INDEX) : -1;
+    return;
+  }
+  Ends e{BINS, BINS, BINS, 0, 0, 0, 0};
+  if (cut) e.find(r, known, s, &shared);
+  const float deepest = e.last() < BINS - 1 ? (float)(e.last() + 1) : INFINITY;  // (one look tells most tokens from those kept)
+  each_part(a, r, [&](int part, int64_t i, const float (&x)[VEC]) {
+    uint64_t sum = 0;
+    bool sure[VEC], any = false;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const float depth = r.depth(x[k]);
+      const int b = Row<LT>::bin_at(depth);
+      sure[k] = depth < deepest && e.sure(b);
+      any |= sure[k];
+      if (depth < deepest && e.open(b)) {
+        const uint32_t at = atomicAdd(&n, 1u);
+        if (at < OPEN) list[at] = (uint32_t)(i + k);
+      }
+    }
+    if (__any(any)) {
+#pragma unroll 4
+      for (int k = 0; k < VEC; ++k) {
+        const double w = r.real(x[k], tab);
+        sum += sure[k] && !(w < r.min_p) ? r.whole(w) : 0;
+      }
+    }
+    if (__any(sum != 0)) {
+      sum = wave_sum64(sum);
+      if ((threadIdx.x & 63) == 0) atomicAdd((unsigned long long*)&sums[part / a.groups], (unsigned long long)sum);
+    }
+  });
+  __syncthreads();
+  const uint32_t mine = n;
+  if (mine && threadIdx.x == 0) base = atomicAdd(&a.listed[row], mine <= OPEN ? mine : LIST + 1);
+  auto put = [](auto* p, auto v) {
+    if constexpr (LAST) __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    else *p = v;
+  };
+  for (int part = blockIdx.x + threadIdx.x * a.groups; part < a.parts; part += THREADS * a.groups)
+    put(a.sums + row * a.parts + part, sums[part / a.groups]);
+  if (mine) {
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < mine && i < OPEN; i += THREADS)
+      if (base + i < LIST) put(a.list + row * LIST + base + i, list[i]);
+  }
+  if constexpr (LAST) {
+    __shared__ Draw d;
+    __shared__ bool last;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (stored where every part of the chip sees it)
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      last = __hip_atomic_fetch_add(a.ended + row, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == a.groups - 1u;
+      d.found = 0x7fffffff;
+    }
+    __syncthreads();
+    if (!last) return;
+    uint32_t first[HELD], count = 0;
+    if (cut) {
+      count = fetch<true>(a.listed + row);
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) first[i] = fetch<true>(a.list + row * LIST + threadIdx.x + i * THREADS);
+    }
+    for (int i = threadIdx.x; i < a.parts; i += THREADS) d.sums[i] = fetch<true>(a.sums + row * a.parts + i);
+    __syncthreads();
+    draw<LT, true>(a, row, r, e, cut, tab, d, count, first);
+  }
+}
+
+template <typename LT>
+__global__ __launch_bounds__(THREADS) void draw_kernel(SampleArgs a) {
+  __shared__ Draw d;
+  __shared__ Ends shared;
+  __shared__ Pow2 tab;
+  const int64_t row = blockIdx.x;
+  Row<LT> r(a, row);
+  const bool cut = a.mass && r.cut();
+  const Known known(a, row, cut);
+  const uint32_t* list = a.list + row * LIST;
+  uint32_t first[HELD], n = 0;
+  if (cut) {
+    n = a.listed[row];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) first[i] = list[threadIdx.x + i * THREADS];  // (as many as there are count)
+  }
+  tab.fill();
+  for (int i = threadIdx.x; i < a.parts; i += THREADS) d.sums[i] = a.sums[row * a.parts + i];  // (of a drawn row)
+  if (threadIdx.x == 0) d.found = 0x7fffffff;
+  const uint64_t best = block_max(known.best, d.p.s);
+  r.largest(best);
+  if (!r.drawn()) {
+    if (threadIdx.x == 0) a.token[row] = r.M > -INFINITY ? (int32_t)(~(uint32_t)best & LAST_INDEX) : -1;
+    return;
+  }
+  Ends e{BINS, BINS, BINS, 0, 0, 0, 0};
+  if (cut) e.find(r, known, d.p.s, &shared);
+  draw<LT, false>(a, row, r, e, cut, tab, d, n, first);
+}
+
 int parts_of(int64_t vocab) { return (int)nsx_cdiv(vocab + VEC - 1, PART); }
 int64_t up16(int64_t v) { return (v + 15) & ~15ll; }
 
@@ -730,8 +791,9 @@ int sample_launch(const SampleArgs& a, int64_t batch, bool cut, bool greedy, hip
   if (const int rc = nsx_launch(best_kernel<LT>, grid, dim3(THREADS), 0, st, a)) return rc;
   if (cut)
     if (const int rc = nsx_launch(bins_kernel<LT>, grid, dim3(THREADS), 0, st, a)) return rc;
+  if (!greedy && a.groups * batch <= FUSED) return nsx_launch(sums_kernel<LT, true>, grid, dim3(THREADS), 0, st, a);
   if (!greedy)
-    if (const int rc = nsx_launch(sums_kernel<LT>, grid, dim3(THREADS), 0, st, a)) return rc;
+    if (const int rc = nsx_launch(sums_kernel<LT, false>, grid, dim3(THREADS), 0, st, a)) return rc;
   return nsx_launch(draw_kernel<LT>, dim3((unsigned)batch), dim3(THREADS), 0, st, a);
 }
 
@@ -739,7 +801,7 @@ int sample_launch(const SampleArgs& a, int64_t batch, bool cut, bool greedy, hip
 
 extern "C" int64_t nsx_sample_workspace_bytes(int64_t batch, int64_t vocab) {
   if (batch <= 0 || vocab <= 0 || vocab > (1 << INDEX)) return -1;
-  return batch * ((int64_t)parts_of(vocab) * 16 + BINS * 12 + LIST * 4) + up16(batch * 4);
+  return batch * ((int64_t)parts_of(vocab) * 16 + BINS * 12 + LIST * 4) + up16(batch * 8);
 }
 
 extern "C" int nsx_sample(const void* logits, int logits_dtype, int64_t row_stride, int64_t batch, int64_t vocab,
@@ -773,7 +835,7 @@ extern "C" int nsx_sample(const void* logits, int logits_dtype, int64_t row_stri
   uint32_t *many = (uint32_t*)(mass + batch * BINS), *list = many + batch * BINS, *listed = list + batch * LIST;
   const SampleArgs a{logits, row_stride, vocab, uniforms, s.temperature, s.top_p, s.min_p, s.top_k, s.temperatures,
                      s.top_ps, s.min_ps, s.top_ks, token, bits, parts, groups, best, sums, cut && !greedy ? mass : nullptr,
-                     many, listed, list};
+                     many, listed, listed + batch, list};
   hipStream_t st = (hipStream_t)stream;
   if (logits_dtype == NSX_DT_F32) return sample_launch<float>(a, batch, cut && !greedy, greedy, st);
   if (logits_dtype == NSX_DT_F16) return sample_launch<_Float16>(a, batch, cut && !greedy, greedy, st);
