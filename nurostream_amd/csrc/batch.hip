@@ -376,8 +376,8 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
 // What it runs at: 64 bf16 tokens of 64 heads of 64 behind 32768 e4m3 rows 64 us (540 TFLOP/s): of the CUs' busy cycles the
 // vector units work in 71 % (per score a scale, half a maximum, an exponential of 4 issue slots, a sum, a scale, half a
 // rounding), the matrix cores in 27 %: the two overlap in part only, with 3 waves a SIMD. 4 x 512 tokens of 32 heads of 128
-// behind 2000 bf16 rows 81 us (700 TFLOP/s): 40 % and 33 % of busy cycles, the CUs being busy 64 % of the time, since sequences
-// of fewer tokens than others leave workgroups without work.
+// behind 2000 bf16 rows 75 us (760 TFLOP/s): 40 % and 33 % of busy cycles, each wave's chain of products, exponentials and
+// products bound by itself: sharing the rows of ragged sequences out evenly over the workgroups made no difference.
 
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float f16v __attribute__((ext_vector_type(16)));
@@ -739,7 +739,9 @@ struct Wave {
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][e] *= by;
     }
-    // 16 keys at a time: their products stand beside the next ones' exponentials
+    // 16 keys at a time: their products stand beside the next ones' exponentials. Over bf16 rows of 128 a SIMD's other wave waits
+    // for these (4 x 512 tokens behind 2000 rows 81 us, so 75; 2 x 300 behind 20000 233 and 217; but 1000 tokens of one
+    // sequence 39.8 and 41.3); over codes that lost as much as it gained, over rows of 64 it made no difference.
     v4u v[D / 32], w[NT];
     auto load = [&](int u, v4u (&to)[D / 32]) {
 #pragma unroll
@@ -770,6 +772,7 @@ struct Wave {
     };
     load(0, v);
     weigh(0, w);
+    if constexpr (D == 128 && KV == NSX_DT_BF16) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int u = 0; u < 2 * NB; ++u) {
       v4u vn[D / 32], wn[NT];
@@ -787,6 +790,7 @@ struct Wave {
         for (int t = 0; t < NT; ++t) w[t] = wn[t];
       }
     }
+    if constexpr (D == 128 && KV == NSX_DT_BF16) __builtin_amdgcn_s_setprio(0);
   }
   __device__ __forceinline__ bool finite() const {
     float z = l * 0.f;

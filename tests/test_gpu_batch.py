@@ -560,3 +560,20 @@ def test_empty_copies(dev):
     b.copy_from(DeviceKV(2, cfg, 30, dev, dtype=torch.float16))
     assert b.pos.tolist() == [0, 0] and b.length == 0
     assert all(t.shape == (2, 2, 0, 64) for t in load_rows(b, 0, 5, 0))
+
+
+@pytest.mark.parametrize("x,t,n_head,n_kv,d,P,pos,n,counts,window", [
+    (torch.bfloat16, torch.bfloat16, 32, 4, 128, 1900, [10, 0, 300], 300, [300, 17, 0], 0),
+    (torch.bfloat16, torch.int8, 32, 4, 64, 2000, [5, 40, 0, 77], 260, [131, 260, 133, 1], 0),
+    (torch.float32, torch.float8_e4m3fn, 32, 4, 64, 1500, [0, 9, 2], 301, [299, 150, 200], 0),
+    (torch.float16, torch.bfloat16, 32, 4, 128, 1900, [0, 1, 2], 290, [0, 0, 290], 0),
+    (torch.bfloat16, torch.bfloat16, 24, 8, 128, 1500, [0] * 5, 250, [250, 200, 100, 60, 249], 700),
+    (torch.bfloat16, torch.bfloat16, 8, 1, 64, None, [100] * 70, 120, [(7 * i) % 121 for i in range(70)], 0),
+    (torch.bfloat16, torch.bfloat16, 32, 4, 64, 1900, [3, 4], 400, [-3, 500], 0)])
+def test_attention_ragged_prompts(dev, x, t, n_head, n_kv, d, P, pos, n, counts, window):
+    """Many tokens of sequences of very different numbers of them."""
+    given, counts = counts, [min(max(c, 0), n) for c in counts]
+    q, cfg, kv, s, cn, got = _attention(dev, x, t, n_head, n_kv, d, P, pos, n, counts, window)
+    if given != counts:  # (counts below 0 and above n count as those)
+        cn = torch.tensor(given, dtype=torch.int32, device=dev)
+        assert torch.equal(batch_attn(q, cfg, kv, 0, s, window, counts=cn, out=torch.full_like(q, math.nan)), got)
