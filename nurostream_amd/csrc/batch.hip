@@ -374,9 +374,9 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
 // exactly. More terms are more products, not more reads.
 //
 // What it runs at: 64 bf16 tokens of 64 heads of 64 behind 32768 e4m3 rows 64 us (540 TFLOP/s): of the CUs' busy cycles the
-// vector units work in 71 % (per score a scale, half a maximum, an exponential of 4 issue slots, a sum, a scale, half a
-// rounding), the matrix cores in 27 %: the two overlap in part only, with 3 waves a SIMD. 4 x 512 tokens of 32 heads of 128
-// behind 2000 bf16 rows 75 us (760 TFLOP/s): 40 % and 33 % of busy cycles, each wave's chain of products, exponentials and
+// vector units work in 75 % (per score a scale, half a maximum, an exponential of 4 issue slots, a sum, a scale, half a
+// rounding), the matrix cores in 31 %: the two overlap in part only, with 3 waves a SIMD. 4 x 512 tokens of 32 heads of 128
+// behind 2000 bf16 rows 75 us (760 TFLOP/s): 48 % and 42 % of busy cycles, each wave's chain of products, exponentials and
 // products bound by itself: sharing the rows of ragged sequences out evenly over the workgroups made no difference.
 
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
