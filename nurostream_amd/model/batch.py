@@ -142,7 +142,9 @@ def _fits(t: torch.Tensor, dtype: torch.dtype, index: int, numel: int) -> bool:
 
 def _tokens(x: torch.Tensor, heads: int, name: str, kv: BatchKV, cfg: AttnConfig, counts) -> int:
     """Checks shared by the calls on tokens -> tokens per sequence."""
-    N.require_device(x)
+    index = kv._index
+    if index < 0 or x.get_device() != index:
+        N.require_device(x)
     if x.dtype not in X_TYPES:
         N.act_dtype_code(x.dtype)
     G, d = kv.heads
@@ -152,9 +154,9 @@ def _tokens(x: torch.Tensor, heads: int, name: str, kv: BatchKV, cfg: AttnConfig
     n = numel // row
     if n < 1 or n * row != numel:
         raise ValueError(f"{name} of shape {tuple(x.shape)} for {kv.n_seq} sequences and rows of {heads * d}")
-    if not _fits(x, x.dtype, kv._index, numel):
+    if x.get_device() != index or not x.is_contiguous():
         _check(name, x, x.dtype, kv.device, numel)
-    if counts is not None and not _fits(counts, torch.int32, kv._index, kv.n_seq):
+    if counts is not None and not _fits(counts, torch.int32, index, kv.n_seq):
         _check("counts", counts, torch.int32, kv.device, kv.n_seq)
     if kv.length + n > kv.ctx_max:
         raise ValueError(f"{n} tokens behind up to {kv.length} rows of a cache of {kv.ctx_max}")
@@ -175,10 +177,13 @@ def append_qkv(qkv: torch.Tensor, bq, bk, bv, cfg: AttnConfig, inv_freq: torch.T
     d, H, G = cfg.head_dim, cfg.n_head, cfg.n_head_kv
     n = _tokens(qkv, H + 2 * G, "qkv", kv, cfg, counts)
     index = kv._index
-    for name, t, m in (("bq", bq, H * d), ("bk", bk, G * d), ("bv", bv, G * d), ("inv_freq", inv_freq, d // 2),
-                       ("q_norm", q_norm, d), ("k_norm", k_norm, d)):
-        if t is not None and not _fits(t, torch.float32, index, m):
-            _check(name, t, torch.float32, kv.device, m)
+    f32, nq, nk = torch.float32, H * d, G * d
+    if not ((bq is None or _fits(bq, f32, index, nq)) and (bk is None or _fits(bk, f32, index, nk)) and
+            (bv is None or _fits(bv, f32, index, nk)) and _fits(inv_freq, f32, index, d // 2) and
+            (q_norm is None or _fits(q_norm, f32, index, d)) and (k_norm is None or _fits(k_norm, f32, index, d))):
+        for name, t, m in (("bq", bq, nq), ("bk", bk, nk), ("bv", bv, nk), ("inv_freq", inv_freq, d // 2), ("q_norm", q_norm, d),
+                           ("k_norm", k_norm, d)):
+            _check(name, t, f32, kv.device, m)
     if out is None:
         q = qkv.new_empty((kv.n_seq, n, H, d))
     else:
@@ -260,7 +265,8 @@ def load_rows(kv: BatchKV, layer: int, start: int | torch.Tensor, n: int,
     if n < 0:
         raise ValueError(f"{n} rows")
     first, start0 = _first(start, kv, n)
-    N.require_device(kv.k_stack)
+    if kv._index < 0:
+        N.require_device(kv.k_stack)
     k = torch.empty((kv.n_seq, G, n, d), dtype=dtype, device=kv.device)
     v = torch.empty_like(k)
     _call("load_rows", N.load().nsx_load_rows, kv.device, kv.rows(layer), kv._kind, G, d, _ptr(first), start0, n,

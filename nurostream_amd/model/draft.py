@@ -67,9 +67,13 @@ def _ptr(t):
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
+# the current device where there is one: 0.1 us for torch.cuda.current_device()'s 0.25
+_current = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _call(what: str, fn, device: torch.device, *args) -> None:
     """fn(*args, the device's current stream), with the device current."""
-    if device.index == torch.cuda.current_device():
+    if device.index == _current():
         rc = fn(*args, _stream(device.index))
     else:
         with torch.cuda.device(device):
