@@ -644,7 +644,7 @@ struct Pitch {
 // A wave's 32 rows over its keys. Scores are K Q^T, so that a lane holds 16 of 32 keys' scores of one row (lane % 32; the
 // other lane of the row holds the others), and its weights are at once the second operand of V^T W^T, of which it holds D / 2
 // values of the same row. The operand's order of keys is the scores' own, and V's rows are read from LDS in it, transposed.
-template <int KV, int D, int NT, int NB>
+template <int KV, int D, int NT, int NB, bool FIRST>
 struct Wave {
   v4u q[NT][D / 16];
   f16v acc[D / 32];
@@ -739,9 +739,11 @@ struct Wave {
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][e] *= by;
     }
-    // 16 keys at a time: their products stand beside the next ones' exponentials. Over bf16 rows of 128 a SIMD's other wave waits
-    // for these (4 x 512 tokens behind 2000 rows 81 us, so 75; 2 x 300 behind 20000 233 and 217; but 1000 tokens of one
-    // sequence 39.8 and 41.3); over codes that lost as much as it gained, over rows of 64 it made no difference.
+    // 16 keys at a time: their products stand beside the next ones' exponentials. FIRST: a SIMD's other waves wait for these. 4 x
+    // 512 tokens of heads of 128 behind 2000 bf16 rows 81 us, so 75, over int8 92 and 88; 2 x 300 of heads of 64 behind 20000 in
+    // bf16 290 and 273, in fp32 734 and 612, over int8 870 and 775; 64 tokens in fp32 behind 32000 int8 rows 115 and 113; but 64
+    // of heads of 128 behind 32000 e4m3 rows 56.6 and 57.8, 1000 of one sequence 39.8 and 41.3. Not where waves share no keys (16
+    // tokens in fp32 behind 32000 int8 rows 42.7 and 43.5) or a SIMD has one (4 x 512 in fp32, heads of 128, 222 and 226).
     v4u v[D / 32], w[NT];
     auto load = [&](int u, v4u (&to)[D / 32]) {
 #pragma unroll
@@ -772,7 +774,7 @@ struct Wave {
     };
     load(0, v);
     weigh(0, w);
-    if constexpr (D == 128 && KV == NSX_DT_BF16) __builtin_amdgcn_s_setprio(1);
+    if constexpr (FIRST) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int u = 0; u < 2 * NB; ++u) {
       v4u vn[D / 32], wn[NT];
@@ -790,7 +792,7 @@ struct Wave {
         for (int t = 0; t < NT; ++t) w[t] = wn[t];
       }
     }
-    if constexpr (D == 128 && KV == NSX_DT_BF16) __builtin_amdgcn_s_setprio(0);
+    if constexpr (FIRST) __builtin_amdgcn_s_setprio(0);
   }
   __device__ __forceinline__ bool finite() const {
     float z = l * 0.f;
@@ -848,7 +850,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Place& p, uint8_
   constexpr int STAGE = Pitch<D>::stage(KEYS), SUMS = 2 * Pitch<D>::stage(64);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i32 = lane & 31, h = lane >> 5;
   const int r = p.r0 + (SHARED ? AT_ROWS * wave : 0) + i32;
-  Wave<KV, D, NT, KEYS / 32> w;
+  Wave<KV, D, NT, KEYS / 32, SHARED && !(NT == 3 && D == 128)> w;
   Stage<KV, D, KEYS, THREADS> st;
   // of each source, the keys that any live row of the workgroup sees, and those that all of the wave's do
   Range range;
