@@ -584,7 +584,8 @@ __device__ __forceinline__ void draw(const SampleArgs& a, int64_t row, const Row
         block_scan(in_k && kept ? hw[0] : 0, p.s, whole);
         whole += e.above_k;
       }
-      if (r.top_p < 1.0) kept = kept && (!in_p || e.above_p + before < r.target(whole));
+      // (what is open past phi, of top-k's last bin, lies behind top-p's end)
+      if (r.top_p < 1.0) kept = kept && in_p && e.above_p + before < r.target(whole);
       last = block_max(kept ? ~ho[0] : 0, p.s);
       last = last ? ~last : 0;
       if (kept && hk[0])
