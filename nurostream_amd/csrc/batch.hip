@@ -1051,17 +1051,18 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
   float M = nsx_row_fmax(fmaxf(m, sink));
   M = fmaxf(M, __shfl_xor(M, 16, 64));
   M = other_half_max(M);
+  // (a split without a key is 0 times 0; a sum or a value that is no number stays none beside any weight)
   const float w = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - M);
-  const float Z = nsx_wave_sum(w == 0.f ? 0.f : w * l) + (a.sinks ? __builtin_amdgcn_exp2f(sink - M) : 0.f);
+  const float Z = nsx_wave_sum(w * l) + (a.sinks ? __builtin_amdgcn_exp2f(sink - M) : 0.f);
   float x[4] = {};
   for (int s0 = 0; s0 < a.splits; s0 += AHEAD * AT_ONCE) {
     if (s0) load(s0);
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
       const int s = s0 + AT_ONCE * i + lane / LPR;
-      const float ws = __shfl(w, min(s, 63), 64);  // (0 in lanes past the last split)
+      const float ws = __shfl(w, min(s, 63), 64);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) x[k] = ws != 0.f ? fmaf(ws, y[i][k], x[k]) : x[k];
+      for (int k = 0; k < 4; ++k) x[k] = s < a.splits ? fmaf(ws, y[i][k], x[k]) : x[k];
     }
   }
 #pragma unroll
