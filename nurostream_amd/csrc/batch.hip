@@ -519,32 +519,36 @@ struct End {
   __device__ __forceinline__ float* part(const At& r) const {
     return a.part + ((int64_t)(r.tok * a.H + r.h) * a.splits + p.slot) * D;
   }
-  // The factor that values are stored with: 1 for a part, what divides by the whole sum for the answer.
-  __device__ __forceinline__ float factor(const At& r, float m, float l, bool first) const {
+  // The factor that values are stored with: 1 for a part, what divides by the whole sum for the answer. `any` false: zeros, of
+  // a token that is not there or sees nothing, whatever the values are.
+  struct Factor {
+    float f;
+    bool any;
+  };
+  __device__ __forceinline__ Factor factor(const At& r, float m, float l, bool first) const {
     if (a.splits > 1) {
       if (first) {
         float2* ml = (float2*)(a.part + (int64_t)(a.kv.n_seq * a.n * a.H) * a.splits * D);
         ml[(int64_t)(r.tok * a.H + r.h) * a.splits + p.slot] = float2{m, l};
       }
-      return 1.f;
+      return {1.f, true};
     }
-    if (!r.live) return 0.f;
     float f = 1.f;
     if (a.sinks) {
       const float sink = a.sinks[r.h] * LOG2E, M = fmaxf(m, sink);
       f = __builtin_amdgcn_exp2f(m - M);
       l = fmaf(l, f, __builtin_amdgcn_exp2f(sink - M));
     }
-    return l == 0.f ? 0.f : f / l;
+    return {f / l, r.live && l != 0.f};
   }
   // Values d .. d + 3
-  __device__ __forceinline__ void store(const At& r, int d, float f, const float (&x)[4]) const {
+  __device__ __forceinline__ void store(const At& r, int d, const Factor& f, const float (&x)[4]) const {
     if (a.splits > 1) {
       *(v4f*)(part(r) + d) = v4f{x[0], x[1], x[2], x[3]};
     } else {
       float y[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = f == 0.f ? 0.f : x[i] * f;  // (a token that is not there: zero whatever x is)
+      for (int i = 0; i < 4; ++i) y[i] = f.any ? x[i] * f.f : 0.f;
       store4((XT*)a.out + (int64_t)(r.tok * a.H + r.h) * D + d, y);
     }
   }
@@ -625,11 +629,11 @@ __device__ __forceinline__ void row_alone(const AttnArgs& a, const Place& p, con
   }
   const End<XT, D> end{a, p};
   const At at{row.tok, row.h, row.live};
-  const float f = end.factor(at, m, l, lane == 0);
+  const auto f = end.factor(at, m, l, lane == 0);
 #pragma unroll
   for (int i = 0; i < D / 64; ++i) {
     if (a.splits > 1) end.part(at)[lane + 64 * i] = acc[i];
-    else from_f(((XT*)a.out + (int64_t)(row.tok * a.H + row.h) * D)[lane + 64 * i], f == 0.f ? 0.f : acc[i] * f);
+    else from_f(((XT*)a.out + (int64_t)(row.tok * a.H + row.h) * D)[lane + 64 * i], f.any ? acc[i] * f.f : 0.f);
   }
 }
 
@@ -921,7 +925,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Place& p, uint8_
   w.l = other_half_sum(w.l);
   if constexpr (SHARED) {
     if (mine && !(bad >> i32 & 1)) {
-      const float f = fin.factor(at, w.m, w.l, h == 0);
+      const auto f = fin.factor(at, w.m, w.l, h == 0);
 #pragma unroll
       for (int i = 0; i < D / 32; ++i)
 #pragma unroll
@@ -963,7 +967,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Place& p, uint8_
     __syncthreads();
     // a wave a quarter of the dimensions of every row, two lanes a row
     if (mine && !(bad >> i32 & 1)) {
-      const float y = fin.factor(at, M, L, threadIdx.x < 32);
+      const auto y = fin.factor(at, M, L, threadIdx.x < 32);
 #pragma unroll
       for (int e = 0; e < D / 8; e += 4) {
         const int d = D / 4 * wave + D / 8 * h + e;
@@ -1069,10 +1073,11 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
   for (int o = LPR; o < 64; o *= 2)
 #pragma unroll
     for (int k = 0; k < 4; ++k) x[k] += __shfl_xor(x[k], o, 64);
-  const float f = !live || Z == 0.f ? 0.f : 1.f / Z;
+  const bool any = live && Z != 0.f;
+  const float f = 1.f / Z;
   if (lane < LPR) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] = f == 0.f ? 0.f : x[k] * f;
+    for (int k = 0; k < 4; ++k) x[k] = any ? x[k] * f : 0.f;
     store4((XT*)a.out + row * D + 4 * lane, x);
   }
 }

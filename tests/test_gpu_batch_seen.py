@@ -1,5 +1,5 @@
 """What a token sees takes part in its attention (model/batch.py), however its keys are shared out over workgroups: an infinity
-or a NaN in a row that is seen shows, whatever weight the row has beside others."""
+or a NaN in a row that is seen shows, whatever weight the row has beside others and beside the sink."""
 from __future__ import annotations
 
 import math
@@ -77,3 +77,23 @@ def test_keys_of_no_weight(dev, x, t, P, bad):
         (k if bad == "key" else v)[:, :, row] = math.nan
         store_rows(k, v, prefix, 0)
         assert torch.isnan(batch_attn(q, cfg, kv, 0, None, 0)).all(), row
+
+
+@pytest.mark.parametrize("x", FLOATS)
+@pytest.mark.parametrize("t", ROWS)
+@pytest.mark.parametrize("P", [100, 2000])
+@pytest.mark.parametrize("bad", ["key", "value"])
+def test_beside_a_heavy_sink(dev, x, t, P, bad):
+    """The same beside a sink of e^1000 of every key's weight; a token that its sequence does not have is still zero."""
+    normal, cfg, prefix, kv = _batch(dev, t, P, [0, 3], seed=2)
+    q, s = normal(2, 1, 8, 64).to(x), torch.full((8,), 1000.0, device=dev)
+    assert not batch_attn(q, cfg, kv, 0, s, 0).any()
+    k, v = normal(1, 2, P, 64), normal(1, 2, P, 64)
+    (k if bad == "key" else v)[:, :, P - 2] = math.nan
+    store_rows(k, v, prefix, 0)
+    assert torch.isnan(batch_attn(q, cfg, kv, 0, s, 0)).all()
+    counts = torch.tensor([0, 1], dtype=torch.int32, device=dev)
+    got = batch_attn(q, cfg, kv, 0, s, 0, counts=counts, out=torch.full_like(q, math.nan))
+    assert not got[0].any() and torch.isnan(got[1]).all()
+    # and by a window that the row lies before
+    assert not batch_attn(q, cfg, kv, 0, s, 1, out=torch.full_like(q, math.nan)).any()
