@@ -762,7 +762,9 @@ class GptOssModel:
         self._fused[layer] = lay
         return lay
 
-    def _ffn_block(self, x: torch.Tensor, layer: int) -> torch.Tensor:
+    def _ffn_block(self, x: torch.Tensor, layer: int, live: torch.Tensor | None = None) -> torch.Tensor:
+        """x + moe(rms_norm(x)). live (T,) bool on the host: the rows that the router statistics count (None:
+        all)."""
         from ..compute.blockffn import BlockPrefetcher, stream_expert_ffn
         c, p = self.cfg, f"blk.{layer}."
         x = x.reshape(-1, c.n_embd).to(self.device, torch.float32).contiguous()
@@ -774,11 +776,11 @@ class GptOssModel:
             if self._capturing is not None:  # no host copy inside a graph capture: recorded after each replay
                 self._capturing.append((layer, ids))
             else:
-                self.router_stats.record(layer, ids)
+                self.router_stats.record(layer, ids if live is None else ids.cpu()[live])
             return x + out
         chosen, ids, weights = self._route(h, layer)
         stats = self.router_stats
-        stats.tokens_routed += h.shape[0]
+        stats.tokens_routed += h.shape[0] if live is None else int(live.sum())
         out = torch.zeros_like(h)
         active = []
         for e in chosen:
@@ -791,7 +793,9 @@ class GptOssModel:
         pf = BlockPrefetcher(self.cache, plan, self.block_rows, self.expert_lookahead)
         try:
             for e, rows, wgt in active:
-                stats.hits[(layer, e)] += rows.numel()
+                hits = rows.numel() if live is None else int(live[rows.cpu()].sum())
+                if hits:
+                    stats.hits[(layer, e)] += hits
                 stats.expert_reads += 1
                 out[rows] += wgt * stream_expert_ffn(self.cache, p, e, h[rows], c.n_ffn_expert, c.n_embd,
                                                      clamped_swiglu, self.block_rows, self.device, torch.float32,
@@ -1054,9 +1058,11 @@ class GptOssModel:
             raise ValueError(f"tokens of shape {tuple(tokens.shape)}, {tokens.dtype}: int32 ({kv.n_seq}, n)")
         B, n = tokens.shape
         x = self.embed(tokens.reshape(-1)).reshape(B * n, self.cfg.n_embd).contiguous()
+        # padding is routed as the other tokens are, but not counted
+        live = None if counts is None else (torch.arange(n) < counts.cpu().reshape(-1, 1)).reshape(-1)
         for layer in range(self.cfg.n_layer):
             x = self._attention_batch(x, layer, kv, counts)
-            x = self._ffn_block(x, layer)
+            x = self._ffn_block(x, layer, live)
         kv.advance(n, counts)
         if last_only and n > 1:
             at = torch.full((B,), n - 1, device=x.device) if counts is None else counts.long().clamp(1, n) - 1

@@ -61,7 +61,7 @@ class RouterStats:
 
     def record(self, layer: int, ids: torch.Tensor) -> None:
         """Count one forward's routing: ids (T, k) of `layer` (device or host)."""
-        flat = ids.reshape(ids.shape[0], -1).cpu()
+        flat = ids.cpu()
         self.tokens_routed += flat.shape[0]
         # hits per expert = tokens routing to it (an expert appears once per token)
         uniq, counts = torch.unique(flat, return_counts=True)
