@@ -1058,8 +1058,10 @@ class GptOssModel:
             raise ValueError(f"tokens of shape {tuple(tokens.shape)}, {tokens.dtype}: int32 ({kv.n_seq}, n)")
         B, n = tokens.shape
         x = self.embed(tokens.reshape(-1)).reshape(B * n, self.cfg.n_embd).contiguous()
-        # padding is routed as the other tokens are, but not counted
-        live = None if counts is None else (torch.arange(n) < counts.cpu().reshape(-1, 1)).reshape(-1)
+        # padding is routed as the other tokens are, but not counted (a graph capture counts nothing here)
+        live = None
+        if counts is not None and self._capturing is None:
+            live = (torch.arange(n) < counts.cpu().reshape(-1, 1)).reshape(-1)
         for layer in range(self.cfg.n_layer):
             x = self._attention_batch(x, layer, kv, counts)
             x = self._ffn_block(x, layer, live)

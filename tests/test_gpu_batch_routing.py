@@ -75,3 +75,30 @@ def test_generate_batch_counts_what_it_runs(dev, tmp_path):
     # (the first token is shared: run once; then 5, 1 and 2 of the prompts, and three of the four drawn of each)
     assert len(steps) == 4 and st.tokens_routed == 2 * (1 + 5 + 1 + 2 + 3 * 3)
     assert sum(st.hits.values()) == st.tokens_routed * cfg.top_k
+
+
+def test_a_captured_pass_of_ragged_steps(dev, tmp_path):
+    """A pass captured as the model's own decode graph is (no statistics on the way) serves other tokens and counts."""
+    ns, _ = _load(tmp_path, True)
+    model, c = ns.model, ns.model.attn_config()
+    eager, kept = (BatchKV(ns.cfg.n_layer, c, 3, 8, dev) for _ in "ab")
+    tokens, counts = torch.ones(3, 2, dtype=torch.int32, device=dev), torch.ones(3, dtype=torch.int32, device=dev)
+    model.forward_batch(tokens, kept, counts)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    model._capturing = []
+    try:
+        with torch.cuda.graph(graph):
+            logits = model.forward_batch(tokens, kept, counts)
+    finally:
+        model._capturing = None
+    kept.reset()
+    for step in range(4):
+        fresh = torch.tensor([[5 + step, 9], [40, 7 * step], [3, 200 + step]], dtype=torch.int32, device=dev)
+        some = torch.tensor([1 + step % 2, 2 - step % 2, int(step < 2)], dtype=torch.int32, device=dev)
+        want = model.forward_batch(fresh, eager, some)
+        tokens.copy_(fresh)
+        counts.copy_(some)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(logits, want) and torch.equal(kept.pos, eager.pos), step
