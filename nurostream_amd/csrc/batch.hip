@@ -95,8 +95,10 @@ __device__ __forceinline__ uint32_t near2(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{lo, hi}), b2));
 }
 // The codes of a lane's 8 elements of a row, and the row's scale. The largest is taken of the elements' bits, which order NaN
-// above infinity above every number. Elements meet the scale's reciprocal, 2^-23 of a code at most beside the quotient, so that
-// none passes the largest code; scales below 2^-100, whose reciprocals end, are divided by.
+// above infinity above every number. A code is the quotient by the scale, to fp32's nearest, then to the code's: the product with
+// the scale's reciprocal (the nearest as well) and one correction by what it leaves, exact in a fused multiply-add, so that
+// an element that is half of a step lies where a division puts it. Scales below 2^-60, beside which what a product leaves
+// may end below the least number, are divided by.
 template <int KV, int D>
 __device__ __forceinline__ void codes8(const float (&x)[8], uint32_t (&c)[2], float& scale) {
   uint32_t m = 0;
@@ -111,8 +113,11 @@ __device__ __forceinline__ void codes8(const float (&x)[8], uint32_t (&c)[2], fl
   const float s = __builtin_bit_cast(float, m) / TOP, r = 1.f / s;
   float y[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = x[i] * r;
-  if (!(s >= 0x1p-100f) || !finite) {
+  for (int i = 0; i < 8; ++i) {
+    const float z = x[i] * r;
+    y[i] = fmaf(fmaf(-z, s, x[i]), r, z);
+  }
+  if (!(s >= 0x1p-60f) || !finite) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       y[i] = finite && s > 0.f ? fminf(fmaxf(x[i] / s, -TOP), TOP) : 0.f;
