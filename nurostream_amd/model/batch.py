@@ -203,7 +203,7 @@ def batch_attn(q: torch.Tensor, cfg: AttnConfig, kv: BatchKV, layer: int, sinks:
     of 24; weights are rounded to 16 bits beside fp16 queries, to 8 beside bf16 ones. Tokens that a sequence does not have
     (`counts`) give zeros."""
     d, H, G = cfg.head_dim, cfg.n_head, cfg.n_head_kv
-    n, window, prefix = _tokens(q, H, "q", kv, cfg, counts), int(window), kv.prefix
+    n, window, prefix = _tokens(q, H, "q", kv, cfg, counts), min(int(window), 2 ** 31 - 1), kv.prefix  # (past it: all rows)
     if sinks is not None and not _fits(sinks, torch.float32, kv._index, H):
         _check("sinks", sinks, torch.float32, kv.device, H)
     if window < 0:

@@ -49,7 +49,7 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor | None = None, *, temper
     lib = N.load()
     nb = max(16, lib.nsx_sample_workspace_bytes(B, V))
     ws = torch.empty(nb, dtype=torch.uint8, device=dev)  # stream-ordered scratch, as the output
-    settings = N.SamplingC(float(t), float(p), float(m), int(k), _ptr(ts), _ptr(ps), _ptr(ms), _ptr(ks))
+    settings = N.SamplingC(float(t), float(p), float(m), max(-1, min(int(k), V)), _ptr(ts), _ptr(ps), _ptr(ms), _ptr(ks))
     _call("sample", lib.nsx_sample, dev, logits.data_ptr(), code, ld, B, V, _ptr(uniforms), C.byref(settings), token.data_ptr(),
           ws.data_ptr(), nb)
     return token
