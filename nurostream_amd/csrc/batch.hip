@@ -295,7 +295,7 @@ struct alignas(16) Eight {
   T e[8];
 };
 // A lane takes 8 consecutive elements of a row, D / 8 lanes a row, a thread RPT rows: all of their loads at once. Bound by
-// memory: 4 x 16000 rows of 8 heads of 64, k and v: bf16 into int8 37.6 us and back 33.2, of 32.7 that a copy of the same 166
+// memory: 4 x 16000 rows of 8 heads of 64, k and v: bf16 into int8 38.9 us and back 33.4, of 32.7 that a copy of the same 166
 // MB takes (with a row a thread 53). 37 rows are launches: 2.5 and 2.7 us.
 template <typename XT, int KV, int D, bool STORE, int RPT>
 __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
@@ -379,10 +379,13 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a) {
 // exactly. More terms are more products, not more reads.
 //
 // What it runs at: 64 bf16 tokens of 64 heads of 64 behind 32768 e4m3 rows 64 us (540 TFLOP/s): of the CUs' busy cycles the
-// vector units work in 75 % (per score a scale, half a maximum, an exponential of 4 issue slots, a sum, a scale, half a
-// rounding), the matrix cores in 31 %: the two overlap in part only, with 3 waves a SIMD. 4 x 512 tokens of 32 heads of 128
+// vector units work in 77 % (per score a scale, half a maximum, an exponential of 4 issue slots, a sum, a scale, half a
+// rounding), the matrix cores in 32 %: the two overlap in part only, with 3 waves a SIMD. 4 x 512 tokens of 32 heads of 128
 // behind 2000 bf16 rows 75 us (760 TFLOP/s): 48 % and 42 % of busy cycles, each wave's chain of products, exponentials and
-// products bound by itself: sharing the rows of ragged sequences out evenly over the workgroups made no difference.
+// products bound by itself: sharing the rows of ragged sequences out evenly over the workgroups made no difference. (A card that
+// has been at work for some time; from rest the first calls of these two take 69 and 96 us, calls that are waited for 66 and 86.)
+// fp32 queries, three products for one: 256 tokens of 64 heads of 64 behind 32000 bf16 rows 335 us, of the 294 that the
+// matrix cores take for 404 GFLOP; 64 tokens behind 32768 108 us of 76, where splits, the join and the exponentials show.
 
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float f16v __attribute__((ext_vector_type(16)));
@@ -1137,7 +1140,8 @@ Plan attn_plan(int G, int rep, int64_t B, int64_t n, int64_t ctx_max, int64_t pr
   p.splits = p.pre.splits + p.own.splits;
   return p;
 }
-// Workgroups of a kernel that a CU holds, by its registers (up to 512, 256 or 168 a lane).
+// Workgroups of a kernel that a CU is taken to hold, by its registers: up to 512, 256 or 168 a lane. (fp16 with heads of 64 needs
+// 168 as well, and three would fit; it is planned for two.)
 int attn_occ(int x_dtype, int head_dim) {
   return x_dtype == NSX_DT_F32 && head_dim == 128 ? 1 : x_dtype == NSX_DT_BF16 && head_dim == 64 ? 3 : 2;
 }

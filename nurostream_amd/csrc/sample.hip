@@ -36,7 +36,11 @@ constexpr int INDEX = 22;               // bits of an index
 constexpr uint32_t LAST_INDEX = (1u << INDEX) - 1;
 constexpr int MAX_PARTS = 1 + (1 << INDEX) / PART;
 constexpr int BINS = 1024;              // 64 octaves of 16: no weight lies lower
-constexpr int LIST = 8192;              // listed tokens; a row with more in its last bins is read again instead
+// Listed tokens. A row with more in its last bins is read again instead, by its one workgroup of the last step, for every digit
+// and sum: one row of 201088 at temperature 0.1 with top-k 50, where fewer than 50 tokens lie within 64 octaves and all others
+// share the last bin, 399 us, with top-p 0.95 as well 683; of logits of deviation 0.1 with top-p 0.95 627; 48 rows of 151936 the
+// same (temperature 0.8: 22 and 39).
+constexpr int LIST = 8192;
 constexpr int HELD = 4;                 // listed tokens that a thread holds in registers
 constexpr int FEW = HELD * THREADS / 2;  // a top-k up to which all tokens that it may keep are listed (see few())
 // Listed tokens up to which each is compared with each, all threads at once, in place of digit after digit: the last step
