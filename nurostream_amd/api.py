@@ -220,14 +220,19 @@ class NeuroStream:
         if temperature <= 0 or not (0 < top_p < 1 or top_k > 0 or min_p > 0):
             return logits
         p_desc, order = torch.sort(torch.softmax(logits.float() / temperature, dim=-1), descending=True, dim=-1, stable=True)
-        gone = p_desc < min_p * p_desc[..., :1]
+        gone = []  # (a filter that is not asked for costs nothing)
+        if min_p > 0:
+            gone.append(p_desc < min_p * p_desc[..., :1])
         if top_k > 0:
-            gone[..., top_k:] = True
+            gone.append(torch.arange(p_desc.shape[-1], device=p_desc.device).expand_as(p_desc) >= top_k)
             p_desc[..., top_k:] = 0
         if 0 < top_p < 1:
             before = torch.cumsum(p_desc, -1) - p_desc
-            gone |= before >= (top_p if top_k <= 0 else top_p * p_desc.sum(-1, keepdim=True))
-        return logits.masked_fill(torch.zeros_like(gone).scatter_(-1, order, gone), float("-inf"))
+            gone.append(before >= (top_p if top_k <= 0 else top_p * p_desc.sum(-1, keepdim=True)))
+        out = gone[0]
+        for more in gone[1:]:
+            out = out | more
+        return logits.masked_fill(torch.zeros_like(out).scatter_(-1, order, out), float("-inf"))
 
     def _generate_drafted(self, ids: list[int], max_tokens: int, temperature: float, top_p: float, stop_on_eos: bool,
                           drafts: int, kv_dtype: torch.dtype, top_k: int = 0, min_p: float = 0.0):
